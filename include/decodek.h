@@ -239,6 +239,63 @@ int dk_lm_head_greedy(const void* x, const void* residual, const void* norm_weig
 int dk_embed_tokens(const int64_t* tokens, const void* embed, int64_t vocab, int64_t hidden, int64_t M,
                     void* out, dk_stream_t stream);
 
+/* ---- paged cache: no reference counterpart (its cache is contiguous, kernels/e2e/model.py:192) ----
+ * k_pages and v_pages are pools [n_pages, n_kv, page_size, head_dim] of fp16 (DK_F16) or bf16 (DK_BF16)
+ * values; row b of page_table (int32, rows ld_table apart, table_width entries each) lists the pages of
+ * sequence b in order. lengths[b] (int32) counts the positions of sequence b with the tokens of this call;
+ * starts (int32 [B + 1], or NULL) gives the rows starts[b] .. starts[b+1] of the T tokens that belong to
+ * sequence b (starts[0] = 0, starts[B] = T), its last positions; NULL means one token per sequence (T = B).
+ * All of these are device pointers read on the device, so one captured launch serves every step.
+ * page_size: a power of two from 16 to 256; head_dim 64 or 128; n_q a multiple of n_kv, at most 16 query heads
+ * per kv head (attention). A length <= 0 marks an unused slot of the batch. Every launch may be captured. */
+#define DK_F16 0
+#define DK_BF16 1
+#define DK_F32 2 /* dk_token_logprobs only */
+/* Rotate q and k by their positions and append k and v to the cache: for each token row of qkv
+ * [T, (n_q + 2 n_kv) * head_dim] (rows ldqkv apart; q heads, k heads, v heads) at own position p, with
+ * half = head_dim / 2: x'[d] = x[d] cos[a][d] - x[d+half] sin[a][d], x'[d+half] = x[d+half] cos[a][d] +
+ * x[d] sin[a][d], a = p + rope_offset, computed in fp32 and rounded once. cos and sin are [rope_rows, half]
+ * (rows ld_rope apart), fp32 with rope_f32 != 0, otherwise of the cache's type. Rotated q -> q_out [T, n_q,
+ * head_dim], rotated k and v -> position p of the sequence's pages. A token of an unused slot appends nothing and
+ * its q_out row is zero; a position without a page in the pool, or an angle outside the tables, appends
+ * nothing and sets DK_DEVERR_BAD_POSITION. */
+int dk_paged_append(const void* qkv, int64_t ldqkv, void* k_pages, void* v_pages, int64_t n_pages, int64_t page_size,
+                    const int32_t* page_table, int64_t ld_table, int64_t table_width, const int32_t* lengths,
+                    const int32_t* starts, const void* cos, const void* sin, int32_t rope_f32, int64_t ld_rope,
+                    int64_t rope_rows, int64_t rope_offset, void* q_out, int64_t T, int64_t B, int64_t nq, int64_t nkv,
+                    int64_t head_dim, int32_t dtype, dk_stream_t stream);
+/* Attention over the pages: q [T, n_q, head_dim] (tokens ldq apart, heads head_dim apart) -> out [T, n_q,
+ * head_dim] contiguous. The row at own position p sees the positions j <= p, and with window > 0 of those only
+ * j > p - window and j < sinks; softmax(scale * q k^T) v over them, zero where there are none. Pages that no row
+ * of the call sees are not read and may be freed: their table entries may hold anything. What a page holds
+ * past its sequence's last position is not used. The workspace (dk_paged_attention_workspace_bytes of the same
+ * sizes, 256-byte aligned) needs no initialization and keeps nothing between calls. */
+int dk_paged_attention_workspace_bytes(int64_t T, int64_t B, int64_t nq, int64_t nkv, int64_t head_dim, int32_t dtype,
+                                       int32_t ragged, int64_t prefix_len, uint64_t* bytes);
+int dk_paged_attention(const void* q, int64_t ldq, const void* k_pages, const void* v_pages, int64_t n_pages,
+                       int64_t page_size, const int32_t* page_table, int64_t ld_table, int64_t table_width,
+                       const int32_t* lengths, const int32_t* starts, int64_t window, int64_t sinks, float scale,
+                       void* out, int64_t T, int64_t B, int64_t nq, int64_t nkv, int64_t head_dim, int32_t dtype,
+                       void* workspace, uint64_t workspace_bytes, dk_stream_t stream);
+/* Attention of a batch whose sequences share a prefix of prefix_len positions, in the pages listed by
+ * prefix_table (int32): every row sees the whole prefix and its own sequence's positions (page_table, lengths,
+ * starts as above, counted without the prefix) up to its own. The prefix is read once for all rows. */
+int dk_shared_prefix_attention(const void* q, int64_t ldq, const void* k_pages, const void* v_pages, int64_t n_pages,
+                               int64_t page_size, const int32_t* prefix_table, int64_t prefix_len,
+                               const int32_t* page_table, int64_t ld_table, int64_t table_width,
+                               const int32_t* lengths, const int32_t* starts, float scale, void* out, int64_t T,
+                               int64_t B, int64_t nq, int64_t nkv, int64_t head_dim, int32_t dtype, void* workspace,
+                               uint64_t workspace_bytes, dk_stream_t stream);
+
+/* ---- log probabilities of given tokens: no reference counterpart -------------------------------
+ * logits [M, V] (rows ld apart; DK_F16, DK_BF16 or DK_F32) in one pass: logprob[m] = x[t] - logsumexp(x) of the target
+ * t = targets[m] (device int64; t < 0: no token, 0; t >= V: NaN and DK_DEVERR_BAD_TOKEN), entropy[m] in nats (a logit of
+ * -inf adds 0), and the top <= 32 largest logits of each row, best first, ties to the lowest index, as top_logprob
+ * [M, top] and top_id [M, top] (int64). fp32 sums. A row with NaN or +inf, or all -inf, has NaN log probabilities. */
+int dk_token_logprobs(const void* logits, int64_t ld, int32_t dtype, const int64_t* targets, int64_t M, int64_t V,
+                      int64_t top, float* logprob, float* entropy, float* top_logprob, int64_t* top_id,
+                      dk_stream_t stream);
+
 /* ---- fused decode step: one persistent kernel per token ------------------------------------
  * One greedy decode step of a Qwen2 model with W4A16 linears and a tied or untied fp16 lm_head, for
  * 1..4 sequences: the reference runner's T == 1 forward (kernels/e2e/model.py:216-253: embedding,

@@ -1,0 +1,197 @@
+// What the paged-cache kernels share: 16-bit element types, the division of a batch's attention work
+// into units and chunks, and the partial results of units that several CTAs work on.
+//
+// A cache is a pool of pages, k and v each [n_pages, n_kv, page_size, head_dim]; row b of the page
+// table lists the pages of sequence b in order, so position j of kv head h is row
+// (table[b][j / page_size] * n_kv + h) * page_size + j % page_size of the pool.
+//
+// The query rows of a launch are cut into tiles of consecutive tokens of one sequence, with the G =
+// n_q / n_kv query heads of one kv head side by side (row r of a tile: token r / G, head r % G), so a
+// tile reads each k and v row once for all of its rows. (kv head, tile) is a unit; its visible
+// positions are cut into chunks of kChunk positions, at least one. All chunks of all units are laid
+// on one line, kv head by kv head, and every CTA of the launch takes an equal contiguous piece of it:
+// long and short sequences, many or few of them, fill the GPU alike. A unit cut by a piece's end
+// leaves its partial results (row maximum, row sum, unnormalized output, fp32) in the workspace, and
+// a second kernel joins them in order of position, so that results do not depend on timing.
+#pragma once
+
+#include <cuda_bf16.h>
+
+#include "common.cuh"
+
+namespace dk {
+namespace paged {
+
+// ---------------------------------------------------------------------------------- element types
+template <typename T>
+struct Elem;
+
+template <>
+struct Elem<__half> {
+  static constexpr CUtensorMapDataType kMapType = CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  __device__ static uint32_t pack(float lo, float hi) {
+    uint32_t d;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+    return d;
+  }
+  __device__ static float2 unpack(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
+  // D(16x8, f32) += A(16x16, row) * B(16x8, col)
+  __device__ static void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                             uint32_t b1) {
+    mma_16816(d, a0, a1, a2, a3, b0, b1);
+  }
+};
+
+template <>
+struct Elem<__nv_bfloat16> {
+  static constexpr CUtensorMapDataType kMapType = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  __device__ static uint32_t pack(float lo, float hi) {
+    uint32_t d;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+    return d;
+  }
+  __device__ static float2 unpack(uint32_t v) {
+    return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+  }
+  __device__ static void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                             uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+};
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// ------------------------------------------------------------------------------------ visible positions
+// A row at position p sees position j when j <= p and (window <= 0 or j > p - window or j < sinks).
+struct Mask {
+  int window, sinks;
+  __device__ bool sees(int p, int j) const { return j <= p && (window <= 0 || j > p - window || j < sinks); }
+};
+
+// The chunks that the rows at positions p0..p1 of one tile need: chunk i of the unit is cache chunk
+// i (i < ns: the sinks) or w0 + i - ns. At least one chunk, so that a tile that sees nothing is still
+// visited once and gets its zeros.
+template <int kChunk>
+struct Span {
+  int end;  // first position after the last visible one
+  int lo;   // first position inside some row's window
+  int ns, w0, n;
+  __device__ Span(int p0, int p1, const Mask& m, int capacity) {
+    end = min(max(p1 + 1, 0), capacity);
+    lo = m.window > 0 ? max(0, p0 - m.window + 1) : 0;
+    const int s = min(m.sinks, lo);
+    w0 = lo / kChunk;
+    ns = m.window > 0 ? (s + kChunk - 1) / kChunk : 0;
+    if (ns > 0 && ns >= w0) ns = w0 = 0;  // the sinks reach the window's first chunk: one run of chunks
+    n = max(1, ns + (end + kChunk - 1) / kChunk - w0);
+  }
+  __device__ int chunk(int i) const { return i < ns ? i : w0 + i - ns; }
+  // Is some position of [j, j + len) visible to some row of the tile?
+  __device__ bool needs(int j, int len, const Mask& m) const {
+    return j < end && (m.window <= 0 || j + len > lo || j < m.sinks);
+  }
+};
+
+// ------------------------------------------------------------------------------------------ launches
+enum Mode {
+  kOneToken = 0,  // tile b is the one token of sequence b
+  kRagged = 1,    // tiles from the plan kernel
+  kPrefix = 2,    // tiles of consecutive tokens of the whole batch, all of the prefix visible to each
+};
+
+struct Problem {
+  const void* q;  // [T, n_q, head_dim], tokens ldq elements apart
+  int64_t ldq;
+  void* out;  // [T, n_q, head_dim]
+  const int32_t* table;
+  int64_t ld_table;
+  const int32_t* lengths;
+  const int32_t* starts;  // [B + 1] or null
+  int T, B, nkv, G;
+  int n_pages, page_size, page_shift, capacity;  // capacity: positions a table row can hold
+  int prefix_len;
+  Mask mask;
+  float scale2;  // scale * log2(e)
+  int mode;
+  int tile_tokens;
+  int n_tiles;  // kOneToken, kPrefix; kRagged: the plan's
+  // kRagged: plan[0] = tiles, plan[1] = chunks of one kv head, then cum[max_tiles + 1], sequence[max_tiles],
+  // first token[max_tiles]
+  const int32_t* plan;
+  int max_tiles;
+  int32_t* cum_out;  // kOneToken: [B + 1], the chunks of one kv head before each sequence
+  // Partial results: a CTA's first piece of a unit that began before it (slot 2 * CTA), its last piece of a unit that
+  // goes on after it (slot 2 * CTA + 1), and with always_partial a slot for each uncut unit after those
+  float* part_o;   // [slots][tile rows][head_dim]
+  float* part_ml;  // [slots][tile rows][2]: row maximum (base 2), row sum
+  int always_partial;  // no unit writes its output itself
+  int* err;
+};
+
+struct Tile {
+  int t0, ntok;  // tokens of q
+  int p0;        // position of the first one
+  const int32_t* table;
+};
+
+__device__ __forceinline__ int plan_cum(const Problem& p, int i) { return p.plan[2 + i]; }
+
+__device__ __forceinline__ Tile tile_at(const Problem& p, int i) {
+  Tile t;
+  if (p.mode == kOneToken) {
+    t.t0 = i;
+    t.ntok = 1;
+    t.p0 = p.lengths[i] - 1;
+    t.table = p.table + i * p.ld_table;
+  } else if (p.mode == kPrefix) {
+    t.t0 = i * p.tile_tokens;
+    t.ntok = min(p.tile_tokens, p.T - t.t0);
+    t.p0 = p.prefix_len - 1;
+    t.table = p.table;
+  } else {
+    const int b = p.plan[3 + p.max_tiles + i];
+    t.t0 = p.plan[3 + 2 * p.max_tiles + i];
+    const int t1 = min(p.starts[b + 1], p.T);
+    t.ntok = min(p.tile_tokens, t1 - t.t0);
+    t.p0 = p.lengths[b] - (t1 - t.t0);
+    t.table = p.table + b * p.ld_table;
+  }
+  return t;
+}
+
+// Last position of a tile's rows (the rows of a prefix launch all sit at its last position).
+__device__ __forceinline__ int tile_last(const Problem& p, const Tile& t) {
+  return p.mode == kPrefix ? t.p0 : t.p0 + t.ntok - 1;
+}
+__device__ __forceinline__ int row_position(const Problem& p, const Tile& t, int tok) {
+  return p.mode == kPrefix ? t.p0 : t.p0 + tok;
+}
+
+__device__ __forceinline__ int64_t partial_slot(int ctas, int cta, bool from_start, bool whole, int unit) {
+  return whole ? 2ll * ctas + unit : 2ll * cta + (from_start ? 1 : 0);
+}
+
+// Largest i with cum[i] <= x, for cum[0] = 0 <= x < cum[n].
+template <typename Cum>
+__device__ __forceinline__ int find_tile(const Cum& cum, int n, int x) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (cum(mid) <= x)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+
+}  // namespace paged
+}  // namespace dk

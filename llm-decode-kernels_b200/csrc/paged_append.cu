@@ -1,0 +1,189 @@
+// Append of keys and values to a paged cache with the rotary positions applied on the way:
+// for every token row of qkv at position p of its sequence b (x: a head of q or k, half = head_dim / 2)
+//   x'[d]        = x[d] * cos[p][d] - x[d + half] * sin[p][d]
+//   x'[d + half] = x[d + half] * cos[p][d] + x[d] * sin[p][d]          (fp32, rounded once)
+// q' goes to q_out, k' and v to row p % page_size of page table[b][p / page_size]. The sequence runner's
+// counterpart for a contiguous cache is the head of csrc/attention.cu (kernels/e2e/model.py:236-241).
+//
+// Memory bound: every element is read once and written once; the angle rows are shared by all heads of a
+// token and come from the caches. One thread turns 8 dims and their 8 partners (two 16-byte loads, two
+// 16-byte stores) or copies 8 dims of v.
+#include "paged.cuh"
+
+namespace dk {
+namespace {
+
+using namespace paged;
+
+struct AppendParams {
+  const void* qkv;
+  int64_t ldqkv;
+  void* k;
+  void* v;
+  const int32_t* table;
+  int64_t ld_table;
+  const int32_t* lengths;
+  const int32_t* starts;
+  const void* cos;
+  const void* sin;
+  int64_t ld_rope;
+  int64_t rope_rows, rope_offset;
+  void* q_out;
+  int T, B, nq, nkv;
+  int n_pages, page_size, page_shift, table_width;
+  int* err;
+};
+
+template <typename T, typename R>
+__device__ __forceinline__ void load8(const R* p, float (&v)[8]) {
+  if constexpr (sizeof(R) == 4) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+  } else {
+    const uint4 a = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = Elem<T>::unpack(w[i]);
+      v[2 * i] = f.x, v[2 * i + 1] = f.y;
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
+  return make_uint4(Elem<T>::pack(v[0], v[1]), Elem<T>::pack(v[2], v[3]), Elem<T>::pack(v[4], v[5]),
+                    Elem<T>::pack(v[6], v[7]));
+}
+
+template <typename T, typename R, int kHd>
+__global__ void __launch_bounds__(256) paged_append_kernel(const AppendParams p) {
+  constexpr int kRot = kHd / 16;  // threads per rotated head
+  constexpr int kCopy = kHd / 8;  // threads per head of v
+  pdl_trigger();
+  pdl_wait();
+  const int rot_items = (p.nq + p.nkv) * kRot;
+  const unsigned per_token = rot_items + p.nkv * kCopy;
+  const int64_t total = static_cast<int64_t>(p.T) * per_token;
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
+    const int t = static_cast<int>(i / per_token);
+    const int e = static_cast<int>(i - static_cast<int64_t>(t) * per_token);
+    int b = t, pos;
+    if (p.starts == nullptr) {
+      pos = p.lengths[t] - 1;
+    } else {
+      b = find_tile([&](int j) { return p.starts[j]; }, p.B, t);
+      pos = p.lengths[b] - (p.starts[b + 1] - t);
+    }
+    const bool is_q = e < p.nq * kRot;
+    // a sequence without positions (an unused slot of the batch) appends nothing
+    const bool live = pos >= 0;
+    int page = -1;
+    if (live && !is_q) {
+      const int at = pos >> p.page_shift;
+      page = at < p.table_width ? p.table[b * p.ld_table + at] : -1;
+      if (page < 0 || page >= p.n_pages) {
+        record_device_error(p.err, DK_DEVERR_BAD_POSITION);
+        continue;
+      }
+    }
+    const int64_t angle = pos + p.rope_offset;
+    const bool turns = live && angle >= 0 && angle < p.rope_rows;
+    if (live && !turns) record_device_error(p.err, DK_DEVERR_BAD_POSITION);
+    if (!turns && !is_q) continue;
+    const T* row = static_cast<const T*>(p.qkv) + t * p.ldqkv;
+    const int64_t in_page = static_cast<int64_t>(pos & (p.page_size - 1)) * kHd;
+    if (e < rot_items) {
+      const int h = e / kRot, d = 8 * (e % kRot);
+      uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+      if (turns) {
+        float a[8], c[8], x[8], y[8], u[8], w[8];
+        load8<T>(row + h * kHd + d, x);
+        load8<T>(row + h * kHd + d + kHd / 2, y);
+        load8<T>(static_cast<const R*>(p.cos) + angle * p.ld_rope + d, a);
+        load8<T>(static_cast<const R*>(p.sin) + angle * p.ld_rope + d, c);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          u[j] = x[j] * a[j] - y[j] * c[j];
+          w[j] = y[j] * a[j] + x[j] * c[j];
+        }
+        lo = pack8<T>(u), hi = pack8<T>(w);
+      }
+      T* dst = is_q ? static_cast<T*>(p.q_out) + (static_cast<int64_t>(t) * p.nq + h) * kHd
+                    : static_cast<T*>(p.k) +
+                          (static_cast<int64_t>(page) * p.nkv + (h - p.nq)) * p.page_size * kHd + in_page;
+      *reinterpret_cast<uint4*>(dst + d) = lo;
+      *reinterpret_cast<uint4*>(dst + d + kHd / 2) = hi;
+    } else {
+      const int h = (e - rot_items) / kCopy, d = 8 * ((e - rot_items) % kCopy);
+      T* dst = static_cast<T*>(p.v) + (static_cast<int64_t>(page) * p.nkv + h) * p.page_size * kHd + in_page;
+      *reinterpret_cast<uint4*>(dst + d) =
+          *reinterpret_cast<const uint4*>(row + static_cast<int64_t>(p.nq + p.nkv + h) * kHd + d);
+    }
+  }
+}
+
+}  // namespace
+}  // namespace dk
+
+using namespace dk;
+
+extern "C" int dk_paged_append(const void* qkv, int64_t ldqkv, void* k_pages, void* v_pages, int64_t n_pages,
+                               int64_t page_size, const int32_t* page_table, int64_t ld_table, int64_t table_width,
+                               const int32_t* lengths, const int32_t* starts, const void* cos, const void* sin,
+                               int32_t rope_f32, int64_t ld_rope, int64_t rope_rows, int64_t rope_offset, void* q_out,
+                               int64_t T, int64_t B, int64_t nq, int64_t nkv, int64_t head_dim, int32_t dtype,
+                               dk_stream_t stream) {
+  if (T < 0 || B <= 0 || nq <= 0 || nkv <= 0 || n_pages <= 0 || table_width <= 0)
+    return set_error(DK_ERR_INVALID, "paged_append: bad sizes");
+  if (head_dim != 64 && head_dim != 128)
+    return set_error(DK_ERR_UNSUPPORTED, "paged_append: head_dim %lld (64 or 128)", (long long)head_dim);
+  if (dtype != DK_F16 && dtype != DK_BF16) return set_error(DK_ERR_UNSUPPORTED, "paged_append: dtype %d", dtype);
+  if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1)))
+    return set_error(DK_ERR_UNSUPPORTED, "paged_append: page_size %lld (a power of two from 16 to 256)",
+                     (long long)page_size);
+  if (T == 0) return DK_OK;
+  if (starts == nullptr && T != B)
+    return set_error(DK_ERR_INVALID, "paged_append: without starts there is one token per sequence");
+  if (T > INT32_MAX || B > INT32_MAX || n_pages > INT32_MAX || table_width > INT32_MAX ||
+      table_width * page_size > INT32_MAX)
+    return set_error(DK_ERR_INVALID, "paged_append: sizes must fit 31 bits");
+  if (!qkv || !k_pages || !v_pages || !page_table || !lengths || !cos || !sin || !q_out)
+    return set_error(DK_ERR_INVALID, "paged_append: NULL pointer");
+  if (!aligned16(qkv) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(q_out) || !aligned16(cos) ||
+      !aligned16(sin) || (ldqkv & 7) || (ld_rope & (rope_f32 ? 3 : 7)))
+    return set_error(DK_ERR_ALIGN, "paged_append: rows of qkv, cos, sin, the pages and q_out need 16-byte alignment");
+  AppendParams p;
+  p.qkv = qkv, p.ldqkv = ldqkv, p.k = k_pages, p.v = v_pages;
+  p.table = page_table, p.ld_table = ld_table, p.lengths = lengths, p.starts = starts;
+  p.cos = cos, p.sin = sin, p.ld_rope = ld_rope, p.rope_rows = rope_rows, p.rope_offset = rope_offset;
+  p.q_out = q_out;
+  p.T = static_cast<int>(T), p.B = static_cast<int>(B), p.nq = static_cast<int>(nq), p.nkv = static_cast<int>(nkv);
+  p.n_pages = static_cast<int>(n_pages), p.page_size = static_cast<int>(page_size);
+  p.page_shift = __builtin_ctzll(page_size);
+  p.table_width = static_cast<int>(table_width);
+  p.err = device_info().err_word;
+  const int64_t items = T * ((nq + nkv) * (head_dim / 16) + nkv * (head_dim / 8));
+  const int64_t blocks = (items + 255) / 256, most = 16ll * device_info().num_sms;
+  const dim3 grid(static_cast<unsigned>(blocks < most ? blocks : most));
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  cudaError_t e;
+#define DK_APPEND(TT, RR)                                                                                    \
+  e = head_dim == 128                                                                                        \
+          ? launch(paged_append_kernel<TT, RR, 128>, grid, dim3(256), 0, st, pdl_enabled(), dim3(1, 1, 1), p) \
+          : launch(paged_append_kernel<TT, RR, 64>, grid, dim3(256), 0, st, pdl_enabled(), dim3(1, 1, 1), p)
+  if (dtype == DK_F16) {
+    if (rope_f32)
+      DK_APPEND(__half, float);
+    else
+      DK_APPEND(__half, __half);
+  } else {
+    if (rope_f32)
+      DK_APPEND(__nv_bfloat16, float);
+    else
+      DK_APPEND(__nv_bfloat16, __nv_bfloat16);
+  }
+#undef DK_APPEND
+  if (e != cudaSuccess) return set_error(DK_ERR_CUDA, "paged_append launch: %s", cudaGetErrorString(e));
+  return DK_OK;
+}

@@ -1,0 +1,816 @@
+// Attention over a paged cache: the plan of ragged launches, the kernel for few query rows per kv head
+// (decode), the kernel that joins the partial results of split units, and the entry points.
+//
+//   out[t] = sum_j p[t][j] v[j],  p[t] = softmax over the visible j of scale * q[t] . k[j]
+// Row t at position p sees j <= p with (window <= 0 or j > p - window or j < sinks); a row that sees
+// nothing is zero. Scores, softmax statistics and sums are fp32; p is rounded to the cache's type for the
+// tensor-core product with v, as its other operand is (the sum of p is not rounded).
+//
+// The decode kernel is bound by the bytes of k and v: each is read once for the G query heads that share
+// it. A producer warp streams chunks of 64 positions, page by page, through a ring of TMA boxes (128-byte
+// swizzle: the ldmatrix reads hit all banks); pages that no row sees are never read, and their table
+// entries may be anything. Four consumer warps take 16 positions each: q.k on the tensor cores with the
+// query heads as the rows, online softmax in registers, p.v on the tensor cores with p taken from the
+// score accumulators. A position that no row of the tile sees reads a zero row instead of v, so whatever
+// the page holds there (infinities and NaN included) stays out; masked scores are replaced, not added to.
+#include <algorithm>
+#include <climits>
+#include <mutex>
+
+#include "paged.cuh"
+
+namespace dk {
+namespace paged {
+namespace {
+
+constexpr int kChunk = 64;
+constexpr int kCWarps = 4;
+constexpr int kThreads = (kCWarps + 1) * 32;
+constexpr int kMaxRing = 4;
+constexpr int kPlanThreads = 1024;
+
+// ------------------------------------------------------------------------------------ ragged plan
+// One CTA cuts the sequences into tiles of tile_tokens tokens and sums up their chunks.
+template <int kUnitChunk>
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Problem p, int32_t* plan) {
+  __shared__ int warp_sum[kPlanThreads / 32];
+  pdl_trigger();
+  pdl_wait();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // inclusive scan over the CTA; returns the exclusive prefix and the total
+  auto scan = [&](int v, int& total) {
+    int s = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += u;
+    }
+    __syncthreads();
+    if (lane == 31) warp_sum[warp] = s;
+    __syncthreads();
+    int w = warp_sum[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, w, o);
+      if (lane >= o) w += u;
+    }
+    total = __shfl_sync(0xffffffffu, w, 31);
+    const int before = __shfl_sync(0xffffffffu, w, warp == 0 ? 0 : warp - 1);
+    return (warp == 0 ? 0 : before) + s - v;
+  };
+  int32_t* cum = plan + 2;
+  int32_t* seq = plan + 3 + p.max_tiles;
+  int32_t* first = plan + 3 + 2 * p.max_tiles;
+  int tiles = 0, chunks = 0;
+  for (int b0 = 0; b0 < p.B; b0 += kPlanThreads) {
+    const int b = b0 + tid;
+    const int t0 = b < p.B ? min(max(p.starts[b], 0), p.T) : 0;
+    const int t1 = b < p.B ? min(max(p.starts[b + 1], t0), p.T) : 0;
+    const int mine = (t1 - t0 + p.tile_tokens - 1) / p.tile_tokens;
+    int total;
+    const int at = tiles + scan(mine, total);
+    for (int i = 0; i < mine && at + i < p.max_tiles; ++i) {
+      seq[at + i] = b;
+      first[at + i] = t0 + i * p.tile_tokens;
+    }
+    tiles += total;
+  }
+  tiles = min(tiles, p.max_tiles);
+  __syncthreads();  // the tiles' sequences and first tokens, written above, are read by other threads below
+  for (int i0 = 0; i0 < tiles; i0 += kPlanThreads) {
+    const int i = i0 + tid;
+    int n = 0;
+    if (i < tiles) {
+      const int b = seq[i], t0 = first[i];
+      const int t1 = min(p.starts[b + 1], p.T), ntok = min(p.tile_tokens, t1 - t0);
+      const int p0 = p.lengths[b] - (t1 - t0);
+      n = Span<kUnitChunk>(p0, p0 + ntok - 1, p.mask, p.capacity).n;
+    }
+    int total;
+    const int at = chunks + scan(n, total);
+    if (i < tiles) cum[i] = at;
+    chunks += total;
+  }
+  if (tid == 0) {
+    cum[tiles] = chunks;
+    plan[0] = tiles;
+    plan[1] = chunks;
+  }
+}
+
+// ------------------------------------------------------------------------------------ decode kernel
+template <int kHd>
+struct Box {
+  static constexpr int kSegs = kHd / 64;
+  // A chunk of k or v: per 64-dim segment 64 rows of 128 bytes, 16-byte piece c of row r at c ^ (r % 8).
+  static constexpr int kSegBytes = kChunk * 128;
+  static constexpr int kTensorBytes = kSegs * kSegBytes;
+  static constexpr int kSlotBytes = 2 * kTensorBytes;
+  __device__ static const uint8_t* at(const uint8_t* t, int r, int d) {
+    return t + (d >> 6) * kSegBytes + r * 128 + ((((d & 63) >> 3) ^ (r & 7)) << 4);
+  }
+};
+
+__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"r"(kCWarps * 32) : "memory"); }
+
+// The chunks of one kv head before tile i (cum), for the three ways a launch is cut into tiles.
+struct Line {
+  const Problem& p;
+  const int* cum_sh;  // kOneToken: in shared memory
+  int per_tile;       // kPrefix
+  int tiles, chunks;  // of one kv head
+  __device__ int cum(int i) const {
+    return p.mode == kOneToken ? cum_sh[i] : p.mode == kPrefix ? i * per_tile : plan_cum(p, i);
+  }
+};
+
+template <typename T, int kHd, int kRows>
+__global__ void __launch_bounds__(kThreads)
+    rows_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const Problem p,
+                int ring, int wait_late) {
+  using B = Box<kHd>;
+  using E = Elem<T>;
+  constexpr int kTiles = kHd / 8;
+  constexpr bool kTwo = kRows == 16;  // rows 8..15 of the MMA in use
+  constexpr int kR = kTwo ? 2 : 1;
+  __shared__ __align__(16) uint4 vzero;
+  __shared__ float pre_ml[kCWarps * kRows * 2];
+  __shared__ float pre_w[kCWarps * kRows];
+  __shared__ float fin[kRows * 2];
+  __shared__ __align__(8) uint64_t full[kMaxRing], empty[kMaxRing];
+  __shared__ int warp_sum[kThreads / 32 + 1];
+  extern __shared__ __align__(128) uint8_t dsm_raw[];
+  uint8_t* slots = dsm_raw + ((1024u - (smem_addr(dsm_raw) & 1023u)) & 1023u);
+  float* pre_o = reinterpret_cast<float*>(slots + ring * B::kSlotBytes);  // [warp][row][dim]
+  int* cum_sh = reinterpret_cast<int*>(pre_o + kCWarps * kRows * kHd);    // kOneToken: [B + 1]
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int i = 0; i < ring; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], kCWarps);
+    }
+    fence_mbar_init();
+    vzero = make_uint4(0, 0, 0, 0);
+    prefetch_tensormap(&mk);
+    prefetch_tensormap(&mv);
+  }
+  if (!wait_late) pdl_wait();
+  pdl_trigger();
+
+  Line line{p, cum_sh, 0, p.n_tiles, 0};
+  if (p.mode == kOneToken) {  // every CTA sums up the sequences' chunks for itself
+    int carry = 0;
+    for (int b0 = 0; b0 < p.B; b0 += kThreads) {
+      const int b = b0 + tid;
+      int n = 0;
+      if (b < p.B) n = Span<kChunk>(p.lengths[b] - 1, p.lengths[b] - 1, p.mask, p.capacity).n;
+      int s = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += u;
+      }
+      __syncthreads();
+      if (lane == 31) warp_sum[warp] = s;
+      __syncthreads();
+      int before = carry;
+      for (int w = 0; w < kThreads / 32; ++w) {
+        const int ws = warp_sum[w];
+        if (w < warp) before += ws;
+        carry += ws;
+      }
+      if (b < p.B) cum_sh[b] = before + s - n;
+    }
+    if (tid == 0) cum_sh[p.B] = carry;
+    line.chunks = carry;
+    __syncthreads();
+    if (blockIdx.x == 0)  // for the join kernel
+      for (int i = tid; i <= p.B; i += kThreads) p.cum_out[i] = cum_sh[i];
+  } else if (p.mode == kPrefix) {
+    line.per_tile = (p.prefix_len + kChunk - 1) / kChunk;
+    line.chunks = line.per_tile * p.n_tiles;
+  } else {
+    line.tiles = p.plan[0];
+    line.chunks = p.plan[1];
+  }
+  __syncthreads();
+
+  const int64_t all = static_cast<int64_t>(line.chunks) * p.nkv;
+  const int64_t per = (all + gridDim.x - 1) / gridDim.x;
+  const int64_t x0 = min(blockIdx.x * per, all), x1 = min(x0 + per, all);
+  bool ok = true;
+  int fill = 0;  // ring fills so far
+
+  if (warp == kCWarps) {
+    // ---------------------------------------------------------------- producer warp: one lane per box
+    const int box = min(p.page_size, kChunk);  // rows of one box
+    const int boxes = kChunk / box;
+    const int kv = lane & 1, sg = (lane >> 1) % B::kSegs, pg = lane / (2 * B::kSegs);
+    for (int64_t x = x0; x < x1 && ok;) {
+      const int h = static_cast<int>(x / line.chunks), r = static_cast<int>(x % line.chunks);
+      const int ti = find_tile([&](int i) { return line.cum(i); }, line.tiles, r);
+      const Tile t = tile_at(p, ti);
+      const Span<kChunk> span(t.p0, tile_last(p, t), p.mask, p.capacity);
+      const int c0 = r - line.cum(ti);
+      const int c1 = static_cast<int>(min(static_cast<int64_t>(span.n), c0 + (x1 - x)));
+      x += c1 - c0;
+      // this lane's page in chunk i of the unit; INT_MIN: none, or nothing that a row sees
+      auto entry = [&](int i) {
+        const int j = span.chunk(i) * kChunk + pg * box;
+        return i < c1 && pg < boxes && span.needs(j, box, p.mask) ? __ldg(t.table + (j >> p.page_shift)) : INT_MIN;
+      };
+      int next = entry(c0);
+      for (int i = c0; i < c1; ++i, ++fill) {
+        const int page = next;
+        next = entry(i + 1);
+        const int s = fill % ring;
+        if (fill >= ring && !mbar_wait(&empty[s], ((fill / ring) - 1) & 1, p.err, DK_DEVERR_WAIT_EMPTY)) ok = false;
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const bool mine = page != INT_MIN;
+        const unsigned want = __ballot_sync(0xffffffffu, mine);
+        if (lane == 0) mbar_arrive_expect_tx(&full[s], __popc(want) * box * 128);
+        __syncwarp();
+        if (mine) {
+          const int j = span.chunk(i) * kChunk + pg * box;
+          // a page outside the pool reads as zeros (a row past the map's end)
+          const int y = page >= 0 && page < p.n_pages
+                            ? (page * p.nkv + h) * p.page_size + (j & (p.page_size - 1))
+                            : p.n_pages * p.nkv * p.page_size;
+          uint8_t* dst = slots + s * B::kSlotBytes + kv * B::kTensorBytes + sg * B::kSegBytes + pg * box * 128;
+          tma_load_2d(dst, kv ? &mv : &mk, sg * 64, y, &full[s]);
+        }
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------- consumer warps
+    const int g = lane >> 2, tq = lane & 3;
+    const int mi = lane >> 3, rr = lane & 7;
+    for (int64_t x = x0; x < x1;) {
+      const int h = static_cast<int>(x / line.chunks), r = static_cast<int>(x % line.chunks);
+      const int ti = find_tile([&](int i) { return line.cum(i); }, line.tiles, r);
+      const Tile t = tile_at(p, ti);
+      const int plast = tile_last(p, t);
+      const Span<kChunk> span(t.p0, plast, p.mask, p.capacity);
+      const int c0 = r - line.cum(ti);
+      const int c1 = static_cast<int>(min(static_cast<int64_t>(span.n), c0 + (x1 - x)));
+      x += c1 - c0;
+      const int rows = t.ntok * p.G;
+      // this lane's rows g and g + 8: positions, and q as the MMA's A operand
+      int pos[kR];
+      uint32_t qa[kHd / 16][2 * kR];
+#pragma unroll
+      for (int e = 0; e < kR; ++e) {
+        const int row = g + 8 * e;
+        const int tok = row / p.G;
+        pos[e] = row < rows ? row_position(p, t, tok) : INT_MIN;
+        const T* qr = static_cast<const T*>(p.q) + (t.t0 + tok) * p.ldq + (h * p.G + row - tok * p.G) * kHd;
+#pragma unroll
+        for (int ks = 0; ks < kHd / 16; ++ks) {
+          qa[ks][e] = row < rows ? *reinterpret_cast<const uint32_t*>(qr + 16 * ks + 2 * tq) : 0u;
+          qa[ks][kR + e] = row < rows ? *reinterpret_cast<const uint32_t*>(qr + 16 * ks + 8 + 2 * tq) : 0u;
+        }
+      }
+      float o[kTiles][4];
+#pragma unroll
+      for (int j = 0; j < kTiles; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+      float m_run[kR], l_run[kR];
+#pragma unroll
+      for (int e = 0; e < kR; ++e) m_run[e] = -INFINITY, l_run[e] = 0.f;
+
+      for (int i = c0; i < c1; ++i, ++fill) {
+        const int s = fill % ring;
+        if (ok && !mbar_wait(&full[s], (fill / ring) & 1, p.err, DK_DEVERR_WAIT_FULL)) ok = false;
+        ok = __all_sync(0xffffffffu, ok);
+        const int j0 = span.chunk(i) * kChunk + 16 * warp;  // this warp's 16 positions
+        if (ok && span.needs(j0, 16, p.mask)) {
+          const uint8_t* kt = slots + s * B::kSlotBytes;
+          const uint8_t* vt = kt + B::kTensorBytes;
+          float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+          const int krow = 16 * warp + 8 * (mi >> 1) + rr;
+#pragma unroll
+          for (int ks = 0; ks < kHd / 16; ++ks) {
+            uint32_t kb[4];
+            ldmatrix_x4(kb, B::at(kt, krow, 16 * ks + 8 * (mi & 1)));
+            const uint32_t a1 = kTwo ? qa[ks][kR - 1] : 0u, a3 = kTwo ? qa[ks][2 * kR - 1] : 0u;
+            E::mma(sc[0], qa[ks][0], a1, qa[ks][kR], a3, kb[0], kb[1]);
+            E::mma(sc[1], qa[ks][0], a1, qa[ks][kR], a3, kb[2], kb[3]);
+          }
+          // every row sees all 16 positions (nothing to mask)?
+          const bool clear = j0 + 15 <= t.p0 && (p.mask.window <= 0 || j0 > plast - p.mask.window || j0 + 15 < p.mask.sinks) &&
+                             j0 + 15 < span.end;
+          uint32_t pa[2][kR];  // p as the MMA's A operand
+#pragma unroll
+          for (int e = 0; e < kR; ++e) {
+            float bm = -INFINITY;
+#pragma unroll
+            for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+              for (int u = 0; u < 2; ++u) {
+                const int j = j0 + 8 * nt + 2 * tq + u;
+                float v = sc[nt][2 * e + u] * p.scale2;
+                if (!clear && !(j < span.end && p.mask.sees(pos[e], j))) v = -INFINITY;
+                sc[nt][2 * e + u] = v;
+                bm = fmaxf(bm, v);
+              }
+            bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 1));
+            bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 2));
+            const float m_new = fmaxf(m_run[e], bm);
+            const float m_use = m_new == -INFINITY ? 0.f : m_new;  // a row that has seen nothing yet
+            const float alpha = exp2_approx(m_run[e] - m_use);
+            float pr[2][2], ls = 0.f;
+#pragma unroll
+            for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+              for (int u = 0; u < 2; ++u) {
+                pr[nt][u] = exp2_approx(sc[nt][2 * e + u] - m_use);
+                ls += pr[nt][u];
+              }
+            l_run[e] = fmaf(l_run[e], alpha, ls);
+            m_run[e] = m_new;
+#pragma unroll
+            for (int j = 0; j < kTiles; ++j) {
+              o[j][2 * e] *= alpha;
+              o[j][2 * e + 1] *= alpha;
+            }
+            pa[0][e] = E::pack(pr[0][0], pr[0][1]);
+            pa[1][e] = E::pack(pr[1][0], pr[1][1]);
+          }
+          const int vrow = 16 * warp + (mi & 1) * 8 + rr;
+          const bool zero = !clear && !span.needs(span.chunk(i) * kChunk + vrow, 1, p.mask);
+          const uint32_t a1 = kTwo ? pa[0][kR - 1] : 0u, a3 = kTwo ? pa[1][kR - 1] : 0u;
+#pragma unroll
+          for (int dp = 0; dp < kHd / 16; ++dp) {
+            uint32_t vb[4];
+            ldmatrix_x4_trans(vb, zero ? reinterpret_cast<const uint8_t*>(&vzero) : B::at(vt, vrow, 16 * dp + (mi >> 1) * 8));
+            E::mma(o[2 * dp], pa[0][0], a1, pa[1][0], a3, vb[0], vb[1]);
+            E::mma(o[2 * dp + 1], pa[0][0], a1, pa[1][0], a3, vb[2], vb[3]);
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[s]);
+      }
+      // the four warps' results of this piece of the unit, joined
+#pragma unroll
+      for (int e = 0; e < kR; ++e) {
+        l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], 1);
+        l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], 2);
+        const int row = g + 8 * e;
+#pragma unroll
+        for (int j = 0; j < kTiles; ++j)
+          *reinterpret_cast<float2*>(&pre_o[(warp * kRows + row) * kHd + 8 * j + 2 * tq]) =
+              make_float2(o[j][2 * e], o[j][2 * e + 1]);
+        if (tq == 0) {
+          pre_ml[(warp * kRows + row) * 2] = m_run[e];
+          pre_ml[(warp * kRows + row) * 2 + 1] = l_run[e];
+        }
+      }
+      consumers_sync();
+      const bool all_of_it = c0 == 0 && c1 == span.n, whole = all_of_it && !p.always_partial;
+      if (tid < kRows) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kCWarps; ++w) mx = fmaxf(mx, pre_ml[(w * kRows + tid) * 2]);
+        const float m_use = mx == -INFINITY ? 0.f : mx;
+        float ls = 0.f;
+#pragma unroll
+        for (int w = 0; w < kCWarps; ++w) {
+          const float wt = exp2_approx(pre_ml[(w * kRows + tid) * 2] - m_use);
+          pre_w[w * kRows + tid] = wt;
+          ls = fmaf(wt, pre_ml[(w * kRows + tid) * 2 + 1], ls);
+        }
+        fin[2 * tid] = mx;
+        fin[2 * tid + 1] = ls;
+      }
+      consumers_sync();
+      const int64_t slot = partial_slot(gridDim.x, blockIdx.x, c0 == 0, all_of_it, h * line.tiles + ti);
+      if (ok) {
+        for (int e = tid; e < rows * (kHd / 4); e += kCWarps * 32) {
+          const int row = e / (kHd / 4), d = 4 * (e % (kHd / 4));
+          float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int w = 0; w < kCWarps; ++w) {
+            const float wt = pre_w[w * kRows + row];
+            const float4 v = *reinterpret_cast<const float4*>(&pre_o[(w * kRows + row) * kHd + d]);
+            a.x = fmaf(wt, v.x, a.x), a.y = fmaf(wt, v.y, a.y), a.z = fmaf(wt, v.z, a.z), a.w = fmaf(wt, v.w, a.w);
+          }
+          if (whole) {
+            const float l = fin[2 * row + 1];
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            const int tok = row / p.G;
+            T* dst = static_cast<T*>(p.out) +
+                     (static_cast<int64_t>(t.t0 + tok) * p.nkv * p.G + h * p.G + row - tok * p.G) * kHd + d;
+            *reinterpret_cast<uint2*>(dst) = make_uint2(E::pack(a.x * inv, a.y * inv), E::pack(a.z * inv, a.w * inv));
+          } else {
+            *reinterpret_cast<float4*>(&p.part_o[(slot * kRows + row) * kHd + d]) = a;
+          }
+        }
+        if (!whole && tid < rows)
+          *reinterpret_cast<float2*>(&p.part_ml[(slot * kRows + tid) * 2]) = make_float2(fin[2 * tid], fin[2 * tid + 1]);
+      }
+      consumers_sync();  // pre_o, pre_ml and fin are written again by the next piece
+    }
+  }
+  if (__syncthreads_or(!ok) && warp == kCWarps && lane == 0) {
+    // a wait gave up: let copies still in flight land before the shared memory goes away (bounded)
+    const uint64_t t0 = globaltimer_ns();
+    for (int s = 0; s < ring; ++s)
+      while (!mbar_try_wait(&full[s], 0) && !mbar_try_wait(&full[s], 1) && globaltimer_ns() - t0 < 500000000ull) {
+      }
+  }
+  if (wait_late) pdl_wait();
+}
+
+// ------------------------------------------------------------------------------------ join
+// Where the partial results of one unit lie: the CTAs first..last of the launch that took its chunks.
+struct Pieces {
+  int first, last;
+  int64_t whole_slot;
+};
+
+__device__ __forceinline__ Pieces pieces_of(int64_t u0, int64_t u1, int64_t per, int ctas, int64_t unit) {
+  return {static_cast<int>(u0 / per), static_cast<int>((u1 - 1) / per), 2ll * ctas + unit};
+}
+
+__device__ __forceinline__ int64_t piece_slot(const Pieces& w, int i) {
+  return w.first == w.last ? w.whole_slot : 2ll * i + (i == w.first ? 1 : 0);
+}
+
+// Adds one unit's partial results of one row to (m, l, acc): kD dims per lane.
+template <int kD>
+__device__ __forceinline__ void add_pieces(const Problem& p, const Pieces& w, int tile_rows, int row, int lane, float& m,
+                                           float& l, float (&acc)[kD]) {
+  float mx = m;
+  for (int i = w.first + lane; i <= w.last; i += 32) mx = fmaxf(mx, p.part_ml[(piece_slot(w, i) * tile_rows + row) * 2]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  const float m_use = mx == -INFINITY ? 0.f : mx;
+  const float keep = exp2_approx(m - m_use);
+  l *= keep;
+#pragma unroll
+  for (int d = 0; d < kD; ++d) acc[d] *= keep;
+  m = mx;
+#pragma unroll 4
+  for (int i = w.first; i <= w.last; ++i) {
+    const int64_t at = piece_slot(w, i) * tile_rows + row;
+    const float2 ml = *reinterpret_cast<const float2*>(&p.part_ml[at * 2]);
+    const float wt = exp2_approx(ml.x - m_use);
+    l = fmaf(wt, ml.y, l);
+    const float* src = &p.part_o[at * (kD * 32) + lane * kD];
+    if constexpr (kD == 4) {
+      const float4 v = *reinterpret_cast<const float4*>(src);
+      acc[0] = fmaf(wt, v.x, acc[0]), acc[1] = fmaf(wt, v.y, acc[1]);
+      acc[2] = fmaf(wt, v.z, acc[2]), acc[3] = fmaf(wt, v.w, acc[3]);
+    } else {
+      const float2 v = *reinterpret_cast<const float2*>(src);
+      acc[0] = fmaf(wt, v.x, acc[0]), acc[1] = fmaf(wt, v.y, acc[1]);
+    }
+  }
+}
+
+template <typename T, int kD>
+__device__ __forceinline__ void store_row(const Problem& p, int t, int head, int lane, float l, const float (&acc)[kD]) {
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  T* dst = static_cast<T*>(p.out) + (static_cast<int64_t>(t) * p.nkv * p.G + head) * (kD * 32) + lane * kD;
+  if constexpr (kD == 4)
+    *reinterpret_cast<uint2*>(dst) =
+        make_uint2(Elem<T>::pack(acc[0] * inv, acc[1] * inv), Elem<T>::pack(acc[2] * inv, acc[3] * inv));
+  else
+    *reinterpret_cast<uint32_t*>(dst) = Elem<T>::pack(acc[0] * inv, acc[1] * inv);
+}
+
+constexpr int kJoinWarps = 8;
+
+__device__ __forceinline__ int line_cum(const Problem& p, int per_tile, int i) {
+  return p.mode == kOneToken ? p.cum_out[i] : p.mode == kPrefix ? i * per_tile : plan_cum(p, i);
+}
+
+// Joins the units that a piece's end cuts. Block (i, y): the unit that holds the end of piece i, if that is the
+// first end inside it; a warp per row.
+template <typename T, int kHd>
+__global__ void __launch_bounds__(kJoinWarps * 32) join_split_kernel(const Problem p, int ctas, int tile_rows) {
+  constexpr int kD = kHd / 32;
+  pdl_trigger();
+  pdl_wait();
+  const int tiles = p.mode == kRagged ? p.plan[0] : p.n_tiles;
+  const int chunks = p.mode == kRagged ? p.plan[1] : p.cum_out[p.B];
+  const int64_t all = static_cast<int64_t>(chunks) * p.nkv, per = (all + ctas - 1) / ctas;
+  const int64_t x = (blockIdx.x + 1ll) * per;
+  if (x >= all) return;
+  const int h = static_cast<int>(x / chunks), r = static_cast<int>(x % chunks);
+  const int ti = find_tile([&](int i) { return line_cum(p, 0, i); }, tiles, r);
+  const int64_t u0 = static_cast<int64_t>(h) * chunks + line_cum(p, 0, ti);
+  const int64_t u1 = static_cast<int64_t>(h) * chunks + line_cum(p, 0, ti + 1);
+  if (u0 / per != blockIdx.x) return;
+  const Pieces w = pieces_of(u0, u1, per, ctas, 0);
+  const Tile t = tile_at(p, ti);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int row = blockIdx.y * kJoinWarps + warp; row < t.ntok * p.G; row += gridDim.y * kJoinWarps) {
+    float m = -INFINITY, l = 0.f, acc[kD] = {};
+    add_pieces<kD>(p, w, tile_rows, row, lane, m, l, acc);
+    store_row<T, kD>(p, t.t0 + row / p.G, h * p.G + row % p.G, lane, l, acc);
+  }
+}
+
+// Joins the prefix's results (`a`) with those of the sequences' own positions (`b`): a warp per (token, head).
+template <typename T, int kHd>
+__global__ void __launch_bounds__(kJoinWarps * 32)
+    join_prefix_kernel(const Problem a, int a_ctas, int a_rows, int a_chunk, const Problem b, int b_ctas, int b_rows) {
+  constexpr int kD = kHd / 32;
+  pdl_trigger();
+  pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t rows = static_cast<int64_t>(a.T) * a.nkv * a.G;
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * kJoinWarps + warp;
+  if (id >= rows) return;
+  const int t = static_cast<int>(id / (a.nkv * a.G)), head = static_cast<int>(id % (a.nkv * a.G));
+  const int h = head / a.G, g = head % a.G;
+  float m = -INFINITY, l = 0.f, acc[kD] = {};
+  {
+    const int per_tile = (a.prefix_len + a_chunk - 1) / a_chunk;
+    const int ti = t / a.tile_tokens, unit = h * a.n_tiles + ti;
+    const int64_t all = static_cast<int64_t>(per_tile) * a.n_tiles * a.nkv, per = (all + a_ctas - 1) / a_ctas;
+    const int64_t u0 = static_cast<int64_t>(unit) * per_tile;
+    add_pieces<kD>(a, pieces_of(u0, u0 + per_tile, per, a_ctas, unit), a_rows, (t % a.tile_tokens) * a.G + g, lane, m, l,
+                   acc);
+  }
+  const int tiles = b.mode == kRagged ? b.plan[0] : b.n_tiles;
+  const int chunks = b.mode == kRagged ? b.plan[1] : b.cum_out[b.B];
+  if (chunks > 0) {
+    const int64_t all = static_cast<int64_t>(chunks) * b.nkv, per = (all + b_ctas - 1) / b_ctas;
+    const int ti = b.mode == kRagged ? find_tile([&](int i) { return b.plan[3 + 2 * b.max_tiles + i]; }, tiles, t) : t;
+    const int t0 = b.mode == kRagged ? b.plan[3 + 2 * b.max_tiles + ti] : t;
+    const int64_t u0 = static_cast<int64_t>(h) * chunks + line_cum(b, 0, ti);
+    const int64_t u1 = static_cast<int64_t>(h) * chunks + line_cum(b, 0, ti + 1);
+    add_pieces<kD>(b, pieces_of(u0, u1, per, b_ctas, h * tiles + ti), b_rows, (t - t0) * b.G + g, lane, m, l, acc);
+  }
+  store_row<T, kD>(b, t, head, lane, l, acc);
+}
+
+}  // namespace
+
+// ------------------------------------------------------------------------------------ host
+namespace {
+
+constexpr int kMaxBatch = 4096;  // kOneToken: the chunk sums of a batch lie in shared memory
+
+// What a rows_kernel launch takes: slots of its ring, shared memory, and the CTAs of one wave (0: it does not fit).
+struct RowsShape {
+  int ring;
+  size_t smem;
+  int ctas;
+};
+
+template <typename T, int kHd, int kRows>
+RowsShape rows_shape(int64_t B) {
+  static std::mutex mu;
+  static int per_sm[2][64];  // by shared memory (batches up to 511 or more) and device; 0: not asked yet
+  RowsShape s;
+  const bool large = B > 511;
+  s.ring = kRows == 8 ? 3 : 4;
+  s.smem = 1024 + static_cast<size_t>(s.ring) * Box<kHd>::kSlotBytes + kCWarps * kRows * kHd * 4 +
+           ((large ? kMaxBatch : 511) + 1) * 4;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  std::lock_guard<std::mutex> lock(mu);
+  int& n = per_sm[large][dev & 63];
+  if (n == 0) {
+    auto k = rows_kernel<T, kHd, kRows>;
+    if (opt_in_dynamic_smem(k) < static_cast<int>(s.smem) ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k, kThreads, s.smem) != cudaSuccess) {
+      cudaGetLastError();
+      n = 0;
+    }
+  }
+  s.ctas = n * device_info().num_sms;
+  return s;
+}
+
+struct Sizes {
+  int64_t T, B, nq, nkv, hd, prefix_len;
+  bool ragged;
+  int dtype;
+};
+
+// Tokens of a tile of up to 16 rows, and the rows a tile's results take.
+int rows_tile_tokens(const Sizes& z) { return z.ragged ? std::max<int>(1, 16 / static_cast<int>(z.nq / z.nkv)) : 1; }
+int rows_of(const Sizes& z, int tokens) { return tokens * (z.nq / z.nkv) <= 8 ? 8 : 16; }
+
+RowsShape rows_shape_of(const Sizes& z, int rows) {
+#define DK_SHAPE(TT) \
+  (z.hd == 128 ? (rows == 8 ? rows_shape<TT, 128, 8>(z.B) : rows_shape<TT, 128, 16>(z.B)) \
+               : (rows == 8 ? rows_shape<TT, 64, 8>(z.B) : rows_shape<TT, 64, 16>(z.B)))
+  return z.dtype == DK_F16 ? DK_SHAPE(__half) : DK_SHAPE(__nv_bfloat16);
+#undef DK_SHAPE
+}
+
+cudaError_t launch_rows(const Sizes& z, int rows, const RowsShape& s, cudaStream_t st, const CUtensorMap& mk,
+                        const CUtensorMap& mv, const Problem& p, int wait_late) {
+#define DK_ROWS(TT, HH, RR) \
+  launch(rows_kernel<TT, HH, RR>, dim3(s.ctas), dim3(kThreads), s.smem, st, pdl_enabled(), dim3(1, 1, 1), mk, mv, p, s.ring, wait_late)
+#define DK_ROWS_T(TT) \
+  (z.hd == 128 ? (rows == 8 ? DK_ROWS(TT, 128, 8) : DK_ROWS(TT, 128, 16)) : (rows == 8 ? DK_ROWS(TT, 64, 8) : DK_ROWS(TT, 64, 16)))
+  return z.dtype == DK_F16 ? DK_ROWS_T(__half) : DK_ROWS_T(__nv_bfloat16);
+#undef DK_ROWS_T
+#undef DK_ROWS
+}
+
+// A workspace cut into aligned areas; with a null base it only counts.
+struct Cutter {
+  char* base;
+  uint64_t used = 0;
+  template <typename T>
+  T* take(uint64_t count) {
+    T* at = base ? reinterpret_cast<T*>(base + used) : nullptr;
+    used += (count * sizeof(T) + 255) / 256 * 256;
+    return at;
+  }
+};
+
+// One launch over the chunks of one kind of tiles, with its areas of the workspace.
+struct Pass {
+  Problem p;
+  RowsShape shape;
+  int rows;
+};
+
+void cut_rows_pass(const Sizes& z, Cutter& c, Pass& a, bool always_partial) {
+  Problem& p = a.p;
+  a.rows = rows_of(z, p.tile_tokens);
+  a.shape = rows_shape_of(z, a.rows);
+  const int64_t tiles = p.mode == kRagged ? p.max_tiles : p.n_tiles;
+  const int64_t slots = 2ll * a.shape.ctas + (always_partial ? z.nkv * tiles : 0);
+  p.always_partial = always_partial;
+  p.part_o = c.take<float>(slots * a.rows * z.hd);
+  p.part_ml = c.take<float>(slots * a.rows * 2);
+  p.cum_out = p.mode == kOneToken ? c.take<int32_t>(z.B + 1) : nullptr;
+  p.plan = p.mode == kRagged ? c.take<int32_t>(3 + 3ll * p.max_tiles) : nullptr;
+}
+
+void shape_own(const Sizes& z, Problem& p) {
+  p.mode = z.ragged ? kRagged : kOneToken;
+  p.tile_tokens = rows_tile_tokens(z);
+  p.max_tiles = z.ragged ? static_cast<int>(z.T / p.tile_tokens + z.B) : 0;
+  p.n_tiles = static_cast<int>(z.B);
+}
+
+void shape_prefix(const Sizes& z, Problem& p) {
+  p.mode = kPrefix;
+  p.tile_tokens = std::max<int>(1, 16 / static_cast<int>(z.nq / z.nkv));
+  p.max_tiles = 0;
+  p.n_tiles = static_cast<int>((z.T + p.tile_tokens - 1) / p.tile_tokens);
+  p.prefix_len = static_cast<int>(z.prefix_len);
+}
+
+int check_sizes(const char* what, const Sizes& z) {
+  if (z.T < 0 || z.B <= 0 || z.nq <= 0 || z.nkv <= 0 || z.prefix_len < 0)
+    return set_error(DK_ERR_INVALID, "%s: bad sizes", what);
+  if (z.hd != 64 && z.hd != 128) return set_error(DK_ERR_UNSUPPORTED, "%s: head_dim %lld (64 or 128)", what, (long long)z.hd);
+  if (z.dtype != DK_F16 && z.dtype != DK_BF16) return set_error(DK_ERR_UNSUPPORTED, "%s: dtype %d", what, z.dtype);
+  if (z.nq % z.nkv != 0 || z.nq / z.nkv > 16)
+    return set_error(DK_ERR_UNSUPPORTED, "%s: %lld query heads over %lld kv heads (a multiple, at most 16 each)", what,
+                     (long long)z.nq, (long long)z.nkv);
+  if (!z.ragged && z.T != z.B) return set_error(DK_ERR_INVALID, "%s: without starts there is one token per sequence", what);
+  if (!z.ragged && z.B > kMaxBatch)
+    return set_error(DK_ERR_UNSUPPORTED, "%s: %lld sequences (at most %d without starts)", what, (long long)z.B, kMaxBatch);
+  if (z.T > (1 << 26) || z.B > (1 << 26) || z.nkv > 65535 || z.prefix_len > (1 << 30))
+    return set_error(DK_ERR_INVALID, "%s: sizes out of range", what);
+  return DK_OK;
+}
+
+template <typename T, int kHd>
+cudaError_t launch_join(const Sizes& z, cudaStream_t st, const Pass* prefix, const Pass& own) {
+  if (prefix == nullptr) {
+    const dim3 grid(static_cast<unsigned>(own.shape.ctas - 1), static_cast<unsigned>((own.rows + kJoinWarps - 1) / kJoinWarps));
+    return launch(join_split_kernel<T, kHd>, grid, dim3(kJoinWarps * 32), 0, st, pdl_enabled(), dim3(1, 1, 1), own.p,
+                  own.shape.ctas, own.rows);
+  }
+  const dim3 grid(static_cast<unsigned>((z.T * z.nq + kJoinWarps - 1) / kJoinWarps));
+  return launch(join_prefix_kernel<T, kHd>, grid, dim3(kJoinWarps * 32), 0, st, pdl_enabled(), dim3(1, 1, 1), prefix->p,
+                prefix->shape.ctas, prefix->rows, kChunk, own.p, own.shape.ctas, own.rows);
+}
+
+uint64_t workspace_of(const Sizes& z) {
+  Cutter c{nullptr};
+  Pass own = {}, pre = {};
+  shape_own(z, own.p);
+  cut_rows_pass(z, c, own, z.prefix_len > 0);
+  if (z.prefix_len > 0) {
+    shape_prefix(z, pre.p);
+    cut_rows_pass(z, c, pre, true);
+  }
+  return c.used;
+}
+
+}  // namespace
+}  // namespace paged
+}  // namespace dk
+
+using namespace dk;
+using namespace dk::paged;
+
+extern "C" int dk_paged_attention_workspace_bytes(int64_t T, int64_t B, int64_t nq, int64_t nkv, int64_t head_dim,
+                                                  int32_t dtype, int32_t ragged, int64_t prefix_len, uint64_t* bytes) {
+  const Sizes z{T, B, nq, nkv, head_dim, prefix_len, ragged != 0, dtype};
+  if (const int rc = check_sizes("paged_attention_workspace_bytes", z)) return rc;
+  if (!bytes) return set_error(DK_ERR_INVALID, "paged_attention_workspace_bytes: bytes is NULL");
+  *bytes = workspace_of(z);
+  return DK_OK;
+}
+
+namespace {
+
+int attention(const char* what, const Sizes& z, const void* q, int64_t ldq, const void* k_pages, const void* v_pages,
+              int64_t n_pages, int64_t page_size, const int32_t* prefix_table, const int32_t* page_table,
+              int64_t ld_table, int64_t table_width, const int32_t* lengths, const int32_t* starts, int64_t window,
+              int64_t sinks, float scale, void* out, void* workspace, uint64_t workspace_bytes, dk_stream_t stream) {
+  if (const int rc = check_sizes(what, z)) return rc;
+  if (n_pages <= 0 || table_width <= 0 || window < 0 || sinks < 0) return set_error(DK_ERR_INVALID, "%s: bad sizes", what);
+  if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1)))
+    return set_error(DK_ERR_UNSUPPORTED, "%s: page_size %lld (a power of two from 16 to 256)", what, (long long)page_size);
+  if (n_pages * z.nkv * page_size + kChunk >= (int64_t(1) << 31) || table_width * page_size >= (int64_t(1) << 31) ||
+      window >= (int64_t(1) << 31) || sinks >= (int64_t(1) << 31))
+    return set_error(DK_ERR_INVALID, "%s: pages x kv heads x page_size, a table row's positions, window and sinks must stay below 2^31", what);
+  if (z.T == 0) return DK_OK;
+  if (!q || !k_pages || !v_pages || !page_table || !lengths || !out || !workspace || (z.prefix_len > 0 && !prefix_table))
+    return set_error(DK_ERR_INVALID, "%s: NULL pointer", what);
+  if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(out) || (ldq & 7) ||
+      (reinterpret_cast<uintptr_t>(workspace) & 255))
+    return set_error(DK_ERR_ALIGN, "%s: q rows, pages and out need 16-byte alignment, the workspace 256", what);
+  Pass own = {}, pre = {};
+  Cutter c{static_cast<char*>(workspace)};
+  shape_own(z, own.p);
+  cut_rows_pass(z, c, own, z.prefix_len > 0);
+  if (z.prefix_len > 0) {
+    shape_prefix(z, pre.p);
+    cut_rows_pass(z, c, pre, true);
+  }
+  if (c.used > workspace_bytes)
+    return set_error(DK_ERR_INVALID, "%s: the workspace has %llu bytes, %llu are needed", what,
+                     (unsigned long long)workspace_bytes, (unsigned long long)c.used);
+  if (own.shape.ctas == 0 || (z.prefix_len > 0 && pre.shape.ctas == 0))
+    return set_error(DK_ERR_UNSUPPORTED, "%s: the kernel's shared memory does not fit this device", what);
+  for (Problem* p : {&own.p, &pre.p}) {
+    p->q = q, p->ldq = ldq, p->out = out;
+    p->table = page_table, p->ld_table = ld_table, p->lengths = lengths, p->starts = starts;
+    p->T = static_cast<int>(z.T), p->B = static_cast<int>(z.B), p->nkv = static_cast<int>(z.nkv);
+    p->G = static_cast<int>(z.nq / z.nkv);
+    p->n_pages = static_cast<int>(n_pages), p->page_size = static_cast<int>(page_size);
+    p->page_shift = __builtin_ctzll(page_size);
+    p->capacity = static_cast<int>(table_width * page_size);
+    p->mask = Mask{static_cast<int>(window), window > 0 ? static_cast<int>(sinks) : 0};
+    p->scale2 = scale * 1.44269504088896341f;
+    p->err = device_info().err_word;
+  }
+  pre.p.table = prefix_table, pre.p.capacity = static_cast<int>(z.prefix_len), pre.p.mask = Mask{0, 0};
+
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const uint64_t rows = static_cast<uint64_t>(n_pages * z.nkv * page_size);
+  const uint32_t box = static_cast<uint32_t>(std::min<int64_t>(page_size, kChunk));
+  const CUtensorMapDataType type = z.dtype == DK_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  CUtensorMap mk, mv;
+  if (!make_tensor_map_2d(&mk, k_pages, type, z.hd, rows, z.hd * 2, 64, box, CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !make_tensor_map_2d(&mv, v_pages, type, z.hd, rows, z.hd * 2, 64, box, CU_TENSOR_MAP_SWIZZLE_128B))
+    return DK_ERR_CUDA;
+  cudaError_t e = cudaSuccess;
+  if (z.ragged)
+    e = launch(plan_kernel<kChunk>, dim3(1), dim3(kPlanThreads), 0, st, pdl_enabled(), dim3(1, 1, 1), own.p,
+               const_cast<int32_t*>(own.p.plan));
+  if (e == cudaSuccess && z.prefix_len > 0) e = launch_rows(z, pre.rows, pre.shape, st, mk, mv, pre.p, 0);
+  if (e == cudaSuccess) e = launch_rows(z, own.rows, own.shape, st, mk, mv, own.p, 0);
+  const Pass* with = z.prefix_len > 0 ? &pre : nullptr;
+  if (e == cudaSuccess) {
+    if (z.dtype == DK_F16)
+      e = z.hd == 128 ? launch_join<__half, 128>(z, st, with, own) : launch_join<__half, 64>(z, st, with, own);
+    else
+      e = z.hd == 128 ? launch_join<__nv_bfloat16, 128>(z, st, with, own) : launch_join<__nv_bfloat16, 64>(z, st, with, own);
+  }
+  if (e != cudaSuccess) return set_error(DK_ERR_CUDA, "%s launch: %s", what, cudaGetErrorString(e));
+  return DK_OK;
+}
+
+}  // namespace
+
+extern "C" int dk_paged_attention(const void* q, int64_t ldq, const void* k_pages, const void* v_pages, int64_t n_pages,
+                                  int64_t page_size, const int32_t* page_table, int64_t ld_table, int64_t table_width,
+                                  const int32_t* lengths, const int32_t* starts, int64_t window, int64_t sinks,
+                                  float scale, void* out, int64_t T, int64_t B, int64_t nq, int64_t nkv,
+                                  int64_t head_dim, int32_t dtype, void* workspace, uint64_t workspace_bytes,
+                                  dk_stream_t stream) {
+  const Sizes z{T, B, nq, nkv, head_dim, 0, starts != nullptr, dtype};
+  return attention("paged_attention", z, q, ldq, k_pages, v_pages, n_pages, page_size, nullptr, page_table, ld_table,
+                   table_width, lengths, starts, window, sinks, scale, out, workspace, workspace_bytes, stream);
+}
+
+extern "C" int dk_shared_prefix_attention(const void* q, int64_t ldq, const void* k_pages, const void* v_pages,
+                                          int64_t n_pages, int64_t page_size, const int32_t* prefix_table,
+                                          int64_t prefix_len, const int32_t* page_table, int64_t ld_table,
+                                          int64_t table_width, const int32_t* lengths, const int32_t* starts,
+                                          float scale, void* out, int64_t T, int64_t B, int64_t nq, int64_t nkv,
+                                          int64_t head_dim, int32_t dtype, void* workspace, uint64_t workspace_bytes,
+                                          dk_stream_t stream) {
+  const Sizes z{T, B, nq, nkv, head_dim, prefix_len, starts != nullptr, dtype};
+  return attention("shared_prefix_attention", z, q, ldq, k_pages, v_pages, n_pages, page_size, prefix_table, page_table,
+                   ld_table, table_width, lengths, starts, 0, 0, scale, out, workspace, workspace_bytes, stream);
+}

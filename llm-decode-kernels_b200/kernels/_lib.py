@@ -98,6 +98,14 @@ SIGNATURES = {
                                   P],
     "dk_w4a16_matmul_reduce_static": [P, I64, P, P, P, P, P, I64, I64, I64, I64, I64, ctypes.POINTER(MatmulConfig),
                                       P],
+    "dk_paged_append": [P, I64, P, P, I64, I64, P, I64, I64, P, P, P, P, I32, I64, I64, I64, P, I64, I64, I64, I64, I64,
+                        I32, P],
+    "dk_paged_attention_workspace_bytes": [I64, I64, I64, I64, I64, I32, I32, I64, ctypes.POINTER(ctypes.c_uint64)],
+    "dk_paged_attention": [P, I64, P, P, I64, I64, P, I64, I64, P, P, I64, I64, F32, P, I64, I64, I64, I64, I64, I32,
+                           P, ctypes.c_uint64, P],
+    "dk_shared_prefix_attention": [P, I64, P, P, I64, I64, P, I64, P, I64, I64, P, P, F32, P, I64, I64, I64, I64, I64,
+                                   I32, P, ctypes.c_uint64, P],
+    "dk_token_logprobs": [P, I64, I32, P, I64, I64, I64, P, P, P, P, P],
     "dk_step_workspace_bytes": [ctypes.POINTER(StepModel), ctypes.POINTER(ctypes.c_uint64)],
     "dk_step_create": [ctypes.POINTER(StepModel), P, ctypes.c_uint64, ctypes.POINTER(P)],
     "dk_step_run": [P, P, P, P, I64, P, P],

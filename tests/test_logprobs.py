@@ -1,0 +1,126 @@
+"""Token log probabilities (kernels.logprobs.token_logprobs, C-ABI dk_token_logprobs) against a plain 64-bit
+implementation: values, entropy, and the top alternatives with their ties."""
+
+import math
+
+import pytest
+import torch
+
+TYPES = [torch.float16, torch.bfloat16, torch.float32]
+
+
+def _exact(x, targets, top):
+    x = x.double().cpu()
+    logp = torch.log_softmax(x, -1)
+    lp = torch.where(targets.cpu() >= 0, logp.gather(1, targets.cpu().clamp(min=0)[:, None])[:, 0], torch.zeros(len(x)).double())
+    entropy = -torch.where(logp > -math.inf, logp.exp() * logp, torch.zeros_like(logp)).sum(-1)
+    value, index = torch.sort(logp, dim=-1, descending=True, stable=True)
+    return lp, entropy, value[:, :top], index[:, :top]
+
+
+def _check(x, targets, top):
+    from kernels.logprobs import token_logprobs
+
+    lp, entropy, value, index = (t.cpu() for t in token_logprobs(x, targets, top))
+    want = _exact(x, targets, top)
+    V = x.shape[1]
+    # A thread adds up at most V / 512 + 32 terms (short rows: one tile), each with a relative error below 2^-21 (the
+    # exponential and its rounded argument), and a tree joins the threads; then roundings of the result's size.
+    eps = (V / 512 + 72) * 2.0 ** -24 + 2.0 ** -21
+    assert ((lp - want[0]).abs() <= eps + want[0].abs() * 2.0 ** -22).all()
+    assert ((entropy - want[1]).abs() <= eps * (2 + 2 * want[1])).all()
+    assert torch.equal(index, want[3])
+    fin = want[2] > -math.inf
+    assert ((value - want[2]).abs()[fin] <= eps + want[2].abs()[fin] * 2.0 ** -22).all()
+    assert torch.equal(value[~fin].double(), want[2][~fin])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,V,top", [
+    (1, 1, 1), (2, 7, 7), (1, 151936, 5), (3, 152064, 20), (5, 1003, 32), (300, 517, 3), (2, 32001, 0), (40, 16385, 16),
+    (1, 65537, 17), (150, 20011, 8),
+])
+def test_logprobs(M, V, top, dtype):
+    g = torch.Generator().manual_seed(M * V + top)
+    x = (torch.randn(M, V, generator=g) * 3).to(dtype).cuda()
+    targets = torch.randint(0, V, (M,), generator=g).cuda()
+    targets[0] = -1 if M > 2 else targets[0]
+    _check(x, targets, top)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_ties_masks_and_orders(dtype):
+    """Equal logits, rising and falling rows, all but a few tokens forbidden (-inf or the type's lowest value)."""
+    V, top = 40000, 20
+    rows = [torch.zeros(V), torch.arange(V) / 4096, -torch.arange(V) / 4096, torch.full((V,), -math.inf),
+            torch.full((V,), torch.finfo(dtype).min), (torch.arange(V) % 7).float(), torch.full((V,), -0.0)]
+    rows[3][[5, 17, 39999]] = torch.tensor([1.0, -2.0, 1.0])
+    rows[4][[39998, 3]] = torch.tensor([0.5, 0.25])
+    rows[6][::3] = 0.0
+    x = torch.stack(rows).to(dtype).cuda()
+    targets = torch.tensor([V - 1, 0, 1, 17, 3, 6, 2]).cuda()
+    _check(x, targets, top)
+    for row in range(len(rows)):  # a row alone is split over several CTAs
+        _check(x[row:row + 1], targets[row:row + 1], top)
+
+
+@pytest.mark.gpu
+def test_strided_and_unaligned_rows():
+    x = torch.randn(9, 5001, device="cuda", dtype=torch.bfloat16)
+    targets = torch.arange(9, device="cuda")
+    for lo in (0, 1, 3, 8):
+        _check(x[:, lo:lo + 4990], targets, 6)
+    y = torch.randn(3, 1001, device="cuda")
+    _check(y[:, 1:], targets[:3], 32)
+
+
+@pytest.mark.gpu
+def test_nothing_allowed_nan_and_infinity():
+    from kernels import _lib
+    from kernels.logprobs import token_logprobs
+
+    x = torch.randn(4, 3000, device="cuda", dtype=torch.float16)
+    x[0] = -math.inf
+    x[1, 100] = math.nan
+    x[2, 200] = math.inf
+    _lib.clear_device_error()
+    lp, entropy, value, index = token_logprobs(x, torch.tensor([1, 2, 3, 3000], device="cuda"), 3)
+    assert _lib.device_error() == 6  # DK_DEVERR_BAD_TOKEN: the last row's target
+    _lib.clear_device_error()
+    assert lp[:3].isnan().all() or (lp[2] == -math.inf and lp[:2].isnan().all())
+    assert lp[3].isnan() and entropy[:3].isnan().all() and entropy[3].isfinite()
+    assert index[0].tolist() == [0, 1, 2] and index[1, 0] == 100 and index[2, 0] == 200
+
+
+@pytest.mark.gpu
+def test_empty_and_captured():
+    from kernels.logprobs import token_logprobs
+
+    lp, entropy, value, index = token_logprobs(torch.zeros(0, 50, device="cuda"), torch.zeros(0, dtype=torch.long, device="cuda"), 4)
+    assert lp.shape == entropy.shape == (0,) and value.shape == index.shape == (0, 4)
+    x, t = torch.randn(2, 9000, device="cuda"), torch.tensor([1, 2], device="cuda")
+    want = token_logprobs(x, t, 5)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = token_logprobs(x, t, 5)
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_refusals_without_a_gpu():
+    from kernels import _lib
+    from kernels.logprobs import token_logprobs
+
+    x, t = torch.zeros(2, 50), torch.zeros(2, dtype=torch.long)
+    for error, a in [(RuntimeError, (x, t)), (ValueError, (x[0], t)), (ValueError, (x, t[:1])), (ValueError, (x, t, 33)),
+                     (ValueError, (x, t, -1)), (ValueError, (x[:, :4], t, 5)), (ValueError, (x.T, t)),
+                     (ValueError, (x[:1].expand(2, 50), t)), (RuntimeError, (x.double(), t)), (RuntimeError, (x, t.int()))]:
+        with pytest.raises(error):
+            token_logprobs(*a)
+    h = _lib.lib()
+    assert h.dk_token_logprobs(None, 50, 0, None, 2, 50, 0, None, None, None, None, None) == -1
+    assert h.dk_token_logprobs(None, 49, 0, None, 2, 50, 0, None, None, None, None, None) == -1
+    assert h.dk_token_logprobs(None, 50, 0, None, 2, 50, 33, None, None, None, None, None) == -3
+    assert h.dk_token_logprobs(None, 50, 7, None, 2, 50, 0, None, None, None, None, None) == -3

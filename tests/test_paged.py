@@ -1,0 +1,331 @@
+"""The paged-cache ops (kernels.paged, C-ABI dk_paged_append, dk_paged_attention, dk_shared_prefix_attention) against
+plain 64-bit implementations, at the sizes and masks where they can go wrong, and their refusals."""
+
+import math
+
+import pytest
+import torch
+
+from _paged import UNIT, Case, assert_within
+
+F16, BF16 = torch.float16, torch.bfloat16
+
+
+# ------------------------------------------------------------------------------------------ append
+def _rope(positions, hd, dtype=torch.float32):
+    angle = torch.arange(positions, dtype=torch.float64)[:, None] / 1e4 ** (torch.arange(0, hd, 2, dtype=torch.float64) / hd)
+    return angle.cos().to(dtype).cuda(), angle.sin().to(dtype).cuda()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sizes,nq,nkv,hd,page,dtype,table_type,offset", [
+    ([(1, 1)], 12, 2, 128, 16, F16, torch.float32, 0),
+    ([(1, 17), (1, 300), (1, 64), (1, 65)], 28, 4, 128, 64, BF16, torch.float32, 0),
+    ([(5, 5), (0, 9), (33, 70), (1, 1), (100, 129)], 7, 1, 64, 32, F16, F16, 0),
+    ([(3, 250), (129, 400)], 8, 8, 64, 256, BF16, BF16, 11),
+    ([(1, 0), (1, 40), (1, -3)], 4, 1, 128, 128, F16, torch.float32, 1000),  # unused slots of the batch
+])
+def test_append(sizes, nq, nkv, hd, page, dtype, table_type, offset):
+    from kernels import _lib
+    from kernels.paged import paged_append
+
+    c = Case(sizes, nq, nkv, hd, page, dtype, spoil=False)
+    qkv = torch.randn(c.T, (nq + 2 * nkv) * hd + 8, device="cuda").to(dtype)[:, :-8]  # strided rows
+    cos, sin = _rope(max(n for _, n in sizes) + offset + 1, hd, table_type)
+    k, v = c.k.clone(), c.v.clone()
+    _lib.clear_device_error()
+    q = paged_append(qkv, k, v, c.table, c.lengths, cos, sin, nq, nkv, starts=c.starts, offset=offset)
+    assert _lib.device_error() == 0
+    x = qkv.double().cpu().view(c.T, nq + 2 * nkv, hd)
+    want_k, want_v, u = c.k.double().cpu(), c.v.double().cpu(), UNIT[dtype]
+    slack_k = torch.zeros_like(want_k)
+    t = 0
+    for b, (new, n) in enumerate(sizes):
+        for i in range(new):
+            p = n - new + i
+            if p < 0:
+                assert not q[t].any()
+                t += 1
+                continue
+            a, s = cos[p + offset].double().cpu(), sin[p + offset].double().cpu()
+            lo, hi = x[t, :nq + nkv, :hd // 2], x[t, :nq + nkv, hd // 2:]
+            turned = torch.cat([lo * a - hi * s, hi * a + lo * s], -1)
+            # fp32: two products and a sum, each rounded; then once to the type
+            size = torch.cat([(lo * a).abs() + (hi * s).abs(), (hi * a).abs() + (lo * s).abs()], -1)
+            slack = u * turned.abs() + (2.0 ** -23 + 2.0 ** -24 * u) * size + 2.0 ** -25
+            assert ((q[t].double().cpu() - turned[:nq]).abs() <= slack[:nq]).all()
+            row = c.table[b, p // page].long().item()
+            want_k[row, :, p % page], slack_k[row, :, p % page] = turned[nq:], slack[nq:]
+            want_v[row, :, p % page] = x[t, nq + nkv:]
+            t += 1
+    assert ((k.double().cpu() - want_k).abs() <= slack_k).all()  # nothing else in the pool changed
+    assert torch.equal(v.double().cpu(), want_v)
+
+
+@pytest.mark.gpu
+def test_append_without_a_page_or_an_angle_writes_nothing():
+    from kernels import _lib
+    from kernels.paged import paged_append
+
+    c = Case([(1, 20), (1, 5)], spoil=False)
+    cos, sin = _rope(64, 128)
+    qkv = torch.randn(2, 16 * 128, device="cuda").half()
+    for spoil in ("table", "pool", "angle"):
+        k, v, table = c.k.clone(), c.v.clone(), c.table.clone()
+        table[:, :] = {"table": -1, "pool": c.k.shape[0], "angle": 0}[spoil]
+        rows = slice(0, 3) if spoil == "angle" else slice(0, 64)
+        _lib.clear_device_error()
+        paged_append(qkv, k, v, table, c.lengths, cos[rows], sin[rows], 12, 2)
+        assert _lib.device_error() == 3  # DK_DEVERR_BAD_POSITION
+        _lib.clear_device_error()
+        assert torch.equal(k, c.k) and torch.equal(v, c.v)
+
+
+# ------------------------------------------------------------------------------------------ attention
+DECODE = [
+    # sizes, nq, nkv, hd, page, dtype, window, sinks
+    ([(1, 1)], 12, 2, 128, 16, F16, 0, 0),
+    ([(1, 640)], 12, 2, 128, 16, F16, 0, 0),
+    ([(1, 63), (1, 64), (1, 65), (1, 1), (1, 0), (1, 129)], 28, 4, 128, 64, BF16, 0, 0),
+    ([(1, 1000), (1, 3), (1, 517)], 16, 1, 128, 32, F16, 0, 0),
+    ([(1, 700), (1, 31)], 8, 8, 64, 128, BF16, 0, 0),
+    ([(1, 300)] * 70, 4, 1, 64, 16, F16, 0, 0),
+    ([(1, 777), (1, 40), (1, 5)], 12, 2, 128, 16, F16, 100, 4),
+    ([(1, 777), (1, 40), (1, 128)], 14, 2, 128, 64, BF16, 1, 0),
+    ([(1, 777), (1, 100)], 7, 1, 128, 32, F16, 64, 70),  # the sinks reach into the second chunk
+    ([(1, 90), (1, 300)], 4, 2, 64, 16, F16, 1 << 30, 3),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sizes,nq,nkv,hd,page,dtype,window,sinks", DECODE)
+def test_attention_one_token(sizes, nq, nkv, hd, page, dtype, window, sinks):
+    from kernels import _lib
+    from kernels.paged import paged_attention
+
+    c = Case(sizes, nq, nkv, hd, page, dtype, seed=1)
+    _lib.clear_device_error()
+    out = paged_attention(c.q, c.k, c.v, c.table, c.lengths, window=window, sinks=sinks)
+    assert _lib.device_error() == 0
+    assert_within(out, *c.attention(window, sinks))
+    assert torch.equal(out, paged_attention(c.q, c.k, c.v, c.table, c.lengths, window=window, sinks=sinks))
+
+
+RAGGED = [
+    ([(1, 1), (2, 2)], 12, 2, 128, 16, F16, 0, 0),
+    ([(7, 7), (0, 30), (130, 200), (1, 90), (64, 64)], 12, 2, 128, 16, BF16, 0, 0),
+    ([(300, 300)], 28, 4, 128, 64, F16, 0, 0),
+    ([(200, 430), (33, 33)], 16, 1, 128, 32, BF16, 0, 0),
+    ([(150, 280), (129, 129)], 8, 8, 64, 128, F16, 0, 0),
+    ([(257, 300), (20, 400)], 5, 1, 64, 256, BF16, 0, 0),
+    ([(5, 3), (4, 0), (6, 6)], 12, 2, 128, 16, F16, 0, 0),  # fewer positions than tokens: rows that see nothing
+    ([(260, 400), (50, 300), (3, 3)], 12, 2, 128, 16, F16, 37, 4),
+    ([(300, 300)], 14, 2, 128, 64, BF16, 1, 2),
+    ([(140, 500)], 7, 1, 64, 32, F16, 128, 0),
+    ([(140, 700)], 3, 1, 128, 32, F16, 130, 129),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sizes,nq,nkv,hd,page,dtype,window,sinks", RAGGED)
+def test_attention_ragged(sizes, nq, nkv, hd, page, dtype, window, sinks):
+    from kernels import _lib
+    from kernels.paged import paged_attention
+
+    c = Case(sizes, nq, nkv, hd, page, dtype, seed=2, one_token=False)
+    _lib.clear_device_error()
+    out = paged_attention(c.q, c.k, c.v, c.table, c.lengths, starts=c.starts, window=window, sinks=sinks)
+    assert _lib.device_error() == 0
+    assert_within(out, *c.attention(window, sinks))
+    assert torch.equal(out, paged_attention(c.q, c.k, c.v, c.table, c.lengths, starts=c.starts, window=window, sinks=sinks))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("one_token", [True, False])
+def test_attention_leaves_freed_pages_alone(one_token):
+    """Pages outside the window and the sinks may be freed: their table entries point nowhere."""
+    from kernels.paged import paged_attention
+
+    sizes = [(1, 700), (1, 130)] if one_token else [(9, 700), (40, 130)]
+    c = Case(sizes, seed=3, one_token=one_token)
+    window, sinks = 50, 4
+    want = c.attention(window, sinks)
+    for b, (new, n) in enumerate(sizes):
+        first, last = 1, (n - new + 1 - window) // c.page
+        for i in range(first, last):
+            page = c.table[b, i].long().item()
+            c.k[page], c.v[page] = math.nan, math.nan
+        c.table[b, first:last] = torch.tensor([-1, 1 << 30]).repeat(last)[:last - first].int()
+    out = paged_attention(c.q, c.k, c.v, c.table, c.lengths, starts=c.starts, window=window, sinks=sinks)
+    assert_within(out, *want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sizes,window,sinks", [([(1, 400), (1, 31)], 0, 0), ([(70, 200), (3, 90)], 40, 2)])
+def test_attention_strides_scale_stream_and_graph(sizes, window, sinks):
+    """q rows inside a wider tensor, a table with spare columns, another scale, a side stream, a captured call."""
+    from kernels.paged import paged_attention
+
+    c = Case(sizes, seed=4)
+    wide = torch.zeros(c.T, c.nq + 5, c.hd, dtype=c.dtype, device="cuda")
+    wide[:, :c.nq] = c.q
+    table = torch.full((len(sizes), c.table.shape[1] + 40), -1, dtype=torch.int32, device="cuda")
+    table[:, :c.table.shape[1]] = c.table
+    args = (wide[:, :c.nq], c.k, c.v, table[:, :c.table.shape[1] + 3], c.lengths)
+    more = dict(starts=c.starts, window=window, sinks=sinks, scale=0.2)
+    want = c.attention(window, sinks, scale=0.2)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out = paged_attention(*args, **more)
+    torch.cuda.current_stream().wait_stream(side)
+    assert_within(out, *want)
+    graph, kept = torch.cuda.CUDAGraph(), torch.empty_like(out)
+    with torch.cuda.graph(graph):
+        paged_attention(*args, out=kept, **more)
+    graph.replay()
+    assert torch.equal(kept, out)
+
+
+@pytest.mark.gpu
+def test_attention_long_context_and_masked_extremes():
+    """The type's lowest value and infinities in k or v at masked positions; scores far apart; long contexts."""
+    from kernels.paged import paged_attention
+
+    c = Case([(1, 5000), (1, 2)], nq=6, nkv=1, page=128, seed=5)
+    c.q[0] *= 3
+    out = paged_attention(c.q, c.k, c.v, c.table, c.lengths)
+    assert_within(out, *c.attention())
+    low = Case([(1, 100)], nq=6, nkv=1, seed=6, spoil=False)
+    want = low.attention(16, 2)
+    page = low.table[0].long()
+    for j in range(2, 84):  # neither a sink nor in the window
+        low.k[page[j // 16], :, j % 16] = torch.finfo(F16).min
+        low.v[page[j // 16], :, j % 16] = math.inf
+    assert_within(paged_attention(low.q, low.k, low.v, low.table, low.lengths, window=16, sinks=2), *want)
+
+
+# ------------------------------------------------------------------------------------------ shared prefix
+@pytest.mark.gpu
+@pytest.mark.parametrize("sizes,prefix,nq,nkv,hd,page,dtype", [
+    ([(1, 1)], 1, 12, 2, 128, 16, F16),
+    ([(1, 40), (1, 1), (1, 65)], 525, 12, 2, 128, 16, F16),
+    ([(1, 3)] * 50, 200, 28, 4, 128, 64, BF16),
+    ([(1, 20), (1, 0), (1, 7)], 64, 8, 8, 64, 32, F16),  # an unused slot: the prefix alone
+    ([(2, 30), (5, 5), (1, 90)], 333, 16, 1, 128, 32, BF16),
+    ([(40, 70), (100, 100)], 130, 7, 1, 64, 128, F16),
+    ([(1, 5)] * 9, 2500, 5, 1, 128, 256, F16),
+])
+def test_shared_prefix(sizes, prefix, nq, nkv, hd, page, dtype):
+    from kernels import _lib
+    from kernels.paged import paged_attention, shared_prefix_attention
+
+    c = Case(sizes, nq, nkv, hd, page, dtype, seed=7, prefix=prefix)
+    _lib.clear_device_error()
+    out = shared_prefix_attention(c.q, c.k, c.v, c.prefix_table, prefix, c.table, c.lengths, starts=c.starts)
+    assert _lib.device_error() == 0
+    exact, tol = c.attention()
+    assert_within(out, exact, tol)
+    again = shared_prefix_attention(c.q, c.k, c.v, c.prefix_table, prefix, c.table, c.lengths, starts=c.starts)
+    assert torch.equal(out, again)
+    none = shared_prefix_attention(c.q, c.k, c.v, c.prefix_table, 0, c.table, c.lengths, starts=c.starts)
+    assert torch.equal(none, paged_attention(c.q, c.k, c.v, c.table, c.lengths, starts=c.starts))
+
+
+# ------------------------------------------------------------------------------------------ refusals
+def _cpu_case(**more):
+    return Case([(1, 20), (1, 5)], spoil=False, device="cpu", **more)
+
+
+def test_refusals_without_a_gpu():
+    """Extents, types and layouts the kernels cannot take are refused before any device work."""
+    from kernels.paged import paged_append, paged_attention, shared_prefix_attention
+
+    c = _cpu_case()
+    args = [c.q, c.k, c.v, c.table, c.lengths]
+    starts = torch.tensor([0, 1, 2], dtype=torch.int32)
+
+    def attend(error, *at, **more):
+        a = list(args)
+        for i, x in at:
+            a[i] = x
+        with pytest.raises(error):
+            paged_attention(*a, **more)
+
+    attend(RuntimeError)  # on the CPU
+    attend(ValueError, (0, c.q[:1]))  # a token per sequence
+    attend(ValueError, (0, c.q[..., :64]))
+    attend(ValueError, (0, c.q[:, :5]))  # 5 query heads over 2 kv heads
+    attend(ValueError, (0, torch.zeros(2, 34, 128).half()))  # 17 query heads for each kv head
+    attend(ValueError, (0, c.q.transpose(1, 2).contiguous().transpose(1, 2)))
+    attend(ValueError, (1, c.k[:, :, :8].contiguous()), (2, c.v[:, :, :8].contiguous()))
+    attend(ValueError, (1, c.k[:-1]))
+    attend(ValueError, (1, c.k.transpose(0, 1)), (2, c.v.transpose(0, 1)))
+    attend(ValueError, (1, c.k[..., :32].contiguous()), (2, c.v[..., :32].contiguous()))
+    attend(ValueError, (3, c.table[:1]))
+    attend(ValueError, (4, c.lengths[:1]))
+    attend(ValueError, starts=starts[:2])
+    attend(ValueError, window=-1)
+    attend(ValueError, sinks=-1)
+    attend(ValueError, out=torch.zeros(2, 12, 64).half())
+    attend(RuntimeError, (0, c.q.float()))
+    attend(RuntimeError, (1, c.k.float()), (2, c.v.float()))
+    attend(RuntimeError, (3, c.table.long()))
+    attend(RuntimeError, starts=starts.long())
+    with pytest.raises(ValueError):
+        shared_prefix_attention(c.q, c.k, c.v, c.table[0], 1000, c.table, c.lengths)
+    with pytest.raises(ValueError):
+        shared_prefix_attention(c.q, c.k, c.v, c.table[0], -1, c.table, c.lengths)
+    with pytest.raises(RuntimeError):
+        shared_prefix_attention(c.q, c.k, c.v, c.table[0].long(), 10, c.table, c.lengths)
+
+    qkv, cos = torch.zeros(2, 16 * 128).half(), torch.zeros(40, 64)
+    good = dict(qkv=qkv, cos=cos, sin=cos, n_heads=12, n_kv=2)
+
+    def append(error, **more):
+        a = {**good, **more}
+        with pytest.raises(error):
+            paged_append(a["qkv"], c.k, c.v, c.table, c.lengths, a["cos"], a["sin"], a["n_heads"], a["n_kv"],
+                         offset=a.get("offset", 0), out=a.get("out"))
+
+    append(RuntimeError)  # on the CPU
+    append(ValueError, qkv=qkv[:, :-128])
+    append(ValueError, qkv=qkv[:1])
+    append(ValueError, n_kv=4)
+    append(ValueError, cos=torch.zeros(40, 128), sin=torch.zeros(40, 128))
+    append(ValueError, sin=torch.zeros(39, 64))
+    append(ValueError, offset=-1)
+    append(ValueError, out=torch.zeros(2, 12, 64).half())
+    append(RuntimeError, qkv=qkv.bfloat16())
+    append(RuntimeError, cos=cos.bfloat16(), sin=cos.bfloat16())
+
+
+def test_c_entries_refuse_without_a_gpu():
+    """The C entry points return a status and a message for what they cannot take, before any CUDA call."""
+    import ctypes
+
+    from kernels import _lib
+
+    h, n = _lib.lib(), ctypes.c_uint64(0)
+
+    def attend(**more):
+        a = dict(T=2, B=2, nq=12, nkv=2, hd=128, page=16, dtype=0, ldq=1536, pages=4, width=2)
+        a.update(more)
+        return h.dk_paged_attention(None, a["ldq"], None, None, a["pages"], a["page"], None, a["width"], a["width"], None,
+                                    None, 0, 0, 1.0, None, a["T"], a["B"], a["nq"], a["nkv"], a["hd"], a["dtype"], None, 0,
+                                    None)
+
+    assert attend() == -1 and b"NULL" in h.dk_last_error()
+    assert attend(T=3) == -1 and b"one token" in h.dk_last_error()
+    assert attend(hd=96) == -3 and b"head_dim" in h.dk_last_error()
+    assert attend(page=24) == -3 and b"page_size" in h.dk_last_error()
+    assert attend(nq=13) == -3 and attend(nq=34) == -3
+    assert attend(dtype=2) == -3
+    assert attend(B=5000, T=5000) == -3 and b"sequences" in h.dk_last_error()
+    assert attend(pages=1 << 26) == -1 and b"2^31" in h.dk_last_error()
+    assert attend(width=1 << 27) == -1
+    assert h.dk_paged_attention_workspace_bytes(2, 2, 12, 2, 96, 0, 0, 0, ctypes.byref(n)) == -3
+    assert h.dk_paged_append(None, 0, None, None, 4, 16, None, 2, 2, None, None, None, None, 1, 64, 10, 0, None, 3, 2, 12,
+                             2, 128, 0, None) == -1
+    assert h.dk_paged_append(None, 0, None, None, 4, 20, None, 2, 2, None, None, None, None, 1, 64, 10, 0, None, 2, 2, 12,
+                             2, 128, 0, None) == -3

@@ -49,26 +49,37 @@ EncodeTiledFn encode_tiled() {
 }
 }  // namespace
 
-bool make_tensor_map_2d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, uint64_t inner,
-                        uint64_t outer, uint64_t row_bytes, uint32_t box_inner, uint32_t box_outer,
-                        CUtensorMapSwizzle swizzle) {
+bool make_tensor_map(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, int rank, const uint64_t* dims,
+                     const uint64_t* strides, const uint32_t* box, CUtensorMapSwizzle swizzle) {
   EncodeTiledFn fn = encode_tiled();
   if (fn == nullptr) {
     set_error(DK_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
     return false;
   }
-  const cuuint64_t dims[2] = {inner, outer};
-  const cuuint64_t strides[1] = {row_bytes};
-  const cuuint32_t box[2] = {box_inner, box_outer};
-  const cuuint32_t estr[2] = {1, 1};
-  CUresult r = fn(map, dtype, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  cuuint64_t d[5], st[4];
+  cuuint32_t b[5], estr[5];
+  for (int i = 0; i < rank; ++i) {
+    d[i] = dims[i];
+    b[i] = box[i];
+    estr[i] = 1;
+    if (i > 0) st[i - 1] = strides[i - 1];
+  }
+  CUresult r = fn(map, dtype, rank, const_cast<void*>(base), d, st, b, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     set_error(DK_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d) for a %llux%llu map, box %ux%u", (int)r,
-              (unsigned long long)inner, (unsigned long long)outer, box_inner, box_outer);
+              (unsigned long long)dims[0], (unsigned long long)dims[1], box[0], box[1]);
     return false;
   }
   return true;
+}
+
+bool make_tensor_map_2d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, uint64_t inner,
+                        uint64_t outer, uint64_t row_bytes, uint32_t box_inner, uint32_t box_outer,
+                        CUtensorMapSwizzle swizzle) {
+  const uint64_t dims[2] = {inner, outer};
+  const uint32_t box[2] = {box_inner, box_outer};
+  return make_tensor_map(map, base, dtype, 2, dims, &row_bytes, box, swizzle);
 }
 
 const DeviceInfo& device_info() {

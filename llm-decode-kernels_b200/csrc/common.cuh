@@ -443,6 +443,10 @@ bool make_tensor_map_2d(CUtensorMap* map, const void* base, CUtensorMapDataType 
                         uint64_t outer, uint64_t row_bytes, uint32_t box_inner, uint32_t box_outer,
                         CUtensorMapSwizzle swizzle);
 
+// The same for any rank up to 5: `dims` elements from the innermost one on, `strides` in bytes of all but that one.
+bool make_tensor_map(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, int rank, const uint64_t* dims,
+                     const uint64_t* strides, const uint32_t* box, CUtensorMapSwizzle swizzle);
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Opt a kernel in to the largest dynamic shared memory the device allows next to its static shared

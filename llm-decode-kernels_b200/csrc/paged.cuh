@@ -122,6 +122,7 @@ struct Problem {
   float scale2;  // scale * log2(e)
   int mode;
   int tile_tokens;
+  int half_tokens;  // tokens of 128 rows (the tensor-core kernel); tile_tokens where a tile has at most 16 rows
   int n_tiles;  // kOneToken, kPrefix; kRagged: the plan's
   // kRagged: plan[0] = tiles, plan[1] = chunks of one kv head, then cum[max_tiles + 1], sequence[max_tiles],
   // first token[max_tiles]
@@ -141,8 +142,6 @@ struct Tile {
   int p0;        // position of the first one
   const int32_t* table;
 };
-
-__device__ __forceinline__ int plan_cum(const Problem& p, int i) { return p.plan[2 + i]; }
 
 __device__ __forceinline__ Tile tile_at(const Problem& p, int i) {
   Tile t;
@@ -179,7 +178,7 @@ __device__ __forceinline__ int64_t partial_slot(int ctas, int cta, bool from_sta
   return whole ? 2ll * ctas + unit : 2ll * cta + (from_start ? 1 : 0);
 }
 
-// Largest i with cum[i] <= x, for cum[0] = 0 <= x < cum[n].
+// Largest i with cum(i) <= x, for cum(0) = 0 <= x < cum(n); one thread.
 template <typename Cum>
 __device__ __forceinline__ int find_tile(const Cum& cum, int n, int x) {
   int lo = 0, hi = n;
@@ -192,6 +191,103 @@ __device__ __forceinline__ int find_tile(const Cum& cum, int n, int x) {
   }
   return lo;
 }
+
+// The same by a whole warp: 32 probes a round instead of one (two dependent loads for 1024 tiles, not ten).
+template <typename Cum>
+__device__ __forceinline__ int find_tile_warp(const Cum& cum, int n, int x, int lane) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) / 32, at = lo + step * (lane + 1);
+    const int below = __popc(__ballot_sync(0xffffffffu, at < hi && cum(at) <= x));
+    lo += step * below;
+    hi = min(hi, lo + step);
+  }
+  return lo;
+}
+
+// The chunks of one kv head before tile i, for the three ways a launch is cut into tiles.
+struct Line {
+  const int* cum_in;  // kOneToken, kRagged
+  int per_tile;       // kPrefix: chunks of each tile
+  int tiles, chunks;  // of one kv head
+  __device__ int cum(int i) const { return cum_in ? cum_in[i] : i * per_tile; }
+};
+
+// The line of a launch whose chunk sums lie in global memory (all but a kOneToken launch before its first CTA wrote them).
+__device__ __forceinline__ Line line_of(const Problem& p, int chunk) {
+  if (p.mode == kPrefix) {
+    const int per_tile = (p.prefix_len + chunk - 1) / chunk;
+    return {nullptr, per_tile, p.n_tiles, per_tile * p.n_tiles};
+  }
+  if (p.mode == kOneToken) return {p.cum_out, 0, p.n_tiles, p.cum_out[p.B]};
+  return {p.plan + 2, 0, p.plan[0], p.plan[1]};
+}
+
+// A CTA's piece of the line, unit by unit. Whole warps walk it.
+template <int kChunk>
+struct Walk {
+  const Problem& p;
+  const Line& line;
+  int64_t x, x1;
+  int next_h, next_t, next_c;
+  // the current part: chunks c0 .. c1 of the unit (h, ti)
+  int h, ti, c0, c1;
+  Tile t;
+  int last;  // the tile's last position
+  __device__ Walk(const Problem& p_, const Line& line_, int cta, int ctas, int lane) : p(p_), line(line_) {
+    const int64_t all = static_cast<int64_t>(line.chunks) * p.nkv, per = (all + ctas - 1) / ctas;
+    x = min(cta * per, all);
+    x1 = min(x + per, all);
+    next_h = next_t = next_c = 0;
+    if (x < x1) {
+      next_h = static_cast<int>(x / line.chunks);
+      const int r = static_cast<int>(x - static_cast<int64_t>(next_h) * line.chunks);
+      next_t = find_tile_warp([&](int i) { return line.cum(i); }, line.tiles, r, lane);
+      next_c = r - line.cum(next_t);
+    }
+  }
+  __device__ bool more() const { return x < x1; }
+  // Moves to the next part and returns the unit's chunks.
+  __device__ Span<kChunk> step() {
+    h = next_h, ti = next_t, c0 = next_c;
+    t = tile_at(p, ti);
+    last = tile_last(p, t);
+    const Span<kChunk> span(t.p0, last, p.mask, p.capacity);
+    c1 = static_cast<int>(min(static_cast<int64_t>(span.n), c0 + (x1 - x)));
+    x += c1 - c0;
+    next_c = 0;
+    if (++next_t == line.tiles) next_t = 0, ++next_h;
+    return span;
+  }
+};
+
+// Where the partial results of one unit lie: the CTAs first..last of the launch that took its chunks.
+struct Pieces {
+  int first, last;
+  int64_t whole_slot;
+};
+
+__device__ __forceinline__ Pieces pieces_of(int64_t u0, int64_t u1, int64_t per, int ctas, int64_t unit) {
+  return {static_cast<int>(u0 / per), static_cast<int>((u1 - 1) / per), 2ll * ctas + unit};
+}
+
+__device__ __forceinline__ int64_t piece_slot(const Pieces& w, int i) {
+  return w.first == w.last ? w.whole_slot : 2ll * i + (i == w.first ? 1 : 0);
+}
+
+// Row of a tile's results that holds head g of its token `tok`: tiles of more than half_tokens tokens have a second
+// half of 128 rows.
+__device__ __forceinline__ int result_row(const Problem& p, int tok, int g) {
+  return tok / p.half_tokens * 128 + tok % p.half_tokens * p.G + g;
+}
+
+// ------------------------------------------------------------------------------------------- host
+// The launch of the 256-row tensor-core kernel (paged_attention_tc.cu): CTAs of one wave (0: it does not fit).
+constexpr int kTcChunk = 128;
+constexpr int kTcRows = 256;
+int tc_ctas(int64_t head_dim, int dtype);
+int tc_launch(const Problem& p, int64_t nq, int64_t head_dim, int dtype, int ctas, const void* k_pages,
+              const void* v_pages, cudaStream_t st);
 
 }  // namespace paged
 }  // namespace dk

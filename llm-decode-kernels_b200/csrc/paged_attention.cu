@@ -113,17 +113,6 @@ struct Box {
 
 __device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"r"(kCWarps * 32) : "memory"); }
 
-// The chunks of one kv head before tile i (cum), for the three ways a launch is cut into tiles.
-struct Line {
-  const Problem& p;
-  const int* cum_sh;  // kOneToken: in shared memory
-  int per_tile;       // kPrefix
-  int tiles, chunks;  // of one kv head
-  __device__ int cum(int i) const {
-    return p.mode == kOneToken ? cum_sh[i] : p.mode == kPrefix ? i * per_tile : plan_cum(p, i);
-  }
-};
-
 template <typename T, int kHd, int kRows>
 __global__ void __launch_bounds__(kThreads)
     rows_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const Problem p,
@@ -158,7 +147,7 @@ __global__ void __launch_bounds__(kThreads)
   if (!wait_late) pdl_wait();
   pdl_trigger();
 
-  Line line{p, cum_sh, 0, p.n_tiles, 0};
+  Line line{cum_sh, 0, p.n_tiles, 0};
   if (p.mode == kOneToken) {  // every CTA sums up the sequences' chunks for itself
     int carry = 0;
     for (int b0 = 0; b0 < p.B; b0 += kThreads) {
@@ -187,18 +176,12 @@ __global__ void __launch_bounds__(kThreads)
     __syncthreads();
     if (blockIdx.x == 0)  // for the join kernel
       for (int i = tid; i <= p.B; i += kThreads) p.cum_out[i] = cum_sh[i];
-  } else if (p.mode == kPrefix) {
-    line.per_tile = (p.prefix_len + kChunk - 1) / kChunk;
-    line.chunks = line.per_tile * p.n_tiles;
   } else {
-    line.tiles = p.plan[0];
-    line.chunks = p.plan[1];
+    line = line_of(p, kChunk);
   }
   __syncthreads();
 
-  const int64_t all = static_cast<int64_t>(line.chunks) * p.nkv;
-  const int64_t per = (all + gridDim.x - 1) / gridDim.x;
-  const int64_t x0 = min(blockIdx.x * per, all), x1 = min(x0 + per, all);
+  Walk<kChunk> walk(p, line, blockIdx.x, gridDim.x, lane);
   bool ok = true;
   int fill = 0;  // ring fills so far
 
@@ -207,18 +190,14 @@ __global__ void __launch_bounds__(kThreads)
     const int box = min(p.page_size, kChunk);  // rows of one box
     const int boxes = kChunk / box;
     const int kv = lane & 1, sg = (lane >> 1) % B::kSegs, pg = lane / (2 * B::kSegs);
-    for (int64_t x = x0; x < x1 && ok;) {
-      const int h = static_cast<int>(x / line.chunks), r = static_cast<int>(x % line.chunks);
-      const int ti = find_tile([&](int i) { return line.cum(i); }, line.tiles, r);
-      const Tile t = tile_at(p, ti);
-      const Span<kChunk> span(t.p0, tile_last(p, t), p.mask, p.capacity);
-      const int c0 = r - line.cum(ti);
-      const int c1 = static_cast<int>(min(static_cast<int64_t>(span.n), c0 + (x1 - x)));
-      x += c1 - c0;
+    while (walk.more() && ok) {
+      const Span<kChunk> span = walk.step();
+      const int h = walk.h, c0 = walk.c0, c1 = walk.c1;
+      const int32_t* table = walk.t.table;
       // this lane's page in chunk i of the unit; INT_MIN: none, or nothing that a row sees
       auto entry = [&](int i) {
         const int j = span.chunk(i) * kChunk + pg * box;
-        return i < c1 && pg < boxes && span.needs(j, box, p.mask) ? __ldg(t.table + (j >> p.page_shift)) : INT_MIN;
+        return i < c1 && pg < boxes && span.needs(j, box, p.mask) ? table[j >> p.page_shift] : INT_MIN;
       };
       int next = entry(c0);
       for (int i = c0; i < c1; ++i, ++fill) {
@@ -247,15 +226,10 @@ __global__ void __launch_bounds__(kThreads)
     // ---------------------------------------------------------------- consumer warps
     const int g = lane >> 2, tq = lane & 3;
     const int mi = lane >> 3, rr = lane & 7;
-    for (int64_t x = x0; x < x1;) {
-      const int h = static_cast<int>(x / line.chunks), r = static_cast<int>(x % line.chunks);
-      const int ti = find_tile([&](int i) { return line.cum(i); }, line.tiles, r);
-      const Tile t = tile_at(p, ti);
-      const int plast = tile_last(p, t);
-      const Span<kChunk> span(t.p0, plast, p.mask, p.capacity);
-      const int c0 = r - line.cum(ti);
-      const int c1 = static_cast<int>(min(static_cast<int64_t>(span.n), c0 + (x1 - x)));
-      x += c1 - c0;
+    while (walk.more()) {
+      const Span<kChunk> span = walk.step();
+      const Tile t = walk.t;
+      const int h = walk.h, c0 = walk.c0, c1 = walk.c1, plast = walk.last;
       const int rows = t.ntok * p.G;
       // this lane's rows g and g + 8: positions, and q as the MMA's A operand
       int pos[kR];
@@ -384,7 +358,7 @@ __global__ void __launch_bounds__(kThreads)
         fin[2 * tid + 1] = ls;
       }
       consumers_sync();
-      const int64_t slot = partial_slot(gridDim.x, blockIdx.x, c0 == 0, all_of_it, h * line.tiles + ti);
+      const int64_t slot = partial_slot(gridDim.x, blockIdx.x, c0 == 0, all_of_it, h * line.tiles + walk.ti);
       if (ok) {
         for (int e = tid; e < rows * (kHd / 4); e += kCWarps * 32) {
           const int row = e / (kHd / 4), d = 4 * (e % (kHd / 4));
@@ -423,20 +397,6 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // ------------------------------------------------------------------------------------ join
-// Where the partial results of one unit lie: the CTAs first..last of the launch that took its chunks.
-struct Pieces {
-  int first, last;
-  int64_t whole_slot;
-};
-
-__device__ __forceinline__ Pieces pieces_of(int64_t u0, int64_t u1, int64_t per, int ctas, int64_t unit) {
-  return {static_cast<int>(u0 / per), static_cast<int>((u1 - 1) / per), 2ll * ctas + unit};
-}
-
-__device__ __forceinline__ int64_t piece_slot(const Pieces& w, int i) {
-  return w.first == w.last ? w.whole_slot : 2ll * i + (i == w.first ? 1 : 0);
-}
-
 // Adds one unit's partial results of one row to (m, l, acc): kD dims per lane.
 template <int kD>
 __device__ __forceinline__ void add_pieces(const Problem& p, const Pieces& w, int tile_rows, int row, int lane, float& m,
@@ -482,10 +442,6 @@ __device__ __forceinline__ void store_row(const Problem& p, int t, int head, int
 
 constexpr int kJoinWarps = 8;
 
-__device__ __forceinline__ int line_cum(const Problem& p, int per_tile, int i) {
-  return p.mode == kOneToken ? p.cum_out[i] : p.mode == kPrefix ? i * per_tile : plan_cum(p, i);
-}
-
 // Joins the units that a piece's end cuts. Block (i, y): the unit that holds the end of piece i, if that is the
 // first end inside it; a warp per row.
 template <typename T, int kHd>
@@ -493,23 +449,23 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_split_kernel(const Probl
   constexpr int kD = kHd / 32;
   pdl_trigger();
   pdl_wait();
-  const int tiles = p.mode == kRagged ? p.plan[0] : p.n_tiles;
-  const int chunks = p.mode == kRagged ? p.plan[1] : p.cum_out[p.B];
-  const int64_t all = static_cast<int64_t>(chunks) * p.nkv, per = (all + ctas - 1) / ctas;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Line line = line_of(p, 1);
+  const int64_t all = static_cast<int64_t>(line.chunks) * p.nkv, per = (all + ctas - 1) / ctas;
   const int64_t x = (blockIdx.x + 1ll) * per;
   if (x >= all) return;
-  const int h = static_cast<int>(x / chunks), r = static_cast<int>(x % chunks);
-  const int ti = find_tile([&](int i) { return line_cum(p, 0, i); }, tiles, r);
-  const int64_t u0 = static_cast<int64_t>(h) * chunks + line_cum(p, 0, ti);
-  const int64_t u1 = static_cast<int64_t>(h) * chunks + line_cum(p, 0, ti + 1);
+  const int h = static_cast<int>(x / line.chunks), r = static_cast<int>(x % line.chunks);
+  const int ti = find_tile_warp([&](int i) { return line.cum(i); }, line.tiles, r, lane);
+  const int64_t u0 = static_cast<int64_t>(h) * line.chunks + line.cum(ti);
+  const int64_t u1 = static_cast<int64_t>(h) * line.chunks + line.cum(ti + 1);
   if (u0 / per != blockIdx.x) return;
   const Pieces w = pieces_of(u0, u1, per, ctas, 0);
   const Tile t = tile_at(p, ti);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int row = blockIdx.y * kJoinWarps + warp; row < t.ntok * p.G; row += gridDim.y * kJoinWarps) {
+  for (int i = blockIdx.y * kJoinWarps + warp; i < t.ntok * p.G; i += gridDim.y * kJoinWarps) {
+    const int tok = i / p.G, g = i % p.G;
     float m = -INFINITY, l = 0.f, acc[kD] = {};
-    add_pieces<kD>(p, w, tile_rows, row, lane, m, l, acc);
-    store_row<T, kD>(p, t.t0 + row / p.G, h * p.G + row % p.G, lane, l, acc);
+    add_pieces<kD>(p, w, tile_rows, result_row(p, tok, g), lane, m, l, acc);
+    store_row<T, kD>(p, t.t0 + tok, h * p.G + g, lane, l, acc);
   }
 }
 
@@ -532,18 +488,18 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
     const int ti = t / a.tile_tokens, unit = h * a.n_tiles + ti;
     const int64_t all = static_cast<int64_t>(per_tile) * a.n_tiles * a.nkv, per = (all + a_ctas - 1) / a_ctas;
     const int64_t u0 = static_cast<int64_t>(unit) * per_tile;
-    add_pieces<kD>(a, pieces_of(u0, u0 + per_tile, per, a_ctas, unit), a_rows, (t % a.tile_tokens) * a.G + g, lane, m, l,
+    add_pieces<kD>(a, pieces_of(u0, u0 + per_tile, per, a_ctas, unit), a_rows, result_row(a, t % a.tile_tokens, g), lane, m, l,
                    acc);
   }
-  const int tiles = b.mode == kRagged ? b.plan[0] : b.n_tiles;
-  const int chunks = b.mode == kRagged ? b.plan[1] : b.cum_out[b.B];
-  if (chunks > 0) {
-    const int64_t all = static_cast<int64_t>(chunks) * b.nkv, per = (all + b_ctas - 1) / b_ctas;
-    const int ti = b.mode == kRagged ? find_tile([&](int i) { return b.plan[3 + 2 * b.max_tiles + i]; }, tiles, t) : t;
-    const int t0 = b.mode == kRagged ? b.plan[3 + 2 * b.max_tiles + ti] : t;
-    const int64_t u0 = static_cast<int64_t>(h) * chunks + line_cum(b, 0, ti);
-    const int64_t u1 = static_cast<int64_t>(h) * chunks + line_cum(b, 0, ti + 1);
-    add_pieces<kD>(b, pieces_of(u0, u1, per, b_ctas, h * tiles + ti), b_rows, (t - t0) * b.G + g, lane, m, l, acc);
+  const Line line = line_of(b, 1);
+  if (line.chunks > 0) {
+    const int64_t all = static_cast<int64_t>(line.chunks) * b.nkv, per = (all + b_ctas - 1) / b_ctas;
+    const int32_t* first = b.plan + 3 + 2 * b.max_tiles;  // kRagged: the tiles' first tokens
+    const int ti = b.mode == kRagged ? find_tile_warp([&](int i) { return first[i]; }, line.tiles, t, lane) : t;
+    const int t0 = b.mode == kRagged ? first[ti] : t;
+    const int64_t u0 = static_cast<int64_t>(h) * line.chunks + line.cum(ti);
+    const int64_t u1 = static_cast<int64_t>(h) * line.chunks + line.cum(ti + 1);
+    add_pieces<kD>(b, pieces_of(u0, u1, per, b_ctas, h * line.tiles + ti), b_rows, result_row(b, t - t0, g), lane, m, l, acc);
   }
   store_row<T, kD>(b, t, head, lane, l, acc);
 }
@@ -631,16 +587,25 @@ struct Cutter {
 // One launch over the chunks of one kind of tiles, with its areas of the workspace.
 struct Pass {
   Problem p;
+  bool tc;  // 256-row tiles on the tensor-core kernel
   RowsShape shape;
-  int rows;
+  int rows, ctas, chunk;
 };
 
-void cut_rows_pass(const Sizes& z, Cutter& c, Pass& a, bool always_partial) {
+void cut_pass(const Sizes& z, Cutter& c, Pass& a, bool always_partial) {
   Problem& p = a.p;
-  a.rows = rows_of(z, p.tile_tokens);
-  a.shape = rows_shape_of(z, a.rows);
+  if (a.tc) {
+    a.rows = kTcRows;
+    a.ctas = tc_ctas(z.hd, z.dtype);
+    a.chunk = kTcChunk;
+  } else {
+    a.rows = rows_of(z, p.tile_tokens);
+    a.shape = rows_shape_of(z, a.rows);
+    a.ctas = a.shape.ctas;
+    a.chunk = kChunk;
+  }
   const int64_t tiles = p.mode == kRagged ? p.max_tiles : p.n_tiles;
-  const int64_t slots = 2ll * a.shape.ctas + (always_partial ? z.nkv * tiles : 0);
+  const int64_t slots = 2ll * a.ctas + (always_partial ? z.nkv * tiles : 0);
   p.always_partial = always_partial;
   p.part_o = c.take<float>(slots * a.rows * z.hd);
   p.part_ml = c.take<float>(slots * a.rows * 2);
@@ -648,19 +613,28 @@ void cut_rows_pass(const Sizes& z, Cutter& c, Pass& a, bool always_partial) {
   p.plan = p.mode == kRagged ? c.take<int32_t>(3 + 3ll * p.max_tiles) : nullptr;
 }
 
-void shape_own(const Sizes& z, Problem& p) {
-  p.mode = z.ragged ? kRagged : kOneToken;
-  p.tile_tokens = rows_tile_tokens(z);
-  p.max_tiles = z.ragged ? static_cast<int>(z.T / p.tile_tokens + z.B) : 0;
-  p.n_tiles = static_cast<int>(z.B);
+// Tokens of a tile: of up to 16 rows, or of two halves of up to 128 rows each.
+void set_tile(const Sizes& z, Pass& a, int tokens16) {
+  const int G = static_cast<int>(z.nq / z.nkv);
+  a.p.half_tokens = a.tc ? 128 / G : tokens16;
+  a.p.tile_tokens = a.tc ? 2 * a.p.half_tokens : tokens16;
 }
 
-void shape_prefix(const Sizes& z, Problem& p) {
-  p.mode = kPrefix;
-  p.tile_tokens = std::max<int>(1, 16 / static_cast<int>(z.nq / z.nkv));
-  p.max_tiles = 0;
-  p.n_tiles = static_cast<int>((z.T + p.tile_tokens - 1) / p.tile_tokens);
-  p.prefix_len = static_cast<int>(z.prefix_len);
+void shape_own(const Sizes& z, Pass& a) {
+  a.tc = z.ragged;
+  a.p.mode = z.ragged ? kRagged : kOneToken;
+  set_tile(z, a, rows_tile_tokens(z));
+  a.p.max_tiles = z.ragged ? static_cast<int>(z.T / a.p.tile_tokens + z.B) : 0;
+  a.p.n_tiles = static_cast<int>(z.B);
+}
+
+void shape_prefix(const Sizes& z, Pass& a) {
+  const int G = static_cast<int>(z.nq / z.nkv);
+  a.tc = z.T * G > 16;  // up to 16 rows read the prefix once on the rows kernel as well
+  a.p.mode = kPrefix;
+  set_tile(z, a, std::max(1, 16 / G));
+  a.p.n_tiles = static_cast<int>((z.T + a.p.tile_tokens - 1) / a.p.tile_tokens);
+  a.p.prefix_len = static_cast<int>(z.prefix_len);
 }
 
 int check_sizes(const char* what, const Sizes& z) {
@@ -682,23 +656,23 @@ int check_sizes(const char* what, const Sizes& z) {
 template <typename T, int kHd>
 cudaError_t launch_join(const Sizes& z, cudaStream_t st, const Pass* prefix, const Pass& own) {
   if (prefix == nullptr) {
-    const dim3 grid(static_cast<unsigned>(own.shape.ctas - 1), static_cast<unsigned>((own.rows + kJoinWarps - 1) / kJoinWarps));
+    const dim3 grid(static_cast<unsigned>(own.ctas - 1), static_cast<unsigned>((own.rows + kJoinWarps - 1) / kJoinWarps));
     return launch(join_split_kernel<T, kHd>, grid, dim3(kJoinWarps * 32), 0, st, pdl_enabled(), dim3(1, 1, 1), own.p,
-                  own.shape.ctas, own.rows);
+                  own.ctas, own.rows);
   }
   const dim3 grid(static_cast<unsigned>((z.T * z.nq + kJoinWarps - 1) / kJoinWarps));
   return launch(join_prefix_kernel<T, kHd>, grid, dim3(kJoinWarps * 32), 0, st, pdl_enabled(), dim3(1, 1, 1), prefix->p,
-                prefix->shape.ctas, prefix->rows, kChunk, own.p, own.shape.ctas, own.rows);
+                prefix->ctas, prefix->rows, prefix->chunk, own.p, own.ctas, own.rows);
 }
 
 uint64_t workspace_of(const Sizes& z) {
   Cutter c{nullptr};
   Pass own = {}, pre = {};
-  shape_own(z, own.p);
-  cut_rows_pass(z, c, own, z.prefix_len > 0);
+  shape_own(z, own);
+  cut_pass(z, c, own, z.prefix_len > 0);
   if (z.prefix_len > 0) {
-    shape_prefix(z, pre.p);
-    cut_rows_pass(z, c, pre, true);
+    shape_prefix(z, pre);
+    cut_pass(z, c, pre, true);
   }
   return c.used;
 }
@@ -740,16 +714,16 @@ int attention(const char* what, const Sizes& z, const void* q, int64_t ldq, cons
     return set_error(DK_ERR_ALIGN, "%s: q rows, pages and out need 16-byte alignment, the workspace 256", what);
   Pass own = {}, pre = {};
   Cutter c{static_cast<char*>(workspace)};
-  shape_own(z, own.p);
-  cut_rows_pass(z, c, own, z.prefix_len > 0);
+  shape_own(z, own);
+  cut_pass(z, c, own, z.prefix_len > 0);
   if (z.prefix_len > 0) {
-    shape_prefix(z, pre.p);
-    cut_rows_pass(z, c, pre, true);
+    shape_prefix(z, pre);
+    cut_pass(z, c, pre, true);
   }
   if (c.used > workspace_bytes)
     return set_error(DK_ERR_INVALID, "%s: the workspace has %llu bytes, %llu are needed", what,
                      (unsigned long long)workspace_bytes, (unsigned long long)c.used);
-  if (own.shape.ctas == 0 || (z.prefix_len > 0 && pre.shape.ctas == 0))
+  if (own.ctas == 0 || (z.prefix_len > 0 && pre.ctas == 0))
     return set_error(DK_ERR_UNSUPPORTED, "%s: the kernel's shared memory does not fit this device", what);
   for (Problem* p : {&own.p, &pre.p}) {
     p->q = q, p->ldq = ldq, p->out = out;
@@ -775,10 +749,16 @@ int attention(const char* what, const Sizes& z, const void* q, int64_t ldq, cons
     return DK_ERR_CUDA;
   cudaError_t e = cudaSuccess;
   if (z.ragged)
-    e = launch(plan_kernel<kChunk>, dim3(1), dim3(kPlanThreads), 0, st, pdl_enabled(), dim3(1, 1, 1), own.p,
+    e = launch(plan_kernel<kTcChunk>, dim3(1), dim3(kPlanThreads), 0, st, pdl_enabled(), dim3(1, 1, 1), own.p,
                const_cast<int32_t*>(own.p.plan));
-  if (e == cudaSuccess && z.prefix_len > 0) e = launch_rows(z, pre.rows, pre.shape, st, mk, mv, pre.p, 0);
-  if (e == cudaSuccess) e = launch_rows(z, own.rows, own.shape, st, mk, mv, own.p, 0);
+  for (const Pass* a : {&pre, &own}) {
+    if (a->ctas == 0 || e != cudaSuccess) continue;
+    if (a->tc) {
+      if (const int rc = tc_launch(a->p, z.nq, z.hd, z.dtype, a->ctas, k_pages, v_pages, st)) return rc;
+    } else {
+      e = launch_rows(z, a->rows, a->shape, st, mk, mv, a->p, 0);
+    }
+  }
   const Pass* with = z.prefix_len > 0 ? &pre : nullptr;
   if (e == cudaSuccess) {
     if (z.dtype == DK_F16)

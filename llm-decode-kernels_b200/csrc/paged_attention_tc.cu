@@ -1,0 +1,480 @@
+// Attention over a paged cache for many query rows per kv head (prompts, and the prefix a batch shares) on the
+// 5th-generation tensor cores.
+//
+// A CTA works on units of 256 query rows (two halves A and B of up to 128 rows: the G heads of 128 / G tokens each) and
+// walks its chunks of 128 positions. Per chunk and half, S = Q K^T and O += P V are 128 x 128 x head_dim products,
+// 4 * 128^2 * head_dim flops, whose operands Q, K and V lie in shared memory and whose accumulators and P lie in tensor
+// memory:
+// * warp 9 streams Q (a box of the half's heads and tokens) and, page by page, K and V (64-dim columns of 128 rows) with
+//   TMA into the 128-byte-swizzled layout that tcgen05.mma reads; K's rows are contiguous along the product's inner
+//   dimension (K-major), V's along its outer one (N-major), so neither is transposed in memory;
+// * warp 8 issues the products, in the order PV_A(i), QK_A(i+1), PV_B(i), QK_B(i+1): while one half's softmax runs, the
+//   other half's products do. Products of one thread run in order, so P(i) may lie where S(i+1) will;
+// * warps 0-3 and 4-7 are the softmax of A and B, a thread per row: S from tensor memory, the row maximum, P = 2^(S - m) in
+//   16 bits back to tensor memory. The maximum that P refers to is raised only when a row's grows by 2^8 or more; then
+//   the row of O is rescaled in tensor memory (P stays below 2^8, far inside fp16; sums are fp32).
+// V rows that no row of the unit sees (past the end, between sinks and window, pages that were not read) are zeroed in
+// shared memory before the product, so that P = 0 does not meet a NaN; masked scores are replaced before the maximum.
+// Every wait is bounded.
+#include <climits>
+#include <mutex>
+
+#include "paged.cuh"
+#include "tcgen05.cuh"
+
+namespace dk {
+namespace paged {
+namespace {
+
+constexpr int kThreads = 384;
+constexpr int kMmaWarp = 8, kLoadWarp = 9;  // warps 10 and 11 only give their registers away
+// The launch holds 168 registers a thread; the softmax warpgroups take what the third one gives up:
+// 256 * 208 + 128 * 88 = 384 * 168.
+constexpr int kRegsLaunch = 168, kRegsSoftmax = 208, kRegsOther = 88;
+static_assert(256 * kRegsSoftmax + 128 * kRegsOther <= kThreads * kRegsLaunch, "register split");
+constexpr int kC = kTcChunk;
+constexpr float kLazy = 8.f;  // growth (base 2) of a row's maximum that P takes without rescaling O
+
+template <int kHd>
+struct Smem {
+  static constexpr int kSegs = kHd / 64;
+  static constexpr int kSegBytes = 128 * 128;            // 128 rows of 64 dims
+  static constexpr int kTileBytes = kSegs * kSegBytes;   // Q half, K chunk or V chunk
+  static constexpr int kSlots = kHd == 128 ? 5 : 10;
+  static constexpr int kBytes = 1024 + (2 + kSlots) * kTileBytes;
+};
+
+struct Barriers {
+  uint64_t kv_full[10], kv_empty[10];
+  uint64_t q_full, q_empty;
+  uint64_t s_full[2], p_full[2], o_full[2];
+  uint64_t drain;
+};
+
+// Shared-memory matrix descriptor of an N-major operand in the 128-byte-swizzled layout: rows of 128 bytes (64 values along
+// N), one row per value along K; 8-row atoms follow each other along K (stride byte offset 1024), blocks of 64 along N
+// lie kSegBytes apart (leading byte offset). The start moves along K by whole atoms.
+__device__ __forceinline__ uint64_t sdesc_n_sw128(uint32_t smem_byte_addr, uint32_t block_bytes) {
+  return static_cast<uint64_t>((smem_byte_addr >> 4) & 0x3FFF) | (static_cast<uint64_t>(block_bytes >> 4) << 16) |
+         (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// Instruction descriptor: fp32 accumulator, A and B both of type T, A K-major, B K-major or N-major.
+template <typename T>
+__host__ __device__ constexpr uint32_t idesc(int M, int N, bool b_n_major) {
+  const uint32_t type = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+  return (1u << 4) | (type << 7) | (type << 10) | (b_n_major ? 1u << 16 : 0u) | (static_cast<uint32_t>(N >> 3) << 17) |
+         (static_cast<uint32_t>(M >> 4) << 24);
+}
+
+// D[tmem] (+)= A[tmem] * B[smem] for one K = 16 slice: A is 128 rows (lanes) of 8 columns of 16-bit pairs.
+__device__ __forceinline__ void mma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+                                           uint32_t accumulate) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+      "[%5];" ::"r"(smem_addr(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar))
+      : "memory");
+}
+
+template <typename T, int kHd>
+__global__ void __launch_bounds__(kThreads, 1)
+    tiles_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+                 const __grid_constant__ CUtensorMap mv, const Problem p) {
+  using L = Smem<kHd>;
+  using E = Elem<T>;
+  constexpr uint32_t kS[2] = {0, 128}, kO[2] = {256, 256 + kHd};  // tensor-memory columns; P(X) lies over S(X)
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
+  uint8_t* q_sm = smem;
+  uint8_t* slots = smem + 2 * L::kTileBytes;
+  __shared__ __align__(8) Barriers bar;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int failed;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int i = 0; i < L::kSlots; ++i) {
+      mbar_init(&bar.kv_full[i], 1);
+      mbar_init(&bar.kv_empty[i], 1);
+    }
+    mbar_init(&bar.q_full, 1);
+    mbar_init(&bar.q_empty, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bar.s_full[i], 1);
+      mbar_init(&bar.p_full[i], 4);
+      mbar_init(&bar.o_full[i], 1);
+    }
+    mbar_init(&bar.drain, 1);
+    failed = 0;
+    fence_mbar_init();
+    prefetch_tensormap(&mq);
+    prefetch_tensormap(&mk);
+    prefetch_tensormap(&mv);
+  }
+  if (warp == kMmaWarp) {
+    tc::tmem_alloc(&tmem_slot, 512);
+    tc::tmem_relinquish();
+    tc::fence_before_sync();
+  }
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = tmem_slot;
+  pdl_wait();
+  pdl_trigger();
+
+  const Line line = line_of(p, kC);
+  Walk<kC> walk(p, line, blockIdx.x, gridDim.x, lane);
+  bool ok = true;
+
+  if (warp >= kMmaWarp) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
+  if (warp == kLoadWarp) {
+    // ---------------------------------------------------------------- loads
+    const int box = min(p.page_size, kC), boxes = kC / box;
+    const int sg = lane % L::kSegs, pg = lane / L::kSegs;
+    int fill = 0;
+    for (int part = 0; walk.more() && ok; ++part) {
+      const Span<kC> span = walk.step();
+      const int h = walk.h, c0 = walk.c0, c1 = walk.c1;
+      const int32_t* table = walk.t.table;
+      const bool two = walk.t.ntok > p.half_tokens;
+      auto entry = [&](int i) {  // this lane's page in chunk i of the unit; INT_MIN: none, or nothing that a row sees
+        const int j = span.chunk(i) * kC + pg * box;
+        return i < c1 && pg < boxes && span.needs(j, box, p.mask) ? table[j >> p.page_shift] : INT_MIN;
+      };
+      auto put = [&](const CUtensorMap* map, int i, int page) {
+        const int s = fill % L::kSlots;
+        if (fill >= L::kSlots && !mbar_wait(&bar.kv_empty[s], ((fill / L::kSlots) - 1) & 1, p.err, DK_DEVERR_WAIT_EMPTY))
+          ok = false;
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) return;
+        const bool mine = page != INT_MIN;
+        const unsigned want = __ballot_sync(0xffffffffu, mine);
+        if (lane == 0) mbar_arrive_expect_tx(&bar.kv_full[s], __popc(want) * box * 128);
+        __syncwarp();
+        if (mine) {
+          const int j = span.chunk(i) * kC + pg * box;
+          // a page outside the pool reads as zeros (a row past the map's end)
+          const int y = page >= 0 && page < p.n_pages ? (page * p.nkv + h) * p.page_size + (j & (p.page_size - 1))
+                                                      : p.n_pages * p.nkv * p.page_size;
+          tma_load_2d(slots + s * L::kTileBytes + sg * L::kSegBytes + pg * box * 128, map, sg * 64, y, &bar.kv_full[s]);
+        }
+        ++fill;
+      };
+      int page = entry(c0);
+      // Q, once the last part's products with it have completed
+      if (part > 0 && !mbar_wait(&bar.q_empty, (part - 1) & 1, p.err, DK_DEVERR_WAIT_EMPTY)) ok = false;
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&bar.q_full, (two ? 2 : 1) * L::kSegs * p.half_tokens * p.G * 128);
+        for (int x = 0; x < (two ? 2 : 1); ++x)
+          for (int s = 0; s < L::kSegs; ++s)
+            tma_load_3d(q_sm + x * L::kTileBytes + s * L::kSegBytes, &mq, s * 64, h * p.G,
+                        walk.t.t0 + x * p.half_tokens, &bar.q_full);
+      }
+      __syncwarp();
+      put(&mk, c0, page);
+      for (int i = c0; i < c1 && ok; ++i) {
+        const int next = entry(i + 1);
+        put(&mv, i, page);
+        if (i + 1 < c1 && ok) put(&mk, i + 1, next);
+        page = next;
+      }
+    }
+  } else if (warp == kMmaWarp) {
+    // ---------------------------------------------------------------- products (lane 0 issues)
+    int fill = 0;         // ring slots consumed
+    unsigned p_seen[2] = {0, 0};
+    auto slot_wait = [&](int f) {
+      if (ok && !mbar_wait(&bar.kv_full[f % L::kSlots], (f / L::kSlots) & 1, p.err, DK_DEVERR_WAIT_FULL)) ok = false;
+      ok = __all_sync(0xffffffffu, ok);
+    };
+    auto slot_at = [&](int f) { return smem_addr(slots + (f % L::kSlots) * L::kTileBytes); };
+    auto qk = [&](int x, int f) {
+      if (lane == 0) {
+        const uint32_t a0 = smem_addr(q_sm + x * L::kTileBytes), b0 = slot_at(f);
+#pragma unroll
+        for (int k = 0; k < kHd / 16; ++k) {
+          const uint32_t off = (k / 4) * L::kSegBytes + (k % 4) * 32;
+          tc::mma_f16(tmem + kS[x], tc::sdesc_k_sw128(a0 + off), tc::sdesc_k_sw128(b0 + off), idesc<T>(128, kC, false), k > 0);
+        }
+        tc::commit(&bar.s_full[x]);
+      }
+    };
+    auto pv = [&](int x, int f, bool first) {
+      if (ok && !mbar_wait(&bar.p_full[x], p_seen[x] & 1, p.err, DK_DEVERR_WAIT_FULL)) ok = false;
+      ++p_seen[x];
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) return;
+      tc::fence_after_sync();
+      if (lane == 0) {
+        const uint32_t b0 = slot_at(f);
+#pragma unroll
+        for (int k = 0; k < kC / 16; ++k)
+          mma_f16_ta(tmem + kO[x], tmem + kS[x] + 8 * k, sdesc_n_sw128(b0 + k * 2048, L::kSegBytes), idesc<T>(128, kHd, true),
+                     !first || k > 0);
+      }
+    };
+    for (int part = 0; walk.more() && ok; ++part) {
+      const Span<kC> span = walk.step();
+      const int n = walk.c1 - walk.c0;
+      const bool two = walk.t.ntok > p.half_tokens;
+      if (!mbar_wait(&bar.q_full, part & 1, p.err, DK_DEVERR_WAIT_FULL)) ok = false;
+      slot_wait(fill);
+      if (!ok) break;
+      tc::fence_after_sync();
+      qk(0, fill);
+      if (two) qk(1, fill);
+      if (lane == 0) {
+        tc::commit(&bar.kv_empty[fill % L::kSlots]);
+        if (n == 1) tc::commit(&bar.q_empty);
+      }
+      for (int i = 0; i < n && ok; ++i) {
+        const int fv = fill + 2 * i + 1, fk = fv + 1;
+        slot_wait(fv);
+        if (!ok) break;
+        const int j0 = span.chunk(walk.c0 + i) * kC;
+        // does every row of v belong to a position that some row of the unit sees?
+        const bool clear = j0 + kC <= span.end && (p.mask.window <= 0 || j0 >= span.lo || j0 + kC <= p.mask.sinks);
+        if (!clear) {
+          uint8_t* v = slots + (fv % L::kSlots) * L::kTileBytes;
+          for (int r = lane; r < kC; r += 32)
+            if (!span.needs(j0 + r, 1, p.mask))
+#pragma unroll
+              for (int c = 0; c < L::kSegs * 8; ++c)
+                *reinterpret_cast<uint4*>(v + (c / 8) * L::kSegBytes + r * 128 + (c % 8) * 16) = make_uint4(0, 0, 0, 0);
+          tc::fence_proxy_async_smem();
+          __syncwarp();
+        }
+        const bool more = i + 1 < n;
+        pv(0, fv, i == 0);
+        if (!ok) break;
+        if (more) {
+          slot_wait(fk);
+          if (!ok) break;
+          qk(0, fk);
+        } else if (lane == 0) {
+          tc::commit(&bar.o_full[0]);
+        }
+        if (two) {
+          pv(1, fv, i == 0);
+          if (!ok) break;
+          if (more)
+            qk(1, fk);
+          else if (lane == 0)
+            tc::commit(&bar.o_full[1]);
+        }
+        if (lane == 0) {
+          tc::commit(&bar.kv_empty[fv % L::kSlots]);
+          if (more) tc::commit(&bar.kv_empty[fk % L::kSlots]);
+          if (i + 2 == n) tc::commit(&bar.q_empty);
+        }
+      }
+      fill += 2 * n;
+    }
+  } else if (warp < kMmaWarp) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+    // ---------------------------------------------------------------- softmax: a thread per row
+    const int x = warp >> 2, r = tid & 127;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t s_col = tmem + lanes + kS[x], o_col = tmem + lanes + kO[x];
+    unsigned s_seen = 0, o_seen = 0;
+    while (walk.more() && ok) {
+      const Span<kC> span = walk.step();
+      const Tile t = walk.t;
+      const int first = x * p.half_tokens;  // this half's first token
+      if (t.ntok <= first) continue;
+      const int tok = first + r / p.G, head = walk.h * p.G + r % p.G;
+      const bool live = r < p.half_tokens * p.G && tok < t.ntok;
+      const int pos = live ? row_position(p, t, tok) : INT_MIN;
+      const int p_lo = row_position(p, t, first), p_hi = row_position(p, t, min(t.ntok, first + p.half_tokens) - 1);
+      float m = -INFINITY, l = 0.f;  // of scale2 * score
+      for (int i = walk.c0; i < walk.c1; ++i) {
+        if (!mbar_wait(&bar.s_full[x], s_seen & 1, p.err, DK_DEVERR_WAIT_FULL)) ok = false;
+        ++s_seen;
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc::fence_after_sync();
+        float s[kC];
+#pragma unroll
+        for (int c = 0; c < kC / 32; ++c) tc::tmem_ld32(s_col + 32 * c, *reinterpret_cast<float(*)[32]>(&s[32 * c]));
+        const int j0 = span.chunk(i) * kC;
+        const bool clear = j0 + kC - 1 <= p_lo && j0 + kC <= span.end &&
+                           (p.mask.window <= 0 || j0 > p_hi - p.mask.window || j0 + kC <= p.mask.sinks);
+        if (!clear) {
+          const int end = min(span.end, pos + 1);  // (INT_MIN + 1 for a row that is none)
+          const int lo = p.mask.window > 0 ? pos - p.mask.window + 1 : INT_MIN;
+#pragma unroll
+          for (int c = 0; c < kC; ++c) {
+            const int j = j0 + c;
+            if (!(j < end && (j >= lo || j < p.mask.sinks))) s[c] = -INFINITY;
+          }
+        }
+        float mx = s[0];
+#pragma unroll
+        for (int c = 1; c < kC; ++c) mx = fmaxf(mx, s[c]);
+        mx *= p.scale2;
+        const bool raise = mx > m + kLazy || (m == -INFINITY && mx > -INFINITY);
+        float keep = 1.f;
+        if (raise) {
+          keep = exp2_approx(m - mx);
+          m = mx;
+          l *= keep;
+        }
+        if (__any_sync(0xffffffffu, raise) && i > walk.c0) {  // O's products up to the last chunk are done: S came after them
+#pragma unroll
+          for (int c = 0; c < kHd / 16; ++c) {
+            float o[16];
+            uint32_t w[16];
+            tc::tmem_ld16(o_col + 16 * c, o);
+#pragma unroll
+            for (int d = 0; d < 16; ++d) w[d] = __float_as_uint(o[d] * keep);
+            tmem_st16(o_col + 16 * c, w);
+          }
+        }
+        const float base = m == -INFINITY ? 0.f : m;
+        float sum = 0.f;
+#pragma unroll
+        for (int c = 0; c < kC / 32; ++c) {
+          uint32_t w[16];
+#pragma unroll
+          for (int d = 0; d < 16; ++d) {
+            const float a = exp2_approx(fmaf(s[32 * c + 2 * d], p.scale2, -base));
+            const float b = exp2_approx(fmaf(s[32 * c + 2 * d + 1], p.scale2, -base));
+            sum += a + b;
+            w[d] = E::pack(a, b);
+          }
+          tmem_st16(s_col + 16 * c, w);
+        }
+        l += sum;
+        tmem_wait_st();
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar.p_full[x]);
+      }
+      if (ok && !mbar_wait(&bar.o_full[x], o_seen & 1, p.err, DK_DEVERR_WAIT_FULL)) ok = false;
+      ++o_seen;
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc::fence_after_sync();
+      const bool all_of_it = walk.c0 == 0 && walk.c1 == span.n, whole = all_of_it && !p.always_partial;
+      const int64_t slot = partial_slot(gridDim.x, blockIdx.x, walk.c0 == 0, all_of_it, walk.h * line.tiles + walk.ti);
+      const int row = x * 128 + r;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      T* out = static_cast<T*>(p.out) + (static_cast<int64_t>(t.t0 + tok) * p.nkv * p.G + head) * kHd;
+      float* part = p.part_o + (slot * kTcRows + row) * kHd;
+#pragma unroll
+      for (int c = 0; c < kHd / 16; ++c) {
+        float o[16];
+        tc::tmem_ld16(o_col + 16 * c, o);
+        if (!live) continue;
+        if (whole) {
+          uint32_t w[8];
+#pragma unroll
+          for (int d = 0; d < 8; ++d) w[d] = E::pack(o[2 * d] * inv, o[2 * d + 1] * inv);
+          *reinterpret_cast<uint4*>(out + 16 * c) = make_uint4(w[0], w[1], w[2], w[3]);
+          *reinterpret_cast<uint4*>(out + 16 * c + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+        } else {
+#pragma unroll
+          for (int d = 0; d < 4; ++d)
+            *reinterpret_cast<float4*>(part + 16 * c + 4 * d) = make_float4(o[4 * d], o[4 * d + 1], o[4 * d + 2], o[4 * d + 3]);
+        }
+      }
+      if (!whole && live) *reinterpret_cast<float2*>(&p.part_ml[(slot * kTcRows + row) * 2]) = make_float2(m, l);
+      tc::fence_before_sync();
+    }
+  }
+
+  __syncwarp();
+  if (!ok && lane == 0) failed = 1;
+  tc::fence_before_sync();
+  __syncthreads();
+  if (failed && warp == kMmaWarp) {
+    // a wait gave up: let products and copies still in flight finish before their memory goes away (bounded)
+    if (lane == 0) {
+      tc::commit(&bar.drain);
+      const uint64_t t0 = globaltimer_ns();
+      while (!mbar_try_wait(&bar.drain, 0) && globaltimer_ns() - t0 < 500000000ull) {
+      }
+      const uint64_t t1 = globaltimer_ns();
+      while (globaltimer_ns() - t1 < 20000000ull) {  // 20 ms: far more than any copy takes
+      }
+    }
+    __syncwarp();
+  }
+  tc::fence_after_sync();
+  if (warp == kMmaWarp) tc::tmem_dealloc(tmem, 512);
+}
+
+bool make_q_map(CUtensorMap* map, const Problem& p, int64_t nq, int64_t hd, CUtensorMapDataType type) {
+  const uint64_t dims[3] = {static_cast<uint64_t>(hd), static_cast<uint64_t>(nq), static_cast<uint64_t>(p.T)};
+  const uint64_t strides[2] = {static_cast<uint64_t>(hd) * 2, static_cast<uint64_t>(p.ldq) * 2};
+  const uint32_t box[3] = {64, static_cast<uint32_t>(p.G), static_cast<uint32_t>(p.half_tokens)};
+  return make_tensor_map(map, p.q, type, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <typename T, int kHd>
+int ctas_of() {
+  static std::mutex mu;
+  static int known[64];  // by device; 0: not asked yet, -1: does not fit
+  int dev = 0;
+  cudaGetDevice(&dev);
+  std::lock_guard<std::mutex> lock(mu);
+  int& n = known[dev & 63];
+  if (n == 0) {
+    cudaFuncAttributes a;  // the register split needs the launch to hold exactly what it divides
+    const bool split = cudaFuncGetAttributes(&a, tiles_kernel<T, kHd>) == cudaSuccess && a.numRegs == kRegsLaunch;
+    n = split && opt_in_dynamic_smem(tiles_kernel<T, kHd>) >= Smem<kHd>::kBytes ? device_info().num_sms : -1;
+  }
+  return n < 0 ? 0 : n;
+}
+
+}  // namespace
+
+int tc_ctas(int64_t head_dim, int dtype) {
+  if (dtype == DK_F16) return head_dim == 128 ? ctas_of<__half, 128>() : ctas_of<__half, 64>();
+  return head_dim == 128 ? ctas_of<__nv_bfloat16, 128>() : ctas_of<__nv_bfloat16, 64>();
+}
+
+int tc_launch(const Problem& p, int64_t nq, int64_t hd, int dtype, int ctas, const void* k_pages, const void* v_pages,
+              cudaStream_t st) {
+  const CUtensorMapDataType type = dtype == DK_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const uint64_t rows = static_cast<uint64_t>(p.n_pages) * p.nkv * p.page_size;
+  const uint32_t box = static_cast<uint32_t>(p.page_size < kC ? p.page_size : kC);
+  CUtensorMap mq, mk, mv;
+  if (!make_q_map(&mq, p, nq, hd, type) ||
+      !make_tensor_map_2d(&mk, k_pages, type, hd, rows, hd * 2, 64, box, CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !make_tensor_map_2d(&mv, v_pages, type, hd, rows, hd * 2, 64, box, CU_TENSOR_MAP_SWIZZLE_128B))
+    return DK_ERR_CUDA;
+  cudaError_t e;
+#define DK_TILES(TT, HH) \
+  launch(tiles_kernel<TT, HH>, dim3(ctas), dim3(kThreads), Smem<HH>::kBytes, st, pdl_enabled(), dim3(1, 1, 1), mq, mk, mv, p)
+  if (dtype == DK_F16)
+    e = hd == 128 ? DK_TILES(__half, 128) : DK_TILES(__half, 64);
+  else
+    e = hd == 128 ? DK_TILES(__nv_bfloat16, 128) : DK_TILES(__nv_bfloat16, 64);
+#undef DK_TILES
+  if (e != cudaSuccess) return set_error(DK_ERR_CUDA, "paged attention (256-row tiles) launch: %s", cudaGetErrorString(e));
+  return DK_OK;
+}
+
+}  // namespace paged
+}  // namespace dk

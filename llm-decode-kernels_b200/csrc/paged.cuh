@@ -69,6 +69,22 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
+// Bounded wait like mbar_wait, for waits on a loop's critical path: the timer, whose read takes longer than most of these
+// waits, is looked at only once in 256 unsuccessful polls.
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, int* err, int code) {
+  uint64_t t0 = 0;
+  for (uint32_t i = 1; !mbar_try_wait(bar, parity); ++i) {
+    if ((i & 255) != 0) continue;
+    const uint64_t now = globaltimer_ns();
+    if (t0 == 0) t0 = now;
+    if (now - t0 > kWaitLimitNs) {
+      record_device_error(err, code);
+      return false;
+    }
+  }
+  return true;
+}
+
 // ------------------------------------------------------------------------------------ visible positions
 // A row at position p sees position j when j <= p and (window <= 0 or j > p - window or j < sinks).
 struct Mask {
@@ -123,10 +139,12 @@ struct Problem {
   int mode;
   int tile_tokens;
   int half_tokens;  // tokens of 128 rows (the tensor-core kernel); tile_tokens where a tile has at most 16 rows
-  int n_tiles;  // kOneToken, kPrefix; kRagged: the plan's
-  // kRagged: plan[0] = tiles, plan[1] = chunks of one kv head, then cum[max_tiles + 1], sequence[max_tiles],
-  // first token[max_tiles]
+  int unit_extra;   // chunks added to a unit's length on the line for what it costs besides its chunks
+  int n_tiles;      // kOneToken, kPrefix; kRagged: the plan's
+  // kRagged: plan[0] = tiles, plan[1] = length of one kv head's line, then cum[max_tiles + 1]; what tile_at needs of
+  // each tile lies in tile_info
   const int32_t* plan;
+  const int4* tile_info;  // {first token, tokens, position of the first one, sequence}
   int max_tiles;
   int32_t* cum_out;  // kOneToken: [B + 1], the chunks of one kv head before each sequence
   // Partial results: a CTA's first piece of a unit that began before it (slot 2 * CTA), its last piece of a unit that
@@ -156,12 +174,9 @@ __device__ __forceinline__ Tile tile_at(const Problem& p, int i) {
     t.p0 = p.prefix_len - 1;
     t.table = p.table;
   } else {
-    const int b = p.plan[3 + p.max_tiles + i];
-    t.t0 = p.plan[3 + 2 * p.max_tiles + i];
-    const int t1 = min(p.starts[b + 1], p.T);
-    t.ntok = min(p.tile_tokens, t1 - t.t0);
-    t.p0 = p.lengths[b] - (t1 - t.t0);
-    t.table = p.table + b * p.ld_table;
+    const int4 v = p.tile_info[i];
+    t.t0 = v.x, t.ntok = v.y, t.p0 = v.z;
+    t.table = p.table + v.w * p.ld_table;
   }
   return t;
 }
@@ -208,7 +223,7 @@ __device__ __forceinline__ int find_tile_warp(const Cum& cum, int n, int x, int 
 // The chunks of one kv head before tile i, for the three ways a launch is cut into tiles.
 struct Line {
   const int* cum_in;  // kOneToken, kRagged
-  int per_tile;       // kPrefix: chunks of each tile
+  int per_tile;       // kPrefix: length of each tile
   int tiles, chunks;  // of one kv head
   __device__ int cum(int i) const { return cum_in ? cum_in[i] : i * per_tile; }
 };
@@ -216,7 +231,7 @@ struct Line {
 // The line of a launch whose chunk sums lie in global memory (all but a kOneToken launch before its first CTA wrote them).
 __device__ __forceinline__ Line line_of(const Problem& p, int chunk) {
   if (p.mode == kPrefix) {
-    const int per_tile = (p.prefix_len + chunk - 1) / chunk;
+    const int per_tile = (p.prefix_len + chunk - 1) / chunk + p.unit_extra;
     return {nullptr, per_tile, p.n_tiles, per_tile * p.n_tiles};
   }
   if (p.mode == kOneToken) return {p.cum_out, 0, p.n_tiles, p.cum_out[p.B]};
@@ -232,8 +247,8 @@ struct Walk {
   int next_h, next_t, next_c;
   // the current part: chunks c0 .. c1 of the unit (h, ti)
   int h, ti, c0, c1;
-  Tile t;
-  int last;  // the tile's last position
+  Tile t, next_tile;  // (the next tile's fields are loaded a part ahead)
+  int last;           // the tile's last position
   __device__ Walk(const Problem& p_, const Line& line_, int cta, int ctas, int lane) : p(p_), line(line_) {
     const int64_t all = static_cast<int64_t>(line.chunks) * p.nkv, per = (all + ctas - 1) / ctas;
     x = min(cta * per, all);
@@ -244,19 +259,23 @@ struct Walk {
       const int r = static_cast<int>(x - static_cast<int64_t>(next_h) * line.chunks);
       next_t = find_tile_warp([&](int i) { return line.cum(i); }, line.tiles, r, lane);
       next_c = r - line.cum(next_t);
+      next_tile = tile_at(p, next_t);
     }
   }
   __device__ bool more() const { return x < x1; }
-  // Moves to the next part and returns the unit's chunks.
+  // Moves to the next part and returns the unit's chunks. A part may be empty (c1 <= c0): the end of a unit's stretch
+  // of the line that stands for its fixed cost.
   __device__ Span<kChunk> step() {
     h = next_h, ti = next_t, c0 = next_c;
-    t = tile_at(p, ti);
+    t = next_tile;
     last = tile_last(p, t);
     const Span<kChunk> span(t.p0, last, p.mask, p.capacity);
-    c1 = static_cast<int>(min(static_cast<int64_t>(span.n), c0 + (x1 - x)));
-    x += c1 - c0;
+    const int to = static_cast<int>(min(static_cast<int64_t>(span.n + p.unit_extra), c0 + (x1 - x)));
+    x += to - c0;
+    c1 = min(to, span.n);
     next_c = 0;
     if (++next_t == line.tiles) next_t = 0, ++next_h;
+    if (x < x1) next_tile = tile_at(p, next_t);
     return span;
   }
 };
@@ -267,8 +286,9 @@ struct Pieces {
   int64_t whole_slot;
 };
 
-__device__ __forceinline__ Pieces pieces_of(int64_t u0, int64_t u1, int64_t per, int ctas, int64_t unit) {
-  return {static_cast<int>(u0 / per), static_cast<int>((u1 - 1) / per), 2ll * ctas + unit};
+// The unit's stretch of the line is u0 .. u1, `extra` of it at its end without chunks.
+__device__ __forceinline__ Pieces pieces_of(int64_t u0, int64_t u1, int extra, int64_t per, int ctas, int64_t unit) {
+  return {static_cast<int>(u0 / per), static_cast<int>((u1 - extra - 1) / per), 2ll * ctas + unit};
 }
 
 __device__ __forceinline__ int64_t piece_slot(const Pieces& w, int i) {
@@ -285,6 +305,7 @@ __device__ __forceinline__ int result_row(const Problem& p, int tok, int g) {
 // The launch of the 256-row tensor-core kernel (paged_attention_tc.cu): CTAs of one wave (0: it does not fit).
 constexpr int kTcChunk = 128;
 constexpr int kTcRows = 256;
+constexpr int kTcUnitExtra = 3;  // a unit's fixed cost (its Q, first and last steps, output) in chunks
 int tc_ctas(int64_t head_dim, int dtype);
 int tc_launch(const Problem& p, int64_t nq, int64_t head_dim, int dtype, int ctas, const void* k_pages,
               const void* v_pages, cudaStream_t st);

@@ -32,8 +32,13 @@ constexpr int kPlanThreads = 1024;
 // ------------------------------------------------------------------------------------ ragged plan
 // One CTA cuts the sequences into tiles of tile_tokens tokens and sums up their chunks.
 template <int kUnitChunk>
-__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Problem p, int32_t* plan) {
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Problem p, int32_t* plan, int4* info) {
+  constexpr int kOwnTiles = 4;  // tiles of a sequence that its own thread writes
   __shared__ int warp_sum[kPlanThreads / 32];
+  __shared__ int long_count;
+  __shared__ int4 long_seq[kPlanThreads];  // {first tile, tiles, first token, end}
+  __shared__ int2 long_len[kPlanThreads];  // {length, sequence}
+  if (threadIdx.x == 0) long_count = 0;
   pdl_trigger();
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -59,9 +64,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Problem p, int
     return (warp == 0 ? 0 : before) + s - v;
   };
   int32_t* cum = plan + 2;
-  int32_t* seq = plan + 3 + p.max_tiles;
-  int32_t* first = plan + 3 + 2 * p.max_tiles;
-  int tiles = 0, chunks = 0;
+  int tiles = 0, length = 0;
   for (int b0 = 0; b0 < p.B; b0 += kPlanThreads) {
     const int b = b0 + tid;
     const int t0 = b < p.B ? min(max(p.starts[b], 0), p.T) : 0;
@@ -69,32 +72,44 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Problem p, int
     const int mine = (t1 - t0 + p.tile_tokens - 1) / p.tile_tokens;
     int total;
     const int at = tiles + scan(mine, total);
-    for (int i = 0; i < mine && at + i < p.max_tiles; ++i) {
-      seq[at + i] = b;
-      first[at + i] = t0 + i * p.tile_tokens;
+    // sequence and first token of each tile; long sequences are filled in by the whole CTA below
+    if (mine > 0 && at < p.max_tiles) info[at] = make_int4(t0, t1, p.lengths[b], b);
+    for (int i = 1; i < min(mine, kOwnTiles) && at + i < p.max_tiles; ++i)
+      info[at + i] = make_int4(t0 + i * p.tile_tokens, t1, p.lengths[b], b);
+    __syncthreads();
+    if (mine > kOwnTiles) {
+      const int k = atomicAdd(&long_count, 1);
+      long_seq[k] = make_int4(at, mine, t0, t1);
+      long_len[k] = make_int2(p.lengths[b], b);
     }
+    __syncthreads();
+    for (int k = 0; k < long_count; ++k)
+      for (int i = kOwnTiles + tid; i < long_seq[k].y && long_seq[k].x + i < p.max_tiles; i += kPlanThreads)
+        info[long_seq[k].x + i] = make_int4(long_seq[k].z + i * p.tile_tokens, long_seq[k].w, long_len[k].x, long_len[k].y);
+    __syncthreads();
+    if (tid == 0) long_count = 0;
     tiles += total;
   }
   tiles = min(tiles, p.max_tiles);
-  __syncthreads();  // the tiles' sequences and first tokens, written above, are read by other threads below
+  __syncthreads();  // the tiles written above are read by other threads below
   for (int i0 = 0; i0 < tiles; i0 += kPlanThreads) {
     const int i = i0 + tid;
     int n = 0;
     if (i < tiles) {
-      const int b = seq[i], t0 = first[i];
-      const int t1 = min(p.starts[b + 1], p.T), ntok = min(p.tile_tokens, t1 - t0);
-      const int p0 = p.lengths[b] - (t1 - t0);
-      n = Span<kUnitChunk>(p0, p0 + ntok - 1, p.mask, p.capacity).n;
+      const int4 v = info[i];  // {first token, sequence's end, length, sequence}
+      const int ntok = min(p.tile_tokens, v.y - v.x), p0 = v.z - (v.y - v.x);
+      info[i] = make_int4(v.x, ntok, p0, v.w);
+      n = Span<kUnitChunk>(p0, p0 + ntok - 1, p.mask, p.capacity).n + p.unit_extra;
     }
     int total;
-    const int at = chunks + scan(n, total);
+    const int at = length + scan(n, total);
     if (i < tiles) cum[i] = at;
-    chunks += total;
+    length += total;
   }
   if (tid == 0) {
-    cum[tiles] = chunks;
+    cum[tiles] = length;
     plan[0] = tiles;
-    plan[1] = chunks;
+    plan[1] = length;
   }
 }
 
@@ -204,7 +219,7 @@ __global__ void __launch_bounds__(kThreads)
         const int page = next;
         next = entry(i + 1);
         const int s = fill % ring;
-        if (fill >= ring && !mbar_wait(&empty[s], ((fill / ring) - 1) & 1, p.err, DK_DEVERR_WAIT_EMPTY)) ok = false;
+        if (fill >= ring && !wait_for(&empty[s], ((fill / ring) - 1) & 1, p.err, DK_DEVERR_WAIT_EMPTY)) ok = false;
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         const bool mine = page != INT_MIN;
@@ -255,7 +270,7 @@ __global__ void __launch_bounds__(kThreads)
 
       for (int i = c0; i < c1; ++i, ++fill) {
         const int s = fill % ring;
-        if (ok && !mbar_wait(&full[s], (fill / ring) & 1, p.err, DK_DEVERR_WAIT_FULL)) ok = false;
+        if (ok && !wait_for(&full[s], (fill / ring) & 1, p.err, DK_DEVERR_WAIT_FULL)) ok = false;
         ok = __all_sync(0xffffffffu, ok);
         const int j0 = span.chunk(i) * kChunk + 16 * warp;  // this warp's 16 positions
         if (ok && span.needs(j0, 16, p.mask)) {
@@ -459,7 +474,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_split_kernel(const Probl
   const int64_t u0 = static_cast<int64_t>(h) * line.chunks + line.cum(ti);
   const int64_t u1 = static_cast<int64_t>(h) * line.chunks + line.cum(ti + 1);
   if (u0 / per != blockIdx.x) return;
-  const Pieces w = pieces_of(u0, u1, per, ctas, 0);
+  const Pieces w = pieces_of(u0, u1, p.unit_extra, per, ctas, 0);
+  if (w.first == w.last) return;
   const Tile t = tile_at(p, ti);
   for (int i = blockIdx.y * kJoinWarps + warp; i < t.ntok * p.G; i += gridDim.y * kJoinWarps) {
     const int tok = i / p.G, g = i % p.G;
@@ -484,22 +500,21 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
   const int h = head / a.G, g = head % a.G;
   float m = -INFINITY, l = 0.f, acc[kD] = {};
   {
-    const int per_tile = (a.prefix_len + a_chunk - 1) / a_chunk;
+    const Line line = line_of(a, a_chunk);
     const int ti = t / a.tile_tokens, unit = h * a.n_tiles + ti;
-    const int64_t all = static_cast<int64_t>(per_tile) * a.n_tiles * a.nkv, per = (all + a_ctas - 1) / a_ctas;
-    const int64_t u0 = static_cast<int64_t>(unit) * per_tile;
-    add_pieces<kD>(a, pieces_of(u0, u0 + per_tile, per, a_ctas, unit), a_rows, result_row(a, t % a.tile_tokens, g), lane, m, l,
+    const int64_t all = static_cast<int64_t>(line.chunks) * a.nkv, per = (all + a_ctas - 1) / a_ctas;
+    const int64_t u0 = static_cast<int64_t>(unit) * line.per_tile;
+    add_pieces<kD>(a, pieces_of(u0, u0 + line.per_tile, a.unit_extra, per, a_ctas, unit), a_rows, result_row(a, t % a.tile_tokens, g), lane, m, l,
                    acc);
   }
   const Line line = line_of(b, 1);
   if (line.chunks > 0) {
     const int64_t all = static_cast<int64_t>(line.chunks) * b.nkv, per = (all + b_ctas - 1) / b_ctas;
-    const int32_t* first = b.plan + 3 + 2 * b.max_tiles;  // kRagged: the tiles' first tokens
-    const int ti = b.mode == kRagged ? find_tile_warp([&](int i) { return first[i]; }, line.tiles, t, lane) : t;
-    const int t0 = b.mode == kRagged ? first[ti] : t;
+    const int ti = b.mode == kRagged ? find_tile_warp([&](int i) { return b.tile_info[i].x; }, line.tiles, t, lane) : t;
+    const int t0 = b.mode == kRagged ? b.tile_info[ti].x : t;
     const int64_t u0 = static_cast<int64_t>(h) * line.chunks + line.cum(ti);
     const int64_t u1 = static_cast<int64_t>(h) * line.chunks + line.cum(ti + 1);
-    add_pieces<kD>(b, pieces_of(u0, u1, per, b_ctas, h * line.tiles + ti), b_rows, result_row(b, t - t0, g), lane, m, l, acc);
+    add_pieces<kD>(b, pieces_of(u0, u1, b.unit_extra, per, b_ctas, h * line.tiles + ti), b_rows, result_row(b, t - t0, g), lane, m, l, acc);
   }
   store_row<T, kD>(b, t, head, lane, l, acc);
 }
@@ -596,6 +611,7 @@ void cut_pass(const Sizes& z, Cutter& c, Pass& a, bool always_partial) {
   Problem& p = a.p;
   if (a.tc) {
     a.rows = kTcRows;
+    p.unit_extra = kTcUnitExtra;
     a.ctas = tc_ctas(z.hd, z.dtype);
     a.chunk = kTcChunk;
   } else {
@@ -610,7 +626,8 @@ void cut_pass(const Sizes& z, Cutter& c, Pass& a, bool always_partial) {
   p.part_o = c.take<float>(slots * a.rows * z.hd);
   p.part_ml = c.take<float>(slots * a.rows * 2);
   p.cum_out = p.mode == kOneToken ? c.take<int32_t>(z.B + 1) : nullptr;
-  p.plan = p.mode == kRagged ? c.take<int32_t>(3 + 3ll * p.max_tiles) : nullptr;
+  p.plan = p.mode == kRagged ? c.take<int32_t>(3 + static_cast<int64_t>(p.max_tiles)) : nullptr;
+  p.tile_info = p.mode == kRagged ? c.take<int4>(p.max_tiles) : nullptr;
 }
 
 // Tokens of a tile: of up to 16 rows, or of two halves of up to 128 rows each.
@@ -750,7 +767,7 @@ int attention(const char* what, const Sizes& z, const void* q, int64_t ldq, cons
   cudaError_t e = cudaSuccess;
   if (z.ragged)
     e = launch(plan_kernel<kTcChunk>, dim3(1), dim3(kPlanThreads), 0, st, pdl_enabled(), dim3(1, 1, 1), own.p,
-               const_cast<int32_t*>(own.p.plan));
+               const_cast<int32_t*>(own.p.plan), const_cast<int4*>(own.p.tile_info));
   for (const Pass* a : {&pre, &own}) {
     if (a->ctas == 0 || e != cudaSuccess) continue;
     if (a->tc) {

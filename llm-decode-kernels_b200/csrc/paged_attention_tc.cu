@@ -67,13 +67,30 @@ __host__ __device__ constexpr uint32_t idesc(int M, int N, bool b_n_major) {
          (static_cast<uint32_t>(M >> 4) << 24);
 }
 
-// D[tmem] (+)= A[tmem] * B[smem] for one K = 16 slice: A is 128 rows (lanes) of 8 columns of 16-bit pairs.
-__device__ __forceinline__ void mma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
-                                           uint32_t accumulate) {
+// The products are issued by whole warps with one lane elected inside the instruction sequence: the operands stay
+// warp-uniform values, where a branch on the lane would make each of them a value of one thread (and a product took
+// about 130 cycles to issue, twice its execution).
+// D[tmem] (+)= A[smem] * B[smem]^T for one K = 16 slice.
+__device__ __forceinline__ void mma_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d_tmem),
+      "{\n.reg .pred p, q;\nelect.sync _|q, 0xffffffff;\nsetp.ne.b32 p, %4, 0;\n"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// D[tmem] (+)= A[tmem] * B[smem] for one K = 16 slice: A is 128 rows (lanes) of 8 columns of 16-bit pairs.
+__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n.reg .pred p, q;\nelect.sync _|q, 0xffffffff;\nsetp.ne.b32 p, %4, 0;\n"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d_tmem),
       "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Arrive on `bar` when all products issued so far have completed (the same elected lane).
+__device__ __forceinline__ void commit_elected(uint64_t* bar) {
+  asm volatile(
+      "{\n.reg .pred q;\nelect.sync _|q, 0xffffffff;\n"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_addr(bar))
       : "memory");
 }
 
@@ -85,6 +102,56 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// 32 columns of one lane per thread, not waited for: the values may be used after tmem_wait_ld and after_wait.
+__device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, float (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
+      "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+        "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]),
+        "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
+        "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// No instructions: every use of v has to come after this, and so after the wait before it.
+__device__ __forceinline__ void after_wait(float (&v)[32]) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 8)
+    asm volatile(""
+                 : "+f"(v[i]), "+f"(v[i + 1]), "+f"(v[i + 2]), "+f"(v[i + 3]), "+f"(v[i + 4]), "+f"(v[i + 5]),
+                   "+f"(v[i + 6]), "+f"(v[i + 7]));
+}
+
+// The lowest n bits, for any n.
+__device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
+
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ uint64_t bits2(float2 v) {
+  return static_cast<uint64_t>(__float_as_uint(v.x)) | (static_cast<uint64_t>(__float_as_uint(v.y)) << 32);
+}
+__device__ __forceinline__ float2 from_bits2(uint64_t v) {
+  return make_float2(__uint_as_float(static_cast<uint32_t>(v)), __uint_as_float(static_cast<uint32_t>(v >> 32)));
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)), "l"(bits2(c)));
+  return from_bits2(d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)));
+  return from_bits2(d);
+}
+
+__device__ __forceinline__ float row_max(const float (&s)[kC]) {
+  float m4[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+  for (int c = 4; c < kC; ++c) m4[c & 3] = fmaxf(m4[c & 3], s[c]);
+  return fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+}
 
 __device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
   asm volatile(
@@ -152,6 +219,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     int fill = 0;
     for (int part = 0; walk.more() && ok; ++part) {
       const Span<kC> span = walk.step();
+      if (walk.c1 <= walk.c0) {
+        --part;
+        continue;
+      }
       const int h = walk.h, c0 = walk.c0, c1 = walk.c1;
       const int32_t* table = walk.t.table;
       const bool two = walk.t.ntok > p.half_tokens;
@@ -161,7 +232,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       auto put = [&](const CUtensorMap* map, int i, int page) {
         const int s = fill % L::kSlots;
-        if (fill >= L::kSlots && !mbar_wait(&bar.kv_empty[s], ((fill / L::kSlots) - 1) & 1, p.err, DK_DEVERR_WAIT_EMPTY))
+        if (fill >= L::kSlots && !wait_for(&bar.kv_empty[s], ((fill / L::kSlots) - 1) & 1, p.err, DK_DEVERR_WAIT_EMPTY))
           ok = false;
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) return;
@@ -180,7 +251,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       int page = entry(c0);
       // Q, once the last part's products with it have completed
-      if (part > 0 && !mbar_wait(&bar.q_empty, (part - 1) & 1, p.err, DK_DEVERR_WAIT_EMPTY)) ok = false;
+      if (part > 0 && !wait_for(&bar.q_empty, (part - 1) & 1, p.err, DK_DEVERR_WAIT_EMPTY)) ok = false;
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       if (lane == 0) {
@@ -200,53 +271,50 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else if (warp == kMmaWarp) {
-    // ---------------------------------------------------------------- products (lane 0 issues)
+    // ---------------------------------------------------------------- products
     int fill = 0;         // ring slots consumed
     unsigned p_seen[2] = {0, 0};
     auto slot_wait = [&](int f) {
-      if (ok && !mbar_wait(&bar.kv_full[f % L::kSlots], (f / L::kSlots) & 1, p.err, DK_DEVERR_WAIT_FULL)) ok = false;
+      if (ok && !wait_for(&bar.kv_full[f % L::kSlots], (f / L::kSlots) & 1, p.err, DK_DEVERR_WAIT_FULL)) ok = false;
       ok = __all_sync(0xffffffffu, ok);
     };
     auto slot_at = [&](int f) { return smem_addr(slots + (f % L::kSlots) * L::kTileBytes); };
     auto qk = [&](int x, int f) {
-      if (lane == 0) {
-        const uint32_t a0 = smem_addr(q_sm + x * L::kTileBytes), b0 = slot_at(f);
+      const uint64_t a = tc::sdesc_k_sw128(smem_addr(q_sm + x * L::kTileBytes)), b = tc::sdesc_k_sw128(slot_at(f));
 #pragma unroll
-        for (int k = 0; k < kHd / 16; ++k) {
-          const uint32_t off = (k / 4) * L::kSegBytes + (k % 4) * 32;
-          tc::mma_f16(tmem + kS[x], tc::sdesc_k_sw128(a0 + off), tc::sdesc_k_sw128(b0 + off), idesc<T>(128, kC, false), k > 0);
-        }
-        tc::commit(&bar.s_full[x]);
+      for (int k = 0; k < kHd / 16; ++k) {
+        const uint32_t off = ((k / 4) * L::kSegBytes + (k % 4) * 32) >> 4;  // (descriptors count 16 bytes)
+        mma_ss(tmem + kS[x], a + off, b + off, idesc<T>(128, kC, false), k > 0);
       }
+      commit_elected(&bar.s_full[x]);
     };
     auto pv = [&](int x, int f, bool first) {
-      if (ok && !mbar_wait(&bar.p_full[x], p_seen[x] & 1, p.err, DK_DEVERR_WAIT_FULL)) ok = false;
+      if (ok && !wait_for(&bar.p_full[x], p_seen[x] & 1, p.err, DK_DEVERR_WAIT_FULL)) ok = false;
       ++p_seen[x];
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) return;
       tc::fence_after_sync();
-      if (lane == 0) {
-        const uint32_t b0 = slot_at(f);
+      const uint64_t b = sdesc_n_sw128(slot_at(f), L::kSegBytes);
 #pragma unroll
-        for (int k = 0; k < kC / 16; ++k)
-          mma_f16_ta(tmem + kO[x], tmem + kS[x] + 8 * k, sdesc_n_sw128(b0 + k * 2048, L::kSegBytes), idesc<T>(128, kHd, true),
-                     !first || k > 0);
-      }
+      for (int k = 0; k < kC / 16; ++k)
+        mma_ts(tmem + kO[x], tmem + kS[x] + 8 * k, b + ((k * 2048) >> 4), idesc<T>(128, kHd, true), !first || k > 0);
     };
     for (int part = 0; walk.more() && ok; ++part) {
       const Span<kC> span = walk.step();
       const int n = walk.c1 - walk.c0;
+      if (n <= 0) {
+        --part;
+        continue;
+      }
       const bool two = walk.t.ntok > p.half_tokens;
-      if (!mbar_wait(&bar.q_full, part & 1, p.err, DK_DEVERR_WAIT_FULL)) ok = false;
+      if (!wait_for(&bar.q_full, part & 1, p.err, DK_DEVERR_WAIT_FULL)) ok = false;
       slot_wait(fill);
       if (!ok) break;
       tc::fence_after_sync();
       qk(0, fill);
       if (two) qk(1, fill);
-      if (lane == 0) {
-        tc::commit(&bar.kv_empty[fill % L::kSlots]);
-        if (n == 1) tc::commit(&bar.q_empty);
-      }
+      commit_elected(&bar.kv_empty[fill % L::kSlots]);
+      if (n == 1) commit_elected(&bar.q_empty);
       for (int i = 0; i < n && ok; ++i) {
         const int fv = fill + 2 * i + 1, fk = fv + 1;
         slot_wait(fv);
@@ -255,12 +323,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         // does every row of v belong to a position that some row of the unit sees?
         const bool clear = j0 + kC <= span.end && (p.mask.window <= 0 || j0 >= span.lo || j0 + kC <= p.mask.sinks);
         if (!clear) {
-          uint8_t* v = slots + (fv % L::kSlots) * L::kTileBytes;
-          for (int r = lane; r < kC; r += 32)
+          uint8_t* v = slots + (fv % L::kSlots) * L::kTileBytes + (lane & 7) * 16;
+          for (int r = lane >> 3; r < kC; r += 4)  // 8 lanes a row of 64 dims
             if (!span.needs(j0 + r, 1, p.mask))
 #pragma unroll
-              for (int c = 0; c < L::kSegs * 8; ++c)
-                *reinterpret_cast<uint4*>(v + (c / 8) * L::kSegBytes + r * 128 + (c % 8) * 16) = make_uint4(0, 0, 0, 0);
+              for (int c = 0; c < L::kSegs; ++c)
+                *reinterpret_cast<uint4*>(v + c * L::kSegBytes + r * 128) = make_uint4(0, 0, 0, 0);
           tc::fence_proxy_async_smem();
           __syncwarp();
         }
@@ -271,22 +339,20 @@ __global__ void __launch_bounds__(kThreads, 1)
           slot_wait(fk);
           if (!ok) break;
           qk(0, fk);
-        } else if (lane == 0) {
-          tc::commit(&bar.o_full[0]);
+        } else {
+          commit_elected(&bar.o_full[0]);
         }
         if (two) {
           pv(1, fv, i == 0);
           if (!ok) break;
           if (more)
             qk(1, fk);
-          else if (lane == 0)
-            tc::commit(&bar.o_full[1]);
+          else
+            commit_elected(&bar.o_full[1]);
         }
-        if (lane == 0) {
-          tc::commit(&bar.kv_empty[fv % L::kSlots]);
-          if (more) tc::commit(&bar.kv_empty[fk % L::kSlots]);
-          if (i + 2 == n) tc::commit(&bar.q_empty);
-        }
+        commit_elected(&bar.kv_empty[fv % L::kSlots]);
+        if (more) commit_elected(&bar.kv_empty[fk % L::kSlots]);
+        if (i + 2 == n) commit_elected(&bar.q_empty);
       }
       fill += 2 * n;
     }
@@ -301,45 +367,71 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Span<kC> span = walk.step();
       const Tile t = walk.t;
       const int first = x * p.half_tokens;  // this half's first token
-      if (t.ntok <= first) continue;
+      if (t.ntok <= first || walk.c1 <= walk.c0) continue;
       const int tok = first + r / p.G, head = walk.h * p.G + r % p.G;
       const bool live = r < p.half_tokens * p.G && tok < t.ntok;
-      const int pos = live ? row_position(p, t, tok) : INT_MIN;
+      const int pos = live ? row_position(p, t, tok) : -1;
       const int p_lo = row_position(p, t, first), p_hi = row_position(p, t, min(t.ntok, first + p.half_tokens) - 1);
       float m = -INFINITY, l = 0.f;  // of scale2 * score
       for (int i = walk.c0; i < walk.c1; ++i) {
-        if (!mbar_wait(&bar.s_full[x], s_seen & 1, p.err, DK_DEVERR_WAIT_FULL)) ok = false;
+        if (!wait_for(&bar.s_full[x], s_seen & 1, p.err, DK_DEVERR_WAIT_FULL)) ok = false;
         ++s_seen;
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc::fence_after_sync();
         float s[kC];
 #pragma unroll
-        for (int c = 0; c < kC / 32; ++c) tc::tmem_ld32(s_col + 32 * c, *reinterpret_cast<float(*)[32]>(&s[32 * c]));
+        for (int c = 0; c < kC / 32; ++c) tmem_ld32_async(s_col + 32 * c, *reinterpret_cast<float(*)[32]>(&s[32 * c]));
+        tmem_wait_ld();
+#pragma unroll
+        for (int c = 0; c < kC / 32; ++c) after_wait(*reinterpret_cast<float(*)[32]>(&s[32 * c]));
         const int j0 = span.chunk(i) * kC;
         const bool clear = j0 + kC - 1 <= p_lo && j0 + kC <= span.end &&
                            (p.mask.window <= 0 || j0 > p_hi - p.mask.window || j0 + kC <= p.mask.sinks);
         if (!clear) {
-          const int end = min(span.end, pos + 1);  // (INT_MIN + 1 for a row that is none)
-          const int lo = p.mask.window > 0 ? pos - p.mask.window + 1 : INT_MIN;
+          // the row's visible positions of this chunk, a bit each: [lo, end) and those below the sinks' end
+          const int end = min(span.end, pos + 1) - j0, sinks = min(p.mask.sinks - j0, end);
+          const int lo = p.mask.window > 0 ? pos - p.mask.window + 1 - j0 : INT_MIN;
 #pragma unroll
-          for (int c = 0; c < kC; ++c) {
-            const int j = j0 + c;
-            if (!(j < end && (j >= lo || j < p.mask.sinks))) s[c] = -INFINITY;
+          for (int c = 0; c < kC / 32; ++c) {
+            const uint32_t see = (low_bits(end - 32 * c) & ~low_bits(lo - 32 * c)) | low_bits(sinks - 32 * c);
+#pragma unroll
+            for (int d = 0; d < 32; ++d) s[32 * c + d] = see & (1u << d) ? s[32 * c + d] : -INFINITY;
           }
         }
-        float mx = s[0];
+        // P refers to the maximum of the chunks before; only when this chunk's turns out to be 2^kLazy above it (or there
+        // was none) is the maximum raised and the chunk done again, so that the exponentials need not wait for it.
+        if (i == walk.c0) m = row_max(s) * p.scale2;
+        float2 sums;
+        for (;;) {
+          const float base = m == -INFINITY ? 0.f : m;
+          const float2 scale = make_float2(p.scale2, p.scale2), off = make_float2(-base, -base);
+          float2 sum[4] = {};
+          float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int c = 1; c < kC; ++c) mx = fmaxf(mx, s[c]);
-        mx *= p.scale2;
-        const bool raise = mx > m + kLazy || (m == -INFINITY && mx > -INFINITY);
-        float keep = 1.f;
-        if (raise) {
-          keep = exp2_approx(m - mx);
-          m = mx;
-          l *= keep;
-        }
-        if (__any_sync(0xffffffffu, raise) && i > walk.c0) {  // O's products up to the last chunk are done: S came after them
+          for (int c = 0; c < kC / 32; ++c) {
+            uint32_t w[16];
+#pragma unroll
+            for (int d = 0; d < 16; ++d) {
+              const float2 x2 = make_float2(s[32 * c + 2 * d], s[32 * c + 2 * d + 1]);
+              top[d & 3] = fmaxf(fmaxf(top[d & 3], x2.x), x2.y);
+              float2 y = fma2(x2, scale, off);
+              y = make_float2(exp2_approx(y.x), exp2_approx(y.y));
+              sum[d & 3] = add2(sum[d & 3], y);
+              w[d] = E::pack(y.x, y.y);
+            }
+            tmem_st16(s_col + 16 * c, w);
+          }
+          sums = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
+          const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale2;
+          const bool raise = mx > m + kLazy || (m == -INFINITY && mx > -INFINITY);
+          if (!__any_sync(0xffffffffu, raise)) break;
+          const float keep = raise ? exp2_approx(m - mx) : 1.f;
+          if (raise) {
+            m = mx;
+            l *= keep;
+          }
+          // O's products up to the last chunk are done: S came after them
 #pragma unroll
           for (int c = 0; c < kHd / 16; ++c) {
             float o[16];
@@ -350,27 +442,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_st16(o_col + 16 * c, w);
           }
         }
-        const float base = m == -INFINITY ? 0.f : m;
-        float sum = 0.f;
-#pragma unroll
-        for (int c = 0; c < kC / 32; ++c) {
-          uint32_t w[16];
-#pragma unroll
-          for (int d = 0; d < 16; ++d) {
-            const float a = exp2_approx(fmaf(s[32 * c + 2 * d], p.scale2, -base));
-            const float b = exp2_approx(fmaf(s[32 * c + 2 * d + 1], p.scale2, -base));
-            sum += a + b;
-            w[d] = E::pack(a, b);
-          }
-          tmem_st16(s_col + 16 * c, w);
-        }
-        l += sum;
+        l += sums.x + sums.y;
         tmem_wait_st();
         tc::fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar.p_full[x]);
       }
-      if (ok && !mbar_wait(&bar.o_full[x], o_seen & 1, p.err, DK_DEVERR_WAIT_FULL)) ok = false;
+      if (ok && !wait_for(&bar.o_full[x], o_seen & 1, p.err, DK_DEVERR_WAIT_FULL)) ok = false;
       ++o_seen;
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
@@ -381,22 +459,22 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float inv = l == 0.f ? 0.f : 1.f / l;
       T* out = static_cast<T*>(p.out) + (static_cast<int64_t>(t.t0 + tok) * p.nkv * p.G + head) * kHd;
       float* part = p.part_o + (slot * kTcRows + row) * kHd;
+      float o[kHd];
 #pragma unroll
-      for (int c = 0; c < kHd / 16; ++c) {
-        float o[16];
-        tc::tmem_ld16(o_col + 16 * c, o);
-        if (!live) continue;
-        if (whole) {
-          uint32_t w[8];
+      for (int c = 0; c < kHd / 32; ++c) tmem_ld32_async(o_col + 32 * c, *reinterpret_cast<float(*)[32]>(&o[32 * c]));
+      tmem_wait_ld();
 #pragma unroll
-          for (int d = 0; d < 8; ++d) w[d] = E::pack(o[2 * d] * inv, o[2 * d + 1] * inv);
-          *reinterpret_cast<uint4*>(out + 16 * c) = make_uint4(w[0], w[1], w[2], w[3]);
-          *reinterpret_cast<uint4*>(out + 16 * c + 8) = make_uint4(w[4], w[5], w[6], w[7]);
-        } else {
+      for (int c = 0; c < kHd / 32; ++c) after_wait(*reinterpret_cast<float(*)[32]>(&o[32 * c]));
+      if (live && whole) {
 #pragma unroll
-          for (int d = 0; d < 4; ++d)
-            *reinterpret_cast<float4*>(part + 16 * c + 4 * d) = make_float4(o[4 * d], o[4 * d + 1], o[4 * d + 2], o[4 * d + 3]);
-        }
+        for (int d = 0; d < kHd; d += 8)
+          *reinterpret_cast<uint4*>(out + d) =
+              make_uint4(E::pack(o[d] * inv, o[d + 1] * inv), E::pack(o[d + 2] * inv, o[d + 3] * inv),
+                         E::pack(o[d + 4] * inv, o[d + 5] * inv), E::pack(o[d + 6] * inv, o[d + 7] * inv));
+      } else if (live) {
+#pragma unroll
+        for (int d = 0; d < kHd; d += 4)
+          *reinterpret_cast<float4*>(part + d) = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
       }
       if (!whole && live) *reinterpret_cast<float2*>(&p.part_ml[(slot * kTcRows + row) * 2]) = make_float2(m, l);
       tc::fence_before_sync();
@@ -409,8 +487,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   if (failed && warp == kMmaWarp) {
     // a wait gave up: let products and copies still in flight finish before their memory goes away (bounded)
+    commit_elected(&bar.drain);
     if (lane == 0) {
-      tc::commit(&bar.drain);
       const uint64_t t0 = globaltimer_ns();
       while (!mbar_try_wait(&bar.drain, 0) && globaltimer_ns() - t0 < 500000000ull) {
       }

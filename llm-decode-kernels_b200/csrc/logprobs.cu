@@ -4,14 +4,19 @@
 // Neither subtracts two large numbers of the row's own size, so fp32 keeps both to a few units in the last place.
 // The maximum, s and w run along (rescaled when the maximum grows), so the row is read once.
 //
-// The top alternatives (by value, ties to the lowest index) come from the same pass: an element is a candidate when
-// it is not below a threshold that at least `top` elements of the row reach. The first tile gives one (the r-th
-// largest of the lanes' maxima in each of A warps, r A >= top, and of those the smallest), so that a few dozen
-// candidates of a long row go to a small list in shared memory. A full list is cut to its `top` best, which raises
-// the threshold. The order in which candidates arrive changes nothing: selection ranks (value, index) pairs.
+// 2^y is taken relative to the largest logit of the CTA's first tile; only a logit 40 above that moves the base (fp32
+// holds e^40 times the row's sum with room to spare), so the common path neither compares nor rescales.
 //
-// Memory bound: one 16-byte load per 8 (fp32: 4) logits. Rows are split over a cluster of CTAs when there are few
-// of them; the parts meet in the first CTA's shared memory.
+// The top alternatives (by value, ties to the lowest index) come from the same pass. The `top`-th largest of the threads'
+// maxima in the first tile is a threshold that `top` elements reach; what is not below it goes to a short list in shared
+// memory (a few hundred of 152064), which is cut to its `top` best once, to raise the threshold, and ranked at the end by
+// (value, index): the order in which candidates arrive changes nothing. -inf is not listed. A list that runs over (many
+// equal logits), or is too short (fewer tokens allowed than asked for), falls back to a search for the `top`-th key over
+// the CTA's part of the row: 16 more reads of it, from L2, counting the keys above three pivots.
+//
+// Bound by HBM, closely followed by the 16 exponentials a cycle that an SM computes (152064 x 2048 logits: 95 us of bytes,
+// 77 us of exponentials). Rows are split over a cluster of CTAs when there are few of them; the parts meet in the first
+// CTA's shared memory.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -22,12 +27,16 @@ namespace {
 using paged::Elem;
 using paged::exp2_approx;
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kVecs = 4;    // vectors a thread loads at once
-constexpr int kCap = 1024;  // candidates the list holds
+constexpr int kVecs = 4;     // vectors a thread loads at once
+constexpr int kCap = 1024;   // candidates the list holds
+constexpr int kCutTile = 2;  // the tile after which the list is cut
 constexpr int kMaxTop = 32;
 constexpr int kMaxCluster = 8;
+constexpr float kLog2e = 1.44269504088896341f;
+constexpr float kRoom = 40.f;
+constexpr float kLow = -1e30f;   // logits below it (the type's lowest value in masks) count as this
 
 struct LogprobParams {
   const void* logits;
@@ -62,59 +71,102 @@ __device__ __forceinline__ uint64_t candidate(float x, int64_t index) {
   return (static_cast<uint64_t>(order_key(x)) << 32) | (0xffffffffu - static_cast<uint32_t>(index));
 }
 
-template <typename T>
-struct Vec {
-  static constexpr int kN = 16 / sizeof(T);
-  float x[kN];
-  __device__ void set(uint4 v) {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(w[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 f = Elem<T>::unpack(w[i]);
-        x[2 * i] = f.x, x[2 * i + 1] = f.y;
-      }
-    }
-  }
-};
-
 __device__ __forceinline__ float to_float(float x) { return x; }
 __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
 __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 
+// 16 bytes of logits of type T.
+template <typename T>
+struct Vec {
+  static constexpr int kN = 16 / sizeof(T);
+  static constexpr int kPairs = kN / 2;
+  uint4 v;
+  __device__ uint32_t word(int i) const { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+  __device__ float2 pair(int i) const {
+    if constexpr (sizeof(T) == 4)
+      return make_float2(__uint_as_float(word(2 * i)), __uint_as_float(word(2 * i + 1)));
+    else
+      return Elem<T>::unpack(word(i));
+  }
+  __device__ float at(int i) const { return i & 1 ? pair(i / 2).y : pair(i / 2).x; }
+  __device__ float max() const {  // NaN if there is one
+    if constexpr (sizeof(T) == 4) {
+      return max_nan(max_nan(at(0), at(1)), max_nan(at(2), at(3)));
+    } else {
+      uint32_t m;
+      if constexpr (std::is_same<T, __half>::value)
+        asm("{.reg .b32 a, b;\nmax.NaN.f16x2 a, %1, %2;\nmax.NaN.f16x2 b, %3, %4;\nmax.NaN.f16x2 %0, a, b;}"
+            : "=r"(m) : "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w));
+      else
+        asm("{.reg .b32 a, b;\nmax.NaN.bf16x2 a, %1, %2;\nmax.NaN.bf16x2 b, %3, %4;\nmax.NaN.bf16x2 %0, a, b;}"
+            : "=r"(m) : "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w));
+      const float2 f = Elem<T>::unpack(m);
+      return max_nan(f.x, f.y);
+    }
+  }
+  // What stands for -inf in sums, so that 0 * y is 0 for it.
+  __device__ static constexpr float lowest() { return std::is_same<T, __half>::value ? -65504.f : -1e30f; }
+  __device__ float2 finite_pair(int i) const {
+    if constexpr (sizeof(T) == 4) {
+      const float2 f = pair(i);
+      return make_float2(max_nan(f.x, -1e30f), max_nan(f.y, -1e30f));
+    } else if constexpr (std::is_same<T, __half>::value) {
+      uint32_t m;
+      asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(m) : "r"(word(i)), "r"(0xfbfffbffu));  // -65504
+      return Elem<T>::unpack(m);
+    } else {
+      uint32_t m;
+      asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(m) : "r"(word(i)), "r"(0xf14af14au));  // just below -1e30
+      return Elem<T>::unpack(m);
+    }
+  }
+};
+
+__device__ __forceinline__ uint64_t bits2(float2 v) {
+  return static_cast<uint64_t>(__float_as_uint(v.x)) | (static_cast<uint64_t>(__float_as_uint(v.y)) << 32);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)), "l"(bits2(c)));
+  return make_float2(__uint_as_float(static_cast<uint32_t>(d)), __uint_as_float(static_cast<uint32_t>(d >> 32)));
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)));
+  return make_float2(__uint_as_float(static_cast<uint32_t>(d)), __uint_as_float(static_cast<uint32_t>(d >> 32)));
+}
+
 struct Stats {
-  float m, s, w;
-  // Adds (m2, s2, w2), whose sums are relative to its own maximum.
+  float m, s, w;  // sums relative to m
+  // Adds (m2, s2, w2), whose sums are relative to its own base.
   __device__ void join(float m2, float s2, float w2) {
     const float n = fmaxf(m, m2);
     const float base = n == -INFINITY ? 0.f : n;
     move(base);
-    const float d2 = fmaxf((m2 - base) * 1.44269504088896341f, -200.f), c2 = exp2_approx(d2);
+    const float d2 = fmaxf((m2 - base) * kLog2e, -200.f), c2 = exp2_approx(d2);
     s = fmaf(s2, c2, s);
     w = fmaf(c2, fmaf(s2, d2, w2), w);
     m = n;
   }
-  // Sums relative to `base` >= m. A maximum far below the new one (or none yet, -inf) leaves 0.
+  // Sums relative to `base` >= m. A base far below the new one (or none yet, -inf) leaves 0.
   __device__ void move(float base) {
-    const float d = fmaxf((m - base) * 1.44269504088896341f, -200.f), c = exp2_approx(d);
+    const float d = fmaxf((m - base) * kLog2e, -200.f), c = exp2_approx(d);
     w = c * fmaf(s, d, w);
     s *= c;
   }
 };
 
 template <typename T, bool kTop>
-__global__ void __launch_bounds__(kThreads, 2) logprob_kernel(const LogprobParams p) {
+__global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const LogprobParams p) {
   constexpr int kN = Vec<T>::kN;
   __shared__ uint64_t list[kTop ? kCap : 1];
   __shared__ uint64_t best[kTop ? kMaxTop : 1];                // this CTA's selection, best first
   __shared__ uint64_t all_best[kTop ? kMaxCluster * kMaxTop : 1];
+  __shared__ __align__(16) float first_max[kThreads];
   __shared__ float stat[kWarps * 3], cta_stat[3];
-  __shared__ float warp_thr[kWarps];
+  __shared__ int tally[kWarps * 3];
   __shared__ int count, n_best;
-  __shared__ uint64_t thr_key;  // candidates have to be above this pair
+  __shared__ float thr_sh;
   const uint32_t C = gridDim.y, rank = blockIdx.y;
   const int row = blockIdx.x;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -124,125 +176,142 @@ __global__ void __launch_bounds__(kThreads, 2) logprob_kernel(const LogprobParam
   // Vectors of 16 aligned bytes that hold the row: the first and the last may be partly outside it.
   const uintptr_t a0 = reinterpret_cast<uintptr_t>(x) & ~uintptr_t(15);
   const int skip = static_cast<int>((reinterpret_cast<uintptr_t>(x) - a0) / sizeof(T));
-  const int64_t nvec = (skip + p.V + kN - 1) / kN;
-  const int64_t share = (nvec + C - 1) / C;
-  const int64_t v0 = min(rank * share, nvec), v1 = min(v0 + share, nvec);
-  const uint4* base = reinterpret_cast<const uint4*>(a0);
-  if (tid == 0) count = 0, thr_key = 0;
+  const int V = static_cast<int>(p.V), nvec = (skip + V + kN - 1) / kN;
+  const int share = (nvec + C - 1) / C;
+  const int v0 = min(static_cast<int>(rank) * share, nvec), v1 = min(v0 + share, nvec);
+  const uint4* base_ptr = reinterpret_cast<const uint4*>(a0);
+  if (tid == 0) count = 0;
 
-  auto fetch = [&](int64_t v, Vec<T>& out) {
-    const int64_t e0 = v * kN - skip;  // row index of the vector's first element
-    if (v < v1 && e0 >= 0 && e0 + kN <= p.V) {
-      out.set(__ldcs(base + v));
+  auto fetch = [&](int v) {
+    Vec<T> out;
+    const int e0 = v * kN - skip;  // row index of the vector's first element
+    if (v < v1 && e0 >= 0 && e0 + kN <= V) {
+      out.v = __ldg(base_ptr + v);
     } else {
-#pragma unroll
-      for (int i = 0; i < kN; ++i)
-        out.x[i] = v < v1 && e0 + i >= 0 && e0 + i < p.V ? to_float(x[e0 + i]) : -INFINITY;
-    }
-  };
-
-  Stats st{-INFINITY, 0.f, 0.f};
-  float thr = -INFINITY;
-  for (int64_t t0 = v0; t0 < v1; t0 += kThreads * kVecs) {
-    Vec<T> v[kVecs];
-    float vmax[kVecs], top = -INFINITY;
-#pragma unroll
-    for (int u = 0; u < kVecs; ++u) fetch(t0 + u * kThreads + tid, v[u]);
-#pragma unroll
-    for (int u = 0; u < kVecs; ++u) {
-      vmax[u] = v[u].x[0];
-#pragma unroll
-      for (int i = 1; i < kN; ++i) vmax[u] = max_nan(vmax[u], v[u].x[i]);
-      top = max_nan(top, vmax[u]);
-    }
-    if (top > st.m) {
-      st.move(top);
-      st.m = top;
-    }
-    const float shift = st.m == -INFINITY ? 0.f : st.m;
-#pragma unroll
-    for (int u = 0; u < kVecs; ++u) {
+      T e[kN];
 #pragma unroll
       for (int i = 0; i < kN; ++i) {
-        const float y = max_nan((v[u].x[i] - shift) * 1.44269504088896341f, -200.f);  // 2^-200 is 0 here
-        const float e = exp2_approx(y);
-        st.s += e;
-        st.w = fmaf(e, y, st.w);
+        const bool in = v < v1 && e0 + i >= 0 && e0 + i < V;
+        if constexpr (sizeof(T) == 4)
+          e[i] = in ? x[e0 + i] : -INFINITY;
+        else if constexpr (std::is_same<T, __half>::value)
+          e[i] = in ? x[e0 + i] : __ushort_as_half(0xfc00);
+        else
+          e[i] = in ? x[e0 + i] : __ushort_as_bfloat16(0xff80);
+      }
+      out.v = *reinterpret_cast<const uint4*>(e);
+    }
+    return out;
+  };
+  auto outside = [&](int v, int i) { return v >= v1 || v * kN - skip + i < 0 || v * kN - skip + i >= V; };
+
+  float base = 0.f, thr = -INFINITY;
+  bool low = false;  // the first tile holds nothing above what -inf is taken for
+  float2 s2 = make_float2(0.f, 0.f), w2 = s2;
+  int tile = 0;
+  for (int t0 = v0; t0 < v1; t0 += kThreads * kVecs, ++tile) {
+    Vec<T> v[kVecs];
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u) v[u] = fetch(t0 + u * kThreads + tid);
+    float vmax[kVecs];
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u) vmax[u] = v[u].max();
+    if (tile == 0) {
+      // The base, and the first threshold: the top-th largest of the threads' maxima (NaN: the largest, as in order_key)
+      float mine = max_nan(max_nan(vmax[0], vmax[1]), max_nan(vmax[2], vmax[3]));
+      first_max[tid] = mine;
+      if (tid == 0) thr_sh = -INFINITY;
+      __syncthreads();
+      int above = 0;
+      float top_max = -INFINITY;
+      const float4* f4 = reinterpret_cast<const float4*>(first_max);
+#pragma unroll 4
+      for (int i = 0; i < kThreads / 4; ++i) {
+        const float4 f = f4[i];
+        top_max = fmaxf(fmaxf(fmaxf(top_max, f.x), fmaxf(f.y, f.z)), f.w);
+        if constexpr (kTop) above += !(f.x <= mine) + !(f.y <= mine) + !(f.z <= mine) + !(f.w <= mine);
+      }
+      low = top_max != -INFINITY && top_max <= Vec<T>::lowest();
+      base = top_max == -INFINITY ? 0.f : fmaxf(top_max, kLow);
+      if constexpr (kTop) {
+        // at most top - 1 threads have a larger maximum, so `mine` bounds the top-th element from below ... from the
+        // smallest such `mine`: the largest value that `top` threads reach
+        int reach = 0;
+        for (int i = 0; i < kThreads / 4 && above < p.top; ++i) {
+          const float4 f = f4[i];
+          reach += !(f.x < mine) + !(f.y < mine) + !(f.z < mine) + !(f.w < mine);
+        }
+        if (above < p.top && reach >= p.top && mine == mine) thr_sh = mine;  // (all such threads hold the same value)
+        __syncthreads();
+        thr = thr_sh;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u) {
+      if (vmax[u] > base + kRoom) {
+        Stats a{base, s2.x, w2.x}, b{base, s2.y, w2.y};
+        base = vmax[u];
+        a.move(base), b.move(base);
+        s2 = make_float2(a.s, b.s), w2 = make_float2(a.w, b.w);
+      }
+      const float2 scale = make_float2(kLog2e, kLog2e), off = make_float2(-base, -base);
+      const float2 none = make_float2(-0.f, -0.f);
+#pragma unroll
+      for (int i = 0; i < Vec<T>::kPairs; ++i) {
+        const float2 y = fma2(add2(v[u].finite_pair(i), off), scale, none);
+        float2 e = make_float2(exp2_approx(y.x), exp2_approx(y.y));
+        if (low) {
+          if (v[u].pair(i).x == -INFINITY) e.x = 0.f;
+          if (v[u].pair(i).y == -INFINITY) e.y = 0.f;
+        }
+        s2 = add2(s2, e);
+        w2 = fma2(e, y, w2);
+      }
+      if constexpr (kTop) {
+        if (!(vmax[u] < thr) && vmax[u] != -INFINITY) {
+          const int at = t0 + u * kThreads + tid;
+#pragma unroll
+          for (int i = 0; i < kN; ++i) {
+            const float f = v[u].at(i);
+            if (f < thr || f == -INFINITY || outside(at, i)) continue;
+            const int place = atomicAdd(&count, 1);
+            if (place < kCap) list[place] = candidate(f, at * kN - skip + i);
+          }
+        }
       }
     }
     if constexpr (kTop) {
-      if (t0 == v0) {  // the first threshold
-        const int64_t nv = min(v1 - v0, static_cast<int64_t>(kThreads * kVecs));
-        const int A = max(1, min(kWarps, static_cast<int>(nv / 32)));
-        const int r = (p.top + A - 1) / A;
-        if (warp < A) {
-          uint32_t key = order_key(top), kth = 0;
-          for (int i = 0; i < min(r, 32); ++i) {
-            kth = __reduce_max_sync(0xffffffffu, key);
-            const unsigned who = __ballot_sync(0xffffffffu, key == kth);
-            if (lane == __ffs(who) - 1) key = 0;
-          }
-          if (lane == 0) warp_thr[warp] = r > 32 ? -INFINITY : key_value(kth);
-        }
+      if (tile == kCutTile && t0 + kThreads * kVecs < v1) {
         __syncthreads();
-        thr = warp_thr[0];
-        for (int i = 1; i < A; ++i) thr = fminf(thr, warp_thr[i]);
-        if (thr != thr) thr = INFINITY;  // NaN rows: only NaN (and +inf) pass
-      }
-      unsigned pending = 0;  // a bit for each of this thread's vectors that may hold candidates
+        const int n = count;
+        if (n >= p.top && n <= kCap) {  // (uniform; a list that ran over stays so)
+          uint64_t mine[kCap / kThreads];
+          int place[kCap / kThreads];
 #pragma unroll
-      for (int u = 0; u < kVecs; ++u)
-        if (!(vmax[u] < thr)) pending |= 1u << u;
-      unsigned done[kVecs] = {};
-      for (;;) {
-        const uint64_t floor_key = thr_key;
-        bool left = false;
+          for (int j = 0; j < kCap / kThreads; ++j) {
+            place[j] = kCap;
+            if (tid + j * kThreads >= n) continue;
+            mine[j] = list[tid + j * kThreads];
+            place[j] = 0;
+            for (int i = 0; i < n; ++i) place[j] += list[i] > mine[j];
+          }
+          __syncthreads();
 #pragma unroll
-        for (int u = 0; u < kVecs; ++u) {
-          if (!(pending >> u & 1)) continue;
-          const int64_t e0 = (t0 + u * kThreads + tid) * kN - skip;
-#pragma unroll
-          for (int i = 0; i < kN; ++i) {
-            if (v[u].x[i] < thr || (done[u] >> i & 1) || e0 + i < 0 || e0 + i >= p.V || t0 + u * kThreads + tid >= v1)
-              continue;
-            const uint64_t c = candidate(v[u].x[i], e0 + i);
-            if (c <= floor_key) continue;
-            const int at = atomicAdd(&count, 1);
-            if (at < kCap) {
-              list[at] = c;
-              done[u] |= 1u << i;
-            } else {
-              left = true;
+          for (int j = 0; j < kCap / kThreads; ++j)
+            if (place[j] < p.top) {
+              list[place[j]] = mine[j];
+              if (place[j] == p.top - 1) thr_sh = key_value(static_cast<uint32_t>(mine[j] >> 32));
             }
-          }
+          if (tid == 0) count = p.top;
+          __syncthreads();
+          if (thr_sh == thr_sh) thr = thr_sh;
         }
-        if (!__syncthreads_or(left)) break;
-        // the list is full: keep its `top` best
-        uint64_t mine[kCap / kThreads];
-        int place[kCap / kThreads];
-#pragma unroll
-        for (int j = 0; j < kCap / kThreads; ++j) {
-          mine[j] = list[tid + j * kThreads];
-          int better = 0;
-          for (int i = 0; i < kCap; ++i) better += list[i] > mine[j];
-          place[j] = better;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < kCap / kThreads; ++j)
-          if (place[j] < p.top) {
-            list[place[j]] = mine[j];
-            if (place[j] == p.top - 1) thr_key = mine[j];
-          }
-        if (tid == 0) count = p.top;
-        __syncthreads();
-        thr = key_value(static_cast<uint32_t>(thr_key >> 32));
-        if (thr != thr) thr = INFINITY;
       }
     }
   }
 
   // ---------------------------------------------------------------- this CTA's sums and selection
+  Stats st{v0 < v1 ? base : -INFINITY, s2.x + s2.y, w2.x + w2.y};
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1)
     st.join(__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o),
@@ -250,7 +319,80 @@ __global__ void __launch_bounds__(kThreads, 2) logprob_kernel(const LogprobParam
   if (lane == 0) stat[3 * warp] = st.m, stat[3 * warp + 1] = st.s, stat[3 * warp + 2] = st.w;
   __syncthreads();
   if constexpr (kTop) {
-    const int n = count;
+    const int here = max(0, min(V, v1 * kN - skip) - max(0, v0 * kN - skip));  // elements of this CTA's part
+    const int want = min(p.top, here);
+    int n = count;
+    if (n > kCap || n < want) {
+      __syncthreads();
+      // The want-th largest key: two bits at a time, the number of keys at or above three pivots.
+      uint32_t kth = 0;
+      for (int bit = 30; bit >= 0; bit -= 2) {
+        int c[3] = {0, 0, 0};
+        for (int v = v0 + tid; v < v1; v += kThreads) {
+          const Vec<T> q = fetch(v);
+#pragma unroll
+          for (int i = 0; i < kN; ++i) {
+            const uint32_t k = outside(v, i) ? 0u : order_key(q.at(i));
+#pragma unroll
+            for (int j = 0; j < 3; ++j) c[j] += k >= (kth | (j + 1u) << bit);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 3; ++j) {
+          const int w = __reduce_add_sync(0xffffffffu, c[j]);
+          if (lane == 0) tally[3 * warp + j] = w;
+        }
+        __syncthreads();
+        uint32_t digit = 0;
+        for (int j = 0; j < 3; ++j) {
+          int sum = 0;
+          for (int w = 0; w < kWarps; ++w) sum += tally[3 * w + j];
+          if (sum >= want) digit = j + 1;
+        }
+        kth |= digit << bit;
+        __syncthreads();
+      }
+      // All keys above it, then those equal to it in order of index until there are enough.
+      if (tid == 0) count = 0;
+      __syncthreads();
+      for (int v = v0 + tid; v < v1; v += kThreads) {
+        const Vec<T> q = fetch(v);
+#pragma unroll
+        for (int i = 0; i < kN; ++i)
+          if (!outside(v, i) && order_key(q.at(i)) > kth) list[atomicAdd(&count, 1)] = candidate(q.at(i), v * kN - skip + i);
+      }
+      __syncthreads();
+      n = count;  // < want
+      for (int t0 = v0; t0 < v1 && n < want; t0 += kThreads) {
+        const Vec<T> q = fetch(t0 + tid);
+        int equal = 0;
+#pragma unroll
+        for (int i = 0; i < kN; ++i) equal += !outside(t0 + tid, i) && order_key(q.at(i)) == kth;
+        int before = equal;  // inclusive scan over the warp, then over the warps
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int u = __shfl_up_sync(0xffffffffu, before, o);
+          if (lane >= o) before += u;
+        }
+        if (lane == 31) tally[warp] = before;
+        __syncthreads();
+        int all = 0, place = n + before - equal;
+        for (int w = 0; w < kWarps; ++w) {
+          if (w < warp) place += tally[w];
+          all += tally[w];
+        }
+#pragma unroll
+        for (int i = 0; i < kN; ++i)
+          if (!outside(t0 + tid, i) && order_key(q.at(i)) == kth) {
+            if (place < want) list[place] = candidate(q.at(i), (t0 + tid) * kN - skip + i);
+            ++place;
+          }
+        n += all;
+        __syncthreads();
+      }
+      n = want;
+      __syncthreads();
+    }
     for (int c = tid; c < n; c += kThreads) {
       const uint64_t mine = list[c];
       int better = 0;
@@ -278,6 +420,11 @@ __global__ void __launch_bounds__(kThreads, 2) logprob_kernel(const LogprobParam
       s.join(ld_shared_cluster_f32(map_shared_rank(&cta_stat[0], q)), ld_shared_cluster_f32(map_shared_rank(&cta_stat[1], q)),
              ld_shared_cluster_f32(map_shared_rank(&cta_stat[2], q)));
     const float ln_s = logf(s.s);
+    auto logprob = [&](float value) {
+      if (s.s == 0.f) return __int_as_float(0x7fc00000);  // no logit above -inf
+      if (value == -INFINITY) return s.s == s.s ? value : s.s;
+      return ((s.m > kLow ? value : max_nan(value, kLow)) - s.m) - ln_s;
+    };
     if (tid == 0) {
       const int64_t t = p.targets[row];
       float lp = 0.f;
@@ -285,14 +432,14 @@ __global__ void __launch_bounds__(kThreads, 2) logprob_kernel(const LogprobParam
         record_device_error(p.err, DK_DEVERR_BAD_TOKEN);
         lp = __int_as_float(0x7fc00000);
       } else if (t >= 0) {
-        lp = (to_float(x[t]) - s.m) - ln_s;
+        lp = logprob(to_float(x[t]));
       }
       p.logprob[row] = lp;
-      p.entropy[row] = 0.693147180559945309f * (log2f(s.s) - s.w / s.s);
+      p.entropy[row] = fmaf(-0.693147180559945309f, s.w / s.s, ln_s);
     }
     if constexpr (kTop) {
       auto put = [&](int place, uint64_t c) {
-        p.top_logprob[static_cast<int64_t>(row) * p.top + place] = (key_value(static_cast<uint32_t>(c >> 32)) - s.m) - ln_s;
+        p.top_logprob[static_cast<int64_t>(row) * p.top + place] = logprob(key_value(static_cast<uint32_t>(c >> 32)));
         p.top_id[static_cast<int64_t>(row) * p.top + place] = 0xffffffffu - static_cast<uint32_t>(c);
       };
       if (C == 1) {
@@ -343,10 +490,10 @@ extern "C" int dk_token_logprobs(const void* logits, int64_t ld, int32_t dtype, 
     return set_error(DK_ERR_ALIGN, "token_logprobs: logits are not aligned to their type");
   LogprobParams p{logits, ld, targets, logprob, entropy, top_logprob, top_id, V, static_cast<int>(M), static_cast<int>(top),
                   device_info().err_word};
-  // CTAs per row: while the rows alone leave SMs without one, and a CTA still gets a tile's worth of vectors
+  // CTAs per row: more while the rows leave SMs with less than two CTAs and a CTA keeps half a tile's worth of vectors
   const int64_t tile = static_cast<int64_t>(kThreads) * kVecs * (dtype == DK_F32 ? 4 : 8);
   int C = 1;
-  while (C < kMaxCluster && M * C * 2 <= device_info().num_sms && V >= C * tile / 2) C *= 2;
+  while (C < kMaxCluster && M * C * 2 <= 2 * device_info().num_sms && V >= C * tile) C *= 2;
   const dim3 grid(static_cast<unsigned>(M), static_cast<unsigned>(C));
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e;

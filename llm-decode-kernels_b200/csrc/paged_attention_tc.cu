@@ -103,26 +103,24 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// 32 columns of one lane per thread, not waited for: the values may be used after tmem_wait_ld and after_wait.
-__device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, float (&v)[32]) {
+// 64 columns of one lane per thread. The wait is part of the statement: until it, the registers must not even be moved.
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, float (&v)[64]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
-      "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
-        "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]),
-        "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
-        "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
+      "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,"
+      "%27,%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,"
+      "%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63"
+      "}, [%64];\ntcgen05.wait::ld.sync.aligned;"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+        "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]),
+        "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]),
+        "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31]),
+        "=f"(v[32]), "=f"(v[33]), "=f"(v[34]), "=f"(v[35]), "=f"(v[36]), "=f"(v[37]), "=f"(v[38]), "=f"(v[39]),
+        "=f"(v[40]), "=f"(v[41]), "=f"(v[42]), "=f"(v[43]), "=f"(v[44]), "=f"(v[45]), "=f"(v[46]), "=f"(v[47]),
+        "=f"(v[48]), "=f"(v[49]), "=f"(v[50]), "=f"(v[51]), "=f"(v[52]), "=f"(v[53]), "=f"(v[54]), "=f"(v[55]),
+        "=f"(v[56]), "=f"(v[57]), "=f"(v[58]), "=f"(v[59]), "=f"(v[60]), "=f"(v[61]), "=f"(v[62]), "=f"(v[63])
       : "r"(taddr)
       : "memory");
-}
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-// No instructions: every use of v has to come after this, and so after the wait before it.
-__device__ __forceinline__ void after_wait(float (&v)[32]) {
-#pragma unroll
-  for (int i = 0; i < 32; i += 8)
-    asm volatile(""
-                 : "+f"(v[i]), "+f"(v[i + 1]), "+f"(v[i + 2]), "+f"(v[i + 3]), "+f"(v[i + 4]), "+f"(v[i + 5]),
-                   "+f"(v[i + 6]), "+f"(v[i + 7]));
 }
 
 // The lowest n bits, for any n.
@@ -381,10 +379,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc::fence_after_sync();
         float s[kC];
 #pragma unroll
-        for (int c = 0; c < kC / 32; ++c) tmem_ld32_async(s_col + 32 * c, *reinterpret_cast<float(*)[32]>(&s[32 * c]));
-        tmem_wait_ld();
-#pragma unroll
-        for (int c = 0; c < kC / 32; ++c) after_wait(*reinterpret_cast<float(*)[32]>(&s[32 * c]));
+        for (int c = 0; c < kC; c += 64) tmem_ld64(s_col + c, *reinterpret_cast<float(*)[64]>(&s[c]));
         const int j0 = span.chunk(i) * kC;
         const bool clear = j0 + kC - 1 <= p_lo && j0 + kC <= span.end &&
                            (p.mask.window <= 0 || j0 > p_hi - p.mask.window || j0 + kC <= p.mask.sinks);
@@ -459,22 +454,22 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float inv = l == 0.f ? 0.f : 1.f / l;
       T* out = static_cast<T*>(p.out) + (static_cast<int64_t>(t.t0 + tok) * p.nkv * p.G + head) * kHd;
       float* part = p.part_o + (slot * kTcRows + row) * kHd;
-      float o[kHd];
 #pragma unroll
-      for (int c = 0; c < kHd / 32; ++c) tmem_ld32_async(o_col + 32 * c, *reinterpret_cast<float(*)[32]>(&o[32 * c]));
-      tmem_wait_ld();
+      for (int c = 0; c < kHd; c += 64) {
+        float o[64];
+        tmem_ld64(o_col + c, o);
+        if (live && whole) {
 #pragma unroll
-      for (int c = 0; c < kHd / 32; ++c) after_wait(*reinterpret_cast<float(*)[32]>(&o[32 * c]));
-      if (live && whole) {
+          for (int d = 0; d < 64; d += 8)
+            *reinterpret_cast<uint4*>(out + c + d) =
+                make_uint4(E::pack(o[d] * inv, o[d + 1] * inv), E::pack(o[d + 2] * inv, o[d + 3] * inv),
+                           E::pack(o[d + 4] * inv, o[d + 5] * inv), E::pack(o[d + 6] * inv, o[d + 7] * inv));
+        } else if (live) {
 #pragma unroll
-        for (int d = 0; d < kHd; d += 8)
-          *reinterpret_cast<uint4*>(out + d) =
-              make_uint4(E::pack(o[d] * inv, o[d + 1] * inv), E::pack(o[d + 2] * inv, o[d + 3] * inv),
-                         E::pack(o[d + 4] * inv, o[d + 5] * inv), E::pack(o[d + 6] * inv, o[d + 7] * inv));
-      } else if (live) {
-#pragma unroll
-        for (int d = 0; d < kHd; d += 4)
-          *reinterpret_cast<float4*>(part + d) = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
+          for (int d = 0; d < 64; d += 4)
+            *reinterpret_cast<float4*>(part + c + d) = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
+        }
+        __syncwarp();
       }
       if (!whole && live) *reinterpret_cast<float2*>(&p.part_ml[(slot * kTcRows + row) * 2]) = make_float2(m, l);
       tc::fence_before_sync();

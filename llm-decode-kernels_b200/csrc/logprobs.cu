@@ -7,17 +7,18 @@
 // 2^y is taken relative to the largest logit of the CTA's first tile; only a logit 40 above that moves the base (fp32
 // holds e^40 times the row's sum with room to spare), so the common path neither compares nor rescales.
 //
-// The top alternatives (by value, ties to the lowest index) come from the same pass. The `top`-th largest of the threads'
-// maxima in the first tile is a threshold that `top` elements reach; what is not below it goes to a short list in shared
-// memory (a few hundred of 152064), which is cut to its `top` best once, to raise the threshold, and ranked at the end by
-// (value, index): the order in which candidates arrive changes nothing. -inf is not listed. A list that runs over (many
-// equal logits), or is too short (fewer tokens allowed than asked for), falls back to a search for the `top`-th key over
-// the CTA's part of the row: 16 more reads of it, from L2, counting the keys above three pivots.
-//
+// The top alternatives (by value, ties to the lowest index) come from the same pass. The `top`-th largest of the maxima that
+// 64 groups of threads have seen is a threshold that `top` elements reach; it is taken after the first tile, again a few
+// tiles later, and at the end. Vectors that hold something not below it are listed (a few hundred of 19008), and at the
+// end opened against the last threshold (a few dozen elements), which are ranked by (value, index): the order in which
+// they arrive changes nothing. -inf is not listed. A list that runs over (many equal logits), or is too short (fewer
+// tokens allowed than asked for), falls back to a search for the `top`-th key over the CTA's part of the row: 16 more reads
+// of it, from L2, counting the keys above three pivots.
 // Bound by HBM, closely followed by the 16 exponentials a cycle that an SM computes (152064 x 2048 logits: 95 us of bytes,
 // 77 us of exponentials). Rows are split over a cluster of CTAs when there are few of them; the parts meet in the first
 // CTA's shared memory.
 #include <algorithm>
+#include <cfloat>
 
 #include "paged.cuh"
 
@@ -29,9 +30,11 @@ using paged::exp2_approx;
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
+constexpr int kGroups = kThreads / 4;
+static_assert(kGroups == 64, "two maxima a lane");
+constexpr int kRaiseTile = 3;  // at this tile the threshold is taken again from all seen so far
 constexpr int kVecs = 4;     // vectors a thread loads at once
 constexpr int kCap = 1024;   // candidates the list holds
-constexpr int kCutTile = 2;  // the tile after which the list is cut
 constexpr int kMaxTop = 32;
 constexpr int kMaxCluster = 8;
 constexpr float kLog2e = 1.44269504088896341f;
@@ -104,6 +107,18 @@ struct Vec {
       return max_nan(f.x, f.y);
     }
   }
+  __device__ static T none() {  // -inf
+    if constexpr (sizeof(T) == 4)
+      return -INFINITY;
+    else if constexpr (std::is_same<T, __half>::value)
+      return __ushort_as_half(0xfc00);
+    else
+      return __ushort_as_bfloat16(0xff80);
+  }
+  __device__ static uint4 none4() {
+    constexpr uint32_t w = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+    return make_uint4(w, w, w, w);
+  }
   // What stands for -inf in sums, so that 0 * y is 0 for it.
   __device__ static constexpr float lowest() { return std::is_same<T, __half>::value ? -65504.f : -1e30f; }
   __device__ float2 finite_pair(int i) const {
@@ -162,9 +177,10 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const LogprobParam
   __shared__ uint64_t list[kTop ? kCap : 1];
   __shared__ uint64_t best[kTop ? kMaxTop : 1];                // this CTA's selection, best first
   __shared__ uint64_t all_best[kTop ? kMaxCluster * kMaxTop : 1];
-  __shared__ __align__(16) float first_max[kThreads];
+  __shared__ float first_max[kGroups];
   __shared__ float stat[kWarps * 3], cta_stat[3];
   __shared__ int tally[kWarps * 3];
+  __shared__ int vec_list[kTop ? kCap : 1], vec_count;  // vectors that hold candidates
   __shared__ int count, n_best;
   __shared__ float thr_sh;
   const uint32_t C = gridDim.y, rank = blockIdx.y;
@@ -179,150 +195,157 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const LogprobParam
   const int V = static_cast<int>(p.V), nvec = (skip + V + kN - 1) / kN;
   const int share = (nvec + C - 1) / C;
   const int v0 = min(static_cast<int>(rank) * share, nvec), v1 = min(v0 + share, nvec);
-  const uint4* base_ptr = reinterpret_cast<const uint4*>(a0);
-  if (tid == 0) count = 0;
+  const uint4* vecs = reinterpret_cast<const uint4*>(a0);
+  // Vectors of this part that lie wholly in the row; its at most two others are taken element by element.
+  const int f0 = v0 * kN < skip ? v0 + 1 : v0, f1 = min(v1, (skip + V) / kN);
+  if (tid == 0) count = vec_count = 0, thr_sh = -INFINITY;
 
+  // element i of vector v: -inf where it is outside the row
   auto fetch = [&](int v) {
     Vec<T> out;
-    const int e0 = v * kN - skip;  // row index of the vector's first element
-    if (v < v1 && e0 >= 0 && e0 + kN <= V) {
-      out.v = __ldg(base_ptr + v);
+    const int e0 = v * kN - skip;
+    if (v >= f0 && v < f1) {
+      out.v = __ldg(vecs + v);
     } else {
       T e[kN];
 #pragma unroll
-      for (int i = 0; i < kN; ++i) {
-        const bool in = v < v1 && e0 + i >= 0 && e0 + i < V;
-        if constexpr (sizeof(T) == 4)
-          e[i] = in ? x[e0 + i] : -INFINITY;
-        else if constexpr (std::is_same<T, __half>::value)
-          e[i] = in ? x[e0 + i] : __ushort_as_half(0xfc00);
-        else
-          e[i] = in ? x[e0 + i] : __ushort_as_bfloat16(0xff80);
-      }
+      for (int i = 0; i < kN; ++i) e[i] = v < v1 && e0 + i >= 0 && e0 + i < V ? x[e0 + i] : Vec<T>::none();
       out.v = *reinterpret_cast<const uint4*>(e);
     }
     return out;
   };
   auto outside = [&](int v, int i) { return v >= v1 || v * kN - skip + i < 0 || v * kN - skip + i >= V; };
+  auto push = [&](float value, int index) {
+    const int place = atomicAdd(&count, 1);
+    if (place < kCap) list[place] = candidate(value, index);
+  };
 
-  float base = 0.f, thr = -INFINITY;
-  bool low = false;  // the first tile holds nothing above what -inf is taken for
+  float base = kLow, thr = -FLT_MAX;
+  float run = -INFINITY;  // the largest logit this thread has seen (NaN: the largest, as in order_key)
+  // Raises the threshold to the top-th largest of the maxima that 64 groups of four threads have seen; all threads.
+  auto raise_threshold = [&] {
+    float group = max_nan(run, __shfl_xor_sync(0xffffffffu, run, 1));
+    group = max_nan(group, __shfl_xor_sync(0xffffffffu, group, 2));
+    if ((lane & 3) == 0) first_max[tid >> 2] = group;
+    __syncthreads();
+    if (kTop && tid < kGroups) {
+      const float me = first_max[tid];
+      int above = 0, reach = 0;
+      for (int i = 0; i < kGroups; ++i) {
+        above += !(first_max[i] <= me);
+        reach += !(first_max[i] < me);
+      }
+      if (above < p.top && reach >= p.top && me == me) thr_sh = me;  // (all such threads hold the same value)
+    }
+    __syncthreads();
+    if (kTop) thr = fmaxf(thr_sh, -FLT_MAX);  // (-inf is below any threshold)
+  };
+
   float2 s2 = make_float2(0.f, 0.f), w2 = s2;
+  bool low = true;  // nothing above what stands for -inf in sums has set the base yet: -inf is told apart one by one
   int tile = 0;
-  for (int t0 = v0; t0 < v1; t0 += kThreads * kVecs, ++tile) {
+  for (int t0 = f0; t0 < f1; t0 += kThreads * kVecs, ++tile) {
     Vec<T> v[kVecs];
-#pragma unroll
-    for (int u = 0; u < kVecs; ++u) v[u] = fetch(t0 + u * kThreads + tid);
     float vmax[kVecs];
 #pragma unroll
-    for (int u = 0; u < kVecs; ++u) vmax[u] = v[u].max();
-    if (tile == 0) {
-      // The base, and the first threshold: the top-th largest of the threads' maxima (NaN: the largest, as in order_key)
-      float mine = max_nan(max_nan(vmax[0], vmax[1]), max_nan(vmax[2], vmax[3]));
-      first_max[tid] = mine;
-      if (tid == 0) thr_sh = -INFINITY;
-      __syncthreads();
-      int above = 0;
-      float top_max = -INFINITY;
-      const float4* f4 = reinterpret_cast<const float4*>(first_max);
-#pragma unroll 4
-      for (int i = 0; i < kThreads / 4; ++i) {
-        const float4 f = f4[i];
-        top_max = fmaxf(fmaxf(fmaxf(top_max, f.x), fmaxf(f.y, f.z)), f.w);
-        if constexpr (kTop) above += !(f.x <= mine) + !(f.y <= mine) + !(f.z <= mine) + !(f.w <= mine);
-      }
-      low = top_max != -INFINITY && top_max <= Vec<T>::lowest();
-      base = top_max == -INFINITY ? 0.f : fmaxf(top_max, kLow);
-      if constexpr (kTop) {
-        // at most top - 1 threads have a larger maximum, so `mine` bounds the top-th element from below ... from the
-        // smallest such `mine`: the largest value that `top` threads reach
-        int reach = 0;
-        for (int i = 0; i < kThreads / 4 && above < p.top; ++i) {
-          const float4 f = f4[i];
-          reach += !(f.x < mine) + !(f.y < mine) + !(f.z < mine) + !(f.w < mine);
-        }
-        if (above < p.top && reach >= p.top && mine == mine) thr_sh = mine;  // (all such threads hold the same value)
-        __syncthreads();
-        thr = thr_sh;
-      }
+    for (int u = 0; u < kVecs; ++u) {
+      const int at = t0 + u * kThreads + tid;
+      v[u].v = at < f1 ? __ldg(vecs + at) : Vec<T>::none4();
     }
 #pragma unroll
-    for (int u = 0; u < kVecs; ++u) {
-      if (vmax[u] > base + kRoom) {
-        Stats a{base, s2.x, w2.x}, b{base, s2.y, w2.y};
-        base = vmax[u];
-        a.move(base), b.move(base);
-        s2 = make_float2(a.s, b.s), w2 = make_float2(a.w, b.w);
-      }
-      const float2 scale = make_float2(kLog2e, kLog2e), off = make_float2(-base, -base);
-      const float2 none = make_float2(-0.f, -0.f);
+    for (int u = 0; u < kVecs; ++u) vmax[u] = v[u].max();
+    const float mine = max_nan(max_nan(vmax[0], vmax[1]), max_nan(vmax[2], vmax[3]));
+    run = max_nan(run, mine);
+    if (tile == 0) {
+      raise_threshold();
+      float top_max = fmaxf(first_max[lane], first_max[lane + 32]);
 #pragma unroll
-      for (int i = 0; i < Vec<T>::kPairs; ++i) {
-        const float2 y = fma2(add2(v[u].finite_pair(i), off), scale, none);
-        float2 e = make_float2(exp2_approx(y.x), exp2_approx(y.y));
-        if (low) {
-          if (v[u].pair(i).x == -INFINITY) e.x = 0.f;
-          if (v[u].pair(i).y == -INFINITY) e.y = 0.f;
-        }
-        s2 = add2(s2, e);
-        w2 = fma2(e, y, w2);
-      }
-      if constexpr (kTop) {
-        if (!(vmax[u] < thr) && vmax[u] != -INFINITY) {
-          const int at = t0 + u * kThreads + tid;
-#pragma unroll
-          for (int i = 0; i < kN; ++i) {
-            const float f = v[u].at(i);
-            if (f < thr || f == -INFINITY || outside(at, i)) continue;
-            const int place = atomicAdd(&count, 1);
-            if (place < kCap) list[place] = candidate(f, at * kN - skip + i);
-          }
-        }
-      }
+      for (int o = 16; o > 0; o >>= 1) top_max = fmaxf(top_max, __shfl_xor_sync(0xffffffffu, top_max, o));
+      low = !(top_max > Vec<T>::lowest());
+      base = fmaxf(top_max, kLow);
+    } else if (kTop && tile == kRaiseTile) {
+      raise_threshold();
+    }
+    // Rare: a logit far above the base, candidates
+    if (mine > base + kRoom) {
+      Stats a{base, s2.x, w2.x}, b{base, s2.y, w2.y};
+      base = mine;
+      a.move(base), b.move(base);
+      s2 = make_float2(a.s, b.s), w2 = make_float2(a.w, b.w);
     }
     if constexpr (kTop) {
-      if (tile == kCutTile && t0 + kThreads * kVecs < v1) {
-        __syncthreads();
-        const int n = count;
-        if (n >= p.top && n <= kCap) {  // (uniform; a list that ran over stays so)
-          uint64_t mine[kCap / kThreads];
-          int place[kCap / kThreads];
+      if (!(mine < thr)) {
 #pragma unroll
-          for (int j = 0; j < kCap / kThreads; ++j) {
-            place[j] = kCap;
-            if (tid + j * kThreads >= n) continue;
-            mine[j] = list[tid + j * kThreads];
-            place[j] = 0;
-            for (int i = 0; i < n; ++i) place[j] += list[i] > mine[j];
+        for (int u = 0; u < kVecs; ++u)
+          if (!(vmax[u] < thr)) {
+            const int place = atomicAdd(&vec_count, 1);
+            if (place < kCap) vec_list[place] = t0 + u * kThreads + tid;
           }
-          __syncthreads();
+      }
+    }
+    const float2 scale = make_float2(kLog2e, kLog2e), off = make_float2(-base, -base), zero = make_float2(-0.f, -0.f);
+    if (!low) {
 #pragma unroll
-          for (int j = 0; j < kCap / kThreads; ++j)
-            if (place[j] < p.top) {
-              list[place[j]] = mine[j];
-              if (place[j] == p.top - 1) thr_sh = key_value(static_cast<uint32_t>(mine[j] >> 32));
-            }
-          if (tid == 0) count = p.top;
-          __syncthreads();
-          if (thr_sh == thr_sh) thr = thr_sh;
+      for (int u = 0; u < kVecs; ++u)
+#pragma unroll
+        for (int i = 0; i < Vec<T>::kPairs; ++i) {
+          const float2 y = fma2(add2(v[u].finite_pair(i), off), scale, zero);
+          const float2 e = make_float2(exp2_approx(y.x), exp2_approx(y.y));
+          s2 = add2(s2, e);
+          w2 = fma2(e, y, w2);
+        }
+    } else {
+      for (int u = 0; u < kVecs; ++u) {
+        const Vec<T> q = u == 0 ? v[0] : u == 1 ? v[1] : u == 2 ? v[2] : v[3];
+#pragma unroll
+        for (int i = 0; i < Vec<T>::kPairs; ++i) {
+          const float2 y = fma2(add2(q.finite_pair(i), off), scale, zero), f = q.pair(i);
+          const float2 e = make_float2(f.x == -INFINITY ? 0.f : exp2_approx(y.x), f.y == -INFINITY ? 0.f : exp2_approx(y.y));
+          s2 = add2(s2, e);
+          w2 = fma2(e, y, w2);
         }
       }
     }
   }
 
   // ---------------------------------------------------------------- this CTA's sums and selection
-  Stats st{v0 < v1 ? base : -INFINITY, s2.x + s2.y, w2.x + w2.y};
+  Stats st{f0 < f1 ? base : -INFINITY, s2.x + s2.y, w2.x + w2.y};
+  if (tid < 2 * kN) {  // the row's ends outside whole vectors: a thread per element
+    const int v = tid < kN ? v0 : v1 - 1;
+    if (v0 < v1 && (v < f0 || v >= f1) && (tid < kN || v > v0) && !outside(v, tid % kN)) {
+      const float f = to_float(x[v * kN - skip + tid % kN]);
+      if (f != -INFINITY) {
+        st.join(f, 1.f, 0.f);
+        if (f != f) st.s = f;
+        run = max_nan(run, f);
+        if constexpr (kTop)
+          if (!(f < thr)) push(f, v * kN - skip + tid % kN);  // (with the loop's threshold: only more)
+      }
+    }
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1)
     st.join(__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o),
             __shfl_xor_sync(0xffffffffu, st.w, o));
   if (lane == 0) stat[3 * warp] = st.m, stat[3 * warp + 1] = st.s, stat[3 * warp + 2] = st.w;
-  __syncthreads();
+  if constexpr (kTop)
+    raise_threshold();
+  else
+    __syncthreads();
   if constexpr (kTop) {
+    // The listed vectors are opened: what is not below the last threshold.
+    const int listed = vec_count;
+    for (int c = tid; c < min(listed, kCap); c += kThreads) {
+      const Vec<T> q = fetch(vec_list[c]);
+#pragma unroll
+      for (int i = 0; i < kN; ++i)
+        if (!(q.at(i) < thr)) push(q.at(i), vec_list[c] * kN - skip + i);
+    }
+    __syncthreads();
     const int here = max(0, min(V, v1 * kN - skip) - max(0, v0 * kN - skip));  // elements of this CTA's part
     const int want = min(p.top, here);
     int n = count;
-    if (n > kCap || n < want) {
+    if (listed > kCap || n > kCap || n < want) {
       __syncthreads();
       // The want-th largest key: two bits at a time, the number of keys at or above three pivots.
       uint32_t kth = 0;

@@ -151,6 +151,7 @@ struct Problem {
   // goes on after it (slot 2 * CTA + 1), and with always_partial a slot for each uncut unit after those
   float* part_o;   // [slots][tile rows][head_dim]
   float* part_ml;  // [slots][tile rows][2]: row maximum (base 2), row sum
+  int4* cut;           // [CTAs] the unit whose chunks a CTA begins but does not end: {first token, tokens, kv head, last CTA}
   int always_partial;  // no unit writes its output itself
   int* err;
 };
@@ -247,10 +248,12 @@ struct Walk {
   int next_h, next_t, next_c;
   // the current part: chunks c0 .. c1 of the unit (h, ti)
   int h, ti, c0, c1;
+  int64_t per, u0;  // length of a CTA's piece; where the unit begins
   Tile t, next_tile;  // (the next tile's fields are loaded a part ahead)
   int last;           // the tile's last position
   __device__ Walk(const Problem& p_, const Line& line_, int cta, int ctas, int lane) : p(p_), line(line_) {
-    const int64_t all = static_cast<int64_t>(line.chunks) * p.nkv, per = (all + ctas - 1) / ctas;
+    const int64_t all = static_cast<int64_t>(line.chunks) * p.nkv;
+    per = (all + ctas - 1) / ctas;
     x = min(cta * per, all);
     x1 = min(x + per, all);
     next_h = next_t = next_c = 0;
@@ -267,6 +270,7 @@ struct Walk {
   // of the line that stands for its fixed cost.
   __device__ Span<kChunk> step() {
     h = next_h, ti = next_t, c0 = next_c;
+    u0 = x - c0;
     t = next_tile;
     last = tile_last(p, t);
     const Span<kChunk> span(t.p0, last, p.mask, p.capacity);
@@ -277,6 +281,11 @@ struct Walk {
     if (++next_t == line.tiles) next_t = 0, ++next_h;
     if (x < x1) next_tile = tile_at(p, next_t);
     return span;
+  }
+  // Does the unit begin in this part and go on in other CTAs' pieces? Then what the join needs of it.
+  __device__ bool cut(const Span<kChunk>& span) const { return c0 == 0 && c1 < span.n; }
+  __device__ int4 cut_record(const Span<kChunk>& span) const {
+    return make_int4(t.t0, t.ntok, h, static_cast<int>((u0 + span.n - 1) / per));
   }
 };
 

@@ -9,7 +9,8 @@
 // The decode kernel is bound by the bytes of k and v: each is read once for the G query heads that share
 // it. A producer warp streams chunks of 64 positions, page by page, through a ring of TMA boxes (128-byte
 // swizzle: the ldmatrix reads hit all banks); pages that no row sees are never read, and their table
-// entries may be anything. Four consumer warps take 16 positions each: q.k on the tensor cores with the
+// entries may be anything. Two groups of four consumer warps take alternate chunks, 16
+// positions a warp: q.k on the tensor cores with the
 // query heads as the rows, online softmax in registers, p.v on the tensor cores with p taken from the
 // score accumulators. A position that no row of the tile sees reads a zero row instead of v, so whatever
 // the page holds there (infinities and NaN included) stays out; masked scores are replaced, not added to.
@@ -24,9 +25,9 @@ namespace paged {
 namespace {
 
 constexpr int kChunk = 64;
-constexpr int kCWarps = 4;
+constexpr int kCWarps = 8;  // two groups of four, for alternate chunks
 constexpr int kThreads = (kCWarps + 1) * 32;
-constexpr int kMaxRing = 4;
+constexpr int kMaxRing = 8;
 constexpr int kPlanThreads = 1024;
 
 // ------------------------------------------------------------------------------------ ragged plan
@@ -152,7 +153,7 @@ __global__ void __launch_bounds__(kThreads)
   if (tid == 0) {
     for (int i = 0; i < ring; ++i) {
       mbar_init(&full[i], 1);
-      mbar_init(&empty[i], kCWarps);
+      mbar_init(&empty[i], kCWarps / 2);
     }
     fence_mbar_init();
     vzero = make_uint4(0, 0, 0, 0);
@@ -241,6 +242,8 @@ __global__ void __launch_bounds__(kThreads)
     // ---------------------------------------------------------------- consumer warps
     const int g = lane >> 2, tq = lane & 3;
     const int mi = lane >> 3, rr = lane & 7;
+    const int group = warp >> 2, sub = warp & 3;
+    if (tid == 0) p.cut[blockIdx.x] = make_int4(0, 0, 0, 0);
     while (walk.more()) {
       const Span<kChunk> span = walk.step();
       const Tile t = walk.t;
@@ -269,15 +272,16 @@ __global__ void __launch_bounds__(kThreads)
       for (int e = 0; e < kR; ++e) m_run[e] = -INFINITY, l_run[e] = 0.f;
 
       for (int i = c0; i < c1; ++i, ++fill) {
+        if ((fill & 1) != group) continue;
         const int s = fill % ring;
         if (ok && !wait_for(&full[s], (fill / ring) & 1, p.err, DK_DEVERR_WAIT_FULL)) ok = false;
         ok = __all_sync(0xffffffffu, ok);
-        const int j0 = span.chunk(i) * kChunk + 16 * warp;  // this warp's 16 positions
+        const int j0 = span.chunk(i) * kChunk + 16 * sub;  // this warp's 16 positions
         if (ok && span.needs(j0, 16, p.mask)) {
           const uint8_t* kt = slots + s * B::kSlotBytes;
           const uint8_t* vt = kt + B::kTensorBytes;
           float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-          const int krow = 16 * warp + 8 * (mi >> 1) + rr;
+          const int krow = 16 * sub + 8 * (mi >> 1) + rr;
 #pragma unroll
           for (int ks = 0; ks < kHd / 16; ++ks) {
             uint32_t kb[4];
@@ -326,7 +330,7 @@ __global__ void __launch_bounds__(kThreads)
             pa[0][e] = E::pack(pr[0][0], pr[0][1]);
             pa[1][e] = E::pack(pr[1][0], pr[1][1]);
           }
-          const int vrow = 16 * warp + (mi & 1) * 8 + rr;
+          const int vrow = 16 * sub + (mi & 1) * 8 + rr;
           const bool zero = !clear && !span.needs(span.chunk(i) * kChunk + vrow, 1, p.mask);
           const uint32_t a1 = kTwo ? pa[0][kR - 1] : 0u, a3 = kTwo ? pa[1][kR - 1] : 0u;
 #pragma unroll
@@ -340,7 +344,8 @@ __global__ void __launch_bounds__(kThreads)
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[s]);
       }
-      // the four warps' results of this piece of the unit, joined
+      // the warps' results of this part of the unit, joined
+      if (tid == 0 && walk.cut(span)) p.cut[blockIdx.x] = walk.cut_record(span);
 #pragma unroll
       for (int e = 0; e < kR; ++e) {
         l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], 1);
@@ -404,45 +409,62 @@ __global__ void __launch_bounds__(kThreads)
   if (__syncthreads_or(!ok) && warp == kCWarps && lane == 0) {
     // a wait gave up: let copies still in flight land before the shared memory goes away (bounded)
     const uint64_t t0 = globaltimer_ns();
-    for (int s = 0; s < ring; ++s)
-      while (!mbar_try_wait(&full[s], 0) && !mbar_try_wait(&full[s], 1) && globaltimer_ns() - t0 < 500000000ull) {
+    for (int f = max(0, fill - ring); f < fill; ++f)
+      while (!mbar_try_wait(&full[f % ring], (f / ring) & 1) && globaltimer_ns() - t0 < 500000000ull) {
       }
   }
   if (wait_late) pdl_wait();
 }
 
 // ------------------------------------------------------------------------------------ join
-// Adds one unit's partial results of one row to (m, l, acc): kD dims per lane.
-template <int kD>
-__device__ __forceinline__ void add_pieces(const Problem& p, const Pieces& w, int tile_rows, int row, int lane, float& m,
-                                           float& l, float (&acc)[kD]) {
-  float mx = m;
-  for (int i = w.first + lane; i <= w.last; i += 32) mx = fmaxf(mx, p.part_ml[(piece_slot(w, i) * tile_rows + row) * 2]);
+// Running result of kRows rows: kD dims per lane of a warp.
+template <int kD, int kRows>
+struct Joined {
+  float m[kRows], l[kRows], acc[kRows][kD];
+  __device__ Joined() {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-  const float m_use = mx == -INFINITY ? 0.f : mx;
-  const float keep = exp2_approx(m - m_use);
-  l *= keep;
+    for (int r = 0; r < kRows; ++r) {
+      m[r] = -INFINITY, l[r] = 0.f;
 #pragma unroll
-  for (int d = 0; d < kD; ++d) acc[d] *= keep;
-  m = mx;
-#pragma unroll 4
-  for (int i = w.first; i <= w.last; ++i) {
-    const int64_t at = piece_slot(w, i) * tile_rows + row;
-    const float2 ml = *reinterpret_cast<const float2*>(&p.part_ml[at * 2]);
-    const float wt = exp2_approx(ml.x - m_use);
-    l = fmaf(wt, ml.y, l);
-    const float* src = &p.part_o[at * (kD * 32) + lane * kD];
-    if constexpr (kD == 4) {
-      const float4 v = *reinterpret_cast<const float4*>(src);
-      acc[0] = fmaf(wt, v.x, acc[0]), acc[1] = fmaf(wt, v.y, acc[1]);
-      acc[2] = fmaf(wt, v.z, acc[2]), acc[3] = fmaf(wt, v.w, acc[3]);
-    } else {
-      const float2 v = *reinterpret_cast<const float2*>(src);
-      acc[0] = fmaf(wt, v.x, acc[0]), acc[1] = fmaf(wt, v.y, acc[1]);
+      for (int d = 0; d < kD; ++d) acc[r][d] = 0.f;
     }
   }
-}
+  // Adds one unit's pieces in order, kAhead of them loaded at a time.
+  template <int kAhead>
+  __device__ void add(const Problem& p, const Pieces& w, int tile_rows, const int (&row)[kRows], int lane) {
+    for (int i0 = w.first; i0 <= w.last; i0 += kAhead) {
+      float2 ml[kAhead][kRows];
+      float o[kAhead][kRows][kD];
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a)
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+          ml[a][r] = make_float2(-INFINITY, 0.f);
+          if (i0 + a > w.last) continue;
+          const int64_t at = piece_slot(w, i0 + a) * tile_rows + row[r];
+          ml[a][r] = *reinterpret_cast<const float2*>(&p.part_ml[at * 2]);
+          const float* src = &p.part_o[at * (kD * 32) + lane * kD];
+          if constexpr (kD == 4)
+            *reinterpret_cast<float4*>(o[a][r]) = *reinterpret_cast<const float4*>(src);
+          else
+            *reinterpret_cast<float2*>(o[a][r]) = *reinterpret_cast<const float2*>(src);
+        }
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) {
+        if (i0 + a > w.last) break;
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+          const float mx = fmaxf(m[r], ml[a][r].x), use = mx == -INFINITY ? 0.f : mx;
+          const float keep = exp2_approx(m[r] - use), take = exp2_approx(ml[a][r].x - use);
+          m[r] = mx;
+          l[r] = fmaf(l[r], keep, ml[a][r].y * take);
+#pragma unroll
+          for (int d = 0; d < kD; ++d) acc[r][d] = fmaf(acc[r][d], keep, o[a][r][d] * take);
+        }
+      }
+    }
+  }
+};
 
 template <typename T, int kD>
 __device__ __forceinline__ void store_row(const Problem& p, int t, int head, int lane, float l, const float (&acc)[kD]) {
@@ -457,31 +479,29 @@ __device__ __forceinline__ void store_row(const Problem& p, int t, int head, int
 
 constexpr int kJoinWarps = 8;
 
-// Joins the units that a piece's end cuts. Block (i, y): the unit that holds the end of piece i, if that is the
-// first end inside it; a warp per row.
-template <typename T, int kHd>
+// Joins the units that a piece's end cuts. Block (i, y): kRows rows a warp of the unit that CTA i began, if there is one.
+template <typename T, int kHd, int kRows>
 __global__ void __launch_bounds__(kJoinWarps * 32) join_split_kernel(const Problem p, int ctas, int tile_rows) {
   constexpr int kD = kHd / 32;
   pdl_trigger();
   pdl_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const Line line = line_of(p, 1);
-  const int64_t all = static_cast<int64_t>(line.chunks) * p.nkv, per = (all + ctas - 1) / ctas;
-  const int64_t x = (blockIdx.x + 1ll) * per;
-  if (x >= all) return;
-  const int h = static_cast<int>(x / line.chunks), r = static_cast<int>(x % line.chunks);
-  const int ti = find_tile_warp([&](int i) { return line.cum(i); }, line.tiles, r, lane);
-  const int64_t u0 = static_cast<int64_t>(h) * line.chunks + line.cum(ti);
-  const int64_t u1 = static_cast<int64_t>(h) * line.chunks + line.cum(ti + 1);
-  if (u0 / per != blockIdx.x) return;
-  const Pieces w = pieces_of(u0, u1, p.unit_extra, per, ctas, 0);
-  if (w.first == w.last) return;
-  const Tile t = tile_at(p, ti);
-  for (int i = blockIdx.y * kJoinWarps + warp; i < t.ntok * p.G; i += gridDim.y * kJoinWarps) {
-    const int tok = i / p.G, g = i % p.G;
-    float m = -INFINITY, l = 0.f, acc[kD] = {};
-    add_pieces<kD>(p, w, tile_rows, result_row(p, tok, g), lane, m, l, acc);
-    store_row<T, kD>(p, t.t0 + tok, h * p.G + g, lane, l, acc);
+  const int4 c = p.cut[blockIdx.x];  // {first token, tokens, kv head, last CTA}
+  const int rows = c.y * p.G, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int i0 = (blockIdx.y * kJoinWarps + warp) * kRows;
+  if (i0 >= rows) return;
+  const Pieces w = {static_cast<int>(blockIdx.x), c.w, 0};
+  int row[kRows];
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    const int i = min(i0 + r, rows - 1);
+    row[r] = result_row(p, i / p.G, i % p.G);
+  }
+  Joined<kD, kRows> sum;
+  sum.template add<8 / kRows>(p, w, tile_rows, row, lane);
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    const int i = i0 + r;
+    if (i < rows) store_row<T, kD>(p, c.x + i / p.G, c.z * p.G + i % p.G, lane, sum.l[r], sum.acc[r]);
   }
 }
 
@@ -498,25 +518,22 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
   if (id >= rows) return;
   const int t = static_cast<int>(id / (a.nkv * a.G)), head = static_cast<int>(id % (a.nkv * a.G));
   const int h = head / a.G, g = head % a.G;
-  float m = -INFINITY, l = 0.f, acc[kD] = {};
-  {
-    const Line line = line_of(a, a_chunk);
-    const int ti = t / a.tile_tokens, unit = h * a.n_tiles + ti;
-    const int64_t all = static_cast<int64_t>(line.chunks) * a.nkv, per = (all + a_ctas - 1) / a_ctas;
-    const int64_t u0 = static_cast<int64_t>(unit) * line.per_tile;
-    add_pieces<kD>(a, pieces_of(u0, u0 + line.per_tile, a.unit_extra, per, a_ctas, unit), a_rows, result_row(a, t % a.tile_tokens, g), lane, m, l,
-                   acc);
-  }
-  const Line line = line_of(b, 1);
-  if (line.chunks > 0) {
-    const int64_t all = static_cast<int64_t>(line.chunks) * b.nkv, per = (all + b_ctas - 1) / b_ctas;
-    const int ti = b.mode == kRagged ? find_tile_warp([&](int i) { return b.tile_info[i].x; }, line.tiles, t, lane) : t;
-    const int t0 = b.mode == kRagged ? b.tile_info[ti].x : t;
-    const int64_t u0 = static_cast<int64_t>(h) * line.chunks + line.cum(ti);
-    const int64_t u1 = static_cast<int64_t>(h) * line.chunks + line.cum(ti + 1);
-    add_pieces<kD>(b, pieces_of(u0, u1, b.unit_extra, per, b_ctas, h * line.tiles + ti), b_rows, result_row(b, t - t0, g), lane, m, l, acc);
-  }
-  store_row<T, kD>(b, t, head, lane, l, acc);
+  const Line own = line_of(b, 1);
+  const int ti = b.mode == kRagged ? find_tile_warp([&](int i) { return b.tile_info[i].x; }, own.tiles, t, lane) : t;
+  const int t0 = b.mode == kRagged ? b.tile_info[ti].x : t;
+  const int64_t b_all = static_cast<int64_t>(own.chunks) * b.nkv, b_per = max((b_all + b_ctas - 1) / b_ctas, int64_t{1});
+  const int64_t b0 = static_cast<int64_t>(h) * own.chunks + own.cum(ti), b1 = static_cast<int64_t>(h) * own.chunks + own.cum(ti + 1);
+
+  const Line line = line_of(a, a_chunk);
+  const int unit = h * a.n_tiles + t / a.tile_tokens;
+  const int64_t a_all = static_cast<int64_t>(line.chunks) * a.nkv, a_per = (a_all + a_ctas - 1) / a_ctas;
+  const int64_t a0 = static_cast<int64_t>(unit) * line.per_tile;
+  Joined<kD, 1> sum;
+  const int a_row[1] = {result_row(a, t % a.tile_tokens, g)}, b_row[1] = {result_row(b, t - t0, g)};
+  sum.template add<8>(a, pieces_of(a0, a0 + line.per_tile, a.unit_extra, a_per, a_ctas, unit), a_rows, a_row, lane);
+  if (own.chunks > 0)
+    sum.template add<2>(b, pieces_of(b0, b1, b.unit_extra, b_per, b_ctas, h * own.tiles + ti), b_rows, b_row, lane);
+  store_row<T, kD>(b, t, head, lane, sum.l[0], sum.acc[0]);
 }
 
 }  // namespace
@@ -539,7 +556,8 @@ RowsShape rows_shape(int64_t B) {
   static int per_sm[2][64];  // by shared memory (batches up to 511 or more) and device; 0: not asked yet
   RowsShape s;
   const bool large = B > 511;
-  s.ring = kRows == 8 ? 3 : 4;
+  // Even: a slot always serves the same group of consumers, whose parity waits then see every phase of it.
+  s.ring = kHd == 64 ? 8 : 4;
   s.smem = 1024 + static_cast<size_t>(s.ring) * Box<kHd>::kSlotBytes + kCWarps * kRows * kHd * 4 +
            ((large ? kMaxBatch : 511) + 1) * 4;
   int dev = 0;
@@ -625,6 +643,7 @@ void cut_pass(const Sizes& z, Cutter& c, Pass& a, bool always_partial) {
   p.always_partial = always_partial;
   p.part_o = c.take<float>(slots * a.rows * z.hd);
   p.part_ml = c.take<float>(slots * a.rows * 2);
+  p.cut = c.take<int4>(a.ctas);
   p.cum_out = p.mode == kOneToken ? c.take<int32_t>(z.B + 1) : nullptr;
   p.plan = p.mode == kRagged ? c.take<int32_t>(3 + static_cast<int64_t>(p.max_tiles)) : nullptr;
   p.tile_info = p.mode == kRagged ? c.take<int4>(p.max_tiles) : nullptr;
@@ -673,9 +692,10 @@ int check_sizes(const char* what, const Sizes& z) {
 template <typename T, int kHd>
 cudaError_t launch_join(const Sizes& z, cudaStream_t st, const Pass* prefix, const Pass& own) {
   if (prefix == nullptr) {
-    const dim3 grid(static_cast<unsigned>(own.ctas - 1), static_cast<unsigned>((own.rows + kJoinWarps - 1) / kJoinWarps));
-    return launch(join_split_kernel<T, kHd>, grid, dim3(kJoinWarps * 32), 0, st, pdl_enabled(), dim3(1, 1, 1), own.p,
-                  own.ctas, own.rows);
+    const int rows = own.tc ? 4 : 1;
+    const dim3 grid(static_cast<unsigned>(own.ctas), static_cast<unsigned>((own.rows + kJoinWarps * rows - 1) / (kJoinWarps * rows)));
+    return launch(own.tc ? join_split_kernel<T, kHd, 4> : join_split_kernel<T, kHd, 1>, grid, dim3(kJoinWarps * 32), 0, st,
+                  pdl_enabled(), dim3(1, 1, 1), own.p, own.ctas, own.rows);
   }
   const dim3 grid(static_cast<unsigned>((z.T * z.nq + kJoinWarps - 1) / kJoinWarps));
   return launch(join_prefix_kernel<T, kHd>, grid, dim3(kJoinWarps * 32), 0, st, pdl_enabled(), dim3(1, 1, 1), prefix->p,

@@ -361,6 +361,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_col = tmem + lanes + kS[x], o_col = tmem + lanes + kO[x];
     unsigned s_seen = 0, o_seen = 0;
+    if (tid == 0) p.cut[blockIdx.x] = make_int4(0, 0, 0, 0);
     while (walk.more() && ok) {
       const Span<kC> span = walk.step();
       const Tile t = walk.t;
@@ -450,6 +451,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc::fence_after_sync();
       const bool all_of_it = walk.c0 == 0 && walk.c1 == span.n, whole = all_of_it && !p.always_partial;
       const int64_t slot = partial_slot(gridDim.x, blockIdx.x, walk.c0 == 0, all_of_it, walk.h * line.tiles + walk.ti);
+      if (tid == 0 && walk.cut(span)) p.cut[blockIdx.x] = walk.cut_record(span);
       const int row = x * 128 + r;
       const float inv = l == 0.f ? 0.f : 1.f / l;
       T* out = static_cast<T*>(p.out) + (static_cast<int64_t>(t.t0 + tok) * p.nkv * p.G + head) * kHd;

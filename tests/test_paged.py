@@ -141,6 +141,26 @@ def test_attention_ragged(sizes, nq, nkv, hd, page, dtype, window, sinks):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("hd,nq", [(128, 8), (64, 8), (128, 80)])
+def test_attention_long_rings(hd, nq):
+    """Many more chunks per CTA than its ring has slots, call after call without a host wait in between: every call gives
+    the first one's bits, and no bounded wait gives up."""
+    from kernels import _lib
+    from kernels.paged import paged_attention
+
+    sizes = [(1, 4000 + 97 * b) for b in range(10)]
+    c = Case(sizes, nq=nq, nkv=8, hd=hd, page=64, seed=8, spoil=False)
+    _lib.clear_device_error()
+    first = paged_attention(c.q, c.k, c.v, c.table, c.lengths)
+    same = torch.ones((), dtype=torch.bool, device="cuda")
+    for _ in range(200):
+        same &= (paged_attention(c.q, c.k, c.v, c.table, c.lengths) == first).all()
+    assert same.item() and _lib.device_error() == 0
+    few = Case(sizes[:2], nq=nq, nkv=8, hd=hd, page=64, seed=9)
+    assert_within(paged_attention(few.q, few.k, few.v, few.table, few.lengths), *few.attention())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("one_token", [True, False])
 def test_attention_leaves_freed_pages_alone(one_token):
     """Pages outside the window and the sinks may be freed: their table entries point nowhere."""

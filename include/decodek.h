@@ -259,11 +259,24 @@ int dk_embed_tokens(const int64_t* tokens, const void* embed, int64_t vocab, int
  * head_dim], rotated k and v -> position p of the sequence's pages. A token of an unused slot appends nothing and
  * its q_out row is zero; a position without a page in the pool, or an angle outside the tables, appends
  * nothing and sets DK_DEVERR_BAD_POSITION. */
-int dk_paged_append(const void* qkv, int64_t ldqkv, void* k_pages, void* v_pages, int64_t n_pages, int64_t page_size,
-                    const int32_t* page_table, int64_t ld_table, int64_t table_width, const int32_t* lengths,
-                    const int32_t* starts, const void* cos, const void* sin, int32_t rope_f32, int64_t ld_rope,
-                    int64_t rope_rows, int64_t rope_offset, void* q_out, int64_t T, int64_t B, int64_t nq, int64_t nkv,
-                    int64_t head_dim, int32_t dtype, dk_stream_t stream);
+typedef struct dk_paged_append_args {
+  const void* qkv;
+  int64_t ldqkv;
+  void* k_pages;
+  void* v_pages;
+  int64_t n_pages, page_size;
+  const int32_t* page_table;
+  int64_t ld_table, table_width;
+  const int32_t* lengths;
+  const int32_t* starts;
+  const void* cos;
+  const void* sin;
+  int64_t rope_f32, ld_rope, rope_rows, rope_offset;
+  void* q_out;
+  int64_t T, B, n_q, n_kv, head_dim, dtype;
+  dk_stream_t stream;
+} dk_paged_append_args;
+int dk_paged_append(const dk_paged_append_args* args);
 /* Attention over the pages: q [T, n_q, head_dim] (tokens ldq apart, heads head_dim apart) -> out [T, n_q,
  * head_dim] contiguous. The row at own position p sees the positions j <= p, and with window > 0 of those only
  * j > p - window and j < sinks; softmax(scale * q k^T) v over them, zero where there are none. Pages that no row
@@ -272,20 +285,31 @@ int dk_paged_append(const void* qkv, int64_t ldqkv, void* k_pages, void* v_pages
  * sizes, 256-byte aligned) needs no initialization and keeps nothing between calls. */
 int dk_paged_attention_workspace_bytes(int64_t T, int64_t B, int64_t nq, int64_t nkv, int64_t head_dim, int32_t dtype,
                                        int32_t ragged, int64_t prefix_len, uint64_t* bytes);
-int dk_paged_attention(const void* q, int64_t ldq, const void* k_pages, const void* v_pages, int64_t n_pages,
-                       int64_t page_size, const int32_t* page_table, int64_t ld_table, int64_t table_width,
-                       const int32_t* lengths, const int32_t* starts, int64_t window, int64_t sinks, float scale,
-                       void* out, int64_t T, int64_t B, int64_t nq, int64_t nkv, int64_t head_dim, int32_t dtype,
-                       void* workspace, uint64_t workspace_bytes, dk_stream_t stream);
+typedef struct dk_paged_attention_args {
+  const void* q;
+  int64_t ldq;
+  const void* k_pages;
+  const void* v_pages;
+  int64_t n_pages, page_size;
+  const int32_t* prefix_table; /* dk_shared_prefix_attention only */
+  int64_t prefix_len;
+  const int32_t* page_table;
+  int64_t ld_table, table_width;
+  const int32_t* lengths;
+  const int32_t* starts;
+  int64_t window, sinks; /* dk_paged_attention only */
+  double scale;
+  void* out;
+  int64_t T, B, n_q, n_kv, head_dim, dtype;
+  void* workspace;
+  uint64_t workspace_bytes;
+  dk_stream_t stream;
+} dk_paged_attention_args;
+int dk_paged_attention(const dk_paged_attention_args* args);
 /* Attention of a batch whose sequences share a prefix of prefix_len positions, in the pages listed by
  * prefix_table (int32): every row sees the whole prefix and its own sequence's positions (page_table, lengths,
  * starts as above, counted without the prefix) up to its own. The prefix is read once for all rows. */
-int dk_shared_prefix_attention(const void* q, int64_t ldq, const void* k_pages, const void* v_pages, int64_t n_pages,
-                               int64_t page_size, const int32_t* prefix_table, int64_t prefix_len,
-                               const int32_t* page_table, int64_t ld_table, int64_t table_width,
-                               const int32_t* lengths, const int32_t* starts, float scale, void* out, int64_t T,
-                               int64_t B, int64_t nq, int64_t nkv, int64_t head_dim, int32_t dtype, void* workspace,
-                               uint64_t workspace_bytes, dk_stream_t stream);
+int dk_shared_prefix_attention(const dk_paged_attention_args* args);
 
 /* ---- log probabilities of given tokens: no reference counterpart -------------------------------
  * logits [M, V] (rows ld apart; DK_F16, DK_BF16 or DK_F32) in one pass: logprob[m] = x[t] - logsumexp(x) of the target

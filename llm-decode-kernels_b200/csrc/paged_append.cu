@@ -128,12 +128,12 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const AppendParams p)
 
 using namespace dk;
 
-extern "C" int dk_paged_append(const void* qkv, int64_t ldqkv, void* k_pages, void* v_pages, int64_t n_pages,
-                               int64_t page_size, const int32_t* page_table, int64_t ld_table, int64_t table_width,
-                               const int32_t* lengths, const int32_t* starts, const void* cos, const void* sin,
-                               int32_t rope_f32, int64_t ld_rope, int64_t rope_rows, int64_t rope_offset, void* q_out,
-                               int64_t T, int64_t B, int64_t nq, int64_t nkv, int64_t head_dim, int32_t dtype,
-                               dk_stream_t stream) {
+extern "C" int dk_paged_append(const dk_paged_append_args* args) {
+  if (args == nullptr) return set_error(DK_ERR_INVALID, "paged_append: NULL arguments");
+  const dk_paged_append_args& a = *args;
+  const int64_t T = a.T, B = a.B, nq = a.n_q, nkv = a.n_kv, head_dim = a.head_dim, n_pages = a.n_pages,
+                page_size = a.page_size, table_width = a.table_width;
+  const int dtype = static_cast<int>(a.dtype);
   if (T < 0 || B <= 0 || nq <= 0 || nkv <= 0 || n_pages <= 0 || table_width <= 0)
     return set_error(DK_ERR_INVALID, "paged_append: bad sizes");
   if (head_dim != 64 && head_dim != 128)
@@ -143,21 +143,21 @@ extern "C" int dk_paged_append(const void* qkv, int64_t ldqkv, void* k_pages, vo
     return set_error(DK_ERR_UNSUPPORTED, "paged_append: page_size %lld (a power of two from 16 to 256)",
                      (long long)page_size);
   if (T == 0) return DK_OK;
-  if (starts == nullptr && T != B)
+  if (a.starts == nullptr && T != B)
     return set_error(DK_ERR_INVALID, "paged_append: without starts there is one token per sequence");
   if (T > INT32_MAX || B > INT32_MAX || n_pages > INT32_MAX || table_width > INT32_MAX ||
       table_width * page_size > INT32_MAX)
     return set_error(DK_ERR_INVALID, "paged_append: sizes must fit 31 bits");
-  if (!qkv || !k_pages || !v_pages || !page_table || !lengths || !cos || !sin || !q_out)
+  if (!a.qkv || !a.k_pages || !a.v_pages || !a.page_table || !a.lengths || !a.cos || !a.sin || !a.q_out)
     return set_error(DK_ERR_INVALID, "paged_append: NULL pointer");
-  if (!aligned16(qkv) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(q_out) || !aligned16(cos) ||
-      !aligned16(sin) || (ldqkv & 7) || (ld_rope & (rope_f32 ? 3 : 7)))
+  if (!aligned16(a.qkv) || !aligned16(a.k_pages) || !aligned16(a.v_pages) || !aligned16(a.q_out) || !aligned16(a.cos) ||
+      !aligned16(a.sin) || (a.ldqkv & 7) || (a.ld_rope & (a.rope_f32 ? 3 : 7)))
     return set_error(DK_ERR_ALIGN, "paged_append: rows of qkv, cos, sin, the pages and q_out need 16-byte alignment");
   AppendParams p;
-  p.qkv = qkv, p.ldqkv = ldqkv, p.k = k_pages, p.v = v_pages;
-  p.table = page_table, p.ld_table = ld_table, p.lengths = lengths, p.starts = starts;
-  p.cos = cos, p.sin = sin, p.ld_rope = ld_rope, p.rope_rows = rope_rows, p.rope_offset = rope_offset;
-  p.q_out = q_out;
+  p.qkv = a.qkv, p.ldqkv = a.ldqkv, p.k = a.k_pages, p.v = a.v_pages;
+  p.table = a.page_table, p.ld_table = a.ld_table, p.lengths = a.lengths, p.starts = a.starts;
+  p.cos = a.cos, p.sin = a.sin, p.ld_rope = a.ld_rope, p.rope_rows = a.rope_rows, p.rope_offset = a.rope_offset;
+  p.q_out = a.q_out;
   p.T = static_cast<int>(T), p.B = static_cast<int>(B), p.nq = static_cast<int>(nq), p.nkv = static_cast<int>(nkv);
   p.n_pages = static_cast<int>(n_pages), p.page_size = static_cast<int>(page_size);
   p.page_shift = __builtin_ctzll(page_size);
@@ -166,19 +166,19 @@ extern "C" int dk_paged_append(const void* qkv, int64_t ldqkv, void* k_pages, vo
   const int64_t items = T * ((nq + nkv) * (head_dim / 16) + nkv * (head_dim / 8));
   const int64_t blocks = (items + 255) / 256, most = 16ll * device_info().num_sms;
   const dim3 grid(static_cast<unsigned>(blocks < most ? blocks : most));
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(a.stream);
   cudaError_t e;
 #define DK_APPEND(TT, RR)                                                                                    \
   e = head_dim == 128                                                                                        \
           ? launch(paged_append_kernel<TT, RR, 128>, grid, dim3(256), 0, st, pdl_enabled(), dim3(1, 1, 1), p) \
           : launch(paged_append_kernel<TT, RR, 64>, grid, dim3(256), 0, st, pdl_enabled(), dim3(1, 1, 1), p)
   if (dtype == DK_F16) {
-    if (rope_f32)
+    if (a.rope_f32)
       DK_APPEND(__half, float);
     else
       DK_APPEND(__half, __half);
   } else {
-    if (rope_f32)
+    if (a.rope_f32)
       DK_APPEND(__nv_bfloat16, float);
     else
       DK_APPEND(__nv_bfloat16, __nv_bfloat16);

@@ -732,10 +732,12 @@ extern "C" int dk_paged_attention_workspace_bytes(int64_t T, int64_t B, int64_t 
 
 namespace {
 
-int attention(const char* what, const Sizes& z, const void* q, int64_t ldq, const void* k_pages, const void* v_pages,
-              int64_t n_pages, int64_t page_size, const int32_t* prefix_table, const int32_t* page_table,
-              int64_t ld_table, int64_t table_width, const int32_t* lengths, const int32_t* starts, int64_t window,
-              int64_t sinks, float scale, void* out, void* workspace, uint64_t workspace_bytes, dk_stream_t stream) {
+int attention(const char* what, const dk_paged_attention_args* args, bool prefix) {
+  if (args == nullptr) return set_error(DK_ERR_INVALID, "%s: NULL arguments", what);
+  const dk_paged_attention_args& a = *args;
+  const Sizes z{a.T, a.B, a.n_q, a.n_kv, a.head_dim, prefix ? a.prefix_len : 0, a.starts != nullptr, static_cast<int>(a.dtype)};
+  const int64_t n_pages = a.n_pages, page_size = a.page_size, table_width = a.table_width;
+  const int64_t window = prefix ? 0 : a.window, sinks = prefix ? 0 : a.sinks;
   if (const int rc = check_sizes(what, z)) return rc;
   if (n_pages <= 0 || table_width <= 0 || window < 0 || sinks < 0) return set_error(DK_ERR_INVALID, "%s: bad sizes", what);
   if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1)))
@@ -744,56 +746,58 @@ int attention(const char* what, const Sizes& z, const void* q, int64_t ldq, cons
       window >= (int64_t(1) << 31) || sinks >= (int64_t(1) << 31))
     return set_error(DK_ERR_INVALID, "%s: pages x kv heads x page_size, a table row's positions, window and sinks must stay below 2^31", what);
   if (z.T == 0) return DK_OK;
-  if (!q || !k_pages || !v_pages || !page_table || !lengths || !out || !workspace || (z.prefix_len > 0 && !prefix_table))
+  if (!a.q || !a.k_pages || !a.v_pages || !a.page_table || !a.lengths || !a.out || !a.workspace ||
+      (z.prefix_len > 0 && !a.prefix_table))
     return set_error(DK_ERR_INVALID, "%s: NULL pointer", what);
-  if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(out) || (ldq & 7) ||
-      (reinterpret_cast<uintptr_t>(workspace) & 255))
+  if (!aligned16(a.q) || !aligned16(a.k_pages) || !aligned16(a.v_pages) || !aligned16(a.out) || (a.ldq & 7) ||
+      (reinterpret_cast<uintptr_t>(a.workspace) & 255))
     return set_error(DK_ERR_ALIGN, "%s: q rows, pages and out need 16-byte alignment, the workspace 256", what);
   Pass own = {}, pre = {};
-  Cutter c{static_cast<char*>(workspace)};
+  Cutter c{static_cast<char*>(a.workspace)};
   shape_own(z, own);
   cut_pass(z, c, own, z.prefix_len > 0);
   if (z.prefix_len > 0) {
     shape_prefix(z, pre);
     cut_pass(z, c, pre, true);
   }
-  if (c.used > workspace_bytes)
+  if (c.used > a.workspace_bytes)
     return set_error(DK_ERR_INVALID, "%s: the workspace has %llu bytes, %llu are needed", what,
-                     (unsigned long long)workspace_bytes, (unsigned long long)c.used);
+                     (unsigned long long)a.workspace_bytes, (unsigned long long)c.used);
   if (own.ctas == 0 || (z.prefix_len > 0 && pre.ctas == 0))
     return set_error(DK_ERR_UNSUPPORTED, "%s: the kernel's shared memory does not fit this device", what);
   for (Problem* p : {&own.p, &pre.p}) {
-    p->q = q, p->ldq = ldq, p->out = out;
-    p->table = page_table, p->ld_table = ld_table, p->lengths = lengths, p->starts = starts;
+    p->q = a.q, p->ldq = a.ldq, p->out = a.out;
+    p->table = a.page_table, p->ld_table = a.ld_table, p->lengths = a.lengths, p->starts = a.starts;
     p->T = static_cast<int>(z.T), p->B = static_cast<int>(z.B), p->nkv = static_cast<int>(z.nkv);
     p->G = static_cast<int>(z.nq / z.nkv);
     p->n_pages = static_cast<int>(n_pages), p->page_size = static_cast<int>(page_size);
     p->page_shift = __builtin_ctzll(page_size);
     p->capacity = static_cast<int>(table_width * page_size);
     p->mask = Mask{static_cast<int>(window), window > 0 ? static_cast<int>(sinks) : 0};
-    p->scale2 = scale * 1.44269504088896341f;
+    p->scale2 = static_cast<float>(a.scale * 1.44269504088896341);
     p->err = device_info().err_word;
   }
-  pre.p.table = prefix_table, pre.p.capacity = static_cast<int>(z.prefix_len), pre.p.mask = Mask{0, 0};
+  pre.p.table = a.prefix_table, pre.p.capacity = static_cast<int>(z.prefix_len), pre.p.mask = Mask{0, 0};
 
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(a.stream);
   const uint64_t rows = static_cast<uint64_t>(n_pages * z.nkv * page_size);
   const uint32_t box = static_cast<uint32_t>(std::min<int64_t>(page_size, kChunk));
   const CUtensorMapDataType type = z.dtype == DK_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   CUtensorMap mk, mv;
-  if (!make_tensor_map_2d(&mk, k_pages, type, z.hd, rows, z.hd * 2, 64, box, CU_TENSOR_MAP_SWIZZLE_128B) ||
-      !make_tensor_map_2d(&mv, v_pages, type, z.hd, rows, z.hd * 2, 64, box, CU_TENSOR_MAP_SWIZZLE_128B))
+  const bool any_rows = !own.tc || (z.prefix_len > 0 && !pre.tc);
+  if (any_rows && (!make_tensor_map_2d(&mk, a.k_pages, type, z.hd, rows, z.hd * 2, 64, box, CU_TENSOR_MAP_SWIZZLE_128B) ||
+                   !make_tensor_map_2d(&mv, a.v_pages, type, z.hd, rows, z.hd * 2, 64, box, CU_TENSOR_MAP_SWIZZLE_128B)))
     return DK_ERR_CUDA;
   cudaError_t e = cudaSuccess;
   if (z.ragged)
     e = launch(plan_kernel<kTcChunk>, dim3(1), dim3(kPlanThreads), 0, st, pdl_enabled(), dim3(1, 1, 1), own.p,
                const_cast<int32_t*>(own.p.plan), const_cast<int4*>(own.p.tile_info));
-  for (const Pass* a : {&pre, &own}) {
-    if (a->ctas == 0 || e != cudaSuccess) continue;
-    if (a->tc) {
-      if (const int rc = tc_launch(a->p, z.nq, z.hd, z.dtype, a->ctas, k_pages, v_pages, st)) return rc;
+  for (const Pass* s : {&pre, &own}) {
+    if (s->ctas == 0 || e != cudaSuccess) continue;
+    if (s->tc) {
+      if (const int rc = tc_launch(s->p, z.nq, z.hd, z.dtype, s->ctas, a.k_pages, a.v_pages, st)) return rc;
     } else {
-      e = launch_rows(z, a->rows, a->shape, st, mk, mv, a->p, 0);
+      e = launch_rows(z, s->rows, s->shape, st, mk, mv, s->p, 0);
     }
   }
   const Pass* with = z.prefix_len > 0 ? &pre : nullptr;
@@ -809,25 +813,8 @@ int attention(const char* what, const Sizes& z, const void* q, int64_t ldq, cons
 
 }  // namespace
 
-extern "C" int dk_paged_attention(const void* q, int64_t ldq, const void* k_pages, const void* v_pages, int64_t n_pages,
-                                  int64_t page_size, const int32_t* page_table, int64_t ld_table, int64_t table_width,
-                                  const int32_t* lengths, const int32_t* starts, int64_t window, int64_t sinks,
-                                  float scale, void* out, int64_t T, int64_t B, int64_t nq, int64_t nkv,
-                                  int64_t head_dim, int32_t dtype, void* workspace, uint64_t workspace_bytes,
-                                  dk_stream_t stream) {
-  const Sizes z{T, B, nq, nkv, head_dim, 0, starts != nullptr, dtype};
-  return attention("paged_attention", z, q, ldq, k_pages, v_pages, n_pages, page_size, nullptr, page_table, ld_table,
-                   table_width, lengths, starts, window, sinks, scale, out, workspace, workspace_bytes, stream);
-}
+extern "C" int dk_paged_attention(const dk_paged_attention_args* args) { return attention("paged_attention", args, false); }
 
-extern "C" int dk_shared_prefix_attention(const void* q, int64_t ldq, const void* k_pages, const void* v_pages,
-                                          int64_t n_pages, int64_t page_size, const int32_t* prefix_table,
-                                          int64_t prefix_len, const int32_t* page_table, int64_t ld_table,
-                                          int64_t table_width, const int32_t* lengths, const int32_t* starts,
-                                          float scale, void* out, int64_t T, int64_t B, int64_t nq, int64_t nkv,
-                                          int64_t head_dim, int32_t dtype, void* workspace, uint64_t workspace_bytes,
-                                          dk_stream_t stream) {
-  const Sizes z{T, B, nq, nkv, head_dim, prefix_len, starts != nullptr, dtype};
-  return attention("shared_prefix_attention", z, q, ldq, k_pages, v_pages, n_pages, page_size, prefix_table, page_table,
-                   ld_table, table_width, lengths, starts, 0, 0, scale, out, workspace, workspace_bytes, stream);
+extern "C" int dk_shared_prefix_attention(const dk_paged_attention_args* args) {
+  return attention("shared_prefix_attention", args, true);
 }

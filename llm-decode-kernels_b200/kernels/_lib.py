@@ -8,6 +8,7 @@ raises. A negative status from the library becomes a RuntimeError carrying `dk_l
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 from pathlib import Path
 
@@ -52,6 +53,11 @@ class StepModel(ctypes.Structure):
                 ("embed", P), ("final_norm", P), ("lm_head", P), ("rope_cos", P), ("rope_sin", P),
                 ("k_cache", P), ("v_cache", P), ("layers", ctypes.POINTER(StepLayer))]
 
+
+# dk_paged_append_args and dk_paged_attention_args (8-byte fields throughout), packed in one step: ctypes takes about
+# 0.1 us for each argument of a call
+PAGED_APPEND_ARGS = struct.Struct("25q")
+PAGED_ATTENTION_ARGS = struct.Struct("15qd10q")
 
 FLAG_STATIC_WEIGHTS = 1
 FLAG_GENERIC = 2
@@ -98,13 +104,10 @@ SIGNATURES = {
                                   P],
     "dk_w4a16_matmul_reduce_static": [P, I64, P, P, P, P, P, I64, I64, I64, I64, I64, ctypes.POINTER(MatmulConfig),
                                       P],
-    "dk_paged_append": [P, I64, P, P, I64, I64, P, I64, I64, P, P, P, P, I32, I64, I64, I64, P, I64, I64, I64, I64, I64,
-                        I32, P],
+    "dk_paged_append": [ctypes.c_char_p],
     "dk_paged_attention_workspace_bytes": [I64, I64, I64, I64, I64, I32, I32, I64, ctypes.POINTER(ctypes.c_uint64)],
-    "dk_paged_attention": [P, I64, P, P, I64, I64, P, I64, I64, P, P, I64, I64, F32, P, I64, I64, I64, I64, I64, I32,
-                           P, ctypes.c_uint64, P],
-    "dk_shared_prefix_attention": [P, I64, P, P, I64, I64, P, I64, P, I64, I64, P, P, F32, P, I64, I64, I64, I64, I64,
-                                   I32, P, ctypes.c_uint64, P],
+    "dk_paged_attention": [ctypes.c_char_p],
+    "dk_shared_prefix_attention": [ctypes.c_char_p],
     "dk_token_logprobs": [P, I64, I32, P, I64, I64, I64, P, P, P, P, P],
     "dk_step_workspace_bytes": [ctypes.POINTER(StepModel), ctypes.POINTER(ctypes.c_uint64)],
     "dk_step_create": [ctypes.POINTER(StepModel), P, ctypes.c_uint64, ctypes.POINTER(P)],

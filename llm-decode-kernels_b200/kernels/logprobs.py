@@ -19,26 +19,31 @@ def token_logprobs(logits, targets, top=0):
     probability is 0. A target >= V gives NaN and sets the device error DK_DEVERR_BAD_TOKEN. Logits of -inf are tokens
     that cannot occur; a row with a NaN or +inf, or nothing but -inf, has NaN log probabilities."""
     what = "token_logprobs"
-    _lib.require_extent(logits.dim() == 2 and logits.shape[1] > 0 and logits.stride(1) == 1,
-                        f"{what}: logits must be [rows, vocab] with unit column stride")
+    if logits.dim() != 2 or logits.shape[1] == 0:
+        raise ValueError(f"{what}: logits must be [rows, vocab]")
     M, V = logits.shape
-    _lib.require_extent(logits.stride(0) >= V or M <= 1, f"{what}: rows of logits overlap")
-    _lib.require_extent(targets.dim() == 1 and targets.shape[0] == M and targets.is_contiguous(),
-                        f"{what}: targets must hold one token per row")
-    _lib.require_extent(0 <= top <= min(MAX_TOP, V), f"{what}: top must be 0..{MAX_TOP}, at most the vocabulary")
-    if logits.dtype not in _DTYPES:
+    ld, unit = logits.stride()
+    if unit != 1 or (ld < V and M > 1):
+        raise ValueError(f"{what}: logits must have unit column stride and rows that do not overlap")
+    if targets.shape != (M,) or not targets.is_contiguous():
+        raise ValueError(f"{what}: targets must hold one token per row")
+    if not 0 <= top <= min(MAX_TOP, V):
+        raise ValueError(f"{what}: top must be 0..{MAX_TOP}, at most the vocabulary")
+    dtype = _DTYPES.get(logits.dtype)
+    if dtype is None:
         raise RuntimeError(f"{what}: logits must be fp16, bf16 or fp32, got {logits.dtype}")
-    if targets.dtype != torch.int64:
+    if targets.dtype is not torch.int64:
         raise RuntimeError(f"{what}: targets must be int64")
-    _lib.require_cuda(what, logits, targets)
-    dev = logits.device
-    if targets.device != dev:
-        raise RuntimeError(f"{what}: tensors on {dev} and {targets.device}")
-    stats = torch.empty((2, M), dtype=torch.float32, device=dev)
-    values = torch.empty((M, top), dtype=torch.float32, device=dev)
-    ids = torch.empty((M, top), dtype=torch.int64, device=dev)
-    lp, entropy = stats[0], stats[1]
-    _lib.call("dk_token_logprobs", logits.data_ptr(), max(logits.stride(0), V), _DTYPES[logits.dtype], targets.data_ptr(),
-              M, V, top, lp.data_ptr(), entropy.data_ptr(), values.data_ptr(), ids.data_ptr(),
-              torch.cuda.current_stream(dev).cuda_stream)
+    device = logits.get_device()
+    if device < 0 or targets.get_device() != device:
+        raise RuntimeError(f"{what}: tensors must be on one CUDA device (no CPU path), got {logits.device} and {targets.device}")
+    lp = logits.new_empty((M,), dtype=torch.float32)
+    entropy = torch.empty_like(lp)
+    values = logits.new_empty((M, top), dtype=torch.float32)
+    ids = targets.new_empty((M, top))
+    status = _lib.lib().dk_token_logprobs(logits.data_ptr(), ld if ld >= V else V, dtype, targets.data_ptr(), M, V, top,
+                                          lp.data_ptr(), entropy.data_ptr(), values.data_ptr(), ids.data_ptr(),
+                                          torch._C._cuda_getCurrentRawStream(device))
+    if status:
+        _lib.check(status, what)
     return lp, entropy, values, ids

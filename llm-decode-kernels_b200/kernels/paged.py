@@ -17,7 +17,6 @@ from __future__ import annotations
 
 import ctypes
 import functools
-import math
 
 import torch
 
@@ -25,43 +24,59 @@ from kernels import _lib
 
 MAX_GROUP = 16  # query heads per kv head
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1}
+_INT32 = torch.int32
+_raw_stream = torch._C._cuda_getCurrentRawStream  # (the public form builds a Stream object, about 1 us of each call)
+
+
+# These calls are small next to their checks, so the checks are plain comparisons whose messages are only put together
+# when one fails.
+def _refuse(what: str, message: str):
+    raise ValueError(f"{what}: {message}")
+
+
+def _wrong_type(what: str, message: str):
+    raise RuntimeError(f"{what}: {message}")
 
 
 def _cache_shape(what, k_pages, v_pages, page_table, lengths, starts, tokens):
     """(n_pages, n_kv, page_size, head_dim, B) of a checked cache and batch."""
-    need = _lib.require_extent
-    need(k_pages.dim() == 4 and k_pages.shape == v_pages.shape,
-         f"{what}: k_pages and v_pages must be [n_pages, n_kv, page_size, head_dim], both alike")
-    need(k_pages.is_contiguous() and v_pages.is_contiguous(), f"{what}: pages must be contiguous")
-    n_pages, n_kv, page, hd = k_pages.shape
-    need(n_pages > 0 and n_kv > 0, f"{what}: an empty pool of pages")
-    need(16 <= page <= 256 and page & (page - 1) == 0, f"{what}: page_size must be a power of two from 16 to 256")
-    need(hd == 64 or hd == 128, f"{what}: head_dim must be 64 or 128")
-    need(page_table.dim() == 2 and page_table.shape[1] > 0 and page_table.stride(1) == 1,
-         f"{what}: page_table must be [sequences, pages] with unit column stride")
+    shape = k_pages.shape
+    if len(shape) != 4 or v_pages.shape != shape:
+        _refuse(what, "k_pages and v_pages must be [n_pages, n_kv, page_size, head_dim], both alike")
+    if not (k_pages.is_contiguous() and v_pages.is_contiguous()):
+        _refuse(what, "pages must be contiguous")
+    n_pages, n_kv, page, hd = shape
+    if n_pages <= 0 or n_kv <= 0:
+        _refuse(what, "an empty pool of pages")
+    if not (16 <= page <= 256 and page & (page - 1) == 0):
+        _refuse(what, "page_size must be a power of two from 16 to 256")
+    if hd != 128 and hd != 64:
+        _refuse(what, "head_dim must be 64 or 128")
+    if page_table.dim() != 2 or page_table.shape[1] == 0 or page_table.stride()[1] != 1:
+        _refuse(what, "page_table must be [sequences, pages] with unit column stride")
     B = page_table.shape[0]
-    need(lengths.dim() == 1 and lengths.shape[0] == B and lengths.is_contiguous(),
-         f"{what}: lengths must hold one count per row of page_table")
+    if lengths.shape != (B,) or not lengths.is_contiguous():
+        _refuse(what, "lengths must hold one count per row of page_table")
     if starts is None:
-        need(tokens == B, f"{what}: without starts there is one token per sequence")
-    else:
-        need(starts.dim() == 1 and starts.shape[0] == B + 1 and starts.is_contiguous(),
-             f"{what}: starts must hold sequences + 1 row numbers")
-    if not (page_table.dtype == lengths.dtype == torch.int32 and (starts is None or starts.dtype == torch.int32)):
-        raise RuntimeError(f"{what}: page_table, lengths and starts must be int32")
-    if k_pages.dtype not in _DTYPES or v_pages.dtype != k_pages.dtype:
-        raise RuntimeError(f"{what}: pages must be fp16 or bf16, both alike")
+        if tokens != B:
+            _refuse(what, "without starts there is one token per sequence")
+    elif starts.shape != (B + 1,) or not starts.is_contiguous():
+        _refuse(what, "starts must hold sequences + 1 row numbers")
+    if not (page_table.dtype is _INT32 and lengths.dtype is _INT32 and (starts is None or starts.dtype is _INT32)):
+        _wrong_type(what, "page_table, lengths and starts must be int32")
+    if k_pages.dtype not in _DTYPES or v_pages.dtype is not k_pages.dtype:
+        _wrong_type(what, "pages must be fp16 or bf16, both alike")
     return n_pages, n_kv, page, hd, B
 
 
-def _on_one_device(what, *tensors):
-    device = tensors[0].device
+def _one_device(what, tensors):
+    """The CUDA device that all tensors (None: left out) lie on."""
+    index = tensors[0].get_device()
     for t in tensors:
-        if t is not None:
-            if not t.is_cuda:
-                raise RuntimeError(f"{what}: tensors must be on a CUDA device (no CPU path), got {t.device}")
-            if t.device != device:
-                raise RuntimeError(f"{what}: tensors on {device} and {t.device}")
+        if t is not None and t.get_device() != index or index < 0:
+            where = {str(t.device) for t in tensors if t is not None}
+            _wrong_type(what, f"tensors must be on one CUDA device (no CPU path), got {', '.join(sorted(where))}")
+    return index
 
 
 def paged_append(qkv, k_pages, v_pages, page_table, lengths, cos, sin, n_heads, n_kv, starts=None, offset=0, out=None):
@@ -72,32 +87,38 @@ def paged_append(qkv, k_pages, v_pages, page_table, lengths, cos, sin, n_heads, 
     head_dim] (`out` if given). A token without a page, or past the tables, appends nothing and sets the device error
     DK_DEVERR_BAD_POSITION; one of an unused slot appends nothing and returns zeros."""
     what = "paged_append"
-    _lib.require_extent(qkv.dim() == 2, f"{what}: qkv must be [tokens, (n_heads + 2 n_kv) * head_dim]")
-    T = qkv.shape[0]
+    if qkv.dim() != 2:
+        _refuse(what, "qkv must be [tokens, (n_heads + 2 n_kv) * head_dim]")
+    T, width = qkv.shape
     n_pages, kv, page, hd, B = _cache_shape(what, k_pages, v_pages, page_table, lengths, starts, T)
-    _lib.require_extent(n_kv == kv and n_heads > 0 and qkv.shape[1] == (n_heads + 2 * n_kv) * hd and qkv.stride(1) == 1,
-                        f"{what}: qkv must be [tokens, (n_heads + 2 n_kv) * head_dim] with the pages' kv heads")
-    _lib.require_extent(cos.dim() == 2 and cos.shape == sin.shape and cos.shape[1] == hd // 2 and cos.stride(1) == 1
-                        and cos.stride() == sin.stride(), f"{what}: cos and sin must be [positions, head_dim / 2]")
-    _lib.require_extent(offset >= 0, f"{what}: offset must not be negative")
-    if qkv.dtype != k_pages.dtype:
-        raise RuntimeError(f"{what}: qkv is {qkv.dtype}, the pages are {k_pages.dtype}")
-    if cos.dtype != sin.dtype or (cos.dtype != torch.float32 and cos.dtype != qkv.dtype):
-        raise RuntimeError(f"{what}: cos and sin must be fp32 or qkv's type")
-    if out is not None:
-        _lib.require_extent(tuple(out.shape) == (T, n_heads, hd) and out.is_contiguous() and out.dtype == qkv.dtype,
-                            f"{what}: out must be a contiguous [tokens, n_heads, head_dim] of qkv's type")
-    _on_one_device(what, qkv, k_pages, v_pages, page_table, lengths, starts, cos, sin, out)
-    q = torch.empty((T, n_heads, hd), dtype=qkv.dtype, device=qkv.device) if out is None else out
-    _lib.call("dk_paged_append", qkv.data_ptr(), qkv.stride(0), k_pages.data_ptr(), v_pages.data_ptr(), n_pages, page,
-              page_table.data_ptr(), page_table.stride(0), page_table.shape[1], lengths.data_ptr(),
-              None if starts is None else starts.data_ptr(), cos.data_ptr(), sin.data_ptr(),
-              1 if cos.dtype == torch.float32 else 0, cos.stride(0), cos.shape[0], offset, q.data_ptr(), T, B, n_heads,
-              n_kv, hd, _DTYPES[qkv.dtype], torch.cuda.current_stream(qkv.device).cuda_stream)
+    ld, unit = qkv.stride()
+    if n_kv != kv or n_heads <= 0 or width != (n_heads + 2 * n_kv) * hd or unit != 1:
+        _refuse(what, "qkv must be [tokens, (n_heads + 2 n_kv) * head_dim] with the pages' kv heads and unit column stride")
+    if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] != hd // 2 or cos.stride() != sin.stride() or cos.stride()[1] != 1:
+        _refuse(what, "cos and sin must be [positions, head_dim / 2]")
+    if offset < 0:
+        _refuse(what, "offset must not be negative")
+    dtype = qkv.dtype
+    if dtype is not k_pages.dtype:
+        _wrong_type(what, f"qkv is {dtype}, the pages are {k_pages.dtype}")
+    f32 = cos.dtype is torch.float32
+    if sin.dtype is not cos.dtype or not (f32 or cos.dtype is dtype):
+        _wrong_type(what, "cos and sin must be fp32 or qkv's type")
+    if out is not None and (out.shape != (T, n_heads, hd) or not out.is_contiguous() or out.dtype is not dtype):
+        _refuse(what, "out must be a contiguous [tokens, n_heads, head_dim] of qkv's type")
+    device = _one_device(what, (qkv, k_pages, v_pages, page_table, lengths, starts, cos, sin, out))
+    q = qkv.new_empty((T, n_heads, hd)) if out is None else out
+    status = _lib.lib().dk_paged_append(_lib.PAGED_APPEND_ARGS.pack(
+        qkv.data_ptr(), ld, k_pages.data_ptr(), v_pages.data_ptr(), n_pages, page, page_table.data_ptr(),
+        page_table.stride()[0], page_table.shape[1], lengths.data_ptr(), 0 if starts is None else starts.data_ptr(),
+        cos.data_ptr(), sin.data_ptr(), f32, cos.stride()[0], cos.shape[0], offset, q.data_ptr(), T, B, n_heads, n_kv, hd,
+        _DTYPES[dtype], _raw_stream(device)))
+    if status:
+        _lib.check(status, what)
     return q
 
 
-@functools.lru_cache(maxsize=1024)
+@functools.lru_cache(maxsize=4096)
 def _workspace_bytes(T, B, nq, nkv, hd, dtype, ragged, prefix, device):
     n = ctypes.c_uint64(0)
     with torch.cuda.device(device):
@@ -105,18 +126,44 @@ def _workspace_bytes(T, B, nq, nkv, hd, dtype, ragged, prefix, device):
     return int(n.value)
 
 
-def _check_queries(what, q, k_pages, n_kv, hd, scale, out):
-    _lib.require_extent(q.dim() == 3 and q.shape[2] == hd and q.stride(2) == 1 and q.stride(1) == hd,
-                        f"{what}: q must be [tokens, heads, head_dim] with its heads side by side")
-    nq = q.shape[1]
-    _lib.require_extent(nq > 0 and nq % n_kv == 0 and nq // n_kv <= MAX_GROUP,
-                        f"{what}: query heads must be a multiple of the kv heads, at most {MAX_GROUP} for each")
-    if q.dtype != k_pages.dtype:
-        raise RuntimeError(f"{what}: q is {q.dtype}, the pages are {k_pages.dtype}")
-    if out is not None:
-        _lib.require_extent(out.shape == q.shape and out.is_contiguous() and out.dtype == q.dtype,
-                            f"{what}: out must be a contiguous tensor of q's shape and type")
-    return hd ** -0.5 if scale is None else float(scale)
+def _attend(what, entry, q, k_pages, v_pages, prefix_table, prefix_len, page_table, lengths, starts, window, sinks, scale, out):
+    if q.dim() != 3:
+        _refuse(what, "q must be [tokens, heads, head_dim]")
+    T, nq, width = q.shape
+    n_pages, n_kv, page, hd, B = _cache_shape(what, k_pages, v_pages, page_table, lengths, starts, T)
+    ld, by_head, unit = q.stride()
+    if width != hd or unit != 1 or by_head != hd:
+        _refuse(what, "q must be [tokens, heads, head_dim] with its heads side by side")
+    if nq <= 0 or nq % n_kv or nq // n_kv > MAX_GROUP:
+        _refuse(what, f"query heads must be a multiple of the kv heads, at most {MAX_GROUP} for each")
+    dtype = q.dtype
+    if dtype is not k_pages.dtype:
+        _wrong_type(what, f"q is {dtype}, the pages are {k_pages.dtype}")
+    if out is None:
+        out = q.new_empty((T, nq, hd))
+    elif out.shape != q.shape or not out.is_contiguous() or out.dtype is not dtype:
+        _refuse(what, "out must be a contiguous tensor of q's shape and type")
+    prefix_at = 0
+    if prefix_len:
+        if prefix_len < 0 or prefix_table.dim() != 1 or not prefix_table.is_contiguous() or \
+                prefix_table.shape[0] * page < prefix_len:
+            _refuse(what, "prefix_table must list the pages of prefix_len positions")
+        if prefix_table.dtype is not _INT32:
+            _wrong_type(what, "prefix_table must be int32")
+        prefix_at = prefix_table.data_ptr()
+    device = _one_device(what, (q, k_pages, v_pages, page_table, lengths, starts, prefix_table, out))
+    code = _DTYPES[dtype]
+    # the prefix's length does not change the size, only whether there is one
+    nbytes = _workspace_bytes(T, B, nq, n_kv, hd, code, starts is not None, 1 if prefix_len else 0, device)
+    ws = q.new_empty((nbytes,), dtype=torch.uint8)
+    status = getattr(_lib.lib(), entry)(_lib.PAGED_ATTENTION_ARGS.pack(
+        q.data_ptr(), ld, k_pages.data_ptr(), v_pages.data_ptr(), n_pages, page, prefix_at, prefix_len,
+        page_table.data_ptr(), page_table.stride()[0], page_table.shape[1], lengths.data_ptr(),
+        0 if starts is None else starts.data_ptr(), window, sinks, hd ** -0.5 if scale is None else scale, out.data_ptr(), T,
+        B, nq, n_kv, hd, code, ws.data_ptr(), nbytes, _raw_stream(device)))
+    if status:
+        _lib.check(status, what)
+    return out
 
 
 def paged_attention(q, k_pages, v_pages, page_table, lengths, starts=None, window=0, sinks=0, scale=None, out=None):
@@ -125,22 +172,10 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, starts=None, windo
     n_heads, head_dim] contiguous (`out` if given); a row that sees nothing is zero. scale: head_dim ** -0.5 if
     None. Pages that no row sees are not read, and their table entries may hold anything. With several tokens of a
     sequence in one call, the keys and values that one of them sees have to be finite for the others too."""
-    what = "paged_attention"
-    T = q.shape[0]
-    n_pages, n_kv, page, hd, B = _cache_shape(what, k_pages, v_pages, page_table, lengths, starts, T)
-    scale = _check_queries(what, q, k_pages, n_kv, hd, scale, out)
-    _lib.require_extent(window >= 0 and sinks >= 0, f"{what}: window and sinks must not be negative")
-    _on_one_device(what, q, k_pages, v_pages, page_table, lengths, starts, out)
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    nq, dtype = q.shape[1], _DTYPES[q.dtype]
-    nbytes = _workspace_bytes(T, B, nq, n_kv, hd, dtype, starts is not None, 0, q.device)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-    _lib.call("dk_paged_attention", q.data_ptr(), q.stride(0), k_pages.data_ptr(), v_pages.data_ptr(), n_pages, page,
-              page_table.data_ptr(), page_table.stride(0), page_table.shape[1], lengths.data_ptr(),
-              None if starts is None else starts.data_ptr(), window, sinks, scale, out.data_ptr(), T, B, nq, n_kv, hd,
-              dtype, ws.data_ptr(), nbytes, torch.cuda.current_stream(q.device).cuda_stream)
-    return out
+    if window < 0 or sinks < 0:
+        _refuse("paged_attention", "window and sinks must not be negative")
+    return _attend("paged_attention", "dk_paged_attention", q, k_pages, v_pages, None, 0, page_table, lengths, starts, window,
+                   sinks, scale, out)
 
 
 def shared_prefix_attention(q, k_pages, v_pages, prefix_table, prefix_len, page_table, lengths, starts=None, scale=None,
@@ -149,26 +184,7 @@ def shared_prefix_attention(q, k_pages, v_pages, prefix_table, prefix_len, page_
     prefix_len positions (in the pages prefix_table lists, int32 [>= pages of the prefix]) and, causally, its own
     sequence's positions (page_table, lengths, starts: counted without the prefix). The prefix's keys and values are
     read once for all rows. Returns [T, n_heads, head_dim] (`out` if given)."""
-    what = "shared_prefix_attention"
     if prefix_len == 0:
         return paged_attention(q, k_pages, v_pages, page_table, lengths, starts, scale=scale, out=out)
-    T = q.shape[0]
-    n_pages, n_kv, page, hd, B = _cache_shape(what, k_pages, v_pages, page_table, lengths, starts, T)
-    scale = _check_queries(what, q, k_pages, n_kv, hd, scale, out)
-    _lib.require_extent(prefix_len > 0 and prefix_table.dim() == 1 and prefix_table.is_contiguous()
-                        and prefix_table.shape[0] >= math.ceil(prefix_len / page),
-                        f"{what}: prefix_table must list the pages of prefix_len positions")
-    if prefix_table.dtype != torch.int32:
-        raise RuntimeError(f"{what}: prefix_table must be int32")
-    _on_one_device(what, q, k_pages, v_pages, prefix_table, page_table, lengths, starts, out)
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    nq, dtype = q.shape[1], _DTYPES[q.dtype]
-    nbytes = _workspace_bytes(T, B, nq, n_kv, hd, dtype, starts is not None, prefix_len, q.device)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-    _lib.call("dk_shared_prefix_attention", q.data_ptr(), q.stride(0), k_pages.data_ptr(), v_pages.data_ptr(), n_pages,
-              page, prefix_table.data_ptr(), prefix_len, page_table.data_ptr(), page_table.stride(0),
-              page_table.shape[1], lengths.data_ptr(), None if starts is None else starts.data_ptr(), scale,
-              out.data_ptr(), T, B, nq, n_kv, hd, dtype, ws.data_ptr(), nbytes,
-              torch.cuda.current_stream(q.device).cuda_stream)
-    return out
+    return _attend("shared_prefix_attention", "dk_shared_prefix_attention", q, k_pages, v_pages, prefix_table, prefix_len,
+                   page_table, lengths, starts, 0, 0, scale, out)

@@ -331,10 +331,15 @@ def test_c_entries_refuse_without_a_gpu():
     def attend(**more):
         a = dict(T=2, B=2, nq=12, nkv=2, hd=128, page=16, dtype=0, ldq=1536, pages=4, width=2)
         a.update(more)
-        return h.dk_paged_attention(None, a["ldq"], None, None, a["pages"], a["page"], None, a["width"], a["width"], None,
-                                    None, 0, 0, 1.0, None, a["T"], a["B"], a["nq"], a["nkv"], a["hd"], a["dtype"], None, 0,
-                                    None)
+        return h.dk_paged_attention(_lib.PAGED_ATTENTION_ARGS.pack(
+            0, a["ldq"], 0, 0, a["pages"], a["page"], 0, 0, 0, a["width"], a["width"], 0, 0, 0, 0, 1.0, 0, a["T"], a["B"],
+            a["nq"], a["nkv"], a["hd"], a["dtype"], 0, 0, 0))
 
+    def append(page):
+        return h.dk_paged_append(_lib.PAGED_APPEND_ARGS.pack(0, 0, 0, 0, 4, page, 0, 2, 2, 0, 0, 0, 0, 1, 64, 10, 0, 0, 3, 2,
+                                                             12, 2, 128, 0, 0))
+
+    assert h.dk_paged_attention(None) == -1 and h.dk_shared_prefix_attention(None) == -1 and h.dk_paged_append(None) == -1
     assert attend() == -1 and b"NULL" in h.dk_last_error()
     assert attend(T=3) == -1 and b"one token" in h.dk_last_error()
     assert attend(hd=96) == -3 and b"head_dim" in h.dk_last_error()
@@ -345,7 +350,5 @@ def test_c_entries_refuse_without_a_gpu():
     assert attend(pages=1 << 26) == -1 and b"2^31" in h.dk_last_error()
     assert attend(width=1 << 27) == -1
     assert h.dk_paged_attention_workspace_bytes(2, 2, 12, 2, 96, 0, 0, 0, ctypes.byref(n)) == -3
-    assert h.dk_paged_append(None, 0, None, None, 4, 16, None, 2, 2, None, None, None, None, 1, 64, 10, 0, None, 3, 2, 12,
-                             2, 128, 0, None) == -1
-    assert h.dk_paged_append(None, 0, None, None, 4, 20, None, 2, 2, None, None, None, None, 1, 64, 10, 0, None, 2, 2, 12,
-                             2, 128, 0, None) == -3
+    assert append(16) == -1 and b"one token" in h.dk_last_error()
+    assert append(20) == -3 and b"page_size" in h.dk_last_error()

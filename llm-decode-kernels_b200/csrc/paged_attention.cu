@@ -9,8 +9,7 @@
 // The decode kernel is bound by the bytes of k and v: each is read once for the G query heads that share
 // it. A producer warp streams chunks of 64 positions, page by page, through a ring of TMA boxes (128-byte
 // swizzle: the ldmatrix reads hit all banks); pages that no row sees are never read, and their table
-// entries may be anything. Two groups of four consumer warps take alternate chunks, 16
-// positions a warp: q.k on the tensor cores with the
+// entries may be anything. Four consumer warps of a group take 16 positions each: q.k on the tensor cores with the
 // query heads as the rows, online softmax in registers, p.v on the tensor cores with p taken from the
 // score accumulators. A position that no row of the tile sees reads a zero row instead of v, so whatever
 // the page holds there (infinities and NaN included) stays out; masked scores are replaced, not added to.
@@ -25,9 +24,10 @@ namespace paged {
 namespace {
 
 constexpr int kChunk = 64;
-constexpr int kCWarps = 8;  // two groups of four, for alternate chunks
-constexpr int kThreads = (kCWarps + 1) * 32;
-constexpr int kMaxRing = 8;
+constexpr int kGroups = 2;   // independent consumer groups of a CTA, each with a piece of the line of its own
+constexpr int kCWarps = 4;   // warps of a group
+constexpr int kThreads = kGroups * (kCWarps + 1) * 32;
+constexpr int kMaxRing = 6;
 constexpr int kPlanThreads = 1024;
 
 // ------------------------------------------------------------------------------------ ragged plan
@@ -127,7 +127,9 @@ struct Box {
   }
 };
 
-__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"r"(kCWarps * 32) : "memory"); }
+__device__ __forceinline__ void group_sync(int group) {
+  asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(kCWarps * 32) : "memory");
+}
 
 template <typename T, int kHd, int kRows>
 __global__ void __launch_bounds__(kThreads)
@@ -139,21 +141,27 @@ __global__ void __launch_bounds__(kThreads)
   constexpr bool kTwo = kRows == 16;  // rows 8..15 of the MMA in use
   constexpr int kR = kTwo ? 2 : 1;
   __shared__ __align__(16) uint4 vzero;
-  __shared__ float pre_ml[kCWarps * kRows * 2];
-  __shared__ float pre_w[kCWarps * kRows];
-  __shared__ float fin[kRows * 2];
-  __shared__ __align__(8) uint64_t full[kMaxRing], empty[kMaxRing];
+  __shared__ float pre_ml_sh[kGroups][kCWarps * kRows * 2];
+  __shared__ float pre_w_sh[kGroups][kCWarps * kRows];
+  __shared__ float fin_sh[kGroups][kRows * 2];
+  __shared__ __align__(8) uint64_t full_sh[kGroups][kMaxRing], empty_sh[kGroups][kMaxRing];
   __shared__ int warp_sum[kThreads / 32 + 1];
   extern __shared__ __align__(128) uint8_t dsm_raw[];
-  uint8_t* slots = dsm_raw + ((1024u - (smem_addr(dsm_raw) & 1023u)) & 1023u);
-  float* pre_o = reinterpret_cast<float*>(slots + ring * B::kSlotBytes);  // [warp][row][dim]
-  int* cum_sh = reinterpret_cast<int*>(pre_o + kCWarps * kRows * kHd);    // kOneToken: [B + 1]
+  uint8_t* base = dsm_raw + ((1024u - (smem_addr(dsm_raw) & 1023u)) & 1023u);
+  int* cum_sh = reinterpret_cast<int*>(base);  // kOneToken: [B + 1], before the first copies land there
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const bool producer = warp >= kGroups * kCWarps;
+  const int group = producer ? warp - kGroups * kCWarps : warp / kCWarps;
+  const int cta = blockIdx.x * kGroups + group, ctas = gridDim.x * kGroups;  // pieces of the line: one a group
+  uint8_t* slots = base + group * ring * B::kSlotBytes;
+  float* pre_o = reinterpret_cast<float*>(base + kGroups * ring * B::kSlotBytes) + group * kCWarps * kRows * kHd;
+  float *pre_ml = pre_ml_sh[group], *pre_w = pre_w_sh[group], *fin = fin_sh[group];
+  uint64_t *full = full_sh[group], *empty = empty_sh[group];
   if (tid == 0) {
-    for (int i = 0; i < ring; ++i) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], kCWarps / 2);
+    for (int i = 0; i < kGroups * kMaxRing; ++i) {
+      mbar_init(&full_sh[0][i], 1);
+      mbar_init(&empty_sh[0][i], kCWarps);
     }
     fence_mbar_init();
     vzero = make_uint4(0, 0, 0, 0);
@@ -197,12 +205,14 @@ __global__ void __launch_bounds__(kThreads)
   }
   __syncthreads();
 
-  Walk<kChunk> walk(p, line, blockIdx.x, gridDim.x, lane);
+  Walk<kChunk> walk(p, line, cta, ctas, lane);
+  __syncthreads();  // the sums have been read: copies may land on them
   bool ok = true;
   int fill = 0;  // ring fills so far
 
-  if (warp == kCWarps) {
-    // ---------------------------------------------------------------- producer warp: one lane per box
+  if (producer) {
+    // ---------------------------------------------------------------- producer warps: one lane per box
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (the sums lay there)
     const int box = min(p.page_size, kChunk);  // rows of one box
     const int boxes = kChunk / box;
     const int kv = lane & 1, sg = (lane >> 1) % B::kSegs, pg = lane / (2 * B::kSegs);
@@ -242,8 +252,8 @@ __global__ void __launch_bounds__(kThreads)
     // ---------------------------------------------------------------- consumer warps
     const int g = lane >> 2, tq = lane & 3;
     const int mi = lane >> 3, rr = lane & 7;
-    const int group = warp >> 2, sub = warp & 3;
-    if (tid == 0) p.cut[blockIdx.x] = make_int4(0, 0, 0, 0);
+    const int sub = warp % kCWarps, gtid = tid - group * kCWarps * 32;
+    if (gtid == 0) p.cut[cta] = make_int4(0, 0, 0, 0);
     while (walk.more()) {
       const Span<kChunk> span = walk.step();
       const Tile t = walk.t;
@@ -272,7 +282,6 @@ __global__ void __launch_bounds__(kThreads)
       for (int e = 0; e < kR; ++e) m_run[e] = -INFINITY, l_run[e] = 0.f;
 
       for (int i = c0; i < c1; ++i, ++fill) {
-        if ((fill & 1) != group) continue;
         const int s = fill % ring;
         if (ok && !wait_for(&full[s], (fill / ring) & 1, p.err, DK_DEVERR_WAIT_FULL)) ok = false;
         ok = __all_sync(0xffffffffu, ok);
@@ -345,7 +354,7 @@ __global__ void __launch_bounds__(kThreads)
         if (lane == 0) mbar_arrive(&empty[s]);
       }
       // the warps' results of this part of the unit, joined
-      if (tid == 0 && walk.cut(span)) p.cut[blockIdx.x] = walk.cut_record(span);
+      if (gtid == 0 && walk.cut(span)) p.cut[cta] = walk.cut_record(span);
 #pragma unroll
       for (int e = 0; e < kR; ++e) {
         l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], 1);
@@ -353,34 +362,34 @@ __global__ void __launch_bounds__(kThreads)
         const int row = g + 8 * e;
 #pragma unroll
         for (int j = 0; j < kTiles; ++j)
-          *reinterpret_cast<float2*>(&pre_o[(warp * kRows + row) * kHd + 8 * j + 2 * tq]) =
+          *reinterpret_cast<float2*>(&pre_o[(sub * kRows + row) * kHd + 8 * j + 2 * tq]) =
               make_float2(o[j][2 * e], o[j][2 * e + 1]);
         if (tq == 0) {
-          pre_ml[(warp * kRows + row) * 2] = m_run[e];
-          pre_ml[(warp * kRows + row) * 2 + 1] = l_run[e];
+          pre_ml[(sub * kRows + row) * 2] = m_run[e];
+          pre_ml[(sub * kRows + row) * 2 + 1] = l_run[e];
         }
       }
-      consumers_sync();
+      group_sync(group);
       const bool all_of_it = c0 == 0 && c1 == span.n, whole = all_of_it && !p.always_partial;
-      if (tid < kRows) {
+      if (gtid < kRows) {
         float mx = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kCWarps; ++w) mx = fmaxf(mx, pre_ml[(w * kRows + tid) * 2]);
+        for (int w = 0; w < kCWarps; ++w) mx = fmaxf(mx, pre_ml[(w * kRows + gtid) * 2]);
         const float m_use = mx == -INFINITY ? 0.f : mx;
         float ls = 0.f;
 #pragma unroll
         for (int w = 0; w < kCWarps; ++w) {
-          const float wt = exp2_approx(pre_ml[(w * kRows + tid) * 2] - m_use);
-          pre_w[w * kRows + tid] = wt;
-          ls = fmaf(wt, pre_ml[(w * kRows + tid) * 2 + 1], ls);
+          const float wt = exp2_approx(pre_ml[(w * kRows + gtid) * 2] - m_use);
+          pre_w[w * kRows + gtid] = wt;
+          ls = fmaf(wt, pre_ml[(w * kRows + gtid) * 2 + 1], ls);
         }
-        fin[2 * tid] = mx;
-        fin[2 * tid + 1] = ls;
+        fin[2 * gtid] = mx;
+        fin[2 * gtid + 1] = ls;
       }
-      consumers_sync();
-      const int64_t slot = partial_slot(gridDim.x, blockIdx.x, c0 == 0, all_of_it, h * line.tiles + walk.ti);
+      group_sync(group);
+      const int64_t slot = partial_slot(ctas, cta, c0 == 0, all_of_it, h * line.tiles + walk.ti);
       if (ok) {
-        for (int e = tid; e < rows * (kHd / 4); e += kCWarps * 32) {
+        for (int e = gtid; e < rows * (kHd / 4); e += kCWarps * 32) {
           const int row = e / (kHd / 4), d = 4 * (e % (kHd / 4));
           float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
@@ -400,13 +409,13 @@ __global__ void __launch_bounds__(kThreads)
             *reinterpret_cast<float4*>(&p.part_o[(slot * kRows + row) * kHd + d]) = a;
           }
         }
-        if (!whole && tid < rows)
-          *reinterpret_cast<float2*>(&p.part_ml[(slot * kRows + tid) * 2]) = make_float2(fin[2 * tid], fin[2 * tid + 1]);
+        if (!whole && gtid < rows)
+          *reinterpret_cast<float2*>(&p.part_ml[(slot * kRows + gtid) * 2]) = make_float2(fin[2 * gtid], fin[2 * gtid + 1]);
       }
-      consumers_sync();  // pre_o, pre_ml and fin are written again by the next piece
+      group_sync(group);  // pre_o, pre_ml and fin are written again by the next piece
     }
   }
-  if (__syncthreads_or(!ok) && warp == kCWarps && lane == 0) {
+  if (__syncthreads_or(!ok) && producer && lane == 0) {
     // a wait gave up: let copies still in flight land before the shared memory goes away (bounded)
     const uint64_t t0 = globaltimer_ns();
     for (int f = max(0, fill - ring); f < fill; ++f)
@@ -551,19 +560,17 @@ struct RowsShape {
 };
 
 template <typename T, int kHd, int kRows>
-RowsShape rows_shape(int64_t B) {
+RowsShape rows_shape() {
   static std::mutex mu;
-  static int per_sm[2][64];  // by shared memory (batches up to 511 or more) and device; 0: not asked yet
+  static int per_sm[64];  // by device; 0: not asked yet
   RowsShape s;
-  const bool large = B > 511;
-  // Even: a slot always serves the same group of consumers, whose parity waits then see every phase of it.
-  s.ring = kHd == 64 ? 8 : 4;
-  s.smem = 1024 + static_cast<size_t>(s.ring) * Box<kHd>::kSlotBytes + kCWarps * kRows * kHd * 4 +
-           ((large ? kMaxBatch : 511) + 1) * 4;
+  s.ring = kHd == 64 ? (kRows == 8 ? 6 : 5) : (kRows == 8 ? 3 : 2);
+  s.smem = 1024 + static_cast<size_t>(kGroups) * (s.ring * Box<kHd>::kSlotBytes + kCWarps * kRows * kHd * 4);
+  static_assert((kMaxBatch + 1) * 4 <= kGroups * 2 * Box<kHd>::kSlotBytes, "the chunk sums fit the ring");
   int dev = 0;
   cudaGetDevice(&dev);
   std::lock_guard<std::mutex> lock(mu);
-  int& n = per_sm[large][dev & 63];
+  int& n = per_sm[dev & 63];
   if (n == 0) {
     auto k = rows_kernel<T, kHd, kRows>;
     if (opt_in_dynamic_smem(k) < static_cast<int>(s.smem) ||
@@ -588,8 +595,8 @@ int rows_of(const Sizes& z, int tokens) { return tokens * (z.nq / z.nkv) <= 8 ? 
 
 RowsShape rows_shape_of(const Sizes& z, int rows) {
 #define DK_SHAPE(TT) \
-  (z.hd == 128 ? (rows == 8 ? rows_shape<TT, 128, 8>(z.B) : rows_shape<TT, 128, 16>(z.B)) \
-               : (rows == 8 ? rows_shape<TT, 64, 8>(z.B) : rows_shape<TT, 64, 16>(z.B)))
+  (z.hd == 128 ? (rows == 8 ? rows_shape<TT, 128, 8>() : rows_shape<TT, 128, 16>()) \
+               : (rows == 8 ? rows_shape<TT, 64, 8>() : rows_shape<TT, 64, 16>()))
   return z.dtype == DK_F16 ? DK_SHAPE(__half) : DK_SHAPE(__nv_bfloat16);
 #undef DK_SHAPE
 }
@@ -635,7 +642,7 @@ void cut_pass(const Sizes& z, Cutter& c, Pass& a, bool always_partial) {
   } else {
     a.rows = rows_of(z, p.tile_tokens);
     a.shape = rows_shape_of(z, a.rows);
-    a.ctas = a.shape.ctas;
+    a.ctas = a.shape.ctas * kGroups;
     a.chunk = kChunk;
   }
   const int64_t tiles = p.mode == kRagged ? p.max_tiles : p.n_tiles;

@@ -139,6 +139,8 @@ struct Problem {
   int mode;
   int tile_tokens;
   int half_tokens;  // tokens of 128 rows (the tensor-core kernel); tile_tokens where a tile has at most 16 rows
+  int early, lead;  // the launch's first `early` pieces are `lead` chunks longer than the others (their CTAs start while
+                    // the kernel before still holds the other SMs)
   int unit_extra;   // chunks added to a unit's length on the line for what it costs besides its chunks
   int n_tiles;      // kOneToken, kPrefix; kRagged: the plan's
   // kRagged: plan[0] = tiles, plan[1] = length of one kv head's line, then cum[max_tiles + 1]; what tile_at needs of
@@ -239,6 +241,24 @@ __device__ __forceinline__ Line line_of(const Problem& p, int chunk) {
   return {p.plan + 2, 0, p.plan[0], p.plan[1]};
 }
 
+// How the line of a launch is cut into one piece for each CTA (or group of one).
+struct Cuts {
+  int64_t long_end, per_long, per;
+  int early;
+  __device__ Cuts(const Problem& p, const Line& line, int ctas) {
+    const int64_t all = static_cast<int64_t>(line.chunks) * p.nkv;
+    early = p.early;
+    const int64_t ahead = static_cast<int64_t>(early) * p.lead;
+    per = all > ahead ? (all - ahead + ctas - 1) / ctas : 0;
+    per_long = early == 0 ? 0 : per > 0 ? per + p.lead : (all + early - 1) / early;
+    long_end = early * per_long;
+  }
+  __device__ int64_t begin(int cta) const { return cta < early ? cta * per_long : long_end + (cta - early) * per; }
+  __device__ int owner(int64_t x) const {
+    return static_cast<int>(x < long_end ? x / per_long : early + (x - long_end) / per);
+  }
+};
+
 // A CTA's piece of the line, unit by unit. Whole warps walk it.
 template <int kChunk>
 struct Walk {
@@ -248,14 +268,15 @@ struct Walk {
   int next_h, next_t, next_c;
   // the current part: chunks c0 .. c1 of the unit (h, ti)
   int h, ti, c0, c1;
-  int64_t per, u0;  // length of a CTA's piece; where the unit begins
+  int64_t u0;  // where the unit begins
+  const Cuts cuts;
   Tile t, next_tile;  // (the next tile's fields are loaded a part ahead)
   int last;           // the tile's last position
-  __device__ Walk(const Problem& p_, const Line& line_, int cta, int ctas, int lane) : p(p_), line(line_) {
+  __device__ Walk(const Problem& p_, const Line& line_, int cta, int ctas, int lane)
+      : p(p_), line(line_), cuts(p_, line_, ctas) {
     const int64_t all = static_cast<int64_t>(line.chunks) * p.nkv;
-    per = (all + ctas - 1) / ctas;
-    x = min(cta * per, all);
-    x1 = min(x + per, all);
+    x = min(cuts.begin(cta), all);
+    x1 = min(cuts.begin(cta + 1), all);
     next_h = next_t = next_c = 0;
     if (x < x1) {
       next_h = static_cast<int>(x / line.chunks);
@@ -285,7 +306,7 @@ struct Walk {
   // Does the unit begin in this part and go on in other CTAs' pieces? Then what the join needs of it.
   __device__ bool cut(const Span<kChunk>& span) const { return c0 == 0 && c1 < span.n; }
   __device__ int4 cut_record(const Span<kChunk>& span) const {
-    return make_int4(t.t0, t.ntok, h, static_cast<int>((u0 + span.n - 1) / per));
+    return make_int4(t.t0, t.ntok, h, cuts.owner(u0 + span.n - 1));
   }
 };
 
@@ -296,8 +317,8 @@ struct Pieces {
 };
 
 // The unit's stretch of the line is u0 .. u1, `extra` of it at its end without chunks.
-__device__ __forceinline__ Pieces pieces_of(int64_t u0, int64_t u1, int extra, int64_t per, int ctas, int64_t unit) {
-  return {static_cast<int>(u0 / per), static_cast<int>((u1 - extra - 1) / per), 2ll * ctas + unit};
+__device__ __forceinline__ Pieces pieces_of(const Cuts& cuts, int64_t u0, int64_t u1, int extra, int ctas, int64_t unit) {
+  return {cuts.owner(u0), cuts.owner(u1 - extra - 1), 2ll * ctas + unit};
 }
 
 __device__ __forceinline__ int64_t piece_slot(const Pieces& w, int i) {
@@ -317,7 +338,7 @@ constexpr int kTcRows = 256;
 constexpr int kTcUnitExtra = 3;  // a unit's fixed cost (its Q, first and last steps, output) in chunks
 int tc_ctas(int64_t head_dim, int dtype);
 int tc_launch(const Problem& p, int64_t nq, int64_t head_dim, int dtype, int ctas, const void* k_pages,
-              const void* v_pages, cudaStream_t st);
+              const void* v_pages, int wait_late, cudaStream_t st);
 
 }  // namespace paged
 }  // namespace dk

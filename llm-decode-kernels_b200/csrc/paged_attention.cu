@@ -29,6 +29,7 @@ constexpr int kCWarps = 4;   // warps of a group
 constexpr int kThreads = kGroups * (kCWarps + 1) * 32;
 constexpr int kMaxRing = 6;
 constexpr int kPlanThreads = 1024;
+constexpr int kRowsUnitExtra = 1;  // a unit's fixed cost (q, joining the warps, output) in chunks
 
 // ------------------------------------------------------------------------------------ ragged plan
 // One CTA cuts the sequences into tiles of tile_tokens tokens and sums up their chunks.
@@ -177,7 +178,7 @@ __global__ void __launch_bounds__(kThreads)
     for (int b0 = 0; b0 < p.B; b0 += kThreads) {
       const int b = b0 + tid;
       int n = 0;
-      if (b < p.B) n = Span<kChunk>(p.lengths[b] - 1, p.lengths[b] - 1, p.mask, p.capacity).n;
+      if (b < p.B) n = Span<kChunk>(p.lengths[b] - 1, p.lengths[b] - 1, p.mask, p.capacity).n + p.unit_extra;
       int s = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -258,6 +259,7 @@ __global__ void __launch_bounds__(kThreads)
       const Span<kChunk> span = walk.step();
       const Tile t = walk.t;
       const int h = walk.h, c0 = walk.c0, c1 = walk.c1, plast = walk.last;
+      if (c1 <= c0) continue;
       const int rows = t.ntok * p.G;
       // this lane's rows g and g + 8: positions, and q as the MMA's A operand
       int pos[kR];
@@ -530,18 +532,16 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
   const Line own = line_of(b, 1);
   const int ti = b.mode == kRagged ? find_tile_warp([&](int i) { return b.tile_info[i].x; }, own.tiles, t, lane) : t;
   const int t0 = b.mode == kRagged ? b.tile_info[ti].x : t;
-  const int64_t b_all = static_cast<int64_t>(own.chunks) * b.nkv, b_per = max((b_all + b_ctas - 1) / b_ctas, int64_t{1});
   const int64_t b0 = static_cast<int64_t>(h) * own.chunks + own.cum(ti), b1 = static_cast<int64_t>(h) * own.chunks + own.cum(ti + 1);
 
   const Line line = line_of(a, a_chunk);
   const int unit = h * a.n_tiles + t / a.tile_tokens;
-  const int64_t a_all = static_cast<int64_t>(line.chunks) * a.nkv, a_per = (a_all + a_ctas - 1) / a_ctas;
   const int64_t a0 = static_cast<int64_t>(unit) * line.per_tile;
   Joined<kD, 1> sum;
   const int a_row[1] = {result_row(a, t % a.tile_tokens, g)}, b_row[1] = {result_row(b, t - t0, g)};
-  sum.template add<8>(a, pieces_of(a0, a0 + line.per_tile, a.unit_extra, a_per, a_ctas, unit), a_rows, a_row, lane);
+  sum.template add<8>(a, pieces_of(Cuts(a, line, a_ctas), a0, a0 + line.per_tile, a.unit_extra, a_ctas, unit), a_rows, a_row, lane);
   if (own.chunks > 0)
-    sum.template add<2>(b, pieces_of(b0, b1, b.unit_extra, b_per, b_ctas, h * own.tiles + ti), b_rows, b_row, lane);
+    sum.template add<2>(b, pieces_of(Cuts(b, own, b_ctas), b0, b1, b.unit_extra, b_ctas, h * own.tiles + ti), b_rows, b_row, lane);
   store_row<T, kD>(b, t, head, lane, sum.l[0], sum.acc[0]);
 }
 
@@ -643,6 +643,7 @@ void cut_pass(const Sizes& z, Cutter& c, Pass& a, bool always_partial) {
     a.rows = rows_of(z, p.tile_tokens);
     a.shape = rows_shape_of(z, a.rows);
     a.ctas = a.shape.ctas * kGroups;
+    p.unit_extra = kRowsUnitExtra;
     a.chunk = kChunk;
   }
   const int64_t tiles = p.mode == kRagged ? p.max_tiles : p.n_tiles;
@@ -678,6 +679,19 @@ void shape_prefix(const Sizes& z, Pass& a) {
   set_tile(z, a, std::max(1, 16 / G));
   a.p.n_tiles = static_cast<int>((z.T + a.p.tile_tokens - 1) / a.p.tile_tokens);
   a.p.prefix_len = static_cast<int>(z.prefix_len);
+}
+
+// The two launches of a call with a prefix run side by side: the prefix's takes most of the SMs, and the own positions'
+// starts on the others right away, with longer pieces there. How long the prefix's takes is known here: a chunk of 256 rows
+// takes about 2 us and a CTA 8 us besides; a chunk of the own positions takes a group about 2 us.
+void share_gpu(Pass& pre, Pass& own) {
+  if (!pre.tc || own.tc || !pdl_enabled()) return;
+  const int sms = device_info().num_sms;
+  const int64_t n = static_cast<int64_t>((pre.p.prefix_len + kTcChunk - 1) / kTcChunk + pre.p.unit_extra) * pre.p.n_tiles * pre.p.nkv;
+  const int64_t most = sms * 7 / 8, per = (n + most - 1) / most;
+  pre.ctas = static_cast<int>((n + per - 1) / per);
+  own.p.early = kGroups * (sms - pre.ctas);
+  own.p.lead = static_cast<int>(4 + per);
 }
 
 int check_sizes(const char* what, const Sizes& z) {
@@ -772,6 +786,7 @@ int attention(const char* what, const dk_paged_attention_args* args, bool prefix
                      (unsigned long long)a.workspace_bytes, (unsigned long long)c.used);
   if (own.ctas == 0 || (z.prefix_len > 0 && pre.ctas == 0))
     return set_error(DK_ERR_UNSUPPORTED, "%s: the kernel's shared memory does not fit this device", what);
+  const int beside = z.prefix_len > 0 && pdl_enabled() ? 1 : 0;
   for (Problem* p : {&own.p, &pre.p}) {
     p->q = a.q, p->ldq = a.ldq, p->out = a.out;
     p->table = a.page_table, p->ld_table = a.ld_table, p->lengths = a.lengths, p->starts = a.starts;
@@ -785,6 +800,7 @@ int attention(const char* what, const dk_paged_attention_args* args, bool prefix
     p->err = device_info().err_word;
   }
   pre.p.table = a.prefix_table, pre.p.capacity = static_cast<int>(z.prefix_len), pre.p.mask = Mask{0, 0};
+  if (z.prefix_len > 0) share_gpu(pre, own);
 
   cudaStream_t st = reinterpret_cast<cudaStream_t>(a.stream);
   const uint64_t rows = static_cast<uint64_t>(n_pages * z.nkv * page_size);
@@ -802,9 +818,9 @@ int attention(const char* what, const dk_paged_attention_args* args, bool prefix
   for (const Pass* s : {&pre, &own}) {
     if (s->ctas == 0 || e != cudaSuccess) continue;
     if (s->tc) {
-      if (const int rc = tc_launch(s->p, z.nq, z.hd, z.dtype, s->ctas, a.k_pages, a.v_pages, st)) return rc;
+      if (const int rc = tc_launch(s->p, z.nq, z.hd, z.dtype, s->ctas, a.k_pages, a.v_pages, s == &own ? beside : 0, st)) return rc;
     } else {
-      e = launch_rows(z, s->rows, s->shape, st, mk, mv, s->p, 0);
+      e = launch_rows(z, s->rows, s->shape, st, mk, mv, s->p, s == &own ? beside : 0);
     }
   }
   const Pass* with = z.prefix_len > 0 ? &pre : nullptr;

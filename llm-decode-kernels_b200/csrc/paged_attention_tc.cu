@@ -162,7 +162,7 @@ __device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* m
 template <typename T, int kHd>
 __global__ void __launch_bounds__(kThreads, 1)
     tiles_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
-                 const __grid_constant__ CUtensorMap mv, const Problem p) {
+                 const __grid_constant__ CUtensorMap mv, const Problem p, int wait_late) {
   using L = Smem<kHd>;
   using E = Elem<T>;
   constexpr uint32_t kS[2] = {0, 128}, kO[2] = {256, 256 + kHd};  // tensor-memory columns; P(X) lies over S(X)
@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem = tmem_slot;
-  pdl_wait();
+  if (!wait_late) pdl_wait();
   pdl_trigger();
 
   const Line line = line_of(p, kC);
@@ -497,6 +497,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   tc::fence_after_sync();
   if (warp == kMmaWarp) tc::tmem_dealloc(tmem, 512);
+  if (wait_late) pdl_wait();
 }
 
 bool make_q_map(CUtensorMap* map, const Problem& p, int64_t nq, int64_t hd, CUtensorMapDataType type) {
@@ -530,7 +531,7 @@ int tc_ctas(int64_t head_dim, int dtype) {
 }
 
 int tc_launch(const Problem& p, int64_t nq, int64_t hd, int dtype, int ctas, const void* k_pages, const void* v_pages,
-              cudaStream_t st) {
+              int wait_late, cudaStream_t st) {
   const CUtensorMapDataType type = dtype == DK_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   const uint64_t rows = static_cast<uint64_t>(p.n_pages) * p.nkv * p.page_size;
   const uint32_t box = static_cast<uint32_t>(p.page_size < kC ? p.page_size : kC);
@@ -541,7 +542,7 @@ int tc_launch(const Problem& p, int64_t nq, int64_t hd, int dtype, int ctas, con
     return DK_ERR_CUDA;
   cudaError_t e;
 #define DK_TILES(TT, HH) \
-  launch(tiles_kernel<TT, HH>, dim3(ctas), dim3(kThreads), Smem<HH>::kBytes, st, pdl_enabled(), dim3(1, 1, 1), mq, mk, mv, p)
+  launch(tiles_kernel<TT, HH>, dim3(ctas), dim3(kThreads), Smem<HH>::kBytes, st, pdl_enabled(), dim3(1, 1, 1), mq, mk, mv, p, wait_late)
   if (dtype == DK_F16)
     e = hd == 128 ? DK_TILES(__half, 128) : DK_TILES(__half, 64);
   else

@@ -29,7 +29,7 @@ constexpr int kCWarps = 4;   // warps of a group
 constexpr int kThreads = kGroups * (kCWarps + 1) * 32;
 constexpr int kMaxRing = 6;
 constexpr int kPlanThreads = 1024;
-constexpr int kRowsUnitExtra = 1;  // a unit's fixed cost (q, joining the warps, output) in chunks
+constexpr int kRowsUnitExtra = 2;  // a unit's fixed cost (q, joining the warps, output) in chunks
 
 // ------------------------------------------------------------------------------------ ragged plan
 // One CTA cuts the sequences into tiles of tile_tokens tokens and sums up their chunks.
@@ -682,8 +682,8 @@ void shape_prefix(const Sizes& z, Pass& a) {
 }
 
 // The two launches of a call with a prefix run side by side: the prefix's takes most of the SMs, and the own positions'
-// starts on the others right away, with longer pieces there. How long the prefix's takes is known here: a chunk of 256 rows
-// takes about 2 us and a CTA 8 us besides; a chunk of the own positions takes a group about 2 us.
+// starts on the others right away, with longer pieces there. How long the prefix's takes is known here: about 6 us and 2 us
+// for each chunk of a CTA's piece; a group of the other takes 1.1 us for a chunk.
 void share_gpu(Pass& pre, Pass& own) {
   if (!pre.tc || own.tc || !pdl_enabled()) return;
   const int sms = device_info().num_sms;
@@ -691,7 +691,7 @@ void share_gpu(Pass& pre, Pass& own) {
   const int64_t most = sms * 7 / 8, per = (n + most - 1) / most;
   pre.ctas = static_cast<int>((n + per - 1) / per);
   own.p.early = kGroups * (sms - pre.ctas);
-  own.p.lead = static_cast<int>(4 + per);
+  own.p.lead = static_cast<int>((60 + 20 * per) / 11);
 }
 
 int check_sizes(const char* what, const Sizes& z) {

@@ -151,9 +151,10 @@ struct Problem {
   int32_t* cum_out;  // kOneToken: [B + 1], the chunks of one kv head before each sequence
   // Partial results: a CTA's first piece of a unit that began before it (slot 2 * CTA), its last piece of a unit that
   // goes on after it (slot 2 * CTA + 1), and with always_partial a slot for each uncut unit after those
-  float* part_o;   // [slots][tile rows][head_dim]
+  float* part_o;   // [slots][tile rows][head_dim], or with rows_inner [slots][head_dim / 4][tile rows][4]
   float* part_ml;  // [slots][tile rows][2]: row maximum (base 2), row sum
   int4* cut;           // [CTAs] the unit whose chunks a CTA begins but does not end: {first token, tokens, kv head, last CTA}
+  int rows_inner;
   int always_partial;  // no unit writes its output itself
   int* err;
 };

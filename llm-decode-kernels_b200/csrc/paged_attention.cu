@@ -428,121 +428,95 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // ------------------------------------------------------------------------------------ join
-// Running result of kRows rows: kD dims per lane of a warp.
-template <int kD, int kRows>
+// A block joins 8 result rows: a lane has row lane % 8 and, of each 16 dims of its warp, the four lane / 8 * 4 ...: in
+// either layout of the partial results a warp's load touches few lines.
+constexpr int kJoinRows = 8;
+
+template <typename T, int kHd>
 struct Joined {
-  float m[kRows], l[kRows], acc[kRows][kD];
-  __device__ Joined() {
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      m[r] = -INFINITY, l[r] = 0.f;
-#pragma unroll
-      for (int d = 0; d < kD; ++d) acc[r][d] = 0.f;
-    }
-  }
-  // Adds one unit's pieces in order, kAhead of them loaded at a time.
+  float m = -INFINITY, l = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  // Adds the pieces of this lane's unit in order, kAhead of them loaded at a time; row < 0: none. d4: the lane's dims / 4.
   template <int kAhead>
-  __device__ void add(const Problem& p, const Pieces& w, int tile_rows, const int (&row)[kRows], int lane) {
+  __device__ void add(const Problem& p, const Pieces& w, int tile_rows, int row, int d4) {
+    if (row < 0) return;
+    const int64_t at = p.rows_inner ? static_cast<int64_t>(d4) * tile_rows + row : static_cast<int64_t>(row) * (kHd / 4) + d4;
     for (int i0 = w.first; i0 <= w.last; i0 += kAhead) {
-      float2 ml[kAhead][kRows];
-      float o[kAhead][kRows][kD];
-#pragma unroll
-      for (int a = 0; a < kAhead; ++a)
-#pragma unroll
-        for (int r = 0; r < kRows; ++r) {
-          ml[a][r] = make_float2(-INFINITY, 0.f);
-          if (i0 + a > w.last) continue;
-          const int64_t at = piece_slot(w, i0 + a) * tile_rows + row[r];
-          ml[a][r] = *reinterpret_cast<const float2*>(&p.part_ml[at * 2]);
-          const float* src = &p.part_o[at * (kD * 32) + lane * kD];
-          if constexpr (kD == 4)
-            *reinterpret_cast<float4*>(o[a][r]) = *reinterpret_cast<const float4*>(src);
-          else
-            *reinterpret_cast<float2*>(o[a][r]) = *reinterpret_cast<const float2*>(src);
-        }
+      float2 ml[kAhead];
+      float4 o[kAhead];
 #pragma unroll
       for (int a = 0; a < kAhead; ++a) {
         if (i0 + a > w.last) break;
+        const int64_t slot = piece_slot(w, i0 + a);
+        ml[a] = *reinterpret_cast<const float2*>(&p.part_ml[(slot * tile_rows + row) * 2]);
+        o[a] = reinterpret_cast<const float4*>(p.part_o)[slot * tile_rows * (kHd / 4) + at];
+      }
 #pragma unroll
-        for (int r = 0; r < kRows; ++r) {
-          const float mx = fmaxf(m[r], ml[a][r].x), use = mx == -INFINITY ? 0.f : mx;
-          const float keep = exp2_approx(m[r] - use), take = exp2_approx(ml[a][r].x - use);
-          m[r] = mx;
-          l[r] = fmaf(l[r], keep, ml[a][r].y * take);
-#pragma unroll
-          for (int d = 0; d < kD; ++d) acc[r][d] = fmaf(acc[r][d], keep, o[a][r][d] * take);
-        }
+      for (int a = 0; a < kAhead; ++a) {
+        if (i0 + a > w.last) break;
+        const float mx = fmaxf(m, ml[a].x), use = mx == -INFINITY ? 0.f : mx;
+        const float keep = exp2_approx(m - use), take = exp2_approx(ml[a].x - use);
+        m = mx;
+        l = fmaf(l, keep, ml[a].y * take);
+        acc.x = fmaf(acc.x, keep, o[a].x * take), acc.y = fmaf(acc.y, keep, o[a].y * take);
+        acc.z = fmaf(acc.z, keep, o[a].z * take), acc.w = fmaf(acc.w, keep, o[a].w * take);
       }
     }
   }
+  // `out`: this lane's row, or null.
+  __device__ void store(T* out, int d4) const {
+    if (out == nullptr) return;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    *reinterpret_cast<uint2*>(out + 4 * d4) = make_uint2(Elem<T>::pack(acc.x * inv, acc.y * inv), Elem<T>::pack(acc.z * inv, acc.w * inv));
+  }
 };
 
-template <typename T, int kD>
-__device__ __forceinline__ void store_row(const Problem& p, int t, int head, int lane, float l, const float (&acc)[kD]) {
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  T* dst = static_cast<T*>(p.out) + (static_cast<int64_t>(t) * p.nkv * p.G + head) * (kD * 32) + lane * kD;
-  if constexpr (kD == 4)
-    *reinterpret_cast<uint2*>(dst) =
-        make_uint2(Elem<T>::pack(acc[0] * inv, acc[1] * inv), Elem<T>::pack(acc[2] * inv, acc[3] * inv));
-  else
-    *reinterpret_cast<uint32_t*>(dst) = Elem<T>::pack(acc[0] * inv, acc[1] * inv);
+template <typename T, int kHd>
+__device__ __forceinline__ T* out_row(const Problem& p, int t, int head) {
+  return static_cast<T*>(p.out) + (static_cast<int64_t>(t) * p.nkv * p.G + head) * kHd;
 }
 
-constexpr int kJoinWarps = 8;
-
-// Joins the units that a piece's end cuts. Block (i, y): kRows rows a warp of the unit that CTA i began, if there is one.
-template <typename T, int kHd, int kRows>
-__global__ void __launch_bounds__(kJoinWarps * 32) join_split_kernel(const Problem p, int ctas, int tile_rows) {
-  constexpr int kD = kHd / 32;
+// Joins the units that a piece's end cuts. Block (i, y): 8 rows of the unit that CTA i began, if there is one.
+// kAhead: 4 for the one-token launch's 8-row units, 2 for the tiles' 256 (fewer pieces, more blocks: 4 costs 3 us there).
+template <typename T, int kHd, int kAhead>
+__global__ void __launch_bounds__(kHd * 2) join_split_kernel(const Problem p, int tile_rows) {
   pdl_trigger();
   pdl_wait();
   const int4 c = p.cut[blockIdx.x];  // {first token, tokens, kv head, last CTA}
-  const int rows = c.y * p.G, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int i0 = (blockIdx.y * kJoinWarps + warp) * kRows;
-  if (i0 >= rows) return;
-  const Pieces w = {static_cast<int>(blockIdx.x), c.w, 0};
-  int row[kRows];
-#pragma unroll
-  for (int r = 0; r < kRows; ++r) {
-    const int i = min(i0 + r, rows - 1);
-    row[r] = result_row(p, i / p.G, i % p.G);
-  }
-  Joined<kD, kRows> sum;
-  sum.template add<8 / kRows>(p, w, tile_rows, row, lane);
-#pragma unroll
-  for (int r = 0; r < kRows; ++r) {
-    const int i = i0 + r;
-    if (i < rows) store_row<T, kD>(p, c.x + i / p.G, c.z * p.G + i % p.G, lane, sum.l[r], sum.acc[r]);
-  }
+  const int rows = c.y * p.G, i = blockIdx.y * kJoinRows + threadIdx.x % kJoinRows, d4 = threadIdx.x / kJoinRows;
+  if (i >= rows) return;
+  Joined<T, kHd> sum;
+  sum.template add<kAhead>(p, {static_cast<int>(blockIdx.x), c.w, 0}, tile_rows, result_row(p, i / p.G, i % p.G), d4);
+  sum.store(out_row<T, kHd>(p, c.x + i / p.G, c.z * p.G + i % p.G), d4);
 }
 
-// Joins the prefix's results (`a`) with those of the sequences' own positions (`b`): a warp per (token, head).
+// Joins the prefix's results (`a`) with those of the sequences' own positions (`b`). Block (x, h): 8 rows (token, head of
+// kv head h).
 template <typename T, int kHd>
-__global__ void __launch_bounds__(kJoinWarps * 32)
+__global__ void __launch_bounds__(kHd * 2)
     join_prefix_kernel(const Problem a, int a_ctas, int a_rows, int a_chunk, const Problem b, int b_ctas, int b_rows) {
-  constexpr int kD = kHd / 32;
   pdl_trigger();
   pdl_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t rows = static_cast<int64_t>(a.T) * a.nkv * a.G;
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * kJoinWarps + warp;
-  if (id >= rows) return;
-  const int t = static_cast<int>(id / (a.nkv * a.G)), head = static_cast<int>(id % (a.nkv * a.G));
-  const int h = head / a.G, g = head % a.G;
-  const Line own = line_of(b, 1);
-  const int ti = b.mode == kRagged ? find_tile_warp([&](int i) { return b.tile_info[i].x; }, own.tiles, t, lane) : t;
-  const int t0 = b.mode == kRagged ? b.tile_info[ti].x : t;
-  const int64_t b0 = static_cast<int64_t>(h) * own.chunks + own.cum(ti), b1 = static_cast<int64_t>(h) * own.chunks + own.cum(ti + 1);
-
-  const Line line = line_of(a, a_chunk);
-  const int unit = h * a.n_tiles + t / a.tile_tokens;
-  const int64_t a0 = static_cast<int64_t>(unit) * line.per_tile;
-  Joined<kD, 1> sum;
-  const int a_row[1] = {result_row(a, t % a.tile_tokens, g)}, b_row[1] = {result_row(b, t - t0, g)};
-  sum.template add<8>(a, pieces_of(Cuts(a, line, a_ctas), a0, a0 + line.per_tile, a.unit_extra, a_ctas, unit), a_rows, a_row, lane);
-  if (own.chunks > 0)
-    sum.template add<2>(b, pieces_of(Cuts(b, own, b_ctas), b0, b1, b.unit_extra, b_ctas, h * own.tiles + ti), b_rows, b_row, lane);
-  store_row<T, kD>(b, t, head, lane, sum.l[0], sum.acc[0]);
+  const int d4 = threadIdx.x / kJoinRows, h = blockIdx.y;
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * kJoinRows + threadIdx.x % kJoinRows;
+  if (id >= static_cast<int64_t>(a.T) * a.G) return;
+  const int t = static_cast<int>(id / a.G), g = static_cast<int>(id % a.G);
+  const Line own = line_of(b, 1), line = line_of(a, a_chunk);
+  Joined<T, kHd> sum;
+  {
+    const int unit = h * a.n_tiles + t / a.tile_tokens;
+    const int64_t u0 = static_cast<int64_t>(unit) * line.per_tile;
+    sum.template add<8>(a, pieces_of(Cuts(a, line, a_ctas), u0, u0 + line.per_tile, a.unit_extra, a_ctas, unit), a_rows,
+                        result_row(a, t % a.tile_tokens, g), d4);
+  }
+  if (own.chunks > 0) {
+    const int ti = b.mode == kRagged ? find_tile([&](int i) { return b.tile_info[i].x; }, own.tiles, t) : t;
+    const int t0 = b.mode == kRagged ? b.tile_info[ti].x : t;
+    const int64_t u0 = static_cast<int64_t>(h) * own.chunks + own.cum(ti), u1 = static_cast<int64_t>(h) * own.chunks + own.cum(ti + 1);
+    sum.template add<2>(b, pieces_of(Cuts(b, own, b_ctas), u0, u1, b.unit_extra, b_ctas, h * own.tiles + ti), b_rows,
+                        result_row(b, t - t0, g), d4);
+  }
+  sum.store(out_row<T, kHd>(b, t, h * b.G + g), d4);
 }
 
 }  // namespace
@@ -637,6 +611,7 @@ void cut_pass(const Sizes& z, Cutter& c, Pass& a, bool always_partial) {
   if (a.tc) {
     a.rows = kTcRows;
     p.unit_extra = kTcUnitExtra;
+    p.rows_inner = 1;
     a.ctas = tc_ctas(z.hd, z.dtype);
     a.chunk = kTcChunk;
   } else {
@@ -713,13 +688,11 @@ int check_sizes(const char* what, const Sizes& z) {
 template <typename T, int kHd>
 cudaError_t launch_join(const Sizes& z, cudaStream_t st, const Pass* prefix, const Pass& own) {
   if (prefix == nullptr) {
-    const int rows = own.tc ? 4 : 1;
-    const dim3 grid(static_cast<unsigned>(own.ctas), static_cast<unsigned>((own.rows + kJoinWarps * rows - 1) / (kJoinWarps * rows)));
-    return launch(own.tc ? join_split_kernel<T, kHd, 4> : join_split_kernel<T, kHd, 1>, grid, dim3(kJoinWarps * 32), 0, st,
-                  pdl_enabled(), dim3(1, 1, 1), own.p, own.ctas, own.rows);
+    const dim3 grid(static_cast<unsigned>(own.ctas), static_cast<unsigned>((own.rows + kJoinRows - 1) / kJoinRows));
+    return launch(own.tc ? join_split_kernel<T, kHd, 2> : join_split_kernel<T, kHd, 4>, grid, dim3(kHd * 2), 0, st, pdl_enabled(), dim3(1, 1, 1), own.p, own.rows);
   }
-  const dim3 grid(static_cast<unsigned>((z.T * z.nq + kJoinWarps - 1) / kJoinWarps));
-  return launch(join_prefix_kernel<T, kHd>, grid, dim3(kJoinWarps * 32), 0, st, pdl_enabled(), dim3(1, 1, 1), prefix->p,
+  const dim3 grid(static_cast<unsigned>((z.T * (z.nq / z.nkv) + kJoinRows - 1) / kJoinRows), static_cast<unsigned>(z.nkv));
+  return launch(join_prefix_kernel<T, kHd>, grid, dim3(kHd * 2), 0, st, pdl_enabled(), dim3(1, 1, 1), prefix->p,
                 prefix->ctas, prefix->rows, prefix->chunk, own.p, own.ctas, own.rows);
 }
 

@@ -144,6 +144,26 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return from_bits2(d);
 }
 
+// Of four lanes' four 16-byte pieces each: lane l of the four gets piece l of all of them.
+__device__ __forceinline__ void exchange(uint4& a, uint4& b, bool upper, int with) {
+  const uint4 send = upper ? a : b;
+  uint4 got;
+  got.x = __shfl_xor_sync(0xffffffffu, send.x, with);
+  got.y = __shfl_xor_sync(0xffffffffu, send.y, with);
+  got.z = __shfl_xor_sync(0xffffffffu, send.z, with);
+  got.w = __shfl_xor_sync(0xffffffffu, send.w, with);
+  if (upper)
+    a = got;
+  else
+    b = got;
+}
+__device__ __forceinline__ void transpose4(uint4 (&w)[4], int lane) {
+  exchange(w[0], w[1], lane & 1, 1);
+  exchange(w[2], w[3], lane & 1, 1);
+  exchange(w[0], w[2], lane & 2, 2);
+  exchange(w[1], w[3], lane & 2, 2);
+}
+
 __device__ __forceinline__ float row_max(const float (&s)[kC]) {
   float m4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
@@ -453,25 +473,49 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int64_t slot = partial_slot(gridDim.x, blockIdx.x, walk.c0 == 0, all_of_it, walk.h * line.tiles + walk.ti);
       if (tid == 0 && walk.cut(span)) p.cut[blockIdx.x] = walk.cut_record(span);
       const int row = x * 128 + r;
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      T* out = static_cast<T*>(p.out) + (static_cast<int64_t>(t.t0 + tok) * p.nkv * p.G + head) * kHd;
-      float* part = p.part_o + (slot * kTcRows + row) * kHd;
+      if (whole) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        // Four lanes exchange 16-byte pieces so that together they store 64 bytes of one row at a time: a lane storing its
+        // own row would touch 32 lines with every instruction.
+        T* out = static_cast<T*>(p.out) + (static_cast<int64_t>(t.t0 + tok) * p.nkv * p.G + head) * kHd;
+        T* row_out[4];
+        bool row_live[4];
 #pragma unroll
-      for (int c = 0; c < kHd; c += 64) {
-        float o[64];
-        tmem_ld64(o_col + c, o);
-        if (live && whole) {
+        for (int k = 0; k < 4; ++k) {
+          row_out[k] = reinterpret_cast<T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(out), (lane & ~3) + k));
+          row_live[k] = __shfl_sync(0xffffffffu, static_cast<int>(live), (lane & ~3) + k) != 0;
+        }
 #pragma unroll
-          for (int d = 0; d < 64; d += 8)
-            *reinterpret_cast<uint4*>(out + c + d) =
-                make_uint4(E::pack(o[d] * inv, o[d + 1] * inv), E::pack(o[d + 2] * inv, o[d + 3] * inv),
-                           E::pack(o[d + 4] * inv, o[d + 5] * inv), E::pack(o[d + 6] * inv, o[d + 7] * inv));
-        } else if (live) {
+        for (int c = 0; c < kHd; c += 64) {
+          float o[64];
+          tmem_ld64(o_col + c, o);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            uint4 w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float* v = &o[32 * half + 8 * k];
+              w[k] = make_uint4(E::pack(v[0] * inv, v[1] * inv), E::pack(v[2] * inv, v[3] * inv),
+                                E::pack(v[4] * inv, v[5] * inv), E::pack(v[6] * inv, v[7] * inv));
+            }
+            transpose4(w, lane);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (row_live[k]) *reinterpret_cast<uint4*>(row_out[k] + c + 32 * half + 8 * (lane & 3)) = w[k];
+          }
+        }
+      } else {
+        // Partial results lie with the rows innermost, [dims / 4][256 rows][4]: a warp stores 512 contiguous bytes.
+        float* part = p.part_o + slot * kTcRows * kHd + row * 4;
+#pragma unroll
+        for (int c = 0; c < kHd; c += 64) {
+          float o[64];
+          tmem_ld64(o_col + c, o);
 #pragma unroll
           for (int d = 0; d < 64; d += 4)
-            *reinterpret_cast<float4*>(part + c + d) = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
+            if (live) *reinterpret_cast<float4*>(part + static_cast<int64_t>(c + d) * kTcRows) = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
+          __syncwarp();
         }
-        __syncwarp();
       }
       if (!whole && live) *reinterpret_cast<float2*>(&p.part_ml[(slot * kTcRows + row) * 2]) = make_float2(m, l);
       tc::fence_before_sync();

@@ -243,21 +243,19 @@ __device__ __forceinline__ Line line_of(const Problem& p, int chunk) {
 }
 
 // How the line of a launch is cut into one piece for each CTA (or group of one).
+// (A launch's line is shorter than 2^31: checked on the host. 64-bit divisions took a microsecond of these kernels' starts.)
 struct Cuts {
-  int64_t long_end, per_long, per;
-  int early;
+  int long_end, per_long, per, early;
   __device__ Cuts(const Problem& p, const Line& line, int ctas) {
-    const int64_t all = static_cast<int64_t>(line.chunks) * p.nkv;
+    const int all = line.chunks * p.nkv;
     early = p.early;
-    const int64_t ahead = static_cast<int64_t>(early) * p.lead;
+    const int ahead = early * p.lead;
     per = all > ahead ? (all - ahead + ctas - 1) / ctas : 0;
     per_long = early == 0 ? 0 : per > 0 ? per + p.lead : (all + early - 1) / early;
     long_end = early * per_long;
   }
-  __device__ int64_t begin(int cta) const { return cta < early ? cta * per_long : long_end + (cta - early) * per; }
-  __device__ int owner(int64_t x) const {
-    return static_cast<int>(x < long_end ? x / per_long : early + (x - long_end) / per);
-  }
+  __device__ int begin(int cta) const { return cta < early ? cta * per_long : long_end + (cta - early) * per; }
+  __device__ int owner(int x) const { return x < long_end ? x / per_long : early + (x - long_end) / per; }
 };
 
 // A CTA's piece of the line, unit by unit. Whole warps walk it.
@@ -265,23 +263,23 @@ template <int kChunk>
 struct Walk {
   const Problem& p;
   const Line& line;
-  int64_t x, x1;
+  int x, x1;
   int next_h, next_t, next_c;
   // the current part: chunks c0 .. c1 of the unit (h, ti)
   int h, ti, c0, c1;
-  int64_t u0;  // where the unit begins
+  int u0;  // where the unit begins
   const Cuts cuts;
   Tile t, next_tile;  // (the next tile's fields are loaded a part ahead)
   int last;           // the tile's last position
   __device__ Walk(const Problem& p_, const Line& line_, int cta, int ctas, int lane)
       : p(p_), line(line_), cuts(p_, line_, ctas) {
-    const int64_t all = static_cast<int64_t>(line.chunks) * p.nkv;
+    const int all = line.chunks * p.nkv;
     x = min(cuts.begin(cta), all);
     x1 = min(cuts.begin(cta + 1), all);
     next_h = next_t = next_c = 0;
     if (x < x1) {
-      next_h = static_cast<int>(x / line.chunks);
-      const int r = static_cast<int>(x - static_cast<int64_t>(next_h) * line.chunks);
+      next_h = x / line.chunks;
+      const int r = x - next_h * line.chunks;
       next_t = find_tile_warp([&](int i) { return line.cum(i); }, line.tiles, r, lane);
       next_c = r - line.cum(next_t);
       next_tile = tile_at(p, next_t);
@@ -296,7 +294,7 @@ struct Walk {
     t = next_tile;
     last = tile_last(p, t);
     const Span<kChunk> span(t.p0, last, p.mask, p.capacity);
-    const int to = static_cast<int>(min(static_cast<int64_t>(span.n + p.unit_extra), c0 + (x1 - x)));
+    const int to = min(span.n + p.unit_extra, c0 + (x1 - x));
     x += to - c0;
     c1 = min(to, span.n);
     next_c = 0;
@@ -318,7 +316,7 @@ struct Pieces {
 };
 
 // The unit's stretch of the line is u0 .. u1, `extra` of it at its end without chunks.
-__device__ __forceinline__ Pieces pieces_of(const Cuts& cuts, int64_t u0, int64_t u1, int extra, int ctas, int64_t unit) {
+__device__ __forceinline__ Pieces pieces_of(const Cuts& cuts, int u0, int u1, int extra, int ctas, int64_t unit) {
   return {cuts.owner(u0), cuts.owner(u1 - extra - 1), 2ll * ctas + unit};
 }
 

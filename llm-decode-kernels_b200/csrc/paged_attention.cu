@@ -500,22 +500,18 @@ __global__ void __launch_bounds__(kHd * 2)
   const int d4 = threadIdx.x / kJoinRows, h = blockIdx.y;
   const int64_t id = static_cast<int64_t>(blockIdx.x) * kJoinRows + threadIdx.x % kJoinRows;
   if (id >= static_cast<int64_t>(a.T) * a.G) return;
-  const int t = static_cast<int>(id / a.G), g = static_cast<int>(id % a.G);
+  const int t = static_cast<int>(id) / a.G, g = static_cast<int>(id) % a.G;
   const Line own = line_of(b, 1), line = line_of(a, a_chunk);
+  const int ti = b.mode == kRagged ? find_tile([&](int i) { return b.tile_info[i].x; }, own.tiles, t) : t;
+  const int t0 = b.mode == kRagged ? b.tile_info[ti].x : t;
+  const int b0 = h * own.chunks + own.cum(ti), b1 = h * own.chunks + own.cum(ti + 1);
   Joined<T, kHd> sum;
-  {
-    const int unit = h * a.n_tiles + t / a.tile_tokens;
-    const int64_t u0 = static_cast<int64_t>(unit) * line.per_tile;
-    sum.template add<8>(a, pieces_of(Cuts(a, line, a_ctas), u0, u0 + line.per_tile, a.unit_extra, a_ctas, unit), a_rows,
-                        result_row(a, t % a.tile_tokens, g), d4);
-  }
-  if (own.chunks > 0) {
-    const int ti = b.mode == kRagged ? find_tile([&](int i) { return b.tile_info[i].x; }, own.tiles, t) : t;
-    const int t0 = b.mode == kRagged ? b.tile_info[ti].x : t;
-    const int64_t u0 = static_cast<int64_t>(h) * own.chunks + own.cum(ti), u1 = static_cast<int64_t>(h) * own.chunks + own.cum(ti + 1);
-    sum.template add<2>(b, pieces_of(Cuts(b, own, b_ctas), u0, u1, b.unit_extra, b_ctas, h * own.tiles + ti), b_rows,
+  const int unit = h * a.n_tiles + t / a.tile_tokens, a0 = unit * line.per_tile;
+  sum.template add<8>(a, pieces_of(Cuts(a, line, a_ctas), a0, a0 + line.per_tile, a.unit_extra, a_ctas, unit), a_rows,
+                      result_row(a, t % a.tile_tokens, g), d4);
+  if (own.chunks > 0)
+    sum.template add<2>(b, pieces_of(Cuts(b, own, b_ctas), b0, b1, b.unit_extra, b_ctas, h * own.tiles + ti), b_rows,
                         result_row(b, t - t0, g), d4);
-  }
   sum.store(out_row<T, kHd>(b, t, h * b.G + g), d4);
 }
 
@@ -753,6 +749,14 @@ int attention(const char* what, const dk_paged_attention_args* args, bool prefix
   if (z.prefix_len > 0) {
     shape_prefix(z, pre);
     cut_pass(z, c, pre, true);
+  }
+  for (const Pass* s : {&pre, &own}) {
+    if (s->chunk == 0) continue;
+    const int64_t tiles = s->p.mode == kRagged ? s->p.max_tiles : s->p.n_tiles;
+    const int64_t positions = s->p.mode == kPrefix ? z.prefix_len : table_width * page_size;
+    if (tiles * ((positions + s->chunk - 1) / s->chunk + 1 + s->p.unit_extra) * z.nkv >= (int64_t(1) << 30))
+      return set_error(DK_ERR_UNSUPPORTED, "%s: the call's work counts more than 2^30 chunks: fewer sequences or narrower page tables",
+                       what);
   }
   if (c.used > a.workspace_bytes)
     return set_error(DK_ERR_INVALID, "%s: the workspace has %llu bytes, %llu are needed", what,

@@ -5,9 +5,12 @@
 // q' goes to q_out, k' and v to row p % page_size of page table[b][p / page_size]. The sequence runner's
 // counterpart for a contiguous cache is the head of csrc/attention.cu (kernels/e2e/model.py:236-241).
 //
-// Memory bound: every element is read once and written once; the angle rows are shared by all heads of a
-// token and come from the caches. One thread turns 8 dims and their 8 partners (two 16-byte loads, two
-// 16-byte stores) or copies 8 dims of v.
+// Memory bound: every element is read once and written once. A warp takes up to kAhead groups of heads of one token at a
+// time (a head's 8 dims and their 8 partners a lane, or 8 dims of v), loads them before it knows where they go - the
+// token's sequence, position and page are a chain of small loads - and its angles once for all of them. With few tokens
+// a token's heads are spread over several warps.
+#include <algorithm>
+
 #include "paged.cuh"
 
 namespace dk {
@@ -56,69 +59,99 @@ __device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
                     Elem<T>::pack(v[6], v[7]));
 }
 
+constexpr int kAhead = 2;  // 4 with half the warps resident: 33.9 against 32.9 us for 164 MB
+constexpr int kWarps = 8;
+
 template <typename T, typename R, int kHd>
-__global__ void __launch_bounds__(256) paged_append_kernel(const AppendParams p) {
-  constexpr int kRot = kHd / 16;  // threads per rotated head
-  constexpr int kCopy = kHd / 8;  // threads per head of v
+__global__ void __launch_bounds__(kWarps * 32, 4) paged_append_kernel(const AppendParams p, int segments, int per_warp) {
+  constexpr int kRot = kHd / 16;         // lanes of a rotated head
+  constexpr int kHeads = 32 / kRot;      // rotated heads of a segment
+  constexpr int kCopy = kHd / 8;         // lanes of a head of v
+  constexpr int kCopyHeads = 32 / kCopy;
   pdl_trigger();
   pdl_wait();
-  const int rot_items = (p.nq + p.nkv) * kRot;
-  const unsigned per_token = rot_items + p.nkv * kCopy;
-  const int64_t total = static_cast<int64_t>(p.T) * per_token;
-  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
-    const int t = static_cast<int>(i / per_token);
-    const int e = static_cast<int>(i - static_cast<int64_t>(t) * per_token);
+  const int lane = threadIdx.x & 31;
+  const int rot_heads = p.nq + p.nkv, rot_segments = (rot_heads + kHeads - 1) / kHeads;
+  const int parts = (segments + per_warp - 1) / per_warp;
+  const int64_t total = static_cast<int64_t>(p.T) * parts;
+  for (int64_t w = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5); w < total; w += static_cast<int64_t>(gridDim.x) * kWarps) {
+    const int t = static_cast<int>(w / parts), s0 = static_cast<int>(w % parts) * per_warp, s1 = min(s0 + per_warp, segments);
+    const T* row = static_cast<const T*>(p.qkv) + t * p.ldqkv;
+    const int d = 8 * (lane % kRot), vd = 8 * (lane % kCopy);
+    // the head of this lane in segment s, or -1
+    auto rot_head = [&](int s) {
+      const int h = s * kHeads + lane / kRot;
+      return s < rot_segments && h < rot_heads ? h : -1;
+    };
+    auto copy_head = [&](int s) {
+      const int h = (s - rot_segments) * kCopyHeads + lane / kCopy;
+      return s >= rot_segments && s < s1 && h < p.nkv ? h : -1;
+    };
+    uint4 lo[kAhead], hi[kAhead];
+    auto load = [&](int s) {
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) {
+        const int h = s + a < s1 ? rot_head(s + a) : -1, vh = copy_head(s + a);
+        if (h >= 0) {
+          lo[a] = *reinterpret_cast<const uint4*>(row + h * kHd + d);
+          hi[a] = *reinterpret_cast<const uint4*>(row + h * kHd + d + kHd / 2);
+        } else if (vh >= 0) {
+          lo[a] = *reinterpret_cast<const uint4*>(row + static_cast<int64_t>(rot_heads + vh) * kHd + vd);
+        }
+      }
+    };
+    load(s0);
     int b = t, pos;
     if (p.starts == nullptr) {
       pos = p.lengths[t] - 1;
     } else {
-      b = find_tile([&](int j) { return p.starts[j]; }, p.B, t);
+      b = find_tile_warp([&](int j) { return p.starts[j]; }, p.B, t, lane);
       pos = p.lengths[b] - (p.starts[b + 1] - t);
     }
-    const bool is_q = e < p.nq * kRot;
-    // a sequence without positions (an unused slot of the batch) appends nothing
-    const bool live = pos >= 0;
-    int page = -1;
-    if (live && !is_q) {
-      const int at = pos >> p.page_shift;
-      page = at < p.table_width ? p.table[b * p.ld_table + at] : -1;
-      if (page < 0 || page >= p.n_pages) {
-        record_device_error(p.err, DK_DEVERR_BAD_POSITION);
-        continue;
-      }
-    }
+    // A sequence without positions (an unused slot of the batch) appends nothing; its q is zero.
     const int64_t angle = pos + p.rope_offset;
-    const bool turns = live && angle >= 0 && angle < p.rope_rows;
-    if (live && !turns) record_device_error(p.err, DK_DEVERR_BAD_POSITION);
-    if (!turns && !is_q) continue;
-    const T* row = static_cast<const T*>(p.qkv) + t * p.ldqkv;
+    const bool live = pos >= 0, turns = live && angle >= 0 && angle < p.rope_rows;
+    const int at = pos >> p.page_shift;
+    const int page = live && at < p.table_width ? p.table[b * p.ld_table + at] : -1;
+    const bool lands = turns && page >= 0 && page < p.n_pages;
+    if (live && !lands && lane == 0) record_device_error(p.err, DK_DEVERR_BAD_POSITION);
+    float co[8], si[8];
+    if (turns) {
+      load8<T>(static_cast<const R*>(p.cos) + angle * p.ld_rope + d, co);
+      load8<T>(static_cast<const R*>(p.sin) + angle * p.ld_rope + d, si);
+    }
     const int64_t in_page = static_cast<int64_t>(pos & (p.page_size - 1)) * kHd;
-    if (e < rot_items) {
-      const int h = e / kRot, d = 8 * (e % kRot);
-      uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
-      if (turns) {
-        float a[8], c[8], x[8], y[8], u[8], w[8];
-        load8<T>(row + h * kHd + d, x);
-        load8<T>(row + h * kHd + d + kHd / 2, y);
-        load8<T>(static_cast<const R*>(p.cos) + angle * p.ld_rope + d, a);
-        load8<T>(static_cast<const R*>(p.sin) + angle * p.ld_rope + d, c);
+    const int64_t page_heads = static_cast<int64_t>(page) * p.nkv;
+    for (int s = s0; s < s1; s += kAhead) {
+      if (s > s0) load(s);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          u[j] = x[j] * a[j] - y[j] * c[j];
-          w[j] = y[j] * a[j] + x[j] * c[j];
+      for (int a = 0; a < kAhead; ++a) {
+        const int h = s + a < s1 ? rot_head(s + a) : -1, vh = copy_head(s + a);
+        if (h >= 0) {
+          const bool is_q = h < p.nq;
+          if (!is_q && !lands) continue;
+          uint4 u = make_uint4(0, 0, 0, 0), v = u;
+          if (turns) {
+            const uint32_t l[4] = {lo[a].x, lo[a].y, lo[a].z, lo[a].w}, r[4] = {hi[a].x, hi[a].y, hi[a].z, hi[a].w};
+            float x[8], y[8];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float2 f = Elem<T>::unpack(l[j]), g = Elem<T>::unpack(r[j]);
+              x[2 * j] = f.x * co[2 * j] - g.x * si[2 * j];
+              x[2 * j + 1] = f.y * co[2 * j + 1] - g.y * si[2 * j + 1];
+              y[2 * j] = g.x * co[2 * j] + f.x * si[2 * j];
+              y[2 * j + 1] = g.y * co[2 * j + 1] + f.y * si[2 * j + 1];
+            }
+            u = pack8<T>(x), v = pack8<T>(y);
+          }
+          T* dst = is_q ? static_cast<T*>(p.q_out) + (static_cast<int64_t>(t) * p.nq + h) * kHd
+                        : static_cast<T*>(p.k) + (page_heads + h - p.nq) * p.page_size * kHd + in_page;
+          *reinterpret_cast<uint4*>(dst + d) = u;
+          *reinterpret_cast<uint4*>(dst + d + kHd / 2) = v;
+        } else if (vh >= 0 && lands) {
+          *reinterpret_cast<uint4*>(static_cast<T*>(p.v) + (page_heads + vh) * p.page_size * kHd + in_page + vd) = lo[a];
         }
-        lo = pack8<T>(u), hi = pack8<T>(w);
       }
-      T* dst = is_q ? static_cast<T*>(p.q_out) + (static_cast<int64_t>(t) * p.nq + h) * kHd
-                    : static_cast<T*>(p.k) +
-                          (static_cast<int64_t>(page) * p.nkv + (h - p.nq)) * p.page_size * kHd + in_page;
-      *reinterpret_cast<uint4*>(dst + d) = lo;
-      *reinterpret_cast<uint4*>(dst + d + kHd / 2) = hi;
-    } else {
-      const int h = (e - rot_items) / kCopy, d = 8 * ((e - rot_items) % kCopy);
-      T* dst = static_cast<T*>(p.v) + (static_cast<int64_t>(page) * p.nkv + h) * p.page_size * kHd + in_page;
-      *reinterpret_cast<uint4*>(dst + d) =
-          *reinterpret_cast<const uint4*>(row + static_cast<int64_t>(p.nq + p.nkv + h) * kHd + d);
     }
   }
 }
@@ -163,15 +196,18 @@ extern "C" int dk_paged_append(const dk_paged_append_args* args) {
   p.page_shift = __builtin_ctzll(page_size);
   p.table_width = static_cast<int>(table_width);
   p.err = device_info().err_word;
-  const int64_t items = T * ((nq + nkv) * (head_dim / 16) + nkv * (head_dim / 8));
-  const int64_t blocks = (items + 255) / 256, most = 16ll * device_info().num_sms;
-  const dim3 grid(static_cast<unsigned>(blocks < most ? blocks : most));
+  const int heads = static_cast<int>(512 / head_dim), copies = static_cast<int>(256 / head_dim);
+  const int segments = static_cast<int>((nq + nkv + heads - 1) / heads + (nkv + copies - 1) / copies);
+  // Whole tokens a warp once there are 16 warps of them for every SM; fewer segments each with fewer tokens.
+  const int64_t want = 16ll * device_info().num_sms;
+  const int per_warp = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(segments, T * segments / want)));
+  const int64_t warps = T * ((segments + per_warp - 1) / per_warp);
+  const dim3 grid(static_cast<unsigned>(std::min<int64_t>((warps + kWarps - 1) / kWarps, 64ll * device_info().num_sms)));
   cudaStream_t st = reinterpret_cast<cudaStream_t>(a.stream);
   cudaError_t e;
 #define DK_APPEND(TT, RR)                                                                                    \
-  e = head_dim == 128                                                                                        \
-          ? launch(paged_append_kernel<TT, RR, 128>, grid, dim3(256), 0, st, pdl_enabled(), dim3(1, 1, 1), p) \
-          : launch(paged_append_kernel<TT, RR, 64>, grid, dim3(256), 0, st, pdl_enabled(), dim3(1, 1, 1), p)
+  e = launch(head_dim == 128 ? paged_append_kernel<TT, RR, 128> : paged_append_kernel<TT, RR, 64>, grid, dim3(kWarps * 32), 0, \
+             st, pdl_enabled(), dim3(1, 1, 1), p, segments, per_warp)
   if (dtype == DK_F16) {
     if (a.rope_f32)
       DK_APPEND(__half, float);

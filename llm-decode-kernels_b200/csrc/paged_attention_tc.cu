@@ -34,6 +34,11 @@ constexpr int kRegsLaunch = 168, kRegsSoftmax = 208, kRegsOther = 88;
 static_assert(256 * kRegsSoftmax + 128 * kRegsOther <= kThreads * kRegsLaunch, "register split");
 constexpr int kC = kTcChunk;
 constexpr float kLazy = 8.f;  // growth (base 2) of a row's maximum that P takes without rescaling O
+// P is handed over in two parts, positions 0..95 and 96..127: the products of the first run while the exponentials of the
+// second are computed, so that only a quarter of P V is left after the softmax (a prompt of 8192: 196 us; 198 us with
+// parts of 64 and 64, 202 us in one piece).
+constexpr int kPartChunks = 3;  // 32-position chunks of the first part
+constexpr int kPartSteps = 2 * kPartChunks;  // its products of 16 positions each
 
 template <int kHd>
 struct Smem {
@@ -47,7 +52,7 @@ struct Smem {
 struct Barriers {
   uint64_t kv_full[10], kv_empty[10];
   uint64_t q_full, q_empty;
-  uint64_t s_full[2], p_full[2], o_full[2];
+  uint64_t s_full[2], p_full[2][2], o_full[2];  // p_full: [half][the two parts of P]
   uint64_t drain;
 };
 
@@ -204,7 +209,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&bar.q_empty, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bar.s_full[i], 1);
-      mbar_init(&bar.p_full[i], 4);
+      mbar_init(&bar.p_full[i][0], 4);
+      mbar_init(&bar.p_full[i][1], 4);
       mbar_init(&bar.o_full[i], 1);
     }
     mbar_init(&bar.drain, 1);
@@ -307,15 +313,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       commit_elected(&bar.s_full[x]);
     };
     auto pv = [&](int x, int f, bool first) {
-      if (ok && !wait_for(&bar.p_full[x], p_seen[x] & 1, p.err, DK_DEVERR_WAIT_FULL)) ok = false;
-      ++p_seen[x];
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) return;
-      tc::fence_after_sync();
       const uint64_t b = sdesc_n_sw128(slot_at(f), L::kSegBytes);
 #pragma unroll
-      for (int k = 0; k < kC / 16; ++k)
-        mma_ts(tmem + kO[x], tmem + kS[x] + 8 * k, b + ((k * 2048) >> 4), idesc<T>(128, kHd, true), !first || k > 0);
+      for (int half = 0; half < 2; ++half) {
+        if (ok && !wait_for(&bar.p_full[x][half], p_seen[x] & 1, p.err, DK_DEVERR_WAIT_FULL)) ok = false;
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) return;
+        tc::fence_after_sync();
+#pragma unroll
+        for (int k = half * kPartSteps; k < (half ? kC / 16 : kPartSteps); ++k)
+          mma_ts(tmem + kO[x], tmem + kS[x] + 8 * k, b + ((k * 2048) >> 4), idesc<T>(128, kHd, true), !first || k > 0);
+      }
+      ++p_seen[x];
     };
     for (int part = 0; walk.more() && ok; ++part) {
       const Span<kC> span = walk.step();
@@ -415,54 +424,50 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int d = 0; d < 32; ++d) s[32 * c + d] = see & (1u << d) ? s[32 * c + d] : -INFINITY;
           }
         }
-        // P refers to the maximum of the chunks before; only when this chunk's turns out to be 2^kLazy above it (or there
-        // was none) is the maximum raised and the chunk done again, so that the exponentials need not wait for it.
-        if (i == walk.c0) m = row_max(s) * p.scale2;
-        float2 sums;
-        for (;;) {
-          const float base = m == -INFINITY ? 0.f : m;
-          const float2 scale = make_float2(p.scale2, p.scale2), off = make_float2(-base, -base);
-          float2 sum[4] = {};
-          float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int c = 0; c < kC / 32; ++c) {
-            uint32_t w[16];
-#pragma unroll
-            for (int d = 0; d < 16; ++d) {
-              const float2 x2 = make_float2(s[32 * c + 2 * d], s[32 * c + 2 * d + 1]);
-              top[d & 3] = fmaxf(fmaxf(top[d & 3], x2.x), x2.y);
-              float2 y = fma2(x2, scale, off);
-              y = make_float2(exp2_approx(y.x), exp2_approx(y.y));
-              sum[d & 3] = add2(sum[d & 3], y);
-              w[d] = E::pack(y.x, y.y);
-            }
-            tmem_st16(s_col + 16 * c, w);
-          }
-          sums = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
-          const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale2;
-          const bool raise = mx > m + kLazy || (m == -INFINITY && mx > -INFINITY);
-          if (!__any_sync(0xffffffffu, raise)) break;
+        // P refers to a maximum that is only raised when a row's grows by 2^kLazy or more.
+        const float mx = row_max(s) * p.scale2;
+        const bool raise = mx > m + kLazy || (m == -INFINITY && mx > -INFINITY);
+        if (__any_sync(0xffffffffu, raise)) {
           const float keep = raise ? exp2_approx(m - mx) : 1.f;
           if (raise) {
             m = mx;
             l *= keep;
           }
-          // O's products up to the last chunk are done: S came after them
+          if (i > walk.c0) {  // O's products up to the last chunk are done: S came after them
 #pragma unroll
-          for (int c = 0; c < kHd / 16; ++c) {
-            float o[16];
-            uint32_t w[16];
-            tc::tmem_ld16(o_col + 16 * c, o);
+            for (int c = 0; c < kHd / 16; ++c) {
+              float o[16];
+              uint32_t w[16];
+              tc::tmem_ld16(o_col + 16 * c, o);
 #pragma unroll
-            for (int d = 0; d < 16; ++d) w[d] = __float_as_uint(o[d] * keep);
-            tmem_st16(o_col + 16 * c, w);
+              for (int d = 0; d < 16; ++d) w[d] = __float_as_uint(o[d] * keep);
+              tmem_st16(o_col + 16 * c, w);
+            }
           }
         }
+        const float base = m == -INFINITY ? 0.f : m;
+        const float2 scale = make_float2(p.scale2, p.scale2), off = make_float2(-base, -base);
+        float2 sum[4] = {};
+#pragma unroll
+        for (int c = 0; c < kC / 32; ++c) {
+          uint32_t w[16];
+#pragma unroll
+          for (int d = 0; d < 16; ++d) {
+            float2 y = fma2(make_float2(s[32 * c + 2 * d], s[32 * c + 2 * d + 1]), scale, off);
+            y = make_float2(exp2_approx(y.x), exp2_approx(y.y));
+            sum[d & 3] = add2(sum[d & 3], y);
+            w[d] = E::pack(y.x, y.y);
+          }
+          tmem_st16(s_col + 16 * c, w);
+          if (c == kPartChunks - 1 || c == kC / 32 - 1) {  // a part of P is complete
+            tmem_wait_st();
+            tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar.p_full[x][c / kPartChunks]);
+          }
+        }
+        const float2 sums = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
         l += sums.x + sums.y;
-        tmem_wait_st();
-        tc::fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bar.p_full[x]);
       }
       if (ok && !wait_for(&bar.o_full[x], o_seen & 1, p.err, DK_DEVERR_WAIT_FULL)) ok = false;
       ++o_seen;

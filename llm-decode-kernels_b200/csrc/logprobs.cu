@@ -199,6 +199,7 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const LogprobParam
   // Vectors of this part that lie wholly in the row; its at most two others are taken element by element.
   const int f0 = v0 * kN < skip ? v0 + 1 : v0, f1 = min(v1, (skip + V) / kN);
   if (tid == 0) count = vec_count = 0, thr_sh = -INFINITY;
+  __syncthreads();
 
   // element i of vector v: -inf where it is outside the row
   auto fetch = [&](int v) {
@@ -505,7 +506,7 @@ extern "C" int dk_token_logprobs(const void* logits, int64_t ld, int32_t dtype, 
                      kMaxTop);
   if (dtype != DK_F16 && dtype != DK_BF16 && dtype != DK_F32)
     return set_error(DK_ERR_UNSUPPORTED, "token_logprobs: dtype %d", dtype);
-  if (M > INT32_MAX || V >= INT32_MAX) return set_error(DK_ERR_INVALID, "token_logprobs: sizes must fit 31 bits");
+  if (M > INT32_MAX || V > INT32_MAX - 16) return set_error(DK_ERR_INVALID, "token_logprobs: sizes must fit 31 bits");
   if (M == 0) return DK_OK;
   if (!logits || !targets || !logprob || !entropy || (top > 0 && (!top_logprob || !top_id)))
     return set_error(DK_ERR_INVALID, "token_logprobs: NULL pointer");

@@ -184,7 +184,7 @@ extern "C" int dk_paged_append(const dk_paged_append_args* args) {
   if (!a.qkv || !a.k_pages || !a.v_pages || !a.page_table || !a.lengths || !a.cos || !a.sin || !a.q_out)
     return set_error(DK_ERR_INVALID, "paged_append: NULL pointer");
   if (!aligned16(a.qkv) || !aligned16(a.k_pages) || !aligned16(a.v_pages) || !aligned16(a.q_out) || !aligned16(a.cos) ||
-      !aligned16(a.sin) || (a.ldqkv & 7) || (a.ld_rope & (a.rope_f32 ? 3 : 7)))
+      !aligned16(a.sin) || (T > 1 && (a.ldqkv & 7)) || (a.ld_rope & (a.rope_f32 ? 3 : 7)))
     return set_error(DK_ERR_ALIGN, "paged_append: rows of qkv, cos, sin, the pages and q_out need 16-byte alignment");
   AppendParams p;
   p.qkv = a.qkv, p.ldqkv = a.ldqkv, p.k = a.k_pages, p.v = a.v_pages;

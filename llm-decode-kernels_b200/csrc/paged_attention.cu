@@ -33,7 +33,6 @@ constexpr int kRowsUnitExtra = 2;  // a unit's fixed cost (q, joining the warps,
 
 // ------------------------------------------------------------------------------------ ragged plan
 // One CTA cuts the sequences into tiles of tile_tokens tokens and sums up their chunks.
-template <int kUnitChunk>
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Problem p, int32_t* plan, int4* info) {
   constexpr int kOwnTiles = 4;  // tiles of a sequence that its own thread writes
   __shared__ int warp_sum[kPlanThreads / 32];
@@ -101,7 +100,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Problem p, int
       const int4 v = info[i];  // {first token, sequence's end, length, sequence}
       const int ntok = min(p.tile_tokens, v.y - v.x), p0 = v.z - (v.y - v.x);
       info[i] = make_int4(v.x, ntok, p0, v.w);
-      n = Span<kUnitChunk>(p0, p0 + ntok - 1, p.mask, p.capacity).n + p.unit_extra;
+      n = Span<kTcChunk>(p0, p0 + ntok - 1, p.mask, p.capacity).n + p.unit_extra;
     }
     int total;
     const int at = length + scan(n, total);
@@ -559,8 +558,7 @@ struct Sizes {
   int dtype;
 };
 
-// Tokens of a tile of up to 16 rows, and the rows a tile's results take.
-int rows_tile_tokens(const Sizes& z) { return z.ragged ? std::max<int>(1, 16 / static_cast<int>(z.nq / z.nkv)) : 1; }
+// Rows that the results of a tile of up to 16 rows take.
 int rows_of(const Sizes& z, int tokens) { return tokens * (z.nq / z.nkv) <= 8 ? 8 : 16; }
 
 RowsShape rows_shape_of(const Sizes& z, int rows) {
@@ -638,7 +636,7 @@ void set_tile(const Sizes& z, Pass& a, int tokens16) {
 void shape_own(const Sizes& z, Pass& a) {
   a.tc = z.ragged;
   a.p.mode = z.ragged ? kRagged : kOneToken;
-  set_tile(z, a, rows_tile_tokens(z));
+  set_tile(z, a, 1);
   a.p.max_tiles = z.ragged ? static_cast<int>(z.T / a.p.tile_tokens + z.B) : 0;
   a.p.n_tiles = static_cast<int>(z.B);
 }
@@ -727,7 +725,8 @@ int attention(const char* what, const dk_paged_attention_args* args, bool prefix
   const dk_paged_attention_args& a = *args;
   const Sizes z{a.T, a.B, a.n_q, a.n_kv, a.head_dim, prefix ? a.prefix_len : 0, a.starts != nullptr, static_cast<int>(a.dtype)};
   const int64_t n_pages = a.n_pages, page_size = a.page_size, table_width = a.table_width;
-  const int64_t window = prefix ? 0 : a.window, sinks = prefix ? 0 : a.sinks;
+  int64_t window = prefix ? 0 : a.window;
+  const int64_t sinks = prefix ? 0 : a.sinks;
   if (const int rc = check_sizes(what, z)) return rc;
   if (n_pages <= 0 || table_width <= 0 || window < 0 || sinks < 0) return set_error(DK_ERR_INVALID, "%s: bad sizes", what);
   if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1)))
@@ -735,11 +734,14 @@ int attention(const char* what, const dk_paged_attention_args* args, bool prefix
   if (n_pages * z.nkv * page_size + kChunk >= (int64_t(1) << 31) || table_width * page_size >= (int64_t(1) << 31) ||
       window >= (int64_t(1) << 31) || sinks >= (int64_t(1) << 31))
     return set_error(DK_ERR_INVALID, "%s: pages x kv heads x page_size, a table row's positions, window and sinks must stay below 2^31", what);
+  window = std::min(window, table_width * page_size);  // a window of all positions or more masks none: p - window stays in range
+  const int64_t ldq = z.T > 1 ? a.ldq : z.nq * z.hd;
   if (z.T == 0) return DK_OK;
+  if (ldq < z.nq * z.hd) return set_error(DK_ERR_INVALID, "%s: q's tokens overlap", what);
   if (!a.q || !a.k_pages || !a.v_pages || !a.page_table || !a.lengths || !a.out || !a.workspace ||
       (z.prefix_len > 0 && !a.prefix_table))
     return set_error(DK_ERR_INVALID, "%s: NULL pointer", what);
-  if (!aligned16(a.q) || !aligned16(a.k_pages) || !aligned16(a.v_pages) || !aligned16(a.out) || (a.ldq & 7) ||
+  if (!aligned16(a.q) || !aligned16(a.k_pages) || !aligned16(a.v_pages) || !aligned16(a.out) || (ldq & 7) ||
       (reinterpret_cast<uintptr_t>(a.workspace) & 255))
     return set_error(DK_ERR_ALIGN, "%s: q rows, pages and out need 16-byte alignment, the workspace 256", what);
   Pass own = {}, pre = {};
@@ -765,7 +767,7 @@ int attention(const char* what, const dk_paged_attention_args* args, bool prefix
     return set_error(DK_ERR_UNSUPPORTED, "%s: the kernel's shared memory does not fit this device", what);
   const int beside = z.prefix_len > 0 && pdl_enabled() ? 1 : 0;
   for (Problem* p : {&own.p, &pre.p}) {
-    p->q = a.q, p->ldq = a.ldq, p->out = a.out;
+    p->q = a.q, p->ldq = ldq, p->out = a.out;
     p->table = a.page_table, p->ld_table = a.ld_table, p->lengths = a.lengths, p->starts = a.starts;
     p->T = static_cast<int>(z.T), p->B = static_cast<int>(z.B), p->nkv = static_cast<int>(z.nkv);
     p->G = static_cast<int>(z.nq / z.nkv);
@@ -790,7 +792,7 @@ int attention(const char* what, const dk_paged_attention_args* args, bool prefix
     return DK_ERR_CUDA;
   cudaError_t e = cudaSuccess;
   if (z.ragged)
-    e = launch(plan_kernel<kTcChunk>, dim3(1), dim3(kPlanThreads), 0, st, pdl_enabled(), dim3(1, 1, 1), own.p,
+    e = launch(plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, pdl_enabled(), dim3(1, 1, 1), own.p,
                const_cast<int32_t*>(own.p.plan), const_cast<int4*>(own.p.tile_info));
   for (const Pass* s : {&pre, &own}) {
     if (s->ctas == 0 || e != cudaSuccess) continue;

@@ -132,8 +132,8 @@ def _attend(what, entry, q, k_pages, v_pages, prefix_table, prefix_len, page_tab
     T, nq, width = q.shape
     n_pages, n_kv, page, hd, B = _cache_shape(what, k_pages, v_pages, page_table, lengths, starts, T)
     ld, by_head, unit = q.stride()
-    if width != hd or unit != 1 or by_head != hd:
-        _refuse(what, "q must be [tokens, heads, head_dim] with its heads side by side")
+    if width != hd or unit != 1 or by_head != hd or ld < nq * hd and T > 1:
+        _refuse(what, "q must be [tokens, heads, head_dim], a token's heads side by side and tokens apart from each other")
     if nq <= 0 or nq % n_kv or nq // n_kv > MAX_GROUP:
         _refuse(what, f"query heads must be a multiple of the kv heads, at most {MAX_GROUP} for each")
     dtype = q.dtype

@@ -227,6 +227,40 @@ def test_attention_long_context_and_masked_extremes():
 
 # ------------------------------------------------------------------------------------------ shared prefix
 @pytest.mark.gpu
+@pytest.mark.parametrize("sizes", [[(1, 300)], [(1, 300), (1, 0), (1, 31)], [(9, 5), (4, 200), (3, 0)]])
+def test_attention_windows_past_every_position(sizes):
+    """A window as long as the table or longer masks nothing, up to the largest; rows before the first position are empty."""
+    from kernels.paged import paged_attention
+
+    c = Case(sizes, one_token=all(n == 1 for n, _ in sizes))
+    args = (c.q, c.k, c.v, c.table, c.lengths, c.starts)
+    plain = paged_attention(*args)
+    exact, tol = c.attention()
+    assert_within(plain, exact, tol)
+    for window in (c.table.shape[1] * c.page, 2 ** 31 - 1):
+        for sinks in (0, 4, 2 ** 31 - 1):
+            assert torch.equal(paged_attention(*args, window=window, sinks=sinks), plain)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ragged", [False, True])
+def test_one_token_of_any_stride(ragged):
+    """The row stride of a single token means nothing, whatever it is."""
+    from kernels.paged import paged_append, paged_attention
+
+    c = Case([(1, 77)], one_token=not ragged)
+    odd = c.q.as_strided(c.q.shape, (3, c.hd, 1))
+    exact, tol = c.attention()
+    assert_within(paged_attention(odd, c.k, c.v, c.table, c.lengths, c.starts), exact, tol)
+    qkv = torch.randn(1, (c.nq + 2 * c.nkv) * c.hd, device="cuda", dtype=c.dtype)
+    angle = torch.rand(100, c.hd // 2, device="cuda")
+    a = paged_append(qkv, c.k.clone(), c.v.clone(), c.table, c.lengths, angle.cos(), angle.sin(), c.nq, c.nkv, c.starts)
+    b = paged_append(qkv.as_strided(qkv.shape, (5, 1)), c.k, c.v, c.table, c.lengths, angle.cos(), angle.sin(), c.nq, c.nkv,
+                     c.starts)
+    assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("sizes,prefix,nq,nkv,hd,page,dtype", [
     ([(1, 1)], 1, 12, 2, 128, 16, F16),
     ([(1, 40), (1, 1), (1, 65)], 525, 12, 2, 128, 16, F16),
@@ -278,6 +312,7 @@ def test_refusals_without_a_gpu():
     attend(ValueError, (0, c.q[:, :5]))  # 5 query heads over 2 kv heads
     attend(ValueError, (0, torch.zeros(2, 34, 128).half()))  # 17 query heads for each kv head
     attend(ValueError, (0, c.q.transpose(1, 2).contiguous().transpose(1, 2)))
+    attend(ValueError, (0, c.q[:1].expand(2, -1, -1)))  # overlapping tokens
     attend(ValueError, (1, c.k[:, :, :8].contiguous()), (2, c.v[:, :, :8].contiguous()))
     attend(ValueError, (1, c.k[:-1]))
     attend(ValueError, (1, c.k.transpose(0, 1)), (2, c.v.transpose(0, 1)))
@@ -347,6 +382,7 @@ def test_c_entries_refuse_without_a_gpu():
     assert attend(nq=13) == -3 and attend(nq=34) == -3
     assert attend(dtype=2) == -3
     assert attend(B=5000, T=5000) == -3 and b"sequences" in h.dk_last_error()
+    assert attend(ldq=8) == -1 and b"overlap" in h.dk_last_error()
     assert attend(pages=1 << 26) == -1 and b"2^31" in h.dk_last_error()
     assert attend(width=1 << 27) == -1
     assert h.dk_paged_attention_workspace_bytes(2, 2, 12, 2, 96, 0, 0, 0, ctypes.byref(n)) == -3

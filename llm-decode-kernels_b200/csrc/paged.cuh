@@ -138,7 +138,7 @@ struct Problem {
   float scale2;  // scale * log2(e)
   int mode;
   int tile_tokens;
-  int half_tokens;  // tokens of 128 rows (the tensor-core kernel); tile_tokens where a tile has at most 16 rows
+  int half_tokens;  // tokens of 128 rows (tiles_kernel); 1 (rows_kernel)
   int early, lead;  // the launch's first `early` pieces are `lead` chunks longer than the others (their CTAs start while
                     // the kernel before still holds the other SMs)
   int unit_extra;   // chunks added to a unit's length on the line for what it costs besides its chunks

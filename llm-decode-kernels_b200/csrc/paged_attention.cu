@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(kThreads)
   __shared__ int warp_sum[kThreads / 32 + 1];
   extern __shared__ __align__(128) uint8_t dsm_raw[];
   uint8_t* base = dsm_raw + ((1024u - (smem_addr(dsm_raw) & 1023u)) & 1023u);
-  int* cum_sh = reinterpret_cast<int*>(base);  // kOneToken: [B + 1], before the first copies land there
+  int* cum_sh = reinterpret_cast<int*>(base);  // [B + 1], before the first copies land there
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const bool producer = warp >= kGroups * kCWarps;
@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(kThreads)
   pdl_trigger();
 
   Line line{cum_sh, 0, p.n_tiles, 0};
-  if (p.mode == kOneToken) {  // every CTA sums up the sequences' chunks for itself
+  {  // every CTA sums up the sequences' chunks for itself
     int carry = 0;
     for (int b0 = 0; b0 < p.B; b0 += kThreads) {
       const int b = b0 + tid;
@@ -200,8 +200,6 @@ __global__ void __launch_bounds__(kThreads)
     __syncthreads();
     if (blockIdx.x == 0)  // for the join kernel
       for (int i = tid; i <= p.B; i += kThreads) p.cum_out[i] = cum_sh[i];
-  } else {
-    line = line_of(p, kChunk);
   }
   __syncthreads();
 
@@ -257,18 +255,17 @@ __global__ void __launch_bounds__(kThreads)
     while (walk.more()) {
       const Span<kChunk> span = walk.step();
       const Tile t = walk.t;
-      const int h = walk.h, c0 = walk.c0, c1 = walk.c1, plast = walk.last;
+      const int h = walk.h, c0 = walk.c0, c1 = walk.c1;
       if (c1 <= c0) continue;
-      const int rows = t.ntok * p.G;
+      const int rows = p.G;  // one token's
       // this lane's rows g and g + 8: positions, and q as the MMA's A operand
       int pos[kR];
       uint32_t qa[kHd / 16][2 * kR];
 #pragma unroll
       for (int e = 0; e < kR; ++e) {
         const int row = g + 8 * e;
-        const int tok = row / p.G;
-        pos[e] = row < rows ? row_position(p, t, tok) : INT_MIN;
-        const T* qr = static_cast<const T*>(p.q) + (t.t0 + tok) * p.ldq + (h * p.G + row - tok * p.G) * kHd;
+        pos[e] = row < rows ? t.p0 : INT_MIN;
+        const T* qr = static_cast<const T*>(p.q) + t.t0 * p.ldq + (h * p.G + row) * kHd;
 #pragma unroll
         for (int ks = 0; ks < kHd / 16; ++ks) {
           qa[ks][e] = row < rows ? *reinterpret_cast<const uint32_t*>(qr + 16 * ks + 2 * tq) : 0u;
@@ -301,7 +298,7 @@ __global__ void __launch_bounds__(kThreads)
             E::mma(sc[1], qa[ks][0], a1, qa[ks][kR], a3, kb[2], kb[3]);
           }
           // every row sees all 16 positions (nothing to mask)?
-          const bool clear = j0 + 15 <= t.p0 && (p.mask.window <= 0 || j0 > plast - p.mask.window || j0 + 15 < p.mask.sinks) &&
+          const bool clear = j0 + 15 <= t.p0 && (p.mask.window <= 0 || j0 > t.p0 - p.mask.window || j0 + 15 < p.mask.sinks) &&
                              j0 + 15 < span.end;
           uint32_t pa[2][kR];  // p as the MMA's A operand
 #pragma unroll
@@ -402,9 +399,7 @@ __global__ void __launch_bounds__(kThreads)
           if (whole) {
             const float l = fin[2 * row + 1];
             const float inv = l == 0.f ? 0.f : 1.f / l;
-            const int tok = row / p.G;
-            T* dst = static_cast<T*>(p.out) +
-                     (static_cast<int64_t>(t.t0 + tok) * p.nkv * p.G + h * p.G + row - tok * p.G) * kHd + d;
+            T* dst = static_cast<T*>(p.out) + (static_cast<int64_t>(t.t0) * p.nkv * p.G + h * p.G + row) * kHd + d;
             *reinterpret_cast<uint2*>(dst) = make_uint2(E::pack(a.x * inv, a.y * inv), E::pack(a.z * inv, a.w * inv));
           } else {
             *reinterpret_cast<float4*>(&p.part_o[(slot * kRows + row) * kHd + d]) = a;
@@ -427,44 +422,70 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // ------------------------------------------------------------------------------------ join
-// A block joins 8 result rows: a lane has row lane % 8 and, of each 16 dims of its warp, the four lane / 8 * 4 ...: in
-// either layout of the partial results a warp's load touches few lines.
-constexpr int kJoinRows = 8;
+// How a join's block takes results: kRows rows, kDims groups of four dims of each (the grid's z has the others), and kParts
+// stretches of a unit's pieces, whose sums are joined in order at the end. A unit cut into many pieces (few sequences, long
+// ones: up to one for every CTA) would otherwise be one long chain of loads on one SM.
+template <int kR, int kD, int kP, int kA>
+struct JoinShape {
+  static constexpr int kRows = kR, kDims = kD, kParts = kP, kAhead = kA;  // kAhead: pieces loaded at a time
+  static constexpr int kLanes = kR * kD, kThreads = kLanes * kP;
+  int lane, part, row, d4;  // of this thread; row: in the whole grid's y (or x)
+  __device__ explicit JoinShape(int y)
+      : lane(threadIdx.x % kLanes), part(threadIdx.x / kLanes), row(y * kR + lane % kR), d4(blockIdx.z * kD + lane / kR) {}
+};
 
 template <typename T, int kHd>
 struct Joined {
   float m = -INFINITY, l = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  // Adds the pieces of this lane's unit in order, kAhead of them loaded at a time; row < 0: none. d4: the lane's dims / 4.
+  __device__ void add(float m2, float l2, const float4& o) {
+    const float mx = fmaxf(m, m2), use = mx == -INFINITY ? 0.f : mx;
+    const float keep = exp2_approx(m - use), take = exp2_approx(m2 - use);
+    m = mx;
+    l = fmaf(l, keep, l2 * take);
+    acc.x = fmaf(acc.x, keep, o.x * take), acc.y = fmaf(acc.y, keep, o.y * take);
+    acc.z = fmaf(acc.z, keep, o.z * take), acc.w = fmaf(acc.w, keep, o.w * take);
+  }
+  // Adds the pieces from..to of a unit's row in order, kAhead of them loaded at a time. d4: the lane's dims / 4.
   template <int kAhead>
-  __device__ void add(const Problem& p, const Pieces& w, int tile_rows, int row, int d4) {
-    if (row < 0) return;
+  __device__ void add(const Problem& p, const Pieces& w, int from, int to, int tile_rows, int row, int d4) {
     const int64_t at = p.rows_inner ? static_cast<int64_t>(d4) * tile_rows + row : static_cast<int64_t>(row) * (kHd / 4) + d4;
-    for (int i0 = w.first; i0 <= w.last; i0 += kAhead) {
+    for (int i0 = from; i0 <= to; i0 += kAhead) {
       float2 ml[kAhead];
       float4 o[kAhead];
 #pragma unroll
       for (int a = 0; a < kAhead; ++a) {
-        if (i0 + a > w.last) break;
+        if (i0 + a > to) break;
         const int64_t slot = piece_slot(w, i0 + a);
         ml[a] = *reinterpret_cast<const float2*>(&p.part_ml[(slot * tile_rows + row) * 2]);
         o[a] = reinterpret_cast<const float4*>(p.part_o)[slot * tile_rows * (kHd / 4) + at];
       }
 #pragma unroll
       for (int a = 0; a < kAhead; ++a) {
-        if (i0 + a > w.last) break;
-        const float mx = fmaxf(m, ml[a].x), use = mx == -INFINITY ? 0.f : mx;
-        const float keep = exp2_approx(m - use), take = exp2_approx(ml[a].x - use);
-        m = mx;
-        l = fmaf(l, keep, ml[a].y * take);
-        acc.x = fmaf(acc.x, keep, o[a].x * take), acc.y = fmaf(acc.y, keep, o[a].y * take);
-        acc.z = fmaf(acc.z, keep, o[a].z * take), acc.w = fmaf(acc.w, keep, o[a].w * take);
+        if (i0 + a > to) break;
+        add(ml[a].x, ml[a].y, o[a]);
       }
     }
   }
-  // `out`: this lane's row, or null.
+  // The same by all parts of a block, called by all of its threads (`live`: this one has a row); the first has the result.
+  template <typename Shape>
+  __device__ void add_parts(const Problem& p, const Pieces& w, int tile_rows, int row, const Shape& at, bool live) {
+    const int n = w.last - w.first + 1, parts = Shape::kParts;
+    if (live)
+      add<Shape::kAhead>(p, w, w.first + n * at.part / parts, w.first + n * (at.part + 1) / parts - 1, tile_rows, row, at.d4);
+    if constexpr (Shape::kParts > 1) {
+      __shared__ float2 part_ml[Shape::kParts - 1][Shape::kLanes];
+      __shared__ float4 part_o[Shape::kParts - 1][Shape::kLanes];
+      if (at.part > 0) {
+        part_ml[at.part - 1][at.lane] = make_float2(m, l);
+        part_o[at.part - 1][at.lane] = acc;
+      }
+      __syncthreads();
+      if (at.part == 0)
+        for (int i = 0; i < Shape::kParts - 1; ++i) add(part_ml[i][at.lane].x, part_ml[i][at.lane].y, part_o[i][at.lane]);
+    }
+  }
   __device__ void store(T* out, int d4) const {
-    if (out == nullptr) return;
     const float inv = l == 0.f ? 0.f : 1.f / l;
     *reinterpret_cast<uint2*>(out + 4 * d4) = make_uint2(Elem<T>::pack(acc.x * inv, acc.y * inv), Elem<T>::pack(acc.z * inv, acc.w * inv));
   }
@@ -475,43 +496,61 @@ __device__ __forceinline__ T* out_row(const Problem& p, int t, int head) {
   return static_cast<T*>(p.out) + (static_cast<int64_t>(t) * p.nkv * p.G + head) * kHd;
 }
 
-// Joins the units that a piece's end cuts. Block (i, y): 8 rows of the unit that CTA i began, if there is one.
-// kAhead: 4 for the one-token launch's 8-row units, 2 for the tiles' 256 (fewer pieces, more blocks: 4 costs 3 us there).
-template <typename T, int kHd, int kAhead>
-__global__ void __launch_bounds__(kHd * 2) join_split_kernel(const Problem p, int tile_rows) {
+// Joins the units that a piece's end cuts. Block (x, y): rows of the unit that CTA x began, if there is one, or with
+// `by_unit` (launches of fewer units than CTAs) of unit x, if it is cut.
+template <typename T, int kHd, typename Shape>
+__global__ void __launch_bounds__(Shape::kThreads) join_split_kernel(const Problem p, int tile_rows, int ctas, int by_unit) {
   pdl_trigger();
   pdl_wait();
-  const int4 c = p.cut[blockIdx.x];  // {first token, tokens, kv head, last CTA}
-  const int rows = c.y * p.G, i = blockIdx.y * kJoinRows + threadIdx.x % kJoinRows, d4 = threadIdx.x / kJoinRows;
-  if (i >= rows) return;
+  int4 c;  // {first token, tokens, kv head, last CTA}
+  Pieces w{static_cast<int>(blockIdx.x), 0, 0};
+  if (by_unit) {
+    const Line line = line_of(p, kTcChunk);
+    const int x = blockIdx.x;
+    if (x >= line.tiles * p.nkv) return;
+    const int h = x / line.tiles, ti = x - h * line.tiles;
+    const Tile t = tile_at(p, ti);
+    w = pieces_of(Cuts(p, line, ctas), h * line.chunks + line.cum(ti), h * line.chunks + line.cum(ti + 1), p.unit_extra, ctas, 0);
+    if (w.first == w.last) return;
+    c = make_int4(t.t0, t.ntok, h, w.last);
+  } else {
+    c = p.cut[blockIdx.x];
+    w.last = c.w;
+  }
+  const Shape at(blockIdx.y);
+  const int rows = c.y * p.G, i = at.row;
+  if (static_cast<int>(blockIdx.y) * Shape::kRows >= rows) return;
   Joined<T, kHd> sum;
-  sum.template add<kAhead>(p, {static_cast<int>(blockIdx.x), c.w, 0}, tile_rows, result_row(p, i / p.G, i % p.G), d4);
-  sum.store(out_row<T, kHd>(p, c.x + i / p.G, c.z * p.G + i % p.G), d4);
+  sum.add_parts(p, w, tile_rows, result_row(p, i / p.G, i % p.G), at, i < rows);
+  if (at.part == 0 && i < rows) sum.store(out_row<T, kHd>(p, c.x + i / p.G, c.z * p.G + i % p.G), at.d4);
 }
 
-// Joins the prefix's results (`a`) with those of the sequences' own positions (`b`). Block (x, h): 8 rows (token, head of
+// Joins the prefix's results (`a`) with those of the sequences' own positions (`b`). Block (x, h): rows (token, head of
 // kv head h).
-template <typename T, int kHd>
-__global__ void __launch_bounds__(kHd * 2)
-    join_prefix_kernel(const Problem a, int a_ctas, int a_rows, int a_chunk, const Problem b, int b_ctas, int b_rows) {
+template <typename T, int kHd, typename Shape>
+__global__ void __launch_bounds__(Shape::kThreads)
+    join_prefix_kernel(const Problem a, int a_ctas, const Problem b, int b_ctas, int b_rows) {
   pdl_trigger();
   pdl_wait();
-  const int d4 = threadIdx.x / kJoinRows, h = blockIdx.y;
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * kJoinRows + threadIdx.x % kJoinRows;
-  if (id >= static_cast<int64_t>(a.T) * a.G) return;
-  const int t = static_cast<int>(id) / a.G, g = static_cast<int>(id) % a.G;
-  const Line own = line_of(b, 1), line = line_of(a, a_chunk);
-  const int ti = b.mode == kRagged ? find_tile([&](int i) { return b.tile_info[i].x; }, own.tiles, t) : t;
-  const int t0 = b.mode == kRagged ? b.tile_info[ti].x : t;
-  const int b0 = h * own.chunks + own.cum(ti), b1 = h * own.chunks + own.cum(ti + 1);
-  Joined<T, kHd> sum;
+  const Shape at(blockIdx.x);
+  const int h = blockIdx.y;
+  const bool live = at.row < a.T * a.G;
+  const int t = live ? at.row / a.G : 0, g = live ? at.row % a.G : 0;
+  const Line line = line_of(a, kTcChunk);
   const int unit = h * a.n_tiles + t / a.tile_tokens, a0 = unit * line.per_tile;
-  sum.template add<8>(a, pieces_of(Cuts(a, line, a_ctas), a0, a0 + line.per_tile, a.unit_extra, a_ctas, unit), a_rows,
-                      result_row(a, t % a.tile_tokens, g), d4);
-  if (own.chunks > 0)
-    sum.template add<2>(b, pieces_of(Cuts(b, own, b_ctas), b0, b1, b.unit_extra, b_ctas, h * own.tiles + ti), b_rows,
-                        result_row(b, t - t0, g), d4);
-  sum.store(out_row<T, kHd>(b, t, h * b.G + g), d4);
+  Joined<T, kHd> sum;
+  sum.add_parts(a, pieces_of(Cuts(a, line, a_ctas), a0, a0 + line.per_tile, a.unit_extra, a_ctas, unit), kTcRows,
+                result_row(a, t % a.tile_tokens, g), at, live);
+  if (at.part > 0 || !live) return;
+  const Line own = line_of(b, 1);
+  if (own.chunks > 0) {
+    const int ti = b.mode == kRagged ? find_tile([&](int i) { return b.tile_info[i].x; }, own.tiles, t) : t;
+    const int t0 = b.mode == kRagged ? b.tile_info[ti].x : t;
+    const int b0 = h * own.chunks + own.cum(ti), b1 = h * own.chunks + own.cum(ti + 1);
+    const Pieces mine = pieces_of(Cuts(b, own, b_ctas), b0, b1, b.unit_extra, b_ctas, h * own.tiles + ti);
+    sum.template add<2>(b, mine, mine.first, mine.last, b_rows, result_row(b, t - t0, g), at.d4);
+  }
+  sum.store(out_row<T, kHd>(b, t, h * b.G + g), at.d4);
 }
 
 }  // namespace
@@ -519,6 +558,7 @@ __global__ void __launch_bounds__(kHd * 2)
 // ------------------------------------------------------------------------------------ host
 namespace {
 
+constexpr int kFewPieces = 8;     // tiles that are cut into more pieces than this, on average, are joined in parts
 constexpr int kMaxBatch = 4096;  // kOneToken: the chunk sums of a batch lie in shared memory
 
 // What a rows_kernel launch takes: slots of its ring, shared memory, and the CTAs of one wave (0: it does not fit).
@@ -558,9 +598,6 @@ struct Sizes {
   int dtype;
 };
 
-// Rows that the results of a tile of up to 16 rows take.
-int rows_of(const Sizes& z, int tokens) { return tokens * (z.nq / z.nkv) <= 8 ? 8 : 16; }
-
 RowsShape rows_shape_of(const Sizes& z, int rows) {
 #define DK_SHAPE(TT) \
   (z.hd == 128 ? (rows == 8 ? rows_shape<TT, 128, 8>() : rows_shape<TT, 128, 16>()) \
@@ -597,7 +634,7 @@ struct Pass {
   Problem p;
   bool tc;  // 256-row tiles on the tensor-core kernel
   RowsShape shape;
-  int rows, ctas, chunk;
+  int rows, ctas;
 };
 
 void cut_pass(const Sizes& z, Cutter& c, Pass& a, bool always_partial) {
@@ -607,13 +644,11 @@ void cut_pass(const Sizes& z, Cutter& c, Pass& a, bool always_partial) {
     p.unit_extra = kTcUnitExtra;
     p.rows_inner = 1;
     a.ctas = tc_ctas(z.hd, z.dtype);
-    a.chunk = kTcChunk;
   } else {
-    a.rows = rows_of(z, p.tile_tokens);
+    a.rows = z.nq / z.nkv <= 8 ? 8 : 16;
     a.shape = rows_shape_of(z, a.rows);
     a.ctas = a.shape.ctas * kGroups;
     p.unit_extra = kRowsUnitExtra;
-    a.chunk = kChunk;
   }
   const int64_t tiles = p.mode == kRagged ? p.max_tiles : p.n_tiles;
   const int64_t slots = 2ll * a.ctas + (always_partial ? z.nkv * tiles : 0);
@@ -626,26 +661,28 @@ void cut_pass(const Sizes& z, Cutter& c, Pass& a, bool always_partial) {
   p.tile_info = p.mode == kRagged ? c.take<int4>(p.max_tiles) : nullptr;
 }
 
-// Tokens of a tile: of up to 16 rows, or of two halves of up to 128 rows each.
-void set_tile(const Sizes& z, Pass& a, int tokens16) {
-  const int G = static_cast<int>(z.nq / z.nkv);
-  a.p.half_tokens = a.tc ? 128 / G : tokens16;
-  a.p.tile_tokens = a.tc ? 2 * a.p.half_tokens : tokens16;
+// Tiles of one token, or of two halves of up to 128 rows each.
+void set_tile(const Sizes& z, Pass& a, bool tc) {
+  a.tc = tc;
+  a.p.half_tokens = tc ? static_cast<int>(128 / (z.nq / z.nkv)) : 1;
+  a.p.tile_tokens = tc ? 2 * a.p.half_tokens : 1;
 }
 
+// One token for each sequence goes to the rows kernel, several to the tiles (64 sequences of 8192, 12 heads over 2 kv heads,
+// one token each, without the host: 91 us on the rows kernel, 108 as tiles; one of 640: 9.4 and 13.6; 4 tokens each as tiles:
+// 109).
 void shape_own(const Sizes& z, Pass& a) {
-  a.tc = z.ragged;
+  set_tile(z, a, z.ragged);
   a.p.mode = z.ragged ? kRagged : kOneToken;
-  set_tile(z, a, 1);
   a.p.max_tiles = z.ragged ? static_cast<int>(z.T / a.p.tile_tokens + z.B) : 0;
   a.p.n_tiles = static_cast<int>(z.B);
 }
 
+// A prefix is read by tiles however few the rows are (8192 positions for one token of 12 heads: 17 us, 29 on the rows
+// kernel).
 void shape_prefix(const Sizes& z, Pass& a) {
-  const int G = static_cast<int>(z.nq / z.nkv);
-  a.tc = z.T * G > 16;  // up to 16 rows read the prefix once on the rows kernel as well
+  set_tile(z, a, true);
   a.p.mode = kPrefix;
-  set_tile(z, a, std::max(1, 16 / G));
   a.p.n_tiles = static_cast<int>((z.T + a.p.tile_tokens - 1) / a.p.tile_tokens);
   a.p.prefix_len = static_cast<int>(z.prefix_len);
 }
@@ -654,7 +691,7 @@ void shape_prefix(const Sizes& z, Pass& a) {
 // starts on the others right away, with longer pieces there. How long the prefix's takes is known here: about 6 us and 2 us
 // for each chunk of a CTA's piece; a group of the other takes 1.1 us for a chunk.
 void share_gpu(Pass& pre, Pass& own) {
-  if (!pre.tc || own.tc || !pdl_enabled()) return;
+  if (own.tc || !pdl_enabled()) return;
   const int sms = device_info().num_sms;
   const int64_t n = static_cast<int64_t>((pre.p.prefix_len + kTcChunk - 1) / kTcChunk + pre.p.unit_extra) * pre.p.n_tiles * pre.p.nkv;
   const int64_t most = sms * 7 / 8, per = (n + most - 1) / most;
@@ -674,20 +711,38 @@ int check_sizes(const char* what, const Sizes& z) {
   if (!z.ragged && z.T != z.B) return set_error(DK_ERR_INVALID, "%s: without starts there is one token per sequence", what);
   if (!z.ragged && z.B > kMaxBatch)
     return set_error(DK_ERR_UNSUPPORTED, "%s: %lld sequences (at most %d without starts)", what, (long long)z.B, kMaxBatch);
-  if (z.T > (1 << 26) || z.B > (1 << 26) || z.nkv > 65535 || z.prefix_len > (1 << 30))
+  if (z.T * (z.nq / z.nkv) > (1 << 30) || z.T > (1 << 26) || z.B > (1 << 26) || z.nkv > 65535 || z.prefix_len > (1 << 30))
     return set_error(DK_ERR_INVALID, "%s: sizes out of range", what);
   return DK_OK;
 }
 
+template <typename Shape>
+dim3 join_grid(int64_t x, int64_t y, int64_t hd) {
+  return dim3(static_cast<unsigned>(x), static_cast<unsigned>(y), static_cast<unsigned>(hd / 4 / Shape::kDims));
+}
+
 template <typename T, int kHd>
 cudaError_t launch_join(const Sizes& z, cudaStream_t st, const Pass* prefix, const Pass& own) {
-  if (prefix == nullptr) {
-    const dim3 grid(static_cast<unsigned>(own.ctas), static_cast<unsigned>((own.rows + kJoinRows - 1) / kJoinRows));
-    return launch(own.tc ? join_split_kernel<T, kHd, 2> : join_split_kernel<T, kHd, 4>, grid, dim3(kHd * 2), 0, st, pdl_enabled(), dim3(1, 1, 1), own.p, own.rows);
+  using Tiles = JoinShape<8, kHd / 4, 1, 2>;
+  using Few = JoinShape<8, 8, 4, 4>;
+  using OneToken = JoinShape<kHd == 128 ? 2 : 4, kHd / 4, 4, 4>;
+  const dim3 one(1, 1, 1);
+  if (prefix != nullptr) {
+    const int64_t rows = z.T * (z.nq / z.nkv);
+    return launch(join_prefix_kernel<T, kHd, Few>, join_grid<Few>((rows + Few::kRows - 1) / Few::kRows, z.nkv, kHd),
+                  dim3(Few::kThreads), 0, st, pdl_enabled(), one, prefix->p, prefix->ctas, own.p, own.ctas, own.rows);
   }
-  const dim3 grid(static_cast<unsigned>((z.T * (z.nq / z.nkv) + kJoinRows - 1) / kJoinRows), static_cast<unsigned>(z.nkv));
-  return launch(join_prefix_kernel<T, kHd>, grid, dim3(kHd * 2), 0, st, pdl_enabled(), dim3(1, 1, 1), prefix->p,
-                prefix->ctas, prefix->rows, prefix->chunk, own.p, own.ctas, own.rows);
+  if (!own.tc)
+    return launch(join_split_kernel<T, kHd, OneToken>, join_grid<OneToken>(own.ctas, own.rows / OneToken::kRows, kHd),
+                  dim3(OneToken::kThreads), 0, st, pdl_enabled(), one, own.p, own.rows, own.ctas, 0);
+  const int64_t units = static_cast<int64_t>(own.p.max_tiles) * z.nkv, x = std::min<int64_t>(units, own.ctas);
+  const int64_t y = (std::min<int64_t>(z.T, own.p.tile_tokens) * (z.nq / z.nkv) + 7) / 8;
+  const int by_unit = units < own.ctas;
+  if (units * kFewPieces <= own.ctas)
+    return launch(join_split_kernel<T, kHd, Few>, join_grid<Few>(x, y, kHd), dim3(Few::kThreads), 0, st, pdl_enabled(), one,
+                  own.p, own.rows, own.ctas, by_unit);
+  return launch(join_split_kernel<T, kHd, Tiles>, join_grid<Tiles>(x, y, kHd), dim3(Tiles::kThreads), 0, st, pdl_enabled(), one,
+                own.p, own.rows, own.ctas, by_unit);
 }
 
 uint64_t workspace_of(const Sizes& z) {
@@ -753,10 +808,11 @@ int attention(const char* what, const dk_paged_attention_args* args, bool prefix
     cut_pass(z, c, pre, true);
   }
   for (const Pass* s : {&pre, &own}) {
-    if (s->chunk == 0) continue;
+    if (s == &pre && z.prefix_len == 0) continue;
+    const int64_t chunk = s->tc ? kTcChunk : kChunk;
     const int64_t tiles = s->p.mode == kRagged ? s->p.max_tiles : s->p.n_tiles;
     const int64_t positions = s->p.mode == kPrefix ? z.prefix_len : table_width * page_size;
-    if (tiles * ((positions + s->chunk - 1) / s->chunk + 1 + s->p.unit_extra) * z.nkv >= (int64_t(1) << 30))
+    if (tiles * ((positions + chunk - 1) / chunk + 1 + s->p.unit_extra) * z.nkv >= (int64_t(1) << 30))
       return set_error(DK_ERR_UNSUPPORTED, "%s: the call's work counts more than 2^30 chunks: fewer sequences or narrower page tables",
                        what);
   }
@@ -786,8 +842,7 @@ int attention(const char* what, const dk_paged_attention_args* args, bool prefix
   const uint32_t box = static_cast<uint32_t>(std::min<int64_t>(page_size, kChunk));
   const CUtensorMapDataType type = z.dtype == DK_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   CUtensorMap mk, mv;
-  const bool any_rows = !own.tc || (z.prefix_len > 0 && !pre.tc);
-  if (any_rows && (!make_tensor_map_2d(&mk, a.k_pages, type, z.hd, rows, z.hd * 2, 64, box, CU_TENSOR_MAP_SWIZZLE_128B) ||
+  if (!own.tc && (!make_tensor_map_2d(&mk, a.k_pages, type, z.hd, rows, z.hd * 2, 64, box, CU_TENSOR_MAP_SWIZZLE_128B) ||
                    !make_tensor_map_2d(&mv, a.v_pages, type, z.hd, rows, z.hd * 2, 64, box, CU_TENSOR_MAP_SWIZZLE_128B)))
     return DK_ERR_CUDA;
   cudaError_t e = cudaSuccess;

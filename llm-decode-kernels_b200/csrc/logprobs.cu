@@ -19,6 +19,7 @@
 // CTA's shared memory.
 #include <algorithm>
 #include <cfloat>
+#include <mutex>
 
 #include "paged.cuh"
 
@@ -30,6 +31,7 @@ using paged::exp2_approx;
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
+constexpr int kResident = 5;  // CTAs an SM holds (2048 rows of 152064 fp16: 124 us; 130 with 4)
 constexpr int kGroups = kThreads / 4;
 static_assert(kGroups == 64, "two maxima a lane");
 constexpr int kRaiseTile = 3;  // at this tile the threshold is taken again from all seen so far
@@ -172,7 +174,7 @@ struct Stats {
 };
 
 template <typename T, bool kTop>
-__global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const LogprobParams p) {
+__global__ void __launch_bounds__(kThreads, kResident) logprob_kernel(const LogprobParams p) {
   constexpr int kN = Vec<T>::kN;
   __shared__ uint64_t list[kTop ? kCap : 1];
   __shared__ uint64_t best[kTop ? kMaxTop : 1];                // this CTA's selection, best first
@@ -492,6 +494,31 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(const LogprobParam
   if (C > 1) cluster_sync();  // the first CTA has read the others' shared memory
 }
 
+// `per_sm`: CTAs of the launch for each SM, or 0 where most SMs stay idle anyhow. Where less than kResident are needed on
+// each, dynamic shared memory that nothing uses keeps more than that away, so that all SMs get the same (148 rows, us: 16.6,
+// 24.7 without).
+template <typename T, bool kTop>
+cudaError_t launch_logprobs(dim3 grid, int64_t per_sm, cudaStream_t st, const LogprobParams& p) {
+  static std::mutex mu;
+  static int limits[64];  // by device; 0: not asked yet
+  auto kernel = logprob_kernel<T, kTop>;
+  const DeviceInfo& device = device_info();
+  int dev = 0, limit;
+  cudaGetDevice(&dev);
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    int& known = limits[dev & 63];
+    if (known == 0) known = opt_in_dynamic_smem(kernel);
+    limit = known;
+  }
+  int64_t bytes = 0;
+  if (per_sm > 0 && per_sm < kResident) {  // per_sm + 1 shall not fit
+    const int64_t own = device.max_smem_optin - limit + 1024;  // static, and what the system takes for each CTA
+    bytes = std::max<int64_t>(0, std::min<int64_t>(limit, device.smem_per_sm / (per_sm + 1) + 128 - own));
+  }
+  return launch(kernel, grid, dim3(kThreads), static_cast<size_t>(bytes), st, pdl_enabled(), dim3(1, grid.y, 1), p);
+}
+
 }  // namespace
 }  // namespace dk
 
@@ -514,16 +541,20 @@ extern "C" int dk_token_logprobs(const void* logits, int64_t ld, int32_t dtype, 
     return set_error(DK_ERR_ALIGN, "token_logprobs: logits are not aligned to their type");
   LogprobParams p{logits, ld, targets, logprob, entropy, top_logprob, top_id, V, static_cast<int>(M), static_cast<int>(top),
                   device_info().err_word};
-  // CTAs per row: more while the rows leave SMs with less than two CTAs and a CTA keeps half a tile's worth of vectors
-  const int64_t tile = static_cast<int64_t>(kThreads) * kVecs * (dtype == DK_F32 ? 4 : 8);
+  // CTAs per row (152064 fp16 logits, us): a row is split over up to 8 CTAs while each gets an SM of its own and a tile or
+  // more (1 row: 16.3 on one, 9.8 on eight; 32 rows: 17.2 on one, 13.7 on four, 15.1 on eight), and over two while the
+  // SMs take all of them at once and each has 4 tiles or more (148 rows: 17.7 and 16.4; 592 rows: 42.8 and 52.3).
+  const int64_t tile = static_cast<int64_t>(kThreads) * kVecs * (dtype == DK_F32 ? 4 : 8), sms = device_info().num_sms;
   int C = 1;
-  while (C < kMaxCluster && M * C * 2 <= 2 * device_info().num_sms && V >= C * tile) C *= 2;
+  while (C < kMaxCluster && M * C * 2 <= sms && V >= 2 * C * tile) C *= 2;
+  if (C == 1 && M * 2 <= 4 * sms && V >= 8 * tile) C = 2;
   const dim3 grid(static_cast<unsigned>(M), static_cast<unsigned>(C));
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const int64_t per_sm = M * C * 2 > sms ? (M * C + sms - 1) / sms : 0;
   cudaError_t e;
-#define DK_LOGPROB(TT)                                                                                                \
-  e = top > 0 ? launch(logprob_kernel<TT, true>, grid, dim3(kThreads), 0, st, pdl_enabled(), dim3(1, C, 1), p)        \
-              : launch(logprob_kernel<TT, false>, grid, dim3(kThreads), 0, st, pdl_enabled(), dim3(1, C, 1), p)
+#define DK_LOGPROB(TT)                                                                                                  \
+  e = top > 0 ? launch_logprobs<TT, true>(grid, per_sm, st, p)                                                          \
+              : launch_logprobs<TT, false>(grid, per_sm, st, p)
   if (dtype == DK_F16)
     DK_LOGPROB(__half);
   else if (dtype == DK_BF16)

@@ -92,25 +92,27 @@ struct Mask {
   __device__ bool sees(int p, int j) const { return j <= p && (window <= 0 || j > p - window || j < sinks); }
 };
 
-// The chunks that the rows at positions p0..p1 of one tile need: chunk i of the unit is cache chunk
-// i (i < ns: the sinks) or w0 + i - ns. At least one chunk, so that a tile that sees nothing is still
-// visited once and gets its zeros.
+// What the rows at positions p0..p1 of one tile visit: the pages (or parts of kChunk positions of larger ones) with sinks and
+// those from the window's first one on, without the positions between. Offsets count the visited positions, chunks of
+// kChunk at a time: offset j is position j below `gap_at`, position j + shift from there on (both multiples of a page's
+// part); a row's position minus shift takes the place of its position in offsets. At least one chunk, so that a tile that
+// sees nothing is still visited once and gets its zeros.
 template <int kChunk>
 struct Span {
-  int end;  // first position after the last visible one
-  int lo;   // first position inside some row's window
-  int ns, w0, n;
-  __device__ Span(int p0, int p1, const Mask& m, int capacity) {
+  int end;  // first offset after the last visible one
+  int lo;   // first offset inside some row's window
+  int gap_at, shift, n;
+  __device__ Span(int p0, int p1, const Mask& m, int capacity, int page_size) {
+    const int part = min(page_size, kChunk);
     end = min(max(p1 + 1, 0), capacity);
     lo = m.window > 0 ? max(0, p0 - m.window + 1) : 0;
-    const int s = min(m.sinks, lo);
-    w0 = lo / kChunk;
-    ns = m.window > 0 ? (s + kChunk - 1) / kChunk : 0;
-    if (ns > 0 && ns >= w0) ns = w0 = 0;  // the sinks reach the window's first chunk: one run of chunks
-    n = max(1, ns + (end + kChunk - 1) / kChunk - w0);
+    gap_at = m.window > 0 ? (min(m.sinks, lo) + part - 1) & -part : 0;
+    shift = max(0, (lo & -part) - gap_at);
+    lo -= shift, end -= shift;
+    n = max(1, (end + kChunk - 1) / kChunk);
   }
-  __device__ int chunk(int i) const { return i < ns ? i : w0 + i - ns; }
-  // Is some position of [j, j + len) visible to some row of the tile?
+  __device__ int position(int j) const { return j < gap_at ? j : j + shift; }
+  // Is some offset of [j, j + len) visible to some row of the tile?
   __device__ bool needs(int j, int len, const Mask& m) const {
     return j < end && (m.window <= 0 || j + len > lo || j < m.sinks);
   }
@@ -293,7 +295,7 @@ struct Walk {
     u0 = x - c0;
     t = next_tile;
     last = tile_last(p, t);
-    const Span<kChunk> span(t.p0, last, p.mask, p.capacity);
+    const Span<kChunk> span(t.p0, last, p.mask, p.capacity, p.page_size);
     const int to = min(span.n + p.unit_extra, c0 + (x1 - x));
     x += to - c0;
     c1 = min(to, span.n);

@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Problem p, int
       const int4 v = info[i];  // {first token, sequence's end, length, sequence}
       const int ntok = min(p.tile_tokens, v.y - v.x), p0 = v.z - (v.y - v.x);
       info[i] = make_int4(v.x, ntok, p0, v.w);
-      n = Span<kTcChunk>(p0, p0 + ntok - 1, p.mask, p.capacity).n + p.unit_extra;
+      n = Span<kTcChunk>(p0, p0 + ntok - 1, p.mask, p.capacity, p.page_size).n + p.unit_extra;
     }
     int total;
     const int at = length + scan(n, total);
@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(kThreads)
     for (int b0 = 0; b0 < p.B; b0 += kThreads) {
       const int b = b0 + tid;
       int n = 0;
-      if (b < p.B) n = Span<kChunk>(p.lengths[b] - 1, p.lengths[b] - 1, p.mask, p.capacity).n + p.unit_extra;
+      if (b < p.B) n = Span<kChunk>(p.lengths[b] - 1, p.lengths[b] - 1, p.mask, p.capacity, p.page_size).n + p.unit_extra;
       int s = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -220,8 +220,8 @@ __global__ void __launch_bounds__(kThreads)
       const int32_t* table = walk.t.table;
       // this lane's page in chunk i of the unit; INT_MIN: none, or nothing that a row sees
       auto entry = [&](int i) {
-        const int j = span.chunk(i) * kChunk + pg * box;
-        return i < c1 && pg < boxes && span.needs(j, box, p.mask) ? table[j >> p.page_shift] : INT_MIN;
+        const int j = i * kChunk + pg * box;
+        return i < c1 && pg < boxes && span.needs(j, box, p.mask) ? table[span.position(j) >> p.page_shift] : INT_MIN;
       };
       int next = entry(c0);
       for (int i = c0; i < c1; ++i, ++fill) {
@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(kThreads)
         if (lane == 0) mbar_arrive_expect_tx(&full[s], __popc(want) * box * 128);
         __syncwarp();
         if (mine) {
-          const int j = span.chunk(i) * kChunk + pg * box;
+          const int j = span.position(i * kChunk + pg * box);
           // a page outside the pool reads as zeros (a row past the map's end)
           const int y = page >= 0 && page < p.n_pages
                             ? (page * p.nkv + h) * p.page_size + (j & (p.page_size - 1))
@@ -258,13 +258,14 @@ __global__ void __launch_bounds__(kThreads)
       const int h = walk.h, c0 = walk.c0, c1 = walk.c1;
       if (c1 <= c0) continue;
       const int rows = p.G;  // one token's
+      const int p0 = t.p0 - span.shift;
       // this lane's rows g and g + 8: positions, and q as the MMA's A operand
       int pos[kR];
       uint32_t qa[kHd / 16][2 * kR];
 #pragma unroll
       for (int e = 0; e < kR; ++e) {
         const int row = g + 8 * e;
-        pos[e] = row < rows ? t.p0 : INT_MIN;
+        pos[e] = row < rows ? p0 : -1;
         const T* qr = static_cast<const T*>(p.q) + t.t0 * p.ldq + (h * p.G + row) * kHd;
 #pragma unroll
         for (int ks = 0; ks < kHd / 16; ++ks) {
@@ -283,7 +284,7 @@ __global__ void __launch_bounds__(kThreads)
         const int s = fill % ring;
         if (ok && !wait_for(&full[s], (fill / ring) & 1, p.err, DK_DEVERR_WAIT_FULL)) ok = false;
         ok = __all_sync(0xffffffffu, ok);
-        const int j0 = span.chunk(i) * kChunk + 16 * sub;  // this warp's 16 positions
+        const int j0 = i * kChunk + 16 * sub;  // this warp's 16 positions
         if (ok && span.needs(j0, 16, p.mask)) {
           const uint8_t* kt = slots + s * B::kSlotBytes;
           const uint8_t* vt = kt + B::kTensorBytes;
@@ -298,7 +299,7 @@ __global__ void __launch_bounds__(kThreads)
             E::mma(sc[1], qa[ks][0], a1, qa[ks][kR], a3, kb[2], kb[3]);
           }
           // every row sees all 16 positions (nothing to mask)?
-          const bool clear = j0 + 15 <= t.p0 && (p.mask.window <= 0 || j0 > t.p0 - p.mask.window || j0 + 15 < p.mask.sinks) &&
+          const bool clear = j0 + 15 <= p0 && (p.mask.window <= 0 || j0 > p0 - p.mask.window || j0 + 15 < p.mask.sinks) &&
                              j0 + 15 < span.end;
           uint32_t pa[2][kR];  // p as the MMA's A operand
 #pragma unroll
@@ -338,7 +339,7 @@ __global__ void __launch_bounds__(kThreads)
             pa[1][e] = E::pack(pr[1][0], pr[1][1]);
           }
           const int vrow = 16 * sub + (mi & 1) * 8 + rr;
-          const bool zero = !clear && !span.needs(span.chunk(i) * kChunk + vrow, 1, p.mask);
+          const bool zero = !clear && !span.needs(i * kChunk + vrow, 1, p.mask);
           const uint32_t a1 = kTwo ? pa[0][kR - 1] : 0u, a3 = kTwo ? pa[1][kR - 1] : 0u;
 #pragma unroll
           for (int dp = 0; dp < kHd / 16; ++dp) {

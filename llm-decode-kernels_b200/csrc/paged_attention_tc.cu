@@ -251,8 +251,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int32_t* table = walk.t.table;
       const bool two = walk.t.ntok > p.half_tokens;
       auto entry = [&](int i) {  // this lane's page in chunk i of the unit; INT_MIN: none, or nothing that a row sees
-        const int j = span.chunk(i) * kC + pg * box;
-        return i < c1 && pg < boxes && span.needs(j, box, p.mask) ? table[j >> p.page_shift] : INT_MIN;
+        const int j = i * kC + pg * box;
+        return i < c1 && pg < boxes && span.needs(j, box, p.mask) ? table[span.position(j) >> p.page_shift] : INT_MIN;
       };
       auto put = [&](const CUtensorMap* map, int i, int page) {
         const int s = fill % L::kSlots;
@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive_expect_tx(&bar.kv_full[s], __popc(want) * box * 128);
         __syncwarp();
         if (mine) {
-          const int j = span.chunk(i) * kC + pg * box;
+          const int j = span.position(i * kC + pg * box);
           // a page outside the pool reads as zeros (a row past the map's end)
           const int y = page >= 0 && page < p.n_pages ? (page * p.nkv + h) * p.page_size + (j & (p.page_size - 1))
                                                       : p.n_pages * p.nkv * p.page_size;
@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int fv = fill + 2 * i + 1, fk = fv + 1;
         slot_wait(fv);
         if (!ok) break;
-        const int j0 = span.chunk(walk.c0 + i) * kC;
+        const int j0 = (walk.c0 + i) * kC;
         // does every row of v belong to a position that some row of the unit sees?
         const bool clear = j0 + kC <= span.end && (p.mask.window <= 0 || j0 >= span.lo || j0 + kC <= p.mask.sinks);
         if (!clear) {
@@ -398,8 +398,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (t.ntok <= first || walk.c1 <= walk.c0) continue;
       const int tok = first + r / p.G, head = walk.h * p.G + r % p.G;
       const bool live = r < p.half_tokens * p.G && tok < t.ntok;
-      const int pos = live ? row_position(p, t, tok) : -1;
-      const int p_lo = row_position(p, t, first), p_hi = row_position(p, t, min(t.ntok, first + p.half_tokens) - 1);
+      const int pos = live ? row_position(p, t, tok) - span.shift : -1;  // (in the span's offsets)
+      const int p_lo = row_position(p, t, first) - span.shift;
+      const int p_hi = row_position(p, t, min(t.ntok, first + p.half_tokens) - 1) - span.shift;
       float m = -INFINITY, l = 0.f;  // of scale2 * score
       for (int i = walk.c0; i < walk.c1; ++i) {
         if (!wait_for(&bar.s_full[x], s_seen & 1, p.err, DK_DEVERR_WAIT_FULL)) ok = false;
@@ -410,7 +411,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         float s[kC];
 #pragma unroll
         for (int c = 0; c < kC; c += 64) tmem_ld64(s_col + c, *reinterpret_cast<float(*)[64]>(&s[c]));
-        const int j0 = span.chunk(i) * kC;
+        const int j0 = i * kC;
         const bool clear = j0 + kC - 1 <= p_lo && j0 + kC <= span.end &&
                            (p.mask.window <= 0 || j0 > p_hi - p.mask.window || j0 + kC <= p.mask.sinks);
         if (!clear) {

@@ -243,6 +243,20 @@ def test_attention_windows_past_every_position(sizes):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("page", [16, 64, 128, 256])
+@pytest.mark.parametrize("sizes", [[(1, 700), (1, 101), (1, 100), (1, 3)], [(60, 700), (50, 120), (2, 100), (9, 9)]])
+def test_attention_sinks_beside_the_window(page, sizes):
+    """Sinks that end in their page, at its end, just before the window's first page, in it and beyond: the positions between
+    are skipped, not seen."""
+    from kernels.paged import paged_attention
+
+    c = Case(sizes, nq=4, nkv=2, hd=64, page=page)
+    for sinks in (0, 1, 16, 17, 64, 256, 511, 512, 513, 599, 600, 690):
+        exact, tol = c.attention(window=100, sinks=sinks)
+        assert_within(paged_attention(c.q, c.k, c.v, c.table, c.lengths, c.starts, window=100, sinks=sinks), exact, tol)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("ragged", [False, True])
 def test_one_token_of_any_stride(ragged):
     """The row stride of a single token means nothing, whatever it is."""

@@ -782,7 +782,7 @@ int attention(const char* what, const dk_paged_attention_args* args, bool prefix
   const Sizes z{a.T, a.B, a.n_q, a.n_kv, a.head_dim, prefix ? a.prefix_len : 0, a.starts != nullptr, static_cast<int>(a.dtype)};
   const int64_t n_pages = a.n_pages, page_size = a.page_size, table_width = a.table_width;
   int64_t window = prefix ? 0 : a.window;
-  const int64_t sinks = prefix ? 0 : a.sinks;
+  int64_t sinks = prefix ? 0 : a.sinks;
   if (const int rc = check_sizes(what, z)) return rc;
   if (n_pages <= 0 || table_width <= 0 || window < 0 || sinks < 0) return set_error(DK_ERR_INVALID, "%s: bad sizes", what);
   if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1)))
@@ -790,7 +790,9 @@ int attention(const char* what, const dk_paged_attention_args* args, bool prefix
   if (n_pages * z.nkv * page_size + kChunk >= (int64_t(1) << 31) || table_width * page_size >= (int64_t(1) << 31) ||
       window >= (int64_t(1) << 31) || sinks >= (int64_t(1) << 31))
     return set_error(DK_ERR_INVALID, "%s: pages x kv heads x page_size, a table row's positions, window and sinks must stay below 2^31", what);
-  window = std::min(window, table_width * page_size);  // a window of all positions or more masks none: p - window stays in range
+  // A window of all positions masks none, and sinks end with the positions: sums with them stay in range.
+  window = std::min(window, table_width * page_size);
+  sinks = std::min(sinks, table_width * page_size);
   const int64_t ldq = z.T > 1 ? a.ldq : z.nq * z.hd;
   if (z.T == 0) return DK_OK;
   if (ldq < z.nq * z.hd) return set_error(DK_ERR_INVALID, "%s: q's tokens overlap", what);

@@ -351,11 +351,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool clear = j0 + kC <= span.end && (p.mask.window <= 0 || j0 >= span.lo || j0 + kC <= p.mask.sinks);
         if (!clear) {
           uint8_t* v = slots + (fv % L::kSlots) * L::kTileBytes + (lane & 7) * 16;
-          for (int r = lane >> 3; r < kC; r += 4)  // 8 lanes a row of 64 dims
-            if (!span.needs(j0 + r, 1, p.mask))
+          auto zero = [&](int from, int to) {  // 8 lanes a row of 64 dims
+            for (int r = min(max(from, 0), kC) + (lane >> 3); r < min(to, kC); r += 4)
 #pragma unroll
               for (int c = 0; c < L::kSegs; ++c)
                 *reinterpret_cast<uint4*>(v + c * L::kSegBytes + r * 128) = make_uint4(0, 0, 0, 0);
+          };
+          zero(p.mask.sinks - j0, min(span.lo, span.end) - j0);
+          zero(span.end - j0, kC);
           tc::fence_proxy_async_smem();
           __syncwarp();
         }
@@ -421,6 +424,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int c = 0; c < kC / 32; ++c) {
             const uint32_t see = (low_bits(end - 32 * c) & ~low_bits(lo - 32 * c)) | low_bits(sinks - 32 * c);
+            if (__all_sync(0xffffffffu, see == 0xffffffffu)) continue;  // (a warp's rows are few tokens: true for most c)
 #pragma unroll
             for (int d = 0; d < 32; ++d) s[32 * c + d] = see & (1u << d) ? s[32 * c + d] : -INFINITY;
           }

@@ -468,12 +468,15 @@ struct Joined {
       }
     }
   }
-  // The same by all parts of a block, called by all of its threads (`live`: this one has a row); the first has the result.
+  // Part `part` of `parts` of a unit's pieces.
+  template <int kAhead>
+  __device__ void add_part(const Problem& p, const Pieces& w, int part, int parts, int tile_rows, int row, int d4) {
+    const int n = w.last - w.first + 1;
+    add<kAhead>(p, w, w.first + n * part / parts, w.first + n * (part + 1) / parts - 1, tile_rows, row, d4);
+  }
+  // Joins the parts of a block in order, called by all of its threads; the first has the result.
   template <typename Shape>
-  __device__ void add_parts(const Problem& p, const Pieces& w, int tile_rows, int row, const Shape& at, bool live) {
-    const int n = w.last - w.first + 1, parts = Shape::kParts;
-    if (live)
-      add<Shape::kAhead>(p, w, w.first + n * at.part / parts, w.first + n * (at.part + 1) / parts - 1, tile_rows, row, at.d4);
+  __device__ void join_parts(const Shape& at) {
     if constexpr (Shape::kParts > 1) {
       __shared__ float2 part_ml[Shape::kParts - 1][Shape::kLanes];
       __shared__ float4 part_o[Shape::kParts - 1][Shape::kLanes];
@@ -522,12 +525,14 @@ __global__ void __launch_bounds__(Shape::kThreads) join_split_kernel(const Probl
   const int rows = c.y * p.G, i = at.row;
   if (static_cast<int>(blockIdx.y) * Shape::kRows >= rows) return;
   Joined<T, kHd> sum;
-  sum.add_parts(p, w, tile_rows, result_row(p, i / p.G, i % p.G), at, i < rows);
+  if (i < rows)
+    sum.template add_part<Shape::kAhead>(p, w, at.part, Shape::kParts, tile_rows, result_row(p, i / p.G, i % p.G), at.d4);
+  sum.join_parts(at);
   if (at.part == 0 && i < rows) sum.store(out_row<T, kHd>(p, c.x + i / p.G, c.z * p.G + i % p.G), at.d4);
 }
 
 // Joins the prefix's results (`a`) with those of the sequences' own positions (`b`). Block (x, h): rows (token, head of
-// kv head h).
+// kv head h). The last part of a block takes the own positions, the others the prefix's pieces.
 template <typename T, int kHd, typename Shape>
 __global__ void __launch_bounds__(Shape::kThreads)
     join_prefix_kernel(const Problem a, int a_ctas, const Problem b, int b_ctas, int b_rows) {
@@ -537,21 +542,24 @@ __global__ void __launch_bounds__(Shape::kThreads)
   const int h = blockIdx.y;
   const bool live = at.row < a.T * a.G;
   const int t = live ? at.row / a.G : 0, g = live ? at.row % a.G : 0;
-  const Line line = line_of(a, kTcChunk);
-  const int unit = h * a.n_tiles + t / a.tile_tokens, a0 = unit * line.per_tile;
   Joined<T, kHd> sum;
-  sum.add_parts(a, pieces_of(Cuts(a, line, a_ctas), a0, a0 + line.per_tile, a.unit_extra, a_ctas, unit), kTcRows,
-                result_row(a, t % a.tile_tokens, g), at, live);
-  if (at.part > 0 || !live) return;
-  const Line own = line_of(b, 1);
-  if (own.chunks > 0) {
-    const int ti = b.mode == kRagged ? find_tile([&](int i) { return b.tile_info[i].x; }, own.tiles, t) : t;
-    const int t0 = b.mode == kRagged ? b.tile_info[ti].x : t;
-    const int b0 = h * own.chunks + own.cum(ti), b1 = h * own.chunks + own.cum(ti + 1);
-    const Pieces mine = pieces_of(Cuts(b, own, b_ctas), b0, b1, b.unit_extra, b_ctas, h * own.tiles + ti);
-    sum.template add<2>(b, mine, mine.first, mine.last, b_rows, result_row(b, t - t0, g), at.d4);
+  if (live && at.part < Shape::kParts - 1) {
+    const Line line = line_of(a, kTcChunk);
+    const int unit = h * a.n_tiles + t / a.tile_tokens, a0 = unit * line.per_tile;
+    const Pieces w = pieces_of(Cuts(a, line, a_ctas), a0, a0 + line.per_tile, a.unit_extra, a_ctas, unit);
+    sum.template add_part<Shape::kAhead>(a, w, at.part, Shape::kParts - 1, kTcRows, result_row(a, t % a.tile_tokens, g), at.d4);
+  } else if (live) {
+    const Line own = line_of(b, 1);
+    if (own.chunks > 0) {
+      const int ti = b.mode == kRagged ? find_tile([&](int i) { return b.tile_info[i].x; }, own.tiles, t) : t;
+      const int t0 = b.mode == kRagged ? b.tile_info[ti].x : t;
+      const int b0 = h * own.chunks + own.cum(ti), b1 = h * own.chunks + own.cum(ti + 1);
+      const Pieces w = pieces_of(Cuts(b, own, b_ctas), b0, b1, b.unit_extra, b_ctas, h * own.tiles + ti);
+      sum.template add<2>(b, w, w.first, w.last, b_rows, result_row(b, t - t0, g), at.d4);
+    }
   }
-  sum.store(out_row<T, kHd>(b, t, h * b.G + g), at.d4);
+  sum.join_parts(at);
+  if (at.part == 0 && live) sum.store(out_row<T, kHd>(b, t, h * b.G + g), at.d4);
 }
 
 }  // namespace

@@ -336,7 +336,7 @@ __device__ __forceinline__ int result_row(const Problem& p, int tok, int g) {
 // The launch of the 256-row tensor-core kernel (paged_attention_tc.cu): CTAs of one wave (0: it does not fit).
 constexpr int kTcChunk = 128;
 constexpr int kTcRows = 256;
-constexpr int kTcUnitExtra = 3;  // a unit's fixed cost (its Q, first and last steps, output) in chunks
+constexpr int kTcUnitExtra = 3;  // a unit's fixed cost (its Q, first and last steps, output) in chunks (2, 4: up to 2 us more)
 int tc_ctas(int64_t head_dim, int dtype);
 int tc_launch(const Problem& p, int64_t nq, int64_t head_dim, int dtype, int ctas, const void* k_pages,
               const void* v_pages, int wait_late, cudaStream_t st);

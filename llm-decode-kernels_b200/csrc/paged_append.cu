@@ -9,6 +9,8 @@
 // time (a head's 8 dims and their 8 partners a lane, or 8 dims of v), loads them before it knows where they go - the
 // token's sequence, position and page are a chain of small loads - and its angles once for all of them. With few tokens
 // a token's heads are spread over several warps.
+// Measured (36 heads of 128): 9000 tokens, 164 MB, 32 us, 78% of the copy rate (64 registers a thread, 4 CTAs an SM: with 5 or
+// 6 of them registers spill, 42 and 53 us); one token 2.3 us without the host.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -198,7 +200,9 @@ extern "C" int dk_paged_append(const dk_paged_append_args* args) {
   p.err = device_info().err_word;
   const int heads = static_cast<int>(512 / head_dim), copies = static_cast<int>(256 / head_dim);
   const int segments = static_cast<int>((nq + nkv + heads - 1) / heads + (nkv + copies - 1) / copies);
-  // Whole tokens a warp once there are 16 warps of them for every SM; fewer segments each with fewer tokens.
+  // Whole tokens a warp once there are 16 warps of them for every SM; fewer segments each with fewer tokens (36 heads of 128,
+  // us: 64 tokens 2.5, 5.6 with whole tokens; 1024 tokens 5.3, 7.6 with whole tokens, 7.3 with single segments; 4096 tokens
+  // 11.8, 21.7 with single segments).
   const int64_t want = 16ll * device_info().num_sms;
   const int per_warp = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(segments, T * segments / want)));
   const int64_t warps = T * ((segments + per_warp - 1) / per_warp);

@@ -8,7 +8,9 @@ Module map (same names as the reference's `kernels` package):
 - `kernels.rmsnorm`    fused residual + RMSNorm                           (reference kernels/rmsnorm.py)
 - `kernels.swiglu`     fused SwiGLU                                       (reference kernels/swiglu.py)
 - `kernels.cuda.w4a16_cuda`  the M <= 16 decode entry point               (reference kernels/cuda/)
-- `kernels.e2e`        Qwen2 runner with swappable backends, CUDA-graph decoder
+- `kernels.paged`      append and attention over a paged KV cache, shared prefixes (no counterpart in the reference)
+- `kernels.logprobs`   log probabilities, entropy and top alternatives of given tokens (no counterpart)
+- `kernels.e2e`        Qwen2 runner with swappable backends, CUDA-graph decoder, samples of one prompt on the paged cache
 - `kernels.bench`      CUDA-graph timing harness with rotating buffers
 
 Every op runs a kernel of `lib/libdecodek.so` through its C ABI (include/decodek.h).

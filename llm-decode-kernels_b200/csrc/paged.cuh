@@ -102,6 +102,7 @@ struct Span {
   int end;  // first offset after the last visible one
   int lo;   // first offset inside some row's window
   int gap_at, shift, n;
+  Span() = default;
   __device__ Span(int p0, int p1, const Mask& m, int capacity, int page_size) {
     const int part = min(page_size, kChunk);
     end = min(max(p1 + 1, 0), capacity);
@@ -271,6 +272,7 @@ struct Walk {
   int h, ti, c0, c1;
   int u0;  // where the unit begins
   const Cuts cuts;
+  Span<kChunk> span;  // the unit's chunks
   Tile t, next_tile;  // (the next tile's fields are loaded a part ahead)
   int last;           // the tile's last position
   __device__ Walk(const Problem& p_, const Line& line_, int cta, int ctas, int lane)
@@ -303,6 +305,14 @@ struct Walk {
     if (++next_t == line.tiles) next_t = 0, ++next_h;
     if (x < x1) next_tile = tile_at(p, next_t);
     return span;
+  }
+  // Moves to the next part that has chunks and whose tile has more than `tokens` tokens; false: there is none.
+  __device__ bool next(int tokens) {
+    while (more()) {
+      span = step();
+      if (c1 > c0 && t.ntok > tokens) return true;
+    }
+    return false;
   }
   // Does the unit begin in this part and go on in other CTAs' pieces? Then what the join needs of it.
   __device__ bool cut(const Span<kChunk>& span) const { return c0 == 0 && c1 < span.n; }

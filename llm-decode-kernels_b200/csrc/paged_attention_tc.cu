@@ -399,18 +399,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t s_col = tmem + lanes + kS[x], o_col = tmem + lanes + kO[x];
     unsigned s_seen = 0, o_seen = 0;
     if (tid == 0) p.cut[blockIdx.x] = make_int4(0, 0, 0, 0);
-    while (walk.more() && ok) {
-      const Span<kC> span = walk.step();
+    const int first = x * p.half_tokens;  // this half's first token
+    const int tok = first + r / p.G, g = r % p.G;
+    bool more_parts = walk.next(first);
+    while (more_parts && ok) {
+      const Span<kC> span = walk.span;
       const Tile t = walk.t;
-      const int first = x * p.half_tokens;  // this half's first token
-      if (t.ntok <= first || walk.c1 <= walk.c0) continue;
-      const int tok = first + r / p.G, head = walk.h * p.G + r % p.G;
+      const int c0 = walk.c0, c1 = walk.c1, head = walk.h * p.G + g;
       const bool live = r < p.half_tokens * p.G && tok < t.ntok;
       const int pos = live ? row_position(p, t, tok) - span.shift : -1;  // (in the span's offsets)
       const int p_lo = row_position(p, t, first) - span.shift;
       const int p_hi = row_position(p, t, min(t.ntok, first + p.half_tokens) - 1) - span.shift;
       float m = -INFINITY, l = 0.f;  // of scale2 * score
-      for (int i = walk.c0; i < walk.c1; ++i) {
+      for (int i = c0; i < c1; ++i) {
         if (!wait_for(&bar.s_full[x], s_seen & 1, p.err, DK_DEVERR_WAIT_FULL)) ok = false;
         ++s_seen;
         ok = __all_sync(0xffffffffu, ok);
@@ -443,7 +444,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             m = mx;
             l *= keep;
           }
-          if (i > walk.c0) {  // O's products up to the last chunk are done: S came after them
+          if (i > c0) {  // O's products up to the last chunk are done: S came after them
 #pragma unroll
             for (int c = 0; c < kHd / 16; ++c) {
               float o[16];
@@ -479,14 +480,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float2 sums = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
         l += sums.x + sums.y;
       }
+      // The next part is looked up while the last products run.
+      const bool all_of_it = c0 == 0 && c1 == span.n, whole = all_of_it && !p.always_partial;
+      const int64_t slot = partial_slot(gridDim.x, blockIdx.x, c0 == 0, all_of_it, walk.h * line.tiles + walk.ti);
+      if (ok && tid == 0 && walk.cut(span)) p.cut[blockIdx.x] = walk.cut_record(span);
+      more_parts = walk.next(first);
       if (ok && !wait_for(&bar.o_full[x], o_seen & 1, p.err, DK_DEVERR_WAIT_FULL)) ok = false;
       ++o_seen;
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc::fence_after_sync();
-      const bool all_of_it = walk.c0 == 0 && walk.c1 == span.n, whole = all_of_it && !p.always_partial;
-      const int64_t slot = partial_slot(gridDim.x, blockIdx.x, walk.c0 == 0, all_of_it, walk.h * line.tiles + walk.ti);
-      if (tid == 0 && walk.cut(span)) p.cut[blockIdx.x] = walk.cut_record(span);
       const int row = x * 128 + r;
       if (whole) {
         const float inv = l == 0.f ? 0.f : 1.f / l;

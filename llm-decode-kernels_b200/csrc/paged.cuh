@@ -348,8 +348,9 @@ constexpr int kTcChunk = 128;
 constexpr int kTcRows = 256;
 constexpr int kTcUnitExtra = 3;  // a unit's fixed cost (its Q, first and last steps, output) in chunks (2, 4: up to 2 us more)
 int tc_ctas(int64_t head_dim, int dtype);
-int tc_launch(const Problem& p, int64_t nq, int64_t head_dim, int dtype, int ctas, const void* k_pages,
-              const void* v_pages, int wait_late, cudaStream_t st);
+// mk, mv: the pages as rows of head_dim, in boxes of 64 dims of min(page_size, kTcChunk) rows, 128-byte swizzle.
+int tc_launch(const Problem& p, int64_t nq, int64_t head_dim, int dtype, int ctas, const CUtensorMap& mk,
+              const CUtensorMap& mv, int wait_late, cudaStream_t st);
 
 }  // namespace paged
 }  // namespace dk

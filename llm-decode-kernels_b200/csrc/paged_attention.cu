@@ -856,20 +856,25 @@ int attention(const char* what, const dk_paged_attention_args* args, bool prefix
 
   cudaStream_t st = reinterpret_cast<cudaStream_t>(a.stream);
   const uint64_t rows = static_cast<uint64_t>(n_pages * z.nkv * page_size);
-  const uint32_t box = static_cast<uint32_t>(std::min<int64_t>(page_size, kChunk));
   const CUtensorMapDataType type = z.dtype == DK_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   CUtensorMap mk, mv;
-  if (!own.tc && (!make_tensor_map_2d(&mk, a.k_pages, type, z.hd, rows, z.hd * 2, 64, box, CU_TENSOR_MAP_SWIZZLE_128B) ||
-                   !make_tensor_map_2d(&mv, a.v_pages, type, z.hd, rows, z.hd * 2, 64, box, CU_TENSOR_MAP_SWIZZLE_128B)))
-    return DK_ERR_CUDA;
+  uint32_t box = 0;
+  auto page_maps = [&](int chunk) {  // in boxes of a page, or of a chunk's positions of one (0.3 us each, so not made twice)
+    const uint32_t want = static_cast<uint32_t>(std::min<int64_t>(page_size, chunk));
+    if (want == box) return true;
+    box = want;
+    return make_tensor_map_2d(&mk, a.k_pages, type, z.hd, rows, z.hd * 2, 64, box, CU_TENSOR_MAP_SWIZZLE_128B) &&
+           make_tensor_map_2d(&mv, a.v_pages, type, z.hd, rows, z.hd * 2, 64, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  };
   cudaError_t e = cudaSuccess;
   if (z.ragged)
     e = launch(plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, pdl_enabled(), dim3(1, 1, 1), own.p,
                const_cast<int32_t*>(own.p.plan), const_cast<int4*>(own.p.tile_info));
   for (const Pass* s : {&pre, &own}) {
     if (s->ctas == 0 || e != cudaSuccess) continue;
+    if (!page_maps(s->tc ? kTcChunk : kChunk)) return DK_ERR_CUDA;
     if (s->tc) {
-      if (const int rc = tc_launch(s->p, z.nq, z.hd, z.dtype, s->ctas, a.k_pages, a.v_pages, s == &own ? beside : 0, st)) return rc;
+      if (const int rc = tc_launch(s->p, z.nq, z.hd, z.dtype, s->ctas, mk, mv, s == &own ? beside : 0, st)) return rc;
     } else {
       e = launch_rows(z, s->rows, s->shape, st, mk, mv, s->p, s == &own ? beside : 0);
     }

@@ -592,16 +592,11 @@ int tc_ctas(int64_t head_dim, int dtype) {
   return head_dim == 128 ? ctas_of<__nv_bfloat16, 128>() : ctas_of<__nv_bfloat16, 64>();
 }
 
-int tc_launch(const Problem& p, int64_t nq, int64_t hd, int dtype, int ctas, const void* k_pages, const void* v_pages,
+int tc_launch(const Problem& p, int64_t nq, int64_t hd, int dtype, int ctas, const CUtensorMap& mk, const CUtensorMap& mv,
               int wait_late, cudaStream_t st) {
   const CUtensorMapDataType type = dtype == DK_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  const uint64_t rows = static_cast<uint64_t>(p.n_pages) * p.nkv * p.page_size;
-  const uint32_t box = static_cast<uint32_t>(p.page_size < kC ? p.page_size : kC);
-  CUtensorMap mq, mk, mv;
-  if (!make_q_map(&mq, p, nq, hd, type) ||
-      !make_tensor_map_2d(&mk, k_pages, type, hd, rows, hd * 2, 64, box, CU_TENSOR_MAP_SWIZZLE_128B) ||
-      !make_tensor_map_2d(&mv, v_pages, type, hd, rows, hd * 2, 64, box, CU_TENSOR_MAP_SWIZZLE_128B))
-    return DK_ERR_CUDA;
+  CUtensorMap mq;
+  if (!make_q_map(&mq, p, nq, hd, type)) return DK_ERR_CUDA;
   cudaError_t e;
 #define DK_TILES(TT, HH) \
   launch(tiles_kernel<TT, HH>, dim3(ctas), dim3(kThreads), Smem<HH>::kBytes, st, pdl_enabled(), dim3(1, 1, 1), mq, mk, mv, p, wait_late)

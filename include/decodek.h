@@ -277,9 +277,9 @@ typedef struct dk_paged_append_args {
   dk_stream_t stream;
 } dk_paged_append_args;
 int dk_paged_append(const dk_paged_append_args* args);
-/* Attention over the pages: q [T, n_q, head_dim] (tokens ldq apart, heads head_dim apart) -> out [T, n_q,
- * head_dim] contiguous. The row at own position p sees the positions j <= p, and with window > 0 of those only
- * j > p - window and j < sinks; softmax(scale * q k^T) v over them, zero where there are none. Pages that no row
+/* Attention over the pages: q [T, n_q, head_dim] (tokens ldq >= n_q * head_dim apart, heads head_dim apart) -> out [T, n_q,
+ * head_dim] contiguous. The row at own position p sees the positions j <= p, and with window > 0 of those only the ones
+ * with j > p - window or j < sinks; softmax(scale * q k^T) v over them, zero where there are none. Pages that no row
  * of the call sees are not read and may be freed: their table entries may hold anything. What a page holds
  * past its sequence's last position is not used. The workspace (dk_paged_attention_workspace_bytes of the same
  * sizes, 256-byte aligned) needs no initialization and keeps nothing between calls. */

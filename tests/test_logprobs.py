@@ -50,6 +50,16 @@ def test_logprobs(M, V, top, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("M,V", [(20, 70001), (60, 70001), (100, 66001), (200, 66001), (400, 9001), (700, 9001)])
+def test_rows_over_the_sms(M, V, dtype):
+    """Rows split over four CTAs, over two on one SM or on several, whole rows with and without room to spare on the SMs."""
+    g = torch.Generator().manual_seed(M)
+    x = (torch.randn(M, V, generator=g) * 2).to(dtype).cuda()
+    _check(x, torch.randint(0, V, (M,), generator=g).cuda(), 4)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
 def test_ties_masks_and_orders(dtype):
     """Equal logits, rising and falling rows, all but a few tokens forbidden (-inf or the type's lowest value)."""

@@ -257,6 +257,23 @@ def test_attention_sinks_beside_the_window(page, sizes):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,hd", [(torch.float16, 64), (torch.bfloat16, 128)])
+@pytest.mark.parametrize("sizes,prefix", [([(1, 9000)], 0), ([(5, 9000)], 0), ([(3, 5000), (70, 6000), (1, 40)], 0),
+                                          ([(1, 3), (1, 700)], 9000), ([(4, 9), (30, 2000)], 5001)])
+def test_units_cut_into_many_pieces(sizes, prefix, dtype, hd):
+    """Few rows over long caches: every CTA works on the same units, whose many partial results are joined in parts."""
+    from kernels.paged import paged_attention, shared_prefix_attention
+
+    c = Case(sizes, nq=6, nkv=2, hd=hd, page=32, dtype=dtype, prefix=prefix)
+    exact, tol = c.attention()
+    if prefix:
+        got = shared_prefix_attention(c.q, c.k, c.v, c.prefix_table, prefix, c.table, c.lengths, c.starts)
+    else:
+        got = paged_attention(c.q, c.k, c.v, c.table, c.lengths, c.starts)
+    assert_within(got, exact, tol)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("ragged", [False, True])
 def test_one_token_of_any_stride(ragged):
     """The row stride of a single token means nothing, whatever it is."""

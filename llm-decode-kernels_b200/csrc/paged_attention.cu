@@ -554,10 +554,11 @@ __global__ void __launch_bounds__(Shape::kThreads)
     const Line own = line_of(b, 1);
     if (own.chunks > 0) {
       const int ti = b.mode == kRagged ? find_tile([&](int i) { return b.tile_info[i].x; }, own.tiles, t) : t;
-      const int t0 = b.mode == kRagged ? b.tile_info[ti].x : t;
+      const Tile tile = tile_at(b, ti);
+      const int tok = t - tile.t0;  // (a row that `starts` leaves out belongs to no tile)
       const int b0 = h * own.chunks + own.cum(ti), b1 = h * own.chunks + own.cum(ti + 1);
       const Pieces w = pieces_of(Cuts(b, own, b_ctas), b0, b1, b.unit_extra, b_ctas, h * own.tiles + ti);
-      sum.template add<2>(b, w, w.first, w.last, b_rows, result_row(b, t - t0, g), at.d4);
+      if (tok >= 0 && tok < tile.ntok) sum.template add<2>(b, w, w.first, w.last, b_rows, result_row(b, tok, g), at.d4);
     }
   }
   sum.join_parts(at);

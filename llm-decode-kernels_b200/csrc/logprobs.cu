@@ -226,12 +226,15 @@ __global__ void __launch_bounds__(kThreads, kResident) logprob_kernel(const Logp
 
   float base = kLow, thr = -FLT_MAX;
   float run = -INFINITY;  // the largest logit this thread has seen (NaN: the largest, as in order_key)
-  // Raises the threshold to the top-th largest of the maxima that 64 groups of four threads have seen; all threads.
+  // Raises the threshold to the top-th largest of the maxima that 64 groups of four threads have seen; all threads. Returns
+  // this lane's part of the largest of them, read before the second barrier: after it a warp ahead of the others may
+  // already write the next round's maxima.
   auto raise_threshold = [&] {
     float group = max_nan(run, __shfl_xor_sync(0xffffffffu, run, 1));
     group = max_nan(group, __shfl_xor_sync(0xffffffffu, group, 2));
     if ((lane & 3) == 0) first_max[tid >> 2] = group;
     __syncthreads();
+    const float top_max = fmaxf(first_max[lane], first_max[lane + 32]);
     if (kTop && tid < kGroups) {
       const float me = first_max[tid];
       int above = 0, reach = 0;
@@ -243,6 +246,7 @@ __global__ void __launch_bounds__(kThreads, kResident) logprob_kernel(const Logp
     }
     __syncthreads();
     if (kTop) thr = fmaxf(thr_sh, -FLT_MAX);  // (-inf is below any threshold)
+    return top_max;
   };
 
   float2 s2 = make_float2(0.f, 0.f), w2 = s2;
@@ -261,8 +265,7 @@ __global__ void __launch_bounds__(kThreads, kResident) logprob_kernel(const Logp
     const float mine = max_nan(max_nan(vmax[0], vmax[1]), max_nan(vmax[2], vmax[3]));
     run = max_nan(run, mine);
     if (tile == 0) {
-      raise_threshold();
-      float top_max = fmaxf(first_max[lane], first_max[lane + 32]);
+      float top_max = raise_threshold();
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) top_max = fmaxf(top_max, __shfl_xor_sync(0xffffffffu, top_max, o));
       low = !(top_max > Vec<T>::lowest());

@@ -134,3 +134,55 @@ def test_refusals_without_a_gpu():
     assert h.dk_token_logprobs(None, 49, 0, None, 2, 50, 0, None, None, None, None, None) == -1
     assert h.dk_token_logprobs(None, 50, 0, None, 2, 50, 33, None, None, None, None, None) == -3
     assert h.dk_token_logprobs(None, 50, 7, None, 2, 50, 0, None, None, None, None, None) == -3
+
+
+def _shared_accesses(warps, rounds, inside):
+    """What the warps of logprobs.cu do with the groups' maxima: [(barriers passed, warp, 'r' or 'w', group)]. Every round a warp
+    writes its 8 groups, waits, reads them for the threshold (the first two warps), waits; in the first one all warps
+    read the largest too, before the second barrier (`inside`) or after it."""
+    got = []
+    for w in range(warps):
+        at = 0
+        for i in range(rounds):
+            got += [(at, w, "w", 8 * w + g) for g in range(8)]
+            at += 1
+            if w < 2 or (inside and i == 0):
+                got += [(at, w, "r", g) for g in range(8 * warps)]
+            at += 1
+            if not inside and i == 0:
+                got += [(at, w, "r", g) for g in range(8 * warps)]
+    return got
+
+
+def _races(accesses):
+    wrote = {}
+    for at, w, kind, g in accesses:
+        if kind == "w":
+            wrote.setdefault((at, g), set()).add(w)
+    return [(at, w, g) for at, w, kind, g in accesses if kind == "r" and wrote.get((at, g), set()) - {w}]
+
+
+@pytest.mark.parametrize("rounds", [1, 2, 3])
+def test_threshold_rounds_do_not_race(rounds):
+    """No warp reads a group's maximum between the same barriers as another warp writes it; the same reads after the second
+    barrier would, from two rounds on."""
+    assert not _races(_shared_accesses(8, rounds, inside=True))
+    assert bool(_races(_shared_accesses(8, rounds, inside=False))) == (rounds > 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,V", [(1, 151936), (300, 20011), (600, 70001)])
+def test_calls_repeat_bit_for_bit(M, V):
+    """Logits that rise along the row, so that the maxima of later rounds differ from the first's: call after call gives the
+    same bits."""
+    from kernels.logprobs import token_logprobs
+
+    g = torch.Generator().manual_seed(M)
+    x = (torch.randn(M, V, generator=g) + torch.arange(V) * (30 / V)).half().cuda()
+    targets = torch.randint(0, V, (M,), generator=g).cuda()
+    want = token_logprobs(x, targets, 5)
+    same = torch.ones((), dtype=torch.bool, device="cuda")
+    for _ in range(50):
+        for a, b in zip(token_logprobs(x, targets, 5), want):
+            same &= (a == b).all()
+    assert same.item()

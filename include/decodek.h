@@ -315,7 +315,8 @@ int dk_shared_prefix_attention(const dk_paged_attention_args* args);
  * logits [M, V] (rows ld apart; DK_F16, DK_BF16 or DK_F32) in one pass: logprob[m] = x[t] - logsumexp(x) of the target
  * t = targets[m] (device int64; t < 0: no token, 0; t >= V: NaN and DK_DEVERR_BAD_TOKEN), entropy[m] in nats (a logit of
  * -inf adds 0), and the top <= 32 largest logits of each row, best first, ties to the lowest index, as top_logprob
- * [M, top] and top_id [M, top] (int64). fp32 sums. A row with NaN or +inf, or all -inf, has NaN log probabilities. */
+ * [M, top] and top_id [M, top] (int64). fp32 sums, in which a logit below -1e30 (the type's lowest value in a mask) counts as
+ * -1e30. A row with NaN or +inf, or all -inf, has NaN log probabilities. */
 int dk_token_logprobs(const void* logits, int64_t ld, int32_t dtype, const int64_t* targets, int64_t M, int64_t V,
                       int64_t top, float* logprob, float* entropy, float* top_logprob, int64_t* top_id,
                       dk_stream_t stream);

@@ -42,7 +42,9 @@ constexpr int kMaxTop = 32;
 constexpr int kMaxCluster = 8;
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kRoom = 40.f;
-constexpr float kLow = -1e30f;   // logits below it (the type's lowest value in masks) count as this
+// Logits below it (the type's lowest value in masks) count as this: just below -1e30, a value of bf16, so that elements
+// clamped in any type and the least base are the same number.
+constexpr float kLow = -0x1.94p99f;
 
 struct LogprobParams {
   const void* logits;
@@ -123,18 +125,18 @@ struct Vec {
     return make_uint4(w, w, w, w);
   }
   // What stands for -inf in sums, so that 0 * y is 0 for it.
-  __device__ static constexpr float lowest() { return std::is_same<T, __half>::value ? -65504.f : -1e30f; }
+  __device__ static constexpr float lowest() { return std::is_same<T, __half>::value ? -65504.f : kLow; }
   __device__ float2 finite_pair(int i) const {
     if constexpr (sizeof(T) == 4) {
       const float2 f = pair(i);
-      return make_float2(max_nan(f.x, -1e30f), max_nan(f.y, -1e30f));
+      return make_float2(max_nan(f.x, kLow), max_nan(f.y, kLow));
     } else if constexpr (std::is_same<T, __half>::value) {
       uint32_t m;
       asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(m) : "r"(word(i)), "r"(0xfbfffbffu));  // -65504
       return Elem<T>::unpack(m);
     } else {
       uint32_t m;
-      asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(m) : "r"(word(i)), "r"(0xf14af14au));  // just below -1e30
+      asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(m) : "r"(word(i)), "r"(0xf14af14au));  // kLow twice
       return Elem<T>::unpack(m);
     }
   }
@@ -322,7 +324,7 @@ __global__ void __launch_bounds__(kThreads, kResident) logprob_kernel(const Logp
     if (v0 < v1 && (v < f0 || v >= f1) && (tid < kN || v > v0) && !outside(v, tid % kN)) {
       const float f = to_float(x[v * kN - skip + tid % kN]);
       if (f != -INFINITY) {
-        st.join(f, 1.f, 0.f);
+        st.join(max_nan(f, kLow), 1.f, 0.f);
         if (f != f) st.s = f;
         run = max_nan(run, f);
         if constexpr (kTop)

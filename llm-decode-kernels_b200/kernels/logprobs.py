@@ -17,7 +17,8 @@ def token_logprobs(logits, targets, top=0):
     [M] of the targets, entropy fp32 [M] in nats, top_logprobs fp32 [M, top], top_ids int64 [M, top]: the `top` <= 32
     largest logits of each row, best first, ties to the lowest index). A negative target stands for no token: its log
     probability is 0. A target >= V gives NaN and sets the device error DK_DEVERR_BAD_TOKEN. Logits of -inf are tokens
-    that cannot occur; a row with a NaN or +inf, or nothing but -inf, has NaN log probabilities."""
+    that cannot occur, logits below -1e30 (the type's lowest value in a mask) count as -1e30; a row with a NaN or +inf, or
+    nothing but -inf, has NaN log probabilities."""
     what = "token_logprobs"
     if logits.dim() != 2 or logits.shape[1] == 0:
         raise ValueError(f"{what}: logits must be [rows, vocab]")

@@ -186,3 +186,19 @@ def test_calls_repeat_bit_for_bit(M, V):
         for a, b in zip(token_logprobs(x, targets, 5), want):
             same &= (a == b).all()
     assert same.item()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V,top", [(1, 0), (3, 0), (3, 3), (7, 2), (20, 0), (40000, 0), (40000, 5)])
+def test_rows_of_the_lowest_value(V, top, dtype):
+    """Rows of nothing but the type's lowest value (a mask added to all tokens), of that and -inf, of that and one ordinary
+    logit: short rows without a whole vector, ends outside whole vectors, and rows of many tiles."""
+    low = torch.finfo(dtype).min
+    rows = torch.full((3, V + 1), low)
+    rows[1, 2::3] = -math.inf
+    rows[2, 1] = 0.5
+    x = rows.to(dtype).cuda()
+    for view in (x[:, :V], x[:, 1:]):  # the second one begins off a vector's boundary
+        for target in (0, V - 1):
+            _check(view, torch.where(view[:, target] == -math.inf, -1, target), top)

@@ -202,3 +202,21 @@ def test_rows_of_the_lowest_value(V, top, dtype):
     for view in (x[:, :V], x[:, 1:]):  # the second one begins off a vector's boundary
         for target in (0, V - 1):
             _check(view, torch.where(view[:, target] == -math.inf, -1, target), top)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V,at", [(3000, 200), (3, 2), (40001, 40000), (40001, 0), (160001, 30000)])
+def test_infinity_and_nan_give_nan(V, at, dtype):
+    """A row with +inf or NaN anywhere has NaN log probabilities, of its finite tokens and of the infinite one, and entropy."""
+    from kernels.logprobs import token_logprobs
+
+    for bad in (math.inf, math.nan):
+        x = torch.randn(2, V + 1, device="cuda").to(dtype)
+        x[:, at] = bad
+        for view in (x[:, :V], x[:1, :V]):
+            for target in (at, (at + 1) % V):
+                for top in (0, 2):
+                    lp, entropy, value, index = token_logprobs(view, torch.full((len(view),), target, device="cuda"), top)
+                    assert lp.isnan().all() and entropy.isnan().all() and value.isnan().all()
+                    assert (index[:, :1] == at).all()

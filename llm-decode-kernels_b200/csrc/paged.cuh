@@ -138,7 +138,8 @@ struct Problem {
   int n_pages, page_size, page_shift, capacity;  // capacity: positions a table row can hold
   int prefix_len;
   Mask mask;
-  float scale2;  // scale * log2(e)
+  float scale2;  // scale * log2(e); tiles_kernel: a positive one, with the sign in `signs`
+  int signs;     // tiles_kernel: what Q is multiplied by in the products with K, -1, 0 or 1
   int mode;
   int tile_tokens;
   int half_tokens;  // tokens of 128 rows (tiles_kernel); 1 (rows_kernel)

@@ -852,6 +852,12 @@ int attention(const char* what, const dk_paged_attention_args* args, bool prefix
     p->scale2 = static_cast<float>(a.scale * 1.44269504088896341);
     p->err = device_info().err_word;
   }
+  for (Pass* s : {&own, &pre}) {  // the tiles take the scale's sign apart from it
+    if (!s->tc) continue;
+    const float scale2 = s->p.scale2;
+    s->p.signs = scale2 < 0.f ? -1 : scale2 == 0.f ? 0 : 1;
+    s->p.scale2 = scale2 < 0.f ? -scale2 : scale2 == 0.f ? 1.f : scale2;
+  }
   pre.p.table = a.prefix_table, pre.p.capacity = static_cast<int>(z.prefix_len), pre.p.mask = Mask{0, 0};
   if (z.prefix_len > 0) share_gpu(pre, own);
 

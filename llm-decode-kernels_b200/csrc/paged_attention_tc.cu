@@ -13,6 +13,8 @@
 // * warps 0-3 and 4-7 are the softmax of A and B, a thread per row: S from tensor memory, the row maximum, P = 2^(S - m) in
 //   16 bits back to tensor memory. The maximum that P refers to is raised only when a row's grows by 2^8 or more; then
 //   the row of O is rescaled in tensor memory (P stays below 2^8, far inside fp16; sums are fp32).
+// The maximum and -inf for a masked score come before the scale, so it has to be positive there: of a negative one the products
+// negate Q, and of zero they get a Q of zeros.
 // V rows that no row of the unit sees (past the end, between sinks and window, pages that were not read) are zeroed in
 // shared memory before the product, so that P = 0 does not meet a NaN; masked scores are replaced before the maximum.
 // Every wait is bounded.
@@ -76,6 +78,8 @@ __host__ __device__ constexpr uint32_t idesc(int M, int N, bool b_n_major) {
   return (1u << 4) | (type << 7) | (type << 10) | (b_n_major ? 1u << 16 : 0u) | (static_cast<uint32_t>(N >> 3) << 17) |
          (static_cast<uint32_t>(M >> 4) << 24);
 }
+
+constexpr uint32_t kNegateA = 1u << 13;
 
 // The products are issued by whole warps with one lane elected inside the instruction sequence: the operands stay
 // warp-uniform values, where a branch on the lane would make each of them a value of one thread (and a product took
@@ -288,7 +292,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int x = 0; x < (two ? 2 : 1); ++x)
           for (int s = 0; s < L::kSegs; ++s)
             tma_load_3d(q_sm + x * L::kTileBytes + s * L::kSegBytes, &mq, s * 64, h * p.G,
-                        walk.t.t0 + x * p.half_tokens, &bar.q_full);
+                        p.signs == 0 ? p.T : walk.t.t0 + x * p.half_tokens, &bar.q_full);  // (past the end: zeros)
       }
       __syncwarp();
       put(&mk, c0, page);
@@ -303,6 +307,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---------------------------------------------------------------- products
     int fill = 0;         // ring slots consumed
     unsigned p_seen[2] = {0, 0};
+    const uint32_t qk_desc = idesc<T>(128, kC, false) | (p.signs < 0 ? kNegateA : 0u);
     auto slot_wait = [&](int f) {
       if (ok && !wait_for(&bar.kv_full[f % L::kSlots], (f / L::kSlots) & 1, p.err, DK_DEVERR_WAIT_FULL)) ok = false;
       ok = __all_sync(0xffffffffu, ok);
@@ -313,7 +318,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int k = 0; k < kHd / 16; ++k) {
         const uint32_t off = ((k / 4) * L::kSegBytes + (k % 4) * 32) >> 4;  // (descriptors count 16 bytes)
-        mma_ss(tmem + kS[x], a + off, b + off, idesc<T>(128, kC, false), k > 0);
+        mma_ss(tmem + kS[x], a + off, b + off, qk_desc, k > 0);
       }
       commit_elected(&bar.s_full[x]);
     };

@@ -169,8 +169,8 @@ def _attend(what, entry, q, k_pages, v_pages, prefix_table, prefix_len, page_tab
 def paged_attention(q, k_pages, v_pages, page_table, lengths, starts=None, window=0, sinks=0, scale=None, out=None):
     """Attention of q [T, n_heads, head_dim] (tokens any stride apart) over the pages: the row at position p sees the
     positions j <= p of its sequence, with window > 0 only those with j > p - window or j < sinks. Returns [T,
-    n_heads, head_dim] contiguous (`out` if given); a row that sees nothing is zero. scale: head_dim ** -0.5 if
-    None. Pages that no row sees are not read, and their table entries may hold anything. With several tokens of a
+    n_heads, head_dim] contiguous (`out` if given); a row that sees nothing is zero. scale: any number,
+    head_dim ** -0.5 if None. Pages that no row sees are not read, and their table entries may hold anything. With several tokens of a
     sequence in one call, the keys and values that one of them sees have to be finite for the others too."""
     if window < 0 or sinks < 0:
         _refuse("paged_attention", "window and sinks must not be negative")

@@ -419,3 +419,24 @@ def test_c_entries_refuse_without_a_gpu():
     assert h.dk_paged_attention_workspace_bytes(2, 2, 12, 2, 96, 0, 0, 0, ctypes.byref(n)) == -3
     assert append(16) == -1 and b"one token" in h.dk_last_error()
     assert append(20) == -3 and b"page_size" in h.dk_last_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,hd", [(F16, 128), (BF16, 128), (BF16, 64)])
+@pytest.mark.parametrize("scale", [0.0, -0.15, 1e-60])
+@pytest.mark.parametrize("sizes,prefix,window,sinks", [
+    ([(1, 200), (1, 3)], 0, 0, 0), ([(60, 300), (9, 9), (4, 2)], 0, 0, 0), ([(140, 400), (1, 90)], 0, 50, 3),
+    ([(1, 70), (1, 0)], 200, 0, 0), ([(5, 30), (50, 60)], 333, 0, 0),
+])
+def test_scale_of_any_sign(sizes, prefix, window, sinks, scale, dtype, hd):
+    """A scale of zero weighs the visible positions alike, a negative one the smallest products most (1e-60 is zero in fp32);
+    masked positions stay out of it. One token each, ragged rows and a shared prefix run different kernels."""
+    from kernels.paged import paged_attention, shared_prefix_attention
+
+    c = Case(sizes, nq=6, nkv=2, hd=hd, page=32, dtype=dtype, prefix=prefix, seed=10)
+    exact, tol = c.attention(window, sinks, scale=scale)
+    if prefix:
+        got = shared_prefix_attention(c.q, c.k, c.v, c.prefix_table, prefix, c.table, c.lengths, c.starts, scale=scale)
+    else:
+        got = paged_attention(c.q, c.k, c.v, c.table, c.lengths, c.starts, window=window, sinks=sinks, scale=scale)
+    assert_within(got, exact, tol)

@@ -244,7 +244,8 @@ int dk_embed_tokens(const int64_t* tokens, const void* embed, int64_t vocab, int
  * values; row b of page_table (int32, rows ld_table apart, table_width entries each) lists the pages of
  * sequence b in order. lengths[b] (int32) counts the positions of sequence b with the tokens of this call;
  * starts (int32 [B + 1], or NULL) gives the rows starts[b] .. starts[b+1] of the T tokens that belong to
- * sequence b (starts[0] = 0, starts[B] = T), its last positions; NULL means one token per sequence (T = B).
+ * sequence b, its last positions; NULL means one token per sequence (T = B). Rows before starts[0] and from starts[B] on belong
+ * to no sequence (a captured call may have more rows than a step needs).
  * All of these are device pointers read on the device, so one captured launch serves every step.
  * page_size: a power of two from 16 to 256; head_dim 64 or 128; n_q a multiple of n_kv, at most 16 query heads
  * per kv head (attention). A length <= 0 marks an unused slot of the batch. Every launch may be captured. */
@@ -256,8 +257,8 @@ int dk_embed_tokens(const int64_t* tokens, const void* embed, int64_t vocab, int
  * half = head_dim / 2: x'[d] = x[d] cos[a][d] - x[d+half] sin[a][d], x'[d+half] = x[d+half] cos[a][d] +
  * x[d] sin[a][d], a = p + rope_offset, computed in fp32 and rounded once. cos and sin are [rope_rows, half]
  * (rows ld_rope apart), fp32 with rope_f32 != 0, otherwise of the cache's type. Rotated q -> q_out [T, n_q,
- * head_dim], rotated k and v -> position p of the sequence's pages. A token of an unused slot appends nothing and
- * its q_out row is zero; a position without a page in the pool, or an angle outside the tables, appends
+ * head_dim], rotated k and v -> position p of the sequence's pages. A token of an unused slot or of no sequence appends
+ * nothing and its q_out row is zero; a position without a page in the pool, or an angle outside the tables, appends
  * nothing and sets DK_DEVERR_BAD_POSITION. */
 typedef struct dk_paged_append_args {
   const void* qkv;

@@ -108,9 +108,10 @@ __global__ void __launch_bounds__(kWarps * 32, 4) paged_append_kernel(const Appe
       pos = p.lengths[t] - 1;
     } else {
       b = find_tile_warp([&](int j) { return p.starts[j]; }, p.B, t, lane);
-      pos = p.lengths[b] - (p.starts[b + 1] - t);
+      const int end = p.starts[b + 1];
+      pos = t >= p.starts[b] && t < end ? p.lengths[b] - (end - t) : -1;
     }
-    // A sequence without positions (an unused slot of the batch) appends nothing; its q is zero.
+    // A row of no sequence, or of one without positions (an unused slot of the batch), appends nothing; its q is zero.
     const int64_t angle = pos + p.rope_offset;
     const bool live = pos >= 0, turns = live && angle >= 0 && angle < p.rope_rows;
     const int at = pos >> p.page_shift;

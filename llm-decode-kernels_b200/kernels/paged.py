@@ -4,7 +4,8 @@ A cache is two pools of pages, `k_pages` and `v_pages` [n_pages, n_kv, page_size
 int32 `page_table` [B, width] whose row b lists the pages of sequence b in order. `lengths` (int32 [B]) counts
 each sequence's positions including the call's own tokens; `starts` (int32 [B + 1]) gives the token rows
 starts[b]..starts[b+1] of sequence b, its last positions, or None: one token per sequence. All of them live on the
-device and are read there, so a captured call serves every step. A length <= 0 marks an unused slot of the batch.
+device and are read there, so a captured call serves every step. A length <= 0 marks an unused slot of the batch; rows
+before starts[0] and from starts[B] on belong to no sequence.
 
 `paged_append` rotates q and k by their positions and writes k and v into the pages; `paged_attention` attends
 causally over the pages, optionally limited to a sliding window and a few first tokens (sinks);
@@ -85,7 +86,7 @@ def paged_append(qkv, k_pages, v_pages, page_table, lengths, cos, sin, n_heads, 
     per pair of dims d, d + head_dim / 2, fp32 or qkv's type, rows taken at the own position + offset (the length
     of a shared prefix). The rotation is computed in fp32 and rounded once. Returns the rotated q [T, n_heads,
     head_dim] (`out` if given). A token without a page, or past the tables, appends nothing and sets the device error
-    DK_DEVERR_BAD_POSITION; one of an unused slot appends nothing and returns zeros."""
+    DK_DEVERR_BAD_POSITION; one of an unused slot or of no sequence appends nothing and returns zeros."""
     what = "paged_append"
     if qkv.dim() != 2:
         _refuse(what, "qkv must be [tokens, (n_heads + 2 n_kv) * head_dim]")

@@ -440,3 +440,27 @@ def test_scale_of_any_sign(sizes, prefix, window, sinks, scale, dtype, hd):
     else:
         got = paged_attention(c.q, c.k, c.v, c.table, c.lengths, c.starts, window=window, sinks=sinks, scale=scale)
     assert_within(got, exact, tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("before,after", [(0, 4), (2, 0), (1, 3)])
+def test_append_rows_outside_starts(before, after):
+    """Rows before starts[0] and from starts[B] on (a captured call of more rows than the step has) belong to no sequence: they
+    append nothing and their q is zero, whatever the last slot's table row lists."""
+    from kernels import _lib
+    from kernels.paged import paged_append
+
+    sizes = [(3, 20), (2, 40), (1, 0)]
+    c = Case(sizes, nkv=2, spoil=False)
+    c.table[2] = c.table[0]  # an unused slot with another sequence's pages still in its row
+    c.table[:, 2:] = c.table[1, 0]
+    cos, sin = _rope(200, 128)
+    qkv = torch.randn(before + c.T + after, 16 * 128, device="cuda").half()
+    want_k, want_v = c.k.clone(), c.v.clone()
+    want = paged_append(qkv[before:before + c.T].contiguous(), want_k, want_v, c.table, c.lengths, cos, sin, 12, 2, starts=c.starts)
+    _lib.clear_device_error()
+    q = paged_append(qkv, c.k, c.v, c.table, c.lengths, cos, sin, 12, 2, starts=c.starts + before)
+    assert _lib.device_error() == 0
+    assert torch.equal(c.k, want_k) and torch.equal(c.v, want_v)
+    assert torch.equal(q[before:before + c.T], want)
+    assert not q[:before].any() and not q[before + c.T:].any()

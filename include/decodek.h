@@ -280,9 +280,9 @@ typedef struct dk_paged_append_args {
 int dk_paged_append(const dk_paged_append_args* args);
 /* Attention over the pages: q [T, n_q, head_dim] (tokens ldq >= n_q * head_dim apart, heads head_dim apart) -> out [T, n_q,
  * head_dim] contiguous. The row at own position p sees the positions j <= p, and with window > 0 of those only the ones
- * with j > p - window or j < sinks; softmax(scale * q k^T) v over them, zero where there are none. Pages that no row
- * of the call sees are not read and may be freed: their table entries may hold anything. What a page holds
- * past its sequence's last position is not used. The workspace (dk_paged_attention_workspace_bytes of the same
+ * with j > p - window or j < sinks; softmax(scale * q k^T) v over them, zero where there are none (rows of no sequence among
+ * them). Pages that no row of the call sees are not read and may be freed: their table entries may hold anything. What a
+ * page holds past its sequence's last position is not used. The workspace (dk_paged_attention_workspace_bytes of the same
  * sizes, 256-byte aligned) needs no initialization and keeps nothing between calls. */
 int dk_paged_attention_workspace_bytes(int64_t T, int64_t B, int64_t nq, int64_t nkv, int64_t head_dim, int32_t dtype,
                                        int32_t ragged, int64_t prefix_len, uint64_t* bytes);
@@ -309,7 +309,8 @@ typedef struct dk_paged_attention_args {
 int dk_paged_attention(const dk_paged_attention_args* args);
 /* Attention of a batch whose sequences share a prefix of prefix_len positions, in the pages listed by
  * prefix_table (int32): every row sees the whole prefix and its own sequence's positions (page_table, lengths,
- * starts as above, counted without the prefix) up to its own. The prefix is read once for all rows. */
+ * starts as above, counted without the prefix) up to its own; a row of an unused slot or of no sequence sees the prefix
+ * alone. The prefix is read once for all rows. */
 int dk_shared_prefix_attention(const dk_paged_attention_args* args);
 
 /* ---- log probabilities of given tokens: no reference counterpart -------------------------------

@@ -34,7 +34,7 @@ namespace paged {
 namespace {
 
 constexpr int kThreads = 384;
-constexpr int kMmaWarp = 8, kLoadWarp = 9;  // warps 10 and 11 only give their registers away
+constexpr int kMmaWarp = 8, kLoadWarp = 9, kZeroWarp = 10;  // warp 11 only gives its registers away
 // The launch holds 168 registers a thread; the softmax warpgroups take what the third one gives up:
 // 256 * 208 + 128 * 88 = 384 * 168.
 constexpr int kRegsLaunch = 168, kRegsSoftmax = 208, kRegsOther = 88;
@@ -542,6 +542,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!whole && live) *reinterpret_cast<float2*>(&p.part_ml[(slot * kTcRows + row) * 2]) = make_float2(m, l);
       tc::fence_before_sync();
+    }
+  }
+
+  if (warp == kZeroWarp && p.mode == kRagged && !p.always_partial) {
+    // Rows that belong to no sequence are in no tile: their outputs are zero. (Beside a prefix the join writes all rows.)
+    const int from = min(max(p.starts[0], 0), p.T), to = max(min(p.starts[p.B], p.T), from);
+    const int vecs = p.nkv * p.G * kHd / 8;  // 16 bytes each
+    for (int t = blockIdx.x; t < p.T - (to - from); t += gridDim.x) {
+      uint4* row = reinterpret_cast<uint4*>(p.out) + static_cast<int64_t>(t < from ? t : t - from + to) * vecs;
+      for (int i = lane; i < vecs; i += 32) row[i] = make_uint4(0, 0, 0, 0);
     }
   }
 

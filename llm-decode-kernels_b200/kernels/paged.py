@@ -170,9 +170,10 @@ def _attend(what, entry, q, k_pages, v_pages, prefix_table, prefix_len, page_tab
 def paged_attention(q, k_pages, v_pages, page_table, lengths, starts=None, window=0, sinks=0, scale=None, out=None):
     """Attention of q [T, n_heads, head_dim] (tokens any stride apart) over the pages: the row at position p sees the
     positions j <= p of its sequence, with window > 0 only those with j > p - window or j < sinks. Returns [T,
-    n_heads, head_dim] contiguous (`out` if given); a row that sees nothing is zero. scale: any number,
-    head_dim ** -0.5 if None. Pages that no row sees are not read, and their table entries may hold anything. With several tokens of a
-    sequence in one call, the keys and values that one of them sees have to be finite for the others too."""
+    n_heads, head_dim] contiguous (`out` if given); a row that sees nothing, or belongs to no sequence, is zero. scale: any
+    number, head_dim ** -0.5 if None. Pages that no row sees are not read, and their table entries may hold anything. With
+    several tokens of a sequence in one call, the keys and values that one of them sees have to be finite for the others
+    too."""
     if window < 0 or sinks < 0:
         _refuse("paged_attention", "window and sinks must not be negative")
     return _attend("paged_attention", "dk_paged_attention", q, k_pages, v_pages, None, 0, page_table, lengths, starts, window,
@@ -183,8 +184,9 @@ def shared_prefix_attention(q, k_pages, v_pages, prefix_table, prefix_len, page_
                             out=None):
     """Attention of a batch whose sequences share a prefix: every row of q [T, n_heads, head_dim] sees the prefix's
     prefix_len positions (in the pages prefix_table lists, int32 [>= pages of the prefix]) and, causally, its own
-    sequence's positions (page_table, lengths, starts: counted without the prefix). The prefix's keys and values are
-    read once for all rows. Returns [T, n_heads, head_dim] (`out` if given)."""
+    sequence's positions (page_table, lengths, starts: counted without the prefix); a row of an unused slot or of no
+    sequence sees the prefix alone. The prefix's keys and values are read once for all rows. Returns [T, n_heads,
+    head_dim] (`out` if given)."""
     if prefix_len == 0:
         return paged_attention(q, k_pages, v_pages, page_table, lengths, starts, scale=scale, out=out)
     return _attend("shared_prefix_attention", "dk_shared_prefix_attention", q, k_pages, v_pages, prefix_table, prefix_len,

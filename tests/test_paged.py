@@ -464,3 +464,27 @@ def test_append_rows_outside_starts(before, after):
     assert torch.equal(c.k, want_k) and torch.equal(c.v, want_v)
     assert torch.equal(q[before:before + c.T], want)
     assert not q[:before].any() and not q[before + c.T:].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("before,after,hd", [(0, 700, 128), (2, 0, 64), (3, 5, 128)])
+def test_attention_rows_outside_starts(before, after, hd):
+    """Rows before starts[0] and from starts[B] on belong to no sequence: zero from attention over the pages, the prefix alone
+    from attention with a prefix."""
+    from kernels.paged import paged_attention, shared_prefix_attention
+
+    c = Case([(3, 20), (150, 200), (1, 0)], hd=hd, one_token=False, prefix=40)
+    q = torch.cat([torch.randn(before, c.nq, hd), torch.zeros(c.T, c.nq, hd), torch.randn(after, c.nq, hd)]).to(c.dtype).cuda()
+    q[before:before + c.T] = c.q
+    live = slice(before, before + c.T)
+    outside = torch.ones(len(q), dtype=torch.bool)
+    outside[live] = False
+    out = torch.full_like(q, math.nan)
+    paged_attention(q, c.k, c.v, c.table, c.lengths, c.starts + before, out=out)
+    assert torch.equal(out[live], paged_attention(c.q, c.k, c.v, c.table, c.lengths, c.starts))
+    assert not out[outside.cuda()].any()
+    out = torch.full_like(q, math.nan)
+    shared_prefix_attention(q, c.k, c.v, c.prefix_table, 40, c.table, c.lengths, c.starts + before, out=out)
+    alone = Case([(1, 0)] * int(outside.sum()), hd=hd, prefix=40)
+    alone.q, alone.k, alone.v, alone.prefix_table = q[outside.cuda()], c.k, c.v, c.prefix_table
+    assert_within(out[outside.cuda()], *alone.attention())

@@ -39,7 +39,7 @@ typedef struct CUstream_st* dk_stream_t; /* same type as cudaStream_t */
 #define DK_DEVERR_NONE 0
 #define DK_DEVERR_WAIT_FULL 1  /* a consumer gave up waiting for a stage's copies */
 #define DK_DEVERR_WAIT_EMPTY 2 /* the producer gave up waiting for a stage to be released */
-#define DK_DEVERR_BAD_POSITION 3 /* decode attention / lm_head greedy: position outside the cache or history (no write done) */
+#define DK_DEVERR_BAD_POSITION 3 /* decode attention / lm_head greedy / paged ops: position outside the cache or history (no write done) */
 #define DK_DEVERR_TP_WAIT 4      /* a fused-allreduce CTA gave up waiting for a peer's partial sums */
 #define DK_DEVERR_STEP_WAIT 5    /* decode step: a CTA gave up waiting for another CTA or for its weight ring */
 #define DK_DEVERR_BAD_TOKEN 6    /* decode step / embed tokens: a token id outside [0, vocab) (row 0 used instead) */
@@ -281,9 +281,11 @@ int dk_paged_append(const dk_paged_append_args* args);
 /* Attention over the pages: q [T, n_q, head_dim] (tokens ldq >= n_q * head_dim apart, heads head_dim apart) -> out [T, n_q,
  * head_dim] contiguous. The row at own position p sees the positions j <= p, and with window > 0 of those only the ones
  * with j > p - window or j < sinks; softmax(scale * q k^T) v over them, zero where there are none (rows of no sequence among
- * them). Pages that no row of the call sees are not read and may be freed: their table entries may hold anything. What a
- * page holds past its sequence's last position is not used. The workspace (dk_paged_attention_workspace_bytes of the same
- * sizes, 256-byte aligned) needs no initialization and keeps nothing between calls. */
+ * them). A visible position whose page is not in the pool counts as zeros, one past the table not at all; both set
+ * DK_DEVERR_BAD_POSITION. Pages that no row of the call sees are not read and may be freed: their table entries may hold
+ * anything. What a page holds past its sequence's last position is not used. The workspace
+ * (dk_paged_attention_workspace_bytes of the same sizes, 256-byte aligned) needs no initialization and keeps nothing
+ * between calls. */
 int dk_paged_attention_workspace_bytes(int64_t T, int64_t B, int64_t nq, int64_t nkv, int64_t head_dim, int32_t dtype,
                                        int32_t ragged, int64_t prefix_len, uint64_t* bytes);
 typedef struct dk_paged_attention_args {

@@ -262,6 +262,14 @@ struct Cuts {
   __device__ int owner(int x) const { return x < long_end ? x / per_long : early + (x - long_end) / per; }
 };
 
+// The pool's row of position j, whose page is `page`, for kv head h. A page outside the pool reads as zeros (a row past the
+// maps' end) and is reported.
+__device__ __forceinline__ int pool_row(const Problem& p, int page, int h, int j) {
+  if (page >= 0 && page < p.n_pages) return (page * p.nkv + h) * p.page_size + (j & (p.page_size - 1));
+  record_device_error(p.err, DK_DEVERR_BAD_POSITION);
+  return p.n_pages * p.nkv * p.page_size;
+}
+
 // A CTA's piece of the line, unit by unit. Whole warps walk it.
 template <int kChunk>
 struct Walk {

@@ -220,6 +220,7 @@ __global__ void __launch_bounds__(kThreads)
       const Span<kChunk> span = walk.step();
       const int h = walk.h, c0 = walk.c0, c1 = walk.c1;
       const int32_t* table = walk.t.table;
+      if (lane == 0 && walk.last >= p.capacity) record_device_error(p.err, DK_DEVERR_BAD_POSITION);  // cut to the table
       // this lane's page in chunk i of the unit; INT_MIN: none, or nothing that a row sees
       auto entry = [&](int i) {
         const int j = i * kChunk + pg * box;
@@ -238,11 +239,7 @@ __global__ void __launch_bounds__(kThreads)
         if (lane == 0) mbar_arrive_expect_tx(&full[s], __popc(want) * box * 128);
         __syncwarp();
         if (mine) {
-          const int j = span.position(i * kChunk + pg * box);
-          // a page outside the pool reads as zeros (a row past the map's end)
-          const int y = page >= 0 && page < p.n_pages
-                            ? (page * p.nkv + h) * p.page_size + (j & (p.page_size - 1))
-                            : p.n_pages * p.nkv * p.page_size;
+          const int y = pool_row(p, page, h, span.position(i * kChunk + pg * box));
           uint8_t* dst = slots + s * B::kSlotBytes + kv * B::kTensorBytes + sg * B::kSegBytes + pg * box * 128;
           tma_load_2d(dst, kv ? &mv : &mk, sg * 64, y, &full[s]);
         }

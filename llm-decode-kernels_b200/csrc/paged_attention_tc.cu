@@ -258,6 +258,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const int h = walk.h, c0 = walk.c0, c1 = walk.c1;
       const int32_t* table = walk.t.table;
+      if (lane == 0 && walk.last >= p.capacity) record_device_error(p.err, DK_DEVERR_BAD_POSITION);  // cut to the table
       const bool two = walk.t.ntok > p.half_tokens;
       auto entry = [&](int i) {  // this lane's page in chunk i of the unit; INT_MIN: none, or nothing that a row sees
         const int j = i * kC + pg * box;
@@ -274,10 +275,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive_expect_tx(&bar.kv_full[s], __popc(want) * box * 128);
         __syncwarp();
         if (mine) {
-          const int j = span.position(i * kC + pg * box);
-          // a page outside the pool reads as zeros (a row past the map's end)
-          const int y = page >= 0 && page < p.n_pages ? (page * p.nkv + h) * p.page_size + (j & (p.page_size - 1))
-                                                      : p.n_pages * p.nkv * p.page_size;
+          const int y = pool_row(p, page, h, span.position(i * kC + pg * box));
           tma_load_2d(slots + s * L::kTileBytes + sg * L::kSegBytes + pg * box * 128, map, sg * 64, y, &bar.kv_full[s]);
         }
         ++fill;

@@ -171,9 +171,10 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, starts=None, windo
     """Attention of q [T, n_heads, head_dim] (tokens any stride apart) over the pages: the row at position p sees the
     positions j <= p of its sequence, with window > 0 only those with j > p - window or j < sinks. Returns [T,
     n_heads, head_dim] contiguous (`out` if given); a row that sees nothing, or belongs to no sequence, is zero. scale: any
-    number, head_dim ** -0.5 if None. Pages that no row sees are not read, and their table entries may hold anything. With
-    several tokens of a sequence in one call, the keys and values that one of them sees have to be finite for the others
-    too."""
+    number, head_dim ** -0.5 if None. Pages that no row sees are not read, and their table entries may hold anything; a
+    visible position without a page in the pool (read as zeros) or past the table (left out) sets the device error
+    DK_DEVERR_BAD_POSITION. With several tokens of a sequence in one call, the keys and values that one of them sees have to
+    be finite for the others too."""
     if window < 0 or sinks < 0:
         _refuse("paged_attention", "window and sinks must not be negative")
     return _attend("paged_attention", "dk_paged_attention", q, k_pages, v_pages, None, 0, page_table, lengths, starts, window,

@@ -488,3 +488,43 @@ def test_attention_rows_outside_starts(before, after, hd):
     alone = Case([(1, 0)] * int(outside.sum()), hd=hd, prefix=40)
     alone.q, alone.k, alone.v, alone.prefix_table = q[outside.cuda()], c.k, c.v, c.prefix_table
     assert_within(out[outside.cuda()], *alone.attention())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("one_token", [True, False])
+@pytest.mark.parametrize("window", [0, 30])
+def test_attention_reports_positions_without_a_page(one_token, window):
+    """A visible position whose table entry names no page of the pool, and a length past the table, set the device error; an
+    entry that no row sees does not."""
+    from kernels import _lib
+    from kernels.paged import paged_attention, shared_prefix_attention
+
+    c = Case([(1, 200), (1, 50)] if one_token else [(40, 200), (3, 50)], one_token=one_token, spoil=False, prefix=100, wide=0)
+    page = c.page
+
+    def error(table=None, lengths=None, prefix_table=None):
+        table, lengths = c.table if table is None else table, c.lengths if lengths is None else lengths
+        _lib.clear_device_error()
+        paged_attention(c.q, c.k, c.v, table, lengths, c.starts, window=window, sinks=2)
+        code = _lib.device_error()
+        if window == 0:
+            _lib.clear_device_error()
+            shared_prefix_attention(c.q, c.k, c.v, c.prefix_table if prefix_table is None else prefix_table, 100, table, lengths,
+                                    c.starts)
+            assert _lib.device_error() == (code if prefix_table is None else 3)
+        _lib.clear_device_error()
+        return code
+
+    assert error() == 0
+    for entry in (-1, c.k.shape[0], 2 ** 31 - 1):
+        table = c.table.clone()
+        table[0, 190 // page] = entry
+        assert error(table) == 3  # DK_DEVERR_BAD_POSITION
+        table = c.table.clone()
+        table[1, 50 // page + 1:] = entry  # after the second sequence's last position
+        assert error(table) == 0
+        if window == 0:
+            wrong = c.prefix_table.clone()
+            wrong[2] = entry
+            error(prefix_table=wrong)
+    assert error(lengths=c.lengths + torch.tensor([table.shape[1] * page - 200 + 1, 0], dtype=torch.int32, device="cuda")) == 3

@@ -59,6 +59,8 @@ class StepModel(ctypes.Structure):
 PAGED_APPEND_ARGS = struct.Struct("25q")
 PAGED_ATTENTION_ARGS = struct.Struct("15qd10q")
 
+_current_device = torch._C._cuda_getDevice  # (the public form takes 0.2 us more; CUDA is up where there is a CUDA tensor)
+
 FLAG_STATIC_WEIGHTS = 1
 FLAG_GENERIC = 2
 FLAG_EXACT_DEQUANT = 4
@@ -178,6 +180,20 @@ def require_cuda(what: str, *tensors: torch.Tensor | None) -> None:
     for t in tensors:
         if t is not None and not t.is_cuda:
             raise RuntimeError(f"{what}: tensors must be on a CUDA device (no CPU path), got {t.device}")
+
+
+def current_device_of(what: str, tensors) -> int:
+    """The index of the CUDA device that all tensors (None: left out) lie on, which has to be the current one: the library
+    launches there, with that device's properties and error word."""
+    index = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != index or index < 0:
+            where = sorted({str(t.device) for t in tensors if t is not None})
+            raise RuntimeError(f"{what}: tensors must be on one CUDA device (no CPU path), got {', '.join(where)}")
+    if index != _current_device():
+        raise RuntimeError(f"{what}: the tensors are on cuda:{index}, the current device is cuda:{_current_device()}: "
+                           f"call it under torch.cuda.device({index})")
+    return index
 
 
 def require_dtype(what: str, dtype: torch.dtype, *tensors: torch.Tensor | None) -> None:

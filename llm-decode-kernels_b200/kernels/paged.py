@@ -70,16 +70,6 @@ def _cache_shape(what, k_pages, v_pages, page_table, lengths, starts, tokens):
     return n_pages, n_kv, page, hd, B
 
 
-def _one_device(what, tensors):
-    """The CUDA device that all tensors (None: left out) lie on."""
-    index = tensors[0].get_device()
-    for t in tensors:
-        if t is not None and t.get_device() != index or index < 0:
-            where = {str(t.device) for t in tensors if t is not None}
-            _wrong_type(what, f"tensors must be on one CUDA device (no CPU path), got {', '.join(sorted(where))}")
-    return index
-
-
 def paged_append(qkv, k_pages, v_pages, page_table, lengths, cos, sin, n_heads, n_kv, starts=None, offset=0, out=None):
     """Rotate q and k of qkv [T, (n_heads + 2 n_kv) * head_dim] (q heads, k heads, v heads; unit column stride) by
     their tokens' positions and append k and v to the pages, in place. cos, sin [positions, head_dim / 2]: one angle
@@ -107,7 +97,7 @@ def paged_append(qkv, k_pages, v_pages, page_table, lengths, cos, sin, n_heads, 
         _wrong_type(what, "cos and sin must be fp32 or qkv's type")
     if out is not None and (out.shape != (T, n_heads, hd) or not out.is_contiguous() or out.dtype is not dtype):
         _refuse(what, "out must be a contiguous [tokens, n_heads, head_dim] of qkv's type")
-    device = _one_device(what, (qkv, k_pages, v_pages, page_table, lengths, starts, cos, sin, out))
+    device = _lib.current_device_of(what, (qkv, k_pages, v_pages, page_table, lengths, starts, cos, sin, out))
     q = qkv.new_empty_strided((T, n_heads, hd), (n_heads * hd, hd, 1)) if out is None else out
     status = _lib.lib().dk_paged_append(_lib.PAGED_APPEND_ARGS.pack(
         qkv.data_ptr(), ld, k_pages.data_ptr(), v_pages.data_ptr(), n_pages, page, page_table.data_ptr(),
@@ -121,9 +111,8 @@ def paged_append(qkv, k_pages, v_pages, page_table, lengths, cos, sin, n_heads, 
 
 @functools.lru_cache(maxsize=4096)
 def _workspace_bytes(T, B, nq, nkv, hd, dtype, ragged, prefix, device):
-    n = ctypes.c_uint64(0)
-    with torch.cuda.device(device):
-        _lib.call("dk_paged_attention_workspace_bytes", T, B, nq, nkv, hd, dtype, ragged, prefix, ctypes.byref(n))
+    n = ctypes.c_uint64(0)  # (`device`: the current one, whose number of SMs the size depends on)
+    _lib.call("dk_paged_attention_workspace_bytes", T, B, nq, nkv, hd, dtype, ragged, prefix, ctypes.byref(n))
     return int(n.value)
 
 
@@ -152,7 +141,7 @@ def _attend(what, entry, q, k_pages, v_pages, prefix_table, prefix_len, page_tab
         if prefix_table.dtype is not _INT32:
             _wrong_type(what, "prefix_table must be int32")
         prefix_at = prefix_table.data_ptr()
-    device = _one_device(what, (q, k_pages, v_pages, page_table, lengths, starts, prefix_table, out))
+    device = _lib.current_device_of(what, (q, k_pages, v_pages, page_table, lengths, starts, prefix_table, out))
     code = _DTYPES[dtype]
     # the prefix's length does not change the size, only whether there is one
     nbytes = _workspace_bytes(T, B, nq, n_kv, hd, code, starts is not None, 1 if prefix_len else 0, device)

@@ -528,3 +528,32 @@ def test_attention_reports_positions_without_a_page(one_token, window):
             wrong[2] = entry
             error(prefix_table=wrong)
     assert error(lengths=c.lengths + torch.tensor([table.shape[1] * page - 200 + 1, 0], dtype=torch.int32, device="cuda")) == 3
+
+
+def test_refuses_a_device_that_is_not_the_current_one(monkeypatch):
+    """The library launches on the current device: tensors of another one are refused, by every op, before the C entry."""
+    from kernels import _lib, logprobs, paged
+
+    class On:
+        def __init__(self, index):
+            self.device, self.get_device = f"cuda:{index}", lambda: index
+
+    monkeypatch.setattr(_lib, "_current_device", lambda: 1)
+    assert _lib.current_device_of("op", (On(1), None, On(1))) == 1
+    for tensors in ((On(0),), (On(0), On(0)), (On(1), On(0)), (On(-1),), (On(2), None)):
+        with pytest.raises(RuntimeError, match="op: "):
+            _lib.current_device_of("op", tensors)
+
+    def no_entry():
+        raise AssertionError("the C entry was reached")
+
+    monkeypatch.setattr(_lib, "lib", no_entry)
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda self: 0)
+    c = _cpu_case()
+    cos = torch.zeros(40, 64)
+    for call in (lambda: paged.paged_attention(c.q, c.k, c.v, c.table, c.lengths),
+                 lambda: paged.shared_prefix_attention(c.q, c.k, c.v, c.table[0], 10, c.table, c.lengths),
+                 lambda: paged.paged_append(torch.zeros(2, 16 * 128).half(), c.k, c.v, c.table, c.lengths, cos, cos, 12, 2),
+                 lambda: logprobs.token_logprobs(torch.zeros(2, 50), torch.zeros(2, dtype=torch.long))):
+        with pytest.raises(RuntimeError, match="current device is cuda:1"):
+            call()

@@ -1,11 +1,14 @@
 // Log probabilities of given tokens, the entropy of each row's distribution and its top alternatives, in one pass
 // over the logits. With m = max x, y = (x - m) log2(e), s = sum 2^y and w = sum 2^y y:
 //   log p(t) = (x_t - m) - ln s        entropy = ln 2 (log2 s - w / s)
-// Neither subtracts two large numbers of the row's own size, so fp32 keeps both to a few units in the last place.
+// s lies between 1 and V and no term of w is positive, so fp32 keeps both to a few units in the last place of ln s, and neither
+// a positive log probability nor a negative entropy comes out.
 // The maximum, s and w run along (rescaled when the maximum grows), so the row is read once.
 //
-// 2^y is taken relative to the largest logit of the CTA's first tile; only a logit 40 above that moves the base (fp32
-// holds e^40 times the row's sum with room to spare), so the common path neither compares nor rescales.
+// A thread takes 2^y relative to its base, the largest of the logits that it and the CTA's first tile have had. Once that
+// tile is known few threads meet a larger one (of random logits, one of 256 threads a tile), so the common path only
+// compares. (A base that may stay up to 40 below the maximum: 138.5 against 138.7 us for 2048 rows, and log probabilities of
+// sure tokens up to 2e-6 above zero.)
 //
 // The top alternatives (by value, ties to the lowest index) come from the same pass. The `top`-th largest of the maxima that
 // 64 groups of threads have seen is a threshold that `top` elements reach; it is taken after the first tile, again a few
@@ -41,7 +44,6 @@ constexpr int kCap = 1024;   // candidates the list holds
 constexpr int kMaxTop = 32;
 constexpr int kMaxCluster = 8;
 constexpr float kLog2e = 1.44269504088896341f;
-constexpr float kRoom = 40.f;
 // Logits below it (the type's lowest value in masks) count as this: just below -1e30, a value of bf16, so that elements
 // clamped in any type and the least base are the same number.
 constexpr float kLow = -0x1.94p99f;
@@ -275,8 +277,8 @@ __global__ void __launch_bounds__(kThreads, kResident) logprob_kernel(const Logp
     } else if (kTop && tile == kRaiseTile) {
       raise_threshold();
     }
-    // Rare: a logit far above the base, candidates
-    if (mine > base + kRoom) {
+    // Rare: a logit above the base, candidates
+    if (mine > base) {
       Stats a{base, s2.x, w2.x}, b{base, s2.y, w2.y};
       base = mine;
       a.move(base), b.move(base);

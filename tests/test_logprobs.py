@@ -220,3 +220,29 @@ def test_infinity_and_nan_give_nan(V, at, dtype):
                     lp, entropy, value, index = token_logprobs(view, torch.full((len(view),), target, device="cuda"), top)
                     assert lp.isnan().all() and entropy.isnan().all() and value.isnan().all()
                     assert (index[:, :1] == at).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_peaked_rows(dtype):
+    """One logit far above the others anywhere in the row, as of a sure token: its log probability and the row's entropy are
+    next to zero and come out so, on the right side of zero.
+
+    Relative to the maximum its own term is 1 without an error. The others are below 2^-31 each, below 2^-24 for one thread, and below
+    2^-20 in all, with a relative error below 2^-15 (their exponents reach 60, and up to V / 512 + 72 roundings). Adding them to 1 loses
+    at most a thread's and rounds at most 22 times (the threads' pairs, two trees of 5 steps, 7 other CTAs, ln s), 2^-24 each."""
+    from kernels.logprobs import token_logprobs
+
+    V, M = 60000, 64
+    g = torch.Generator().manual_seed(20)
+    x = torch.randn(M, V, generator=g).clamp(-4, 4)
+    at = torch.randint(0, V, (M,), generator=g)
+    x[torch.arange(M), at] = 26 + 12 * torch.rand(M, generator=g)
+    x, at = x.to(dtype).cuda(), at.cuda()
+    for rows in (slice(0, M), slice(0, 1), slice(1, 2)):
+        lp, entropy, value, index = (t.cpu() for t in token_logprobs(x[rows], at[rows], 2))
+        want = _exact(x[rows], at[rows], 2)
+        eps = 23 * 2.0 ** -24
+        assert ((lp - want[0]).abs() <= eps + 2.0 ** -15 * want[0].abs()).all() and (lp <= 0).all()
+        assert ((entropy - want[1]).abs() <= eps + 2.0 ** -15 * want[1]).all() and (entropy >= 0).all()
+        assert torch.equal(index, want[3])

@@ -163,6 +163,10 @@ struct Problem {
   int* err;
 };
 
+// Positions of sequence b; an unused slot has none, however negative its length (positions counted back from the lowest
+// number would wrap).
+__device__ __forceinline__ int length_of(const int32_t* lengths, int b) { return max(lengths[b], 0); }
+
 struct Tile {
   int t0, ntok;  // tokens of q
   int p0;        // position of the first one
@@ -174,7 +178,7 @@ __device__ __forceinline__ Tile tile_at(const Problem& p, int i) {
   if (p.mode == kOneToken) {
     t.t0 = i;
     t.ntok = 1;
-    t.p0 = p.lengths[i] - 1;
+    t.p0 = length_of(p.lengths, i) - 1;
     t.table = p.table + i * p.ld_table;
   } else if (p.mode == kPrefix) {
     t.t0 = i * p.tile_tokens;

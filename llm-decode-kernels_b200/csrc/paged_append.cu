@@ -105,11 +105,11 @@ __global__ void __launch_bounds__(kWarps * 32, 4) paged_append_kernel(const Appe
     load(s0);
     int b = t, pos;
     if (p.starts == nullptr) {
-      pos = p.lengths[t] - 1;
+      pos = length_of(p.lengths, t) - 1;
     } else {
       b = find_tile_warp([&](int j) { return p.starts[j]; }, p.B, t, lane);
       const int end = p.starts[b + 1];
-      pos = t >= p.starts[b] && t < end ? p.lengths[b] - (end - t) : -1;
+      pos = t >= p.starts[b] && t < end ? length_of(p.lengths, b) - (end - t) : -1;
     }
     // A row of no sequence, or of one without positions (an unused slot of the batch), appends nothing; its q is zero.
     const int64_t angle = pos + p.rope_offset;

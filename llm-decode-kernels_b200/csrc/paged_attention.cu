@@ -76,14 +76,14 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Problem p, int
     int total;
     const int at = tiles + scan(mine, total);
     // sequence and first token of each tile; long sequences are filled in by the whole CTA below
-    if (mine > 0 && at < p.max_tiles) info[at] = make_int4(t0, t1, p.lengths[b], b);
+    if (mine > 0 && at < p.max_tiles) info[at] = make_int4(t0, t1, length_of(p.lengths, b), b);
     for (int i = 1; i < min(mine, kOwnTiles) && at + i < p.max_tiles; ++i)
-      info[at + i] = make_int4(t0 + i * p.tile_tokens, t1, p.lengths[b], b);
+      info[at + i] = make_int4(t0 + i * p.tile_tokens, t1, length_of(p.lengths, b), b);
     __syncthreads();
     if (mine > kOwnTiles) {
       const int k = atomicAdd(&long_count, 1);
       long_seq[k] = make_int4(at, mine, t0, t1);
-      long_len[k] = make_int2(p.lengths[b], b);
+      long_len[k] = make_int2(length_of(p.lengths, b), b);
     }
     __syncthreads();
     for (int k = 0; k < long_count; ++k)
@@ -179,7 +179,10 @@ __global__ void __launch_bounds__(kThreads)
     for (int b0 = 0; b0 < p.B; b0 += kThreads) {
       const int b = b0 + tid;
       int n = 0;
-      if (b < p.B) n = Span<kChunk>(p.lengths[b] - 1, p.lengths[b] - 1, p.mask, p.capacity, p.page_size).n + p.unit_extra;
+      if (b < p.B) {
+        const int last = length_of(p.lengths, b) - 1;
+        n = Span<kChunk>(last, last, p.mask, p.capacity, p.page_size).n + p.unit_extra;
+      }
       int s = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {

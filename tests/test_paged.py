@@ -557,3 +557,25 @@ def test_refuses_a_device_that_is_not_the_current_one(monkeypatch):
                  lambda: logprobs.token_logprobs(torch.zeros(2, 50), torch.zeros(2, dtype=torch.long))):
         with pytest.raises(RuntimeError, match="current device is cuda:1"):
             call()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ragged", [False, True])
+@pytest.mark.parametrize("window", [0, 20])
+def test_unused_slots_of_any_negative_length(ragged, window):
+    """A length of the type's lowest value is an unused slot like any other <= 0."""
+    from kernels import _lib
+    from kernels.paged import paged_append, paged_attention
+
+    c = Case([(3, 40), (3, 0), (2, 20), (3, 0)] if ragged else [(1, 40), (1, 0), (1, 20), (1, 0)], one_token=not ragged, spoil=False)
+    low = torch.tensor([40, -2 ** 31, 20, -2 ** 31 + 2], dtype=torch.int32, device="cuda")
+    want = paged_attention(c.q, c.k, c.v, c.table, c.lengths, c.starts, window=window, sinks=2)
+    _lib.clear_device_error()
+    assert torch.equal(paged_attention(c.q, c.k, c.v, c.table, low, c.starts, window=window, sinks=2), want)
+    cos, sin = _rope(64, 128)
+    qkv = torch.randn(c.T, 16 * 128, device="cuda").half()
+    k, v = c.k.clone(), c.v.clone()
+    want = paged_append(qkv, k, v, c.table, c.lengths, cos, sin, 12, 2, starts=c.starts)
+    assert torch.equal(paged_append(qkv, c.k, c.v, c.table, low, cos, sin, 12, 2, starts=c.starts), want)
+    assert torch.equal(c.k, k) and torch.equal(c.v, v)
+    assert _lib.device_error() == 0

@@ -802,9 +802,14 @@ int attention(const char* what, const dk_paged_attention_args* args, bool prefix
   if (n_pages <= 0 || table_width <= 0 || window < 0 || sinks < 0) return set_error(DK_ERR_INVALID, "%s: bad sizes", what);
   if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1)))
     return set_error(DK_ERR_UNSUPPORTED, "%s: page_size %lld (a power of two from 16 to 256)", what, (long long)page_size);
-  if (n_pages * z.nkv * page_size + kChunk >= (int64_t(1) << 31) || table_width * page_size >= (int64_t(1) << 31) ||
-      window >= (int64_t(1) << 31) || sinks >= (int64_t(1) << 31))
-    return set_error(DK_ERR_INVALID, "%s: pages x kv heads x page_size, a table row's positions, window and sinks must stay below 2^31", what);
+  // Positions and offsets are 32-bit: the largest sums are a position rounded up to whole chunks with their boxes, and the
+  // window before the position of a row that comes up to T rows before its sequence's first one.
+  constexpr int64_t kMaxPositions = (int64_t(1) << 31) - 1024;
+  if (n_pages > INT32_MAX || table_width > INT32_MAX || n_pages * z.nkv > INT32_MAX ||
+      n_pages * z.nkv * page_size + kChunk > INT32_MAX || table_width * page_size + z.T > kMaxPositions ||
+      window > INT32_MAX || sinks > INT32_MAX)
+    return set_error(DK_ERR_INVALID,
+                     "%s: pages x kv heads x page_size, window and sinks must stay below 2^31, a table row's positions with T 1024 below", what);
   // A window of all positions masks none, and sinks end with the positions: sums with them stay in range.
   window = std::min(window, table_width * page_size);
   sinks = std::min(sinks, table_width * page_size);

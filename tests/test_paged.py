@@ -579,3 +579,23 @@ def test_unused_slots_of_any_negative_length(ragged, window):
     assert torch.equal(paged_append(qkv, c.k, c.v, c.table, low, cos, sin, 12, 2, starts=c.starts), want)
     assert torch.equal(c.k, k) and torch.equal(c.v, v)
     assert _lib.device_error() == 0
+
+
+def test_tables_whose_positions_pass_31_bits_are_refused():
+    """Positions rounded up to whole chunks, and windows before the first position, have to fit 32 bits; products of sizes that
+    pass 64 bits do not slip through."""
+    from kernels import _lib
+
+    h = _lib.lib()
+
+    def attend(T=2, width=2, page=16, pages=4, window=0, sinks=0):
+        return h.dk_paged_attention(_lib.PAGED_ATTENTION_ARGS.pack(
+            0, 1536, 0, 0, pages, page, 0, 0, 0, width, width, 0, 256, window, sinks, 1.0, 0, T, 2, 12, 2, 128, 0, 0, 0, 0))
+
+    most = (1 << 31) - 1024
+    for page in (16, 256):
+        assert attend(width=(most - 2) // page, page=page) == -1 and b"NULL" in h.dk_last_error()  # as far as the pointers
+        assert attend(width=(most - 2) // page + 1, page=page) == -1 and b"2^31" in h.dk_last_error()
+    assert attend(width=most // 16 - 100, T=2000) == -1 and b"2^31" in h.dk_last_error()
+    for more in (dict(width=1 << 60), dict(pages=1 << 59), dict(pages=1 << 62), dict(window=1 << 31), dict(sinks=1 << 40)):
+        assert attend(**more) == -1 and b"2^31" in h.dk_last_error(), more

@@ -248,7 +248,8 @@ int dk_embed_tokens(const int64_t* tokens, const void* embed, int64_t vocab, int
  * to no sequence (a captured call may have more rows than a step needs).
  * All of these are device pointers read on the device, so one captured launch serves every step.
  * page_size: a power of two from 16 to 256; head_dim 64 or 128; n_q a multiple of n_kv, at most 16 query heads
- * per kv head (attention); table_width * page_size + T at most 2^31 - 1024 (attention). A length <= 0 marks an unused slot of the batch. Every launch may be captured. */
+ * per kv head (attention); table_width * page_size + T at most 2^31 - 1024 (attention). A length <= 0 marks an unused
+ * slot of the batch; a call of no tokens (T = 0, with B = 0 too) does nothing. Every launch may be captured. */
 #define DK_F16 0
 #define DK_BF16 1
 #define DK_F32 2 /* dk_token_logprobs only */

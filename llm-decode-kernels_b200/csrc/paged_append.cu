@@ -170,7 +170,7 @@ extern "C" int dk_paged_append(const dk_paged_append_args* args) {
   const int64_t T = a.T, B = a.B, nq = a.n_q, nkv = a.n_kv, head_dim = a.head_dim, n_pages = a.n_pages,
                 page_size = a.page_size, table_width = a.table_width;
   const int dtype = static_cast<int>(a.dtype);
-  if (T < 0 || B <= 0 || nq <= 0 || nkv <= 0 || n_pages <= 0 || table_width <= 0)
+  if (T < 0 || B < 0 || (B == 0 && T > 0) || nq <= 0 || nkv <= 0 || n_pages <= 0 || table_width <= 0)
     return set_error(DK_ERR_INVALID, "paged_append: bad sizes");
   if (head_dim != 64 && head_dim != 128)
     return set_error(DK_ERR_UNSUPPORTED, "paged_append: head_dim %lld (64 or 128)", (long long)head_dim);

@@ -715,7 +715,7 @@ void share_gpu(Pass& pre, Pass& own) {
 }
 
 int check_sizes(const char* what, const Sizes& z) {
-  if (z.T < 0 || z.B <= 0 || z.nq <= 0 || z.nkv <= 0 || z.prefix_len < 0)
+  if (z.T < 0 || z.B < 0 || (z.B == 0 && z.T > 0) || z.nq <= 0 || z.nkv <= 0 || z.prefix_len < 0)
     return set_error(DK_ERR_INVALID, "%s: bad sizes", what);
   if (z.hd != 64 && z.hd != 128) return set_error(DK_ERR_UNSUPPORTED, "%s: head_dim %lld (64 or 128)", what, (long long)z.hd);
   if (z.dtype != DK_F16 && z.dtype != DK_BF16) return set_error(DK_ERR_UNSUPPORTED, "%s: dtype %d", what, z.dtype);

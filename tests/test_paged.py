@@ -599,3 +599,37 @@ def test_tables_whose_positions_pass_31_bits_are_refused():
     assert attend(width=most // 16 - 100, T=2000) == -1 and b"2^31" in h.dk_last_error()
     for more in (dict(width=1 << 60), dict(pages=1 << 59), dict(pages=1 << 62), dict(window=1 << 31), dict(sinks=1 << 40)):
         assert attend(**more) == -1 and b"2^31" in h.dk_last_error(), more
+
+
+def test_c_entries_take_a_step_without_sequences():
+    """A call of no tokens, of no sequences too, does nothing; tokens without a sequence are refused."""
+    from kernels import _lib
+
+    h = _lib.lib()
+
+    def attend(T, B, starts=0):
+        return h.dk_paged_attention(_lib.PAGED_ATTENTION_ARGS.pack(0, 1536, 0, 0, 4, 16, 0, 0, 0, 2, 2, 0, starts, 0, 0, 1.0, 0, T, B, 12,
+                                                                   2, 128, 0, 0, 0, 0))
+
+    def append(T, B):
+        return h.dk_paged_append(_lib.PAGED_APPEND_ARGS.pack(0, 0, 0, 0, 4, 16, 0, 2, 2, 0, 0, 0, 0, 1, 64, 10, 0, 0, T, B, 12, 2, 128,
+                                                             0, 0))
+
+    assert attend(0, 0) == attend(0, 0, starts=256) == attend(0, 3, starts=256) == 0
+    assert append(0, 0) == 0
+    assert attend(2, 0, starts=256) == append(2, 0) == -1 and attend(0, -1) == append(0, -1) == -1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B", [0, 3])
+def test_a_step_without_tokens(B):
+    from kernels.paged import paged_append, paged_attention, shared_prefix_attention
+
+    c = Case([(1, 20)] * 3, prefix=16, spoil=False)
+    starts = torch.zeros(B + 1, dtype=torch.int32, device="cuda") if B else None
+    table, lengths, k, v = c.table[:B], c.lengths[:B], c.k.clone(), c.v.clone()
+    cos, sin = _rope(64, 128)
+    assert paged_append(c.q.new_zeros(0, 16 * 128), c.k, c.v, table, lengths, cos, sin, 12, 2, starts).shape == (0, 12, 128)
+    assert torch.equal(c.k, k) and torch.equal(c.v, v)
+    assert paged_attention(c.q[:0], c.k, c.v, table, lengths, starts).shape == (0, 12, 128)
+    assert shared_prefix_attention(c.q[:0], c.k, c.v, c.prefix_table, 16, table, lengths, starts).shape == (0, 12, 128)

@@ -24,7 +24,7 @@ def token_logprobs(logits, targets, top=0):
         raise ValueError(f"{what}: logits must be [rows, vocab]")
     M, V = logits.shape
     ld, unit = logits.stride()
-    if unit != 1 or (ld < V and M > 1):
+    if (unit != 1 and V > 1) or (ld < V and M > 1):
         raise ValueError(f"{what}: logits must have unit column stride and rows that do not overlap")
     if targets.shape != (M,) or not targets.is_contiguous():
         raise ValueError(f"{what}: targets must hold one token per row")

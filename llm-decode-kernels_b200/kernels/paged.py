@@ -53,7 +53,7 @@ def _cache_shape(what, k_pages, v_pages, page_table, lengths, starts, tokens):
         _refuse(what, "page_size must be a power of two from 16 to 256")
     if hd != 128 and hd != 64:
         _refuse(what, "head_dim must be 64 or 128")
-    if page_table.dim() != 2 or page_table.shape[1] == 0 or page_table.stride()[1] != 1:
+    if page_table.dim() != 2 or page_table.shape[1] == 0 or page_table.stride()[1] != 1 and page_table.shape[1] > 1:
         _refuse(what, "page_table must be [sequences, pages] with unit column stride")
     B = page_table.shape[0]
     if lengths.shape != (B,) or not lengths.is_contiguous():
@@ -85,8 +85,15 @@ def paged_append(qkv, k_pages, v_pages, page_table, lengths, cos, sin, n_heads, 
     ld, unit = qkv.stride()
     if n_kv != kv or n_heads <= 0 or width != (n_heads + 2 * n_kv) * hd or unit != 1:
         _refuse(what, "qkv must be [tokens, (n_heads + 2 n_kv) * head_dim] with the pages' kv heads and unit column stride")
-    if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] != hd // 2 or cos.stride() != sin.stride() or cos.stride()[1] != 1:
+    if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] != hd // 2:
         _refuse(what, "cos and sin must be [positions, head_dim / 2]")
+    ld_rope, unit = cos.stride()
+    if cos.shape[0] == 1:  # (a single row's stride means nothing)
+        ld_rope = 0
+    elif sin.stride()[0] != ld_rope:
+        _refuse(what, "cos and sin must have the same row stride")
+    if unit != 1 or sin.stride()[1] != 1:
+        _refuse(what, "cos and sin must have unit column stride")
     if offset < 0:
         _refuse(what, "offset must not be negative")
     dtype = qkv.dtype
@@ -102,7 +109,7 @@ def paged_append(qkv, k_pages, v_pages, page_table, lengths, cos, sin, n_heads, 
     status = _lib.lib().dk_paged_append(_lib.PAGED_APPEND_ARGS.pack(
         qkv.data_ptr(), ld, k_pages.data_ptr(), v_pages.data_ptr(), n_pages, page, page_table.data_ptr(),
         page_table.stride()[0], page_table.shape[1], lengths.data_ptr(), 0 if starts is None else starts.data_ptr(),
-        cos.data_ptr(), sin.data_ptr(), f32, cos.stride()[0], cos.shape[0], offset, q.data_ptr(), T, B, n_heads, n_kv, hd,
+        cos.data_ptr(), sin.data_ptr(), f32, ld_rope, cos.shape[0], offset, q.data_ptr(), T, B, n_heads, n_kv, hd,
         _DTYPES[dtype], _raw_stream(device)))
     if status:
         _lib.check(status, what)
@@ -122,7 +129,7 @@ def _attend(what, entry, q, k_pages, v_pages, prefix_table, prefix_len, page_tab
     T, nq, width = q.shape
     n_pages, n_kv, page, hd, B = _cache_shape(what, k_pages, v_pages, page_table, lengths, starts, T)
     ld, by_head, unit = q.stride()
-    if width != hd or unit != 1 or by_head != hd or ld < nq * hd and T > 1:
+    if width != hd or unit != 1 or by_head != hd and nq > 1 or ld < nq * hd and T > 1:
         _refuse(what, "q must be [tokens, heads, head_dim], a token's heads side by side and tokens apart from each other")
     if nq <= 0 or nq % n_kv or nq // n_kv > MAX_GROUP:
         _refuse(what, f"query heads must be a multiple of the kv heads, at most {MAX_GROUP} for each")

@@ -633,3 +633,41 @@ def test_a_step_without_tokens(B):
     assert torch.equal(c.k, k) and torch.equal(c.v, v)
     assert paged_attention(c.q[:0], c.k, c.v, table, lengths, starts).shape == (0, 12, 128)
     assert shared_prefix_attention(c.q[:0], c.k, c.v, c.prefix_table, 16, table, lengths, starts).shape == (0, 12, 128)
+
+
+def _one_wide(c):
+    """Layouts whose strides differ from the usual only where an extent is 1: one head, one column of pages, one row of angles."""
+    q = torch.randn(1, c.T, c.hd).to(c.dtype).to(c.q.device).transpose(0, 1)  # [T, 1, hd], heads T * hd apart
+    table = c.table[:, :1].t().contiguous().t()  # [B, 1], columns B apart
+    cos, sin = torch.ones(1, c.hd // 2, device=c.q.device), torch.zeros(3, c.hd // 2, device=c.q.device).as_strided((1, c.hd // 2), (7, 1))
+    return q, table, cos.as_strided(cos.shape, (5, 1)), sin
+
+
+def test_strides_of_extent_one_are_not_looked_at():
+    """They pass the checks of layouts; the CPU tensors are refused after those."""
+    from kernels.logprobs import token_logprobs
+    from kernels.paged import paged_append, paged_attention
+
+    c = Case([(1, 1), (1, 1)], nq=1, nkv=1, spoil=False, device="cpu")
+    q, table, cos, sin = _one_wide(c)
+    for call in (lambda: paged_attention(q, c.k, c.v, c.table, c.lengths), lambda: paged_attention(c.q, c.k, c.v, table, c.lengths),
+                 lambda: paged_append(torch.zeros(2, 3 * 128).half(), c.k, c.v, table, c.lengths, cos, sin, 1, 1),
+                 lambda: token_logprobs(torch.zeros(2, 4).t()[:, :1].as_strided((2, 1), (1, 9)), torch.zeros(2, dtype=torch.long))):
+        with pytest.raises(RuntimeError, match="CUDA device"):
+            call()
+
+
+@pytest.mark.gpu
+def test_one_head_one_page_one_angle():
+    from kernels.logprobs import token_logprobs
+    from kernels.paged import paged_append, paged_attention
+
+    c = Case([(1, 1), (1, 1), (1, 1)], nq=1, nkv=1, spoil=False)
+    q, table, cos, sin = _one_wide(c)
+    want = paged_attention(q.contiguous().view(3, 1, 128), c.k, c.v, c.table, c.lengths)
+    assert torch.equal(paged_attention(q, c.k, c.v, table, c.lengths), want)
+    qkv = torch.randn(3, 3 * 128, device="cuda").half()
+    out = paged_append(qkv, c.k, c.v, table, c.lengths, cos, sin, 1, 1)
+    assert torch.equal(out.view(3, 128), qkv[:, :128])  # an angle of zero
+    lp = token_logprobs(torch.randn(2, 1, device="cuda").as_strided((2, 1), (1, 9)), torch.zeros(2, dtype=torch.long, device="cuda"))[0]
+    assert not lp.any()

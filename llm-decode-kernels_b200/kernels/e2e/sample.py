@@ -46,6 +46,7 @@ class PagedSampler:
         angle = positions[:, None].float() * runner.inv_freq[None, :]
         self.cos, self.sin = angle.cos(), angle.sin()
         self.prompt = 0
+        self.left = 0  # tokens that each sample may still be fed; none before a prompt
         self.lengths = torch.zeros(samples, dtype=torch.int32, device=dev)
 
     def _layers(self, x, attend):
@@ -79,7 +80,7 @@ class PagedSampler:
                                    sinks=self.sinks).view(P, -1)
 
         h = self._layers(F.embedding(ids, r.embed), attend)
-        self.prompt = P
+        self.prompt, self.left = P, self.max_new
         if self.window > 0:  # positions go on where the prompt ends: its full pages are shared, the rest of it is copied
             full = P // self.page
             self.table = torch.cat([self.prompt_table[:full].expand(self.n, full), self.own_table], 1)
@@ -94,8 +95,11 @@ class PagedSampler:
 
     @torch.no_grad()
     def step(self, tokens: torch.Tensor) -> torch.Tensor:
-        """Feed one token to each sample (tokens int64 [n]); the logits [n, V] after it."""
+        """Feed one token to each sample (tokens int64 [n]), up to max_new times after a prompt; the logits [n, V] after it."""
         r = self.r
+        if self.left <= 0:
+            raise ValueError(f"PagedSampler: prefill a prompt first, and feed at most {self.max_new} tokens after it")
+        self.left -= 1
         self.lengths += 1
         offset = 0 if self.window > 0 else self.prompt
 

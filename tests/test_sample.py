@@ -76,3 +76,23 @@ def test_refusals():
         sampler.prefill(torch.zeros(17, dtype=torch.long, device="cuda"))
     with pytest.raises(ValueError):
         sampler.generate(torch.zeros(4, dtype=torch.long, device="cuda"), 9)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("window", [0, 6])
+def test_steps_are_counted(window):
+    """A step without a prompt, or past max_new, is refused before it changes anything; a new prompt starts the count again."""
+    from kernels.e2e.sample import PagedSampler
+
+    sampler = PagedSampler(_runner("fp16"), 2, 16, 3, page_size=16, window=window, sinks=1)
+    token = torch.zeros(2, dtype=torch.long, device="cuda")
+    with pytest.raises(ValueError):
+        sampler.step(token)
+    for prompt in (4, 16):
+        sampler.prefill(torch.arange(prompt, device="cuda"))
+        for _ in range(3):
+            assert sampler.step(token).isfinite().all()
+        lengths = sampler.lengths.clone()
+        with pytest.raises(ValueError):
+            sampler.step(token)
+        assert torch.equal(sampler.lengths, lengths)

@@ -305,7 +305,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---------------------------------------------------------------- products
     int fill = 0;         // ring slots consumed
     unsigned p_seen[2] = {0, 0};
-    const uint32_t qk_desc = idesc<T>(128, kC, false) | (p.signs < 0 ? kNegateA : 0u);
     auto slot_wait = [&](int f) {
       if (ok && !wait_for(&bar.kv_full[f % L::kSlots], (f / L::kSlots) & 1, p.err, DK_DEVERR_WAIT_FULL)) ok = false;
       ok = __all_sync(0xffffffffu, ok);
@@ -316,7 +315,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int k = 0; k < kHd / 16; ++k) {
         const uint32_t off = ((k / 4) * L::kSegBytes + (k % 4) * 32) >> 4;  // (descriptors count 16 bytes)
-        mma_ss(tmem + kS[x], a + off, b + off, qk_desc, k > 0);
+        mma_ss(tmem + kS[x], a + off, b + off, idesc<T>(128, kC, false) | (p.signs < 0 ? kNegateA : 0u), k > 0);
       }
       commit_elected(&bar.s_full[x]);
     };

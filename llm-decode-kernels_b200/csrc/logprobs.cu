@@ -19,7 +19,7 @@
 // of it, from L2, counting the keys above three pivots.
 // Bound by HBM, closely followed by the 16 exponentials a cycle that an SM computes (152064 x 2048 bf16 logits: 95 us of
 // bytes, 66 us of exponentials at 1.97 GHz; measured 130 us, 4.8 TB/s, with the exponentials' pipe 62% and the issue slots 67%
-// busy; 139 us under the power cap). Rows are split over a cluster of CTAs when there are few of them; the parts meet in the first
+// busy; 141 us under the power cap). Rows are split over a cluster of CTAs when there are few of them; the parts meet in the first
 // CTA's shared memory.
 #include <algorithm>
 #include <cfloat>

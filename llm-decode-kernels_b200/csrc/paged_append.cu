@@ -9,8 +9,8 @@
 // time (a head's 8 dims and their 8 partners a lane, or 8 dims of v), loads them before it knows where they go - the
 // token's sequence, position and page are a chain of small loads - and its angles once for all of them. With few tokens
 // a token's heads are spread over several warps.
-// Measured (36 heads of 128): 9000 tokens, 164 MB, 32 us, 78% of the copy rate (64 registers a thread, 4 CTAs an SM: with 5 or
-// 6 of them registers spill, 42 and 53 us); one token 2.3 us without the host.
+// Measured (36 heads of 128): 9000 tokens, 164 MB, 32 us, 78% of the copy rate (64 registers a thread, 4 CTAs an SM, 20 bytes of
+// it spilled; with 5 or 6 CTAs 92 to 300 bytes spill, 42 and 53 us); one token 2.3 us without the host.
 #include <algorithm>
 
 #include "paged.cuh"

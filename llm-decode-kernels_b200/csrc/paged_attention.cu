@@ -13,8 +13,9 @@
 // query heads as the rows, online softmax in registers, p.v on the tensor cores with p taken from the
 // score accumulators. A position that no row of the tile sees reads a zero row instead of v, so whatever
 // the page holds there (infinities and NaN included) stays out; masked scores are replaced, not added to.
-// Measured (28 heads over 4 kv heads of 128, bf16): 64 sequences of 8192, 1.07 GB, 171 us, 6.3 TB/s, 96% of the copy rate;
-// one of 640 (12 heads over 2) 7.5 us without the host, of 32768 16 us: bound by the chain of launch, first copies, join.
+// Measured (28 heads over 4 kv heads of 128, bf16): 64 sequences of 8192, 1.07 GB, 174 us, 6.2 TB/s, 94% of the copy rate (168
+// registers a thread, 20 to 28 bytes spilled); one of 640 (12 heads over 2) 7.8 us without the host, of 32768 16 us: a
+// chain of launch, first copies and the join's launch.
 #include <algorithm>
 #include <climits>
 #include <mutex>
@@ -683,7 +684,7 @@ void set_tile(const Sizes& z, Pass& a, bool tc) {
 }
 
 // One token for each sequence goes to the rows kernel, several to the tiles (64 sequences of 8192, 12 heads over 2 kv heads,
-// one token each, without the host: 91 us on the rows kernel, 108 as tiles; one of 640: 9.4 and 13.6; 4 tokens each as tiles:
+// one token each, without the host: 91 us on the rows kernel, 111 as tiles; one of 640: 9.4 and 13.6; 4 tokens each as tiles:
 // 109).
 void shape_own(const Sizes& z, Pass& a) {
   set_tile(z, a, z.ragged);

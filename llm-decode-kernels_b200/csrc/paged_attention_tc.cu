@@ -20,8 +20,9 @@
 // Every wait is bounded.
 // What bounds it: a chunk's four products take 4 x 8 x 65 = 2080 cycles at head_dim 128, its 32768 exponentials 2048 (16 a
 // cycle), and they run beside each other; a pair of half chunks takes about 1.65 us (1.15 at least), a unit's start, masks
-// and output about 5 us more. Measured: a prompt of 8192, 12 heads over 2 of 128, 195 us, 1.06 PFLOP/s, 64% of the cuBLAS
-// rate; under the power cap (1.69 GHz) 226 us, 66% of cuBLAS's there. 16 softmax warps, two a row: 362 us. Exponentials
+// and output about 5 us more. Measured: a prompt of 8192, 12 heads over 2 of 128, 197 us in short bursts, 1.05 PFLOP/s, 64%
+// of the cuBLAS rate; under the power cap (1.69 GHz) 228 us, 65% of cuBLAS's there. 220 to 228 bytes of a thread's registers are
+// spilled. 16 softmax warps, two a row: 362 us. Exponentials
 // on the FMA units for an eighth of the positions: 206 us. Steps of 64 positions: their products take nearly as long (58 cycles).
 #include <climits>
 #include <mutex>

@@ -183,7 +183,8 @@ def shared_prefix_attention(q, k_pages, v_pages, prefix_table, prefix_len, page_
     prefix_len positions (in the pages prefix_table lists, int32 [>= pages of the prefix]) and, causally, its own
     sequence's positions (page_table, lengths, starts: counted without the prefix); a row of an unused slot or of no
     sequence sees the prefix alone. The prefix's keys and values are read once for all rows. Returns [T, n_heads,
-    head_dim] (`out` if given)."""
+    head_dim] (`out` if given). With starts, all results pass through a workspace in fp32: 1 KB x head_dim for each kv head
+    and tile of up to 256 rows, of the prefix's and of the sequences' (1 GB for 32768 tokens of 28 heads over 4)."""
     if prefix_len == 0:
         return paged_attention(q, k_pages, v_pages, page_table, lengths, starts, scale=scale, out=out)
     return _attend("shared_prefix_attention", "dk_shared_prefix_attention", q, k_pages, v_pages, prefix_table, prefix_len,

@@ -109,7 +109,8 @@ struct Span {
     lo = m.window > 0 ? max(0, p0 - m.window + 1) : 0;
     gap_at = m.window > 0 ? (min(m.sinks, lo) + part - 1) & -part : 0;
     shift = max(0, (lo & -part) - gap_at);
-    lo -= shift, end -= shift;
+    lo -= shift;
+    end = max(end - shift, min(end, gap_at));  // (a window wholly past the table leaves the sinks)
     n = max(1, (end + kChunk - 1) / kChunk);
   }
   __device__ int position(int j) const { return j < gap_at ? j : j + shift; }

@@ -671,3 +671,35 @@ def test_one_head_one_page_one_angle():
     assert torch.equal(out.view(3, 128), qkv[:, :128])  # an angle of zero
     lp = token_logprobs(torch.randn(2, 1, device="cuda").as_strided((2, 1), (1, 9)), torch.zeros(2, dtype=torch.long, device="cuda"))[0]
     assert not lp.any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("one_token", [True, False])
+@pytest.mark.parametrize("hd,page", [(128, 16), (64, 256)])
+@pytest.mark.parametrize("sinks", [0, 3, 40])
+def test_windows_wholly_past_the_table_leave_the_sinks(one_token, hd, page, sinks):
+    """A length far past the table is reported; what counts is what the table has, here the sinks alone."""
+    from kernels import _lib
+    from kernels.paged import paged_attention
+
+    c = Case([(1, 60), (1, 30)] if one_token else [(5, 60), (40, 45)], hd=hd, page=page, one_token=one_token, wide=0)
+    for length in (c.table.shape[1] * page + 100, 2 ** 31 - 1):
+        lengths = c.lengths.clone()
+        lengths[0] = length
+        _lib.clear_device_error()
+        out = paged_attention(c.q, c.k, c.v, c.table, lengths, c.starts, window=20, sinks=sinks)
+        assert _lib.device_error() == 3  # DK_DEVERR_BAD_POSITION
+        _lib.clear_device_error()
+        exact, tol = c.attention(20, sinks)
+        n = c.sizes[0][0]
+        k, v, group = c.sequence(c.k, 0)[:sinks], c.sequence(c.v, 0)[:sinks], c.nq // c.nkv
+        for t in range(n):  # over the positions 0..sinks - 1, with the tolerance of Case.attention
+            if sinks == 0:
+                exact[t], tol[t] = 0, 0
+                continue
+            a = torch.softmax(torch.einsum("hd,jhd->hj", c.q[t].double().cpu(), k.repeat_interleave(group, 1)) * hd ** -0.5, -1)
+            vs = v.repeat_interleave(group, 1)
+            exact[t] = torch.einsum("hj,jhd->hd", a, vs)
+            u, spread = UNIT[c.dtype], torch.einsum("hj,jhd->hd", a, vs.abs())
+            tol[t] = u * exact[t].abs() + (u + 2.0 ** -13) * spread + sinks * 2.0 ** -25 * vs.abs().max()
+        assert_within(out, exact, tol)

@@ -317,6 +317,45 @@ int dk_paged_attention(const dk_paged_attention_args* args);
  * prefix and once for the own positions (1 GB for 32768 tokens of 28 heads over 4). */
 int dk_shared_prefix_attention(const dk_paged_attention_args* args);
 
+/* ---- a paged cache held in 4 bits: no reference counterpart ------------------------------------
+ * The ops above over pools of codes: k_pages and v_pages [n_pages, n_kv, page_size, head_dim * 9 / 16] bytes, whose block of a
+ * (page, kv head) holds first the codes, head_dim / 2 bytes a position (dim 2 i in the low half of byte i), then the scales,
+ * head_dim / 16 bytes a position. A value is code * scale * k_scale (v_scale): an E2M1 code, an E4M3 scale for each 16 dims and a power of
+ * two from 2^-64 to 2^64 for the pool; code * scale is exact in fp16 and bf16. `dtype` in these calls is qkv's, q's, out's. */
+/* Append: scale = E4M3(max |x| / 6) and code = E2M1(x / scale) of x / k_scale (v_scale), both rounded to nearest, ties to even,
+ * and saturating; x are the values dk_paged_append would store, but the rotation of k is rounded once, from its exact
+ * value in fp64. A NaN makes its group's scale NaN. */
+typedef struct dk_paged_append_fp4_args {
+  dk_paged_append_args append;
+  double k_scale, v_scale;
+} dk_paged_append_fp4_args;
+int dk_paged_append_fp4(const dk_paged_append_fp4_args* args);
+/* Read back: row t of k_out and v_out [T, n_kv, head_dim] (fp16 or bf16) is the position of the cache that token t of such a call
+ * has (lengths, starts as above). Rows of no sequence are zero; so is a position without a page in the pool, which sets
+ * DK_DEVERR_BAD_POSITION. */
+typedef struct dk_paged_read_fp4_args {
+  const void* k_pages;
+  const void* v_pages;
+  int64_t n_pages, page_size;
+  const int32_t* page_table;
+  int64_t ld_table, table_width;
+  const int32_t* lengths;
+  const int32_t* starts;
+  double k_scale, v_scale;
+  void* k_out;
+  void* v_out;
+  int64_t T, B, n_kv, head_dim, dtype;
+  dk_stream_t stream;
+} dk_paged_read_fp4_args;
+int dk_paged_read_fp4(const dk_paged_read_fp4_args* args);
+/* dk_paged_attention and dk_shared_prefix_attention over such pools, with the same arguments, masks and errors. */
+typedef struct dk_paged_attention_fp4_args {
+  dk_paged_attention_args attention;
+  double k_scale, v_scale;
+} dk_paged_attention_fp4_args;
+int dk_paged_attention_fp4(const dk_paged_attention_fp4_args* args);
+int dk_shared_prefix_attention_fp4(const dk_paged_attention_fp4_args* args);
+
 /* ---- log probabilities of given tokens: no reference counterpart -------------------------------
  * logits [M, V] (rows ld apart; DK_F16, DK_BF16 or DK_F32) in one pass: logprob[m] = x[t] - logsumexp(x) of the target
  * t = targets[m] (device int64; t < 0: no token, 0; t >= V: NaN and DK_DEVERR_BAD_TOKEN), entropy[m] in nats (a logit of

@@ -9,11 +9,14 @@
 // time (a head's 8 dims and their 8 partners a lane, or 8 dims of v), loads them before it knows where they go - the
 // token's sequence, position and page are a chain of small loads - and its angles once for all of them. With few tokens
 // a token's heads are spread over several warps.
+// With kFp4 k' and v go to a cache of 4-bit codes (paged_fp4.cuh). What a code is can hang on the last bit of k', so k is then
+// rotated in fp64, where the two products are exact, and rounded to T once before it is quantised: a code does not depend on
+// the order or the fusing of the operations. q is rotated as without.
 // Measured (36 heads of 128): 9000 tokens, 164 MB, 32 us, 78% of the copy rate (64 registers a thread, 4 CTAs an SM, 20 bytes of
 // it spilled; with 5 or 6 CTAs 92 to 300 bytes spill, 42 and 53 us); one token 2.3 us without the host.
 #include <algorithm>
 
-#include "paged.cuh"
+#include "paged_fp4.cuh"
 
 namespace dk {
 namespace {
@@ -36,6 +39,7 @@ struct AppendParams {
   void* q_out;
   int T, B, nq, nkv;
   int n_pages, page_size, page_shift, table_width;
+  float k_inv, v_inv;  // kFp4: 1 / the pools' powers of two
   int* err;
 };
 
@@ -64,7 +68,22 @@ __device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
 constexpr int kAhead = 2;  // 4 with half the warps resident: 33.9 against 32.9 us for 164 MB
 constexpr int kWarps = 8;
 
-template <typename T, typename R, int kHd>
+// x c - y s and y c + x s of 8 pairs, rounded to T: in fp64 (the products of T and fp32 values are exact there).
+template <typename T>
+__device__ __forceinline__ void rotate8_exactly(const uint4& lo, const uint4& hi, const float (&co)[8], const float (&si)[8], float (&u)[8],
+                                                float (&v)[8]) {
+  const uint32_t l[4] = {lo.x, lo.y, lo.z, lo.w}, r[4] = {hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 f = Elem<T>::unpack(l[j]), g = Elem<T>::unpack(r[j]);
+    const double c0 = co[2 * j], c1 = co[2 * j + 1], s0 = si[2 * j], s1 = si[2 * j + 1];
+    const float2 x = Elem<T>::unpack(Elem<T>::pack(__double2float_rn(f.x * c0 - g.x * s0), __double2float_rn(f.y * c1 - g.y * s1)));
+    const float2 y = Elem<T>::unpack(Elem<T>::pack(__double2float_rn(g.x * c0 + f.x * s0), __double2float_rn(g.y * c1 + f.y * s1)));
+    u[2 * j] = x.x, u[2 * j + 1] = x.y, v[2 * j] = y.x, v[2 * j + 1] = y.y;
+  }
+}
+
+template <typename T, typename R, int kHd, bool kFp4>
 __global__ void __launch_bounds__(kWarps * 32, 4) paged_append_kernel(const AppendParams p, int segments, int per_warp) {
   constexpr int kRot = kHd / 16;         // lanes of a rotated head
   constexpr int kHeads = 32 / kRot;      // rotated heads of a segment
@@ -125,6 +144,14 @@ __global__ void __launch_bounds__(kWarps * 32, 4) paged_append_kernel(const Appe
     }
     const int64_t in_page = static_cast<int64_t>(pos & (p.page_size - 1)) * kHd;
     const int64_t page_heads = static_cast<int64_t>(page) * p.nkv;
+    // 8 values from dim `dim` on into a pool of codes
+    auto put_fp4 = [&](void* pool, int head, int dim, const float (&x)[8], float inv_power) {
+      uint8_t scale;
+      const uint32_t code = fp4_quantise8(x, inv_power, lane, scale);
+      uint8_t* block = static_cast<uint8_t*>(pool) + (page_heads + head) * p.page_size * Fp4<kHd>::kRow;
+      *reinterpret_cast<uint32_t*>(block + (in_page + dim) / 2) = code;
+      if ((lane & 1) == 0) block[p.page_size * Fp4<kHd>::kCodes + (in_page + dim) / 16] = scale;
+    };
     for (int s = s0; s < s1; s += kAhead) {
       if (s > s0) load(s);
 #pragma unroll
@@ -133,6 +160,15 @@ __global__ void __launch_bounds__(kWarps * 32, 4) paged_append_kernel(const Appe
         if (h >= 0) {
           const bool is_q = h < p.nq;
           if (!is_q && !lands) continue;
+          if constexpr (kFp4) {
+            if (!is_q) {
+              float x[8], y[8];
+              rotate8_exactly<T>(lo[a], hi[a], co, si, x, y);
+              put_fp4(p.k, h - p.nq, d, x, p.k_inv);
+              put_fp4(p.k, h - p.nq, d + kHd / 2, y, p.k_inv);
+              continue;
+            }
+          }
           uint4 u = make_uint4(0, 0, 0, 0), v = u;
           if (turns) {
             const uint32_t l[4] = {lo[a].x, lo[a].y, lo[a].z, lo[a].w}, r[4] = {hi[a].x, hi[a].y, hi[a].z, hi[a].w};
@@ -151,6 +187,10 @@ __global__ void __launch_bounds__(kWarps * 32, 4) paged_append_kernel(const Appe
                         : static_cast<T*>(p.k) + (page_heads + h - p.nq) * p.page_size * kHd + in_page;
           *reinterpret_cast<uint4*>(dst + d) = u;
           *reinterpret_cast<uint4*>(dst + d + kHd / 2) = v;
+        } else if (kFp4 && vh >= 0 && lands) {
+          float x[8];
+          load8<T>(reinterpret_cast<const T*>(&lo[a]), x);
+          put_fp4(p.v, vh, vd, x, p.v_inv);
         } else if (vh >= 0 && lands) {
           *reinterpret_cast<uint4*>(static_cast<T*>(p.v) + (page_heads + vh) * p.page_size * kHd + in_page + vd) = lo[a];
         }
@@ -164,31 +204,33 @@ __global__ void __launch_bounds__(kWarps * 32, 4) paged_append_kernel(const Appe
 
 using namespace dk;
 
-extern "C" int dk_paged_append(const dk_paged_append_args* args) {
-  if (args == nullptr) return set_error(DK_ERR_INVALID, "paged_append: NULL arguments");
-  const dk_paged_append_args& a = *args;
+namespace {
+
+int append(const char* what, const dk_paged_append_args& a, bool fp4, double k_scale, double v_scale) {
   const int64_t T = a.T, B = a.B, nq = a.n_q, nkv = a.n_kv, head_dim = a.head_dim, n_pages = a.n_pages,
                 page_size = a.page_size, table_width = a.table_width;
   const int dtype = static_cast<int>(a.dtype);
   if (T < 0 || B < 0 || (B == 0 && T > 0) || nq <= 0 || nkv <= 0 || n_pages <= 0 || table_width <= 0)
-    return set_error(DK_ERR_INVALID, "paged_append: bad sizes");
+    return set_error(DK_ERR_INVALID, "%s: bad sizes", what);
   if (head_dim != 64 && head_dim != 128)
-    return set_error(DK_ERR_UNSUPPORTED, "paged_append: head_dim %lld (64 or 128)", (long long)head_dim);
-  if (dtype != DK_F16 && dtype != DK_BF16) return set_error(DK_ERR_UNSUPPORTED, "paged_append: dtype %d", dtype);
+    return set_error(DK_ERR_UNSUPPORTED, "%s: head_dim %lld (64 or 128)", what, (long long)head_dim);
+  if (dtype != DK_F16 && dtype != DK_BF16) return set_error(DK_ERR_UNSUPPORTED, "%s: dtype %d", what, dtype);
   if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1)))
-    return set_error(DK_ERR_UNSUPPORTED, "paged_append: page_size %lld (a power of two from 16 to 256)",
+    return set_error(DK_ERR_UNSUPPORTED, "%s: page_size %lld (a power of two from 16 to 256)", what,
                      (long long)page_size);
+  if (!fp4_power(k_scale) || !fp4_power(v_scale))
+    return set_error(DK_ERR_INVALID, "%s: k_scale and v_scale must be powers of two from 2^-64 to 2^64", what);
   if (T == 0) return DK_OK;
   if (a.starts == nullptr && T != B)
-    return set_error(DK_ERR_INVALID, "paged_append: without starts there is one token per sequence");
+    return set_error(DK_ERR_INVALID, "%s: without starts there is one token per sequence", what);
   if (T > INT32_MAX || B > INT32_MAX || n_pages > INT32_MAX || table_width > INT32_MAX ||
       table_width * page_size > INT32_MAX)
-    return set_error(DK_ERR_INVALID, "paged_append: sizes must fit 31 bits");
+    return set_error(DK_ERR_INVALID, "%s: sizes must fit 31 bits", what);
   if (!a.qkv || !a.k_pages || !a.v_pages || !a.page_table || !a.lengths || !a.cos || !a.sin || !a.q_out)
-    return set_error(DK_ERR_INVALID, "paged_append: NULL pointer");
+    return set_error(DK_ERR_INVALID, "%s: NULL pointer", what);
   if (!aligned16(a.qkv) || !aligned16(a.k_pages) || !aligned16(a.v_pages) || !aligned16(a.q_out) || !aligned16(a.cos) ||
       !aligned16(a.sin) || (T > 1 && (a.ldqkv & 7)) || (a.ld_rope & (a.rope_f32 ? 3 : 7)))
-    return set_error(DK_ERR_ALIGN, "paged_append: rows of qkv, cos, sin, the pages and q_out need 16-byte alignment");
+    return set_error(DK_ERR_ALIGN, "%s: rows of qkv, cos, sin, the pages and q_out need 16-byte alignment", what);
   AppendParams p;
   p.qkv = a.qkv, p.ldqkv = a.ldqkv, p.k = a.k_pages, p.v = a.v_pages;
   p.table = a.page_table, p.ld_table = a.ld_table, p.lengths = a.lengths, p.starts = a.starts;
@@ -198,6 +240,7 @@ extern "C" int dk_paged_append(const dk_paged_append_args* args) {
   p.n_pages = static_cast<int>(n_pages), p.page_size = static_cast<int>(page_size);
   p.page_shift = __builtin_ctzll(page_size);
   p.table_width = static_cast<int>(table_width);
+  p.k_inv = static_cast<float>(1. / k_scale), p.v_inv = static_cast<float>(1. / v_scale);
   p.err = device_info().err_word;
   const int heads = static_cast<int>(512 / head_dim), copies = static_cast<int>(256 / head_dim);
   const int segments = static_cast<int>((nq + nkv + heads - 1) / heads + (nkv + copies - 1) / copies);
@@ -210,9 +253,10 @@ extern "C" int dk_paged_append(const dk_paged_append_args* args) {
   const dim3 grid(static_cast<unsigned>(std::min<int64_t>((warps + kWarps - 1) / kWarps, 64ll * device_info().num_sms)));
   cudaStream_t st = reinterpret_cast<cudaStream_t>(a.stream);
   cudaError_t e;
-#define DK_APPEND(TT, RR)                                                                                    \
-  e = launch(head_dim == 128 ? paged_append_kernel<TT, RR, 128> : paged_append_kernel<TT, RR, 64>, grid, dim3(kWarps * 32), 0, \
-             st, pdl_enabled(), dim3(1, 1, 1), p, segments, per_warp)
+#define DK_KERNEL(TT, RR, F) (head_dim == 128 ? paged_append_kernel<TT, RR, 128, F> : paged_append_kernel<TT, RR, 64, F>)
+#define DK_APPEND(TT, RR)                                                                                       \
+  e = launch(fp4 ? DK_KERNEL(TT, RR, true) : DK_KERNEL(TT, RR, false), grid, dim3(kWarps * 32), 0, st, pdl_enabled(), \
+             dim3(1, 1, 1), p, segments, per_warp)
   if (dtype == DK_F16) {
     if (a.rope_f32)
       DK_APPEND(__half, float);
@@ -225,6 +269,19 @@ extern "C" int dk_paged_append(const dk_paged_append_args* args) {
       DK_APPEND(__nv_bfloat16, __nv_bfloat16);
   }
 #undef DK_APPEND
-  if (e != cudaSuccess) return set_error(DK_ERR_CUDA, "paged_append launch: %s", cudaGetErrorString(e));
+#undef DK_KERNEL
+  if (e != cudaSuccess) return set_error(DK_ERR_CUDA, "%s launch: %s", what, cudaGetErrorString(e));
   return DK_OK;
+}
+
+}  // namespace
+
+extern "C" int dk_paged_append(const dk_paged_append_args* args) {
+  if (args == nullptr) return set_error(DK_ERR_INVALID, "paged_append: NULL arguments");
+  return append("paged_append", *args, false, 1., 1.);
+}
+
+extern "C" int dk_paged_append_fp4(const dk_paged_append_fp4_args* args) {
+  if (args == nullptr) return set_error(DK_ERR_INVALID, "paged_append_fp4: NULL arguments");
+  return append("paged_append_fp4", args->append, true, args->k_scale, args->v_scale);
 }

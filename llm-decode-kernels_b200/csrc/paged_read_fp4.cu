@@ -1,0 +1,127 @@
+// Positions of a 4-bit paged cache read back as 16-bit values, k and v: row t of the call is a position of a sequence (the
+// last ones of each, as in the other paged ops), value = code * scale * power, exact in T unless outside its range.
+//
+// Memory bound: 9 bytes are read for 32 written. A warp takes a token: 8 dims (4 bytes of codes, half a group) of one tensor a
+// lane at a time, so that it stores 512 contiguous bytes.
+#include <algorithm>
+
+#include "paged_fp4.cuh"
+
+namespace dk {
+namespace {
+
+using namespace paged;
+
+struct ReadParams {
+  const uint8_t* pool[2];
+  void* out[2];
+  float power[2];
+  const int32_t* table;
+  int64_t ld_table;
+  const int32_t* lengths;
+  const int32_t* starts;
+  int T, B, nkv;
+  int n_pages, page_size, page_shift, table_width;
+  int* err;
+};
+
+constexpr int kWarps = 8;
+
+template <typename T, int kHd>
+__global__ void __launch_bounds__(kWarps * 32) paged_read_fp4_kernel(const ReadParams p) {
+  using F = Fp4<kHd>;
+  pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const int pieces = p.nkv * (kHd / 8);  // of 8 dims, of one tensor
+  for (int64_t w = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5); w < p.T; w += static_cast<int64_t>(gridDim.x) * kWarps) {
+    const int t = static_cast<int>(w);
+    int b = t, pos;
+    if (p.starts == nullptr) {
+      pos = length_of(p.lengths, t) - 1;
+    } else {
+      b = find_tile_warp([&](int j) { return p.starts[j]; }, p.B, t, lane);
+      const int end = p.starts[b + 1];
+      pos = t >= p.starts[b] && t < end ? length_of(p.lengths, b) - (end - t) : -1;
+    }
+    // A row of no sequence, or before its sequence's first position, is zero; so is a position without a page, which is reported.
+    const int at = pos >> p.page_shift;
+    const int page = pos >= 0 && at < p.table_width ? p.table[b * p.ld_table + at] : -1;
+    const bool there = page >= 0 && page < p.n_pages;
+    if (pos >= 0 && !there && lane == 0) record_device_error(p.err, DK_DEVERR_BAD_POSITION);
+    const int slot = pos & (p.page_size - 1);
+    for (int i = lane; i < 2 * pieces; i += 32) {
+      const int which = i >= pieces, piece = i - which * pieces;
+      const int h = piece / (kHd / 8), c = piece % (kHd / 8);
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (there) {
+        const uint8_t* block = p.pool[which] + (static_cast<int64_t>(page) * p.nkv + h) * p.page_size * F::kRow;
+        const uint32_t code = *reinterpret_cast<const uint32_t*>(block + slot * F::kCodes + 4 * c);
+        const float s = fp4_scale(block[p.page_size * F::kCodes + slot * F::kScales + c / 2]) * p.power[which];
+        uint32_t x[4];
+        fp4_codes(code, x);
+        uint32_t y[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 f = Elem<__half>::unpack(x[j]);
+          y[j] = Elem<T>::pack(f.x * s, f.y * s);
+        }
+        v = make_uint4(y[0], y[1], y[2], y[3]);
+      }
+      *reinterpret_cast<uint4*>(static_cast<T*>(p.out[which]) + (static_cast<int64_t>(t) * pieces + piece) * 8) = v;
+    }
+  }
+}
+
+}  // namespace
+}  // namespace dk
+
+using namespace dk;
+
+extern "C" int dk_paged_read_fp4(const dk_paged_read_fp4_args* args) {
+  if (args == nullptr) return set_error(DK_ERR_INVALID, "paged_read_fp4: NULL arguments");
+  const dk_paged_read_fp4_args& a = *args;
+  const int64_t T = a.T, B = a.B, nkv = a.n_kv, head_dim = a.head_dim, page_size = a.page_size, width = a.table_width;
+  const int dtype = static_cast<int>(a.dtype);
+  if (T < 0 || B < 0 || (B == 0 && T > 0) || nkv <= 0 || a.n_pages <= 0 || width <= 0)
+    return set_error(DK_ERR_INVALID, "paged_read_fp4: bad sizes");
+  if (head_dim != 64 && head_dim != 128)
+    return set_error(DK_ERR_UNSUPPORTED, "paged_read_fp4: head_dim %lld (64 or 128)", (long long)head_dim);
+  if (dtype != DK_F16 && dtype != DK_BF16) return set_error(DK_ERR_UNSUPPORTED, "paged_read_fp4: dtype %d", dtype);
+  if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1)))
+    return set_error(DK_ERR_UNSUPPORTED, "paged_read_fp4: page_size %lld (a power of two from 16 to 256)", (long long)page_size);
+  if (!fp4_power(a.k_scale) || !fp4_power(a.v_scale))
+    return set_error(DK_ERR_INVALID, "paged_read_fp4: k_scale and v_scale must be powers of two from 2^-64 to 2^64");
+  if (T == 0) return DK_OK;
+  if (a.starts == nullptr && T != B)
+    return set_error(DK_ERR_INVALID, "paged_read_fp4: without starts there is one row per sequence");
+  if (T > INT32_MAX || B > INT32_MAX || a.n_pages > INT32_MAX || width > INT32_MAX || width * page_size > INT32_MAX || nkv > 65535)
+    return set_error(DK_ERR_INVALID, "paged_read_fp4: sizes must fit 31 bits");
+  if (!a.k_pages || !a.v_pages || !a.page_table || !a.lengths || !a.k_out || !a.v_out)
+    return set_error(DK_ERR_INVALID, "paged_read_fp4: NULL pointer");
+  if (!aligned16(a.k_pages) || !aligned16(a.v_pages) || !aligned16(a.k_out) || !aligned16(a.v_out))
+    return set_error(DK_ERR_ALIGN, "paged_read_fp4: pages and outputs need 16-byte alignment");
+  ReadParams p;
+  p.pool[0] = static_cast<const uint8_t*>(a.k_pages), p.pool[1] = static_cast<const uint8_t*>(a.v_pages);
+  p.out[0] = a.k_out, p.out[1] = a.v_out;
+  p.power[0] = static_cast<float>(a.k_scale), p.power[1] = static_cast<float>(a.v_scale);
+  p.table = a.page_table, p.ld_table = a.ld_table, p.lengths = a.lengths, p.starts = a.starts;
+  p.T = static_cast<int>(T), p.B = static_cast<int>(B), p.nkv = static_cast<int>(nkv);
+  p.n_pages = static_cast<int>(a.n_pages), p.page_size = static_cast<int>(page_size);
+  p.page_shift = __builtin_ctzll(page_size);
+  p.table_width = static_cast<int>(width);
+  p.err = device_info().err_word;
+  const dim3 grid(static_cast<unsigned>(std::min<int64_t>((T + kWarps - 1) / kWarps, 64ll * device_info().num_sms)));
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(a.stream);
+  cudaError_t e;
+#define DK_READ(TT) \
+  e = launch(head_dim == 128 ? paged_read_fp4_kernel<TT, 128> : paged_read_fp4_kernel<TT, 64>, grid, dim3(kWarps * 32), 0, st, \
+             pdl_enabled(), dim3(1, 1, 1), p)
+  if (dtype == DK_F16)
+    DK_READ(__half);
+  else
+    DK_READ(__nv_bfloat16);
+#undef DK_READ
+  if (e != cudaSuccess) return set_error(DK_ERR_CUDA, "paged_read_fp4 launch: %s", cudaGetErrorString(e));
+  return DK_OK;
+}

@@ -54,10 +54,13 @@ class StepModel(ctypes.Structure):
                 ("k_cache", P), ("v_cache", P), ("layers", ctypes.POINTER(StepLayer))]
 
 
-# dk_paged_append_args and dk_paged_attention_args (8-byte fields throughout), packed in one step: ctypes takes about
+# dk_paged_append_args, dk_paged_attention_args and those of a 4-bit cache (8-byte fields throughout), packed in one step: ctypes takes about
 # 0.1 us for each argument of a call
 PAGED_APPEND_ARGS = struct.Struct("25q")
 PAGED_ATTENTION_ARGS = struct.Struct("15qd10q")
+PAGED_APPEND_FP4_ARGS = struct.Struct("25q2d")
+PAGED_READ_FP4_ARGS = struct.Struct("9q2d8q")
+PAGED_ATTENTION_FP4_ARGS = struct.Struct("15qd10q2d")
 
 _current_device = torch._C._cuda_getDevice  # (the public form takes 0.2 us more; CUDA is up where there is a CUDA tensor)
 
@@ -110,6 +113,10 @@ SIGNATURES = {
     "dk_paged_attention_workspace_bytes": [I64, I64, I64, I64, I64, I32, I32, I64, ctypes.POINTER(ctypes.c_uint64)],
     "dk_paged_attention": [ctypes.c_char_p],
     "dk_shared_prefix_attention": [ctypes.c_char_p],
+    "dk_paged_append_fp4": [ctypes.c_char_p],
+    "dk_paged_read_fp4": [ctypes.c_char_p],
+    "dk_paged_attention_fp4": [ctypes.c_char_p],
+    "dk_shared_prefix_attention_fp4": [ctypes.c_char_p],
     "dk_token_logprobs": [P, I64, I32, P, I64, I64, I64, P, P, P, P, P],
     "dk_step_workspace_bytes": [ctypes.POINTER(StepModel), ctypes.POINTER(ctypes.c_uint64)],
     "dk_step_create": [ctypes.POINTER(StepModel), P, ctypes.c_uint64, ctypes.POINTER(P)],

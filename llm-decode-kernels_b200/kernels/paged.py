@@ -39,14 +39,19 @@ def _wrong_type(what: str, message: str):
     raise RuntimeError(f"{what}: {message}")
 
 
-def _cache_shape(what, k_pages, v_pages, page_table, lengths, starts, tokens):
-    """(n_pages, n_kv, page_size, head_dim, B) of a checked cache and batch."""
+_FP4_ROWS = {72: 128, 36: 64}  # head_dim by the bytes of a position in a cache of 4-bit codes
+
+
+def _cache_shape(what, k_pages, v_pages, page_table, lengths, starts, tokens, fp4=False):
+    """(n_pages, n_kv, page_size, head_dim, B) of a checked cache (fp4: of 4-bit codes, kernels.paged_fp4) and batch."""
     shape = k_pages.shape
     if len(shape) != 4 or v_pages.shape != shape:
-        _refuse(what, "k_pages and v_pages must be [n_pages, n_kv, page_size, head_dim], both alike")
+        _refuse(what, f"k_pages and v_pages must be [n_pages, n_kv, page_size, {'9/16 ' if fp4 else ''}head_dim], both alike")
     if not (k_pages.is_contiguous() and v_pages.is_contiguous()):
         _refuse(what, "pages must be contiguous")
     n_pages, n_kv, page, hd = shape
+    if fp4:
+        hd = _FP4_ROWS.get(hd, 0)
     if n_pages <= 0 or n_kv <= 0:
         _refuse(what, "an empty pool of pages")
     if not (16 <= page <= 256 and page & (page - 1) == 0):
@@ -65,7 +70,10 @@ def _cache_shape(what, k_pages, v_pages, page_table, lengths, starts, tokens):
         _refuse(what, "starts must hold sequences + 1 row numbers")
     if not (page_table.dtype is _INT32 and lengths.dtype is _INT32 and (starts is None or starts.dtype is _INT32)):
         _wrong_type(what, "page_table, lengths and starts must be int32")
-    if k_pages.dtype not in _DTYPES or v_pages.dtype is not k_pages.dtype:
+    if fp4:
+        if k_pages.dtype is not torch.uint8 or v_pages.dtype is not torch.uint8:
+            _wrong_type(what, "pages must be uint8, both of them")
+    elif k_pages.dtype not in _DTYPES or v_pages.dtype is not k_pages.dtype:
         _wrong_type(what, "pages must be fp16 or bf16, both alike")
     return n_pages, n_kv, page, hd, B
 
@@ -77,11 +85,15 @@ def paged_append(qkv, k_pages, v_pages, page_table, lengths, cos, sin, n_heads, 
     of a shared prefix). The rotation is computed in fp32 and rounded once. Returns the rotated q [T, n_heads,
     head_dim] (`out` if given). A token without a page, or past the tables, appends nothing and sets the device error
     DK_DEVERR_BAD_POSITION; one of an unused slot or of no sequence appends nothing and returns zeros."""
-    what = "paged_append"
+    return _append("paged_append", qkv, k_pages, v_pages, page_table, lengths, cos, sin, n_heads, n_kv, starts, offset, out, None)
+
+
+def _append(what, qkv, k_pages, v_pages, page_table, lengths, cos, sin, n_heads, n_kv, starts, offset, out, scales):
+    """`scales`: (k_scale, v_scale) of a cache of 4-bit codes, or None."""
     if qkv.dim() != 2:
         _refuse(what, "qkv must be [tokens, (n_heads + 2 n_kv) * head_dim]")
     T, width = qkv.shape
-    n_pages, kv, page, hd, B = _cache_shape(what, k_pages, v_pages, page_table, lengths, starts, T)
+    n_pages, kv, page, hd, B = _cache_shape(what, k_pages, v_pages, page_table, lengths, starts, T, scales is not None)
     ld, unit = qkv.stride()
     if n_kv != kv or n_heads <= 0 or width != (n_heads + 2 * n_kv) * hd or unit != 1:
         _refuse(what, "qkv must be [tokens, (n_heads + 2 n_kv) * head_dim] with the pages' kv heads and unit column stride")
@@ -97,8 +109,10 @@ def paged_append(qkv, k_pages, v_pages, page_table, lengths, cos, sin, n_heads, 
     if offset < 0:
         _refuse(what, "offset must not be negative")
     dtype = qkv.dtype
-    if dtype is not k_pages.dtype:
+    if dtype is not k_pages.dtype and scales is None:
         _wrong_type(what, f"qkv is {dtype}, the pages are {k_pages.dtype}")
+    if dtype not in _DTYPES:
+        _wrong_type(what, f"qkv must be fp16 or bf16, got {dtype}")
     f32 = cos.dtype is torch.float32
     if sin.dtype is not cos.dtype or not (f32 or cos.dtype is dtype):
         _wrong_type(what, "cos and sin must be fp32 or qkv's type")
@@ -106,11 +120,15 @@ def paged_append(qkv, k_pages, v_pages, page_table, lengths, cos, sin, n_heads, 
         _refuse(what, "out must be a contiguous [tokens, n_heads, head_dim] of qkv's type")
     device = _lib.current_device_of(what, (qkv, k_pages, v_pages, page_table, lengths, starts, cos, sin, out))
     q = qkv.new_empty_strided((T, n_heads, hd), (n_heads * hd, hd, 1)) if out is None else out
-    status = _lib.lib().dk_paged_append(_lib.PAGED_APPEND_ARGS.pack(
+    args = (
         qkv.data_ptr(), ld, k_pages.data_ptr(), v_pages.data_ptr(), n_pages, page, page_table.data_ptr(),
         page_table.stride()[0], page_table.shape[1], lengths.data_ptr(), 0 if starts is None else starts.data_ptr(),
         cos.data_ptr(), sin.data_ptr(), f32, ld_rope, cos.shape[0], offset, q.data_ptr(), T, B, n_heads, n_kv, hd,
-        _DTYPES[dtype], _raw_stream(device)))
+        _DTYPES[dtype], _raw_stream(device))
+    if scales is None:
+        status = _lib.lib().dk_paged_append(_lib.PAGED_APPEND_ARGS.pack(*args))
+    else:
+        status = _lib.lib().dk_paged_append_fp4(_lib.PAGED_APPEND_FP4_ARGS.pack(*args, *scales))
     if status:
         _lib.check(status, what)
     return q
@@ -123,19 +141,23 @@ def _workspace_bytes(T, B, nq, nkv, hd, dtype, ragged, prefix, device):
     return int(n.value)
 
 
-def _attend(what, entry, q, k_pages, v_pages, prefix_table, prefix_len, page_table, lengths, starts, window, sinks, scale, out):
+def _attend(what, entry, q, k_pages, v_pages, prefix_table, prefix_len, page_table, lengths, starts, window, sinks, scale, out,
+            scales=None):
+    """`scales`: (k_scale, v_scale) of a cache of 4-bit codes, or None."""
     if q.dim() != 3:
         _refuse(what, "q must be [tokens, heads, head_dim]")
     T, nq, width = q.shape
-    n_pages, n_kv, page, hd, B = _cache_shape(what, k_pages, v_pages, page_table, lengths, starts, T)
+    n_pages, n_kv, page, hd, B = _cache_shape(what, k_pages, v_pages, page_table, lengths, starts, T, scales is not None)
     ld, by_head, unit = q.stride()
     if width != hd or unit != 1 or by_head != hd and nq > 1 or ld < nq * hd and T > 1:
         _refuse(what, "q must be [tokens, heads, head_dim], a token's heads side by side and tokens apart from each other")
     if nq <= 0 or nq % n_kv or nq // n_kv > MAX_GROUP:
         _refuse(what, f"query heads must be a multiple of the kv heads, at most {MAX_GROUP} for each")
     dtype = q.dtype
-    if dtype is not k_pages.dtype:
+    if dtype is not k_pages.dtype and scales is None:
         _wrong_type(what, f"q is {dtype}, the pages are {k_pages.dtype}")
+    if dtype not in _DTYPES:
+        _wrong_type(what, f"q must be fp16 or bf16, got {dtype}")
     if out is None:
         out = q.new_empty_strided((T, nq, hd), (nq * hd, hd, 1))
     elif out.shape != q.shape or not out.is_contiguous() or out.dtype is not dtype:
@@ -153,11 +175,13 @@ def _attend(what, entry, q, k_pages, v_pages, prefix_table, prefix_len, page_tab
     # the prefix's length does not change the size, only whether there is one
     nbytes = _workspace_bytes(T, B, nq, n_kv, hd, code, starts is not None, 1 if prefix_len else 0, device)
     ws = q.new_empty_strided(((nbytes + 1) // 2,), (1,))  # (of a 16-bit type)
-    status = getattr(_lib.lib(), entry)(_lib.PAGED_ATTENTION_ARGS.pack(
+    args = (
         q.data_ptr(), ld, k_pages.data_ptr(), v_pages.data_ptr(), n_pages, page, prefix_at, prefix_len,
         page_table.data_ptr(), page_table.stride()[0], page_table.shape[1], lengths.data_ptr(),
         0 if starts is None else starts.data_ptr(), window, sinks, hd ** -0.5 if scale is None else scale, out.data_ptr(), T,
-        B, nq, n_kv, hd, code, ws.data_ptr(), nbytes, _raw_stream(device)))
+        B, nq, n_kv, hd, code, ws.data_ptr(), nbytes, _raw_stream(device))
+    pack = _lib.PAGED_ATTENTION_ARGS.pack(*args) if scales is None else _lib.PAGED_ATTENTION_FP4_ARGS.pack(*args, *scales)
+    status = getattr(_lib.lib(), entry)(pack)
     if status:
         _lib.check(status, what)
     return out

@@ -162,6 +162,9 @@ struct Problem {
   int rows_inner;
   int always_partial;  // no unit writes its output itself
   int* err;
+  // a cache held in 4 bits (paged_fp4.cuh)
+  const uint8_t* pool[2];  // k and v
+  float out_scale;         // what results are multiplied by: v's power of two; 1 for a 16-bit cache
 };
 
 // Positions of sequence b; an unused slot has none, however negative its length (positions counted back from the lowest
@@ -357,6 +360,20 @@ __device__ __forceinline__ int result_row(const Problem& p, int tok, int g) {
 }
 
 // ------------------------------------------------------------------------------------------- host
+constexpr int kMaxBatch = 4096;  // kOneToken: the chunk sums of a batch lie in shared memory
+
+// What a launch of a kernel for few rows takes: slots of its ring, shared memory, and the CTAs of one wave (0: it does not fit).
+struct RowsShape {
+  int ring;
+  size_t smem;
+  int ctas;
+};
+// Such a launch over a cache held in 4 bits (paged_attention_fp4.cu), with tiles of 8 or 16 rows; kFp4Groups pieces of the line a CTA.
+constexpr int kFp4Groups = 2;
+constexpr int kFp4Chunk = 64;
+RowsShape fp4_rows_shape(int64_t hd, int dtype, int rows);
+cudaError_t fp4_rows_launch(const Problem& p, int64_t hd, int dtype, int rows, const RowsShape& s, int wait_late, cudaStream_t st);
+
 // The launch of the 256-row tensor-core kernel (paged_attention_tc.cu): CTAs of one wave (0: it does not fit).
 constexpr int kTcChunk = 128;
 constexpr int kTcRows = 256;

@@ -20,10 +20,11 @@
 #include <climits>
 #include <mutex>
 
-#include "paged.cuh"
+#include "paged_fp4.cuh"
 
 namespace dk {
 namespace paged {
+int simple_fp4(const char* what, const dk_paged_attention_fp4_args* args, bool prefix);
 namespace {
 
 constexpr int kChunk = 64;
@@ -492,8 +493,8 @@ struct Joined {
         for (int i = 0; i < Shape::kParts - 1; ++i) add(part_ml[i][at.lane].x, part_ml[i][at.lane].y, part_o[i][at.lane]);
     }
   }
-  __device__ void store(T* out, int d4) const {
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+  __device__ void store(T* out, int d4, float scale) const {
+    const float inv = l == 0.f ? 0.f : scale / l;
     *reinterpret_cast<uint2*>(out + 4 * d4) = make_uint2(Elem<T>::pack(acc.x * inv, acc.y * inv), Elem<T>::pack(acc.z * inv, acc.w * inv));
   }
 };
@@ -531,7 +532,7 @@ __global__ void __launch_bounds__(Shape::kThreads) join_split_kernel(const Probl
   if (i < rows)
     sum.template add_part<Shape::kAhead>(p, w, at.part, Shape::kParts, tile_rows, result_row(p, i / p.G, i % p.G), at.d4);
   sum.join_parts(at);
-  if (at.part == 0 && i < rows) sum.store(out_row<T, kHd>(p, c.x + i / p.G, c.z * p.G + i % p.G), at.d4);
+  if (at.part == 0 && i < rows) sum.store(out_row<T, kHd>(p, c.x + i / p.G, c.z * p.G + i % p.G), at.d4, p.out_scale);
 }
 
 // Joins the prefix's results (`a`) with those of the sequences' own positions (`b`). Block (x, h): rows (token, head of
@@ -563,7 +564,7 @@ __global__ void __launch_bounds__(Shape::kThreads)
     }
   }
   sum.join_parts(at);
-  if (at.part == 0 && live) sum.store(out_row<T, kHd>(b, t, h * b.G + g), at.d4);
+  if (at.part == 0 && live) sum.store(out_row<T, kHd>(b, t, h * b.G + g), at.d4, b.out_scale);
 }
 
 }  // namespace
@@ -574,14 +575,6 @@ namespace {
 // Tiles that are cut into more pieces than this, on average, are joined in parts (42 tokens after 32768 positions: 28 us, 46
 // without; one short sequence 12.1, 12.2; 16 sequences of 8192 with 4 tokens each, 9 pieces a unit: 44, 40).
 constexpr int kFewPieces = 8;
-constexpr int kMaxBatch = 4096;  // kOneToken: the chunk sums of a batch lie in shared memory
-
-// What a rows_kernel launch takes: slots of its ring, shared memory, and the CTAs of one wave (0: it does not fit).
-struct RowsShape {
-  int ring;
-  size_t smem;
-  int ctas;
-};
 
 template <typename T, int kHd, int kRows>
 RowsShape rows_shape() {
@@ -611,9 +604,11 @@ struct Sizes {
   int64_t T, B, nq, nkv, hd, prefix_len;
   bool ragged;
   int dtype;
+  bool fp4;  // the cache is held in 4 bits
 };
 
 RowsShape rows_shape_of(const Sizes& z, int rows) {
+  if (z.fp4) return fp4_rows_shape(z.hd, z.dtype, rows);
 #define DK_SHAPE(TT) \
   (z.hd == 128 ? (rows == 8 ? rows_shape<TT, 128, 8>() : rows_shape<TT, 128, 16>()) \
                : (rows == 8 ? rows_shape<TT, 64, 8>() : rows_shape<TT, 64, 16>()))
@@ -623,6 +618,7 @@ RowsShape rows_shape_of(const Sizes& z, int rows) {
 
 cudaError_t launch_rows(const Sizes& z, int rows, const RowsShape& s, cudaStream_t st, const CUtensorMap& mk,
                         const CUtensorMap& mv, const Problem& p, int wait_late) {
+  if (z.fp4) return fp4_rows_launch(p, z.hd, z.dtype, rows, s, wait_late, st);
 #define DK_ROWS(TT, HH, RR) \
   launch(rows_kernel<TT, HH, RR>, dim3(s.ctas), dim3(kThreads), s.smem, st, pdl_enabled(), dim3(1, 1, 1), mk, mv, p, s.ring, wait_late)
 #define DK_ROWS_T(TT) \
@@ -662,7 +658,7 @@ void cut_pass(const Sizes& z, Cutter& c, Pass& a, bool always_partial) {
   } else {
     a.rows = z.nq / z.nkv <= 8 ? 8 : 16;
     a.shape = rows_shape_of(z, a.rows);
-    a.ctas = a.shape.ctas * kGroups;
+    a.ctas = a.shape.ctas * (z.fp4 ? kFp4Groups : kGroups);
     p.unit_extra = kRowsUnitExtra;
   }
   const int64_t tiles = p.mode == kRagged ? p.max_tiles : p.n_tiles;
@@ -781,21 +777,31 @@ uint64_t workspace_of(const Sizes& z) {
 using namespace dk;
 using namespace dk::paged;
 
-extern "C" int dk_paged_attention_workspace_bytes(int64_t T, int64_t B, int64_t nq, int64_t nkv, int64_t head_dim,
-                                                  int32_t dtype, int32_t ragged, int64_t prefix_len, uint64_t* bytes) {
-  const Sizes z{T, B, nq, nkv, head_dim, prefix_len, ragged != 0, dtype};
-  if (const int rc = check_sizes("paged_attention_workspace_bytes", z)) return rc;
-  if (!bytes) return set_error(DK_ERR_INVALID, "paged_attention_workspace_bytes: bytes is NULL");
+namespace {
+
+int workspace_bytes(const char* what, const Sizes& z, uint64_t* bytes) {
+  if (const int rc = check_sizes(what, z)) return rc;
+  if (!bytes) return set_error(DK_ERR_INVALID, "%s: bytes is NULL", what);
   *bytes = workspace_of(z);
   return DK_OK;
 }
 
+}  // namespace
+
+extern "C" int dk_paged_attention_workspace_bytes(int64_t T, int64_t B, int64_t nq, int64_t nkv, int64_t head_dim,
+                                                  int32_t dtype, int32_t ragged, int64_t prefix_len, uint64_t* bytes) {
+  return workspace_bytes("paged_attention_workspace_bytes", Sizes{T, B, nq, nkv, head_dim, prefix_len, ragged != 0, dtype, false}, bytes);
+}
+
+extern "C" int dk_paged_attention_fp4_workspace_bytes(int64_t T, int64_t B, int64_t nq, int64_t nkv, int64_t head_dim,
+                                                      int32_t dtype, int32_t ragged, int64_t prefix_len, uint64_t* bytes) {
+  return workspace_bytes("paged_attention_fp4_workspace_bytes", Sizes{T, B, nq, nkv, head_dim, prefix_len, ragged != 0, dtype, true}, bytes);
+}
+
 namespace {
 
-int attention(const char* what, const dk_paged_attention_args* args, bool prefix) {
-  if (args == nullptr) return set_error(DK_ERR_INVALID, "%s: NULL arguments", what);
-  const dk_paged_attention_args& a = *args;
-  const Sizes z{a.T, a.B, a.n_q, a.n_kv, a.head_dim, prefix ? a.prefix_len : 0, a.starts != nullptr, static_cast<int>(a.dtype)};
+int attention(const char* what, const dk_paged_attention_args& a, bool prefix, bool fp4, double k_scale, double v_scale) {
+  const Sizes z{a.T, a.B, a.n_q, a.n_kv, a.head_dim, prefix ? a.prefix_len : 0, a.starts != nullptr, static_cast<int>(a.dtype), fp4};
   const int64_t n_pages = a.n_pages, page_size = a.page_size, table_width = a.table_width;
   int64_t window = prefix ? 0 : a.window;
   int64_t sinks = prefix ? 0 : a.sinks;
@@ -811,6 +817,8 @@ int attention(const char* what, const dk_paged_attention_args* args, bool prefix
       window > INT32_MAX || sinks > INT32_MAX)
     return set_error(DK_ERR_INVALID,
                      "%s: pages x kv heads x page_size, window and sinks must stay below 2^31, a table row's positions with T 1024 below", what);
+  if (!fp4_power(k_scale) || !fp4_power(v_scale))
+    return set_error(DK_ERR_INVALID, "%s: k_scale and v_scale must be powers of two from 2^-64 to 2^64", what);
   // A window of all positions masks none, and sinks end with the positions: sums with them stay in range.
   window = std::min(window, table_width * page_size);
   sinks = std::min(sinks, table_width * page_size);
@@ -855,7 +863,9 @@ int attention(const char* what, const dk_paged_attention_args* args, bool prefix
     p->page_shift = __builtin_ctzll(page_size);
     p->capacity = static_cast<int>(table_width * page_size);
     p->mask = Mask{static_cast<int>(window), window > 0 ? static_cast<int>(sinks) : 0};
-    p->scale2 = static_cast<float>(a.scale * 1.44269504088896341);
+    p->scale2 = static_cast<float>(a.scale * k_scale * 1.44269504088896341);
+    p->pool[0] = static_cast<const uint8_t*>(a.k_pages), p->pool[1] = static_cast<const uint8_t*>(a.v_pages);
+    p->out_scale = static_cast<float>(v_scale);
     p->err = device_info().err_word;
   }
   for (Pass* s : {&own, &pre}) {  // the tiles take the scale's sign apart from it
@@ -885,7 +895,7 @@ int attention(const char* what, const dk_paged_attention_args* args, bool prefix
                const_cast<int32_t*>(own.p.plan), const_cast<int4*>(own.p.tile_info));
   for (const Pass* s : {&pre, &own}) {
     if (s->ctas == 0 || e != cudaSuccess) continue;
-    if (!page_maps(s->tc ? kTcChunk : kChunk)) return DK_ERR_CUDA;
+    if (!z.fp4 && !page_maps(s->tc ? kTcChunk : kChunk)) return DK_ERR_CUDA;
     if (s->tc) {
       if (const int rc = tc_launch(s->p, z.nq, z.hd, z.dtype, s->ctas, mk, mv, s == &own ? beside : 0, st)) return rc;
     } else {
@@ -905,8 +915,23 @@ int attention(const char* what, const dk_paged_attention_args* args, bool prefix
 
 }  // namespace
 
-extern "C" int dk_paged_attention(const dk_paged_attention_args* args) { return attention("paged_attention", args, false); }
+extern "C" int dk_paged_attention(const dk_paged_attention_args* args) {
+  if (args == nullptr) return set_error(DK_ERR_INVALID, "paged_attention: NULL arguments");
+  return attention("paged_attention", *args, false, false, 1., 1.);
+}
 
 extern "C" int dk_shared_prefix_attention(const dk_paged_attention_args* args) {
-  return attention("shared_prefix_attention", args, true);
+  if (args == nullptr) return set_error(DK_ERR_INVALID, "shared_prefix_attention: NULL arguments");
+  return attention("shared_prefix_attention", *args, true, false, 1., 1.);
+}
+
+extern "C" int dk_paged_attention_fp4(const dk_paged_attention_fp4_args* args) {
+  if (args == nullptr) return set_error(DK_ERR_INVALID, "paged_attention_fp4: NULL arguments");
+  if (args->attention.starts) return simple_fp4("paged_attention_fp4", args, false);
+  return attention("paged_attention_fp4", args->attention, false, true, args->k_scale, args->v_scale);
+}
+
+extern "C" int dk_shared_prefix_attention_fp4(const dk_paged_attention_fp4_args* args) {
+  if (args == nullptr) return set_error(DK_ERR_INVALID, "shared_prefix_attention_fp4: NULL arguments");
+  return simple_fp4("shared_prefix_attention_fp4", args, true);
 }

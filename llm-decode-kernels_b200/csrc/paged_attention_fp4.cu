@@ -1,10 +1,29 @@
-// Attention over a paged cache held in 4 bits, in its simplest form: a CTA for each row and kv head, whose warps take every
-// fourth position and join at the end.
+// Attention over a paged cache held in 4 bits for few query rows per kv head (decode steps).
+//
 //   out[t] = sum_j p[t][j] v[j],  p[t] = softmax over the visible j of scale * q[t] . k[j]
-// Row t at position p sees j <= p with (window <= 0 or j > p - window or j < sinks), and with a prefix all of it; a row that
-// sees nothing is zero. Everything is fp32 but the inputs and the output.
+// with the masks, units, pieces and joins of paged_attention.cu; here is the kernel between them.
+//
+// The bytes of k and v are 9/32 of a 16-bit cache's, so the conversion of codes competes with them: at the copy rate an SM gets
+// 41 values a cycle, and one costs at least a conversion and a product with its scale for each pair. So every value is converted
+// once, in registers, right in the place where the tensor-core product takes it from:
+// * the cache's values are the 16 rows of the product (m16n8k16), the query heads its 8 columns: S^T = K Q^T, O^T = V^T P^T.
+//   The other way round the 16 rows would be half empty for groups of up to 8 heads and each value would cost twice the products;
+// * a lane takes the codes of one position as 16 contiguous bytes (k: a quarter of the dims, in the order they lie in; the product's
+//   inner index runs over the dims in that order, and q is loaded to match) or 8 (v: 16 dims, one scale's). In v's product
+//   the inner index runs over positions, so the pairs that a register holds are of two positions: the halves of the bytes are
+//   exchanged between two positions' words first (four operations for eight registers);
+// * p in fp16 goes from the accumulators' layout to the operand's by transposing 8 x 8 blocks between lanes (movmatrix). The 16
+//   positions of a product are dealt to its rows such that each load of v reads 4 neighbouring positions: no bank conflicts.
+// code * scale is exact in fp16, and so is q once its row is scaled by a power of two (bf16 rows; their largest value comes to 2^14,
+// and what falls below 2^-24 there counts for nothing beside it): the products are those of the cache's values. p is rounded to
+// fp16 for the product with v; its reference is 2^6 below the maximum seen when it was set, and it is set anew when a score
+// passes it by 2^14, so that p has 38 binades above fp16's smallest step.
+// A producer warp a group streams chunks through a ring of bulk copies, as in the 16-bit kernel. A position that no row of the tile
+// sees gets a scale of zero in place of v's, whatever its page holds; a page outside the pool gets scales of zero in
+// shared memory. Codes are finite whatever they are.
 #include <algorithm>
 #include <climits>
+#include <mutex>
 
 #include "paged_fp4.cuh"
 
@@ -12,182 +31,473 @@ namespace dk {
 namespace paged {
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kMaxGroup = 16;
+constexpr int kCWarps = 4;  // warps of a group
+constexpr int kSub = 1;     // 16-position tiles of a warp in a chunk
+constexpr int kChunk = kFp4Chunk;
+static_assert(kChunk == kCWarps * kSub * 16, "a chunk is one round of the warps");
+constexpr int kThreads = kFp4Groups * (kCWarps + 1) * 32;
+constexpr int kMaxRing = 10;
+constexpr float kRefBelow = 6.f, kRefReach = 14.f;
 
-struct Simple {
-  const void* q;
-  int64_t ldq;
-  const uint8_t* pool[2];
-  void* out;
-  const int32_t* table;
-  int64_t ld_table;
-  const int32_t* lengths;
-  const int32_t* starts;
-  const int32_t* prefix_table;
-  int prefix_len;
-  int T, B, nkv, G, n_pages, page_size, page_shift, capacity;
-  Mask mask;
-  float scale2, v_power;
-  int* err;
+// A chunk in shared memory: for k and v each the codes of kChunk positions, then their scales.
+template <int kHd>
+struct Slot {
+  static constexpr int kScalesAt = kChunk * Fp4<kHd>::kCodes;
+  static constexpr int kTensor = kChunk * Fp4<kHd>::kRow;
+  static constexpr int kBytes = 2 * kTensor;
 };
 
-template <typename T, int kHd>
-__global__ void __launch_bounds__(kWarps * 32) simple_kernel(const Simple p) {
-  using F = Fp4<kHd>;
-  constexpr int kDims = kHd / 32;  // of a lane
-  __shared__ float q_sh[kMaxGroup][kHd];
-  __shared__ float o_sh[kWarps][kMaxGroup][kHd];
-  __shared__ float m_sh[kWarps][kMaxGroup], l_sh[kWarps][kMaxGroup];
-  pdl_trigger();
-  pdl_wait();
-  const int t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int b = t, pos;
-  if (p.starts == nullptr) {
-    pos = length_of(p.lengths, t) - 1;
-  } else {
-    b = find_tile_warp([&](int j) { return p.starts[j]; }, p.B, t, lane);
-    const int end = p.starts[b + 1];
-    pos = t >= p.starts[b] && t < end ? length_of(p.lengths, b) - (end - t) : -1;
-  }
-  for (int i = threadIdx.x; i < p.G * kHd; i += kWarps * 32)
-    q_sh[i / kHd][i % kHd] = static_cast<float>(static_cast<const T*>(p.q)[t * p.ldq + (h * p.G + i / kHd) * kHd + i % kHd]) * p.scale2;
-  if (pos >= p.capacity && threadIdx.x == 0) record_device_error(p.err, DK_DEVERR_BAD_POSITION);
-  __syncthreads();
-  float m[kMaxGroup], l[kMaxGroup], o[kMaxGroup][kDims];
-#pragma unroll
-  for (int g = 0; g < kMaxGroup; ++g) {
-    m[g] = -INFINITY, l[g] = 0.f;
-#pragma unroll
-    for (int d = 0; d < kDims; ++d) o[g][d] = 0.f;
-  }
-  // a lane's dims are kDims * lane on; values of a position, zeros without a page
-  auto value = [&](int which, int page, int j, float (&x)[kDims]) {
-    const uint8_t* block = p.pool[which] + (static_cast<int64_t>(page) * p.nkv + h) * p.page_size * F::kRow;
-    const int slot = j & (p.page_size - 1);
-    const float s = fp4_scale(block[p.page_size * F::kCodes + slot * F::kScales + kDims * lane / 16]);
-    uint32_t w[4];  // of the aligned four bytes that hold the lane's
-    fp4_codes(*reinterpret_cast<const uint32_t*>(block + slot * F::kCodes + (kDims * lane / 2 & ~3)), w);
-    if constexpr (kDims == 4) {
-      const float2 f = Elem<__half>::unpack(lane & 1 ? w[2] : w[0]), g = Elem<__half>::unpack(lane & 1 ? w[3] : w[1]);
-      x[0] = f.x * s, x[1] = f.y * s, x[2] = g.x * s, x[3] = g.y * s;
-    } else {
-      const uint32_t u = lane & 2 ? (lane & 1 ? w[3] : w[2]) : (lane & 1 ? w[1] : w[0]);
-      const float2 f = Elem<__half>::unpack(u);
-      x[0] = f.x * s, x[1] = f.y * s;
-    }
-  };
-  auto take = [&](const int32_t* table, int j) {
-    const int page = table[j >> p.page_shift];
-    const bool there = page >= 0 && page < p.n_pages;
-    if (!there) record_device_error(p.err, DK_DEVERR_BAD_POSITION);
-    float k[kDims] = {}, v[kDims] = {};
-    if (there) {
-      value(0, page, j, k);
-      value(1, page, j, v);
-    }
-#pragma unroll
-    for (int g = 0; g < kMaxGroup; ++g) {
-      if (g >= p.G) break;
-      float s = 0.f;
-#pragma unroll
-      for (int d = 0; d < kDims; ++d) s = fmaf(q_sh[g][kDims * lane + d], k[d], s);
-#pragma unroll
-      for (int i = 16; i > 0; i >>= 1) s += __shfl_xor_sync(0xffffffffu, s, i);
-      const float mx = fmaxf(m[g], s), keep = exp2f(m[g] - mx), w = exp2f(s - mx);
-      m[g] = mx, l[g] = fmaf(l[g], keep, w);
-#pragma unroll
-      for (int d = 0; d < kDims; ++d) o[g][d] = fmaf(o[g][d], keep, w * v[d]);
-    }
-  };
-  for (int j = warp; j < p.prefix_len; j += kWarps) take(p.prefix_table, j);
-  const int end = min(pos + 1, p.capacity);
-  const int lo = p.mask.window > 0 ? max(0, pos - p.mask.window + 1) : 0, sinks = min(p.mask.sinks, min(lo, end));
-  for (int i = warp; i < sinks + max(end - lo, 0); i += kWarps) take(p.table + b * p.ld_table, i < sinks ? i : lo + i - sinks);
-#pragma unroll
-  for (int g = 0; g < kMaxGroup; ++g) {
-    if (g >= p.G) break;
-    if (lane == 0) m_sh[warp][g] = m[g], l_sh[warp][g] = l[g];
-#pragma unroll
-    for (int d = 0; d < kDims; ++d) o_sh[warp][g][kDims * lane + d] = o[g][d];
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < p.G * kHd; i += kWarps * 32) {
-    const int g = i / kHd, d = i % kHd;
-    float mx = -INFINITY, sum = 0.f, acc = 0.f;
-    for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, m_sh[w][g]);
-    if (mx != -INFINITY)
-      for (int w = 0; w < kWarps; ++w) {
-        const float a = exp2f(m_sh[w][g] - mx);
-        sum = fmaf(a, l_sh[w][g], sum), acc = fmaf(a, o_sh[w][g][d], acc);
-      }
-    static_cast<T*>(p.out)[(static_cast<int64_t>(t) * p.nkv * p.G + h * p.G + g) * kHd + d] =
-        static_cast<T>(sum == 0.f ? 0.f : acc / sum * p.v_power);
-  }
+__device__ __forceinline__ void group_sync(int group) {
+  asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(kCWarps * 32) : "memory");
 }
 
-int attention_fp4(const char* what, const dk_paged_attention_fp4_args* args, bool prefix) {
-  if (args == nullptr) return set_error(DK_ERR_INVALID, "%s: NULL arguments", what);
-  const dk_paged_attention_args& a = args->attention;
-  const int64_t T = a.T, B = a.B, nq = a.n_q, nkv = a.n_kv, hd = a.head_dim, prefix_len = prefix ? a.prefix_len : 0;
-  const int64_t positions = a.table_width * a.page_size;
-  if (T < 0 || B < 0 || (B == 0 && T > 0) || nq <= 0 || nkv <= 0 || prefix_len < 0)
-    return set_error(DK_ERR_INVALID, "%s: bad sizes", what);
-  if (hd != 64 && hd != 128) return set_error(DK_ERR_UNSUPPORTED, "%s: head_dim %lld (64 or 128)", what, (long long)hd);
-  if (a.dtype != DK_F16 && a.dtype != DK_BF16) return set_error(DK_ERR_UNSUPPORTED, "%s: dtype %lld", what, (long long)a.dtype);
-  if (nq % nkv != 0 || nq / nkv > kMaxGroup)
-    return set_error(DK_ERR_UNSUPPORTED, "%s: %lld query heads over %lld kv heads (a multiple, at most 16 each)", what,
-                     (long long)nq, (long long)nkv);
-  if (a.starts == nullptr && T != B) return set_error(DK_ERR_INVALID, "%s: without starts there is one token per sequence", what);
-  if (a.n_pages <= 0 || a.table_width <= 0 || a.window < 0 || a.sinks < 0) return set_error(DK_ERR_INVALID, "%s: bad sizes", what);
-  if (a.page_size < 16 || a.page_size > 256 || (a.page_size & (a.page_size - 1)))
-    return set_error(DK_ERR_UNSUPPORTED, "%s: page_size %lld (a power of two from 16 to 256)", what, (long long)a.page_size);
-  if (a.n_pages > INT32_MAX || a.table_width > INT32_MAX || a.n_pages * nkv > INT32_MAX || a.n_pages * nkv * a.page_size > INT32_MAX ||
-      positions + T > (int64_t(1) << 31) - 1024 || a.window > INT32_MAX || a.sinks > INT32_MAX || prefix_len > (1 << 30) || nkv > 65535)
-    return set_error(DK_ERR_INVALID, "%s: sizes must stay below 2^31", what);
-  if (!fp4_power(args->k_scale) || !fp4_power(args->v_scale))
-    return set_error(DK_ERR_INVALID, "%s: k_scale and v_scale must be powers of two from 2^-64 to 2^64", what);
-  if (T == 0) return DK_OK;
-  const int64_t ldq = T > 1 ? a.ldq : nq * hd;
-  if (ldq < nq * hd) return set_error(DK_ERR_INVALID, "%s: q's tokens overlap", what);
-  if (!a.q || !a.k_pages || !a.v_pages || !a.page_table || !a.lengths || !a.out || (prefix_len > 0 && !a.prefix_table))
-    return set_error(DK_ERR_INVALID, "%s: NULL pointer", what);
-  if (!aligned16(a.q) || !aligned16(a.k_pages) || !aligned16(a.v_pages) || !aligned16(a.out) || (ldq & 7))
-    return set_error(DK_ERR_ALIGN, "%s: q rows, pages and out need 16-byte alignment", what);
-  Simple p;
-  p.q = a.q, p.ldq = ldq, p.out = a.out;
-  p.pool[0] = static_cast<const uint8_t*>(a.k_pages), p.pool[1] = static_cast<const uint8_t*>(a.v_pages);
-  p.table = a.page_table, p.ld_table = a.ld_table, p.lengths = a.lengths, p.starts = a.starts;
-  p.prefix_table = a.prefix_table, p.prefix_len = static_cast<int>(prefix_len);
-  p.T = static_cast<int>(T), p.B = static_cast<int>(B), p.nkv = static_cast<int>(nkv), p.G = static_cast<int>(nq / nkv);
-  p.n_pages = static_cast<int>(a.n_pages), p.page_size = static_cast<int>(a.page_size);
-  p.page_shift = __builtin_ctzll(a.page_size), p.capacity = static_cast<int>(positions);
-  const int64_t window = prefix ? 0 : std::min(a.window, positions), sinks = prefix ? 0 : std::min(a.sinks, positions);
-  p.mask = Mask{static_cast<int>(window), window > 0 ? static_cast<int>(sinks) : 0};
-  p.scale2 = static_cast<float>(a.scale * args->k_scale * 1.44269504088896341), p.v_power = static_cast<float>(args->v_scale);
-  p.err = device_info().err_word;
-  const dim3 grid(static_cast<unsigned>(T), static_cast<unsigned>(nkv));
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(a.stream);
-  cudaError_t e;
-#define DK_SIMPLE(TT) \
-  e = launch(hd == 128 ? simple_kernel<TT, 128> : simple_kernel<TT, 64>, grid, dim3(kWarps * 32), 0, st, pdl_enabled(), dim3(1, 1, 1), p)
-  if (a.dtype == DK_F16)
-    DK_SIMPLE(__half);
-  else
-    DK_SIMPLE(__nv_bfloat16);
-#undef DK_SIMPLE
-  if (e != cudaSuccess) return set_error(DK_ERR_CUDA, "%s launch: %s", what, cudaGetErrorString(e));
-  return DK_OK;
+// An 8 x 8 block of 16-bit values, a row's pair a lane, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
+  return d;
+}
+
+// Bits of a where m has ones, of b elsewhere.
+__device__ __forceinline__ uint32_t choose(uint32_t a, uint32_t b, uint32_t m) { return (a & m) | (b & ~m); }
+
+__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((127 + e) << 23); }
+
+template <typename T, int kHd, int kBlocks>
+__global__ void __launch_bounds__(kThreads, kBlocks == 1 ? 2 : 1) fp4_rows_kernel(const Problem p, int ring, int wait_late) {
+  using F = Fp4<kHd>;
+  using S = Slot<kHd>;
+  constexpr int kRows = 8 * kBlocks;      // query rows: the product's columns
+  constexpr int kSteps = kHd / 16;        // products of a tile of k, and tiles of v's product
+  constexpr int kWords = kHd / 32;        // words of a lane's codes of k; v's has kHd / 64
+  constexpr uint32_t kLow = 0x0f0f0f0fu;
+  __shared__ float pre_ml_sh[kFp4Groups][kCWarps * kRows * 2];
+  __shared__ float pre_w_sh[kFp4Groups][kCWarps * kRows];
+  __shared__ float fin_sh[kFp4Groups][kRows * 2];
+  __shared__ __align__(8) uint64_t full_sh[kFp4Groups][kMaxRing], empty_sh[kFp4Groups][kMaxRing];
+  __shared__ int warp_sum[kThreads / 32 + 1];
+  extern __shared__ __align__(128) uint8_t base[];
+  int* cum_sh = reinterpret_cast<int*>(base);  // [B + 1], before the first copies land there
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const bool producer = warp >= kFp4Groups * kCWarps;
+  const int group = producer ? warp - kFp4Groups * kCWarps : warp / kCWarps;
+  const int cta = blockIdx.x * kFp4Groups + group, ctas = gridDim.x * kFp4Groups;  // pieces of the line: one a group
+  uint8_t* slots = base + group * ring * S::kBytes;
+  float* pre_o = reinterpret_cast<float*>(base + kFp4Groups * ring * S::kBytes) + group * kCWarps * kRows * kHd;
+  float *pre_ml = pre_ml_sh[group], *pre_w = pre_w_sh[group], *fin = fin_sh[group];
+  uint64_t *full = full_sh[group], *empty = empty_sh[group];
+  if (tid == 0) {
+    for (int i = 0; i < kFp4Groups * kMaxRing; ++i) {
+      mbar_init(&full_sh[0][i], 1);
+      mbar_init(&empty_sh[0][i], kCWarps);
+    }
+    fence_mbar_init();
+  }
+  if (!wait_late) pdl_wait();
+  pdl_trigger();
+
+  Line line{cum_sh, 0, p.n_tiles, 0};
+  {  // every CTA sums up the sequences' chunks for itself
+    int carry = 0;
+    for (int b0 = 0; b0 < p.B; b0 += kThreads) {
+      const int b = b0 + tid;
+      int n = 0;
+      if (b < p.B) {
+        const int last = length_of(p.lengths, b) - 1;
+        n = Span<kChunk>(last, last, p.mask, p.capacity, p.page_size).n + p.unit_extra;
+      }
+      int s = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += u;
+      }
+      __syncthreads();
+      if (lane == 31) warp_sum[warp] = s;
+      __syncthreads();
+      int before = carry;
+      for (int w = 0; w < kThreads / 32; ++w) {
+        const int ws = warp_sum[w];
+        if (w < warp) before += ws;
+        carry += ws;
+      }
+      if (b < p.B) cum_sh[b] = before + s - n;
+    }
+    if (tid == 0) cum_sh[p.B] = carry;
+    line.chunks = carry;
+    __syncthreads();
+    if (blockIdx.x == 0)  // for the join kernel
+      for (int i = tid; i <= p.B; i += kThreads) p.cum_out[i] = cum_sh[i];
+  }
+  __syncthreads();
+
+  Walk<kChunk> walk(p, line, cta, ctas, lane);
+  __syncthreads();  // the sums have been read: copies may land on them
+  bool ok = true;
+  int fill = 0;  // ring fills so far
+
+  if (producer) {
+    // ---------------------------------------------------------------- producer warps: one lane per copy
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (the sums lay there)
+    const int box = min(p.page_size, kChunk);  // positions of one copy
+    const int boxes = kChunk / box;
+    const int kv = lane & 1, scales = (lane >> 1) & 1, pg = lane >> 2;
+    const int row_bytes = scales ? F::kScales : F::kCodes;
+    const uint32_t bytes = box * row_bytes;
+    const uint8_t* pool = p.pool[kv] + (scales ? p.page_size * F::kCodes : 0);
+    uint8_t* dst = slots + kv * S::kTensor + (scales ? S::kScalesAt : 0) + pg * bytes;
+    while (walk.more() && ok) {
+      const Span<kChunk> span = walk.step();
+      const int h = walk.h, c0 = walk.c0, c1 = walk.c1;
+      const int32_t* table = walk.t.table;
+      if (lane == 0 && walk.last >= p.capacity) record_device_error(p.err, DK_DEVERR_BAD_POSITION);  // cut to the table
+      // this lane's page in chunk i of the unit; INT_MIN: none, or nothing that a row sees
+      auto entry = [&](int i) {
+        const int j = i * kChunk + pg * box;
+        return i < c1 && pg < boxes && span.needs(j, box, p.mask) ? table[span.position(j) >> p.page_shift] : INT_MIN;
+      };
+      int next = entry(c0);
+      for (int i = c0; i < c1; ++i, ++fill) {
+        const int page = next;
+        next = entry(i + 1);
+        const int s = fill % ring;
+        if (fill >= ring && !wait_for(&empty[s], ((fill / ring) - 1) & 1, p.err, DK_DEVERR_WAIT_EMPTY)) ok = false;
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        uint8_t* at = dst + s * S::kBytes;
+        const bool wanted = page != INT_MIN, mine = wanted && page >= 0 && page < p.n_pages;
+        if (wanted && !mine) {  // no page of the pool: scales of zero
+          record_device_error(p.err, DK_DEVERR_BAD_POSITION);
+          if (scales)
+            for (uint32_t b = 0; b < bytes; b += 16) *reinterpret_cast<uint4*>(at + b) = make_uint4(0, 0, 0, 0);
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        const unsigned codes = __popc(__ballot_sync(0xffffffffu, mine && !scales)), grids = __popc(__ballot_sync(0xffffffffu, mine && scales));
+        if (lane == 0) mbar_arrive_expect_tx(&full[s], box * (codes * F::kCodes + grids * F::kScales));
+        __syncwarp();
+        if (mine) {
+          const int in_page = span.position(i * kChunk + pg * box) & (p.page_size - 1);
+          bulk_g2s(at, pool + (static_cast<int64_t>(page) * p.nkv + h) * (p.page_size * F::kRow) + in_page * row_bytes, bytes, &full[s]);
+        }
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------- consumer warps
+    const int g = lane >> 2, tq = lane & 3;
+    const int sub = warp % kCWarps, gtid = tid - group * kCWarps * 32;
+    const int row_a = (g >> 1) + 4 * (g & 1);  // the position of a tile in the products' row g; row g + 8 has the one 8 on
+    if (gtid == 0) p.cut[cta] = make_int4(0, 0, 0, 0);
+    while (walk.more()) {
+      const Span<kChunk> span = walk.step();
+      const Tile t = walk.t;
+      const int h = walk.h, c0 = walk.c0, c1 = walk.c1;
+      if (c1 <= c0) continue;
+      const int rows = p.G;  // one token's
+      const int p0 = t.p0 - span.shift;
+      // q as the products' column operand: column g has query row 8 * block + g, the lane its dims from tq * kHd / 4 on
+      uint32_t qb[kBlocks][kSteps][2];
+      float scale2[kBlocks][2];  // of columns 2 tq and 2 tq + 1
+#pragma unroll
+      for (int nb = 0; nb < kBlocks; ++nb) {
+        const int row = 8 * nb + g;
+        const T* qr = static_cast<const T*>(p.q) + t.t0 * p.ldq + (h * p.G + row) * kHd + tq * (kHd / 4);
+        uint4 raw[kSteps / 2];
+#pragma unroll
+        for (int i = 0; i < kSteps / 2; ++i)
+          raw[i] = row < rows ? *reinterpret_cast<const uint4*>(qr + 8 * i) : make_uint4(0, 0, 0, 0);
+        int e = 0;  // q is taken times 2^e
+        if constexpr (!std::is_same<T, __half>::value) {
+          float most = 0.f;
+#pragma unroll
+          for (int i = 0; i < kSteps / 2; ++i) {
+            const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float2 f = Elem<T>::unpack(w[k]);
+              most = fmaxf(most, fmaxf(fabsf(f.x), fabsf(f.y)));
+            }
+          }
+          most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+          most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+          e = most == 0.f ? 0 : min(100, 14 + 127 - static_cast<int>(__float_as_uint(most) >> 23));
+        }
+#pragma unroll
+        for (int i = 0; i < kSteps / 2; ++i) {
+          const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            uint32_t v = w[k];
+            if constexpr (!std::is_same<T, __half>::value) {
+              const float2 f = Elem<T>::unpack(v);
+              const float by = power_of_two(e);
+              v = Elem<__half>::pack(f.x * by, f.y * by);
+            }
+            qb[nb][2 * i + (k >> 1)][k & 1] = v;
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) scale2[nb][u] = p.scale2 * power_of_two(-__shfl_sync(0xffffffffu, e, 4 * (2 * tq + u)));
+      }
+      float o[kBlocks][kSteps][4];
+      float ref[kBlocks][2], l[kBlocks][2];
+#pragma unroll
+      for (int nb = 0; nb < kBlocks; ++nb) {
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) o[nb][i][0] = o[nb][i][1] = o[nb][i][2] = o[nb][i][3] = 0.f;
+        ref[nb][0] = ref[nb][1] = -INFINITY, l[nb][0] = l[nb][1] = 0.f;
+      }
+
+      for (int i = c0; i < c1; ++i, ++fill) {
+        const int s = fill % ring;
+        if (ok && !wait_for(&full[s], (fill / ring) & 1, p.err, DK_DEVERR_WAIT_FULL)) ok = false;
+        ok = __all_sync(0xffffffffu, ok);
+#pragma unroll
+        for (int tile = 0; tile < kSub; ++tile) {
+          const int r0 = 16 * (sub * kSub + tile), j0 = i * kChunk + r0;  // the warp's 16 positions
+          if (!ok || !span.needs(j0, 16, p.mask)) continue;
+          const uint8_t* kt = slots + s * S::kBytes;
+          const uint8_t* vt = kt + S::kTensor;
+          // S^T: rows are positions, columns query rows
+          float sc[kBlocks][4];
+#pragma unroll
+          for (int nb = 0; nb < kBlocks; ++nb) sc[nb][0] = sc[nb][1] = sc[nb][2] = sc[nb][3] = 0.f;
+          {
+            uint32_t kw[2][kWords], ks[2][2];  // codes and scales (of both halves of a lane's dims) of rows g and g + 8
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int r = r0 + row_a + 8 * e;
+              if constexpr (kHd == 128) {
+                const uint4 w = *reinterpret_cast<const uint4*>(kt + r * F::kCodes + 16 * tq);
+                kw[e][0] = w.x, kw[e][1] = w.y, kw[e][2] = w.z, kw[e][3] = w.w;
+                const uint32_t two = fp4_scales(*reinterpret_cast<const uint16_t*>(kt + S::kScalesAt + r * F::kScales + 2 * tq));
+                ks[e][0] = prmt(two, two, 0x1010), ks[e][1] = prmt(two, two, 0x3232);
+              } else {
+                const uint2 w = *reinterpret_cast<const uint2*>(kt + r * F::kCodes + 8 * tq);
+                kw[e][0] = w.x, kw[e][1] = w.y;
+                const uint32_t one = fp4_scales(kt[S::kScalesAt + r * F::kScales + tq]);
+                ks[e][0] = ks[e][1] = prmt(one, one, 0x1010);
+              }
+            }
+#pragma unroll
+            for (int w = 0; w < kWords; ++w) {
+              uint32_t a[2][4];
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                fp4_codes(kw[e][w], a[e]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) a[e][k] = hmul2_rn(a[e][k], ks[e][2 * w / kWords]);
+              }
+#pragma unroll
+              for (int nb = 0; nb < kBlocks; ++nb) {
+                mma_16816(sc[nb], a[0][0], a[1][0], a[0][1], a[1][1], qb[nb][2 * w][0], qb[nb][2 * w][1]);
+                mma_16816(sc[nb], a[0][2], a[1][2], a[0][3], a[1][3], qb[nb][2 * w + 1][0], qb[nb][2 * w + 1][1]);
+              }
+            }
+          }
+          // every row sees all 16 positions (nothing to mask)?
+          const bool clear = j0 + 15 <= p0 && (p.mask.window <= 0 || j0 > p0 - p.mask.window || j0 + 15 < p.mask.sinks) &&
+                             j0 + 15 < span.end;
+          uint32_t pb[kBlocks][2];  // p as the products' column operand
+#pragma unroll
+          for (int nb = 0; nb < kBlocks; ++nb) {
+            float y[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              y[e] = sc[nb][e] * scale2[nb][e & 1];
+              const int j = j0 + row_a + 8 * (e >> 1);
+              if (!clear && !(j < span.end && p.mask.sees(p0, j))) y[e] = -INFINITY;
+            }
+            bool raise = false;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const float top = fmaxf(y[u], y[u + 2]);
+              raise |= top > ref[nb][u] + kRefReach;  // (a reference of -inf: any score)
+            }
+            if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+              for (int u = 0; u < 2; ++u) {
+                float top = fmaxf(y[u], y[u + 2]);
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                if (top > ref[nb][u] + kRefReach) {
+                  const float to = top - kRefBelow, keep = exp2_approx(ref[nb][u] - to);
+                  ref[nb][u] = to;
+                  l[nb][u] *= keep;
+#pragma unroll
+                  for (int k = 0; k < kSteps; ++k) {
+                    o[nb][k][u] *= keep;
+                    o[nb][k][u + 2] *= keep;
+                  }
+                }
+              }
+            }
+            float w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              w[e] = exp2_approx(y[e] - (ref[nb][e & 1] == -INFINITY ? 0.f : ref[nb][e & 1]));
+              l[nb][e & 1] += w[e];
+            }
+            pb[nb][0] = transpose8(Elem<__half>::pack(w[0], w[1]));
+            pb[nb][1] = transpose8(Elem<__half>::pack(w[2], w[3]));
+          }
+          // O^T: rows are dims (row g of tile k: the lane's dim 2 k, row g + 8: 2 k + 1), the inner index runs over positions:
+          // the lane's four are tq, tq + 4, tq + 8, tq + 12
+          {
+            uint32_t vw[4][kHd / 64], vs[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int r = r0 + tq + 4 * e;
+              if constexpr (kHd == 128) {
+                const uint2 w = *reinterpret_cast<const uint2*>(vt + r * F::kCodes + 8 * g);
+                vw[e][0] = w.x, vw[e][1] = w.y;
+                vs[e] = vt[S::kScalesAt + r * F::kScales + g];
+              } else {
+                vw[e][0] = *reinterpret_cast<const uint32_t*>(vt + r * F::kCodes + 4 * g);
+                vs[e] = vt[S::kScalesAt + r * F::kScales + (g >> 1)];
+              }
+              if (!clear && !span.needs(i * kChunk + r, 1, p.mask)) vs[e] = 0;
+            }
+            const uint32_t s01 = fp4_scales(vs[0] | vs[1] << 8), s23 = fp4_scales(vs[2] | vs[3] << 8);
+#pragma unroll
+            for (int w = 0; w < kHd / 64; ++w) {
+              uint32_t a[4][4];
+              fp4_codes(choose(vw[0][w], vw[1][w] << 4, kLow), a[0]);
+              fp4_codes(choose(vw[0][w] >> 4, vw[1][w], kLow), a[1]);
+              fp4_codes(choose(vw[2][w], vw[3][w] << 4, kLow), a[2]);
+              fp4_codes(choose(vw[2][w] >> 4, vw[3][w], kLow), a[3]);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const uint32_t a0 = hmul2_rn(a[0][k], s01), a1 = hmul2_rn(a[1][k], s01), a2 = hmul2_rn(a[2][k], s23), a3 = hmul2_rn(a[3][k], s23);
+#pragma unroll
+                for (int nb = 0; nb < kBlocks; ++nb) mma_16816(o[nb][4 * w + k], a0, a1, a2, a3, pb[nb][0], pb[nb][1]);
+              }
+            }
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[s]);
+      }
+      // the warps' results of this part of the unit, joined
+      if (gtid == 0 && walk.cut(span)) p.cut[cta] = walk.cut_record(span);
+#pragma unroll
+      for (int nb = 0; nb < kBlocks; ++nb)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          float sum = l[nb][u];
+          sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+          const int row = sub * kRows + 8 * nb + 2 * tq + u;
+          float* to = &pre_o[row * kHd + g * (kHd / 8)];
+#pragma unroll
+          for (int k = 0; k < kSteps; k += 2)
+            *reinterpret_cast<float4*>(to + 2 * k) = make_float4(o[nb][k][u], o[nb][k][u + 2], o[nb][k + 1][u], o[nb][k + 1][u + 2]);
+          if (g == 0) {
+            pre_ml[row * 2] = ref[nb][u];
+            pre_ml[row * 2 + 1] = sum;
+          }
+        }
+      group_sync(group);
+      const bool all_of_it = c0 == 0 && c1 == span.n, whole = all_of_it && !p.always_partial;
+      if (gtid < kRows) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kCWarps; ++w) mx = fmaxf(mx, pre_ml[(w * kRows + gtid) * 2]);
+        const float m_use = mx == -INFINITY ? 0.f : mx;
+        float ls = 0.f;
+#pragma unroll
+        for (int w = 0; w < kCWarps; ++w) {
+          const float wt = exp2_approx(pre_ml[(w * kRows + gtid) * 2] - m_use);
+          pre_w[w * kRows + gtid] = wt;
+          ls = fmaf(wt, pre_ml[(w * kRows + gtid) * 2 + 1], ls);
+        }
+        fin[2 * gtid] = mx;
+        fin[2 * gtid + 1] = ls;
+      }
+      group_sync(group);
+      const int64_t slot = partial_slot(ctas, cta, c0 == 0, all_of_it, h * line.tiles + walk.ti);
+      if (ok) {
+        for (int e = gtid; e < rows * (kHd / 4); e += kCWarps * 32) {
+          const int row = e / (kHd / 4), d = 4 * (e % (kHd / 4));
+          float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int w = 0; w < kCWarps; ++w) {
+            const float wt = pre_w[w * kRows + row];
+            const float4 v = *reinterpret_cast<const float4*>(&pre_o[(w * kRows + row) * kHd + d]);
+            a.x = fmaf(wt, v.x, a.x), a.y = fmaf(wt, v.y, a.y), a.z = fmaf(wt, v.z, a.z), a.w = fmaf(wt, v.w, a.w);
+          }
+          if (whole) {
+            const float sum = fin[2 * row + 1];
+            const float inv = sum == 0.f ? 0.f : p.out_scale / sum;
+            T* dst = static_cast<T*>(p.out) + (static_cast<int64_t>(t.t0) * p.nkv * p.G + h * p.G + row) * kHd + d;
+            *reinterpret_cast<uint2*>(dst) = make_uint2(Elem<T>::pack(a.x * inv, a.y * inv), Elem<T>::pack(a.z * inv, a.w * inv));
+          } else {
+            *reinterpret_cast<float4*>(&p.part_o[(slot * kRows + row) * kHd + d]) = a;
+          }
+        }
+        if (!whole && gtid < rows)
+          *reinterpret_cast<float2*>(&p.part_ml[(slot * kRows + gtid) * 2]) = make_float2(fin[2 * gtid], fin[2 * gtid + 1]);
+      }
+      group_sync(group);  // pre_o, pre_ml and fin are written again by the next piece
+    }
+  }
+  if (__syncthreads_or(!ok) && producer && lane == 0) {
+    // a wait gave up: let copies still in flight land before the shared memory goes away (bounded)
+    const uint64_t t0 = globaltimer_ns();
+    for (int f = max(0, fill - ring); f < fill; ++f)
+      while (!mbar_try_wait(&full[f % ring], (f / ring) & 1) && globaltimer_ns() - t0 < 500000000ull) {
+      }
+  }
+  if (wait_late) pdl_wait();
+}
+
+template <typename T, int kHd, int kBlocks>
+RowsShape shape() {
+  static std::mutex mu;
+  static int per_sm[64];  // by device; 0: not asked yet
+  RowsShape s;
+  s.ring = kHd == 64 ? (kBlocks == 1 ? 8 : 10) : (kBlocks == 1 ? 4 : 6);
+  s.smem = static_cast<size_t>(kFp4Groups) * (s.ring * Slot<kHd>::kBytes + kCWarps * 8 * kBlocks * kHd * 4);
+  static_assert((kMaxBatch + 1) * 4 <= kFp4Groups * 4 * Slot<128>::kBytes && (kMaxBatch + 1) * 4 <= kFp4Groups * 8 * Slot<64>::kBytes,
+                "the chunk sums fit the ring");
+  int dev = 0;
+  cudaGetDevice(&dev);
+  std::lock_guard<std::mutex> lock(mu);
+  int& n = per_sm[dev & 63];
+  if (n == 0) {
+    auto k = fp4_rows_kernel<T, kHd, kBlocks>;
+    if (opt_in_dynamic_smem(k) < static_cast<int>(s.smem) ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k, kThreads, s.smem) != cudaSuccess) {
+      cudaGetLastError();
+      n = 0;
+    }
+  }
+  s.ctas = n * device_info().num_sms;
+  return s;
 }
 
 }  // namespace
+
+#define DK_BY_KIND(CALL)                                                                                          \
+  (dtype == DK_F16 ? (hd == 128 ? (rows == 8 ? CALL(__half, 128, 1) : CALL(__half, 128, 2))                       \
+                                : (rows == 8 ? CALL(__half, 64, 1) : CALL(__half, 64, 2)))                        \
+                   : (hd == 128 ? (rows == 8 ? CALL(__nv_bfloat16, 128, 1) : CALL(__nv_bfloat16, 128, 2))         \
+                                : (rows == 8 ? CALL(__nv_bfloat16, 64, 1) : CALL(__nv_bfloat16, 64, 2))))
+
+RowsShape fp4_rows_shape(int64_t hd, int dtype, int rows) {
+#define DK_SHAPE(TT, HH, NB) shape<TT, HH, NB>()
+  return DK_BY_KIND(DK_SHAPE);
+#undef DK_SHAPE
+}
+
+cudaError_t fp4_rows_launch(const Problem& p, int64_t hd, int dtype, int rows, const RowsShape& s, int wait_late, cudaStream_t st) {
+#define DK_ROWS(TT, HH, NB) \
+  launch(fp4_rows_kernel<TT, HH, NB>, dim3(s.ctas), dim3(kThreads), s.smem, st, pdl_enabled(), dim3(1, 1, 1), p, s.ring, wait_late)
+  return DK_BY_KIND(DK_ROWS);
+#undef DK_ROWS
+}
+
 }  // namespace paged
 }  // namespace dk
-
-extern "C" int dk_paged_attention_fp4(const dk_paged_attention_fp4_args* args) {
-  return dk::paged::attention_fp4("paged_attention_fp4", args, false);
-}
-
-extern "C" int dk_shared_prefix_attention_fp4(const dk_paged_attention_fp4_args* args) {
-  return dk::paged::attention_fp4("shared_prefix_attention_fp4", args, true);
-}

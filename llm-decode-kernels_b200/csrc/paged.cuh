@@ -378,9 +378,9 @@ cudaError_t fp4_rows_launch(const Problem& p, int64_t hd, int dtype, int rows, c
 constexpr int kTcChunk = 128;
 constexpr int kTcRows = 256;
 constexpr int kTcUnitExtra = 3;  // a unit's fixed cost (its Q, first and last steps, output) in chunks (2, 4: up to 2 us more)
-int tc_ctas(int64_t head_dim, int dtype);
-// mk, mv: the pages as rows of head_dim, in boxes of 64 dims of min(page_size, kTcChunk) rows, 128-byte swizzle.
-int tc_launch(const Problem& p, int64_t nq, int64_t head_dim, int dtype, int ctas, const CUtensorMap& mk,
+int tc_ctas(int64_t hd, int dtype, bool fp4);
+// mk, mv: the pages as rows of head_dim, in boxes of 64 dims of min(page_size, kTcChunk) rows, 128-byte swizzle (not used with fp4).
+int tc_launch(const Problem& p, int64_t nq, int64_t hd, int dtype, bool fp4, int ctas, const CUtensorMap& mk,
               const CUtensorMap& mv, int wait_late, cudaStream_t st);
 
 }  // namespace paged

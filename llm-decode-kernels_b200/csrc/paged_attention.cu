@@ -24,7 +24,6 @@
 
 namespace dk {
 namespace paged {
-int simple_fp4(const char* what, const dk_paged_attention_fp4_args* args, bool prefix);
 namespace {
 
 constexpr int kChunk = 64;
@@ -646,6 +645,7 @@ struct Pass {
   bool tc;  // 256-row tiles on the tensor-core kernel
   RowsShape shape;
   int rows, ctas;
+  int groups;  // of a CTA, each with a piece of the line (not tc)
 };
 
 void cut_pass(const Sizes& z, Cutter& c, Pass& a, bool always_partial) {
@@ -654,11 +654,12 @@ void cut_pass(const Sizes& z, Cutter& c, Pass& a, bool always_partial) {
     a.rows = kTcRows;
     p.unit_extra = kTcUnitExtra;
     p.rows_inner = 1;
-    a.ctas = tc_ctas(z.hd, z.dtype);
+    a.ctas = tc_ctas(z.hd, z.dtype, z.fp4);
   } else {
     a.rows = z.nq / z.nkv <= 8 ? 8 : 16;
     a.shape = rows_shape_of(z, a.rows);
-    a.ctas = a.shape.ctas * (z.fp4 ? kFp4Groups : kGroups);
+    a.groups = z.fp4 ? kFp4Groups : kGroups;
+    a.ctas = a.shape.ctas * a.groups;
     p.unit_extra = kRowsUnitExtra;
   }
   const int64_t tiles = p.mode == kRagged ? p.max_tiles : p.n_tiles;
@@ -707,7 +708,7 @@ void share_gpu(Pass& pre, Pass& own) {
   const int64_t n = static_cast<int64_t>((pre.p.prefix_len + kTcChunk - 1) / kTcChunk + pre.p.unit_extra) * pre.p.n_tiles * pre.p.nkv;
   const int64_t most = sms * 7 / 8, per = (n + most - 1) / most;
   pre.ctas = static_cast<int>((n + per - 1) / per);
-  own.p.early = kGroups * (sms - pre.ctas);
+  own.p.early = own.groups * (sms - pre.ctas);
   own.p.lead = static_cast<int>((60 + 20 * per) / 11);
 }
 
@@ -897,7 +898,7 @@ int attention(const char* what, const dk_paged_attention_args& a, bool prefix, b
     if (s->ctas == 0 || e != cudaSuccess) continue;
     if (!z.fp4 && !page_maps(s->tc ? kTcChunk : kChunk)) return DK_ERR_CUDA;
     if (s->tc) {
-      if (const int rc = tc_launch(s->p, z.nq, z.hd, z.dtype, s->ctas, mk, mv, s == &own ? beside : 0, st)) return rc;
+      if (const int rc = tc_launch(s->p, z.nq, z.hd, z.dtype, z.fp4, s->ctas, mk, mv, s == &own ? beside : 0, st)) return rc;
     } else {
       e = launch_rows(z, s->rows, s->shape, st, mk, mv, s->p, s == &own ? beside : 0);
     }
@@ -927,11 +928,10 @@ extern "C" int dk_shared_prefix_attention(const dk_paged_attention_args* args) {
 
 extern "C" int dk_paged_attention_fp4(const dk_paged_attention_fp4_args* args) {
   if (args == nullptr) return set_error(DK_ERR_INVALID, "paged_attention_fp4: NULL arguments");
-  if (args->attention.starts) return simple_fp4("paged_attention_fp4", args, false);
   return attention("paged_attention_fp4", args->attention, false, true, args->k_scale, args->v_scale);
 }
 
 extern "C" int dk_shared_prefix_attention_fp4(const dk_paged_attention_fp4_args* args) {
   if (args == nullptr) return set_error(DK_ERR_INVALID, "shared_prefix_attention_fp4: NULL arguments");
-  return simple_fp4("shared_prefix_attention_fp4", args, true);
+  return attention("shared_prefix_attention_fp4", args->attention, true, true, args->k_scale, args->v_scale);
 }

@@ -173,6 +173,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks == 1 ? 2 : 1) fp4_rows_kerne
             for (uint32_t b = 0; b < bytes; b += 16) *reinterpret_cast<uint4*>(at + b) = make_uint4(0, 0, 0, 0);
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
+        __syncwarp();
         const unsigned codes = __popc(__ballot_sync(0xffffffffu, mine && !scales)), grids = __popc(__ballot_sync(0xffffffffu, mine && scales));
         if (lane == 0) mbar_arrive_expect_tx(&full[s], box * (codes * F::kCodes + grids * F::kScales));
         __syncwarp();

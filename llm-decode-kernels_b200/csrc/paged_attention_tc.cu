@@ -27,7 +27,7 @@
 #include <climits>
 #include <mutex>
 
-#include "paged.cuh"
+#include "paged_fp4.cuh"
 #include "tcgen05.cuh"
 
 namespace dk {
@@ -35,7 +35,8 @@ namespace paged {
 namespace {
 
 constexpr int kThreads = 384;
-constexpr int kMmaWarp = 8, kLoadWarp = 9, kZeroWarp = 10;  // warp 11 only gives its registers away
+constexpr int kMmaWarp = 8, kLoadWarp = 9, kZeroWarp = 10;  // without kFp4 warp 11 only gives its registers away
+constexpr int kConvertWarp = 10, kConvertWarps = 2;         // kFp4
 // The launch holds 168 registers a thread; the softmax warpgroups take what the third one gives up:
 // 256 * 208 + 128 * 88 = 384 * 168.
 constexpr int kRegsLaunch = 168, kRegsSoftmax = 208, kRegsOther = 88;
@@ -48,18 +49,24 @@ constexpr float kLazy = 8.f;  // growth (base 2) of a row's maximum that P takes
 constexpr int kPartChunks = 3;  // 32-position chunks of the first part
 constexpr int kPartSteps = 2 * kPartChunks;  // its products of 16 positions each
 
-template <int kHd>
+template <int kHd, bool kFp4>
 struct Smem {
   static constexpr int kSegs = kHd / 64;
   static constexpr int kSegBytes = 128 * 128;            // 128 rows of 64 dims
   static constexpr int kTileBytes = kSegs * kSegBytes;   // Q half, K chunk or V chunk
-  static constexpr int kSlots = kHd == 128 ? 5 : 10;
-  static constexpr int kBytes = 1024 + (2 + kSlots) * kTileBytes;
+  static constexpr int kSlots = (kHd == 128 ? 5 : 10) - (kFp4 ? (kHd == 128 ? 1 : 2) : 0);
+  // kFp4: a K or V chunk as it lies in the pages, its codes before its scales
+  static constexpr int kRawScalesAt = kC * Fp4<kHd>::kCodes;
+  static constexpr int kRawBytes = kC * Fp4<kHd>::kRow;
+  static constexpr int kRaw = kFp4 ? (kHd == 128 ? 3 : 6) : 0;
+  static constexpr int kBytes = 1024 + (2 + kSlots) * kTileBytes + kRaw * kRawBytes;
 };
 
 struct Barriers {
   uint64_t kv_full[10], kv_empty[10];
-  uint64_t q_full, q_empty;
+  uint64_t q_full[2], q_empty;  // kFp4: a half's own; otherwise the first of both
+  uint64_t q_ready[2];          // kFp4, bf16: the half's Q is in fp16
+  uint64_t raw_full[6], raw_empty[6];  // kFp4
   uint64_t s_full[2], p_full[2][2], o_full[2];  // p_full: [half][the two parts of P]
   uint64_t drain;
 };
@@ -194,17 +201,47 @@ __device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* m
       : "memory");
 }
 
-template <typename T, int kHd>
+// kFp4. A row of Q in shared memory from bf16 to fp16, times the power of two that brings its largest value to 2^14: what falls
+// below fp16's smallest step then is 2^-38 of that. Returns the power's exponent. One thread per row; swizzled 16-byte pieces are
+// taken in an order that spreads a warp's rows over the banks.
+template <int kHd, bool kFp4>
+__device__ __forceinline__ int q_to_fp16(uint8_t* row, int r) {
+  using L = Smem<kHd, kFp4>;
+  uint4 w[kHd / 8];
+  uint32_t most = 0;
+#pragma unroll
+  for (int i = 0; i < kHd / 8; ++i) {
+    w[i] = *reinterpret_cast<const uint4*>(row + (i >> 3) * L::kSegBytes + (((i & 7) ^ (r & 7)) << 4));
+    const uint32_t m = 0x7fff7fffu;
+    most = __vmaxu2(most, __vmaxu2(__vmaxu2(w[i].x & m, w[i].y & m), __vmaxu2(w[i].z & m, w[i].w & m)));
+  }
+  most = max(most >> 16, most & 0xffffu);
+  const int e = most == 0 ? 0 : min(100, 14 + 127 - static_cast<int>(most >> 7));
+  const float by = __int_as_float((127 + e) << 23);
+  auto turn = [&](uint32_t v) {
+    const float2 f = Elem<__nv_bfloat16>::unpack(v);
+    return Elem<__half>::pack(f.x * by, f.y * by);
+  };
+#pragma unroll
+  for (int i = 0; i < kHd / 8; ++i)
+    *reinterpret_cast<uint4*>(row + (i >> 3) * L::kSegBytes + (((i & 7) ^ (r & 7)) << 4)) =
+        make_uint4(turn(w[i].x), turn(w[i].y), turn(w[i].z), turn(w[i].w));
+  return e;
+}
+
+template <typename T, int kHd, bool kFp4>
 __global__ void __launch_bounds__(kThreads, 1)
     tiles_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                  const __grid_constant__ CUtensorMap mv, const Problem p, int wait_late) {
-  using L = Smem<kHd>;
-  using E = Elem<T>;
+  using L = Smem<kHd, kFp4>;
+  using M = typename std::conditional<kFp4, __half, T>::type;  // of the products' operands
+  constexpr bool kTurnQ = kFp4 && !std::is_same<T, __half>::value;
   constexpr uint32_t kS[2] = {0, 128}, kO[2] = {256, 256 + kHd};  // tensor-memory columns; P(X) lies over S(X)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
   uint8_t* q_sm = smem;
   uint8_t* slots = smem + 2 * L::kTileBytes;
+  uint8_t* raw = slots + L::kSlots * L::kTileBytes;
   __shared__ __align__(8) Barriers bar;
   __shared__ uint32_t tmem_slot;
   __shared__ int failed;
@@ -212,12 +249,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     for (int i = 0; i < L::kSlots; ++i) {
-      mbar_init(&bar.kv_full[i], 1);
+      mbar_init(&bar.kv_full[i], kFp4 ? kConvertWarps : 1);
       mbar_init(&bar.kv_empty[i], 1);
     }
-    mbar_init(&bar.q_full, 1);
+    for (int i = 0; i < L::kRaw; ++i) {
+      mbar_init(&bar.raw_full[i], 1);
+      mbar_init(&bar.raw_empty[i], kConvertWarps);
+    }
     mbar_init(&bar.q_empty, 1);
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&bar.q_full[i], 1);
+      mbar_init(&bar.q_ready[i], 4);
       mbar_init(&bar.s_full[i], 1);
       mbar_init(&bar.p_full[i][0], 4);
       mbar_init(&bar.p_full[i][1], 4);
@@ -227,8 +269,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     failed = 0;
     fence_mbar_init();
     prefetch_tensormap(&mq);
-    prefetch_tensormap(&mk);
-    prefetch_tensormap(&mv);
+    if constexpr (!kFp4) {
+      prefetch_tensormap(&mk);
+      prefetch_tensormap(&mv);
+    }
   }
   if (warp == kMmaWarp) {
     tc::tmem_alloc(&tmem_slot, 512);
@@ -249,8 +293,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == kLoadWarp) {
     // ---------------------------------------------------------------- loads
     const int box = min(p.page_size, kC), boxes = kC / box;
-    const int sg = lane % L::kSegs, pg = lane / L::kSegs;
+    const int sg = lane % L::kSegs, pg = kFp4 ? lane >> 1 : lane / L::kSegs;
     int fill = 0;
+    // kFp4: a lane copies the codes or the scales of its page
+    const int row_bytes = lane & 1 ? Fp4<kHd>::kScales : Fp4<kHd>::kCodes;
     for (int part = 0; walk.more() && ok; ++part) {
       const Span<kC> span = walk.step();
       if (walk.c1 <= walk.c0) {
@@ -281,31 +327,68 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         ++fill;
       };
+      auto put_raw = [&](int kv, int i, int page) {
+        const int s = fill % max(L::kRaw, 1);
+        if (fill >= L::kRaw && !wait_for(&bar.raw_empty[s], ((fill / max(L::kRaw, 1)) - 1) & 1, p.err, DK_DEVERR_WAIT_EMPTY)) ok = false;
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) return;
+        const uint32_t bytes = box * row_bytes;
+        uint8_t* at = raw + s * L::kRawBytes + (lane & 1 ? L::kRawScalesAt : 0) + pg * bytes;
+        const bool wanted = page != INT_MIN, mine = wanted && page >= 0 && page < p.n_pages;
+        if (wanted && !mine) {  // no page of the pool: scales of zero
+          record_device_error(p.err, DK_DEVERR_BAD_POSITION);
+          if (lane & 1)
+            for (uint32_t b = 0; b < bytes; b += 16) *reinterpret_cast<uint4*>(at + b) = make_uint4(0, 0, 0, 0);
+          tc::fence_proxy_async_smem();
+        }
+        __syncwarp();
+        const unsigned pages = __popc(__ballot_sync(0xffffffffu, mine)) / 2;
+        if (lane == 0) mbar_arrive_expect_tx(&bar.raw_full[s], pages * box * Fp4<kHd>::kRow);
+        __syncwarp();
+        if (mine) {
+          const int in_page = span.position(i * kC + pg * box) & (p.page_size - 1);
+          bulk_g2s(at, p.pool[kv] + (static_cast<int64_t>(page) * p.nkv + h) * (p.page_size * Fp4<kHd>::kRow) +
+                           (lane & 1 ? p.page_size * Fp4<kHd>::kCodes : 0) + in_page * row_bytes,
+                   bytes, &bar.raw_full[s]);
+        }
+        ++fill;
+      };
+      auto put_chunk = [&](int kv, int i, int page) {
+        if constexpr (kFp4)
+          put_raw(kv, i, page);
+        else
+          put(kv ? &mv : &mk, i, page);
+      };
       int page = entry(c0);
       // Q, once the last part's products with it have completed
       if (part > 0 && !wait_for(&bar.q_empty, (part - 1) & 1, p.err, DK_DEVERR_WAIT_EMPTY)) ok = false;
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       if (lane == 0) {
-        mbar_arrive_expect_tx(&bar.q_full, (two ? 2 : 1) * L::kSegs * p.half_tokens * p.G * 128);
-        for (int x = 0; x < (two ? 2 : 1); ++x)
+        if constexpr (!kFp4) mbar_arrive_expect_tx(&bar.q_full[0], (two ? 2 : 1) * L::kSegs * p.half_tokens * p.G * 128);
+        for (int x = 0; x < (two ? 2 : 1); ++x) {
+          if constexpr (kFp4) mbar_arrive_expect_tx(&bar.q_full[x], L::kSegs * p.half_tokens * p.G * 128);
           for (int s = 0; s < L::kSegs; ++s)
             tma_load_3d(q_sm + x * L::kTileBytes + s * L::kSegBytes, &mq, s * 64, h * p.G,
-                        p.signs == 0 ? p.T : walk.t.t0 + x * p.half_tokens, &bar.q_full);  // (past the end: zeros)
+                        p.signs == 0 ? p.T : walk.t.t0 + x * p.half_tokens, &bar.q_full[kFp4 ? x : 0]);  // (past the end: zeros)
+        }
       }
       __syncwarp();
-      put(&mk, c0, page);
+      put_chunk(0, c0, page);
       for (int i = c0; i < c1 && ok; ++i) {
         const int next = entry(i + 1);
-        put(&mv, i, page);
-        if (i + 1 < c1 && ok) put(&mk, i + 1, next);
+        put_chunk(1, i, page);
+        if (i + 1 < c1 && ok) put_chunk(0, i + 1, next);
         page = next;
       }
     }
   } else if (warp == kMmaWarp) {
     // ---------------------------------------------------------------- products
     int fill = 0;         // ring slots consumed
-    unsigned p_seen[2] = {0, 0};
+    unsigned p_seen[2] = {0, 0}, q_seen[2] = {0, 0};
+    auto q_wait = [&](int x) {
+      if (!wait_for(kTurnQ ? &bar.q_ready[x] : &bar.q_full[x], q_seen[x]++ & 1, p.err, DK_DEVERR_WAIT_FULL)) ok = false;
+    };
     auto slot_wait = [&](int f) {
       if (ok && !wait_for(&bar.kv_full[f % L::kSlots], (f / L::kSlots) & 1, p.err, DK_DEVERR_WAIT_FULL)) ok = false;
       ok = __all_sync(0xffffffffu, ok);
@@ -316,7 +399,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int k = 0; k < kHd / 16; ++k) {
         const uint32_t off = ((k / 4) * L::kSegBytes + (k % 4) * 32) >> 4;  // (descriptors count 16 bytes)
-        mma_ss(tmem + kS[x], a + off, b + off, idesc<T>(128, kC, false) | (p.signs < 0 ? kNegateA : 0u), k > 0);
+        mma_ss(tmem + kS[x], a + off, b + off, idesc<M>(128, kC, false) | (p.signs < 0 ? kNegateA : 0u), k > 0);
       }
       commit_elected(&bar.s_full[x]);
     };
@@ -330,19 +413,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc::fence_after_sync();
 #pragma unroll
         for (int k = half * kPartSteps; k < (half ? kC / 16 : kPartSteps); ++k)
-          mma_ts(tmem + kO[x], tmem + kS[x] + 8 * k, b + ((k * 2048) >> 4), idesc<T>(128, kHd, true), !first || k > 0);
+          mma_ts(tmem + kO[x], tmem + kS[x] + 8 * k, b + ((k * 2048) >> 4), idesc<M>(128, kHd, true), !first || k > 0);
       }
       ++p_seen[x];
     };
-    for (int part = 0; walk.more() && ok; ++part) {
+    while (walk.more() && ok) {
       const Span<kC> span = walk.step();
       const int n = walk.c1 - walk.c0;
-      if (n <= 0) {
-        --part;
-        continue;
-      }
+      if (n <= 0) continue;
       const bool two = walk.t.ntok > p.half_tokens;
-      if (!wait_for(&bar.q_full, part & 1, p.err, DK_DEVERR_WAIT_FULL)) ok = false;
+      q_wait(0);
+      if (kFp4 && two) q_wait(1);
       slot_wait(fill);
       if (!ok) break;
       tc::fence_after_sync();
@@ -357,7 +438,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int j0 = (walk.c0 + i) * kC;
         // does every row of v belong to a position that some row of the unit sees?
         const bool clear = j0 + kC <= span.end && (p.mask.window <= 0 || j0 >= span.lo || j0 + kC <= p.mask.sinks);
-        if (!clear) {
+        if (!kFp4 && !clear) {
           uint8_t* v = slots + (fv % L::kSlots) * L::kTileBytes + (lane & 7) * 16;
           auto zero = [&](int from, int to) {  // 8 lanes a row of 64 dims
             for (int r = min(max(from, 0), kC) + (lane >> 3); r < min(to, kC); r += 4)
@@ -413,6 +494,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int pos = live ? row_position(p, t, tok) - span.shift : -1;  // (in the span's offsets)
       const int p_lo = row_position(p, t, first) - span.shift;
       const int p_hi = row_position(p, t, min(t.ntok, first + p.half_tokens) - 1) - span.shift;
+      float scale2 = p.scale2;
+      if constexpr (kTurnQ) {
+        if (!wait_for(&bar.q_full[x], o_seen & 1, p.err, DK_DEVERR_WAIT_FULL)) ok = false;
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        scale2 *= __int_as_float((127 - q_to_fp16<kHd, kFp4>(q_sm + x * L::kTileBytes + r * 128, r)) << 23);
+        tc::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar.q_ready[x]);
+      }
       float m = -INFINITY, l = 0.f;  // of scale2 * score
       for (int i = c0; i < c1; ++i) {
         if (!wait_for(&bar.s_full[x], s_seen & 1, p.err, DK_DEVERR_WAIT_FULL)) ok = false;
@@ -439,7 +530,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         // P refers to a maximum that is only raised when a row's grows by 2^kLazy or more.
-        const float mx = row_max(s) * p.scale2;
+        const float mx = row_max(s) * scale2;
         const bool raise = mx > m + kLazy || (m == -INFINITY && mx > -INFINITY);
         if (__any_sync(0xffffffffu, raise)) {
           const float keep = raise ? exp2_approx(m - mx) : 1.f;
@@ -460,7 +551,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         const float base = m == -INFINITY ? 0.f : m;
-        const float2 scale = make_float2(p.scale2, p.scale2), off = make_float2(-base, -base);
+        const float2 scale = make_float2(scale2, scale2), off = make_float2(-base, -base);
         float2 sum[4] = {};
 #pragma unroll
         for (int c = 0; c < kC / 32; ++c) {
@@ -470,7 +561,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             float2 y = fma2(make_float2(s[32 * c + 2 * d], s[32 * c + 2 * d + 1]), scale, off);
             y = make_float2(exp2_approx(y.x), exp2_approx(y.y));
             sum[d & 3] = add2(sum[d & 3], y);
-            w[d] = E::pack(y.x, y.y);
+            w[d] = Elem<M>::pack(y.x, y.y);
           }
           tmem_st16(s_col + 16 * c, w);
           if (c == kPartChunks - 1 || c == kC / 32 - 1) {  // a part of P is complete
@@ -495,7 +586,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc::fence_after_sync();
       const int row = x * 128 + r;
       if (whole) {
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const float inv = l == 0.f ? 0.f : (kFp4 ? p.out_scale : 1.f) / l;
         // Four lanes exchange 16-byte pieces so that together they store 64 bytes of one row at a time: a lane storing its
         // own row would touch 32 lines with every instruction.
         T* out = static_cast<T*>(p.out) + (static_cast<int64_t>(t.t0 + tok) * p.nkv * p.G + head) * kHd;
@@ -516,8 +607,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               const float* v = &o[32 * half + 8 * k];
-              w[k] = make_uint4(E::pack(v[0] * inv, v[1] * inv), E::pack(v[2] * inv, v[3] * inv),
-                                E::pack(v[4] * inv, v[5] * inv), E::pack(v[6] * inv, v[7] * inv));
+              w[k] = make_uint4(Elem<T>::pack(v[0] * inv, v[1] * inv), Elem<T>::pack(v[2] * inv, v[3] * inv),
+                                Elem<T>::pack(v[4] * inv, v[5] * inv), Elem<T>::pack(v[6] * inv, v[7] * inv));
             }
             transpose4(w, lane);
 #pragma unroll
@@ -543,6 +634,54 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
 
+  if (kFp4 && warp >= kConvertWarp) {
+    // ---------------------------------------------------------------- conversion: half of a chunk's rows each, K and V in turn
+    // A lane takes 16 bytes of codes, 32 dims of a row, to four 16-byte pieces. The second segment's lanes (head_dim 128) take their
+    // pieces in another order, so that 8 lanes' stores hit all banks.
+    constexpr int kRowLanes = kHd / 32, kRowsAtOnce = 32 / kRowLanes;
+    const int q = lane % kRowLanes, flip = q & 2;
+    int fill = 0;
+    while (walk.more() && ok) {
+      const Span<kC> span = walk.step();
+      for (int i = 2 * walk.c0; i < 2 * walk.c1; ++i, ++fill) {
+        const int from = fill % max(L::kRaw, 1), s = fill % L::kSlots;
+        if (!wait_for(&bar.raw_full[from], (fill / max(L::kRaw, 1)) & 1, p.err, DK_DEVERR_WAIT_FULL)) ok = false;
+        if (ok && fill >= L::kSlots && !wait_for(&bar.kv_empty[s], ((fill / L::kSlots) - 1) & 1, p.err, DK_DEVERR_WAIT_EMPTY)) ok = false;
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const uint8_t* in = raw + from * L::kRawBytes;
+        uint8_t* out = slots + s * L::kTileBytes + (q >> 1) * L::kSegBytes;
+        const int j0 = (i >> 1) * kC;
+        // V rows of positions that no row of the unit sees become zeros (codes are finite whatever they are)
+        const bool clear = (i & 1) == 0 || (j0 + kC <= span.end && (p.mask.window <= 0 || j0 >= span.lo || j0 + kC <= p.mask.sinks));
+#pragma unroll 2
+        for (int r = (warp - kConvertWarp) * (kC / kConvertWarps) + lane / kRowLanes; r < (warp - kConvertWarp + 1) * (kC / kConvertWarps);
+             r += kRowsAtOnce) {
+          const uint4 codes = *reinterpret_cast<const uint4*>(in + r * Fp4<kHd>::kCodes + 16 * q);
+          uint32_t two = *reinterpret_cast<const uint16_t*>(in + L::kRawScalesAt + r * Fp4<kHd>::kScales + 2 * q);
+          if (!clear && !span.needs(j0 + r, 1, p.mask)) two = 0;
+          two = fp4_scales(two);
+          const uint32_t lo = prmt(two, two, 0x1010), hi = prmt(two, two, 0x3232);
+          const uint32_t w[4] = {flip ? codes.z : codes.x, flip ? codes.w : codes.y, flip ? codes.x : codes.z, flip ? codes.y : codes.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t scale = (k < 2) == (flip == 0) ? lo : hi;
+            uint32_t v[4];
+            fp4_codes(w[k], v);
+            const int piece = (q & 1) * 4 + (k ^ flip);
+            *reinterpret_cast<uint4*>(out + r * 128 + ((piece ^ (r & 7)) << 4)) =
+                make_uint4(hmul2_rn(v[0], scale), hmul2_rn(v[1], scale), hmul2_rn(v[2], scale), hmul2_rn(v[3], scale));
+          }
+        }
+        tc::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&bar.kv_full[s]);
+          mbar_arrive(&bar.raw_empty[from]);
+        }
+      }
+    }
+  }
   if (warp == kZeroWarp && p.mode == kRagged && !p.always_partial) {
     // Rows that belong to no sequence are in no tile: their outputs are zero. (Beside a prefix the join writes all rows.)
     const int from = min(max(p.starts[0], 0), p.T), to = max(min(p.starts[p.B], p.T), from);
@@ -582,7 +721,7 @@ bool make_q_map(CUtensorMap* map, const Problem& p, int64_t nq, int64_t hd, CUte
   return make_tensor_map(map, p.q, type, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <typename T, int kHd>
+template <typename T, int kHd, bool kFp4>
 int ctas_of() {
   static std::mutex mu;
   static int known[64];  // by device; 0: not asked yet, -1: does not fit
@@ -592,31 +731,35 @@ int ctas_of() {
   int& n = known[dev & 63];
   if (n == 0) {
     cudaFuncAttributes a;  // the register split needs the launch to hold exactly what it divides
-    const bool split = cudaFuncGetAttributes(&a, tiles_kernel<T, kHd>) == cudaSuccess && a.numRegs == kRegsLaunch;
-    n = split && opt_in_dynamic_smem(tiles_kernel<T, kHd>) >= Smem<kHd>::kBytes ? device_info().num_sms : -1;
+    const bool split = cudaFuncGetAttributes(&a, tiles_kernel<T, kHd, kFp4>) == cudaSuccess && a.numRegs == kRegsLaunch;
+    n = split && opt_in_dynamic_smem(tiles_kernel<T, kHd, kFp4>) >= Smem<kHd, kFp4>::kBytes ? device_info().num_sms : -1;
   }
   return n < 0 ? 0 : n;
 }
 
 }  // namespace
 
-int tc_ctas(int64_t head_dim, int dtype) {
-  if (dtype == DK_F16) return head_dim == 128 ? ctas_of<__half, 128>() : ctas_of<__half, 64>();
-  return head_dim == 128 ? ctas_of<__nv_bfloat16, 128>() : ctas_of<__nv_bfloat16, 64>();
+#define DK_BY_KIND(CALL)                                                                                      \
+  (dtype == DK_F16 ? (hd == 128 ? (fp4 ? CALL(__half, 128, true) : CALL(__half, 128, false))                  \
+                                : (fp4 ? CALL(__half, 64, true) : CALL(__half, 64, false)))                   \
+                   : (hd == 128 ? (fp4 ? CALL(__nv_bfloat16, 128, true) : CALL(__nv_bfloat16, 128, false))    \
+                                : (fp4 ? CALL(__nv_bfloat16, 64, true) : CALL(__nv_bfloat16, 64, false))))
+
+int tc_ctas(int64_t hd, int dtype, bool fp4) {
+#define DK_CTAS(TT, HH, FF) ctas_of<TT, HH, FF>()
+  return DK_BY_KIND(DK_CTAS);
+#undef DK_CTAS
 }
 
-int tc_launch(const Problem& p, int64_t nq, int64_t hd, int dtype, int ctas, const CUtensorMap& mk, const CUtensorMap& mv,
+int tc_launch(const Problem& p, int64_t nq, int64_t hd, int dtype, bool fp4, int ctas, const CUtensorMap& mk, const CUtensorMap& mv,
               int wait_late, cudaStream_t st) {
   const CUtensorMapDataType type = dtype == DK_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   CUtensorMap mq;
   if (!make_q_map(&mq, p, nq, hd, type)) return DK_ERR_CUDA;
-  cudaError_t e;
-#define DK_TILES(TT, HH) \
-  launch(tiles_kernel<TT, HH>, dim3(ctas), dim3(kThreads), Smem<HH>::kBytes, st, pdl_enabled(), dim3(1, 1, 1), mq, mk, mv, p, wait_late)
-  if (dtype == DK_F16)
-    e = hd == 128 ? DK_TILES(__half, 128) : DK_TILES(__half, 64);
-  else
-    e = hd == 128 ? DK_TILES(__nv_bfloat16, 128) : DK_TILES(__nv_bfloat16, 64);
+#define DK_TILES(TT, HH, FF)                                                                                                        \
+  launch(tiles_kernel<TT, HH, FF>, dim3(ctas), dim3(kThreads), Smem<HH, FF>::kBytes, st, pdl_enabled(), dim3(1, 1, 1), mq, mk, mv, p, \
+         wait_late)
+  const cudaError_t e = DK_BY_KIND(DK_TILES);
 #undef DK_TILES
   if (e != cudaSuccess) return set_error(DK_ERR_CUDA, "paged attention (256-row tiles) launch: %s", cudaGetErrorString(e));
   return DK_OK;

@@ -370,7 +370,7 @@ struct RowsShape {
 };
 // Such a launch over a cache held in 4 bits (paged_attention_fp4.cu), with tiles of 8 or 16 rows; kFp4Groups pieces of the line a CTA.
 constexpr int kFp4Groups = 2;
-constexpr int kFp4Chunk = 64;
+constexpr int kFp4Chunk = 128;
 RowsShape fp4_rows_shape(int64_t hd, int dtype, int rows);
 cudaError_t fp4_rows_launch(const Problem& p, int64_t hd, int dtype, int rows, const RowsShape& s, int wait_late, cudaStream_t st);
 

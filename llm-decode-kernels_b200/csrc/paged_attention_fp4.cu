@@ -32,11 +32,13 @@ namespace paged {
 namespace {
 
 constexpr int kCWarps = 4;  // warps of a group
-constexpr int kSub = 1;     // 16-position tiles of a warp in a chunk
+constexpr int kSub = 2;     // 16-position tiles of a warp in a chunk
 constexpr int kChunk = kFp4Chunk;
 static_assert(kChunk == kCWarps * kSub * 16, "a chunk is one round of the warps");
 constexpr int kThreads = kFp4Groups * (kCWarps + 1) * 32;
-constexpr int kMaxRing = 10;
+// Slots of a group's ring: what fits the shared memory of two CTAs an SM (one with 16 rows).
+template <int kHd, int kBlocks>
+constexpr int kRing = kHd == 64 ? (kBlocks == 1 ? 8 : 10) / kSub : (kBlocks == 1 ? 4 : 6) / kSub;
 constexpr float kRefBelow = 6.f, kRefReach = 14.f;
 
 // A chunk in shared memory: for k and v each the codes of kChunk positions, then their scales.
@@ -64,7 +66,8 @@ __device__ __forceinline__ uint32_t choose(uint32_t a, uint32_t b, uint32_t m) {
 __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((127 + e) << 23); }
 
 template <typename T, int kHd, int kBlocks>
-__global__ void __launch_bounds__(kThreads, kBlocks == 1 ? 2 : 1) fp4_rows_kernel(const Problem p, int ring, int wait_late) {
+__global__ void __launch_bounds__(kThreads, kBlocks == 1 ? 2 : 1) fp4_rows_kernel(const Problem p, int wait_late) {
+  constexpr int ring = kRing<kHd, kBlocks>;
   using F = Fp4<kHd>;
   using S = Slot<kHd>;
   constexpr int kRows = 8 * kBlocks;      // query rows: the product's columns
@@ -74,7 +77,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks == 1 ? 2 : 1) fp4_rows_kerne
   __shared__ float pre_ml_sh[kFp4Groups][kCWarps * kRows * 2];
   __shared__ float pre_w_sh[kFp4Groups][kCWarps * kRows];
   __shared__ float fin_sh[kFp4Groups][kRows * 2];
-  __shared__ __align__(8) uint64_t full_sh[kFp4Groups][kMaxRing], empty_sh[kFp4Groups][kMaxRing];
+  __shared__ __align__(8) uint64_t full_sh[kFp4Groups][ring], empty_sh[kFp4Groups][ring];
   __shared__ int warp_sum[kThreads / 32 + 1];
   extern __shared__ __align__(128) uint8_t base[];
   int* cum_sh = reinterpret_cast<int*>(base);  // [B + 1], before the first copies land there
@@ -88,7 +91,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks == 1 ? 2 : 1) fp4_rows_kerne
   float *pre_ml = pre_ml_sh[group], *pre_w = pre_w_sh[group], *fin = fin_sh[group];
   uint64_t *full = full_sh[group], *empty = empty_sh[group];
   if (tid == 0) {
-    for (int i = 0; i < kFp4Groups * kMaxRing; ++i) {
+    for (int i = 0; i < kFp4Groups * ring; ++i) {
       mbar_init(&full_sh[0][i], 1);
       mbar_init(&empty_sh[0][i], kCWarps);
     }
@@ -135,7 +138,12 @@ __global__ void __launch_bounds__(kThreads, kBlocks == 1 ? 2 : 1) fp4_rows_kerne
   Walk<kChunk> walk(p, line, cta, ctas, lane);
   __syncthreads();  // the sums have been read: copies may land on them
   bool ok = true;
-  int fill = 0;  // ring fills so far
+  int fill = 0;         // ring fills so far,
+  int s = 0, round = 0;  // fill % ring and fill / ring
+  auto filled = [&] {
+    ++fill;
+    if (++s == ring) s = 0, ++round;
+  };
 
   if (producer) {
     // ---------------------------------------------------------------- producer warps: one lane per copy
@@ -145,7 +153,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks == 1 ? 2 : 1) fp4_rows_kerne
     const int kv = lane & 1, scales = (lane >> 1) & 1, pg = lane >> 2;
     const int row_bytes = scales ? F::kScales : F::kCodes;
     const uint32_t bytes = box * row_bytes;
-    const uint8_t* pool = p.pool[kv] + (scales ? p.page_size * F::kCodes : 0);
+    const uint8_t* pool = (kv ? p.pool[1] : p.pool[0]) + (scales ? p.page_size * F::kCodes : 0);
     uint8_t* dst = slots + kv * S::kTensor + (scales ? S::kScalesAt : 0) + pg * bytes;
     while (walk.more() && ok) {
       const Span<kChunk> span = walk.step();
@@ -158,11 +166,10 @@ __global__ void __launch_bounds__(kThreads, kBlocks == 1 ? 2 : 1) fp4_rows_kerne
         return i < c1 && pg < boxes && span.needs(j, box, p.mask) ? table[span.position(j) >> p.page_shift] : INT_MIN;
       };
       int next = entry(c0);
-      for (int i = c0; i < c1; ++i, ++fill) {
+      for (int i = c0; i < c1; ++i, filled()) {
         const int page = next;
         next = entry(i + 1);
-        const int s = fill % ring;
-        if (fill >= ring && !wait_for(&empty[s], ((fill / ring) - 1) & 1, p.err, DK_DEVERR_WAIT_EMPTY)) ok = false;
+        if (round > 0 && !wait_for(&empty[s], (round - 1) & 1, p.err, DK_DEVERR_WAIT_EMPTY)) ok = false;
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         uint8_t* at = dst + s * S::kBytes;
@@ -196,6 +203,9 @@ __global__ void __launch_bounds__(kThreads, kBlocks == 1 ? 2 : 1) fp4_rows_kerne
       if (c1 <= c0) continue;
       const int rows = p.G;  // one token's
       const int p0 = t.p0 - span.shift;
+      // the chunks that every row sees all of (nothing to mask)
+      const int clear_from = p.mask.window > 0 ? (max(0, p0 - p.mask.window + 1) + kChunk - 1) / kChunk : 0;
+      const int clear_to = max(min(p0 + 1, span.end), 0) / kChunk;
       // q as the products' column operand: column g has query row 8 * block + g, the lane its dims from tq * kHd / 4 on
       uint32_t qb[kBlocks][kSteps][2];
       float scale2[kBlocks][2];  // of columns 2 tq and 2 tq + 1
@@ -241,141 +251,165 @@ __global__ void __launch_bounds__(kThreads, kBlocks == 1 ? 2 : 1) fp4_rows_kerne
         for (int u = 0; u < 2; ++u) scale2[nb][u] = p.scale2 * power_of_two(-__shfl_sync(0xffffffffu, e, 4 * (2 * tq + u)));
       }
       float o[kBlocks][kSteps][4];
-      float ref[kBlocks][2], l[kBlocks][2];
+      float base[kBlocks][2], reach[kBlocks][2], l[kBlocks][2];  // p = 2^(score - base); a score past base + reach sets it anew
 #pragma unroll
       for (int nb = 0; nb < kBlocks; ++nb) {
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) o[nb][i][0] = o[nb][i][1] = o[nb][i][2] = o[nb][i][3] = 0.f;
-        ref[nb][0] = ref[nb][1] = -INFINITY, l[nb][0] = l[nb][1] = 0.f;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) base[nb][u] = 0.f, reach[nb][u] = -INFINITY, l[nb][u] = 0.f;
       }
 
-      for (int i = c0; i < c1; ++i, ++fill) {
-        const int s = fill % ring;
-        if (ok && !wait_for(&full[s], (fill / ring) & 1, p.err, DK_DEVERR_WAIT_FULL)) ok = false;
-        ok = __all_sync(0xffffffffu, ok);
+      // The warp's kSub tiles of chunk i, in slot s. kClear: every row sees all of the positions.
+      auto tiles = [&](int i, auto all_seen) {
+        constexpr bool kClear = decltype(all_seen)::value;
+        const int r0 = 16 * kSub * sub;
+        const uint8_t* kt = slots + s * S::kBytes;
+        const uint8_t* vt = kt + S::kTensor;
+        // S^T: rows are positions, columns query rows
+        float sc[kSub][kBlocks][4];
+        uint32_t ks[kSub][2][2];  // scales of rows g and g + 8, of both halves of a lane's dims
 #pragma unroll
         for (int tile = 0; tile < kSub; ++tile) {
-          const int r0 = 16 * (sub * kSub + tile), j0 = i * kChunk + r0;  // the warp's 16 positions
-          if (!ok || !span.needs(j0, 16, p.mask)) continue;
-          const uint8_t* kt = slots + s * S::kBytes;
-          const uint8_t* vt = kt + S::kTensor;
-          // S^T: rows are positions, columns query rows
-          float sc[kBlocks][4];
 #pragma unroll
-          for (int nb = 0; nb < kBlocks; ++nb) sc[nb][0] = sc[nb][1] = sc[nb][2] = sc[nb][3] = 0.f;
-          {
-            uint32_t kw[2][kWords], ks[2][2];  // codes and scales (of both halves of a lane's dims) of rows g and g + 8
+          for (int nb = 0; nb < kBlocks; ++nb) sc[tile][nb][0] = sc[tile][nb][1] = sc[tile][nb][2] = sc[tile][nb][3] = 0.f;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int r = r0 + 16 * tile + row_a + 8 * e;
+            if constexpr (kHd == 128) {
+              const uint32_t two = fp4_scales(*reinterpret_cast<const uint16_t*>(kt + S::kScalesAt + r * F::kScales + 2 * tq));
+              ks[tile][e][0] = prmt(two, two, 0x1010), ks[tile][e][1] = prmt(two, two, 0x3232);
+            } else {
+              const uint32_t one = fp4_scales(kt[S::kScalesAt + r * F::kScales + tq]);
+              ks[tile][e][0] = ks[tile][e][1] = prmt(one, one, 0x1010);
+            }
+          }
+        }
+        uint32_t kw[kSub][2][kWords];
+#pragma unroll
+        for (int tile = 0; tile < kSub; ++tile)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint8_t* at = kt + (r0 + 16 * tile + row_a + 8 * e) * F::kCodes + (kHd / 8) * tq;
+            if constexpr (kHd == 128) {
+              const uint4 w = *reinterpret_cast<const uint4*>(at);
+              kw[tile][e][0] = w.x, kw[tile][e][1] = w.y, kw[tile][e][2] = w.z, kw[tile][e][3] = w.w;
+            } else {
+              const uint2 w = *reinterpret_cast<const uint2*>(at);
+              kw[tile][e][0] = w.x, kw[tile][e][1] = w.y;
+            }
+          }
+#pragma unroll
+        for (int w = 0; w < kWords; ++w)
+#pragma unroll
+          for (int tile = 0; tile < kSub; ++tile) {
+            uint32_t a[2][4];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const int r = r0 + row_a + 8 * e;
-              if constexpr (kHd == 128) {
-                const uint4 w = *reinterpret_cast<const uint4*>(kt + r * F::kCodes + 16 * tq);
-                kw[e][0] = w.x, kw[e][1] = w.y, kw[e][2] = w.z, kw[e][3] = w.w;
-                const uint32_t two = fp4_scales(*reinterpret_cast<const uint16_t*>(kt + S::kScalesAt + r * F::kScales + 2 * tq));
-                ks[e][0] = prmt(two, two, 0x1010), ks[e][1] = prmt(two, two, 0x3232);
-              } else {
-                const uint2 w = *reinterpret_cast<const uint2*>(kt + r * F::kCodes + 8 * tq);
-                kw[e][0] = w.x, kw[e][1] = w.y;
-                const uint32_t one = fp4_scales(kt[S::kScalesAt + r * F::kScales + tq]);
-                ks[e][0] = ks[e][1] = prmt(one, one, 0x1010);
-              }
+              fp4_codes(kw[tile][e][w], a[e]);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) a[e][k] = hmul2_rn(a[e][k], ks[tile][e][2 * w / kWords]);
             }
 #pragma unroll
-            for (int w = 0; w < kWords; ++w) {
-              uint32_t a[2][4];
+            for (int nb = 0; nb < kBlocks; ++nb) {
+              mma_16816(sc[tile][nb], a[0][0], a[1][0], a[0][1], a[1][1], qb[nb][2 * w][0], qb[nb][2 * w][1]);
+              mma_16816(sc[tile][nb], a[0][2], a[1][2], a[0][3], a[1][3], qb[nb][2 * w + 1][0], qb[nb][2 * w + 1][1]);
+            }
+          }
+        uint32_t pb[kSub][kBlocks][2];  // p as the products' column operand
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                fp4_codes(kw[e][w], a[e]);
+        for (int nb = 0; nb < kBlocks; ++nb) {
+          float y[kSub][4], top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                for (int k = 0; k < 4; ++k) a[e][k] = hmul2_rn(a[e][k], ks[e][2 * w / kWords]);
+          for (int tile = 0; tile < kSub; ++tile)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              y[tile][e] = fmaf(sc[tile][nb][e], scale2[nb][e & 1], -base[nb][e & 1]);
+              if constexpr (!kClear) {
+                const int j = i * kChunk + r0 + 16 * tile + row_a + 8 * (e >> 1);
+                if (!(j < span.end && p.mask.sees(p0, j))) y[tile][e] = -INFINITY;
               }
+              top[e & 1] = fmaxf(top[e & 1], y[tile][e]);
+            }
+          if (__any_sync(0xffffffffu, top[0] > reach[nb][0] || top[1] > reach[nb][1])) {
 #pragma unroll
-              for (int nb = 0; nb < kBlocks; ++nb) {
-                mma_16816(sc[nb], a[0][0], a[1][0], a[0][1], a[1][1], qb[nb][2 * w][0], qb[nb][2 * w][1]);
-                mma_16816(sc[nb], a[0][2], a[1][2], a[0][3], a[1][3], qb[nb][2 * w + 1][0], qb[nb][2 * w + 1][1]);
+            for (int u = 0; u < 2; ++u) {
+              float most = top[u];
+              most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 4));
+              most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 8));
+              most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 16));
+              if (most > reach[nb][u]) {
+                const float to = base[nb][u] + (most - kRefBelow), up = to - base[nb][u];
+                const float keep = reach[nb][u] == -INFINITY ? 0.f : exp2_approx(-up);
+                base[nb][u] = to;
+                reach[nb][u] = kRefReach;
+                l[nb][u] *= keep;
+#pragma unroll
+                for (int k = 0; k < kSteps; ++k) {
+                  o[nb][k][u] *= keep;
+                  o[nb][k][u + 2] *= keep;
+                }
+#pragma unroll
+                for (int tile = 0; tile < kSub; ++tile) y[tile][u] -= up, y[tile][u + 2] -= up;
               }
             }
           }
-          // every row sees all 16 positions (nothing to mask)?
-          const bool clear = j0 + 15 <= p0 && (p.mask.window <= 0 || j0 > p0 - p.mask.window || j0 + 15 < p.mask.sinks) &&
-                             j0 + 15 < span.end;
-          uint32_t pb[kBlocks][2];  // p as the products' column operand
 #pragma unroll
-          for (int nb = 0; nb < kBlocks; ++nb) {
-            float y[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              y[e] = sc[nb][e] * scale2[nb][e & 1];
-              const int j = j0 + row_a + 8 * (e >> 1);
-              if (!clear && !(j < span.end && p.mask.sees(p0, j))) y[e] = -INFINITY;
-            }
-            bool raise = false;
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              const float top = fmaxf(y[u], y[u + 2]);
-              raise |= top > ref[nb][u] + kRefReach;  // (a reference of -inf: any score)
-            }
-            if (__any_sync(0xffffffffu, raise)) {
-#pragma unroll
-              for (int u = 0; u < 2; ++u) {
-                float top = fmaxf(y[u], y[u + 2]);
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                if (top > ref[nb][u] + kRefReach) {
-                  const float to = top - kRefBelow, keep = exp2_approx(ref[nb][u] - to);
-                  ref[nb][u] = to;
-                  l[nb][u] *= keep;
-#pragma unroll
-                  for (int k = 0; k < kSteps; ++k) {
-                    o[nb][k][u] *= keep;
-                    o[nb][k][u + 2] *= keep;
-                  }
-                }
-              }
-            }
+          for (int tile = 0; tile < kSub; ++tile) {
             float w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              w[e] = exp2_approx(y[e] - (ref[nb][e & 1] == -INFINITY ? 0.f : ref[nb][e & 1]));
+              w[e] = exp2_approx(y[tile][e]);
               l[nb][e & 1] += w[e];
             }
-            pb[nb][0] = transpose8(Elem<__half>::pack(w[0], w[1]));
-            pb[nb][1] = transpose8(Elem<__half>::pack(w[2], w[3]));
+            pb[tile][nb][0] = transpose8(Elem<__half>::pack(w[0], w[1]));
+            pb[tile][nb][1] = transpose8(Elem<__half>::pack(w[2], w[3]));
           }
-          // O^T: rows are dims (row g of tile k: the lane's dim 2 k, row g + 8: 2 k + 1), the inner index runs over positions:
-          // the lane's four are tq, tq + 4, tq + 8, tq + 12
-          {
-            uint32_t vw[4][kHd / 64], vs[4];
+        }
+        // O^T: rows are dims (row g of tile k: the lane's dim 2 k, row g + 8: 2 k + 1), the inner index runs over positions:
+        // the lane's four are tq, tq + 4, tq + 8, tq + 12
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int r = r0 + tq + 4 * e;
-              if constexpr (kHd == 128) {
-                const uint2 w = *reinterpret_cast<const uint2*>(vt + r * F::kCodes + 8 * g);
-                vw[e][0] = w.x, vw[e][1] = w.y;
-                vs[e] = vt[S::kScalesAt + r * F::kScales + g];
-              } else {
-                vw[e][0] = *reinterpret_cast<const uint32_t*>(vt + r * F::kCodes + 4 * g);
-                vs[e] = vt[S::kScalesAt + r * F::kScales + (g >> 1)];
-              }
-              if (!clear && !span.needs(i * kChunk + r, 1, p.mask)) vs[e] = 0;
+        for (int tile = 0; tile < kSub; ++tile) {
+          uint32_t vw[4][kHd / 64], vs[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = r0 + 16 * tile + tq + 4 * e;
+            if constexpr (kHd == 128) {
+              const uint2 w = *reinterpret_cast<const uint2*>(vt + r * F::kCodes + 8 * g);
+              vw[e][0] = w.x, vw[e][1] = w.y;
+              vs[e] = vt[S::kScalesAt + r * F::kScales + g];
+            } else {
+              vw[e][0] = *reinterpret_cast<const uint32_t*>(vt + r * F::kCodes + 4 * g);
+              vs[e] = vt[S::kScalesAt + r * F::kScales + (g >> 1)];
             }
-            const uint32_t s01 = fp4_scales(vs[0] | vs[1] << 8), s23 = fp4_scales(vs[2] | vs[3] << 8);
+            if constexpr (!kClear)
+              if (!span.needs(i * kChunk + r, 1, p.mask)) vs[e] = 0;
+          }
+          const uint32_t s01 = fp4_scales(vs[0] | vs[1] << 8), s23 = fp4_scales(vs[2] | vs[3] << 8);
 #pragma unroll
-            for (int w = 0; w < kHd / 64; ++w) {
-              uint32_t a[4][4];
-              fp4_codes(choose(vw[0][w], vw[1][w] << 4, kLow), a[0]);
-              fp4_codes(choose(vw[0][w] >> 4, vw[1][w], kLow), a[1]);
-              fp4_codes(choose(vw[2][w], vw[3][w] << 4, kLow), a[2]);
-              fp4_codes(choose(vw[2][w] >> 4, vw[3][w], kLow), a[3]);
+          for (int w = 0; w < kHd / 64; ++w) {
+            uint32_t a[4][4];
+            fp4_codes(choose(vw[0][w], vw[1][w] << 4, kLow), a[0]);
+            fp4_codes(choose(vw[0][w] >> 4, vw[1][w], kLow), a[1]);
+            fp4_codes(choose(vw[2][w], vw[3][w] << 4, kLow), a[2]);
+            fp4_codes(choose(vw[2][w] >> 4, vw[3][w], kLow), a[3]);
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const uint32_t a0 = hmul2_rn(a[0][k], s01), a1 = hmul2_rn(a[1][k], s01), a2 = hmul2_rn(a[2][k], s23), a3 = hmul2_rn(a[3][k], s23);
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t a0 = hmul2_rn(a[0][k], s01), a1 = hmul2_rn(a[1][k], s01), a2 = hmul2_rn(a[2][k], s23), a3 = hmul2_rn(a[3][k], s23);
 #pragma unroll
-                for (int nb = 0; nb < kBlocks; ++nb) mma_16816(o[nb][4 * w + k], a0, a1, a2, a3, pb[nb][0], pb[nb][1]);
-              }
+              for (int nb = 0; nb < kBlocks; ++nb) mma_16816(o[nb][4 * w + k], a0, a1, a2, a3, pb[tile][nb][0], pb[tile][nb][1]);
             }
           }
+        }
+      };
+      for (int i = c0; i < c1; ++i, filled()) {
+        if (ok && !wait_for(&full[s], round & 1, p.err, DK_DEVERR_WAIT_FULL)) ok = false;
+        ok = __all_sync(0xffffffffu, ok);
+        if (ok) {
+          if (i >= clear_from && i < clear_to)
+            tiles(i, std::true_type());
+          else if (span.needs(i * kChunk + 16 * kSub * sub, 16 * kSub, p.mask))
+            tiles(i, std::false_type());
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[s]);
@@ -396,7 +430,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks == 1 ? 2 : 1) fp4_rows_kerne
           for (int k = 0; k < kSteps; k += 2)
             *reinterpret_cast<float4*>(to + 2 * k) = make_float4(o[nb][k][u], o[nb][k][u + 2], o[nb][k + 1][u], o[nb][k + 1][u + 2]);
           if (g == 0) {
-            pre_ml[row * 2] = ref[nb][u];
+            pre_ml[row * 2] = reach[nb][u] == -INFINITY ? -INFINITY : base[nb][u];
             pre_ml[row * 2 + 1] = sum;
           }
         }
@@ -459,9 +493,9 @@ RowsShape shape() {
   static std::mutex mu;
   static int per_sm[64];  // by device; 0: not asked yet
   RowsShape s;
-  s.ring = kHd == 64 ? (kBlocks == 1 ? 8 : 10) : (kBlocks == 1 ? 4 : 6);
+  s.ring = kRing<kHd, kBlocks>;
   s.smem = static_cast<size_t>(kFp4Groups) * (s.ring * Slot<kHd>::kBytes + kCWarps * 8 * kBlocks * kHd * 4);
-  static_assert((kMaxBatch + 1) * 4 <= kFp4Groups * 4 * Slot<128>::kBytes && (kMaxBatch + 1) * 4 <= kFp4Groups * 8 * Slot<64>::kBytes,
+  static_assert((kMaxBatch + 1) * 4 <= kFp4Groups * kRing<kHd, kBlocks> * Slot<kHd>::kBytes,
                 "the chunk sums fit the ring");
   int dev = 0;
   cudaGetDevice(&dev);
@@ -495,7 +529,7 @@ RowsShape fp4_rows_shape(int64_t hd, int dtype, int rows) {
 
 cudaError_t fp4_rows_launch(const Problem& p, int64_t hd, int dtype, int rows, const RowsShape& s, int wait_late, cudaStream_t st) {
 #define DK_ROWS(TT, HH, NB) \
-  launch(fp4_rows_kernel<TT, HH, NB>, dim3(s.ctas), dim3(kThreads), s.smem, st, pdl_enabled(), dim3(1, 1, 1), p, s.ring, wait_late)
+  launch(fp4_rows_kernel<TT, HH, NB>, dim3(s.ctas), dim3(kThreads), s.smem, st, pdl_enabled(), dim3(1, 1, 1), p, wait_late)
   return DK_BY_KIND(DK_ROWS);
 #undef DK_ROWS
 }

@@ -1,8 +1,9 @@
 // Positions of a 4-bit paged cache read back as 16-bit values, k and v: row t of the call is a position of a sequence (the
 // last ones of each, as in the other paged ops), value = code * scale * power, exact in T unless outside its range.
 //
-// Memory bound: 9 bytes are read for 32 written. A warp takes a token: 8 dims (4 bytes of codes, half a group) of one tensor a
-// lane at a time, so that it stores 512 contiguous bytes.
+// Memory bound: 9 bytes are read for 32 written. A CTA takes up to 32 rows: its first threads look up where they lie, side by side (a
+// chain of small loads each), then a warp takes a row's columns, 8 dims (4 bytes of codes, half a group) a lane, so that it
+// stores 512 contiguous bytes, with the loads of several rows in flight.
 #include <algorithm>
 
 #include "paged_fp4.cuh"
@@ -26,49 +27,80 @@ struct ReadParams {
 };
 
 constexpr int kWarps = 8;
+constexpr int kMaxRows = 32;  // of a CTA
+constexpr int kAhead = 4;     // items loaded at a time
 
+// CTA x: rows per * x .. + per. A row has `columns` items of 32 pieces of 8 dims, of k, then of v.
 template <typename T, int kHd>
-__global__ void __launch_bounds__(kWarps * 32) paged_read_fp4_kernel(const ReadParams p) {
+__global__ void __launch_bounds__(kWarps * 32) paged_read_fp4_kernel(const ReadParams p, int columns, int per) {
   using F = Fp4<kHd>;
+  __shared__ int2 place[kMaxRows];  // {page, row in it}; page -1: zeros
   pdl_trigger();
   pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const int pieces = p.nkv * (kHd / 8);  // of 8 dims, of one tensor
-  for (int64_t w = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5); w < p.T; w += static_cast<int64_t>(gridDim.x) * kWarps) {
-    const int t = static_cast<int>(w);
-    int b = t, pos;
+  const int t0 = blockIdx.x * per, n = min(per, p.T - t0);
+  if (static_cast<int>(threadIdx.x) < n) {
+    // A row of no sequence, or before its sequence's first position, has no place; nor has a position without a page, which is
+    // reported.
+    const int t = t0 + threadIdx.x;
+    int b = t, pos, page = -1;
     if (p.starts == nullptr) {
       pos = length_of(p.lengths, t) - 1;
     } else {
-      b = find_tile_warp([&](int j) { return p.starts[j]; }, p.B, t, lane);
+      b = find_tile([&](int j) { return p.starts[j]; }, p.B, t);
       const int end = p.starts[b + 1];
       pos = t >= p.starts[b] && t < end ? length_of(p.lengths, b) - (end - t) : -1;
     }
-    // A row of no sequence, or before its sequence's first position, is zero; so is a position without a page, which is reported.
-    const int at = pos >> p.page_shift;
-    const int page = pos >= 0 && at < p.table_width ? p.table[b * p.ld_table + at] : -1;
-    const bool there = page >= 0 && page < p.n_pages;
-    if (pos >= 0 && !there && lane == 0) record_device_error(p.err, DK_DEVERR_BAD_POSITION);
-    const int slot = pos & (p.page_size - 1);
-    for (int i = lane; i < 2 * pieces; i += 32) {
-      const int which = i >= pieces, piece = i - which * pieces;
-      const int h = piece / (kHd / 8), c = piece % (kHd / 8);
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (there) {
-        const uint8_t* block = p.pool[which] + (static_cast<int64_t>(page) * p.nkv + h) * p.page_size * F::kRow;
-        const uint32_t code = *reinterpret_cast<const uint32_t*>(block + slot * F::kCodes + 4 * c);
-        const float s = fp4_scale(block[p.page_size * F::kCodes + slot * F::kScales + c / 2]) * p.power[which];
-        uint32_t x[4];
-        fp4_codes(code, x);
-        uint32_t y[4];
+    if (pos >= 0) {
+      const int at = pos >> p.page_shift;
+      page = at < p.table_width ? p.table[b * p.ld_table + at] : -1;
+      if (page < 0 || page >= p.n_pages) {
+        page = -1;
+        record_device_error(p.err, DK_DEVERR_BAD_POSITION);
+      }
+    }
+    place[threadIdx.x] = make_int2(page, pos & (p.page_size - 1));
+  }
+  __syncthreads();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int pieces = p.nkv * (kHd / 8), half = columns / 2;
+  const int64_t page_bytes = static_cast<int64_t>(p.nkv) * p.page_size * F::kRow;
+  const int scales_at = p.page_size * F::kCodes;
+  // A warp keeps its column where there are no more than warps (then they share it out by rows), so that little is computed for each item.
+  const int step = columns <= kWarps ? kWarps / columns : 1;
+  for (int column = warp % columns; column < columns; column += kWarps) {
+    const int which = column >= half, piece = (column - which * half) * 32 + lane;
+    if (columns <= kWarps && warp >= step * columns) break;
+    const int h = piece / (kHd / 8), c = piece % (kHd / 8);
+    const uint8_t* pool = (which ? p.pool[1] : p.pool[0]) + static_cast<int64_t>(h) * p.page_size * F::kRow;
+    const uint8_t *codes = pool + 4 * c, *scales = pool + scales_at + c / 2;
+    const float power = which ? p.power[1] : p.power[0];
+    uint4* out = reinterpret_cast<uint4*>(which ? p.out[1] : p.out[0]) + static_cast<int64_t>(t0) * pieces + piece;
+    if (piece >= pieces) continue;
+    for (int i = columns <= kWarps ? warp / columns : 0; i < n; i += kAhead * step) {
+      uint32_t code[kAhead];
+      uint8_t scale[kAhead];
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) {
+        const int2 at = place[min(i + a * step, n - 1)];
+        code[a] = 0, scale[a] = 0;
+        if (at.x >= 0) {
+          code[a] = *reinterpret_cast<const uint32_t*>(codes + at.x * page_bytes + at.y * F::kCodes);
+          scale[a] = scales[at.x * page_bytes + at.y * F::kScales];
+        }
+      }
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) {
+        if (i + a * step >= n) break;
+        const float s = fp4_scale(scale[a]) * power;
+        uint32_t x[4], y[4];
+        fp4_codes(code[a], x);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const float2 f = Elem<__half>::unpack(x[j]);
           y[j] = Elem<T>::pack(f.x * s, f.y * s);
         }
-        v = make_uint4(y[0], y[1], y[2], y[3]);
+        out[static_cast<int64_t>(i + a * step) * pieces] = make_uint4(y[0], y[1], y[2], y[3]);
       }
-      *reinterpret_cast<uint4*>(static_cast<T*>(p.out[which]) + (static_cast<int64_t>(t) * pieces + piece) * 8) = v;
     }
   }
 }
@@ -111,12 +143,15 @@ extern "C" int dk_paged_read_fp4(const dk_paged_read_fp4_args* args) {
   p.page_shift = __builtin_ctzll(page_size);
   p.table_width = static_cast<int>(width);
   p.err = device_info().err_word;
-  const dim3 grid(static_cast<unsigned>(std::min<int64_t>((T + kWarps - 1) / kWarps, 64ll * device_info().num_sms)));
+  // Up to 32 rows a CTA once every SM has 8 CTAs.
+  const int64_t columns = 2 * ((nkv * (head_dim / 8) + 31) / 32);
+  const int64_t per = std::max<int64_t>(1, std::min<int64_t>(kMaxRows, T / (8ll * device_info().num_sms)));
+  const dim3 grid(static_cast<unsigned>((T + per - 1) / per));
   cudaStream_t st = reinterpret_cast<cudaStream_t>(a.stream);
   cudaError_t e;
 #define DK_READ(TT) \
   e = launch(head_dim == 128 ? paged_read_fp4_kernel<TT, 128> : paged_read_fp4_kernel<TT, 64>, grid, dim3(kWarps * 32), 0, st, \
-             pdl_enabled(), dim3(1, 1, 1), p)
+             pdl_enabled(), dim3(1, 1, 1), p, static_cast<int>(columns), static_cast<int>(per))
   if (dtype == DK_F16)
     DK_READ(__half);
   else

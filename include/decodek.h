@@ -349,9 +349,10 @@ typedef struct dk_paged_read_fp4_args {
 } dk_paged_read_fp4_args;
 int dk_paged_read_fp4(const dk_paged_read_fp4_args* args);
 /* dk_paged_attention and dk_shared_prefix_attention over such pools, with the same arguments, masks and errors, and a workspace of
- * dk_paged_attention_fp4_workspace_bytes. */
+ * dk_paged_attention_fp4_workspace_bytes, for whose `positions` (table_width * page_size) it may hold a 16-bit copy of what prompts
+ * see, up to 1 GB. */
 int dk_paged_attention_fp4_workspace_bytes(int64_t T, int64_t B, int64_t nq, int64_t nkv, int64_t head_dim, int32_t dtype,
-                                           int32_t ragged, int64_t prefix_len, uint64_t* bytes);
+                                           int32_t ragged, int64_t prefix_len, int64_t positions, uint64_t* bytes);
 typedef struct dk_paged_attention_fp4_args {
   dk_paged_attention_args attention;
   double k_scale, v_scale;

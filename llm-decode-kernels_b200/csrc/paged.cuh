@@ -374,6 +374,10 @@ constexpr int kFp4Chunk = 128;
 RowsShape fp4_rows_shape(int64_t hd, int dtype, int rows);
 cudaError_t fp4_rows_launch(const Problem& p, int64_t hd, int dtype, int rows, const RowsShape& s, int wait_late, cudaStream_t st);
 
+// Writes the pages that a ragged call over a 4-bit cache sees in 16 bits, k and v [B * table width, n_kv, page_size, hd] with the tables
+// that list them [B, table width] (paged_read_fp4.cu).
+cudaError_t fp4_copy_launch(const Problem& p, int64_t hd, int dtype, void* k, void* v, int32_t* table, cudaStream_t st);
+
 // The launch of the 256-row tensor-core kernel (paged_attention_tc.cu): CTAs of one wave (0: it does not fit).
 constexpr int kTcChunk = 128;
 constexpr int kTcRows = 256;

@@ -603,8 +603,17 @@ struct Sizes {
   int64_t T, B, nq, nkv, hd, prefix_len;
   bool ragged;
   int dtype;
-  bool fp4;  // the cache is held in 4 bits
+  bool fp4;           // the cache is held in 4 bits,
+  int64_t positions;  // in a row of the page table
 };
+
+// Prompts over a 4-bit cache first have the pages that they see copied in 16 bits, which the tiles then read, instead of converting
+// each chunk for every tile anew. TODO figures
+constexpr int64_t kCopyTokens = 32, kCopyBytes = int64_t(1) << 30;
+bool copies(const Sizes& z) {
+  return z.fp4 && z.ragged && z.prefix_len == 0 && z.T >= kCopyTokens * z.B && z.T > 0 &&
+         z.positions <= kCopyBytes / (4 * z.hd) / z.nkv / z.B;
+}
 
 RowsShape rows_shape_of(const Sizes& z, int rows) {
   if (z.fp4) return fp4_rows_shape(z.hd, z.dtype, rows);
@@ -654,7 +663,7 @@ void cut_pass(const Sizes& z, Cutter& c, Pass& a, bool always_partial) {
     a.rows = kTcRows;
     p.unit_extra = kTcUnitExtra;
     p.rows_inner = 1;
-    a.ctas = tc_ctas(z.hd, z.dtype, z.fp4);
+    a.ctas = tc_ctas(z.hd, z.dtype, z.fp4 && !copies(z));
   } else {
     a.rows = z.nq / z.nkv <= 8 ? 8 : 16;
     a.shape = rows_shape_of(z, a.rows);
@@ -671,6 +680,16 @@ void cut_pass(const Sizes& z, Cutter& c, Pass& a, bool always_partial) {
   p.cum_out = p.mode == kOneToken ? c.take<int32_t>(z.B + 1) : nullptr;
   p.plan = p.mode == kRagged ? c.take<int32_t>(3 + static_cast<int64_t>(p.max_tiles)) : nullptr;
   p.tile_info = p.mode == kRagged ? c.take<int4>(p.max_tiles) : nullptr;
+}
+
+// The copy of the pages and the tables that list them.
+struct Copy {
+  void *k, *v;
+  int32_t* table;
+};
+Copy cut_copy(const Sizes& z, Cutter& c) {
+  const uint64_t positions = static_cast<uint64_t>(z.B * z.positions), bytes = positions * z.nkv * z.hd * 2;
+  return {c.take<char>(bytes), c.take<char>(bytes), c.take<int32_t>(positions / 16)};  // (a page has 16 positions at least)
 }
 
 // Tiles of one token, or of two halves of up to 128 rows each.
@@ -768,6 +787,7 @@ uint64_t workspace_of(const Sizes& z) {
     shape_prefix(z, pre);
     cut_pass(z, c, pre, true);
   }
+  if (copies(z)) cut_copy(z, c);
   return c.used;
 }
 
@@ -791,18 +811,22 @@ int workspace_bytes(const char* what, const Sizes& z, uint64_t* bytes) {
 
 extern "C" int dk_paged_attention_workspace_bytes(int64_t T, int64_t B, int64_t nq, int64_t nkv, int64_t head_dim,
                                                   int32_t dtype, int32_t ragged, int64_t prefix_len, uint64_t* bytes) {
-  return workspace_bytes("paged_attention_workspace_bytes", Sizes{T, B, nq, nkv, head_dim, prefix_len, ragged != 0, dtype, false}, bytes);
+  return workspace_bytes("paged_attention_workspace_bytes", Sizes{T, B, nq, nkv, head_dim, prefix_len, ragged != 0, dtype, false, 0}, bytes);
 }
 
 extern "C" int dk_paged_attention_fp4_workspace_bytes(int64_t T, int64_t B, int64_t nq, int64_t nkv, int64_t head_dim,
-                                                      int32_t dtype, int32_t ragged, int64_t prefix_len, uint64_t* bytes) {
-  return workspace_bytes("paged_attention_fp4_workspace_bytes", Sizes{T, B, nq, nkv, head_dim, prefix_len, ragged != 0, dtype, true}, bytes);
+                                                      int32_t dtype, int32_t ragged, int64_t prefix_len, int64_t positions,
+                                                      uint64_t* bytes) {
+  if (positions <= 0) return set_error(DK_ERR_INVALID, "paged_attention_fp4_workspace_bytes: bad sizes");
+  return workspace_bytes("paged_attention_fp4_workspace_bytes",
+                         Sizes{T, B, nq, nkv, head_dim, prefix_len, ragged != 0, dtype, true, positions}, bytes);
 }
 
 namespace {
 
 int attention(const char* what, const dk_paged_attention_args& a, bool prefix, bool fp4, double k_scale, double v_scale) {
-  const Sizes z{a.T, a.B, a.n_q, a.n_kv, a.head_dim, prefix ? a.prefix_len : 0, a.starts != nullptr, static_cast<int>(a.dtype), fp4};
+  const Sizes z{a.T, a.B, a.n_q, a.n_kv, a.head_dim, prefix ? a.prefix_len : 0, a.starts != nullptr, static_cast<int>(a.dtype), fp4,
+                a.table_width <= INT32_MAX ? a.table_width * a.page_size : 0};
   const int64_t n_pages = a.n_pages, page_size = a.page_size, table_width = a.table_width;
   int64_t window = prefix ? 0 : a.window;
   int64_t sinks = prefix ? 0 : a.sinks;
@@ -840,6 +864,8 @@ int attention(const char* what, const dk_paged_attention_args& a, bool prefix, b
     shape_prefix(z, pre);
     cut_pass(z, c, pre, true);
   }
+  const bool copied = copies(z);
+  const Copy copy = copied ? cut_copy(z, c) : Copy{};
   for (const Pass* s : {&pre, &own}) {
     if (s == &pre && z.prefix_len == 0) continue;
     const int64_t chunk = s->tc ? kTcChunk : kChunk;
@@ -879,7 +905,17 @@ int attention(const char* what, const dk_paged_attention_args& a, bool prefix, b
   if (z.prefix_len > 0) share_gpu(pre, own);
 
   cudaStream_t st = reinterpret_cast<cudaStream_t>(a.stream);
-  const uint64_t rows = static_cast<uint64_t>(n_pages * z.nkv * page_size);
+  cudaError_t e = cudaSuccess;
+  if (z.ragged)
+    e = launch(plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, pdl_enabled(), dim3(1, 1, 1), own.p,
+               const_cast<int32_t*>(own.p.plan), const_cast<int4*>(own.p.tile_info));
+  if (copied) {
+    if (e == cudaSuccess) e = fp4_copy_launch(own.p, z.hd, z.dtype, copy.k, copy.v, copy.table, st);
+    own.p.table = copy.table, own.p.ld_table = table_width;
+    own.p.n_pages = static_cast<int>(z.B * table_width);
+  }
+  const void *k_pages = copied ? copy.k : a.k_pages, *v_pages = copied ? copy.v : a.v_pages;
+  const uint64_t rows = static_cast<uint64_t>(own.p.n_pages * z.nkv * page_size);
   const CUtensorMapDataType type = z.dtype == DK_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   CUtensorMap mk, mv;
   uint32_t box = 0;
@@ -887,18 +923,14 @@ int attention(const char* what, const dk_paged_attention_args& a, bool prefix, b
     const uint32_t want = static_cast<uint32_t>(std::min<int64_t>(page_size, chunk));
     if (want == box) return true;
     box = want;
-    return make_tensor_map_2d(&mk, a.k_pages, type, z.hd, rows, z.hd * 2, 64, box, CU_TENSOR_MAP_SWIZZLE_128B) &&
-           make_tensor_map_2d(&mv, a.v_pages, type, z.hd, rows, z.hd * 2, 64, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    return make_tensor_map_2d(&mk, k_pages, type, z.hd, rows, z.hd * 2, 64, box, CU_TENSOR_MAP_SWIZZLE_128B) &&
+           make_tensor_map_2d(&mv, v_pages, type, z.hd, rows, z.hd * 2, 64, box, CU_TENSOR_MAP_SWIZZLE_128B);
   };
-  cudaError_t e = cudaSuccess;
-  if (z.ragged)
-    e = launch(plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, pdl_enabled(), dim3(1, 1, 1), own.p,
-               const_cast<int32_t*>(own.p.plan), const_cast<int4*>(own.p.tile_info));
   for (const Pass* s : {&pre, &own}) {
     if (s->ctas == 0 || e != cudaSuccess) continue;
-    if (!z.fp4 && !page_maps(s->tc ? kTcChunk : kChunk)) return DK_ERR_CUDA;
+    if ((!z.fp4 || copied) && !page_maps(s->tc ? kTcChunk : kChunk)) return DK_ERR_CUDA;
     if (s->tc) {
-      if (const int rc = tc_launch(s->p, z.nq, z.hd, z.dtype, z.fp4, s->ctas, mk, mv, s == &own ? beside : 0, st)) return rc;
+      if (const int rc = tc_launch(s->p, z.nq, z.hd, z.dtype, z.fp4 && !copied, s->ctas, mk, mv, s == &own ? beside : 0, st)) return rc;
     } else {
       e = launch_rows(z, s->rows, s->shape, st, mk, mv, s->p, s == &own ? beside : 0);
     }

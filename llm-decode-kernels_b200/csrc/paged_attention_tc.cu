@@ -34,13 +34,20 @@ namespace dk {
 namespace paged {
 namespace {
 
-constexpr int kThreads = 384;
-constexpr int kMmaWarp = 8, kLoadWarp = 9, kZeroWarp = 10;  // without kFp4 warp 11 only gives its registers away
-constexpr int kConvertWarp = 10, kConvertWarps = 2;         // kFp4
-// The launch holds 168 registers a thread; the softmax warpgroups take what the third one gives up:
-// 256 * 208 + 128 * 88 = 384 * 168.
-constexpr int kRegsLaunch = 168, kRegsSoftmax = 208, kRegsOther = 88;
-static_assert(256 * kRegsSoftmax + 128 * kRegsOther <= kThreads * kRegsLaunch, "register split");
+constexpr int kMmaWarp = 8, kLoadWarp = 9, kZeroWarp = 10;
+constexpr int kConvertWarp = 10, kConvertWarps = 4;  // kFp4: of warps 10..15; without it warps 10 and 11 only give their registers away
+// The softmax warpgroups take what the others give up of the registers that the launch holds:
+// 256 * 208 + 128 * 88 = 384 * 168, and with two warpgroups more 256 * 208 + 256 * 48 = 512 * 128.
+template <bool kFp4>
+constexpr int kThreads = kFp4 ? 512 : 384;
+template <bool kFp4>
+constexpr int kRegsLaunch = kFp4 ? 128 : 168;
+template <bool kFp4>
+constexpr int kRegsOther = kFp4 ? 48 : 88;
+constexpr int kRegsSoftmax = 208;
+static_assert(256 * kRegsSoftmax + 128 * kRegsOther<false> <= kThreads<false> * kRegsLaunch<false> &&
+                  256 * kRegsSoftmax + 256 * kRegsOther<true> <= kThreads<true> * kRegsLaunch<true>,
+              "register split");
 constexpr int kC = kTcChunk;
 constexpr float kLazy = 8.f;  // growth (base 2) of a row's maximum that P takes without rescaling O
 // P is handed over in two parts, positions 0..95 and 96..127: the products of the first run while the exponentials of the
@@ -230,7 +237,7 @@ __device__ __forceinline__ int q_to_fp16(uint8_t* row, int r) {
 }
 
 template <typename T, int kHd, bool kFp4>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads<kFp4>, 1)
     tiles_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                  const __grid_constant__ CUtensorMap mv, const Problem p, int wait_late) {
   using L = Smem<kHd, kFp4>;
@@ -289,7 +296,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   Walk<kC> walk(p, line, blockIdx.x, gridDim.x, lane);
   bool ok = true;
 
-  if (warp >= kMmaWarp) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
+  if (warp >= kMmaWarp) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther<kFp4>));
   if (warp == kLoadWarp) {
     // ---------------------------------------------------------------- loads
     const int box = min(p.page_size, kC), boxes = kC / box;
@@ -586,7 +593,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc::fence_after_sync();
       const int row = x * 128 + r;
       if (whole) {
-        const float inv = l == 0.f ? 0.f : (kFp4 ? p.out_scale : 1.f) / l;
+        const float inv = l == 0.f ? 0.f : p.out_scale / l;
         // Four lanes exchange 16-byte pieces so that together they store 64 bytes of one row at a time: a lane storing its
         // own row would touch 32 lines with every instruction.
         T* out = static_cast<T*>(p.out) + (static_cast<int64_t>(t.t0 + tok) * p.nkv * p.G + head) * kHd;
@@ -634,12 +641,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
 
-  if (kFp4 && warp >= kConvertWarp) {
-    // ---------------------------------------------------------------- conversion: half of a chunk's rows each, K and V in turn
+  if (kFp4 && warp >= kConvertWarp && warp < kConvertWarp + kConvertWarps) {
+    // ---------------------------------------------------------------- conversion: a quarter of a chunk's rows each, K and V in turn
     // A lane takes 16 bytes of codes, 32 dims of a row, to four 16-byte pieces. The second segment's lanes (head_dim 128) take their
     // pieces in another order, so that 8 lanes' stores hit all banks.
-    constexpr int kRowLanes = kHd / 32, kRowsAtOnce = 32 / kRowLanes;
+    constexpr int kRowLanes = kHd / 32, kRowsAtOnce = 32 / kRowLanes, kSteps = kC / kConvertWarps / kRowsAtOnce;
+    constexpr int kAhead = 2;  // steps whose codes are loaded at a time
     const int q = lane % kRowLanes, flip = q & 2;
+    const int first = (warp - kConvertWarp) * (kC / kConvertWarps) + lane / kRowLanes;  // this lane's rows: first + i * kRowsAtOnce
     int fill = 0;
     while (walk.more() && ok) {
       const Span<kC> span = walk.step();
@@ -649,28 +658,43 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (ok && fill >= L::kSlots && !wait_for(&bar.kv_empty[s], ((fill / L::kSlots) - 1) & 1, p.err, DK_DEVERR_WAIT_EMPTY)) ok = false;
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        const uint8_t* in = raw + from * L::kRawBytes;
-        uint8_t* out = slots + s * L::kTileBytes + (q >> 1) * L::kSegBytes;
+        const uint8_t* codes_in = raw + from * L::kRawBytes + first * Fp4<kHd>::kCodes + 16 * q;
+        const uint8_t* scales_in = raw + from * L::kRawBytes + L::kRawScalesAt + first * Fp4<kHd>::kScales + 2 * q;
+        uint8_t* out = slots + s * L::kTileBytes + (q >> 1) * L::kSegBytes + first * 128;
+        uint8_t* piece[4];  // (the rows of a lane are alike modulo 8, and so is their swizzle)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) piece[k] = out + ((((q & 1) * 4 + (k ^ flip)) ^ (first & 7)) << 4);
         const int j0 = (i >> 1) * kC;
         // V rows of positions that no row of the unit sees become zeros (codes are finite whatever they are)
         const bool clear = (i & 1) == 0 || (j0 + kC <= span.end && (p.mask.window <= 0 || j0 >= span.lo || j0 + kC <= p.mask.sinks));
-#pragma unroll 2
-        for (int r = (warp - kConvertWarp) * (kC / kConvertWarps) + lane / kRowLanes; r < (warp - kConvertWarp + 1) * (kC / kConvertWarps);
-             r += kRowsAtOnce) {
-          const uint4 codes = *reinterpret_cast<const uint4*>(in + r * Fp4<kHd>::kCodes + 16 * q);
-          uint32_t two = *reinterpret_cast<const uint16_t*>(in + L::kRawScalesAt + r * Fp4<kHd>::kScales + 2 * q);
-          if (!clear && !span.needs(j0 + r, 1, p.mask)) two = 0;
-          two = fp4_scales(two);
-          const uint32_t lo = prmt(two, two, 0x1010), hi = prmt(two, two, 0x3232);
-          const uint32_t w[4] = {flip ? codes.z : codes.x, flip ? codes.w : codes.y, flip ? codes.x : codes.z, flip ? codes.y : codes.w};
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint32_t scale = (k < 2) == (flip == 0) ? lo : hi;
-            uint32_t v[4];
-            fp4_codes(w[k], v);
-            const int piece = (q & 1) * 4 + (k ^ flip);
-            *reinterpret_cast<uint4*>(out + r * 128 + ((piece ^ (r & 7)) << 4)) =
-                make_uint4(hmul2_rn(v[0], scale), hmul2_rn(v[1], scale), hmul2_rn(v[2], scale), hmul2_rn(v[3], scale));
+        for (int r0 = 0; r0 < kSteps; r0 += kAhead) {
+          uint4 codes[kAhead];
+          uint32_t scales[kAhead];
+#pragma unroll
+          for (int a = 0; a < kAhead; ++a) {
+            codes[a] = *reinterpret_cast<const uint4*>(codes_in + (r0 + a) * kRowsAtOnce * Fp4<kHd>::kCodes);
+            scales[a] = *reinterpret_cast<const uint16_t*>(scales_in + (r0 + a) * kRowsAtOnce * Fp4<kHd>::kScales);
+          }
+          if (!clear) {
+#pragma unroll
+            for (int a = 0; a < kAhead; ++a)
+              if (!span.needs(j0 + first + (r0 + a) * kRowsAtOnce, 1, p.mask)) scales[a] = 0;
+          }
+#pragma unroll
+          for (int a = 0; a < kAhead; ++a) {
+            const uint32_t two = fp4_scales(scales[a]);
+            const uint32_t lo = prmt(two, two, flip ? 0x3232 : 0x1010), hi = prmt(two, two, flip ? 0x1010 : 0x3232);
+            const uint4 c = codes[a];
+            const uint32_t w[4] = {flip ? c.z : c.x, flip ? c.w : c.y, flip ? c.x : c.z, flip ? c.y : c.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t scale = k < 2 ? lo : hi;
+              uint32_t v[4];
+              fp4_codes(w[k], v);
+              *reinterpret_cast<uint4*>(piece[k] + (r0 + a) * kRowsAtOnce * 128) =
+                  make_uint4(hmul2_rn(v[0], scale), hmul2_rn(v[1], scale), hmul2_rn(v[2], scale), hmul2_rn(v[3], scale));
+            }
           }
         }
         tc::fence_proxy_async_smem();
@@ -731,7 +755,7 @@ int ctas_of() {
   int& n = known[dev & 63];
   if (n == 0) {
     cudaFuncAttributes a;  // the register split needs the launch to hold exactly what it divides
-    const bool split = cudaFuncGetAttributes(&a, tiles_kernel<T, kHd, kFp4>) == cudaSuccess && a.numRegs == kRegsLaunch;
+    const bool split = cudaFuncGetAttributes(&a, tiles_kernel<T, kHd, kFp4>) == cudaSuccess && a.numRegs == kRegsLaunch<kFp4>;
     n = split && opt_in_dynamic_smem(tiles_kernel<T, kHd, kFp4>) >= Smem<kHd, kFp4>::kBytes ? device_info().num_sms : -1;
   }
   return n < 0 ? 0 : n;
@@ -757,7 +781,7 @@ int tc_launch(const Problem& p, int64_t nq, int64_t hd, int dtype, bool fp4, int
   CUtensorMap mq;
   if (!make_q_map(&mq, p, nq, hd, type)) return DK_ERR_CUDA;
 #define DK_TILES(TT, HH, FF)                                                                                                        \
-  launch(tiles_kernel<TT, HH, FF>, dim3(ctas), dim3(kThreads), Smem<HH, FF>::kBytes, st, pdl_enabled(), dim3(1, 1, 1), mq, mk, mv, p, \
+  launch(tiles_kernel<TT, HH, FF>, dim3(ctas), dim3(kThreads<FF>), Smem<HH, FF>::kBytes, st, pdl_enabled(), dim3(1, 1, 1), mq, mk, mv, p, \
          wait_late)
   const cudaError_t e = DK_BY_KIND(DK_TILES);
 #undef DK_TILES

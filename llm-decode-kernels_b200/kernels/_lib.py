@@ -115,7 +115,7 @@ SIGNATURES = {
     "dk_shared_prefix_attention": [ctypes.c_char_p],
     "dk_paged_append_fp4": [ctypes.c_char_p],
     "dk_paged_read_fp4": [ctypes.c_char_p],
-    "dk_paged_attention_fp4_workspace_bytes": [I64, I64, I64, I64, I64, I32, I32, I64, ctypes.POINTER(ctypes.c_uint64)],
+    "dk_paged_attention_fp4_workspace_bytes": [I64, I64, I64, I64, I64, I32, I32, I64, I64, ctypes.POINTER(ctypes.c_uint64)],
     "dk_paged_attention_fp4": [ctypes.c_char_p],
     "dk_shared_prefix_attention_fp4": [ctypes.c_char_p],
     "dk_token_logprobs": [P, I64, I32, P, I64, I64, I64, P, P, P, P, P],

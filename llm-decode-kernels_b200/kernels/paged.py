@@ -135,9 +135,12 @@ def _append(what, qkv, k_pages, v_pages, page_table, lengths, cos, sin, n_heads,
 
 
 @functools.lru_cache(maxsize=4096)
-def _workspace_bytes(T, B, nq, nkv, hd, dtype, ragged, prefix, device, fp4):
+def _workspace_bytes(T, B, nq, nkv, hd, dtype, ragged, prefix, device, positions):
     n = ctypes.c_uint64(0)  # (`device`: the current one, whose number of SMs the size depends on)
-    _lib.call("dk_paged_attention_fp4_workspace_bytes" if fp4 else "dk_paged_attention_workspace_bytes", T, B, nq, nkv, hd, dtype, ragged, prefix, ctypes.byref(n))
+    if positions:  # a cache of 4-bit codes
+        _lib.call("dk_paged_attention_fp4_workspace_bytes", T, B, nq, nkv, hd, dtype, ragged, prefix, positions, ctypes.byref(n))
+    else:
+        _lib.call("dk_paged_attention_workspace_bytes", T, B, nq, nkv, hd, dtype, ragged, prefix, ctypes.byref(n))
     return int(n.value)
 
 
@@ -174,7 +177,7 @@ def _attend(what, entry, q, k_pages, v_pages, prefix_table, prefix_len, page_tab
     code = _DTYPES[dtype]
     # the prefix's length does not change the size, only whether there is one
     nbytes = _workspace_bytes(T, B, nq, n_kv, hd, code, starts is not None, 1 if prefix_len else 0, device,
-                              scales is not None)
+                              0 if scales is None else page_table.shape[1] * page)
     ws = q.new_empty_strided(((nbytes + 1) // 2,), (1,))  # (of a 16-bit type)
     args = (
         q.data_ptr(), ld, k_pages.data_ptr(), v_pages.data_ptr(), n_pages, page, prefix_at, prefix_len,

@@ -153,6 +153,9 @@ struct Problem {
   const int32_t* plan;
   const int4* tile_info;  // {first token, tokens, position of the first one, sequence}
   int max_tiles;
+  int chunk;               // kRagged: positions of a chunk
+  int above, most;         // kRagged: the sequences with more than `above` and at most `most` tokens are the launch's
+  int zero_outside;        // kRagged: the launch writes zeros to rows that belong to no sequence
   int32_t* cum_out;  // kOneToken: [B + 1], the chunks of one kv head before each sequence
   // Partial results: a CTA's first piece of a unit that began before it (slot 2 * CTA), its last piece of a unit that
   // goes on after it (slot 2 * CTA + 1), and with always_partial a slot for each uncut unit after those
@@ -371,8 +374,9 @@ struct RowsShape {
 // Such a launch over a cache held in 4 bits (paged_attention_fp4.cu), with tiles of 8 or 16 rows; kFp4Groups pieces of the line a CTA.
 constexpr int kFp4Groups = 2;
 constexpr int kFp4Chunk = 128;
-RowsShape fp4_rows_shape(int64_t hd, int dtype, int rows);
-cudaError_t fp4_rows_launch(const Problem& p, int64_t hd, int dtype, int rows, const RowsShape& s, int wait_late, cudaStream_t st);
+RowsShape fp4_rows_shape(int64_t hd, int dtype, int rows, bool ragged);
+cudaError_t fp4_rows_launch(const Problem& p, int64_t hd, int dtype, int rows, bool ragged, const RowsShape& s, int wait_late,
+                            cudaStream_t st);
 
 // Writes the pages that a ragged call over a 4-bit cache sees in 16 bits, k and v [B * table width, n_kv, page_size, hd] with the tables
 // that list them [B, table width] (paged_read_fp4.cu).

@@ -32,11 +32,15 @@ constexpr int kCWarps = 4;   // warps of a group
 constexpr int kThreads = kGroups * (kCWarps + 1) * 32;
 constexpr int kMaxRing = 6;
 constexpr int kPlanThreads = 1024;
+constexpr int kFp4UnitExtra = 1;   // the same over a 4-bit cache, whose chunks are longer
 constexpr int kRowsUnitExtra = 2;  // a unit's fixed cost (q, joining the warps, output) in chunks
 
 // ------------------------------------------------------------------------------------ ragged plan
-// One CTA cuts the sequences into tiles of tile_tokens tokens and sums up their chunks.
-__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Problem p, int32_t* plan, int4* info) {
+// One CTA cuts the launch's sequences into tiles of tile_tokens tokens and sums up their chunks. A second one plans a second launch.
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Problem pa, const Problem pb) {
+  const Problem& p = blockIdx.x == 0 ? pa : pb;
+  int32_t* plan = const_cast<int32_t*>(p.plan);
+  int4* info = const_cast<int4*>(p.tile_info);
   constexpr int kOwnTiles = 4;  // tiles of a sequence that its own thread writes
   __shared__ int warp_sum[kPlanThreads / 32];
   __shared__ int long_count;
@@ -73,7 +77,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Problem p, int
     const int b = b0 + tid;
     const int t0 = b < p.B ? min(max(p.starts[b], 0), p.T) : 0;
     const int t1 = b < p.B ? min(max(p.starts[b + 1], t0), p.T) : 0;
-    const int mine = (t1 - t0 + p.tile_tokens - 1) / p.tile_tokens;
+    const int mine = t1 - t0 > p.above && t1 - t0 <= p.most ? (t1 - t0 + p.tile_tokens - 1) / p.tile_tokens : 0;
     int total;
     const int at = tiles + scan(mine, total);
     // sequence and first token of each tile; long sequences are filled in by the whole CTA below
@@ -103,7 +107,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Problem p, int
       const int4 v = info[i];  // {first token, sequence's end, length, sequence}
       const int ntok = min(p.tile_tokens, v.y - v.x), p0 = v.z - (v.y - v.x);
       info[i] = make_int4(v.x, ntok, p0, v.w);
-      n = Span<kTcChunk>(p0, p0 + ntok - 1, p.mask, p.capacity, p.page_size).n + p.unit_extra;
+      n = (p.chunk == kTcChunk ? Span<kTcChunk>(p0, p0 + ntok - 1, p.mask, p.capacity, p.page_size).n
+                               : Span<kFp4Chunk>(p0, p0 + ntok - 1, p.mask, p.capacity, p.page_size).n) + p.unit_extra;
     }
     int total;
     const int at = length + scan(n, total);
@@ -607,16 +612,32 @@ struct Sizes {
   int64_t positions;  // in a row of the page table
 };
 
+// A ragged call over a 4-bit cache: sequences of few tokens (drafted ones to check, decode steps beside prompts) go to the rows kernel,
+// in tiles of up to 16 rows that each read the sequence again, up to kFewTiles of them; longer ones to the 256-row tiles. Which
+// there are only the device knows. A call whose sequences have kManyTokens on average is taken for prompts: then the tiles take
+// all of them. TODO figures
+constexpr int kFewTiles = 3, kManyTokens = 256;
+struct Split {
+  bool few, many;  // which kernels are launched
+  int limit;       // the most tokens of a sequence of the first
+};
+Split split_of(const Sizes& z) {
+  const int64_t limit = kFewTiles * (16 / (z.nq / z.nkv));
+  if (!z.fp4 || !z.ragged || z.prefix_len > 0 || z.T >= kManyTokens * z.B) return {false, true, 0};
+  if (z.T <= limit) return {true, false, INT_MAX};
+  return {z.B > 1, true, z.B > 1 ? static_cast<int>(limit) : 0};
+}
+
 // Prompts over a 4-bit cache first have the pages that they see copied in 16 bits, which the tiles then read, instead of converting
 // each chunk for every tile anew. TODO figures
 constexpr int64_t kCopyTokens = 32, kCopyBytes = int64_t(1) << 30;
 bool copies(const Sizes& z) {
-  return z.fp4 && z.ragged && z.prefix_len == 0 && z.T >= kCopyTokens * z.B && z.T > 0 &&
+  return z.fp4 && z.ragged && z.prefix_len == 0 && split_of(z).many && z.T >= kCopyTokens * z.B && z.T > 0 &&
          z.positions <= kCopyBytes / (4 * z.hd) / z.nkv / z.B;
 }
 
 RowsShape rows_shape_of(const Sizes& z, int rows) {
-  if (z.fp4) return fp4_rows_shape(z.hd, z.dtype, rows);
+  if (z.fp4) return fp4_rows_shape(z.hd, z.dtype, rows, z.ragged);
 #define DK_SHAPE(TT) \
   (z.hd == 128 ? (rows == 8 ? rows_shape<TT, 128, 8>() : rows_shape<TT, 128, 16>()) \
                : (rows == 8 ? rows_shape<TT, 64, 8>() : rows_shape<TT, 64, 16>()))
@@ -626,7 +647,7 @@ RowsShape rows_shape_of(const Sizes& z, int rows) {
 
 cudaError_t launch_rows(const Sizes& z, int rows, const RowsShape& s, cudaStream_t st, const CUtensorMap& mk,
                         const CUtensorMap& mv, const Problem& p, int wait_late) {
-  if (z.fp4) return fp4_rows_launch(p, z.hd, z.dtype, rows, s, wait_late, st);
+  if (z.fp4) return fp4_rows_launch(p, z.hd, z.dtype, rows, z.ragged, s, wait_late, st);
 #define DK_ROWS(TT, HH, RR) \
   launch(rows_kernel<TT, HH, RR>, dim3(s.ctas), dim3(kThreads), s.smem, st, pdl_enabled(), dim3(1, 1, 1), mk, mv, p, s.ring, wait_late)
 #define DK_ROWS_T(TT) \
@@ -665,11 +686,11 @@ void cut_pass(const Sizes& z, Cutter& c, Pass& a, bool always_partial) {
     p.rows_inner = 1;
     a.ctas = tc_ctas(z.hd, z.dtype, z.fp4 && !copies(z));
   } else {
-    a.rows = z.nq / z.nkv <= 8 ? 8 : 16;
+    a.rows = z.nq / z.nkv <= 8 && !z.ragged ? 8 : 16;
     a.shape = rows_shape_of(z, a.rows);
     a.groups = z.fp4 ? kFp4Groups : kGroups;
     a.ctas = a.shape.ctas * a.groups;
-    p.unit_extra = kRowsUnitExtra;
+    p.unit_extra = z.fp4 ? kFp4UnitExtra : kRowsUnitExtra;
   }
   const int64_t tiles = p.mode == kRagged ? p.max_tiles : p.n_tiles;
   const int64_t slots = 2ll * a.ctas + (always_partial ? z.nkv * tiles : 0);
@@ -692,21 +713,36 @@ Copy cut_copy(const Sizes& z, Cutter& c) {
   return {c.take<char>(bytes), c.take<char>(bytes), c.take<int32_t>(positions / 16)};  // (a page has 16 positions at least)
 }
 
-// Tiles of one token, or of two halves of up to 128 rows each.
+// Tiles of one token (ragged: of up to 16 rows), or of two halves of up to 128 rows each.
 void set_tile(const Sizes& z, Pass& a, bool tc) {
+  const int group = static_cast<int>(z.nq / z.nkv);
   a.tc = tc;
-  a.p.half_tokens = tc ? static_cast<int>(128 / (z.nq / z.nkv)) : 1;
-  a.p.tile_tokens = tc ? 2 * a.p.half_tokens : 1;
+  a.p.half_tokens = tc ? 128 / group : z.ragged ? 16 / group : 1;
+  a.p.tile_tokens = tc ? 2 * a.p.half_tokens : a.p.half_tokens;
+  a.p.chunk = tc ? kTcChunk : kFp4Chunk;
+}
+
+void set_ragged(const Sizes& z, Pass& a, int above, int most) {
+  a.p.mode = kRagged;
+  a.p.max_tiles = static_cast<int>(z.T / a.p.tile_tokens + z.B);
+  a.p.above = above, a.p.most = most;
 }
 
 // One token for each sequence goes to the rows kernel, several to the tiles (64 sequences of 8192, 12 heads over 2 kv heads,
 // one token each, without the host: 91 us on the rows kernel, 111 as tiles; one of 640: 9.4 and 13.6; 4 tokens each as tiles:
 // 109).
 void shape_own(const Sizes& z, Pass& a) {
-  set_tile(z, a, z.ragged);
-  a.p.mode = z.ragged ? kRagged : kOneToken;
-  a.p.max_tiles = z.ragged ? static_cast<int>(z.T / a.p.tile_tokens + z.B) : 0;
+  const Split split = split_of(z);
+  set_tile(z, a, z.ragged && split.many);
   a.p.n_tiles = static_cast<int>(z.B);
+  if (z.ragged) set_ragged(z, a, split.many ? split.limit : 0, INT_MAX);
+  a.p.zero_outside = z.ragged && z.prefix_len == 0;
+}
+
+// The sequences of few tokens of a ragged call that has others too.
+void shape_few(const Sizes& z, Pass& a) {
+  set_tile(z, a, false);
+  set_ragged(z, a, 0, split_of(z).limit);
 }
 
 // A prefix is read by tiles however few the rows are (8192 positions for one token of 12 heads: 17 us, 29 on the rows
@@ -721,14 +757,14 @@ void shape_prefix(const Sizes& z, Pass& a) {
 // The two launches of a call with a prefix run side by side: the prefix's takes most of the SMs, and the own positions'
 // starts on the others right away, with longer pieces there. How long the prefix's takes is known here: about 6 us and 2 us
 // for each chunk of a CTA's piece; a group of the other takes 1.1 us for a chunk.
-void share_gpu(Pass& pre, Pass& own) {
+void share_gpu(const Sizes& z, Pass& pre, Pass& own) {
   if (own.tc || !pdl_enabled()) return;
   const int sms = device_info().num_sms;
   const int64_t n = static_cast<int64_t>((pre.p.prefix_len + kTcChunk - 1) / kTcChunk + pre.p.unit_extra) * pre.p.n_tiles * pre.p.nkv;
   const int64_t most = sms * 7 / 8, per = (n + most - 1) / most;
   pre.ctas = static_cast<int>((n + per - 1) / per);
   own.p.early = own.groups * (sms - pre.ctas);
-  own.p.lead = static_cast<int>((60 + 20 * per) / 11);
+  own.p.lead = static_cast<int>(z.fp4 ? (60 + 20 * per) / 22 : (60 + 20 * per) / 11);
 }
 
 int check_sizes(const char* what, const Sizes& z) {
@@ -786,6 +822,11 @@ uint64_t workspace_of(const Sizes& z) {
   if (z.prefix_len > 0) {
     shape_prefix(z, pre);
     cut_pass(z, c, pre, true);
+  }
+  if (split_of(z).few && split_of(z).many) {
+    Pass few = {};
+    shape_few(z, few);
+    cut_pass(z, c, few, false);
   }
   if (copies(z)) cut_copy(z, c);
   return c.used;
@@ -856,7 +897,7 @@ int attention(const char* what, const dk_paged_attention_args& a, bool prefix, b
   if (!aligned16(a.q) || !aligned16(a.k_pages) || !aligned16(a.v_pages) || !aligned16(a.out) || (ldq & 7) ||
       (reinterpret_cast<uintptr_t>(a.workspace) & 255))
     return set_error(DK_ERR_ALIGN, "%s: q rows, pages and out need 16-byte alignment, the workspace 256", what);
-  Pass own = {}, pre = {};
+  Pass own = {}, pre = {}, few = {};
   Cutter c{static_cast<char*>(a.workspace)};
   shape_own(z, own);
   cut_pass(z, c, own, z.prefix_len > 0);
@@ -864,10 +905,15 @@ int attention(const char* what, const dk_paged_attention_args& a, bool prefix, b
     shape_prefix(z, pre);
     cut_pass(z, c, pre, true);
   }
+  const bool has_few = split_of(z).few && split_of(z).many;
+  if (has_few) {
+    shape_few(z, few);
+    cut_pass(z, c, few, false);
+  }
   const bool copied = copies(z);
   const Copy copy = copied ? cut_copy(z, c) : Copy{};
-  for (const Pass* s : {&pre, &own}) {
-    if (s == &pre && z.prefix_len == 0) continue;
+  for (const Pass* s : {&pre, &few, &own}) {
+    if ((s == &pre && z.prefix_len == 0) || (s == &few && !has_few)) continue;
     const int64_t chunk = s->tc ? kTcChunk : kChunk;
     const int64_t tiles = s->p.mode == kRagged ? s->p.max_tiles : s->p.n_tiles;
     const int64_t positions = s->p.mode == kPrefix ? z.prefix_len : table_width * page_size;
@@ -878,10 +924,10 @@ int attention(const char* what, const dk_paged_attention_args& a, bool prefix, b
   if (c.used > a.workspace_bytes)
     return set_error(DK_ERR_INVALID, "%s: the workspace has %llu bytes, %llu are needed", what,
                      (unsigned long long)a.workspace_bytes, (unsigned long long)c.used);
-  if (own.ctas == 0 || (z.prefix_len > 0 && pre.ctas == 0))
+  if (own.ctas == 0 || (z.prefix_len > 0 && pre.ctas == 0) || (has_few && few.ctas == 0))
     return set_error(DK_ERR_UNSUPPORTED, "%s: the kernel's shared memory does not fit this device", what);
   const int beside = z.prefix_len > 0 && pdl_enabled() ? 1 : 0;
-  for (Problem* p : {&own.p, &pre.p}) {
+  for (Problem* p : {&own.p, &pre.p, &few.p}) {
     p->q = a.q, p->ldq = ldq, p->out = a.out;
     p->table = a.page_table, p->ld_table = a.ld_table, p->lengths = a.lengths, p->starts = a.starts;
     p->T = static_cast<int>(z.T), p->B = static_cast<int>(z.B), p->nkv = static_cast<int>(z.nkv);
@@ -902,13 +948,12 @@ int attention(const char* what, const dk_paged_attention_args& a, bool prefix, b
     s->p.scale2 = scale2 < 0.f ? -scale2 : scale2 == 0.f ? 1.f : scale2;
   }
   pre.p.table = a.prefix_table, pre.p.capacity = static_cast<int>(z.prefix_len), pre.p.mask = Mask{0, 0};
-  if (z.prefix_len > 0) share_gpu(pre, own);
+  if (z.prefix_len > 0) share_gpu(z, pre, own);
 
   cudaStream_t st = reinterpret_cast<cudaStream_t>(a.stream);
   cudaError_t e = cudaSuccess;
   if (z.ragged)
-    e = launch(plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, pdl_enabled(), dim3(1, 1, 1), own.p,
-               const_cast<int32_t*>(own.p.plan), const_cast<int4*>(own.p.tile_info));
+    e = launch(plan_kernel, dim3(has_few ? 2 : 1), dim3(kPlanThreads), 0, st, pdl_enabled(), dim3(1, 1, 1), own.p, few.p);
   if (copied) {
     if (e == cudaSuccess) e = fp4_copy_launch(own.p, z.hd, z.dtype, copy.k, copy.v, copy.table, st);
     own.p.table = copy.table, own.p.ld_table = table_width;
@@ -926,21 +971,22 @@ int attention(const char* what, const dk_paged_attention_args& a, bool prefix, b
     return make_tensor_map_2d(&mk, k_pages, type, z.hd, rows, z.hd * 2, 64, box, CU_TENSOR_MAP_SWIZZLE_128B) &&
            make_tensor_map_2d(&mv, v_pages, type, z.hd, rows, z.hd * 2, 64, box, CU_TENSOR_MAP_SWIZZLE_128B);
   };
-  for (const Pass* s : {&pre, &own}) {
+  for (const Pass* s : {&pre, &few, &own}) {
     if (s->ctas == 0 || e != cudaSuccess) continue;
-    if ((!z.fp4 || copied) && !page_maps(s->tc ? kTcChunk : kChunk)) return DK_ERR_CUDA;
+    if ((!z.fp4 || (copied && s->tc)) && !page_maps(s->tc ? kTcChunk : kChunk)) return DK_ERR_CUDA;
     if (s->tc) {
       if (const int rc = tc_launch(s->p, z.nq, z.hd, z.dtype, z.fp4 && !copied, s->ctas, mk, mv, s == &own ? beside : 0, st)) return rc;
     } else {
       e = launch_rows(z, s->rows, s->shape, st, mk, mv, s->p, s == &own ? beside : 0);
     }
   }
-  const Pass* with = z.prefix_len > 0 ? &pre : nullptr;
-  if (e == cudaSuccess) {
+  for (const Pass* s : {&few, &own}) {
+    if (s->ctas == 0 || e != cudaSuccess) continue;
+    const Pass* with = z.prefix_len > 0 ? &pre : nullptr;
     if (z.dtype == DK_F16)
-      e = z.hd == 128 ? launch_join<__half, 128>(z, st, with, own) : launch_join<__half, 64>(z, st, with, own);
+      e = z.hd == 128 ? launch_join<__half, 128>(z, st, with, *s) : launch_join<__half, 64>(z, st, with, *s);
     else
-      e = z.hd == 128 ? launch_join<__nv_bfloat16, 128>(z, st, with, own) : launch_join<__nv_bfloat16, 64>(z, st, with, own);
+      e = z.hd == 128 ? launch_join<__nv_bfloat16, 128>(z, st, with, *s) : launch_join<__nv_bfloat16, 64>(z, st, with, *s);
   }
   if (e != cudaSuccess) return set_error(DK_ERR_CUDA, "%s launch: %s", what, cudaGetErrorString(e));
   return DK_OK;

@@ -38,7 +38,7 @@ static_assert(kChunk == kCWarps * kSub * 16, "a chunk is one round of the warps"
 constexpr int kThreads = kFp4Groups * (kCWarps + 1) * 32;
 // Slots of a group's ring: what fits the shared memory of two CTAs an SM (one with 16 rows).
 template <int kHd, int kBlocks>
-constexpr int kRing = kHd == 64 ? (kBlocks == 1 ? 8 : 10) / kSub : (kBlocks == 1 ? 4 : 6) / kSub;
+constexpr int kRing = kHd == 64 ? (kBlocks == 1 ? 4 : 5) : (kBlocks == 1 ? 2 : 3);
 constexpr float kRefBelow = 6.f, kRefReach = 14.f;
 
 // A chunk in shared memory: for k and v each the codes of kChunk positions, then their scales.
@@ -65,7 +65,8 @@ __device__ __forceinline__ uint32_t choose(uint32_t a, uint32_t b, uint32_t m) {
 
 __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((127 + e) << 23); }
 
-template <typename T, int kHd, int kBlocks>
+// kRagged: tiles of the plan, a few tokens each; otherwise tile b is the one token of sequence b.
+template <typename T, int kHd, int kBlocks, bool kRaggedTiles>
 __global__ void __launch_bounds__(kThreads, kBlocks == 1 ? 2 : 1) fp4_rows_kernel(const Problem p, int wait_late) {
   constexpr int ring = kRing<kHd, kBlocks>;
   using F = Fp4<kHd>;
@@ -74,9 +75,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks == 1 ? 2 : 1) fp4_rows_kerne
   constexpr int kSteps = kHd / 16;        // products of a tile of k, and tiles of v's product
   constexpr int kWords = kHd / 32;        // words of a lane's codes of k; v's has kHd / 64
   constexpr uint32_t kLow = 0x0f0f0f0fu;
-  __shared__ float pre_ml_sh[kFp4Groups][kCWarps * kRows * 2];
-  __shared__ float pre_w_sh[kFp4Groups][kCWarps * kRows];
-  __shared__ float fin_sh[kFp4Groups][kRows * 2];
+  __shared__ float2 pre_ml_sh[kFp4Groups][kRows * kCWarps];
   __shared__ __align__(8) uint64_t full_sh[kFp4Groups][ring], empty_sh[kFp4Groups][ring];
   __shared__ int warp_sum[kThreads / 32 + 1];
   extern __shared__ __align__(128) uint8_t base[];
@@ -88,7 +87,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks == 1 ? 2 : 1) fp4_rows_kerne
   const int cta = blockIdx.x * kFp4Groups + group, ctas = gridDim.x * kFp4Groups;  // pieces of the line: one a group
   uint8_t* slots = base + group * ring * S::kBytes;
   float* pre_o = reinterpret_cast<float*>(base + kFp4Groups * ring * S::kBytes) + group * kCWarps * kRows * kHd;
-  float *pre_ml = pre_ml_sh[group], *pre_w = pre_w_sh[group], *fin = fin_sh[group];
+  float2* pre_ml = pre_ml_sh[group];
   uint64_t *full = full_sh[group], *empty = empty_sh[group];
   if (tid == 0) {
     for (int i = 0; i < kFp4Groups * ring; ++i) {
@@ -101,7 +100,9 @@ __global__ void __launch_bounds__(kThreads, kBlocks == 1 ? 2 : 1) fp4_rows_kerne
   pdl_trigger();
 
   Line line{cum_sh, 0, p.n_tiles, 0};
-  {  // every CTA sums up the sequences' chunks for itself
+  if constexpr (kRaggedTiles) {
+    line = line_of(p, kChunk);
+  } else {  // every CTA sums up the sequences' chunks for itself
     int carry = 0;
     for (int b0 = 0; b0 < p.B; b0 += kThreads) {
       const int b = b0 + tid;
@@ -196,23 +197,25 @@ __global__ void __launch_bounds__(kThreads, kBlocks == 1 ? 2 : 1) fp4_rows_kerne
     const int sub = warp % kCWarps, gtid = tid - group * kCWarps * 32;
     const int row_a = (g >> 1) + 4 * (g & 1);  // the position of a tile in the products' row g; row g + 8 has the one 8 on
     if (gtid == 0) p.cut[cta] = make_int4(0, 0, 0, 0);
+    bool joined = false;
     while (walk.more()) {
       const Span<kChunk> span = walk.step();
       const Tile t = walk.t;
       const int h = walk.h, c0 = walk.c0, c1 = walk.c1;
       if (c1 <= c0) continue;
-      const int rows = p.G;  // one token's
-      const int p0 = t.p0 - span.shift;
+      const int rows = t.ntok * p.G, p0 = t.p0 - span.shift, p1 = p0 + t.ntok - 1;  // (positions in the span's offsets)
       // the chunks that every row sees all of (nothing to mask)
-      const int clear_from = p.mask.window > 0 ? (max(0, p0 - p.mask.window + 1) + kChunk - 1) / kChunk : 0;
+      const int clear_from = p.mask.window > 0 ? (max(0, p1 - p.mask.window + 1) + kChunk - 1) / kChunk : 0;
       const int clear_to = max(min(p0 + 1, span.end), 0) / kChunk;
+      int pos[kBlocks][2];  // of the rows in columns 2 tq and 2 tq + 1
       // q as the products' column operand: column g has query row 8 * block + g, the lane its dims from tq * kHd / 4 on
       uint32_t qb[kBlocks][kSteps][2];
       float scale2[kBlocks][2];  // of columns 2 tq and 2 tq + 1
 #pragma unroll
       for (int nb = 0; nb < kBlocks; ++nb) {
         const int row = 8 * nb + g;
-        const T* qr = static_cast<const T*>(p.q) + t.t0 * p.ldq + (h * p.G + row) * kHd + tq * (kHd / 4);
+        const int tok = kRaggedTiles ? row / p.G : 0;
+        const T* qr = static_cast<const T*>(p.q) + (t.t0 + tok) * p.ldq + (h * p.G + row - tok * p.G) * kHd + tq * (kHd / 4);
         uint4 raw[kSteps / 2];
 #pragma unroll
         for (int i = 0; i < kSteps / 2; ++i)
@@ -248,6 +251,8 @@ __global__ void __launch_bounds__(kThreads, kBlocks == 1 ? 2 : 1) fp4_rows_kerne
           }
         }
 #pragma unroll
+        for (int u = 0; u < 2; ++u) pos[nb][u] = p0 + (kRaggedTiles ? (8 * nb + 2 * tq + u) / p.G : 0);
+#pragma unroll
         for (int u = 0; u < 2; ++u) scale2[nb][u] = p.scale2 * power_of_two(-__shfl_sync(0xffffffffu, e, 4 * (2 * tq + u)));
       }
       float o[kBlocks][kSteps][4];
@@ -260,9 +265,8 @@ __global__ void __launch_bounds__(kThreads, kBlocks == 1 ? 2 : 1) fp4_rows_kerne
         for (int u = 0; u < 2; ++u) base[nb][u] = 0.f, reach[nb][u] = -INFINITY, l[nb][u] = 0.f;
       }
 
-      // The warp's kSub tiles of chunk i, in slot s. kClear: every row sees all of the positions.
-      auto tiles = [&](int i, auto all_seen) {
-        constexpr bool kClear = decltype(all_seen)::value;
+      // The warp's kSub tiles of chunk i, in slot s. clear: every row sees all of the positions.
+      auto tiles = [&](int i, bool clear) {
         const int r0 = 16 * kSub * sub;
         const uint8_t* kt = slots + s * S::kBytes;
         const uint8_t* vt = kt + S::kTensor;
@@ -325,12 +329,20 @@ __global__ void __launch_bounds__(kThreads, kBlocks == 1 ? 2 : 1) fp4_rows_kerne
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               y[tile][e] = fmaf(sc[tile][nb][e], scale2[nb][e & 1], -base[nb][e & 1]);
-              if constexpr (!kClear) {
-                const int j = i * kChunk + r0 + 16 * tile + row_a + 8 * (e >> 1);
-                if (!(j < span.end && p.mask.sees(p0, j))) y[tile][e] = -INFINITY;
-              }
-              top[e & 1] = fmaxf(top[e & 1], y[tile][e]);
             }
+          if (!clear) {
+#pragma unroll
+            for (int tile = 0; tile < kSub; ++tile)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int j = i * kChunk + r0 + 16 * tile + row_a + 8 * (e >> 1);
+                if (!(j < span.end && p.mask.sees(pos[nb][e & 1], j))) y[tile][e] = -INFINITY;
+              }
+          }
+#pragma unroll
+          for (int tile = 0; tile < kSub; ++tile)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) top[e & 1] = fmaxf(top[e & 1], y[tile][e]);
           if (__any_sync(0xffffffffu, top[0] > reach[nb][0] || top[1] > reach[nb][1])) {
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
@@ -382,8 +394,11 @@ __global__ void __launch_bounds__(kThreads, kBlocks == 1 ? 2 : 1) fp4_rows_kerne
               vw[e][0] = *reinterpret_cast<const uint32_t*>(vt + r * F::kCodes + 4 * g);
               vs[e] = vt[S::kScalesAt + r * F::kScales + (g >> 1)];
             }
-            if constexpr (!kClear)
-              if (!span.needs(i * kChunk + r, 1, p.mask)) vs[e] = 0;
+          }
+          if (!clear) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (!span.needs(i * kChunk + r0 + 16 * tile + tq + 4 * e, 1, p.mask)) vs[e] = 0;
           }
           const uint32_t s01 = fp4_scales(vs[0] | vs[1] << 8), s23 = fp4_scales(vs[2] | vs[3] << 8);
 #pragma unroll
@@ -406,16 +421,16 @@ __global__ void __launch_bounds__(kThreads, kBlocks == 1 ? 2 : 1) fp4_rows_kerne
         if (ok && !wait_for(&full[s], round & 1, p.err, DK_DEVERR_WAIT_FULL)) ok = false;
         ok = __all_sync(0xffffffffu, ok);
         if (ok) {
-          if (i >= clear_from && i < clear_to)
-            tiles(i, std::true_type());
-          else if (span.needs(i * kChunk + 16 * kSub * sub, 16 * kSub, p.mask))
-            tiles(i, std::false_type());
+          const bool clear = i >= clear_from && i < clear_to;
+                    if (clear || span.needs(i * kChunk + 16 * kSub * sub, 16 * kSub, p.mask)) tiles(i, clear);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[s]);
       }
       // the warps' results of this part of the unit, joined
       if (gtid == 0 && walk.cut(span)) p.cut[cta] = walk.cut_record(span);
+      if (joined) group_sync(group);  // (the last part's results have been read)
+      joined = true;
 #pragma unroll
       for (int nb = 0; nb < kBlocks; ++nb)
 #pragma unroll
@@ -424,58 +439,52 @@ __global__ void __launch_bounds__(kThreads, kBlocks == 1 ? 2 : 1) fp4_rows_kerne
           sum += __shfl_xor_sync(0xffffffffu, sum, 4);
           sum += __shfl_xor_sync(0xffffffffu, sum, 8);
           sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-          const int row = sub * kRows + 8 * nb + 2 * tq + u;
-          float* to = &pre_o[row * kHd + g * (kHd / 8)];
+          const int row = 8 * nb + 2 * tq + u;
+          float* to = &pre_o[(sub * kRows + row) * kHd + g * (kHd / 8)];
 #pragma unroll
           for (int k = 0; k < kSteps; k += 2)
             *reinterpret_cast<float4*>(to + 2 * k) = make_float4(o[nb][k][u], o[nb][k][u + 2], o[nb][k + 1][u], o[nb][k + 1][u + 2]);
-          if (g == 0) {
-            pre_ml[row * 2] = reach[nb][u] == -INFINITY ? -INFINITY : base[nb][u];
-            pre_ml[row * 2 + 1] = sum;
-          }
+          if (g == 0) pre_ml[row * kCWarps + sub] = make_float2(reach[nb][u] == -INFINITY ? -INFINITY : base[nb][u], sum);
         }
       group_sync(group);
       const bool all_of_it = c0 == 0 && c1 == span.n, whole = all_of_it && !p.always_partial;
-      if (gtid < kRows) {
-        float mx = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < kCWarps; ++w) mx = fmaxf(mx, pre_ml[(w * kRows + gtid) * 2]);
-        const float m_use = mx == -INFINITY ? 0.f : mx;
-        float ls = 0.f;
+      const int64_t slot = partial_slot(ctas, cta, c0 == 0, all_of_it, h * line.tiles + walk.ti);
+      for (int e = gtid; e < rows * (kHd / 4) && ok; e += kCWarps * 32) {
+        const int row = e / (kHd / 4), d = 4 * (e % (kHd / 4));
+        float2 ml[kCWarps];
+        float m = -INFINITY, sum = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < kCWarps; ++w) {
-          const float wt = exp2_approx(pre_ml[(w * kRows + gtid) * 2] - m_use);
-          pre_w[w * kRows + gtid] = wt;
-          ls = fmaf(wt, pre_ml[(w * kRows + gtid) * 2 + 1], ls);
+          ml[w] = pre_ml[row * kCWarps + w];
+          m = fmaxf(m, ml[w].x);
         }
-        fin[2 * gtid] = mx;
-        fin[2 * gtid + 1] = ls;
-      }
-      group_sync(group);
-      const int64_t slot = partial_slot(ctas, cta, c0 == 0, all_of_it, h * line.tiles + walk.ti);
-      if (ok) {
-        for (int e = gtid; e < rows * (kHd / 4); e += kCWarps * 32) {
-          const int row = e / (kHd / 4), d = 4 * (e % (kHd / 4));
-          float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        const float use = m == -INFINITY ? 0.f : m;
 #pragma unroll
-          for (int w = 0; w < kCWarps; ++w) {
-            const float wt = pre_w[w * kRows + row];
-            const float4 v = *reinterpret_cast<const float4*>(&pre_o[(w * kRows + row) * kHd + d]);
-            a.x = fmaf(wt, v.x, a.x), a.y = fmaf(wt, v.y, a.y), a.z = fmaf(wt, v.z, a.z), a.w = fmaf(wt, v.w, a.w);
-          }
-          if (whole) {
-            const float sum = fin[2 * row + 1];
-            const float inv = sum == 0.f ? 0.f : p.out_scale / sum;
-            T* dst = static_cast<T*>(p.out) + (static_cast<int64_t>(t.t0) * p.nkv * p.G + h * p.G + row) * kHd + d;
-            *reinterpret_cast<uint2*>(dst) = make_uint2(Elem<T>::pack(a.x * inv, a.y * inv), Elem<T>::pack(a.z * inv, a.w * inv));
-          } else {
-            *reinterpret_cast<float4*>(&p.part_o[(slot * kRows + row) * kHd + d]) = a;
-          }
+        for (int w = 0; w < kCWarps; ++w) {
+          const float wt = exp2_approx(ml[w].x - use);
+          const float4 v = *reinterpret_cast<const float4*>(&pre_o[(w * kRows + row) * kHd + d]);
+          sum = fmaf(wt, ml[w].y, sum);
+          acc.x = fmaf(wt, v.x, acc.x), acc.y = fmaf(wt, v.y, acc.y), acc.z = fmaf(wt, v.z, acc.z), acc.w = fmaf(wt, v.w, acc.w);
         }
-        if (!whole && gtid < rows)
-          *reinterpret_cast<float2*>(&p.part_ml[(slot * kRows + gtid) * 2]) = make_float2(fin[2 * gtid], fin[2 * gtid + 1]);
+        if (whole) {
+          const float inv = sum == 0.f ? 0.f : p.out_scale / sum;
+          const int tok = kRaggedTiles ? row / p.G : 0;
+          T* dst = static_cast<T*>(p.out) + ((static_cast<int64_t>(t.t0 + tok) * p.nkv + h) * p.G + row - tok * p.G) * kHd + d;
+          *reinterpret_cast<uint2*>(dst) = make_uint2(Elem<T>::pack(acc.x * inv, acc.y * inv), Elem<T>::pack(acc.z * inv, acc.w * inv));
+        } else {
+          *reinterpret_cast<float4*>(&p.part_o[(slot * kRows + row) * kHd + d]) = acc;
+          if (d == 0) *reinterpret_cast<float2*>(&p.part_ml[(slot * kRows + row) * 2]) = make_float2(m, sum);
+        }
       }
-      group_sync(group);  // pre_o, pre_ml and fin are written again by the next piece
+    }
+  }
+  if (kRaggedTiles && p.zero_outside && producer) {  // rows that belong to no sequence are in no tile: their outputs are zero
+    const int from = min(max(p.starts[0], 0), p.T), to = max(min(p.starts[p.B], p.T), from);
+    const int vecs = p.nkv * p.G * kHd / 8;  // 16 bytes each
+    for (int r = cta; r < p.T - (to - from); r += ctas) {
+      uint4* row = reinterpret_cast<uint4*>(p.out) + static_cast<int64_t>(r < from ? r : r - from + to) * vecs;
+      for (int i = lane; i < vecs; i += 32) row[i] = make_uint4(0, 0, 0, 0);
     }
   }
   if (__syncthreads_or(!ok) && producer && lane == 0) {
@@ -488,7 +497,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks == 1 ? 2 : 1) fp4_rows_kerne
   if (wait_late) pdl_wait();
 }
 
-template <typename T, int kHd, int kBlocks>
+template <typename T, int kHd, int kBlocks, bool kRaggedTiles>
 RowsShape shape() {
   static std::mutex mu;
   static int per_sm[64];  // by device; 0: not asked yet
@@ -502,7 +511,7 @@ RowsShape shape() {
   std::lock_guard<std::mutex> lock(mu);
   int& n = per_sm[dev & 63];
   if (n == 0) {
-    auto k = fp4_rows_kernel<T, kHd, kBlocks>;
+    auto k = fp4_rows_kernel<T, kHd, kBlocks, kRaggedTiles>;
     if (opt_in_dynamic_smem(k) < static_cast<int>(s.smem) ||
         cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k, kThreads, s.smem) != cudaSuccess) {
       cudaGetLastError();
@@ -515,22 +524,23 @@ RowsShape shape() {
 
 }  // namespace
 
-#define DK_BY_KIND(CALL)                                                                                          \
-  (dtype == DK_F16 ? (hd == 128 ? (rows == 8 ? CALL(__half, 128, 1) : CALL(__half, 128, 2))                       \
-                                : (rows == 8 ? CALL(__half, 64, 1) : CALL(__half, 64, 2)))                        \
-                   : (hd == 128 ? (rows == 8 ? CALL(__nv_bfloat16, 128, 1) : CALL(__nv_bfloat16, 128, 2))         \
-                                : (rows == 8 ? CALL(__nv_bfloat16, 64, 1) : CALL(__nv_bfloat16, 64, 2))))
+// One token each: tiles of 8 or 16 rows; ragged: of 16.
+#define DK_BY_KIND(CALL, TT, HH) (ragged ? CALL(TT, HH, 2, true) : rows == 8 ? CALL(TT, HH, 1, false) : CALL(TT, HH, 2, false))
+#define DK_BY_TYPE(CALL)                                                                                  \
+  (dtype == DK_F16 ? (hd == 128 ? DK_BY_KIND(CALL, __half, 128) : DK_BY_KIND(CALL, __half, 64))           \
+                   : (hd == 128 ? DK_BY_KIND(CALL, __nv_bfloat16, 128) : DK_BY_KIND(CALL, __nv_bfloat16, 64)))
 
-RowsShape fp4_rows_shape(int64_t hd, int dtype, int rows) {
-#define DK_SHAPE(TT, HH, NB) shape<TT, HH, NB>()
-  return DK_BY_KIND(DK_SHAPE);
+RowsShape fp4_rows_shape(int64_t hd, int dtype, int rows, bool ragged) {
+#define DK_SHAPE(TT, HH, NB, RR) shape<TT, HH, NB, RR>()
+  return DK_BY_TYPE(DK_SHAPE);
 #undef DK_SHAPE
 }
 
-cudaError_t fp4_rows_launch(const Problem& p, int64_t hd, int dtype, int rows, const RowsShape& s, int wait_late, cudaStream_t st) {
-#define DK_ROWS(TT, HH, NB) \
-  launch(fp4_rows_kernel<TT, HH, NB>, dim3(s.ctas), dim3(kThreads), s.smem, st, pdl_enabled(), dim3(1, 1, 1), p, wait_late)
-  return DK_BY_KIND(DK_ROWS);
+cudaError_t fp4_rows_launch(const Problem& p, int64_t hd, int dtype, int rows, bool ragged, const RowsShape& s, int wait_late,
+                            cudaStream_t st) {
+#define DK_ROWS(TT, HH, NB, RR) \
+  launch(fp4_rows_kernel<TT, HH, NB, RR>, dim3(s.ctas), dim3(kThreads), s.smem, st, pdl_enabled(), dim3(1, 1, 1), p, wait_late)
+  return DK_BY_TYPE(DK_ROWS);
 #undef DK_ROWS
 }
 

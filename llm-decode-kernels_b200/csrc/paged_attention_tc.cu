@@ -706,7 +706,7 @@ __global__ void __launch_bounds__(kThreads<kFp4>, 1)
       }
     }
   }
-  if (warp == kZeroWarp && p.mode == kRagged && !p.always_partial) {
+  if (warp == kZeroWarp && p.zero_outside) {
     // Rows that belong to no sequence are in no tile: their outputs are zero. (Beside a prefix the join writes all rows.)
     const int from = min(max(p.starts[0], 0), p.T), to = max(min(p.starts[p.B], p.T), from);
     const int vecs = p.nkv * p.G * kHd / 8;  // 16 bytes each

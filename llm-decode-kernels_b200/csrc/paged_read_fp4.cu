@@ -117,6 +117,7 @@ struct CopyParams {
   const int32_t* lengths;
   const int32_t* starts;
   int T, B, nkv, n_pages, page_size, page_shift, width;
+  int above;  // sequences of more tokens are copied
   Mask mask;
   int* err;
 };
@@ -134,7 +135,7 @@ __global__ void __launch_bounds__(kWarps * 32) fp4_copy_kernel(const CopyParams 
     // seen: below the length, and from the first row's window on or below the sinks
     const int t0 = min(max(p.starts[b], 0), p.T), rows = min(max(p.starts[b + 1], t0), p.T) - t0;
     const int length = length_of(p.lengths, b);
-    if (rows == 0 || j0 >= length) continue;
+    if (rows <= p.above || j0 >= length) continue;
     if (p.mask.window > 0 && j0 + 15 <= length - rows - p.mask.window && j0 >= p.mask.sinks) continue;
     const int at = j0 >> p.page_shift, page = p.table[b * p.ld_table + at];
     const int64_t to = static_cast<int64_t>(b) * p.width + at;
@@ -186,7 +187,7 @@ cudaError_t fp4_copy_launch(const Problem& p, int64_t hd, int dtype, void* k, vo
   c.pool[0] = p.pool[0], c.pool[1] = p.pool[1], c.out[0] = k, c.out[1] = v, c.table_out = table;
   c.table = p.table, c.ld_table = p.ld_table, c.lengths = p.lengths, c.starts = p.starts;
   c.T = p.T, c.B = p.B, c.nkv = p.nkv, c.n_pages = p.n_pages, c.page_size = p.page_size, c.page_shift = p.page_shift;
-  c.width = p.capacity >> p.page_shift, c.mask = p.mask, c.err = p.err;
+  c.above = p.above, c.width = p.capacity >> p.page_shift, c.mask = p.mask, c.err = p.err;
   const int64_t units = static_cast<int64_t>(p.B) * (p.capacity / 16);
   const dim3 grid(static_cast<unsigned>(std::min<int64_t>((units + kWarps - 1) / kWarps, 8ll * device_info().num_sms)));
 #define DK_COPY(TT) \

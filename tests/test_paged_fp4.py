@@ -309,6 +309,14 @@ RAGGED = [
     ([(4, 900), (2, 31), (5, 500), (1, 64), (3, 2)], 12, 2, 128, 32, BF16, 0, 0),  # drafted tokens
     ([(2, 700), (6, 333), (5, 90)], 4, 1, 64, 16, F16, 70, 3),
     ([(3, 700), (2, 333)], 14, 1, 128, 64, F16, 0, 0),
+    ([(300, 500)] + [(0, 10)] * 15 + [(90, 90)], 12, 2, 128, 32, BF16, 0, 0),  # few tokens a slot: chunks converted for each tile
+    ([(300, 500)] + [(0, 10)] * 15, 12, 2, 128, 64, F16, 130, 9),
+    ([(200, 333)] + [(0, 0)] * 9, 6, 2, 64, 16, F16, 0, 0),
+    ([(1, 700), (6, 90), (7, 90), (50, 400), (1, 0), (1, 1), (3, 333), (2, 2)], 12, 2, 128, 16, F16, 0, 0),  # decode beside prompts
+    ([(1, 700), (6, 90), (7, 90), (500, 600), (1, 0), (1, 1), (3, 333), (2, 2)], 12, 2, 128, 16, BF16, 100, 3),
+    ([(1, 257), (30, 100), (50, 60), (48, 300), (49, 300)], 2, 2, 64, 256, BF16, 0, 0),
+    ([(4, 4)], 16, 2, 128, 16, F16, 0, 0),
+    ([(9, 7)], 4, 2, 64, 16, BF16, 3, 0),
 ]
 
 
@@ -516,23 +524,32 @@ def test_scale_of_any_sign(sizes, prefix, window, sinks, scale, dtype, hd):
     assert_within(got, exact, tol)
 
 
+def _without_prefix(c, q):
+    """Case.attention of c's sequences with the queries q, as if there were no prefix."""
+    kept = c.q, c.prefix
+    c.q, c.prefix = q, 0
+    got = c.attention()
+    c.q, c.prefix = kept
+    return got
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("before,after,hd", [(0, 700, 128), (2, 0, 64), (3, 5, 128)])
-def test_attention_rows_outside_starts(before, after, hd):
+@pytest.mark.parametrize("sizes", [[(3, 20), (150, 200), (1, 0)], [(3, 20), (2, 200), (1, 0)]])
+def test_attention_rows_outside_starts(before, after, hd, sizes):
     """Rows before starts[0] and from starts[B] on belong to no sequence: zero from attention over the pages, the prefix alone
     from attention with a prefix."""
-    c = Fp4Case([(3, 20), (150, 200), (1, 0)], hd=hd, one_token=False, prefix=40)
+    c = Fp4Case(sizes, hd=hd, one_token=False, prefix=40)
     own, live = c.q, slice(before, before + c.T)
     c.q = torch.cat([torch.randn(before, c.nq, hd), torch.zeros(c.T, c.nq, hd), torch.randn(after, c.nq, hd)]).to(c.dtype).cuda()
     c.q[live] = own
     outside = torch.ones(len(c.q), dtype=torch.bool)
     outside[live] = False
-    plain = Fp4Case([(3, 20), (150, 200), (1, 0)], hd=hd, one_token=False, prefix=40)
-    want = _attend(plain)
+    exact, tol = _without_prefix(c, own)
     c.starts = c.starts + before
     out = torch.full_like(c.q, math.nan)
     _attend(c, out=out)
-    assert torch.equal(out[live], want)
+    assert_within(out[live], exact, tol)
     assert not out[outside.cuda()].any()
     out = torch.full_like(c.q, math.nan)
     _attend_prefix(c, out=out)

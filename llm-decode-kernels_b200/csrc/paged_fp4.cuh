@@ -40,47 +40,49 @@ __device__ __forceinline__ float fp4_scale(uint8_t w) {
   return __low2float(*reinterpret_cast<const __half2*>(&d));
 }
 
-// max that keeps a NaN
+// max and min that keep a NaN
 __device__ __forceinline__ float max_nan(float a, float b) {
   float d;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float d;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
   return d;
 }
 
 // Quantises the 8 values of this lane, whose 16-dim group the lane's neighbour (lane ^ 1) has the other half of: the codes as 4
 // bytes, and the group's scale. The values come from a 16-bit type; inv_power is a power of two.
 //   scale = E4M3(max |x| / 6),  code = E2M1(x / scale), both to nearest, ties to even; infinities saturate, a NaN makes the scale NaN
-// The division by the scale is a product with its reciprocal, off by 2^-23 of the ratio. A ratio either is a border between two
-// codes, which has at most 3 bits, or is 2^-13 away from it at least: x has 11 bits, border * scale 7, so their difference is
-// a unit of x's last place or more, and the smallest border is 1/4. So the ratio is first rounded to a multiple of 2^-16
-// (adding and taking away 192, whose neighbours are 2^-16 apart), which puts exact borders back in their places.
+// Both divisions are products with a reciprocal, off by less than 2^-21 of the ratio, which is then rounded to a grid that has the
+// borders between the results on it and is far finer than the distance of any other ratio from a border:
+// * max / 6 to 16 bits (t 257 - (t 257 - t)). A border between two scales has 5 bits and 6 times it 7, the maximum 11: where they
+//   differ, it is by the maximum's last place, 2^-11 of it, or more;
+// * x / scale to multiples of 2^-16 (adding and taking away 192, whose neighbours are 2^-16 apart). A border has at most 3 bits and
+//   border * scale 7, x 11: where they differ, the ratio is 2^-13 away from the border or more, the smallest border being 1/4.
 __device__ __forceinline__ uint32_t fp4_quantise8(const float (&x)[8], float inv_power, int lane, uint8_t& scale) {
-  float y[8], m = 0.f;
+  float m = fabsf(x[0]);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    y[i] = x[i] * inv_power;
-    m = max_nan(m, fabsf(y[i]));
-  }
+  for (int i = 1; i < 8; ++i) m = max_nan(m, fabsf(x[i]));
   m = max_nan(m, __shfl_xor_sync(3u << (lane & 30), m, 1));  // (the two lanes of a group are always in the same branch)
+  const float t = min_nan(m * inv_power * (1.f / 6.f), 512.f), c = __fmul_rn(t, 257.f);
   uint16_t bits;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(bits) : "f"(0.f), "f"(__fdiv_rn(m, 6.f)));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(bits) : "f"(0.f), "f"(__fsub_rn(c, __fsub_rn(c, t))));
   scale = static_cast<uint8_t>(bits);
-  const float s = fp4_scale(scale), r = s == 0.f ? 0.f : __frcp_rn(s);
-  uint32_t code = 0;
+  const float s = fp4_scale(scale);
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
+  r = s == 0.f ? 0.f : r * inv_power;
+  float a[8];
 #pragma unroll
-  for (int i = 0; i < 8; i += 2) {
-    float a[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const float t = fabsf(y[i + j]) * r;
-      a[j] = copysignf(__fsub_rn(__fadd_rn(t, 192.f), 192.f), x[i + j]);
-    }
-    uint32_t byte;
-    asm("{\n.reg .b8 a, z;\nmov.b16 {z, _}, 0;\ncvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\nmov.b32 %0, {a, z, z, z};\n}"
-        : "=r"(byte)
-        : "f"(a[0]), "f"(a[1]));
-    code |= byte << (4 * i);
-  }
+  for (int i = 0; i < 8; ++i) a[i] = copysignf(__fsub_rn(__fadd_rn(fabsf(x[i] * r), 192.f), 192.f), x[i]);
+  uint32_t code;
+  asm("{\n.reg .b8 a, b, c, e;\n"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\ncvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\ncvt.rn.satfinite.e2m1x2.f32 e, %8, %7;\nmov.b32 %0, {a, b, c, e};\n}"
+      : "=r"(code)
+      : "f"(a[0]), "f"(a[1]), "f"(a[2]), "f"(a[3]), "f"(a[4]), "f"(a[5]), "f"(a[6]), "f"(a[7]));
   return code;
 }
 

@@ -3,16 +3,18 @@
 The prompt runs once, in one call per layer of `paged_append` and `paged_attention`, into pages that all samples share.
 Each step then appends every sample's token to pages of its own and attends with `shared_prefix_attention`, which reads
 the prompt's keys and values once for all samples, or with a window with `paged_attention` (window, sinks) over page
-tables that list the shared pages first. `token_logprobs` scores the picked tokens. The projections are the runner's
+tables that list the shared pages first. With a cache held in 4 bits the same runs on the ops of `kernels.paged_fp4`, from
+the same projections. `token_logprobs` scores the picked tokens. The projections are the runner's
 backend (kernels.e2e.model). The reference decodes one sequence, or a batch with a cache each
 (kernels/e2e/model.py:192, 216-253); it has no counterpart of this.
 
-    python -m kernels.e2e.sample --layers 4 --samples 16 --prompt 2048 --steps 32
+    python -m kernels.e2e.sample --layers 4 --samples 16 --prompt 2048 --steps 32 [--cache fp4]
 """
 
 from __future__ import annotations
 
 import argparse
+import functools
 import time
 
 import torch
@@ -20,25 +22,36 @@ import torch.nn.functional as F
 
 from kernels.logprobs import token_logprobs
 from kernels.paged import paged_append, paged_attention, shared_prefix_attention
+from kernels.paged_fp4 import fp4_pages, paged_append_fp4, paged_attention_fp4, shared_prefix_attention_fp4
 
 
 class PagedSampler:
     """`samples` continuations of a prompt of up to max_prompt tokens, each of up to max_new tokens, by a QwenRunner's
     weights (fp16 or bf16, head_dim 64 or 128, one GPU). window > 0 limits attention to the last `window` positions and
-    the first `sinks`."""
+    the first `sinks`. cache: "16" in the weights' type, "fp4" in 4 bits, with the powers of two k_scale and v_scale of
+    kernels.paged_fp4."""
 
     def __init__(self, runner, samples: int, max_prompt: int, max_new: int, page_size: int = 64, window: int = 0,
-                 sinks: int = 0):
+                 sinks: int = 0, cache: str = "16", k_scale: float = 1.0, v_scale: float = 1.0):
         if runner.tp is not None:
             raise ValueError("PagedSampler: one GPU (the runner is tensor parallel)")
+        if cache not in ("16", "fp4"):
+            raise ValueError(f"PagedSampler: a cache of {cache} (16 or fp4)")
         self.r, self.n, self.page, self.window, self.sinks = runner, samples, page_size, window, sinks
         self.max_prompt, self.max_new = max_prompt, max_new
         dev = runner.embed.device
         shared = -(-max_prompt // page_size)
         own = -(-max_new // page_size) + 1  # one more: with a window the prompt's last, partly filled page is copied
         pages = shared + samples * own
-        shape = (len(runner.layers), pages, runner.n_kv, page_size, runner.head_dim)
-        self.k = torch.empty(shape, dtype=runner.embed.dtype, device=dev)
+        if cache == "fp4":
+            self.k = fp4_pages(len(runner.layers) * pages, runner.n_kv, page_size, runner.head_dim, dev).unflatten(0, (-1, pages))
+            scales = {"k_scale": k_scale, "v_scale": v_scale}
+            ops = paged_append_fp4, paged_attention_fp4, shared_prefix_attention_fp4
+            self.append, self.attention, self.behind_prefix = (functools.partial(op, **scales) for op in ops)
+        else:
+            shape = (len(runner.layers), pages, runner.n_kv, page_size, runner.head_dim)
+            self.k = torch.empty(shape, dtype=runner.embed.dtype, device=dev)
+            self.append, self.attention, self.behind_prefix = paged_append, paged_attention, shared_prefix_attention
         self.v = torch.empty_like(self.k)
         self.prompt_table = torch.arange(shared, dtype=torch.int32, device=dev)
         self.own_table = torch.arange(shared, pages, dtype=torch.int32, device=dev).view(samples, own)
@@ -75,9 +88,9 @@ class PagedSampler:
         length, table = starts[1:], self.prompt_table[None]
 
         def attend(i, qkv):
-            q = paged_append(qkv, self.k[i], self.v[i], table, length, self.cos, self.sin, r.n_heads, r.n_kv, starts=starts)
-            return paged_attention(q, self.k[i], self.v[i], table, length, starts=starts, window=self.window,
-                                   sinks=self.sinks).view(P, -1)
+            q = self.append(qkv, self.k[i], self.v[i], table, length, self.cos, self.sin, r.n_heads, r.n_kv, starts=starts)
+            return self.attention(q, self.k[i], self.v[i], table, length, starts=starts, window=self.window,
+                                  sinks=self.sinks).view(P, -1)
 
         h = self._layers(F.embedding(ids, r.embed), attend)
         self.prompt, self.left = P, self.max_new
@@ -105,11 +118,11 @@ class PagedSampler:
 
         def attend(i, qkv):
             k, v = self.k[i], self.v[i]
-            q = paged_append(qkv, k, v, self.table, self.lengths, self.cos, self.sin, r.n_heads, r.n_kv, offset=offset)
+            q = self.append(qkv, k, v, self.table, self.lengths, self.cos, self.sin, r.n_heads, r.n_kv, offset=offset)
             if self.window > 0:
-                out = paged_attention(q, k, v, self.table, self.lengths, window=self.window, sinks=self.sinks)
+                out = self.attention(q, k, v, self.table, self.lengths, window=self.window, sinks=self.sinks)
             else:
-                out = shared_prefix_attention(q, k, v, self.prompt_table, self.prompt, self.table, self.lengths)
+                out = self.behind_prefix(q, k, v, self.prompt_table, self.prompt, self.table, self.lengths)
             return out.view(self.n, -1)
 
         return self._logits(self._layers(F.embedding(tokens, r.embed), attend))
@@ -144,10 +157,11 @@ def main():
     ap.add_argument("--window", type=int, default=0)
     ap.add_argument("--sinks", type=int, default=4)
     ap.add_argument("--backend", default="ours")
+    ap.add_argument("--cache", default="16", choices=("16", "fp4"))
     a = ap.parse_args()
     model = random_qwen2({**config.QWEN15, "num_hidden_layers": a.layers})
     runner = QwenRunner(model, make_backend(a.backend), max_len=64)
-    sampler = PagedSampler(runner, a.samples, a.prompt, a.steps, window=a.window, sinks=a.sinks)
+    sampler = PagedSampler(runner, a.samples, a.prompt, a.steps, window=a.window, sinks=a.sinks, cache=a.cache)
     g = torch.Generator(device="cuda").manual_seed(0)
     ids = torch.randint(0, config.QWEN15["vocab_size"], (a.prompt,), generator=g, device="cuda")
 

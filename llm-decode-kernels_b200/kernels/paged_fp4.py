@@ -14,6 +14,7 @@ results are fp16 or bf16. The reference's cache is fp16 (kernels/e2e/model.py:19
 
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -29,11 +30,12 @@ def fp4_pages(n_pages: int, n_kv: int, page_size: int, head_dim: int, device=Non
     return torch.empty(n_pages, n_kv, page_size, head_dim * 9 // 16, dtype=torch.uint8, device=device)
 
 
-def _powers(what, k_scale, v_scale):
+@functools.lru_cache(maxsize=256)  # (of numbers only: a model has a pair of them)
+def _powers(what, k_scale: float, v_scale: float):
     for x in (k_scale, v_scale):
-        if x != 1.0 and not (2.0 ** -64 <= x <= 2.0 ** 64 and math.frexp(x)[0] == 0.5):
-            _refuse(what, "k_scale and v_scale must be powers of two from 2^-64 to 2^64")
-    return k_scale, v_scale
+        if not (isinstance(x, (int, float)) and 2.0 ** -64 <= x <= 2.0 ** 64 and math.frexp(x)[0] == 0.5):
+            _refuse(what, "k_scale and v_scale must be numbers, powers of two from 2^-64 to 2^64")
+    return float(k_scale), float(v_scale)
 
 
 def paged_append_fp4(qkv, k_pages, v_pages, page_table, lengths, cos, sin, n_heads, n_kv, starts=None, offset=0, k_scale=1.0,

@@ -797,6 +797,7 @@ def test_refusals_without_a_gpu():
     for bad in (0.0, -1.0, 3.0, 1.5, math.inf, math.nan, 2.0 ** 65, 2.0 ** -65):
         attend(ValueError, k_scale=bad)
         attend(ValueError, v_scale=bad)
+    attend(ValueError, k_scale=torch.ones(()))  # a number, not a tensor whose value may change
     for k in (1, 2.0 ** -64, 2.0 ** 64):
         attend(RuntimeError, k_scale=k)  # as far as the device
     for table, n in ((c.table[0], 1000), (c.table[0], -1)):

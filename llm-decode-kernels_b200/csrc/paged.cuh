@@ -371,8 +371,8 @@ struct RowsShape {
   size_t smem;
   int ctas;
 };
-// Such a launch over a cache held in 4 bits (paged_attention_fp4.cu), with tiles of 8 or 16 rows; kFp4Groups pieces of the line a CTA.
-constexpr int kFp4Groups = 2;
+// Such a launch over a cache held in 4 bits (paged_attention_fp4.cu), with tiles of 8 or 16 rows; fp4_groups pieces of the line a CTA.
+constexpr int fp4_groups(int rows) { return rows == 8 ? 3 : 2; }
 constexpr int kFp4Chunk = 128;
 RowsShape fp4_rows_shape(int64_t hd, int dtype, int rows, bool ragged);
 cudaError_t fp4_rows_launch(const Problem& p, int64_t hd, int dtype, int rows, bool ragged, const RowsShape& s, int wait_late,

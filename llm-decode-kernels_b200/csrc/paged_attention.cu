@@ -688,7 +688,7 @@ void cut_pass(const Sizes& z, Cutter& c, Pass& a, bool always_partial) {
   } else {
     a.rows = z.nq / z.nkv <= 8 && !z.ragged ? 8 : 16;
     a.shape = rows_shape_of(z, a.rows);
-    a.groups = z.fp4 ? kFp4Groups : kGroups;
+    a.groups = z.fp4 ? fp4_groups(a.rows) : kGroups;
     a.ctas = a.shape.ctas * a.groups;
     p.unit_extra = z.fp4 ? kFp4UnitExtra : kRowsUnitExtra;
   }

@@ -35,10 +35,15 @@ constexpr int kCWarps = 4;  // warps of a group
 constexpr int kSub = 2;     // 16-position tiles of a warp in a chunk
 constexpr int kChunk = kFp4Chunk;
 static_assert(kChunk == kCWarps * kSub * 16, "a chunk is one round of the warps");
-constexpr int kThreads = kFp4Groups * (kCWarps + 1) * 32;
-// Slots of a group's ring: what fits the shared memory of two CTAs an SM (one with 16 rows).
+// Groups of a CTA, one CTA an SM, each with a piece of the line and a producer warp of its own. What counts is the registers of a
+// thread: with 8 rows 3 groups have 128 and keep a chunk's operands in them; 4 groups have 96 (64 x 8192: 59 us against 52).
+template <int kBlocks>
+constexpr int kGroups = fp4_groups(8 * kBlocks);
+template <int kBlocks>
+constexpr int kThreads = kGroups<kBlocks> * (kCWarps + 1) * 32;
+// Slots of a group's ring: what fits beside the warps' results.
 template <int kHd, int kBlocks>
-constexpr int kRing = kHd == 64 ? (kBlocks == 1 ? 4 : 5) : (kBlocks == 1 ? 2 : 3);
+constexpr int kRing = (kHd == 64 ? 2 : 1) * 3;
 constexpr float kRefBelow = 6.f, kRefReach = 14.f;
 
 // A chunk in shared memory: for k and v each the codes of kChunk positions, then their scales.
@@ -67,30 +72,31 @@ __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((12
 
 // kRagged: tiles of the plan, a few tokens each; otherwise tile b is the one token of sequence b.
 template <typename T, int kHd, int kBlocks, bool kRaggedTiles>
-__global__ void __launch_bounds__(kThreads, kBlocks == 1 ? 2 : 1) fp4_rows_kernel(const Problem p, int wait_late) {
+__global__ void __launch_bounds__(kThreads<kBlocks>, 1) fp4_rows_kernel(const Problem p, int wait_late) {
   constexpr int ring = kRing<kHd, kBlocks>;
   using F = Fp4<kHd>;
   using S = Slot<kHd>;
+  constexpr int kG = kGroups<kBlocks>, kT = kThreads<kBlocks>;
   constexpr int kRows = 8 * kBlocks;      // query rows: the product's columns
   constexpr int kSteps = kHd / 16;        // products of a tile of k, and tiles of v's product
   constexpr int kWords = kHd / 32;        // words of a lane's codes of k; v's has kHd / 64
   constexpr uint32_t kLow = 0x0f0f0f0fu;
-  __shared__ float2 pre_ml_sh[kFp4Groups][kRows * kCWarps];
-  __shared__ __align__(8) uint64_t full_sh[kFp4Groups][ring], empty_sh[kFp4Groups][ring];
-  __shared__ int warp_sum[kThreads / 32 + 1];
+  __shared__ float2 pre_ml_sh[kG][kRows * kCWarps];
+  __shared__ __align__(8) uint64_t full_sh[kG][ring], empty_sh[kG][ring];
+  __shared__ int warp_sum[kT / 32 + 1];
   extern __shared__ __align__(128) uint8_t base[];
   int* cum_sh = reinterpret_cast<int*>(base);  // [B + 1], before the first copies land there
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const bool producer = warp >= kFp4Groups * kCWarps;
-  const int group = producer ? warp - kFp4Groups * kCWarps : warp / kCWarps;
-  const int cta = blockIdx.x * kFp4Groups + group, ctas = gridDim.x * kFp4Groups;  // pieces of the line: one a group
+  const bool producer = warp >= kG * kCWarps;
+  const int group = producer ? warp - kG * kCWarps : warp / kCWarps;
+  const int cta = blockIdx.x * kG + group, ctas = gridDim.x * kG;  // pieces of the line: one a group
   uint8_t* slots = base + group * ring * S::kBytes;
-  float* pre_o = reinterpret_cast<float*>(base + kFp4Groups * ring * S::kBytes) + group * kCWarps * kRows * kHd;
+  float* pre_o = reinterpret_cast<float*>(base + kG * ring * S::kBytes) + group * kCWarps * kRows * kHd;
   float2* pre_ml = pre_ml_sh[group];
   uint64_t *full = full_sh[group], *empty = empty_sh[group];
   if (tid == 0) {
-    for (int i = 0; i < kFp4Groups * ring; ++i) {
+    for (int i = 0; i < kG * ring; ++i) {
       mbar_init(&full_sh[0][i], 1);
       mbar_init(&empty_sh[0][i], kCWarps);
     }
@@ -104,7 +110,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks == 1 ? 2 : 1) fp4_rows_kerne
     line = line_of(p, kChunk);
   } else {  // every CTA sums up the sequences' chunks for itself
     int carry = 0;
-    for (int b0 = 0; b0 < p.B; b0 += kThreads) {
+    for (int b0 = 0; b0 < p.B; b0 += kT) {
       const int b = b0 + tid;
       int n = 0;
       if (b < p.B) {
@@ -121,7 +127,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks == 1 ? 2 : 1) fp4_rows_kerne
       if (lane == 31) warp_sum[warp] = s;
       __syncthreads();
       int before = carry;
-      for (int w = 0; w < kThreads / 32; ++w) {
+      for (int w = 0; w < kT / 32; ++w) {
         const int ws = warp_sum[w];
         if (w < warp) before += ws;
         carry += ws;
@@ -132,7 +138,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks == 1 ? 2 : 1) fp4_rows_kerne
     line.chunks = carry;
     __syncthreads();
     if (blockIdx.x == 0)  // for the join kernel
-      for (int i = tid; i <= p.B; i += kThreads) p.cum_out[i] = cum_sh[i];
+      for (int i = tid; i <= p.B; i += kT) p.cum_out[i] = cum_sh[i];
   }
   __syncthreads();
 
@@ -422,7 +428,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks == 1 ? 2 : 1) fp4_rows_kerne
         ok = __all_sync(0xffffffffu, ok);
         if (ok) {
           const bool clear = i >= clear_from && i < clear_to;
-                    if (clear || span.needs(i * kChunk + 16 * kSub * sub, 16 * kSub, p.mask)) tiles(i, clear);
+          if (clear || span.needs(i * kChunk + 16 * kSub * sub, 16 * kSub, p.mask)) tiles(i, clear);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[s]);
@@ -503,8 +509,8 @@ RowsShape shape() {
   static int per_sm[64];  // by device; 0: not asked yet
   RowsShape s;
   s.ring = kRing<kHd, kBlocks>;
-  s.smem = static_cast<size_t>(kFp4Groups) * (s.ring * Slot<kHd>::kBytes + kCWarps * 8 * kBlocks * kHd * 4);
-  static_assert((kMaxBatch + 1) * 4 <= kFp4Groups * kRing<kHd, kBlocks> * Slot<kHd>::kBytes,
+  s.smem = static_cast<size_t>(kGroups<kBlocks>) * (s.ring * Slot<kHd>::kBytes + kCWarps * 8 * kBlocks * kHd * 4);
+  static_assert((kMaxBatch + 1) * 4 <= kGroups<kBlocks> * kRing<kHd, kBlocks> * Slot<kHd>::kBytes,
                 "the chunk sums fit the ring");
   int dev = 0;
   cudaGetDevice(&dev);
@@ -513,7 +519,7 @@ RowsShape shape() {
   if (n == 0) {
     auto k = fp4_rows_kernel<T, kHd, kBlocks, kRaggedTiles>;
     if (opt_in_dynamic_smem(k) < static_cast<int>(s.smem) ||
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k, kThreads, s.smem) != cudaSuccess) {
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k, kThreads<kBlocks>, s.smem) != cudaSuccess) {
       cudaGetLastError();
       n = 0;
     }
@@ -539,7 +545,7 @@ RowsShape fp4_rows_shape(int64_t hd, int dtype, int rows, bool ragged) {
 cudaError_t fp4_rows_launch(const Problem& p, int64_t hd, int dtype, int rows, bool ragged, const RowsShape& s, int wait_late,
                             cudaStream_t st) {
 #define DK_ROWS(TT, HH, NB, RR) \
-  launch(fp4_rows_kernel<TT, HH, NB, RR>, dim3(s.ctas), dim3(kThreads), s.smem, st, pdl_enabled(), dim3(1, 1, 1), p, wait_late)
+  launch(fp4_rows_kernel<TT, HH, NB, RR>, dim3(s.ctas), dim3(kThreads<NB>), s.smem, st, pdl_enabled(), dim3(1, 1, 1), p, wait_late)
   return DK_BY_TYPE(DK_ROWS);
 #undef DK_ROWS
 }

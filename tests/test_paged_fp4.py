@@ -207,6 +207,10 @@ def test_append_and_read_rows_outside_starts(before, after):
     ([(70, 70), (0, 5), (33, 100)], 1, 64, 32, F16, 1.0, 2.0 ** -6),
     ([(300, 300), (5, 3), (4, 0)], 8, 64, 256, BF16, 2.0 ** 40, 2.0 ** -40),
     ([(513, 513)], 3, 128, 128, F16, 0.5, 1.0),
+    ([(333, 400), (1, 20)], 5, 128, 16, BF16, 1.0, 1.0),  # columns that do not fill the warps of a block,
+    ([(700, 700), (2, 9)], 20, 128, 64, F16, 1.0, 0.5),  # more of them than warps
+    ([(19500, 19500), (3, 1)], 1, 64, 256, BF16, 1.0, 1.0),  # whole batches of rows
+    ([(5000, 5003), (1, 4)], 2, 128, 32, F16, 2.0, 1.0),
 ])
 def test_read(sizes, nkv, hd, page, dtype, k_scale, v_scale):
     """Exactly what the codes stand for; rows before a sequence's first position are zero."""

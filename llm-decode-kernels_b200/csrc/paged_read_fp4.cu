@@ -109,8 +109,8 @@ __global__ void __launch_bounds__(kWarps * 32) paged_read_fp4_kernel(const ReadP
 }
 
 // Pages in 16 bits of what a call's rows see, for the 256-row tiles (paged_attention_tc.cu): a page of the copy for each entry of
-// the page tables, and tables that list them. A warp takes 16 positions of a sequence, all heads; the powers are left out (the scores'
-// scale and the output's have them).
+// the page tables, and tables that list them. A warp takes 16 positions of a head's k or v; the powers are left out (the scores' scale
+// and the output's have them).
 struct CopyParams {
   const uint8_t* pool[2];
   void* out[2];  // [B * width, nkv, page_size, kHd]
@@ -131,10 +131,11 @@ __global__ void __launch_bounds__(kWarps * 32) fp4_copy_kernel(const CopyParams 
   constexpr int kPieces = 16 * kHd / 8;  // of 8 dims of 16 positions of a head
   pdl_trigger();
   pdl_wait();
-  const int lane = threadIdx.x & 31, per_seq = p.width << (p.page_shift - 4);
-  const int64_t units = static_cast<int64_t>(p.B) * per_seq;
+  const int lane = threadIdx.x & 31, per_seq = p.width << (p.page_shift - 4), heads = 2 * p.nkv;
+  const int64_t units = static_cast<int64_t>(p.B) * per_seq * heads;
   for (int64_t u = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5); u < units; u += static_cast<int64_t>(gridDim.x) * kWarps) {
-    const int b = static_cast<int>(u / per_seq), j0 = static_cast<int>(u - static_cast<int64_t>(b) * per_seq) * 16;
+    const int64_t group = u / heads;
+    const int b = static_cast<int>(group / per_seq), j0 = static_cast<int>(group - static_cast<int64_t>(b) * per_seq) * 16;
     // seen: below the length, and from the first row's window on or below the sinks
     const int t0 = min(max(p.starts[b], 0), p.T), rows = min(max(p.starts[b + 1], t0), p.T) - t0;
     const int length = length_of(p.lengths, b);
@@ -143,41 +144,38 @@ __global__ void __launch_bounds__(kWarps * 32) fp4_copy_kernel(const CopyParams 
     const int at = j0 >> p.page_shift, page = p.table[b * p.ld_table + at];
     const int64_t to = static_cast<int64_t>(b) * p.width + at;
     const bool there = page >= 0 && page < p.n_pages;
-    if (lane == 0) {
+    const int head = static_cast<int>(u - group * heads), which = head >= p.nkv, h = head - which * p.nkv;
+    if (lane == 0 && head == 0) {
       p.table_out[to] = static_cast<int32_t>(to);
       if (!there) record_device_error(p.err, DK_DEVERR_BAD_POSITION);  // (zeros)
     }
     const int slot = j0 & (p.page_size - 1);
-    for (int h = 0; h < p.nkv; ++h)
+    const uint8_t* block = (which ? p.pool[1] : p.pool[0]) + (static_cast<int64_t>(there ? page : 0) * p.nkv + h) * p.page_size * F::kRow;
+    const uint32_t* codes = reinterpret_cast<const uint32_t*>(block + slot * F::kCodes) + lane;
+    const uint8_t* scales = block + p.page_size * F::kCodes + slot * F::kScales + lane / 2;
+    uint32_t code[kPieces / 32];
+    uint8_t scale[kPieces / 32];
 #pragma unroll
-      for (int which = 0; which < 2; ++which) {
-        const uint8_t* block = p.pool[which] + (static_cast<int64_t>(there ? page : 0) * p.nkv + h) * p.page_size * F::kRow;
-        const uint32_t* codes = reinterpret_cast<const uint32_t*>(block + slot * F::kCodes) + lane;
-        const uint8_t* scales = block + p.page_size * F::kCodes + slot * F::kScales + lane / 2;
-        uint32_t code[kPieces / 32];
-        uint8_t scale[kPieces / 32];
+    for (int i = 0; i < kPieces / 32; ++i) {
+      code[i] = there ? codes[32 * i] : 0;
+      scale[i] = there ? scales[16 * i] : 0;
+    }
+    uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(which ? p.out[1] : p.out[0]) + ((to * p.nkv + h) * p.page_size + slot) * kHd) + lane;
 #pragma unroll
-        for (int i = 0; i < kPieces / 32; ++i) {
-          code[i] = there ? codes[32 * i] : 0;
-          scale[i] = there ? scales[16 * i] : 0;
-        }
-        uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(p.out[which]) + ((to * p.nkv + h) * p.page_size + slot) * kHd) + lane;
+    for (int i = 0; i < kPieces / 32; ++i) {
+      uint32_t x[4], one = fp4_scales(scale[i]);
+      fp4_codes(code[i], x);
+      one = prmt(one, one, 0x1010);
 #pragma unroll
-        for (int i = 0; i < kPieces / 32; ++i) {
-          uint32_t x[4], one = fp4_scales(scale[i]);
-          fp4_codes(code[i], x);
-          one = prmt(one, one, 0x1010);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            x[k] = hmul2_rn(x[k], one);
-            if constexpr (!std::is_same<T, __half>::value) {
-              const float2 f = Elem<__half>::unpack(x[k]);
-              x[k] = Elem<T>::pack(f.x, f.y);
-            }
-          }
-          out[32 * i] = make_uint4(x[0], x[1], x[2], x[3]);
+      for (int k = 0; k < 4; ++k) {
+        x[k] = hmul2_rn(x[k], one);
+        if constexpr (!std::is_same<T, __half>::value) {
+          const float2 f = Elem<__half>::unpack(x[k]);
+          x[k] = Elem<T>::pack(f.x, f.y);
         }
       }
+      out[32 * i] = make_uint4(x[0], x[1], x[2], x[3]);
+    }
   }
 }
 
@@ -191,7 +189,7 @@ cudaError_t fp4_copy_launch(const Problem& p, int64_t hd, int dtype, void* k, vo
   c.table = p.table, c.ld_table = p.ld_table, c.lengths = p.lengths, c.starts = p.starts;
   c.T = p.T, c.B = p.B, c.nkv = p.nkv, c.n_pages = p.n_pages, c.page_size = p.page_size, c.page_shift = p.page_shift;
   c.above = p.above, c.width = p.capacity >> p.page_shift, c.mask = p.mask, c.err = p.err;
-  const int64_t units = static_cast<int64_t>(p.B) * (p.capacity / 16);
+  const int64_t units = static_cast<int64_t>(p.B) * (p.capacity / 16) * 2 * p.nkv;
   const dim3 grid(static_cast<unsigned>(std::min<int64_t>((units + kWarps - 1) / kWarps, 8ll * device_info().num_sms)));
 #define DK_COPY(TT) \
   launch(hd == 128 ? fp4_copy_kernel<TT, 128> : fp4_copy_kernel<TT, 64>, grid, dim3(kWarps * 32), 0, st, pdl_enabled(), dim3(1, 1, 1), c)

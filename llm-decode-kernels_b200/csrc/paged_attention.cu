@@ -613,9 +613,11 @@ struct Sizes {
 };
 
 // A ragged call over a 4-bit cache: sequences of few tokens (drafted ones to check, decode steps beside prompts) go to the rows kernel,
-// in tiles of up to 16 rows that each read the sequence again, up to kFewTiles of them; longer ones to the 256-row tiles. Which
-// there are only the device knows. A call whose sequences have kManyTokens on average is taken for prompts: then the tiles take
-// all of them. TODO figures
+// in tiles of up to 16 rows that each read the sequence again, up to kFewTiles of them; longer ones to the 256-row tiles (32 sequences
+// of 4096, 28 heads over 4, tiles of 2 tokens, us on the rows kernel and as 256-row tiles: 2 tokens 31, 61; 4 39, 62; 6 53,
+// 62; 8 62, 63; 12 93, 57. 16 of 4096, 8 over 8, tiles of 16: 32 44, 60; 64 69, 61). Which there are only the device
+// knows, and a launch without any takes 5 us with its join. A call whose sequences have kManyTokens on average is taken for
+// prompts: then the tiles take all of them.
 constexpr int kFewTiles = 3, kManyTokens = 256;
 struct Split {
   bool few, many;  // which kernels are launched
@@ -629,10 +631,13 @@ Split split_of(const Sizes& z) {
 }
 
 // Prompts over a 4-bit cache first have the pages that they see copied in 16 bits, which the tiles then read, instead of converting
-// each chunk for every tile anew. TODO figures
-constexpr int64_t kCopyTokens = 32, kCopyBytes = int64_t(1) << 30;
+// each chunk for every tile anew: from kCopyTiles tiles a sequence on (positions, tokens each; us without and with a copy): 32
+// sequences of 4096, 28 heads over 4, tiles of 36 tokens: 64 115, 126; 128 195, 175; 256 316, 252. 2 of 8192, 12 over 2, 42:
+// 64 29, 30; 128 39, 38; 256 50, 44. 16 of 4096, 8 over 8, 256: 256 79, 103. The copy takes at most 1 GB of the workspace.
+constexpr int64_t kCopyTiles = 3, kCopyBytes = int64_t(1) << 30;
 bool copies(const Sizes& z) {
-  return z.fp4 && z.ragged && z.prefix_len == 0 && split_of(z).many && z.T >= kCopyTokens * z.B && z.T > 0 &&
+  const int64_t tile = 2 * (128 / (z.nq / z.nkv));
+  return z.fp4 && z.ragged && z.prefix_len == 0 && split_of(z).many && z.T > 0 && z.T >= kCopyTiles * tile * z.B &&
          z.positions <= kCopyBytes / (4 * z.hd) / z.nkv / z.B;
 }
 

@@ -320,6 +320,10 @@ RAGGED = [
     ([(1, 700), (6, 90), (7, 90), (500, 600), (1, 0), (1, 1), (3, 333), (2, 2)], 12, 2, 128, 16, BF16, 100, 3),
     ([(1, 257), (30, 100), (50, 60), (48, 300), (49, 300)], 2, 2, 64, 256, BF16, 0, 0),
     ([(4, 4)], 16, 2, 128, 16, F16, 0, 0),
+    ([(200, 260), (4, 77), (180, 180), (150, 400)], 12, 2, 128, 16, BF16, 0, 0),  # prompts of several tiles: copied first
+    ([(200, 260), (4, 77), (180, 180), (150, 400)], 28, 4, 64, 64, F16, 60, 5),
+    ([(250, 300)], 16, 1, 128, 256, F16, 0, 0),
+    ([(130, 500), (1, 0), (1, 9)], 14, 1, 128, 32, F16, 25, 17),
     ([(9, 7)], 4, 2, 64, 16, BF16, 3, 0),
 ]
 

@@ -43,7 +43,8 @@ _FP4_ROWS = {72: 128, 36: 64}  # head_dim by the bytes of a position in a cache 
 
 
 def _cache_shape(what, k_pages, v_pages, page_table, lengths, starts, tokens, fp4=False):
-    """(n_pages, n_kv, page_size, head_dim, B) of a checked cache (fp4: of 4-bit codes, kernels.paged_fp4) and batch."""
+    """(n_pages, n_kv, page_size, head_dim, B, the table's row stride, its width) of a checked cache (fp4: of 4-bit codes,
+    kernels.paged_fp4) and batch."""
     shape = k_pages.shape
     if len(shape) != 4 or v_pages.shape != shape:
         _refuse(what, f"k_pages and v_pages must be [n_pages, n_kv, page_size, {'9/16 ' if fp4 else ''}head_dim], both alike")
@@ -58,9 +59,12 @@ def _cache_shape(what, k_pages, v_pages, page_table, lengths, starts, tokens, fp
         _refuse(what, "page_size must be a power of two from 16 to 256")
     if hd != 128 and hd != 64:
         _refuse(what, "head_dim must be 64 or 128")
-    if page_table.dim() != 2 or page_table.shape[1] == 0 or page_table.stride()[1] != 1 and page_table.shape[1] > 1:
+    if page_table.dim() != 2:
         _refuse(what, "page_table must be [sequences, pages] with unit column stride")
-    B = page_table.shape[0]
+    B, table_width = page_table.shape
+    ld_table, unit = page_table.stride()
+    if table_width == 0 or unit != 1 and table_width > 1:
+        _refuse(what, "page_table must be [sequences, pages] with unit column stride")
     if lengths.shape != (B,) or not lengths.is_contiguous():
         _refuse(what, "lengths must hold one count per row of page_table")
     if starts is None:
@@ -75,7 +79,7 @@ def _cache_shape(what, k_pages, v_pages, page_table, lengths, starts, tokens, fp
             _wrong_type(what, "pages must be uint8, both of them")
     elif k_pages.dtype not in _DTYPES or v_pages.dtype is not k_pages.dtype:
         _wrong_type(what, "pages must be fp16 or bf16, both alike")
-    return n_pages, n_kv, page, hd, B
+    return n_pages, n_kv, page, hd, B, ld_table, table_width
 
 
 def paged_append(qkv, k_pages, v_pages, page_table, lengths, cos, sin, n_heads, n_kv, starts=None, offset=0, out=None):
@@ -93,7 +97,8 @@ def _append(what, qkv, k_pages, v_pages, page_table, lengths, cos, sin, n_heads,
     if qkv.dim() != 2:
         _refuse(what, "qkv must be [tokens, (n_heads + 2 n_kv) * head_dim]")
     T, width = qkv.shape
-    n_pages, kv, page, hd, B = _cache_shape(what, k_pages, v_pages, page_table, lengths, starts, T, scales is not None)
+    n_pages, kv, page, hd, B, ld_table, table_width = _cache_shape(what, k_pages, v_pages, page_table, lengths, starts, T,
+                                                                   scales is not None)
     ld, unit = qkv.stride()
     if n_kv != kv or n_heads <= 0 or width != (n_heads + 2 * n_kv) * hd or unit != 1:
         _refuse(what, "qkv must be [tokens, (n_heads + 2 n_kv) * head_dim] with the pages' kv heads and unit column stride")
@@ -122,8 +127,8 @@ def _append(what, qkv, k_pages, v_pages, page_table, lengths, cos, sin, n_heads,
     q = qkv.new_empty_strided((T, n_heads, hd), (n_heads * hd, hd, 1)) if out is None else out
     args = (
         qkv.data_ptr(), ld, k_pages.data_ptr(), v_pages.data_ptr(), n_pages, page, page_table.data_ptr(),
-        page_table.stride()[0], page_table.shape[1], lengths.data_ptr(), 0 if starts is None else starts.data_ptr(),
-        cos.data_ptr(), sin.data_ptr(), f32, ld_rope, cos.shape[0], offset, q.data_ptr(), T, B, n_heads, n_kv, hd,
+        ld_table, table_width, lengths.data_ptr(), 0 if starts is None else starts.data_ptr(), cos.data_ptr(), sin.data_ptr(),
+        f32, ld_rope, cos.shape[0], offset, q.data_ptr(), T, B, n_heads, n_kv, hd,
         _DTYPES[dtype], _raw_stream(device))
     if scales is None:
         status = _lib.lib().dk_paged_append(_lib.PAGED_APPEND_ARGS.pack(*args))
@@ -150,7 +155,8 @@ def _attend(what, entry, q, k_pages, v_pages, prefix_table, prefix_len, page_tab
     if q.dim() != 3:
         _refuse(what, "q must be [tokens, heads, head_dim]")
     T, nq, width = q.shape
-    n_pages, n_kv, page, hd, B = _cache_shape(what, k_pages, v_pages, page_table, lengths, starts, T, scales is not None)
+    n_pages, n_kv, page, hd, B, ld_table, table_width = _cache_shape(what, k_pages, v_pages, page_table, lengths, starts, T,
+                                                                     scales is not None)
     ld, by_head, unit = q.stride()
     if width != hd or unit != 1 or by_head != hd and nq > 1 or ld < nq * hd and T > 1:
         _refuse(what, "q must be [tokens, heads, head_dim], a token's heads side by side and tokens apart from each other")
@@ -177,11 +183,11 @@ def _attend(what, entry, q, k_pages, v_pages, prefix_table, prefix_len, page_tab
     code = _DTYPES[dtype]
     # the prefix's length does not change the size, only whether there is one
     nbytes = _workspace_bytes(T, B, nq, n_kv, hd, code, starts is not None, 1 if prefix_len else 0, device,
-                              0 if scales is None else page_table.shape[1] * page)
+                              0 if scales is None else table_width * page)
     ws = q.new_empty_strided(((nbytes + 1) // 2,), (1,))  # (of a 16-bit type)
     args = (
         q.data_ptr(), ld, k_pages.data_ptr(), v_pages.data_ptr(), n_pages, page, prefix_at, prefix_len,
-        page_table.data_ptr(), page_table.stride()[0], page_table.shape[1], lengths.data_ptr(),
+        page_table.data_ptr(), ld_table, table_width, lengths.data_ptr(),
         0 if starts is None else starts.data_ptr(), window, sinks, hd ** -0.5 if scale is None else scale, out.data_ptr(), T,
         B, nq, n_kv, hd, code, ws.data_ptr(), nbytes, _raw_stream(device))
     pack = _lib.PAGED_ATTENTION_ARGS.pack(*args) if scales is None else _lib.PAGED_ATTENTION_FP4_ARGS.pack(*args, *scales)

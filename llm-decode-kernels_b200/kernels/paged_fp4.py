@@ -65,7 +65,7 @@ def paged_read_fp4(k_pages, v_pages, page_table, lengths, starts=None, tokens=No
         tokens = page_table.shape[0]
     if tokens < 0:
         _refuse(what, "tokens must not be negative")
-    n_pages, n_kv, page, hd, B = _cache_shape(what, k_pages, v_pages, page_table, lengths, starts, tokens, True)
+    n_pages, n_kv, page, hd, B, ld_table, table_width = _cache_shape(what, k_pages, v_pages, page_table, lengths, starts, tokens, True)
     k_scale, v_scale = _powers(what, k_scale, v_scale)
     if dtype not in _DTYPES:
         _wrong_type(what, f"values are fp16 or bf16, not {dtype}")
@@ -73,11 +73,13 @@ def paged_read_fp4(k_pages, v_pages, page_table, lengths, starts=None, tokens=No
     if out is not None and not all(x.shape == shape and x.is_contiguous() and x.dtype is dtype for x in out):
         _refuse(what, "out must be two contiguous [tokens, n_kv, head_dim] of one type")
     device = _lib.current_device_of(what, (k_pages, v_pages, page_table, lengths, starts, *(out or ())))
-    strides = (n_kv * hd, hd, 1)
-    k, v = out if out is not None else (k_pages.new_empty_strided(shape, strides, dtype=dtype),
-                                        k_pages.new_empty_strided(shape, strides, dtype=dtype))
+    if out is None:
+        k = k_pages.new_empty_strided(shape, (n_kv * hd, hd, 1), dtype=dtype)
+        v = torch.empty_like(k)
+    else:
+        k, v = out
     status = _lib.lib().dk_paged_read_fp4(_lib.PAGED_READ_FP4_ARGS.pack(
-        k_pages.data_ptr(), v_pages.data_ptr(), n_pages, page, page_table.data_ptr(), page_table.stride()[0], page_table.shape[1],
+        k_pages.data_ptr(), v_pages.data_ptr(), n_pages, page, page_table.data_ptr(), ld_table, table_width,
         lengths.data_ptr(), 0 if starts is None else starts.data_ptr(), k_scale, v_scale, k.data_ptr(), v.data_ptr(), tokens, B,
         n_kv, hd, _DTYPES[dtype], _raw_stream(device)))
     if status:

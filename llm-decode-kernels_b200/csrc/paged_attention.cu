@@ -919,7 +919,7 @@ int attention(const char* what, const dk_paged_attention_args& a, bool prefix, b
   const Copy copy = copied ? cut_copy(z, c) : Copy{};
   for (const Pass* s : {&pre, &few, &own}) {
     if ((s == &pre && z.prefix_len == 0) || (s == &few && !has_few)) continue;
-    const int64_t chunk = s->tc ? kTcChunk : kChunk;
+    const int64_t chunk = s->tc ? kTcChunk : z.fp4 ? kFp4Chunk : kChunk;
     const int64_t tiles = s->p.mode == kRagged ? s->p.max_tiles : s->p.n_tiles;
     const int64_t positions = s->p.mode == kPrefix ? z.prefix_len : table_width * page_size;
     if (tiles * ((positions + chunk - 1) / chunk + 1 + s->p.unit_extra) * z.nkv >= (int64_t(1) << 30))

@@ -685,6 +685,57 @@ def test_windows_wholly_past_the_table_leave_the_sinks(one_token, hd, page, sink
         assert_within(out, exact, tol)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,hd", [(F16, 128), (BF16, 64)])
+@pytest.mark.parametrize("sizes", [[(1, 90), (1, 70)], [(5, 90), (4, 70)], [(150, 200), (140, 140)], [(40, 200), (35, 140)]])
+def test_a_nan_reaches_the_rows_that_see_it(sizes, dtype, hd):
+    """A NaN scale at a visible position makes the results of its kv head NaN, in its sequence only. (Every row of the first sequence
+    sees its position 3; one token each, few and many of them run different kernels.)"""
+    for pool in ("k_pool", "v_pool"):
+        c = Fp4Case(sizes, nq=4, nkv=2, hd=hd, page=16, dtype=dtype, seed=12)
+        flat = getattr(c, pool)[c.table[0, 0].long(), 1].view(-1)  # kv head 1 of the first page
+        flat[16 * hd // 2 + 3 * hd // 16] = 0x7f
+        out = _attend(c)
+        n = sizes[0][0]
+        bad = out[:n, 2:].isnan()
+        assert bad.all() if pool == "k_pool" else bad[..., :16].all() and not bad[..., 16:].any()
+        assert out[:n, :2].isfinite().all() and out[n:].isfinite().all()
+
+
+@pytest.mark.gpu
+def test_pools_off_their_alignment_are_refused():
+    from kernels.paged_fp4 import paged_append_fp4, paged_attention_fp4, paged_read_fp4
+
+    c = Fp4Case([(1, 20)], spoil=False)
+    room = torch.zeros(c.k_pool.numel() + 16, dtype=torch.uint8, device="cuda")
+    odd = room[8:8 + c.k_pool.numel()].view(c.k_pool.shape)
+    cos, sin = _rope(64, 128)
+    qkv = torch.zeros(1, 16 * 128, device="cuda").half()
+    for k, v in ((odd, c.v_pool), (c.k_pool, odd)):
+        for call in (lambda: paged_attention_fp4(c.q, k, v, c.table, c.lengths), lambda: paged_read_fp4(k, v, c.table, c.lengths),
+                     lambda: paged_append_fp4(qkv, k, v, c.table, c.lengths, cos, sin, 12, 2)):
+            with pytest.raises(RuntimeError, match="alignment"):
+                call()
+
+
+@pytest.mark.gpu
+def test_calls_on_two_streams_at_once():
+    """Each call has a workspace of its own: calls side by side give what they give alone."""
+    cases = [Fp4Case([(1, 900 + 50 * b) for b in range(6)], seed=20, spoil=False), Fp4Case([(3, 700), (140, 300), (1, 50)], seed=21, spoil=False),
+             Fp4Case([(200, 1200), (260, 700)], seed=22, dtype=BF16, spoil=False), Fp4Case([(1, 40), (1, 90)], seed=23, prefix=600, spoil=False)]
+    run = [_attend, _attend, _attend, _attend_prefix]
+    want = [f(c) for f, c in zip(run, cases)]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    same = []
+    for _ in range(20):
+        for f, c, s, w in zip(run, cases, streams, want):
+            with torch.cuda.stream(s):
+                same.append((f(c) == w).all())
+    torch.cuda.synchronize()
+    assert torch.stack(same).all()
+
+
 # ------------------------------------------------------------------------------------------ together
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype,hd", [(F16, 128), (BF16, 64)])

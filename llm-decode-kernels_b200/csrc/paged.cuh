@@ -362,6 +362,17 @@ __device__ __forceinline__ int result_row(const Problem& p, int tok, int g) {
   return tok / p.half_tokens * 128 + tok % p.half_tokens * p.G + g;
 }
 
+// Rows that belong to no sequence are in no tile: their outputs are zero. Warp `first` of `step` that share them.
+template <int kHd>
+__device__ __forceinline__ void zero_outside_rows(const Problem& p, int first, int step, int lane) {
+  const int from = min(max(p.starts[0], 0), p.T), to = max(min(p.starts[p.B], p.T), from);
+  const int vecs = p.nkv * p.G * kHd / 8;  // 16 bytes each
+  for (int t = first; t < p.T - (to - from); t += step) {
+    uint4* row = reinterpret_cast<uint4*>(p.out) + static_cast<int64_t>(t < from ? t : t - from + to) * vecs;
+    for (int i = lane; i < vecs; i += 32) row[i] = make_uint4(0, 0, 0, 0);
+  }
+}
+
 // ------------------------------------------------------------------------------------------- host
 constexpr int kMaxBatch = 4096;  // kOneToken: the chunk sums of a batch lie in shared memory
 

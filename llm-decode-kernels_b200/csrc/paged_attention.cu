@@ -439,8 +439,8 @@ struct JoinShape {
   static constexpr int kRows = kR, kDims = kD, kParts = kP, kAhead = kA;  // kAhead: pieces loaded at a time
   static constexpr int kLanes = kR * kD, kThreads = kLanes * kP;
   int lane, part, row, d4;  // of this thread; row: in the whole grid's y (or x)
-  __device__ explicit JoinShape(int y)
-      : lane(threadIdx.x % kLanes), part(threadIdx.x / kLanes), row(y * kR + lane % kR), d4(blockIdx.z * kD + lane / kR) {}
+  __device__ JoinShape(int y, int z)
+      : lane(threadIdx.x % kLanes), part(threadIdx.x / kLanes), row(y * kR + lane % kR), d4(z * kD + lane / kR) {}
 };
 
 template <typename T, int kHd>
@@ -508,17 +508,14 @@ __device__ __forceinline__ T* out_row(const Problem& p, int t, int head) {
   return static_cast<T*>(p.out) + (static_cast<int64_t>(t) * p.nkv * p.G + head) * kHd;
 }
 
-// Joins the units that a piece's end cuts. Block (x, y): rows of the unit that CTA x began, if there is one, or with
+// Joins the units that a piece's end cuts. Block (x, y, z): rows of the unit that CTA x began, if there is one, or with
 // `by_unit` (launches of fewer units than CTAs) of unit x, if it is cut.
 template <typename T, int kHd, typename Shape>
-__global__ void __launch_bounds__(Shape::kThreads) join_split_kernel(const Problem p, int tile_rows, int ctas, int by_unit) {
-  pdl_trigger();
-  pdl_wait();
+__device__ __forceinline__ void join_split(const Problem& p, int tile_rows, int ctas, int by_unit, int x, int y, int z) {
   int4 c;  // {first token, tokens, kv head, last CTA}
-  Pieces w{static_cast<int>(blockIdx.x), 0, 0};
+  Pieces w{x, 0, 0};
   if (by_unit) {
     const Line line = line_of(p, kTcChunk);
-    const int x = blockIdx.x;
     if (x >= line.tiles * p.nkv) return;
     const int h = x / line.tiles, ti = x - h * line.tiles;
     const Tile t = tile_at(p, ti);
@@ -526,17 +523,39 @@ __global__ void __launch_bounds__(Shape::kThreads) join_split_kernel(const Probl
     if (w.first == w.last) return;
     c = make_int4(t.t0, t.ntok, h, w.last);
   } else {
-    c = p.cut[blockIdx.x];
+    c = p.cut[x];
     w.last = c.w;
   }
-  const Shape at(blockIdx.y);
+  const Shape at(y, z);
   const int rows = c.y * p.G, i = at.row;
-  if (static_cast<int>(blockIdx.y) * Shape::kRows >= rows) return;
+  if (y * Shape::kRows >= rows) return;
   Joined<T, kHd> sum;
   if (i < rows)
     sum.template add_part<Shape::kAhead>(p, w, at.part, Shape::kParts, tile_rows, result_row(p, i / p.G, i % p.G), at.d4);
   sum.join_parts(at);
   if (at.part == 0 && i < rows) sum.store(out_row<T, kHd>(p, c.x + i / p.G, c.z * p.G + i % p.G), at.d4, p.out_scale);
+}
+
+template <typename T, int kHd, typename Shape>
+__global__ void __launch_bounds__(Shape::kThreads) join_split_kernel(const Problem p, int tile_rows, int ctas, int by_unit) {
+  pdl_trigger();
+  pdl_wait();
+  join_split<T, kHd, Shape>(p, tile_rows, ctas, by_unit, blockIdx.x, blockIdx.y, blockIdx.z);
+}
+
+// The same for the two launches of a call at once: the first `blocks` blocks are a's, (x, y) with y < ay, the others b's.
+template <typename T, int kHd, typename ShapeA, typename ShapeB>
+__global__ void __launch_bounds__(ShapeA::kThreads)
+    join_both_kernel(const Problem a, int a_rows, int a_ctas, int blocks, int ay, const Problem b, int b_rows, int b_ctas, int by_unit, int by) {
+  static_assert(ShapeA::kThreads == ShapeB::kThreads, "one block size");
+  constexpr int kZ = kHd / 4 / ShapeB::kDims;
+  pdl_trigger();
+  pdl_wait();
+  int x = blockIdx.x;
+  if (x < blocks)
+    return join_split<T, kHd, ShapeA>(a, a_rows, a_ctas, 0, x / ay, x % ay, 0);
+  x -= blocks;
+  join_split<T, kHd, ShapeB>(b, b_rows, b_ctas, by_unit, x / kZ / by, x / kZ % by, x % kZ);
 }
 
 // Joins the prefix's results (`a`) with those of the sequences' own positions (`b`). Block (x, h): rows (token, head of
@@ -546,7 +565,7 @@ __global__ void __launch_bounds__(Shape::kThreads)
     join_prefix_kernel(const Problem a, int a_ctas, const Problem b, int b_ctas, int b_rows) {
   pdl_trigger();
   pdl_wait();
-  const Shape at(blockIdx.x);
+  const Shape at(blockIdx.x, blockIdx.z);
   const int h = blockIdx.y;
   const bool live = at.row < a.T * a.G;
   const int t = live ? at.row / a.G : 0, g = live ? at.row % a.G : 0;
@@ -795,7 +814,7 @@ dim3 join_grid(int64_t x, int64_t y, int64_t hd) {
 }
 
 template <typename T, int kHd>
-cudaError_t launch_join(const Sizes& z, cudaStream_t st, const Pass* prefix, const Pass& own) {
+cudaError_t launch_join(const Sizes& z, cudaStream_t st, const Pass* prefix, const Pass* few, const Pass& own) {
   // Tiles are bound by the bytes of their pieces (for a prompt of 8192 about 40 MB in L2, 6 us) and by the number of blocks:
   // two or four rows a thread, or fewer blocks that loop, came out the same or slower.
   using Tiles = JoinShape<8, kHd / 4, 1, 2>;
@@ -813,6 +832,15 @@ cudaError_t launch_join(const Sizes& z, cudaStream_t st, const Pass* prefix, con
   const int64_t units = static_cast<int64_t>(own.p.max_tiles) * z.nkv, x = std::min<int64_t>(units, own.ctas);
   const int64_t y = (std::min<int64_t>(z.T, own.p.tile_tokens) * (z.nq / z.nkv) + 7) / 8;
   const int by_unit = units < own.ctas;
+  if (few != nullptr) {
+    using Wide = JoinShape<kHd == 128 ? 8 : 16, kHd / 4, 1, 2>;  // (Tiles in blocks of the other shapes' size)
+    const int64_t ay = few->rows / OneToken::kRows, blocks = few->ctas * ay;
+    const bool in_parts = units * kFewPieces <= own.ctas;
+    const int64_t by = in_parts ? y : (y * 8 + Wide::kRows - 1) / Wide::kRows, bz = in_parts ? kHd / 4 / Few::kDims : 1;
+    return launch(in_parts ? join_both_kernel<T, kHd, OneToken, Few> : join_both_kernel<T, kHd, OneToken, Wide>,
+                  dim3(static_cast<unsigned>(blocks + x * by * bz)), dim3(Few::kThreads), 0, st, pdl_enabled(), one, few->p, few->rows,
+                  few->ctas, static_cast<int>(blocks), static_cast<int>(ay), own.p, own.rows, own.ctas, by_unit, static_cast<int>(by));
+  }
   if (units * kFewPieces <= own.ctas)
     return launch(join_split_kernel<T, kHd, Few>, join_grid<Few>(x, y, kHd), dim3(Few::kThreads), 0, st, pdl_enabled(), one,
                   own.p, own.rows, own.ctas, by_unit);
@@ -986,13 +1014,13 @@ int attention(const char* what, const dk_paged_attention_args& a, bool prefix, b
       e = launch_rows(z, s->rows, s->shape, st, mk, mv, s->p, s == &own ? beside : 0);
     }
   }
-  for (const Pass* s : {&few, &own}) {
-    if (s->ctas == 0 || e != cudaSuccess) continue;
-    const Pass* with = z.prefix_len > 0 ? &pre : nullptr;
+  if (e == cudaSuccess) {
+    const Pass *with = z.prefix_len > 0 ? &pre : nullptr, *beside_it = has_few ? &few : nullptr;
     if (z.dtype == DK_F16)
-      e = z.hd == 128 ? launch_join<__half, 128>(z, st, with, *s) : launch_join<__half, 64>(z, st, with, *s);
+      e = z.hd == 128 ? launch_join<__half, 128>(z, st, with, beside_it, own) : launch_join<__half, 64>(z, st, with, beside_it, own);
     else
-      e = z.hd == 128 ? launch_join<__nv_bfloat16, 128>(z, st, with, *s) : launch_join<__nv_bfloat16, 64>(z, st, with, *s);
+      e = z.hd == 128 ? launch_join<__nv_bfloat16, 128>(z, st, with, beside_it, own)
+                      : launch_join<__nv_bfloat16, 64>(z, st, with, beside_it, own);
   }
   if (e != cudaSuccess) return set_error(DK_ERR_CUDA, "%s launch: %s", what, cudaGetErrorString(e));
   return DK_OK;

@@ -493,14 +493,7 @@ __global__ void __launch_bounds__(kThreads<kBlocks>, 1) fp4_rows_kernel(const Pr
       }
     }
   }
-  if (kRaggedTiles && p.zero_outside && producer) {  // rows that belong to no sequence are in no tile: their outputs are zero
-    const int from = min(max(p.starts[0], 0), p.T), to = max(min(p.starts[p.B], p.T), from);
-    const int vecs = p.nkv * p.G * kHd / 8;  // 16 bytes each
-    for (int r = cta; r < p.T - (to - from); r += ctas) {
-      uint4* row = reinterpret_cast<uint4*>(p.out) + static_cast<int64_t>(r < from ? r : r - from + to) * vecs;
-      for (int i = lane; i < vecs; i += 32) row[i] = make_uint4(0, 0, 0, 0);
-    }
-  }
+  if (kRaggedTiles && p.zero_outside && producer) zero_outside_rows<kHd>(p, cta, ctas, lane);
   if (__syncthreads_or(!ok) && producer && lane == 0) {
     // a wait gave up: let copies still in flight land before the shared memory goes away (bounded)
     const uint64_t t0 = globaltimer_ns();

@@ -261,6 +261,14 @@ __global__ void __launch_bounds__(kThreads<kFp4>, 1)
   __shared__ int failed;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (kFp4 && p.above > 0) {  // beside a launch for the sequences of few tokens: there may be no others
+    pdl_wait();
+    if (p.plan[0] == 0) {
+      pdl_trigger();
+      if (warp == kZeroWarp && p.zero_outside) zero_outside_rows<kHd>(p, blockIdx.x, gridDim.x, lane);
+      return;
+    }
+  }
   if (tid == 0) {
     for (int i = 0; i < L::kSlots; ++i) {
       mbar_init(&bar.kv_full[i], kFp4 ? kConvertWarps : 1);
@@ -713,15 +721,7 @@ __global__ void __launch_bounds__(kThreads<kFp4>, 1)
       }
     }
   }
-  if (warp == kZeroWarp && p.zero_outside) {
-    // Rows that belong to no sequence are in no tile: their outputs are zero. (Beside a prefix the join writes all rows.)
-    const int from = min(max(p.starts[0], 0), p.T), to = max(min(p.starts[p.B], p.T), from);
-    const int vecs = p.nkv * p.G * kHd / 8;  // 16 bytes each
-    for (int t = blockIdx.x; t < p.T - (to - from); t += gridDim.x) {
-      uint4* row = reinterpret_cast<uint4*>(p.out) + static_cast<int64_t>(t < from ? t : t - from + to) * vecs;
-      for (int i = lane; i < vecs; i += 32) row[i] = make_uint4(0, 0, 0, 0);
-    }
-  }
+  if (warp == kZeroWarp && p.zero_outside) zero_outside_rows<kHd>(p, blockIdx.x, gridDim.x, lane);
 
   __syncwarp();
   if (!ok && lane == 0) failed = 1;

@@ -635,7 +635,7 @@ struct Sizes {
 // in tiles of up to 16 rows that each read the sequence again, up to kFewTiles of them; longer ones to the 256-row tiles (32 sequences
 // of 4096, 28 heads over 4, tiles of 2 tokens, us on the rows kernel and as 256-row tiles: 2 tokens 31, 61; 4 39, 62; 6 53,
 // 62; 8 62, 63; 12 93, 57. 16 of 4096, 8 over 8, tiles of 16: 32 44, 60; 64 69, 61). Which there are only the device
-// knows, and a launch without any takes 5 us with its join. A call whose sequences have kManyTokens on average is taken for
+// knows, and a launch without any takes 3 to 5 us. A call whose sequences have kManyTokens on average is taken for
 // prompts: then the tiles take all of them.
 constexpr int kFewTiles = 3, kManyTokens = 256;
 struct Split {
@@ -781,7 +781,7 @@ void shape_prefix(const Sizes& z, Pass& a) {
 // The two launches of a call with a prefix run side by side: the prefix's takes most of the SMs, and the own positions'
 // starts on the others right away, with longer pieces there. How long the prefix's takes is known here: about 6 us and 2 us
 // for each chunk of a CTA's piece; a group of the other takes 1.1 us for a chunk. Over a 4-bit cache a chunk of the other takes twice that
-// (prefix 64 x 8192: 39.4 us; leads of 26 and 32 in place of 20: 40.1, 42.1).
+// (prefix 64 x 8192: 37.1 us; a third more or less of that lead: 37.1, 37.6).
 void share_gpu(const Sizes& z, Pass& pre, Pass& own) {
   if (own.tc || !pdl_enabled()) return;
   const int sms = device_info().num_sms;

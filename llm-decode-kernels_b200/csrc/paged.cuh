@@ -373,6 +373,94 @@ __device__ __forceinline__ void zero_outside_rows(const Problem& p, int first, i
   }
 }
 
+// ------------------------------------------------------------------------------------ ragged plan
+constexpr int kPlanThreads = 1024;
+constexpr int kTcChunk = 128;   // positions of a chunk of the 256-row tiles,
+constexpr int kFp4Chunk = 128;  // and of the kernel for few rows over a 4-bit cache
+
+// One CTA cuts the launch's sequences into tiles of tile_tokens tokens and sums up their chunks.
+__device__ __forceinline__ void make_plan(const Problem& p) {
+  int32_t* plan = const_cast<int32_t*>(p.plan);
+  int4* info = const_cast<int4*>(p.tile_info);
+  constexpr int kOwnTiles = 4;  // tiles of a sequence that its own thread writes
+  __shared__ int warp_sum[kPlanThreads / 32];
+  __shared__ int long_count;
+  __shared__ int4 long_seq[kPlanThreads];  // {first tile, tiles, first token, end}
+  __shared__ int2 long_len[kPlanThreads];  // {length, sequence}
+  if (threadIdx.x == 0) long_count = 0;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // inclusive scan over the CTA; returns the exclusive prefix and the total
+  auto scan = [&](int v, int& total) {
+    int s = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += u;
+    }
+    __syncthreads();
+    if (lane == 31) warp_sum[warp] = s;
+    __syncthreads();
+    int w = warp_sum[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, w, o);
+      if (lane >= o) w += u;
+    }
+    total = __shfl_sync(0xffffffffu, w, 31);
+    const int before = __shfl_sync(0xffffffffu, w, warp == 0 ? 0 : warp - 1);
+    return (warp == 0 ? 0 : before) + s - v;
+  };
+  int32_t* cum = plan + 2;
+  int tiles = 0, length = 0;
+  for (int b0 = 0; b0 < p.B; b0 += kPlanThreads) {
+    const int b = b0 + tid;
+    const int t0 = b < p.B ? min(max(p.starts[b], 0), p.T) : 0;
+    const int t1 = b < p.B ? min(max(p.starts[b + 1], t0), p.T) : 0;
+    const int mine = t1 - t0 > p.above && t1 - t0 <= p.most ? (t1 - t0 + p.tile_tokens - 1) / p.tile_tokens : 0;
+    int total;
+    const int at = tiles + scan(mine, total);
+    // sequence and first token of each tile; long sequences are filled in by the whole CTA below
+    if (mine > 0 && at < p.max_tiles) info[at] = make_int4(t0, t1, length_of(p.lengths, b), b);
+    for (int i = 1; i < min(mine, kOwnTiles) && at + i < p.max_tiles; ++i)
+      info[at + i] = make_int4(t0 + i * p.tile_tokens, t1, length_of(p.lengths, b), b);
+    __syncthreads();
+    if (mine > kOwnTiles) {
+      const int k = atomicAdd(&long_count, 1);
+      long_seq[k] = make_int4(at, mine, t0, t1);
+      long_len[k] = make_int2(length_of(p.lengths, b), b);
+    }
+    __syncthreads();
+    for (int k = 0; k < long_count; ++k)
+      for (int i = kOwnTiles + tid; i < long_seq[k].y && long_seq[k].x + i < p.max_tiles; i += kPlanThreads)
+        info[long_seq[k].x + i] = make_int4(long_seq[k].z + i * p.tile_tokens, long_seq[k].w, long_len[k].x, long_len[k].y);
+    __syncthreads();
+    if (tid == 0) long_count = 0;
+    tiles += total;
+  }
+  tiles = min(tiles, p.max_tiles);
+  __syncthreads();  // the tiles written above are read by other threads below
+  for (int i0 = 0; i0 < tiles; i0 += kPlanThreads) {
+    const int i = i0 + tid;
+    int n = 0;
+    if (i < tiles) {
+      const int4 v = info[i];  // {first token, sequence's end, length, sequence}
+      const int ntok = min(p.tile_tokens, v.y - v.x), p0 = v.z - (v.y - v.x);
+      info[i] = make_int4(v.x, ntok, p0, v.w);
+      n = (p.chunk == kTcChunk ? Span<kTcChunk>(p0, p0 + ntok - 1, p.mask, p.capacity, p.page_size).n
+                               : Span<kFp4Chunk>(p0, p0 + ntok - 1, p.mask, p.capacity, p.page_size).n) + p.unit_extra;
+    }
+    int total;
+    const int at = length + scan(n, total);
+    if (i < tiles) cum[i] = at;
+    length += total;
+  }
+  if (tid == 0) {
+    cum[tiles] = length;
+    plan[0] = tiles;
+    plan[1] = length;
+  }
+}
+
 // ------------------------------------------------------------------------------------------- host
 constexpr int kMaxBatch = 4096;  // kOneToken: the chunk sums of a batch lie in shared memory
 
@@ -384,17 +472,16 @@ struct RowsShape {
 };
 // Such a launch over a cache held in 4 bits (paged_attention_fp4.cu), with tiles of 8 or 16 rows; fp4_groups pieces of the line a CTA.
 constexpr int fp4_groups(int rows) { return rows == 8 ? 3 : 2; }
-constexpr int kFp4Chunk = 128;
 RowsShape fp4_rows_shape(int64_t hd, int dtype, int rows, bool ragged);
 cudaError_t fp4_rows_launch(const Problem& p, int64_t hd, int dtype, int rows, bool ragged, const RowsShape& s, int wait_late,
                             cudaStream_t st);
 
 // Writes the pages that a ragged call over a 4-bit cache sees in 16 bits, k and v [B * table width, n_kv, page_size, hd] with the tables
-// that list them [B, table width] (paged_read_fp4.cu).
-cudaError_t fp4_copy_launch(const Problem& p, int64_t hd, int dtype, void* k, void* v, int32_t* table, cudaStream_t st);
+// that list them [B, table width], and beside that the plans of a and, with `plans` = 2, of b (paged_read_fp4.cu).
+cudaError_t fp4_copy_launch(const Problem& a, const Problem& b, int plans, int64_t hd, int dtype, void* k, void* v, int32_t* table,
+                            cudaStream_t st);
 
 // The launch of the 256-row tensor-core kernel (paged_attention_tc.cu): CTAs of one wave (0: it does not fit).
-constexpr int kTcChunk = 128;
 constexpr int kTcRows = 256;
 constexpr int kTcUnitExtra = 3;  // a unit's fixed cost (its Q, first and last steps, output) in chunks (2, 4: up to 2 us more)
 int tc_ctas(int64_t hd, int dtype, bool fp4);

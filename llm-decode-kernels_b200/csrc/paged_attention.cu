@@ -31,95 +31,15 @@ constexpr int kGroups = 2;   // independent consumer groups of a CTA, each with 
 constexpr int kCWarps = 4;   // warps of a group
 constexpr int kThreads = kGroups * (kCWarps + 1) * 32;
 constexpr int kMaxRing = 6;
-constexpr int kPlanThreads = 1024;
 constexpr int kFp4UnitExtra = 1;   // the same over a 4-bit cache, whose chunks are longer
 constexpr int kRowsUnitExtra = 2;  // a unit's fixed cost (q, joining the warps, output) in chunks
 
 // ------------------------------------------------------------------------------------ ragged plan
-// One CTA cuts the launch's sequences into tiles of tile_tokens tokens and sums up their chunks. A second one plans a second launch.
+// A second CTA plans a second launch.
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Problem pa, const Problem pb) {
-  const Problem& p = blockIdx.x == 0 ? pa : pb;
-  int32_t* plan = const_cast<int32_t*>(p.plan);
-  int4* info = const_cast<int4*>(p.tile_info);
-  constexpr int kOwnTiles = 4;  // tiles of a sequence that its own thread writes
-  __shared__ int warp_sum[kPlanThreads / 32];
-  __shared__ int long_count;
-  __shared__ int4 long_seq[kPlanThreads];  // {first tile, tiles, first token, end}
-  __shared__ int2 long_len[kPlanThreads];  // {length, sequence}
-  if (threadIdx.x == 0) long_count = 0;
   pdl_trigger();
   pdl_wait();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  // inclusive scan over the CTA; returns the exclusive prefix and the total
-  auto scan = [&](int v, int& total) {
-    int s = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, s, o);
-      if (lane >= o) s += u;
-    }
-    __syncthreads();
-    if (lane == 31) warp_sum[warp] = s;
-    __syncthreads();
-    int w = warp_sum[lane];
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, w, o);
-      if (lane >= o) w += u;
-    }
-    total = __shfl_sync(0xffffffffu, w, 31);
-    const int before = __shfl_sync(0xffffffffu, w, warp == 0 ? 0 : warp - 1);
-    return (warp == 0 ? 0 : before) + s - v;
-  };
-  int32_t* cum = plan + 2;
-  int tiles = 0, length = 0;
-  for (int b0 = 0; b0 < p.B; b0 += kPlanThreads) {
-    const int b = b0 + tid;
-    const int t0 = b < p.B ? min(max(p.starts[b], 0), p.T) : 0;
-    const int t1 = b < p.B ? min(max(p.starts[b + 1], t0), p.T) : 0;
-    const int mine = t1 - t0 > p.above && t1 - t0 <= p.most ? (t1 - t0 + p.tile_tokens - 1) / p.tile_tokens : 0;
-    int total;
-    const int at = tiles + scan(mine, total);
-    // sequence and first token of each tile; long sequences are filled in by the whole CTA below
-    if (mine > 0 && at < p.max_tiles) info[at] = make_int4(t0, t1, length_of(p.lengths, b), b);
-    for (int i = 1; i < min(mine, kOwnTiles) && at + i < p.max_tiles; ++i)
-      info[at + i] = make_int4(t0 + i * p.tile_tokens, t1, length_of(p.lengths, b), b);
-    __syncthreads();
-    if (mine > kOwnTiles) {
-      const int k = atomicAdd(&long_count, 1);
-      long_seq[k] = make_int4(at, mine, t0, t1);
-      long_len[k] = make_int2(length_of(p.lengths, b), b);
-    }
-    __syncthreads();
-    for (int k = 0; k < long_count; ++k)
-      for (int i = kOwnTiles + tid; i < long_seq[k].y && long_seq[k].x + i < p.max_tiles; i += kPlanThreads)
-        info[long_seq[k].x + i] = make_int4(long_seq[k].z + i * p.tile_tokens, long_seq[k].w, long_len[k].x, long_len[k].y);
-    __syncthreads();
-    if (tid == 0) long_count = 0;
-    tiles += total;
-  }
-  tiles = min(tiles, p.max_tiles);
-  __syncthreads();  // the tiles written above are read by other threads below
-  for (int i0 = 0; i0 < tiles; i0 += kPlanThreads) {
-    const int i = i0 + tid;
-    int n = 0;
-    if (i < tiles) {
-      const int4 v = info[i];  // {first token, sequence's end, length, sequence}
-      const int ntok = min(p.tile_tokens, v.y - v.x), p0 = v.z - (v.y - v.x);
-      info[i] = make_int4(v.x, ntok, p0, v.w);
-      n = (p.chunk == kTcChunk ? Span<kTcChunk>(p0, p0 + ntok - 1, p.mask, p.capacity, p.page_size).n
-                               : Span<kFp4Chunk>(p0, p0 + ntok - 1, p.mask, p.capacity, p.page_size).n) + p.unit_extra;
-    }
-    int total;
-    const int at = length + scan(n, total);
-    if (i < tiles) cum[i] = at;
-    length += total;
-  }
-  if (tid == 0) {
-    cum[tiles] = length;
-    plan[0] = tiles;
-    plan[1] = length;
-  }
+  make_plan(blockIdx.x == 0 ? pa : pb);
 }
 
 // ------------------------------------------------------------------------------------ decode kernel
@@ -986,10 +906,10 @@ int attention(const char* what, const dk_paged_attention_args& a, bool prefix, b
 
   cudaStream_t st = reinterpret_cast<cudaStream_t>(a.stream);
   cudaError_t e = cudaSuccess;
-  if (z.ragged)
+  if (z.ragged && !copied)
     e = launch(plan_kernel, dim3(has_few ? 2 : 1), dim3(kPlanThreads), 0, st, pdl_enabled(), dim3(1, 1, 1), own.p, few.p);
   if (copied) {
-    if (e == cudaSuccess) e = fp4_copy_launch(own.p, z.hd, z.dtype, copy.k, copy.v, copy.table, st);
+    e = fp4_copy_launch(own.p, few.p, has_few ? 2 : 1, z.hd, z.dtype, copy.k, copy.v, copy.table, st);
     own.p.table = copy.table, own.p.ld_table = table_width;
     own.p.n_pages = static_cast<int>(z.B * table_width);
   }

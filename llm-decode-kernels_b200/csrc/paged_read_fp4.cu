@@ -127,15 +127,19 @@ struct CopyParams {
   int* err;
 };
 
+// The first `plans` CTAs make the plans of the launches that follow: neither waits for the other.
 template <typename T, int kHd>
-__global__ void __launch_bounds__(kWarps * 32) fp4_copy_kernel(const CopyParams p) {
+__global__ void __launch_bounds__(kPlanThreads) fp4_copy_kernel(const CopyParams p, const Problem pa, const Problem pb, int plans) {
   using F = Fp4<kHd>;
   constexpr int kPieces = 16 * kHd / 8;  // of 8 dims of 16 positions of a head
+  constexpr int kWarps = kPlanThreads / 32;
   pdl_trigger();
   pdl_wait();
+  const int cta = static_cast<int>(blockIdx.x) - plans, ctas = static_cast<int>(gridDim.x) - plans;
+  if (cta < 0) return make_plan(blockIdx.x == 0 ? pa : pb);
   const int lane = threadIdx.x & 31, per_seq = p.width << (p.page_shift - 4), heads = 2 * p.nkv;
   const int64_t units = static_cast<int64_t>(p.B) * per_seq * heads;
-  for (int64_t u = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5); u < units; u += static_cast<int64_t>(gridDim.x) * kWarps) {
+  for (int64_t u = static_cast<int64_t>(cta) * kWarps + (threadIdx.x >> 5); u < units; u += static_cast<int64_t>(ctas) * kWarps) {
     const int64_t group = u / heads;
     const int b = static_cast<int>(group / per_seq), j0 = static_cast<int>(group - static_cast<int64_t>(b) * per_seq) * 16;
     // seen: below the length, and from the first row's window on or below the sinks
@@ -185,16 +189,19 @@ __global__ void __launch_bounds__(kWarps * 32) fp4_copy_kernel(const CopyParams 
 
 namespace paged {
 
-cudaError_t fp4_copy_launch(const Problem& p, int64_t hd, int dtype, void* k, void* v, int32_t* table, cudaStream_t st) {
+cudaError_t fp4_copy_launch(const Problem& p, const Problem& b, int plans, int64_t hd, int dtype, void* k, void* v, int32_t* table,
+                            cudaStream_t st) {
   CopyParams c;
   c.pool[0] = p.pool[0], c.pool[1] = p.pool[1], c.out[0] = k, c.out[1] = v, c.table_out = table;
   c.table = p.table, c.ld_table = p.ld_table, c.lengths = p.lengths, c.starts = p.starts;
   c.T = p.T, c.B = p.B, c.nkv = p.nkv, c.n_pages = p.n_pages, c.page_size = p.page_size, c.page_shift = p.page_shift;
   c.above = p.above, c.width = p.capacity >> p.page_shift, c.mask = p.mask, c.err = p.err;
   const int64_t units = static_cast<int64_t>(p.B) * (p.capacity / 16) * 2 * p.nkv;
-  const dim3 grid(static_cast<unsigned>(std::min<int64_t>((units + kWarps - 1) / kWarps, 8ll * device_info().num_sms)));
-#define DK_COPY(TT) \
-  launch(hd == 128 ? fp4_copy_kernel<TT, 128> : fp4_copy_kernel<TT, 64>, grid, dim3(kWarps * 32), 0, st, pdl_enabled(), dim3(1, 1, 1), c)
+  constexpr int kCopyWarps = kPlanThreads / 32;
+  const dim3 grid(static_cast<unsigned>(plans + std::min<int64_t>((units + kCopyWarps - 1) / kCopyWarps, 2ll * device_info().num_sms)));
+#define DK_COPY(TT)                                                                                                              \
+  launch(hd == 128 ? fp4_copy_kernel<TT, 128> : fp4_copy_kernel<TT, 64>, grid, dim3(kPlanThreads), 0, st, pdl_enabled(), dim3(1, 1, 1), \
+         c, p, b, plans)
   return dtype == DK_F16 ? DK_COPY(__half) : DK_COPY(__nv_bfloat16);
 #undef DK_COPY
 }

@@ -78,7 +78,7 @@ __device__ __forceinline__ uint32_t choose(uint32_t a, uint32_t b, uint32_t m) {
 
 __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((127 + e) << 23); }
 
-// kRagged: tiles of the plan, a few tokens each; otherwise tile b is the one token of sequence b.
+// kRaggedTiles: tiles of the plan, a few tokens each; otherwise tile b is the one token of sequence b.
 template <typename T, int kHd, int kBlocks, bool kRaggedTiles>
 __global__ void __launch_bounds__(kThreads<kBlocks>, 1) fp4_rows_kernel(const Problem p, int wait_late) {
   constexpr int ring = kRing<kHd, kBlocks>;
@@ -92,15 +92,15 @@ __global__ void __launch_bounds__(kThreads<kBlocks>, 1) fp4_rows_kernel(const Pr
   __shared__ float2 pre_ml_sh[kG][kRows * kCWarps];
   __shared__ __align__(8) uint64_t full_sh[kG][ring], empty_sh[kG][ring];
   __shared__ int warp_sum[kT / 32 + 1];
-  extern __shared__ __align__(128) uint8_t base[];
-  int* cum_sh = reinterpret_cast<int*>(base);  // [B + 1], before the first copies land there
+  extern __shared__ __align__(128) uint8_t dsm[];
+  int* cum_sh = reinterpret_cast<int*>(dsm);  // [B + 1], before the first copies land there
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const bool producer = warp >= kG * kCWarps;
   const int group = producer ? warp - kG * kCWarps : warp / kCWarps;
   const int cta = blockIdx.x * kG + group, ctas = gridDim.x * kG;  // pieces of the line: one a group
-  uint8_t* slots = base + group * ring * S::kBytes;
-  float* pre_o = reinterpret_cast<float*>(base + kG * ring * S::kBytes) + group * kCWarps * kRows * kHd;
+  uint8_t* slots = dsm + group * ring * S::kBytes;
+  float* pre_o = reinterpret_cast<float*>(dsm + kG * ring * S::kBytes) + group * kCWarps * kRows * kHd;
   float2* pre_ml = pre_ml_sh[group];
   uint64_t *full = full_sh[group], *empty = empty_sh[group];
   if (tid == 0) {
@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(kThreads<kBlocks>, 1) fp4_rows_kernel(const Pr
   Walk<kChunk> walk(p, line, cta, ctas, lane);
   __syncthreads();  // the sums have been read: copies may land on them
   bool ok = true;
-  int fill = 0;         // ring fills so far,
+  int fill = 0;          // ring fills so far,
   int s = 0, round = 0;  // fill % ring and fill / ring
   auto filled = [&] {
     ++fill;

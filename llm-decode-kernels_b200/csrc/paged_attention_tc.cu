@@ -265,6 +265,7 @@ __global__ void __launch_bounds__(kThreads<kFp4>, 1)
     pdl_wait();
     if (p.plan[0] == 0) {
       pdl_trigger();
+      if (tid == 0) p.cut[blockIdx.x] = make_int4(0, 0, 0, 0);  // (the join reads every CTA's)
       if (warp == kZeroWarp && p.zero_outside) zero_outside_rows<kHd>(p, blockIdx.x, gridDim.x, lane);
       return;
     }

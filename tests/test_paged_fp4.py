@@ -382,6 +382,52 @@ def test_attention_long_rings(hd, nq):
     assert_within(_attend(few), *few.attention())
 
 
+def _attend_in(c, fill, window=0, sinks=0):
+    """The call's output, made in a workspace that holds `fill` in each of its 32-bit words."""
+    import ctypes
+
+    from kernels import _lib
+    from kernels.paged import _DTYPES
+
+    T, B, code, width = c.q.shape[0], c.lengths.numel(), _DTYPES[c.dtype], c.table.shape[1]
+    n, prefix = ctypes.c_uint64(0), c.prefix if c.prefix else 0
+    _lib.call("dk_paged_attention_fp4_workspace_bytes", T, B, c.nq, c.nkv, c.hd, code, c.starts is not None, prefix, width * c.page,
+              ctypes.byref(n))
+    ws = torch.full((n.value // 4,), fill, dtype=torch.int32, device="cuda")
+    out = torch.full((T, c.nq, c.hd), torch.nan, dtype=c.dtype, device="cuda")
+    args = _lib.PAGED_ATTENTION_FP4_ARGS.pack(
+        c.q.data_ptr(), c.q.stride(0), c.k_pool.data_ptr(), c.v_pool.data_ptr(), c.k_pool.shape[0], c.page,
+        c.prefix_table.data_ptr() if prefix else 0, prefix, c.table.data_ptr(), c.table.stride(0), width, c.lengths.data_ptr(),
+        0 if c.starts is None else c.starts.data_ptr(), window, sinks, c.hd ** -0.5, out.data_ptr(), T, B, c.nq, c.nkv, c.hd, code,
+        ws.data_ptr(), n.value, torch.cuda.current_stream().cuda_stream, c.scales["k_scale"], c.scales["v_scale"])
+    entry = "dk_shared_prefix_attention_fp4" if prefix else "dk_paged_attention_fp4"
+    _lib.check(getattr(_lib.lib(), entry)(args), entry)
+    return out
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,hd", [(BF16, 128), (F16, 64)])
+@pytest.mark.parametrize("sizes,prefix", [
+    ([(2, 40)] * 70, 0),  # as many units of tiles as CTAs may come, none does
+    ([(1, 900), (2, 40)] * 40, 0),
+    ([(2, 40)] * 69 + [(60, 300)], 0),
+    ([(3, 40)] * 4, 0),
+    ([(1, 500)], 0),
+    ([(1, 33)] * 300, 0),
+    ([(130, 400), (7, 9), (1, 3000)], 0),
+    ([(600, 900), (500, 600)], 0),  # copied
+    ([(1, 40)] * 20, 300),
+    ([(2, 40), (90, 100)] * 10, 300),
+])
+def test_workspaces_may_hold_anything(sizes, prefix, dtype, hd):
+    """What a workspace held before a call changes nothing of it: not zeros, nor NaN, nor words that could be records of
+    the call's own."""
+    c = Fp4Case(sizes, nq=8, nkv=4, hd=hd, page=16, dtype=dtype, prefix=prefix, seed=11)
+    out = _attend_in(c, 1)
+    assert_within(out, *c.attention())
+    assert torch.equal(out, _attend_in(c, 0)) and torch.equal(out, _attend_in(c, -1))
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("hd,dtype", [(64, BF16), (128, BF16), (128, F16)])
 @pytest.mark.parametrize("sizes", [

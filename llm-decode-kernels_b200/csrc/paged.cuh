@@ -147,6 +147,7 @@ struct Problem {
   int early, lead;  // the launch's first `early` pieces are `lead` chunks longer than the others (their CTAs start while
                     // the kernel before still holds the other SMs)
   int unit_extra;   // chunks added to a unit's length on the line for what it costs besides its chunks
+  int unit_len;     // fp4_rows_kernel: above 0, no unit is cut (Walk)
   int n_tiles;      // kOneToken, kPrefix; kRagged: the plan's
   // kRagged: plan[0] = tiles, plan[1] = length of one kv head's line, then cum[max_tiles + 1]; what tile_at needs of
   // each tile lies in tile_info
@@ -261,11 +262,12 @@ __device__ __forceinline__ Line line_of(const Problem& p, int chunk) {
 // (A launch's line is shorter than 2^31: checked on the host. 64-bit divisions took a microsecond of these kernels' starts.)
 struct Cuts {
   int long_end, per_long, per, early;
-  __device__ Cuts(const Problem& p, const Line& line, int ctas) {
+  __device__ Cuts(const Problem& p, const Line& line, int ctas, int whole = 0) {
     const int all = line.chunks * p.nkv;
     early = p.early;
     const int ahead = early * p.lead;
     per = all > ahead ? (all - ahead + ctas - 1) / ctas : 0;
+    if (whole > 0) per = (per + whole - 1) / whole * whole;  // (no lead there)
     per_long = early == 0 ? 0 : per > 0 ? per + p.lead : (all + early - 1) / early;
     long_end = early * per_long;
   }
@@ -281,8 +283,9 @@ __device__ __forceinline__ int pool_row(const Problem& p, int page, int h, int j
   return p.n_pages * p.nkv * p.page_size;
 }
 
-// A CTA's piece of the line, unit by unit. Whole warps walk it.
-template <int kChunk>
+// A CTA's piece of the line, unit by unit. Whole warps walk it. kMayBeWhole: with p.unit_len above 0 each unit has that length on the
+// line, however many of them are chunks, and pieces end between units.
+template <int kChunk, bool kMayBeWhole = false>
 struct Walk {
   const Problem& p;
   const Line& line;
@@ -296,7 +299,7 @@ struct Walk {
   Tile t, next_tile;  // (the next tile's fields are loaded a part ahead)
   int last;           // the tile's last position
   __device__ Walk(const Problem& p_, const Line& line_, int cta, int ctas, int lane)
-      : p(p_), line(line_), cuts(p_, line_, ctas) {
+      : p(p_), line(line_), cuts(p_, line_, ctas, kMayBeWhole ? p_.unit_len : 0) {
     const int all = line.chunks * p.nkv;
     x = min(cuts.begin(cta), all);
     x1 = min(cuts.begin(cta + 1), all);
@@ -318,7 +321,8 @@ struct Walk {
     t = next_tile;
     last = tile_last(p, t);
     const Span<kChunk> span(t.p0, last, p.mask, p.capacity, p.page_size);
-    const int to = min(span.n + p.unit_extra, c0 + (x1 - x));
+    const int length = kMayBeWhole && p.unit_len > 0 ? p.unit_len : span.n + p.unit_extra;
+    const int to = min(length, c0 + (x1 - x));
     x += to - c0;
     c1 = min(to, span.n);
     next_c = 0;

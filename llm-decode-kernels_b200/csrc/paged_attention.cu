@@ -683,6 +683,24 @@ void shape_own(const Sizes& z, Pass& a) {
   a.p.zero_outside = z.ragged && z.prefix_len == 0;
 }
 
+// Over a 4-bit cache: the chunks of a rows pass's longest unit if the units are short, else 0. Short units are not cut, and no join follows:
+// up to 3 chunks (short page tables or windows), and up to kShortUnit where the units keep two fifths of the groups busy in one
+// round (one token each; us cut and joined, and whole, replayed from a graph; sequences, kv heads: positions): 1, 2: 60 8.4, 4.9;
+// 380 9.8, 9.0; 500 9.7, 10.8. 16, 8: 380 10.9, 9.9; 500 10.9, 12.0. 48, 4: 380 12.7, 10.6; 640 15.1, 14.4; 760 15.3, 16.2.
+// 64, 4: 500 15.0, 12.5; 640 15.4, 14.8. 112, 4 (a second round): 250 14.6, 13.8; 380 16.6, 17.1; 500 17.4, 20.2. 256, 4: 380 24.0, 23.1.
+// Launched one by one, these calls of one launch take 12 us instead of 14.
+constexpr int64_t kShortUnit = 5;
+int short_unit(const Sizes& z, const Pass& a) {
+  // A window takes its own positions, from the first token's to the last's, and parts of pages before them and at the sinks' end.
+  const int64_t part = std::min(a.p.page_size, kFp4Chunk), all = a.p.capacity;
+  const int64_t most = a.p.mask.window > 0
+                           ? std::min<int64_t>(all, int64_t(a.p.mask.window) + a.p.mask.sinks + a.p.tile_tokens + 2 * part)
+                           : all;
+  const int64_t chunks = (most + kFp4Chunk - 1) / kFp4Chunk, units = z.B * z.nkv;
+  const bool one_round = 5 * units >= 2 * a.ctas && units <= a.ctas;
+  return chunks <= (one_round ? kShortUnit : 3) ? static_cast<int>(chunks) : 0;
+}
+
 // The sequences of few tokens of a ragged call that has others too.
 void shape_few(const Sizes& z, Pass& a) {
   set_tile(z, a, false);
@@ -903,6 +921,7 @@ int attention(const char* what, const dk_paged_attention_args& a, bool prefix, b
   }
   pre.p.table = a.prefix_table, pre.p.capacity = static_cast<int>(z.prefix_len), pre.p.mask = Mask{0, 0};
   if (z.prefix_len > 0) share_gpu(z, pre, own);
+  else if (z.fp4 && !own.tc) own.p.unit_len = short_unit(z, own);
 
   cudaStream_t st = reinterpret_cast<cudaStream_t>(a.stream);
   cudaError_t e = cudaSuccess;
@@ -934,7 +953,7 @@ int attention(const char* what, const dk_paged_attention_args& a, bool prefix, b
       e = launch_rows(z, s->rows, s->shape, st, mk, mv, s->p, s == &own ? beside : 0);
     }
   }
-  if (e == cudaSuccess) {
+  if (e == cudaSuccess && own.p.unit_len == 0) {
     const Pass *with = z.prefix_len > 0 ? &pre : nullptr, *beside_it = has_few ? &few : nullptr;
     if (z.dtype == DK_F16)
       e = z.hd == 128 ? launch_join<__half, 128>(z, st, with, beside_it, own) : launch_join<__half, 64>(z, st, with, beside_it, own);

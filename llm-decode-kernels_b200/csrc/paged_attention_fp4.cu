@@ -114,7 +114,10 @@ __global__ void __launch_bounds__(kThreads<kBlocks>, 1) fp4_rows_kernel(const Pr
   pdl_trigger();
 
   Line line{cum_sh, 0, p.n_tiles, 0};
-  if constexpr (kRaggedTiles) {
+  if (p.unit_len > 0) {
+    const int tiles = kRaggedTiles ? p.plan[0] : p.n_tiles;
+    line = {nullptr, p.unit_len, tiles, tiles * p.unit_len};
+  } else if constexpr (kRaggedTiles) {
     line = line_of(p, kChunk);
   } else {  // every CTA sums up the sequences' chunks for itself
     int carry = 0;
@@ -150,7 +153,7 @@ __global__ void __launch_bounds__(kThreads<kBlocks>, 1) fp4_rows_kernel(const Pr
   }
   __syncthreads();
 
-  Walk<kChunk> walk(p, line, cta, ctas, lane);
+  Walk<kChunk, true> walk(p, line, cta, ctas, lane);
   __syncthreads();  // the sums have been read: copies may land on them
   bool ok = true;
   int fill = 0;          // ring fills so far,

@@ -429,6 +429,26 @@ def test_workspaces_may_hold_anything(sizes, prefix, dtype, hd):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("hd,nq,nkv,dtype,page", [(128, 28, 4, BF16, 16), (64, 6, 2, F16, 256), (128, 9, 1, BF16, 64)])
+@pytest.mark.parametrize("sizes,window,sinks", [
+    ([(1, 1)], 0, 0),
+    ([(1, 0), (1, 256), (1, 200), (1, 0)], 0, 0),
+    ([(1, 1 + 7 * b % 384) for b in range(150)], 0, 0),  # more units than groups, or fewer
+    ([(1, 640 - b) for b in range(56)], 0, 0),
+    ([(1, 1500), (1, 3), (1, 90)], 60, 5),  # short windows over long caches
+    ([(1, 1500), (1, 3), (1, 90)] * 20, 130, 140),
+    ([(2, 300), (0, 0), (1, 20), (3, 2)], 0, 0),
+    ([(2, 900), (0, 10), (1, 20), (2, 1)], 33, 1),
+])
+def test_attention_of_short_units(sizes, window, sinks, hd, nq, nkv, dtype, page):
+    """Short page tables and short windows: no sequence's work is cut."""
+    c = Fp4Case(sizes, nq=nq, nkv=nkv, hd=hd, page=page, dtype=dtype, seed=12)
+    out = _attend_in(c, 1, window, sinks)
+    assert_within(out, *c.attention(window, sinks))
+    assert torch.equal(out, _attend(c, window=window, sinks=sinks))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("hd,dtype", [(64, BF16), (128, BF16), (128, F16)])
 @pytest.mark.parametrize("sizes", [
     [(900, 2500), (300, 1500)],  # copied, 16-bit tiles

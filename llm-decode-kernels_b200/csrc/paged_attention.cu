@@ -558,6 +558,13 @@ struct Sizes {
 // knows, and a launch without any takes 3 to 5 us. A call whose sequences have kManyTokens on average is taken for
 // prompts: then the tiles take all of them.
 constexpr int kFewTiles = 3, kManyTokens = 256;
+// Calls of little work, whatever their sequences have of it, all go to the rows kernel, which needs no second launch and mostly no join: up to
+// kSmallFew chunks a group where the sequences have few tokens on average, kSmallMany else (up to that many tokens each, split by sequence
+// or as tiles, and on the rows kernel, us; in brackets chunks a group). 28 heads over 4: 8 x 5: 250 17.4, 13.6; 4000 25.3, 23.0 (9). 64 x
+// 2: 250 26.2, 13.3; 500 29.0, 16.4; 1000 32.6, 26.0 (12). 32 x 5: 500 27.2, 16.9. 16 x 20, 8 over 8: 2000 34.1, 29.2 (13). 12 over 2:
+// 1 x 100: 500 19.6, 17.3 (1); 1000 20.3, 20.1 (3); 2000 21.6, 25.2 (6). 8 x 64: 500 27.9, 25.2 (5); 1000 28.9, 31.7 (10). 8 x 200, 8 over
+// 8: 250 29.8, 22.4 (4); 500 33.6, 35.7 (8).
+constexpr int64_t kSmallFew = 16, kSmallMany = 4;
 struct Split {
   bool few, many;  // which kernels are launched
   int limit;       // the most tokens of a sequence of the first
@@ -565,7 +572,10 @@ struct Split {
 Split split_of(const Sizes& z) {
   const int64_t limit = kFewTiles * (16 / (z.nq / z.nkv));
   if (!z.fp4 || !z.ragged || z.prefix_len > 0 || z.T >= kManyTokens * z.B) return {false, true, 0};
-  if (z.T <= limit) return {true, false, INT_MAX};
+  const int64_t token = 16 / (z.nq / z.nkv), tiles = (z.T + token - 1) / token + z.B;
+  const int64_t chunks = tiles * z.nkv * ((z.positions + kFp4Chunk - 1) / kFp4Chunk);
+  const int64_t small = (z.T <= limit * z.B ? kSmallFew : kSmallMany) * fp4_groups(16) * device_info().num_sms;
+  if (z.T <= limit || chunks <= small) return {true, false, INT_MAX};
   return {z.B > 1, true, z.B > 1 ? static_cast<int>(limit) : 0};
 }
 

@@ -342,6 +342,26 @@ def test_attention_ragged(sizes, nq, nkv, hd, page, dtype, window, sinks):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("sizes,nq,nkv,hd,page,dtype,window,sinks", RAGGED + [
+    ([(60, 700), (50, 120), (2, 100), (9, 9)], 8, 2, 64, 256, F16, 100, 5),
+    ([(60, 700), (50, 120), (2, 100), (9, 9)], 12, 2, 128, 128, BF16, 100, 70),
+    ([(9, 5), (40, 200), (3, 0)], 12, 2, 128, 16, F16, 1 << 30, 3),
+    ([(70, 200), (3, 90)], 12, 2, 128, 32, BF16, 40, 2),
+    ([(2, 40)] * 70 + [(30, 31)], 8, 4, 64, 16, BF16, 33, 1),
+])
+def test_attention_ragged_in_wide_tables(sizes, nq, nkv, hd, page, dtype, window, sinks):
+    """Page tables so wide that the call might be a large one: split by the sequences' tokens between two kernels."""
+    from kernels import _lib
+
+    c = Fp4Case(sizes, nq, nkv, hd, page, dtype, seed=2, one_token=False, wide=1 << 16)
+    _lib.clear_device_error()
+    out = _attend_in(c, 1, window, sinks)
+    assert _lib.device_error() == 0
+    assert_within(out, *c.attention(window, sinks))
+    assert torch.equal(out, _attend(c, window=window, sinks=sinks))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("sizes,prefix,nq,nkv,hd,page,dtype", [
     ([(1, 1)], 1, 12, 2, 128, 16, F16),
     ([(1, 40), (1, 1), (1, 65)], 525, 12, 2, 128, 16, F16),

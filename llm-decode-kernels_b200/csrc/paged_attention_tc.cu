@@ -23,7 +23,7 @@
 // all operands are fp16 (code * scale is exact there), so bf16 Q is turned into fp16 by its rows' softmax threads first, times a
 // power of two that the row's scale takes back. For prompts the conversion of every chunk for every tile costs more than it
 // saves: MMAs read shared memory at nearly its full rate, and the converted tiles are stored beside that (a prompt of 8192, 12 heads
-// over 2: 271 us, 280 with two converting warps of twice the registers; copied to 16-bit pages first 197). It is used for prefixes
+// over 2: 271 us, 280 with two converting warps of twice the registers; copied to 16-bit pages first 193). It is used for prefixes
 // and for ragged calls of fewer tokens.
 // What bounds it: a chunk's four products take 4 x 8 x 65 = 2080 cycles at head_dim 128, its 32768 exponentials 2048 (16 a
 // cycle), and they run beside each other; a pair of half chunks takes about 1.65 us (1.15 at least), a unit's start, masks

@@ -112,7 +112,8 @@ __global__ void __launch_bounds__(kWarps * 32) paged_read_fp4_kernel(const ReadP
 
 // Pages in 16 bits of what a call's rows see, for the 256-row tiles (paged_attention_tc.cu): a page of the copy for each entry of
 // the page tables, and tables that list them. A warp takes 16 positions of a head's k or v; the powers are left out (the scores' scale
-// and the output's have them). Measured: 8192 positions of 2 kv heads of 128, 2.4 MB read and 8.4 written, 5.1 us with its launch.
+// and the output's have them). Measured: 8192 positions of 2 kv heads of 128, 2.4 MB read and 8.4 written, 5.1 us with its launch
+// (the plan, a launch before it, then added 4; now a CTA or two beside the copy make it).
 struct CopyParams {
   const uint8_t* pool[2];
   void* out[2];  // [B * width, nkv, page_size, kHd]

@@ -480,17 +480,22 @@ RowsShape fp4_rows_shape(int64_t hd, int dtype, int rows, bool ragged);
 cudaError_t fp4_rows_launch(const Problem& p, int64_t hd, int dtype, int rows, bool ragged, const RowsShape& s, int wait_late,
                             cudaStream_t st);
 
-// Writes the pages that a ragged call over a 4-bit cache sees in 16 bits, k and v [B * table width, n_kv, page_size, hd] with the tables
-// that list them [B, table width], and beside that the plans of a and, with `plans` = 2, of b (paged_read_fp4.cu).
+// Writes the pages that a ragged call over a 4-bit cache sees in 16 bits, k (of type `dtype`) and v (fp16) [B * table width, n_kv,
+// page_size, hd] with the tables that list them [B, table width], and beside that the plans of a and, with `plans` = 2, of b (paged_read_fp4.cu).
 cudaError_t fp4_copy_launch(const Problem& a, const Problem& b, int plans, int64_t hd, int dtype, void* k, void* v, int32_t* table,
                             cudaStream_t st);
 
 // The launch of the 256-row tensor-core kernel (paged_attention_tc.cu): CTAs of one wave (0: it does not fit).
 constexpr int kTcRows = 256;
 constexpr int kTcUnitExtra = 3;  // a unit's fixed cost (its Q, first and last steps, output) in chunks (2, 4: up to 2 us more)
-int tc_ctas(int64_t hd, int dtype, bool fp4);
-// mk, mv: the pages as rows of head_dim, in boxes of 64 dims of min(page_size, kTcChunk) rows, 128-byte swizzle (not used with fp4).
-int tc_launch(const Problem& p, int64_t nq, int64_t hd, int dtype, bool fp4, int ctas, const CUtensorMap& mk,
+enum class Pages {  // what it reads: pages of q's type, of 4-bit codes, or the 16-bit copy of those
+  kPlain,
+  kCodes,
+  kCopy,
+};
+int tc_ctas(int64_t hd, int dtype, Pages pages);
+// mk, mv: the pages as rows of head_dim, in boxes of 64 dims of min(page_size, kTcChunk) rows, 128-byte swizzle (not used with codes).
+int tc_launch(const Problem& p, int64_t nq, int64_t hd, int dtype, Pages pages, int ctas, const CUtensorMap& mk,
               const CUtensorMap& mv, int wait_late, cudaStream_t st);
 
 }  // namespace paged

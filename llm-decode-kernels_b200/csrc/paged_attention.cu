@@ -590,6 +590,8 @@ bool copies(const Sizes& z) {
          z.positions <= kCopyBytes / (4 * z.hd) / z.nkv / z.B;
 }
 
+Pages pages_of(const Sizes& z) { return !z.fp4 ? Pages::kPlain : copies(z) ? Pages::kCopy : Pages::kCodes; }
+
 RowsShape rows_shape_of(const Sizes& z, int rows) {
   if (z.fp4) return fp4_rows_shape(z.hd, z.dtype, rows, z.ragged);
 #define DK_SHAPE(TT) \
@@ -638,7 +640,7 @@ void cut_pass(const Sizes& z, Cutter& c, Pass& a, bool always_partial) {
     a.rows = kTcRows;
     p.unit_extra = kTcUnitExtra;
     p.rows_inner = 1;
-    a.ctas = tc_ctas(z.hd, z.dtype, z.fp4 && !copies(z));
+    a.ctas = tc_ctas(z.hd, z.dtype, pages_of(z));
   } else {
     a.rows = z.nq / z.nkv <= 8 && !z.ragged ? 8 : 16;
     a.shape = rows_shape_of(z, a.rows);
@@ -944,21 +946,22 @@ int attention(const char* what, const dk_paged_attention_args& a, bool prefix, b
   }
   const void *k_pages = copied ? copy.k : a.k_pages, *v_pages = copied ? copy.v : a.v_pages;
   const uint64_t rows = static_cast<uint64_t>(own.p.n_pages * z.nkv * page_size);
-  const CUtensorMapDataType type = z.dtype == DK_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const CUtensorMapDataType k_type = z.dtype == DK_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const CUtensorMapDataType v_type = copied ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : k_type;
   CUtensorMap mk, mv;
   uint32_t box = 0;
   auto page_maps = [&](int chunk) {  // in boxes of a page, or of a chunk's positions of one (0.3 us each, so not made twice)
     const uint32_t want = static_cast<uint32_t>(std::min<int64_t>(page_size, chunk));
     if (want == box) return true;
     box = want;
-    return make_tensor_map_2d(&mk, k_pages, type, z.hd, rows, z.hd * 2, 64, box, CU_TENSOR_MAP_SWIZZLE_128B) &&
-           make_tensor_map_2d(&mv, v_pages, type, z.hd, rows, z.hd * 2, 64, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    return make_tensor_map_2d(&mk, k_pages, k_type, z.hd, rows, z.hd * 2, 64, box, CU_TENSOR_MAP_SWIZZLE_128B) &&
+           make_tensor_map_2d(&mv, v_pages, v_type, z.hd, rows, z.hd * 2, 64, box, CU_TENSOR_MAP_SWIZZLE_128B);
   };
   for (const Pass* s : {&pre, &few, &own}) {
     if (s->ctas == 0 || e != cudaSuccess) continue;
     if ((!z.fp4 || (copied && s->tc)) && !page_maps(s->tc ? kTcChunk : kChunk)) return DK_ERR_CUDA;
     if (s->tc) {
-      if (const int rc = tc_launch(s->p, z.nq, z.hd, z.dtype, z.fp4 && !copied, s->ctas, mk, mv, s == &own ? beside : 0, st)) return rc;
+      if (const int rc = tc_launch(s->p, z.nq, z.hd, z.dtype, pages_of(z), s->ctas, mk, mv, s == &own ? beside : 0, st)) return rc;
     } else {
       e = launch_rows(z, s->rows, s->shape, st, mk, mv, s->p, s == &own ? beside : 0);
     }

@@ -243,13 +243,14 @@ __device__ __forceinline__ int q_to_fp16(uint8_t* row, int r) {
   return e;
 }
 
-template <typename T, int kHd, bool kFp4>
+// P: the type of P and V in their product. K and Q are of type T, with kFp4 fp16.
+template <typename T, int kHd, bool kFp4, typename P>
 __global__ void __launch_bounds__(kThreads<kFp4>, 1)
     tiles_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                  const __grid_constant__ CUtensorMap mv, const Problem p, int wait_late) {
   using L = Smem<kHd, kFp4>;
-  using M = typename std::conditional<kFp4, __half, T>::type;  // of the products' operands
-  constexpr bool kTurnQ = kFp4 && !std::is_same<T, __half>::value;
+  using K = typename std::conditional<kFp4, __half, T>::type;
+  constexpr bool kTurnQ = !std::is_same<T, K>::value;
   constexpr uint32_t kS[2] = {0, 128}, kO[2] = {256, 256 + kHd};  // tensor-memory columns; P(X) lies over S(X)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
@@ -422,7 +423,7 @@ __global__ void __launch_bounds__(kThreads<kFp4>, 1)
 #pragma unroll
       for (int k = 0; k < kHd / 16; ++k) {
         const uint32_t off = ((k / 4) * L::kSegBytes + (k % 4) * 32) >> 4;  // (descriptors count 16 bytes)
-        mma_ss(tmem + kS[x], a + off, b + off, idesc<M>(128, kC, false) | (p.signs < 0 ? kNegateA : 0u), k > 0);
+        mma_ss(tmem + kS[x], a + off, b + off, idesc<K>(128, kC, false) | (p.signs < 0 ? kNegateA : 0u), k > 0);
       }
       commit_elected(&bar.s_full[x]);
     };
@@ -436,7 +437,7 @@ __global__ void __launch_bounds__(kThreads<kFp4>, 1)
         tc::fence_after_sync();
 #pragma unroll
         for (int k = half * kPartSteps; k < (half ? kC / 16 : kPartSteps); ++k)
-          mma_ts(tmem + kO[x], tmem + kS[x] + 8 * k, b + ((k * 2048) >> 4), idesc<M>(128, kHd, true), !first || k > 0);
+          mma_ts(tmem + kO[x], tmem + kS[x] + 8 * k, b + ((k * 2048) >> 4), idesc<P>(128, kHd, true), !first || k > 0);
       }
       ++p_seen[x];
     };
@@ -584,7 +585,7 @@ __global__ void __launch_bounds__(kThreads<kFp4>, 1)
             float2 y = fma2(make_float2(s[32 * c + 2 * d], s[32 * c + 2 * d + 1]), scale, off);
             y = make_float2(exp2_approx(y.x), exp2_approx(y.y));
             sum[d & 3] = add2(sum[d & 3], y);
-            w[d] = Elem<M>::pack(y.x, y.y);
+            w[d] = Elem<P>::pack(y.x, y.y);
           }
           tmem_st16(s_col + 16 * c, w);
           if (c == kPartChunks - 1 || c == kC / 32 - 1) {  // a part of P is complete
@@ -753,7 +754,7 @@ bool make_q_map(CUtensorMap* map, const Problem& p, int64_t nq, int64_t hd, CUte
   return make_tensor_map(map, p.q, type, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <typename T, int kHd, bool kFp4>
+template <typename T, int kHd, bool kFp4, typename P>
 int ctas_of() {
   static std::mutex mu;
   static int known[64];  // by device; 0: not asked yet, -1: does not fit
@@ -763,34 +764,35 @@ int ctas_of() {
   int& n = known[dev & 63];
   if (n == 0) {
     cudaFuncAttributes a;  // the register split needs the launch to hold exactly what it divides
-    const bool split = cudaFuncGetAttributes(&a, tiles_kernel<T, kHd, kFp4>) == cudaSuccess && a.numRegs == kRegsLaunch<kFp4>;
-    n = split && opt_in_dynamic_smem(tiles_kernel<T, kHd, kFp4>) >= Smem<kHd, kFp4>::kBytes ? device_info().num_sms : -1;
+    const bool split = cudaFuncGetAttributes(&a, tiles_kernel<T, kHd, kFp4, P>) == cudaSuccess && a.numRegs == kRegsLaunch<kFp4>;
+    n = split && opt_in_dynamic_smem(tiles_kernel<T, kHd, kFp4, P>) >= Smem<kHd, kFp4>::kBytes ? device_info().num_sms : -1;
   }
   return n < 0 ? 0 : n;
 }
 
 }  // namespace
 
-#define DK_BY_KIND(CALL)                                                                                      \
-  (dtype == DK_F16 ? (hd == 128 ? (fp4 ? CALL(__half, 128, true) : CALL(__half, 128, false))                  \
-                                : (fp4 ? CALL(__half, 64, true) : CALL(__half, 64, false)))                   \
-                   : (hd == 128 ? (fp4 ? CALL(__nv_bfloat16, 128, true) : CALL(__nv_bfloat16, 128, false))    \
-                                : (fp4 ? CALL(__nv_bfloat16, 64, true) : CALL(__nv_bfloat16, 64, false))))
+#define DK_BY_PAGES(CALL, TT, HH)                       \
+  (pages == Pages::kCodes  ? CALL(TT, HH, true, __half) \
+   : pages == Pages::kCopy ? CALL(TT, HH, false, __half) : CALL(TT, HH, false, TT))
+#define DK_BY_KIND(CALL)                                                                          \
+  (dtype == DK_F16 ? (hd == 128 ? DK_BY_PAGES(CALL, __half, 128) : DK_BY_PAGES(CALL, __half, 64)) \
+                   : (hd == 128 ? DK_BY_PAGES(CALL, __nv_bfloat16, 128) : DK_BY_PAGES(CALL, __nv_bfloat16, 64)))
 
-int tc_ctas(int64_t hd, int dtype, bool fp4) {
-#define DK_CTAS(TT, HH, FF) ctas_of<TT, HH, FF>()
+int tc_ctas(int64_t hd, int dtype, Pages pages) {
+#define DK_CTAS(TT, HH, FF, PP) ctas_of<TT, HH, FF, PP>()
   return DK_BY_KIND(DK_CTAS);
 #undef DK_CTAS
 }
 
-int tc_launch(const Problem& p, int64_t nq, int64_t hd, int dtype, bool fp4, int ctas, const CUtensorMap& mk, const CUtensorMap& mv,
+int tc_launch(const Problem& p, int64_t nq, int64_t hd, int dtype, Pages pages, int ctas, const CUtensorMap& mk, const CUtensorMap& mv,
               int wait_late, cudaStream_t st) {
   const CUtensorMapDataType type = dtype == DK_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   CUtensorMap mq;
   if (!make_q_map(&mq, p, nq, hd, type)) return DK_ERR_CUDA;
-#define DK_TILES(TT, HH, FF)                                                                                                        \
-  launch(tiles_kernel<TT, HH, FF>, dim3(ctas), dim3(kThreads<FF>), Smem<HH, FF>::kBytes, st, pdl_enabled(), dim3(1, 1, 1), mq, mk, mv, p, \
-         wait_late)
+#define DK_TILES(TT, HH, FF, PP)                                                                                                    \
+  launch(tiles_kernel<TT, HH, FF, PP>, dim3(ctas), dim3(kThreads<FF>), Smem<HH, FF>::kBytes, st, pdl_enabled(), dim3(1, 1, 1), mq, mk, \
+         mv, p, wait_late)
   const cudaError_t e = DK_BY_KIND(DK_TILES);
 #undef DK_TILES
   if (e != cudaSuccess) return set_error(DK_ERR_CUDA, "paged attention (256-row tiles) launch: %s", cudaGetErrorString(e));

@@ -112,11 +112,13 @@ __global__ void __launch_bounds__(kWarps * 32) paged_read_fp4_kernel(const ReadP
 
 // Pages in 16 bits of what a call's rows see, for the 256-row tiles (paged_attention_tc.cu): a page of the copy for each entry of
 // the page tables, and tables that list them. A warp takes 16 positions of a head's k or v; the powers are left out (the scores' scale
-// and the output's have them). Measured: 8192 positions of 2 kv heads of 128, 2.4 MB read and 8.4 written, 5.1 us with its launch
-// (the plan, a launch before it, then added 4; now a CTA or two beside the copy make it).
+// and the output's have them). code * scale is exact in either type: k is of the call's, so that q is the other factor as it is, and
+// v is fp16, so that p keeps 11 bits beside it as in the other kernels over such a cache (bf16 would leave it 8).
+// Measured: 8192 positions of 2 kv heads of 128, 2.4 MB read and 8.4 written, 5.1 us with its launch (the plan, a launch before it,
+// then added 4; now a CTA or two beside the copy make it).
 struct CopyParams {
   const uint8_t* pool[2];
-  void* out[2];  // [B * width, nkv, page_size, kHd]
+  void* out[2];  // [B * width, nkv, page_size, kHd]: k of type T, v fp16
   int32_t* table_out;
   const int32_t* table;
   int64_t ld_table;
@@ -167,7 +169,7 @@ __global__ void __launch_bounds__(kPlanThreads) fp4_copy_kernel(const CopyParams
       code[i] = there ? codes[32 * i] : 0;
       scale[i] = there ? scales[16 * i] : 0;
     }
-    uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(which ? p.out[1] : p.out[0]) + ((to * p.nkv + h) * p.page_size + slot) * kHd) + lane;
+    uint4* out = static_cast<uint4*>(which ? p.out[1] : p.out[0]) + ((to * p.nkv + h) * p.page_size + slot) * (kHd / 8) + lane;
 #pragma unroll
     for (int i = 0; i < kPieces / 32; ++i) {
       uint32_t x[4], one = fp4_scales(scale[i]);
@@ -176,7 +178,7 @@ __global__ void __launch_bounds__(kPlanThreads) fp4_copy_kernel(const CopyParams
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         x[k] = hmul2_rn(x[k], one);
-        if constexpr (!std::is_same<T, __half>::value) {
+        if (!std::is_same<T, __half>::value && !which) {
           const float2 f = Elem<__half>::unpack(x[k]);
           x[k] = Elem<T>::pack(f.x, f.y);
         }

@@ -680,7 +680,8 @@ void set_tile(const Sizes& z, Pass& a, bool tc) {
 
 void set_ragged(const Sizes& z, Pass& a, int above, int most) {
   a.p.mode = kRagged;
-  a.p.max_tiles = static_cast<int>(z.T / a.p.tile_tokens + z.B);
+  const int64_t of_one = (int64_t(most) + a.p.tile_tokens - 1) / a.p.tile_tokens;  // tiles of a sequence, at most
+  a.p.max_tiles = static_cast<int>(std::min(z.T / a.p.tile_tokens + z.B, of_one * z.B));
   a.p.above = above, a.p.most = most;
 }
 

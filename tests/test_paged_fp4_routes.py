@@ -31,3 +31,20 @@ def test_bf16_calls_keep_p_in_fp16(sizes, wide, route, hd, tmp_path):
     c.dtype = F16
     _, tol = c.attention(window, sinks)  # fp16's roundoff in every term: the output's is exchanged for bf16's
     assert_within(_attend(c, window=window, sinks=sinks), exact, tol + (2.0 ** -8 - 2.0 ** -11) * exact.abs())
+
+
+def test_split_calls_count_each_launch_by_what_it_takes():
+    """Of a call that is split by its sequences' tokens, the launch for the short ones has three tiles a sequence at most, however many
+    tokens the others bring: 2048 sequences of 195 tokens on average, 64 heads over 8, tables of 131072 positions are no more work than
+    the library takes (as far as the workspace, of which there is none), 65536 such sequences are."""
+    from kernels import _lib
+
+    h = _lib.lib()
+
+    def attend(T, B):
+        at, width = 1 << 20, 131072 // 64  # addresses that are looked at for their alignment alone
+        return h.dk_paged_attention_fp4(_lib.PAGED_ATTENTION_FP4_ARGS.pack(
+            at, 64 * 128, at, at, 1 << 20, 64, 0, 0, at, width, width, at, at, 0, 0, 1.0, at, T, B, 64, 8, 128, 0, at, 0, 0, 1.0, 1.0))
+
+    assert attend(400_000, 2048) == -1 and b"the workspace has 0 bytes" in h.dk_last_error()
+    assert attend(12_800_000, 65536) == -3 and b"chunks" in h.dk_last_error()

@@ -323,8 +323,8 @@ int dk_shared_prefix_attention(const dk_paged_attention_args* args);
  * head_dim / 16 bytes a position. A value is code * scale * k_scale (v_scale): an E2M1 code, an E4M3 scale for each 16 dims and a power of
  * two from 2^-64 to 2^64 for the pool; code * scale is exact in fp16 and bf16. `dtype` in these calls is qkv's, q's, out's. */
 /* Append: scale = E4M3(max |x| / 6) and code = E2M1(x / scale) of x / k_scale (v_scale), both rounded to nearest, ties to even,
- * and saturating; x are the values dk_paged_append would store, but the rotation of k is rounded once, from its exact
- * value in fp64. A NaN makes its group's scale NaN. */
+ * and saturating; x are the values dk_paged_append would store, but the rotation of k is computed in fp64, where its
+ * products are exact, rounded to fp32 and from there to qkv's type. A NaN makes its group's scale NaN. */
 typedef struct dk_paged_append_fp4_args {
   dk_paged_append_args append;
   double k_scale, v_scale;

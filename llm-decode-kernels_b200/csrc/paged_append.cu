@@ -10,8 +10,9 @@
 // token's sequence, position and page are a chain of small loads - and its angles once for all of them. With few tokens
 // a token's heads are spread over several warps.
 // With kFp4 k' and v go to a cache of 4-bit codes (paged_fp4.cuh). What a code is can hang on the last bit of k', so k is then
-// rotated in fp64, where the two products are exact, and rounded to T once before it is quantised: a code does not depend on
-// the order or the fusing of the operations. q is rotated as without. Measured (36 heads of 128, bf16): 11000 tokens, 127 MB of q, k, v in
+// rotated in fp64, where the two products are exact and only their sum is rounded, and goes to T by way of fp32: a code does not
+// depend on the order or the fusing of the operations. (Of fp16 keys about one in 17000 lies so close to the middle of two values that a
+// single rounding would give the other; these steps are what the cache's contents are defined by.) q is rotated as without. Measured (36 heads of 128, bf16): 11000 tokens, 127 MB of q, k, v in
 // and q out, 5 MB of codes, 33.6 us (30 without quantising, 1.5 more in fp64 than in fp32); 64 tokens 3 us without the host.
 // 3 CTAs an SM (80 registers, 20 bytes of them spilled instead of 88 to 104) come out 1 us slower.
 // Measured (36 heads of 128): 9000 tokens, 164 MB, 32 us, 78% of the copy rate (64 registers a thread, 4 CTAs an SM, 20 bytes of
@@ -70,9 +71,9 @@ __device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
 constexpr int kAhead = 2;  // 4 with half the warps resident: 33.9 against 32.9 us for 164 MB
 constexpr int kWarps = 8;
 
-// x c - y s and y c + x s of 8 pairs, rounded to T: in fp64 (the products of T and fp32 values are exact there).
+// x c - y s and y c + x s of 8 pairs in fp64 (the products of T and fp32 values are exact there), rounded to fp32, then to T.
 template <typename T>
-__device__ __forceinline__ void rotate8_exactly(const uint4& lo, const uint4& hi, const float (&co)[8], const float (&si)[8], float (&u)[8],
+__device__ __forceinline__ void rotate8_in_fp64(const uint4& lo, const uint4& hi, const float (&co)[8], const float (&si)[8], float (&u)[8],
                                                 float (&v)[8]) {
   const uint32_t l[4] = {lo.x, lo.y, lo.z, lo.w}, r[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
@@ -165,7 +166,7 @@ __global__ void __launch_bounds__(kWarps * 32, 4) paged_append_kernel(const Appe
           if constexpr (kFp4) {
             if (!is_q) {
               float x[8], y[8];
-              rotate8_exactly<T>(lo[a], hi[a], co, si, x, y);
+              rotate8_in_fp64<T>(lo[a], hi[a], co, si, x, y);
               put_fp4(p.k, h - p.nq, d, x, p.k_inv);
               put_fp4(p.k, h - p.nq, d + kHd / 2, y, p.k_inv);
               continue;

@@ -42,8 +42,8 @@ def paged_append_fp4(qkv, k_pages, v_pages, page_table, lengths, cos, sin, n_hea
                      v_scale=1.0, out=None):
     """`paged_append` into a 4-bit cache: rotates q and k of qkv [T, (n_heads + 2 n_kv) * head_dim] and writes k and v. Each 16 dims of
     a position get scale = E4M3(max |x| / 6) and codes E2M1(x / scale) of x / k_scale (x / v_scale for v), rounded to nearest,
-    ties to even; what is too large saturates, a NaN makes its 16 dims NaN. The rotation of k is exact before its one rounding to
-    qkv's type, so that the codes do not hang on how it is computed. Returns the rotated q [T, n_heads, head_dim] (`out`)."""
+    ties to even; what is too large saturates, a NaN makes its 16 dims NaN. The rotation of k is computed in fp64, where its
+    products are exact, rounded to fp32 and from there to qkv's type, so that the codes do not hang on the order of operations. Returns the rotated q [T, n_heads, head_dim] (`out`)."""
     what = "paged_append_fp4"
     return _append(what, qkv, k_pages, v_pages, page_table, lengths, cos, sin, n_heads, n_kv, starts, offset, out,
                    _powers(what, k_scale, v_scale))

@@ -1,0 +1,37 @@
+"""Edges of the ops over a 4-bit paged cache: roundings on the borders of the format, and calls whose arguments contradict one another."""
+
+import pytest
+import torch
+
+from _paged_fp4 import quantise, unpack
+
+F16, BF16 = torch.float16, torch.bfloat16
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_keys_are_rounded_by_way_of_fp32(dtype):
+    """A rotated key is a sum in fp64, rounded to fp32 and from there to the type. Two keys a hair (2^-40) beside the middle between two
+    values of the type, one of which is a border between codes: fp32 rounds them to that middle, the type to the border, and the border goes
+    to the even code. A single rounding would give the other neighbour, and the other code."""
+    from kernels.paged_fp4 import fp4_pages, paged_append_fp4
+
+    half_step = 2.0 ** -10 if dtype is F16 else 2.0 ** -7  # of the type, between 2 and 4
+    x, cos, sin = torch.zeros(64, dtype=torch.float64), torch.ones(1, 32, dtype=torch.float64), torch.zeros(1, 32, dtype=torch.float64)
+    x[1] = 6  # the group's scale is 1
+    for dim, border, side in ((0, 2.5, 1), (2, 3.5, -1)):
+        x[dim], x[dim + 32] = 1, 2.0 ** -14
+        cos[0, dim], sin[0, dim] = border + side * half_step, -side * 2.0 ** -26
+    turned = torch.cat([x[:32] * cos[0] - x[32:] * sin[0], x[32:] * cos[0] + x[:32] * sin[0]])
+    assert turned[0] > 2.5 + half_step and turned[2] < 3.5 - half_step
+    assert torch.equal(cos, cos.float().double()) and torch.equal(x, x.to(dtype).double())
+    rounded = turned.float().to(dtype)
+    assert rounded[0] == 2.5 and rounded[2] == 3.5
+    k, v = (fp4_pages(1, 1, 16, 64, "cuda").zero_() for _ in range(2))
+    qkv = torch.cat([torch.zeros(64), x, torch.zeros(64)]).to(dtype).cuda()[None]
+    one = torch.ones(1, dtype=torch.int32, device="cuda")
+    paged_append_fp4(qkv, k, v, one[None] - 1, one, cos.float().cuda(), sin.float().cuda(), 1, 1)
+    codes, scales = unpack(k.cpu())
+    want = quantise(rounded)
+    assert torch.equal(codes[0, 0, 0], want[0]) and torch.equal(scales[0, 0, 0], want[1])
+    assert codes[0, 0, 0, :3].tolist() == [4, 7, 6]  # 2 and not 3, 6, 4 and not 3

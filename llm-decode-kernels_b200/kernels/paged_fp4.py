@@ -58,7 +58,12 @@ def paged_read_fp4(k_pages, v_pages, page_table, lengths, starts=None, tokens=No
     position without a page in the pool is zero and sets the device error DK_DEVERR_BAD_POSITION."""
     what = "paged_read_fp4"
     if out is not None:
-        tokens, dtype = out[0].shape[0], out[0].dtype
+        if len(out) != 2:
+            _refuse(what, "out must be two contiguous [tokens, n_kv, head_dim] of one type")
+        rows, dtype = out[0].shape[0], out[0].dtype
+        if tokens is not None and tokens != rows:
+            _refuse(what, f"out has {rows} rows, tokens says {tokens}")
+        tokens = rows
     elif tokens is None:
         if starts is not None:
             _refuse(what, "with starts, tokens says how many rows there are")

@@ -35,3 +35,22 @@ def test_keys_are_rounded_by_way_of_fp32(dtype):
     want = quantise(rounded)
     assert torch.equal(codes[0, 0, 0], want[0]) and torch.equal(scales[0, 0, 0], want[1])
     assert codes[0, 0, 0, :3].tolist() == [4, 7, 6]  # 2 and not 3, 6, 4 and not 3
+
+
+def test_a_read_whose_rows_contradict_its_outputs_is_refused():
+    """`out` and `tokens` both say how many rows there are; one that says otherwise is not dropped silently."""
+    from _paged_fp4 import Fp4Case
+    from kernels.paged_fp4 import paged_read_fp4
+
+    c = Fp4Case([(3, 20), (2, 5)], spoil=False, device="cpu", one_token=False)
+    out = tuple(torch.zeros(5, 2, 128, dtype=F16) for _ in range(2))
+    args = (c.k_pool, c.v_pool, c.table, c.lengths, c.starts)
+    for tokens in (0, 3, 6):
+        with pytest.raises(ValueError, match="tokens"):
+            paged_read_fp4(*args, tokens=tokens, out=out)
+    for tokens in (None, 5):  # as far as the device
+        with pytest.raises(RuntimeError, match="CUDA device"):
+            paged_read_fp4(*args, tokens=tokens, out=out)
+    for pair in (out[:1], (*out, out[0])):
+        with pytest.raises(ValueError, match="out must be two"):
+            paged_read_fp4(*args, out=pair)

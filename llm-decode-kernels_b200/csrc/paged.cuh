@@ -154,7 +154,6 @@ struct Problem {
   const int32_t* plan;
   const int4* tile_info;  // {first token, tokens, position of the first one, sequence}
   int max_tiles;
-  int chunk;               // kRagged: positions of a chunk
   int above, most;         // kRagged: the sequences with more than `above` and at most `most` tokens are the launch's
   int zero_outside;        // kRagged: the launch writes zeros to rows that belong to no sequence
   int32_t* cum_out;  // kOneToken: [B + 1], the chunks of one kv head before each sequence
@@ -381,6 +380,7 @@ __device__ __forceinline__ void zero_outside_rows(const Problem& p, int first, i
 constexpr int kPlanThreads = 1024;
 constexpr int kTcChunk = 128;   // positions of a chunk of the 256-row tiles,
 constexpr int kFp4Chunk = 128;  // and of the kernel for few rows over a 4-bit cache
+static_assert(kTcChunk == kFp4Chunk, "a plan counts the chunks of either kernel");
 
 // One CTA cuts the launch's sequences into tiles of tile_tokens tokens and sums up their chunks.
 __device__ __forceinline__ void make_plan(const Problem& p) {
@@ -450,8 +450,7 @@ __device__ __forceinline__ void make_plan(const Problem& p) {
       const int4 v = info[i];  // {first token, sequence's end, length, sequence}
       const int ntok = min(p.tile_tokens, v.y - v.x), p0 = v.z - (v.y - v.x);
       info[i] = make_int4(v.x, ntok, p0, v.w);
-      n = (p.chunk == kTcChunk ? Span<kTcChunk>(p0, p0 + ntok - 1, p.mask, p.capacity, p.page_size).n
-                               : Span<kFp4Chunk>(p0, p0 + ntok - 1, p.mask, p.capacity, p.page_size).n) + p.unit_extra;
+      n = Span<kTcChunk>(p0, p0 + ntok - 1, p.mask, p.capacity, p.page_size).n + p.unit_extra;
     }
     int total;
     const int at = length + scan(n, total);

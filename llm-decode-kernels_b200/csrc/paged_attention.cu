@@ -675,7 +675,6 @@ void set_tile(const Sizes& z, Pass& a, bool tc) {
   a.tc = tc;
   a.p.half_tokens = tc ? 128 / group : z.ragged ? 16 / group : 1;
   a.p.tile_tokens = tc ? 2 * a.p.half_tokens : a.p.half_tokens;
-  a.p.chunk = tc ? kTcChunk : kFp4Chunk;
 }
 
 void set_ragged(const Sizes& z, Pass& a, int above, int most) {

@@ -573,9 +573,9 @@ Split split_of(const Sizes& z) {
   const int64_t limit = kFewTiles * (16 / (z.nq / z.nkv));
   if (!z.fp4 || !z.ragged || z.prefix_len > 0 || z.T >= kManyTokens * z.B) return {false, true, 0};
   const int64_t token = 16 / (z.nq / z.nkv), tiles = (z.T + token - 1) / token + z.B;
-  const int64_t chunks = tiles * z.nkv * ((z.positions + kFp4Chunk - 1) / kFp4Chunk);
+  const int64_t chunks = tiles * ((z.positions + kFp4Chunk - 1) / kFp4Chunk);  // of a kv head
   const int64_t small = (z.T <= limit * z.B ? kSmallFew : kSmallMany) * fp4_groups(16) * device_info().num_sms;
-  if (z.T <= limit || chunks <= small) return {true, false, INT_MAX};
+  if (z.T <= limit || chunks <= small / z.nkv) return {true, false, INT_MAX};
   return {z.B > 1, true, z.B > 1 ? static_cast<int>(limit) : 0};
 }
 
@@ -842,7 +842,7 @@ extern "C" int dk_paged_attention_workspace_bytes(int64_t T, int64_t B, int64_t 
 extern "C" int dk_paged_attention_fp4_workspace_bytes(int64_t T, int64_t B, int64_t nq, int64_t nkv, int64_t head_dim,
                                                       int32_t dtype, int32_t ragged, int64_t prefix_len, int64_t positions,
                                                       uint64_t* bytes) {
-  if (positions <= 0) return set_error(DK_ERR_INVALID, "paged_attention_fp4_workspace_bytes: bad sizes");
+  if (positions <= 0 || positions > INT32_MAX) return set_error(DK_ERR_INVALID, "paged_attention_fp4_workspace_bytes: bad sizes");
   return workspace_bytes("paged_attention_fp4_workspace_bytes",
                          Sizes{T, B, nq, nkv, head_dim, prefix_len, ragged != 0, dtype, true, positions}, bytes);
 }
@@ -901,7 +901,7 @@ int attention(const char* what, const dk_paged_attention_args& a, bool prefix, b
     const int64_t chunk = s->tc ? kTcChunk : z.fp4 ? kFp4Chunk : kChunk;
     const int64_t tiles = s->p.mode == kRagged ? s->p.max_tiles : s->p.n_tiles;
     const int64_t positions = s->p.mode == kPrefix ? z.prefix_len : table_width * page_size;
-    if (tiles * ((positions + chunk - 1) / chunk + 1 + s->p.unit_extra) * z.nkv >= (int64_t(1) << 30))
+    if (tiles * ((positions + chunk - 1) / chunk + 1 + s->p.unit_extra) > ((int64_t(1) << 30) - 1) / z.nkv)  // (the product may pass 2^63)
       return set_error(DK_ERR_UNSUPPORTED, "%s: the call's work counts more than 2^30 chunks: fewer sequences or narrower page tables",
                        what);
   }

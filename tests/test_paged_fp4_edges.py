@@ -54,3 +54,27 @@ def test_a_read_whose_rows_contradict_its_outputs_is_refused():
     for pair in (out[:1], (*out, out[0])):
         with pytest.raises(ValueError, match="out must be two"):
             paged_read_fp4(*args, out=pair)
+
+
+@pytest.mark.parametrize("fp4", [True, False])
+@pytest.mark.parametrize("tokens", [1, 100])
+def test_a_call_whose_chunks_pass_64_bits_is_refused(fp4, tokens):
+    """2^26 sequences that share a row of 2^26 pages (a table of stride 0), 65535 kv heads: 2^65 chunks are more than 2^30, although
+    their number's low 64 bits are less."""
+    from kernels import _lib
+
+    h, at, B, nkv, width = _lib.lib(), 1 << 20, 1 << 26, 65535, 1 << 26  # addresses that are looked at for their alignment alone
+    args = (at, nkv * 64, at, at, 1, 16, 0, 0, at, 0, width, at, at, 0, 0, 1.0, at, tokens, B, nkv, nkv, 64, 0, at, 0, 0)
+    status = (h.dk_paged_attention_fp4(_lib.PAGED_ATTENTION_FP4_ARGS.pack(*args, 1.0, 1.0)) if fp4
+              else h.dk_paged_attention(_lib.PAGED_ATTENTION_ARGS.pack(*args)))
+    assert status == -3 and b"more than 2^30 chunks" in h.dk_last_error()
+
+
+def test_workspaces_of_more_positions_than_a_table_can_have_are_refused():
+    import ctypes
+
+    from kernels import _lib
+
+    n = ctypes.c_uint64(0)
+    for positions, status in ((0, -1), (2 ** 31, -1), (2 ** 63 - 1, -1), (2 ** 31 - 1, 0)):
+        assert _lib.lib().dk_paged_attention_fp4_workspace_bytes(1, 1, 12, 2, 128, 0, 1, 0, positions, ctypes.byref(n)) == status

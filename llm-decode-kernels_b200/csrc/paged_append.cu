@@ -12,9 +12,10 @@
 // With kFp4 k' and v go to a cache of 4-bit codes (paged_fp4.cuh). What a code is can hang on the last bit of k', so k is then
 // rotated in fp64, where the two products are exact and only their sum is rounded, and goes to T by way of fp32: a code does not
 // depend on the order or the fusing of the operations. (Of fp16 keys about one in 17000 lies so close to the middle of two values that a
-// single rounding would give the other; these steps are what the cache's contents are defined by.) q is rotated as without. Measured (36 heads of 128, bf16): 11000 tokens, 127 MB of q, k, v in
-// and q out, 5 MB of codes, 33.6 us (30 without quantising, 1.5 more in fp64 than in fp32); 64 tokens 3 us without the host.
-// 3 CTAs an SM (80 registers, 20 bytes of them spilled instead of 88 to 104) come out 1 us slower.
+// single rounding would give the other; these steps are what the cache's contents are defined by.) q is rotated as without.
+// Measured (36 heads of 128, bf16): 8802 tokens, 144 MB of q, k, v in and q out, 5 MB of codes, 33.6 us, 4.4 TB/s (30 without quantising, 1.5
+// more in fp64 than in fp32); 64 tokens 3 us without the host. 51% of issue and 44% of DRAM's nominal peak: a warp has two segments in
+// flight, and 64 registers leave 80 to 88 bytes spilled. 3 CTAs an SM (80 registers) come out 1 us slower.
 // Measured (36 heads of 128): 9000 tokens, 164 MB, 32 us, 78% of the copy rate (64 registers a thread, 4 CTAs an SM, 20 bytes of
 // it spilled; with 5 or 6 CTAs 92 to 300 bytes spill, 42 and 53 us); one token 2.3 us without the host.
 #include <algorithm>

@@ -18,15 +18,16 @@
 // code * scale is exact in fp16, and so is q once its row is scaled by a power of two (bf16 rows; their largest value comes to 2^14,
 // and what falls below 2^-24 there counts for nothing beside it): the products are those of the cache's values. p is rounded to
 // fp16 for the product with v; its reference is 2^6 below the maximum seen when it was set, and it is set anew when a score
-// passes it by 2^14, so that p has 38 binades above fp16's smallest step.
+// passes it by 2^14, so that the largest p lies 30 to 38 binades above fp16's smallest step.
 // A producer warp a group streams chunks of 128 positions through a ring of bulk copies, as in the 16-bit kernel; a consumer warp
 // takes 32 of them, so that the operands of two tiles are on their way at a time. A position that no row of the tile
 // sees gets a scale of zero in place of v's, whatever its page holds; a page outside the pool gets scales of zero in
 // shared memory. Codes are finite whatever they are.
-// What bounds it: issue. A tile of 16 positions takes a warp about 260 instructions (64 conversions, 64 products with scales, 16
-// tensor-core products, 16 exchanges of halves) besides 80 for the chunk, the part and the kernel's start; measured (28 heads over 4 kv
-// heads of 128, bf16, 64 sequences of up to 8192, 212 MB): 52 us with the join, 4.1 TB/s, 62% of the copy rate (58% of issue, 51% of
-// the ALU, 50% of DRAM over the launch; without any arithmetic the same loads take 40). 16-bit pages of the same take 116 us.
+// What bounds it: no unit is full. Measured (28 heads over 4 kv heads of 128, bf16, 64 sequences of up to 8192, 212 MB): 52 us with the
+// join, 4.1 TB/s, 62% of the copy rate; over the launch 59% of issue, 51% of the ALU, 51% of DRAM's nominal peak. Start, join and tail take
+// 12 us of it, without any arithmetic the same loads take 40, and 12 consumer warps an SM do not cover one another's waits and conversions:
+// a tile of 16 positions takes a warp about 260 instructions (64 conversions, 64 products with scales, 16 tensor-core products, 16
+// exchanges of halves) besides 80 for the chunk, the part and the kernel's start, all of them 26 us of issue. 16-bit pages take 116 us.
 // Chunks of 64 (a tile a warp): 61 us, but one sequence of 640 8.5 us instead of 9.4. 4 groups an SM, 96 registers a thread: 59.
 // 32 sequences of 4096 with 2 to 5 tokens each: 41 us for three tiles a sequence.
 #include <algorithm>

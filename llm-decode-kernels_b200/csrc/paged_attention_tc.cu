@@ -29,7 +29,7 @@
 // cycle), and they run beside each other; a pair of half chunks takes about 1.65 us (1.15 at least), a unit's start, masks
 // and output about 5 us more. Measured: a prompt of 8192, 12 heads over 2 of 128, 197 us in short bursts, 1.05 PFLOP/s, 64%
 // of the cuBLAS rate; under the power cap (1.69 GHz) 228 us, 65% of cuBLAS's there. 220 to 228 bytes of a thread's registers are
-// spilled. 16 softmax warps, two a row: 362 us. Exponentials
+// spilled, 428 to 520 with kFp4 (128 registers at launch). 16 softmax warps, two a row: 362 us. Exponentials
 // on the FMA units for an eighth of the positions: 206 us. Steps of 64 positions: their products take nearly as long (58 cycles).
 #include <climits>
 #include <mutex>

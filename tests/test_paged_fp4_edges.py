@@ -37,6 +37,27 @@ def test_keys_are_rounded_by_way_of_fp32(dtype):
     assert codes[0, 0, 0, :3].tolist() == [4, 7, 6]  # 2 and not 3, 6, 4 and not 3
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("power", [2.0 ** 64, 2.0 ** -64])
+def test_append_and_read_at_the_ends_of_the_powers_range(power):
+    """Values around the power, from too small for the smallest scale to too large for the largest."""
+    from kernels.paged_fp4 import fp4_pages, paged_append_fp4, paged_read_fp4
+
+    T, hd = 64, 128
+    g = torch.Generator().manual_seed(5)
+    x = torch.randn(T, hd, generator=g, dtype=torch.float64) * torch.logspace(-4, 5, T, dtype=torch.float64)[:, None] * power
+    x = x.to(BF16)
+    k, v = (fp4_pages(4, 1, 16, hd, "cuda") for _ in range(2))
+    table, length = torch.tensor([[2, 0, 3, 1]], dtype=torch.int32, device="cuda"), torch.tensor([T], dtype=torch.int32, device="cuda")
+    starts = torch.tensor([0, T], dtype=torch.int32, device="cuda")
+    cos, sin = torch.ones(T, hd // 2, device="cuda"), torch.zeros(T, hd // 2, device="cuda")
+    scales = {"k_scale": power, "v_scale": power}
+    paged_append_fp4(torch.cat([x, x, x], 1).cuda(), k, v, table, length, cos, sin, 1, 1, starts, **scales)
+    want = quantise(x, power)[2]
+    for got in paged_read_fp4(k, v, table, length, starts, tokens=T, dtype=BF16, **scales):
+        assert torch.equal(got[:, 0].double().cpu(), want)
+
+
 def test_a_read_whose_rows_contradict_its_outputs_is_refused():
     """`out` and `tokens` both say how many rows there are; one that says otherwise is not dropped silently."""
     from _paged_fp4 import Fp4Case

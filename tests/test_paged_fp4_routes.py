@@ -178,6 +178,17 @@ def test_scales_of_any_sign(route, scale, dtype, hd, tmp_path):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("k_scale,v_scale", [(2.0 ** 64, 2.0 ** -64), (2.0 ** -64, 2.0 ** 64)])
+@pytest.mark.parametrize("route", ROUTES)
+def test_powers_at_the_ends_of_their_range(route, k_scale, v_scale, tmp_path):
+    """Queries as small (as large) as the keys' power is large (small): all of it is shifts of exponents."""
+    c = _case(route, dtype=BF16, seed=17, k_scale=k_scale, v_scale=v_scale)
+    for window, sinks in ((0, 0), (40, 3)):
+        assert_within(_attend(c, window=window, sinks=sinks), *c.attention(window, sinks))
+    _takes(route, c, tmp_path)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype,hd", [(F16, 64), (BF16, 128)])
 @pytest.mark.parametrize("before,after", [(2, 0), (0, 5), (3, 7)])
 @pytest.mark.parametrize("route", ROUTES)

@@ -486,7 +486,7 @@ __global__ void __launch_bounds__(kThreads<kBlocks>, 1) fp4_rows_kernel(const Pr
           acc.x = fmaf(wt, v.x, acc.x), acc.y = fmaf(wt, v.y, acc.y), acc.z = fmaf(wt, v.z, acc.z), acc.w = fmaf(wt, v.w, acc.w);
         }
         if (whole) {
-          const float inv = sum == 0.f ? 0.f : p.out_scale / sum;
+          const float inv = sum == 0.f ? 0.f : 1.f / sum * p.out_scale;
           const int tok = kRaggedTiles ? row / p.G : 0;
           T* dst = static_cast<T*>(p.out) + ((static_cast<int64_t>(t.t0 + tok) * p.nkv + h) * p.G + row - tok * p.G) * kHd + d;
           *reinterpret_cast<uint2*>(dst) = make_uint2(Elem<T>::pack(acc.x * inv, acc.y * inv), Elem<T>::pack(acc.z * inv, acc.w * inv));

@@ -610,7 +610,7 @@ __global__ void __launch_bounds__(kThreads<kFp4>, 1)
       tc::fence_after_sync();
       const int row = x * 128 + r;
       if (whole) {
-        const float inv = l == 0.f ? 0.f : p.out_scale / l;
+        const float inv = l == 0.f ? 0.f : 1.f / l * p.out_scale;
         // Four lanes exchange 16-byte pieces so that together they store 64 bytes of one row at a time: a lane storing its
         // own row would touch 32 lines with every instruction.
         T* out = static_cast<T*>(p.out) + (static_cast<int64_t>(t.t0 + tok) * p.nkv * p.G + head) * kHd;

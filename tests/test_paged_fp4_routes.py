@@ -38,7 +38,7 @@ def test_bf16_calls_keep_p_in_fp16(sizes, wide, route, hd, tmp_path):
 # sequence and more, taken by the 256-row tiles, which read a 16-bit copy where a sequence has three tiles and the copy fits.
 ROUTES = {
     "rows": ([(9, 200), (4, 140), (5, 60)], 6, 2, 1, {"plan", "fp4_rows"}),
-    "split": ([(60, 300), (9, 90), (4, 200)], 6, 2, 1 << 16, {"plan", "fp4_rows", "tiles_codes"}),
+    "split": ([(60, 300), (9, 90), (4, 200)], 6, 2, 1 << 16, {"plan_both", "fp4_rows", "tiles_codes"}),
     "tiles": ([(300, 420), (230, 260)], 6, 2, 1 << 16, {"plan", "tiles_codes"}),
     "copied": ([(300, 420), (230, 260)], 6, 2, 1, {"fp4_copy", "tiles"}),
     "copied, split": ([(200, 260), (3, 77), (90, 180), (60, 400)], 16, 1, 200, {"fp4_copy", "fp4_rows", "tiles"}),
